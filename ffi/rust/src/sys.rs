@@ -148,6 +148,64 @@ pub const WH_ROUTER_SQRT_SOFTPLUS: i32 = 1;
 pub const WH_NO_SHARED_EXPERT: u32 = 0xFFFF_FFFF;
 pub const WH_NOALLOC_SCRATCH_BYTES: usize = 8 << 20;
 
+/// A paged 4-bit attention cache by its device buffers.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct WhKv4Cache {
+    pub k_codes: *mut u8,
+    pub k_scales: *mut u8,
+    pub v_codes: *mut u8,
+    pub v_scales: *mut u8,
+    pub n_pages: usize,
+    pub page_size: usize,
+    pub kv_heads: usize,
+    pub head_dim: usize,
+}
+
+/// One step's plan of lengths, pages and slots.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct WhKvPlan {
+    pub n_requests: usize,
+    pub old_lens_dev: *const u32,
+    pub new_lens_dev: *const u32,
+    pub tables_dev: *mut u32,
+    pub table_stride: usize,
+    pub page_size: usize,
+    pub n_pages: usize,
+    pub free_dev: *const u32,
+    pub free_count_dev: *const u32,
+    pub free_out_dev: *mut u32,
+    pub free_count_out_dev: *mut u32,
+    pub max_tokens: usize,
+    pub starts_dev: *mut u32,
+    pub slots_dev: *mut u32,
+    pub positions_dev: *mut u32,
+}
+
+/// Attention of new tokens over a 4-bit cache.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct WhKv4Attention {
+    pub q_dev: *const c_void,
+    pub q_stride: usize,
+    pub out_dev: *mut c_void,
+    pub out_stride: usize,
+    pub is_bf16: c_int,
+    pub n_tokens: usize,
+    pub n_requests: usize,
+    pub starts_dev: *const u32,
+    pub lens_dev: *const u32,
+    pub tables_dev: *const u32,
+    pub table_stride: usize,
+    pub max_len: usize,
+    pub heads: usize,
+    pub scale: f32,
+    pub window: usize,
+    pub first: usize,
+    pub sink: *const f32,
+}
+
 extern "C" {
     pub fn wh_init(device: c_int, out_: *mut *mut WhCtx) -> c_int;
     pub fn wh_shutdown(ctx: *mut WhCtx) -> c_int;
@@ -301,4 +359,13 @@ extern "C" {
                                              npos: usize, hidden_dev: *mut f32, kv_cache_dev: *mut f32,
                                              kv_stride: usize, kv_capacity: usize, comp_dev: *const *const f32,
                                              n_comp: *const usize, token_ids: *const i64) -> c_int;
+    pub fn wh_kv_plan_async(ctx: *mut WhCtx, plan: *const WhKvPlan) -> c_int;
+    pub fn wh_kv4_write_async(ctx: *mut WhCtx, cache: *const WhKv4Cache, k_dev: *const c_void, k_stride: usize,
+                              v_dev: *const c_void, v_stride: usize, is_bf16: c_int, slots_dev: *const u32,
+                              n: usize) -> c_int;
+    pub fn wh_kv4_read_async(ctx: *mut WhCtx, cache: *const WhKv4Cache, slots_dev: *const u32, n: usize,
+                             k_dev: *mut c_void, k_stride: usize, v_dev: *mut c_void, v_stride: usize,
+                             is_bf16: c_int) -> c_int;
+    pub fn wh_kv4_attention_async(ctx: *mut WhCtx, cache: *const WhKv4Cache,
+                                  attention: *const WhKv4Attention) -> c_int;
 }

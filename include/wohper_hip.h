@@ -810,6 +810,130 @@ int wh_deepseek_mhc_layer_batch_async(wh_ctx* ctx, const wh_mhc_layer* layer, co
                                       float* hidden_dev, float* kv_cache_dev, size_t kv_stride, size_t kv_capacity,
                                       const float* const* comp_dev, const size_t* n_comp, const int64_t* token_ids);
 
+/* ------------------------------------------------------------------
+ * A paged attention cache in 4 bits, no counterpart in the reference (its
+ * cache is one request's f32 rows).  A row of head_dim values is E2M1 codes,
+ * two a byte (low nibble: the even dim), and one UE8M0 scale byte for every
+ * 32 dims: value = grid[code] * 2^(byte - 127) with the OCP grid 0, .5, 1,
+ * 1.5, 2, 3, 4, 6 and its negatives (not the weights', whose second magnitude
+ * is 0.125); byte 0 stands for 0.0 and 255 for NaN.  That is 0.53 bytes a
+ * value.  Rows lie in pages of page_size rows, a power of two: codes
+ * [page][kv head][row][head_dim / 2], scales [page][kv head][row][head_dim /
+ * 32].  A row's slot is page * page_size + row; 0xFFFFFFFF is no slot.
+ *
+ * The four calls make a serving step: the plan (lengths to slots), the rows
+ * of the new tokens in, attention, and rows back out where a dense path needs
+ * them.  Request lengths, tables and slots are device arrays, so a step whose
+ * lengths only the device knows can be captured once and replayed.
+ * ------------------------------------------------------------------ */
+
+/* k_codes .. v_scales are device pointers, 16-byte aligned, the caller's.
+ * v_codes and v_scales both NULL: the values are the keys (MLA's latent
+ * rows).  head_dim 64, 128, 256 or 512 and page_size a power of two up to
+ * 65536, else WH_UNSUPPORTED; n_pages * page_size below 2^32 - 1. */
+typedef struct {
+    uint8_t* k_codes;
+    uint8_t* k_scales;
+    uint8_t* v_codes;
+    uint8_t* v_scales;
+    size_t n_pages, page_size, kv_heads, head_dim;
+} wh_kv4_cache;
+
+/* One step's lengths: request b goes from old_lens[b] to new_lens[b] cached
+ * rows.  It holds ceil(len / page_size) pages, tables_dev[b * table_stride +
+ * i] its i-th.  A request that shrinks gives its last pages back (0: all of
+ * them; drafted tokens that were not accepted), one that grows takes new ones
+ * and gets slots for positions old_lens[b] .. new_lens[b] - 1.  In request
+ * order, the pages given back go onto the stack of free pages, free_dev[0 ..
+ * *free_count_dev), then the new ones come off its top.  Outputs:
+ *   tables_dev: the entries of new pages; all others stay as they are
+ *   free_out_dev [n_pages], free_count_out_dev: the stack with the pages given
+ *     back (those above the new count are the ones that were taken); both may
+ *     be free_dev and free_count_dev
+ *   starts_dev [n_requests + 1]: each request's first new token, and their sum
+ *   slots_dev, positions_dev [max_tokens]: of the new tokens, request by
+ *     request; past the last one no slot and 0
+ * A plan that does not fit takes, gives and numbers nothing: starts are 0, no
+ * token has a slot, the stack is as before, and wh_stream_status reports
+ * WH_OUT_OF_MEMORY (not enough pages) or WH_OUTPUT_TOO_SMALL (max_tokens,
+ * table_stride).  A page id of n_pages or more reports WH_NOT_RESIDENT and
+ * its tokens get no slot.  At most 4096 requests; apart from the stack no
+ * output may overlap an input. */
+typedef struct {
+    size_t n_requests;
+    const uint32_t* old_lens_dev;
+    const uint32_t* new_lens_dev;
+    uint32_t* tables_dev;
+    size_t table_stride, page_size, n_pages;
+    const uint32_t* free_dev;
+    const uint32_t* free_count_dev;
+    uint32_t* free_out_dev;
+    uint32_t* free_count_out_dev;
+    size_t max_tokens;
+    uint32_t* starts_dev;
+    uint32_t* slots_dev;
+    uint32_t* positions_dev;
+} wh_kv_plan;
+int wh_kv_plan_async(wh_ctx* ctx, const wh_kv_plan* plan);
+
+/* Rounds n rows of kv_heads * head_dim values (f32, or bf16 with is_bf16) into
+ * the cache: row i at k_dev + i * k_stride, and its values at v_dev + i *
+ * v_stride unless the cache has none (v_dev NULL), to slots_dev[i].  A group
+ * of 32 gets the least power of two under which its largest magnitude is at
+ * most 6 and each value the nearest code whose value is finite, ties to even;
+ * a group with an infinity or NaN reads back as NaN.  Rows of no slot are passed over; a slot
+ * behind the cache reports WH_NOT_RESIDENT.  Slots of one call differ, else
+ * the slot holds a mix of its rows.  Row pointers 16-byte aligned, strides a
+ * multiple of 16 bytes. */
+int wh_kv4_write_async(wh_ctx* ctx, const wh_kv4_cache* cache, const void* k_dev, size_t k_stride, const void* v_dev,
+                       size_t v_stride, int is_bf16, const uint32_t* slots_dev, size_t n);
+
+/* The values that the rows of n slots stand for, exact in f32 and in bf16:
+ * keys to k_dev, values to v_dev (either may be NULL).  Rows of no slot are
+ * left as they are; alignment and slots as in wh_kv4_write_async. */
+int wh_kv4_read_async(wh_ctx* ctx, const wh_kv4_cache* cache, const uint32_t* slots_dev, size_t n, void* k_dev,
+                      size_t k_stride, void* v_dev, size_t v_stride, int is_bf16);
+
+/* Attention of new tokens over the cached rows of their requests: one token a
+ * request (decode), a few (speculative verify) or a prompt's (prefill), in any
+ * mix.  Request b's tokens are rows starts_dev[b] .. starts_dev[b + 1] of q and
+ * out, the last positions of its lens_dev[b] cached rows (their own included).
+ * Head h reads key head h / (heads / kv_heads).  A token at position p sees
+ * key j <= p, with a window only j > p - window or j < first (the first tokens
+ * stay visible); weights are the softmax of scale * q . key, with the optional
+ * logit sink[h] in the denominator.  A row that sees nothing is 0.
+ *
+ * q and out: [n_tokens] rows of heads * head_dim values, f32 or (is_bf16) bf16,
+ * 16-byte aligned with strides of a multiple of 16 bytes; rows from
+ * starts_dev[n_requests] on are left as they are.  q and out must not
+ * overlap.
+ * max_len: at least the largest of lens_dev; it only sizes the split of long
+ * key lists and the context's scratch for it, not the result.  A table entry
+ * of n_pages or more, or a length above table_stride * page_size, reports
+ * WH_NOT_RESIDENT.  A visible row that holds NaN makes its heads' outputs NaN;
+ * rows that are not visible do nothing, whatever their bytes.
+ * Sums are f32 in both types and in both numerics modes; an f32 result is
+ * within a few units of f32 rounding of the sums' size. */
+typedef struct {
+    const void* q_dev;
+    size_t q_stride;
+    void* out_dev;
+    size_t out_stride;
+    int is_bf16;
+    size_t n_tokens, n_requests;
+    const uint32_t* starts_dev;
+    const uint32_t* lens_dev;
+    const uint32_t* tables_dev;
+    size_t table_stride;
+    size_t max_len;
+    size_t heads;
+    float scale;
+    size_t window;      /* 0: none */
+    size_t first;
+    const float* sink;  /* device [heads] or NULL */
+} wh_kv4_attention;
+int wh_kv4_attention_async(wh_ctx* ctx, const wh_kv4_cache* cache, const wh_kv4_attention* attention);
+
 #ifdef __cplusplus
 }
 #endif

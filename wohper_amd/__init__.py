@@ -94,6 +94,7 @@ EXPORTED = (
     "wh_hc_split_sinkhorn_async", "wh_hc_pre_async", "wh_hc_post_async",
     "wh_graph_begin", "wh_graph_end", "wh_graph_launch", "wh_graph_release",
     "wh_routed_and_shared_experts_dev_async", "wh_deepseek_mhc_layer_async", "wh_deepseek_mhc_layer_batch_async",
+    "wh_kv_plan_async", "wh_kv4_write_async", "wh_kv4_read_async", "wh_kv4_attention_async",
 )
 
 ROUTER_RAW_LOGITS = 0
@@ -160,6 +161,33 @@ class WhMhcLayer(ctypes.Structure):
                 ("ffn_norm_bf16", ctypes.c_void_p), ("attn", WhMlaLayer), ("layer_id", ctypes.c_uint32),
                 ("active", ctypes.c_size_t), ("available_dev", ctypes.c_void_p), ("n_available", ctypes.c_size_t),
                 ("route", WhRouteOptions), ("shared_layer", ctypes.c_uint32), ("shared_expert", ctypes.c_uint32)]
+
+
+class WhKv4Cache(ctypes.Structure):
+    """A paged 4-bit cache by its device buffers (wh_kv4_cache)."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p), ("n_pages", ctypes.c_size_t), ("page_size", ctypes.c_size_t),
+                ("kv_heads", ctypes.c_size_t), ("head_dim", ctypes.c_size_t)]
+
+
+class WhKvPlan(ctypes.Structure):
+    """One step's plan of lengths, pages and slots (wh_kv_plan)."""
+    _fields_ = [("n_requests", ctypes.c_size_t), ("old_lens_dev", ctypes.c_void_p), ("new_lens_dev", ctypes.c_void_p),
+                ("tables_dev", ctypes.c_void_p), ("table_stride", ctypes.c_size_t), ("page_size", ctypes.c_size_t),
+                ("n_pages", ctypes.c_size_t), ("free_dev", ctypes.c_void_p), ("free_count_dev", ctypes.c_void_p),
+                ("free_out_dev", ctypes.c_void_p), ("free_count_out_dev", ctypes.c_void_p),
+                ("max_tokens", ctypes.c_size_t), ("starts_dev", ctypes.c_void_p), ("slots_dev", ctypes.c_void_p),
+                ("positions_dev", ctypes.c_void_p)]
+
+
+class WhKv4Attention(ctypes.Structure):
+    """Attention of new tokens over a 4-bit cache (wh_kv4_attention)."""
+    _fields_ = [("q_dev", ctypes.c_void_p), ("q_stride", ctypes.c_size_t), ("out_dev", ctypes.c_void_p),
+                ("out_stride", ctypes.c_size_t), ("is_bf16", ctypes.c_int), ("n_tokens", ctypes.c_size_t),
+                ("n_requests", ctypes.c_size_t), ("starts_dev", ctypes.c_void_p), ("lens_dev", ctypes.c_void_p),
+                ("tables_dev", ctypes.c_void_p), ("table_stride", ctypes.c_size_t), ("max_len", ctypes.c_size_t),
+                ("heads", ctypes.c_size_t), ("scale", ctypes.c_float), ("window", ctypes.c_size_t),
+                ("first", ctypes.c_size_t), ("sink", ctypes.c_void_p)]
 
 
 class WhExpertPackEntry(ctypes.Structure):
@@ -278,6 +306,10 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         "wh_hc_split_sinkhorn_async": (c.c_int, [vp, vp, vp, vp, sz, sz, c.c_float, vp, vp, vp]),
         "wh_hc_pre_async": (c.c_int, [vp, vp, vp, vp, sz, sz, sz, c.c_float, vp, vp, vp, vp]),
         "wh_hc_post_async": (c.c_int, [vp, vp, vp, vp, vp, vp, sz, sz]),
+        "wh_kv_plan_async": (c.c_int, [vp, c.POINTER(WhKvPlan)]),
+        "wh_kv4_write_async": (c.c_int, [vp, c.POINTER(WhKv4Cache), vp, sz, vp, sz, c.c_int, vp, sz]),
+        "wh_kv4_read_async": (c.c_int, [vp, c.POINTER(WhKv4Cache), vp, sz, vp, sz, vp, sz, c.c_int]),
+        "wh_kv4_attention_async": (c.c_int, [vp, c.POINTER(WhKv4Cache), c.POINTER(WhKv4Attention)]),
         "wh_route_experts_async": (c.c_int, [vp, c.c_uint32, vp, sz, sz, vp, sz, c.POINTER(WhRouteOptions), vp, vp,
                                              vp]),
     }
@@ -855,6 +887,28 @@ class Context:
         us = ctypes.c_double()
         _check(self.lib.wh_timer_stop(self._h, ctypes.byref(us)), "timer_stop")
         return us.value
+
+    # ------------------------------------------------- paged 4-bit cache
+    def kv_plan_async(self, plan: WhKvPlan):
+        """Pages, slots and positions of a step from its requests' lengths."""
+        _check(self.lib.wh_kv_plan_async(self._h, ctypes.byref(plan)), "kv_plan_async")
+
+    def kv4_write_async(self, cache: WhKv4Cache, k_ptr: int, k_stride: int, v_ptr: Optional[int], v_stride: int,
+                        is_bf16: bool, slots_ptr: int, n: int):
+        """Rounds n rows into the cache at their slots."""
+        _check(self.lib.wh_kv4_write_async(self._h, ctypes.byref(cache), k_ptr, k_stride, v_ptr, v_stride, is_bf16,
+                                           slots_ptr, n), "kv4_write_async")
+
+    def kv4_read_async(self, cache: WhKv4Cache, slots_ptr: int, n: int, k_ptr: Optional[int], k_stride: int,
+                       v_ptr: Optional[int], v_stride: int, is_bf16: bool):
+        """The values that the rows of n slots stand for."""
+        _check(self.lib.wh_kv4_read_async(self._h, ctypes.byref(cache), slots_ptr, n, k_ptr, k_stride, v_ptr, v_stride,
+                                          is_bf16), "kv4_read_async")
+
+    def kv4_attention_async(self, cache: WhKv4Cache, attention: WhKv4Attention):
+        """Attention of new tokens over their requests' cached rows."""
+        _check(self.lib.wh_kv4_attention_async(self._h, ctypes.byref(cache), ctypes.byref(attention)),
+               "kv4_attention_async")
 
     def debug_eval(self, fn: int, x) -> np.ndarray:
         x = _f32(x)

@@ -2,7 +2,7 @@
 
 Steps: compile and run the libm table generator (host glibc is the
 specification it verifies against; the table is cached by content hash of
-its inputs), then hipcc the single HIP translation unit.
+its inputs), then hipcc the HIP translation units side by side and link them.
 """
 from __future__ import annotations
 
@@ -24,10 +24,13 @@ HIP_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
+
+
+# the HIP translation units of the library
+UNITS = ("wohper_hip", "kv4")
 
 
 def _hipcc() -> str:
@@ -68,6 +71,24 @@ def build_libm_tables(verbose: bool = True) -> Path:
     return inc
 
 
+def _run_all(cmds, verbose: bool) -> None:
+    """Runs commands side by side; raises if one fails."""
+    if verbose:
+        for cmd in cmds:
+            print("[wohper_amd] " + " ".join(cmd), flush=True)
+    runs = [subprocess.Popen(cmd, stdout=subprocess.DEVNULL, stderr=subprocess.PIPE, text=True) for cmd in cmds]
+    failed = False
+    for run in runs:
+        err = run.communicate()[1]
+        # hipcc's host pass reports the device-only feature flag as unknown: harmless
+        noise = [ln for ln in err.splitlines() if "packed-fp32-ops" not in ln]
+        if noise and (verbose or run.returncode != 0):
+            sys.stderr.write("\n".join(noise) + "\n")
+        failed |= run.returncode != 0
+    if failed:
+        raise RuntimeError("hipcc failed building libwohper_hip.so")
+
+
 def build(verbose: bool = True, timeline: Path | None = None) -> Path:
     """Builds libwohper_hip.so in the package.  timeline: instead build the
     per-wave timeline variant (-DWH_TIMELINE: the persistent expert kernels
@@ -75,18 +96,11 @@ def build(verbose: bool = True, timeline: Path | None = None) -> Path:
     to that path; it is a measuring build, not the product."""
     build_libm_tables(verbose)
     out = Path(timeline) if timeline else LIB
-    cmd = [_hipcc(), *HIP_FLAGS, *(["-DWH_TIMELINE"] if timeline else []), "-I", str(ROOT / "include"),
-           "-I", str(CSRC), "-I", str(GEN), "-o", str(out) + ".tmp", str(CSRC / "wohper_hip.hip")]
-    if verbose:
-        print("[wohper_amd] " + " ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    # hipcc's host pass reports the device-only feature flag as unknown: harmless
-    noise = [ln for ln in res.stderr.splitlines() if "packed-fp32-ops" not in ln]
-    if res.returncode != 0:
-        sys.stderr.write("\n".join(noise) + "\n")
-        raise RuntimeError("hipcc failed building libwohper_hip.so")
-    if noise and verbose:
-        sys.stderr.write("\n".join(noise) + "\n")
+    flags = [*HIP_FLAGS, *(["-DWH_TIMELINE"] if timeline else []), "-I", str(ROOT / "include"), "-I", str(CSRC),
+             "-I", str(GEN)]
+    objs = [GEN / f"{unit}{'_timeline' if timeline else ''}.o" for unit in UNITS]
+    _run_all([[_hipcc(), *flags, "-c", "-o", str(o), str(CSRC / f"{unit}.hip")] for unit, o in zip(UNITS, objs)], verbose)
+    _run_all([[_hipcc(), *HIP_FLAGS, "-shared", "-o", str(out) + ".tmp", *map(str, objs)]], verbose)
     os.replace(str(out) + ".tmp", out)
     return out
 

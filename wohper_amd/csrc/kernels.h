@@ -14,11 +14,6 @@ __device__ const uint64_t kExpTab[WH_EXP_TAB_LEN] = {WH_EXP_TAB_INIT};
 __device__ const uint32_t kLog2Thr[254] = {WH_LOG2F_THR_INIT};
 __device__ const uint32_t kExpfExc[WH_EXPF_EXC_COUNT ? 2 * WH_EXPF_EXC_COUNT : 2] = {WH_EXPF_EXC_INIT};
 
-// status word bits, OR-ed by kernels, read by the host after the stream syncs
-#define WH_ST_NONFINITE_OUTPUT 1u
-#define WH_ST_NONFINITE_INPUT 2u
-#define WH_ST_NOT_RESIDENT 4u
-
 #define WH_MAX_EXPERTS 16
 
 // ------------------------------------------------------------------ shapes

@@ -16,6 +16,13 @@
 
 #include "libm_emul.h"
 
+// status word bits, OR-ed by kernels, read by the host after the stream syncs
+#define WH_ST_NONFINITE_OUTPUT 1u
+#define WH_ST_NONFINITE_INPUT 2u
+#define WH_ST_NOT_RESIDENT 4u
+#define WH_ST_KV_PAGES 8u    // a cache plan needs more pages than there are
+#define WH_ST_KV_NARROW 16u  // a cache plan's table rows or token buffers are too small
+
 typedef float wh_f2 __attribute__((ext_vector_type(2)));
 typedef float wh_f4 __attribute__((ext_vector_type(4)));
 

@@ -30,6 +30,7 @@
 #include "fp8_tol.h"
 #include "fp8_exact_mm.h"
 #include "fp8_multi.h"
+#include "kv4.h"
 #include "moe_bmx.h"
 #include "probe.h"
 #include "quant_block.h"
@@ -300,6 +301,7 @@ struct wh_ctx {
     Scratch fp8mm_ws, fp8mm_cnt;            // their partial tiles and arrival counters
     Scratch moe_dyn;                        // a device route list resolved for the experts (wh_moe_dyn)
     Scratch attn_max;                       // attn_mx.h: the score tiles' maxima, of a fixed size
+    Scratch kv4_part, kv4_ticket;           // the 4-bit cache: partial outputs of split attention, a plan's arrivals
     Scratch layer;                          // the decode layer's state and activations between its steps
     bool exact = true;                      // routed experts in the reference's summation order
     int token_kernels = 1;                  // MFMA token kernels: bit 0 gate/up, bit 1 down on k_*_tok (else k_*_px)
@@ -319,7 +321,7 @@ struct wh_ctx {
     hipStream_t base_stream = nullptr, cap_stream = nullptr;
     std::vector<Scratch*> scratch() {
         return {&x_in, &y_out, &h, &ybuf, &cnt_y, &tmp, &batch, &routes, &bout, &gu, &relayout, &rtr, &rtr_cnt,
-                &mla, &hcs, &fp8mm_ws, &fp8mm_cnt, &moe_dyn, &attn_max, &layer};
+                &mla, &hcs, &fp8mm_ws, &fp8mm_cnt, &moe_dyn, &attn_max, &kv4_part, &kv4_ticket, &layer};
     }
 };
 
@@ -359,6 +361,8 @@ int read_status(wh_ctx* c) {
         WH_HIP(hipStreamSynchronize(c->stream));
     }
     if (st & WH_ST_NOT_RESIDENT) return WH_NOT_RESIDENT;
+    if (st & WH_ST_KV_PAGES) return WH_OUT_OF_MEMORY;
+    if (st & WH_ST_KV_NARROW) return WH_OUTPUT_TOO_SMALL;
     if (st & WH_ST_NONFINITE_INPUT) return WH_NON_FINITE_INPUT;
     if (st & WH_ST_NONFINITE_OUTPUT) return WH_NON_FINITE_OUTPUT;
     return WH_OK;
@@ -2098,6 +2102,7 @@ int wh_init(int device, wh_ctx** out) {
     if (e == hipSuccess) e = hipEventCreate(&c->timer[1]);
     if (e == hipSuccess)
         e = c->attn_max.ensure((size_t)WH_POS_BATCH * WH_ATTN_MX_HEADS * WH_ATTN_MX_TILES * sizeof(float), false);
+    if (e == hipSuccess) e = c->kv4_ticket.ensure(sizeof(uint32_t), true);
     if (e != hipSuccess) {
         delete c;
         return hip_status(e);
@@ -4643,4 +4648,170 @@ int wh_deepseek_mhc_layer_batch_async(wh_ctx* c, const wh_mhc_layer* L, const si
                        token_ids, ids, w, count));
     WH_TRY(wh_moe_batch_async(c, L->layer_id, ids, w, npos, slots, L->shared_layer, L->shared_expert, g, 0, z));
     return hc_post_launch(c, z, state, post2, comb2, hidden_dev, hc, hidden, npos);
+}
+
+// ------------------------------------------------ the paged 4-bit cache
+
+namespace {
+// Checks a cache descriptor and takes its geometry; v: whether it has values
+// of its own.
+int kv4_shape(const wh_kv4_cache* cache, wh_kv4_shape* s, bool* v) {
+    if (!cache || !cache->k_codes || !cache->k_scales || !cache->v_codes != !cache->v_scales) return WH_INVALID_ARGUMENT;
+    for (const void* p : {(const void*)cache->k_codes, (const void*)cache->k_scales, (const void*)cache->v_codes,
+                          (const void*)cache->v_scales})
+        if ((uintptr_t)p & 15) return WH_INVALID_ARGUMENT;
+    const size_t d = cache->head_dim, page = cache->page_size;
+    if (cache->n_pages == 0 || cache->kv_heads == 0 || d == 0 || page == 0) return WH_EMPTY_SHAPE;
+    if ((d != 64 && d != 128 && d != 256 && d != 512) || (page & (page - 1)) || page > 65536 || cache->kv_heads > 65535)
+        return WH_UNSUPPORTED;
+    if (cache->n_pages > 0xfffffffeu / page) return WH_UNSUPPORTED;  // a slot is 32 bits, the last value none
+    s->n_pages = (uint32_t)cache->n_pages;
+    s->shift = 0;
+    while (((size_t)1 << s->shift) < page) ++s->shift;
+    s->kv_heads = (uint32_t)cache->kv_heads;
+    s->head_dim = (uint32_t)d;
+    *v = cache->v_codes != nullptr;
+    return WH_OK;
+}
+
+// A row pointer and stride (values) whose rows start on 16 bytes.
+int kv4_row_check(const void* p, size_t stride, size_t width, int bf16) {
+    if (!p || ((uintptr_t)p & 15) || stride % (bf16 ? 8 : 4)) return WH_INVALID_ARGUMENT;
+    return stride < width ? WH_INVALID_SHAPE : WH_OK;
+}
+
+int kv4_rows_args(const wh_kv4_cache* cache, void* k, size_t k_stride, void* v, size_t v_stride, int bf16,
+                  const uint32_t* slots, size_t n, bool out, wh_kv4_rows_args* a) {
+    bool has_v = false;
+    WH_TRY(kv4_shape(cache, &a->s, &has_v));
+    // values of their own go in with the keys; either may be read alone
+    if (!has_v && v) return WH_INVALID_ARGUMENT;
+    if (out ? !k && !v : !k || (has_v && !v)) return WH_INVALID_ARGUMENT;
+    if (n && !slots) return WH_INVALID_ARGUMENT;
+    const size_t width = cache->kv_heads * cache->head_dim;
+    if (n > 0x7fffffffu || n * (width / 8) > (size_t)0x7fffffff * 256) return WH_UNSUPPORTED;
+    if (k) {
+        WH_TRY(kv4_row_check(k, k_stride, width, bf16));
+        a->plane[0] = {cache->k_codes, cache->k_scales};
+        a->rows[0] = k;
+        a->stride[0] = k_stride;
+        a->planes = 1;
+    }
+    if (v) {
+        WH_TRY(kv4_row_check(v, v_stride, width, bf16));
+        a->plane[a->planes] = {cache->v_codes, cache->v_scales};
+        a->rows[a->planes] = v;
+        a->stride[a->planes] = v_stride;
+        ++a->planes;
+    }
+    a->slots = slots;
+    a->n = (uint32_t)n;
+    return WH_OK;
+}
+}  // namespace
+
+int wh_kv_plan_async(wh_ctx* c, const wh_kv_plan* d) {
+    if (!c || !d || !d->starts_dev || !d->free_dev || !d->free_count_dev || !d->free_out_dev || !d->free_count_out_dev ||
+        (d->n_requests && (!d->old_lens_dev || !d->new_lens_dev || !d->tables_dev)) ||
+        (d->max_tokens && (!d->slots_dev || !d->positions_dev)))
+        return WH_INVALID_ARGUMENT;
+    const size_t page = d->page_size;
+    if (page == 0 || d->n_pages == 0) return WH_EMPTY_SHAPE;
+    if ((page & (page - 1)) || page > 65536 || d->n_pages > 0xfffffffeu / page || d->n_requests > WH_KV_MAX_REQUESTS ||
+        d->max_tokens > 0x7fffffffu)
+        return WH_UNSUPPORTED;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    WH_HIP(hipSetDevice(c->device));
+    wh_kv_plan_args a{};
+    a.old_lens = d->old_lens_dev;
+    a.new_lens = d->new_lens_dev;
+    a.free_in = d->free_dev;
+    a.free_count = d->free_count_dev;
+    a.tables = d->tables_dev;
+    a.free_out = d->free_out_dev;
+    a.free_count_out = d->free_count_out_dev;
+    a.starts = d->starts_dev;
+    a.slots = d->slots_dev;
+    a.positions = d->positions_dev;
+    a.table_stride = d->table_stride;
+    a.n = (uint32_t)d->n_requests;
+    while (((size_t)1 << a.shift) < page) ++a.shift;
+    a.n_pages = (uint32_t)d->n_pages;
+    a.max_tokens = (uint32_t)d->max_tokens;
+    a.ticket = c->kv4_ticket.as<uint32_t>();
+    a.status = c->status;
+    WH_HIP(wh_kv_plan_launch(a, c->stream));
+    return WH_OK;
+}
+
+int wh_kv4_write_async(wh_ctx* c, const wh_kv4_cache* cache, const void* k_dev, size_t k_stride, const void* v_dev,
+                       size_t v_stride, int is_bf16, const uint32_t* slots_dev, size_t n) {
+    if (!c) return WH_INVALID_ARGUMENT;
+    wh_kv4_rows_args a{};
+    WH_TRY(kv4_rows_args(cache, (void*)k_dev, k_stride, (void*)v_dev, v_stride, is_bf16, slots_dev, n, false, &a));
+    if (n == 0) return WH_OK;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    WH_HIP(hipSetDevice(c->device));
+    a.status = c->status;
+    WH_HIP(wh_kv4_write_launch(a, is_bf16 != 0, c->stream));
+    return WH_OK;
+}
+
+int wh_kv4_read_async(wh_ctx* c, const wh_kv4_cache* cache, const uint32_t* slots_dev, size_t n, void* k_dev,
+                      size_t k_stride, void* v_dev, size_t v_stride, int is_bf16) {
+    if (!c) return WH_INVALID_ARGUMENT;
+    wh_kv4_rows_args a{};
+    WH_TRY(kv4_rows_args(cache, k_dev, k_stride, v_dev, v_stride, is_bf16, slots_dev, n, true, &a));
+    if (n == 0) return WH_OK;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    WH_HIP(hipSetDevice(c->device));
+    a.status = c->status;
+    WH_HIP(wh_kv4_read_launch(a, is_bf16 != 0, c->stream));
+    return WH_OK;
+}
+
+int wh_kv4_attention_async(wh_ctx* c, const wh_kv4_cache* cache, const wh_kv4_attention* d) {
+    if (!c || !d) return WH_INVALID_ARGUMENT;
+    wh_kv4_attn_args a{};
+    bool has_v = false;
+    WH_TRY(kv4_shape(cache, &a.s, &has_v));
+    if (d->heads == 0) return WH_EMPTY_SHAPE;
+    if (d->heads % cache->kv_heads) return WH_INVALID_SHAPE;
+    if (d->n_tokens == 0 || d->n_requests == 0) return WH_OK;
+    if (!d->starts_dev || !d->lens_dev || !d->tables_dev) return WH_INVALID_ARGUMENT;
+    const size_t width = d->heads * cache->head_dim, group = d->heads / cache->kv_heads;
+    WH_TRY(kv4_row_check(d->q_dev, d->q_stride, width, d->is_bf16));
+    WH_TRY(kv4_row_check(d->out_dev, d->out_stride, width, d->is_bf16));
+    if (d->n_tokens > 0x3fffffffu || d->n_requests > 0x3fffffffu || d->heads > 65536 ||
+        d->n_tokens * group > 0x3fffffffu || d->table_stride > 0xffffffffu)
+        return WH_UNSUPPORTED;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    WH_HIP(hipSetDevice(c->device));
+    a.k = {cache->k_codes, cache->k_scales};
+    a.v = has_v ? wh_kv4_plane{cache->v_codes, cache->v_scales} : a.k;
+    a.q = d->q_dev;
+    a.out = d->out_dev;
+    a.q_stride = d->q_stride;
+    a.out_stride = d->out_stride;
+    a.starts = d->starts_dev;
+    a.lens = d->lens_dev;
+    a.tables = d->tables_dev;
+    a.table_stride = d->table_stride;
+    a.sink = d->sink;
+    a.n_tokens = (uint32_t)d->n_tokens;
+    a.n_requests = (uint32_t)d->n_requests;
+    a.group = (uint32_t)group;
+    // positions are below 2^31: a longer window hides nothing
+    a.window = d->window > 0x7fffffffu ? 0 : (uint32_t)d->window;
+    a.first = (uint32_t)std::min<size_t>(d->first, 0x7fffffffu);
+    a.scale_log2 = d->scale * 1.44269504088896340736f;
+    a.status = c->status;
+    const wh_kv4_attn_plan p = wh_kv4_attn_plan_of(a, d->is_bf16 != 0, !has_v, d->max_len);
+    a.splits = p.splits;
+    a.min_blocks = p.min_blocks;
+    a.n_tiles = p.n_tiles;
+    WH_HIP(c->kv4_part.ensure(p.part_bytes, false));
+    a.part = c->kv4_part.as<float>();
+    WH_HIP(wh_kv4_attn_launch(a, d->is_bf16 != 0, !has_v, c->stream));
+    return WH_OK;
 }
