@@ -52,12 +52,14 @@ struct wh_kv4_attn_args {
     float* part;        // [tile][kv head][split][rows][head_dim + 2]: normalised outputs, maxima, sums
     uint32_t n_tokens, n_requests, group, window, first;
     uint32_t splits, min_blocks, n_tiles;
+    bool wide;          // tiles of 64 (f32: 32) rows instead of 16
     float scale_log2;   // scale * log2(e)
     uint32_t* status;
 };
 // How a call is cut up: by sizes the host knows.
 struct wh_kv4_attn_plan {
     uint32_t splits, min_blocks, n_tiles;
+    bool wide;
     size_t part_bytes;  // scratch for partial results, 0 for one split
 };
 wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, bool latent, size_t max_len);

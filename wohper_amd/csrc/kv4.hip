@@ -9,6 +9,7 @@
 #include "kv4.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "wh_device.h"
 
@@ -288,6 +289,7 @@ __global__ void __launch_bounds__(256) k_kv4_read(wh_kv4_rows_args a) {
 // a bf16 output keeps beside its sign) or, for f32, split into two.  Maxima,
 // sums of weights and outputs are f32.
 
+#define kMinusInf (-__builtin_inff())
 constexpr float kMinusBig = -1.0e30f;  // the maximum of no key: finite, so that differences are
 constexpr float kUp = 10.0f;           // weights are held times 2^10: f16 keeps small ones
 constexpr float kSlack = 5.0f;         // the maximum is raised once a score is 2^5 above it
@@ -343,6 +345,13 @@ __device__ __forceinline__ void kv_wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// A barrier that orders LDS only: loads in flight go on.
+__device__ __forceinline__ void kv_lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 template <int HD>
 struct wh_kv4_dims {
     static constexpr int kSteps = HD / 32;                // products of 32 dims
@@ -354,15 +363,15 @@ struct wh_kv4_dims {
     static constexpr int kStage = 32 * kLd * 2;           // bytes of a wave's block
 };
 
-// Raw rows of a lane: key lane % 16 of two blocks of 16.
-template <int HD>
+// Raw rows of a lane: key lane % 16 of kN blocks of 16.
+template <int HD, int kN>
 struct wh_kv4_raw {
-    uint32_t c[2][wh_kv4_dims<HD>::kPieces][wh_kv4_dims<HD>::kWords];
-    uint32_t s[2][wh_kv4_dims<HD>::kScaleWords];
+    uint32_t c[kN][wh_kv4_dims<HD>::kPieces][wh_kv4_dims<HD>::kWords];
+    uint32_t s[kN][wh_kv4_dims<HD>::kScaleWords];
 };
 
-template <int HD>
-__device__ __forceinline__ void kv_load(wh_kv4_raw<HD>& r, int half, const wh_kv4_plane& p, uint64_t line, uint32_t g) {
+template <int HD, int kN>
+__device__ __forceinline__ void kv_load(wh_kv4_raw<HD, kN>& r, int half, const wh_kv4_plane& p, uint64_t line, uint32_t g) {
     using D = wh_kv4_dims<HD>;
     const uint8_t* c = p.codes + line * (HD / 2) + g * (4 * D::kWords);
 #pragma unroll
@@ -392,20 +401,104 @@ __device__ __forceinline__ void kv_load(wh_kv4_raw<HD>& r, int half, const wh_kv
 }
 
 // The largest scale byte of a raw row.
-template <int HD>
-__device__ __forceinline__ uint32_t kv_top_byte(const wh_kv4_raw<HD>& r, int half) {
+template <int HD, int kN>
+__device__ __forceinline__ uint32_t kv_top_byte(const wh_kv4_raw<HD, kN>& r, int half) {
     uint32_t m = 0;
 #pragma unroll
     for (int k = 0; k < wh_kv4_dims<HD>::kScaleWords; ++k) m = max(m, kv_max_bytes(r.s[half][k]));
     return m;
 }
 
-// Scale of piece j relative to the row's largest byte; 0 where the row is none or holds NaN.
-template <int HD>
-__device__ __forceinline__ float kv_rel(const wh_kv4_raw<HD>& r, int half, int j, uint32_t g, uint32_t top, bool dead) {
+// Scale of piece j relative to the row's largest byte: 2^0 at most, so that
+// decoded values are finite whatever the bytes are.
+template <int HD, int kN>
+__device__ __forceinline__ float kv_rel(const wh_kv4_raw<HD, kN>& r, int half, int j, uint32_t g, uint32_t top) {
     const uint32_t b = HD == 64 ? (r.s[half][0] >> (8 * (g >> 1))) & 0xff : (r.s[half][j] >> (8 * g)) & 0xff;
-    const int e = (int)b - (int)top + 127;
-    return dead ? 0.0f : kv_bits((uint32_t)max(e, 0) << 23);
+    return kv_bits((uint32_t)max((int)b - (int)top + 127, 0) << 23);
+}
+
+// 2^(byte - 127) of a key row, or NaN where it or its value row holds one: the
+// score is NaN then, and with it the weight, in the rows that see the key.
+__device__ __forceinline__ float kv_key_scale(uint32_t ktop, uint32_t vtop) {
+    return ktop == 255 || vtop == 255 ? kv_bits(0x7fc00000u) : kv_bits(ktop << 23);
+}
+// A value row's power of two against the reference; finite.
+__device__ __forceinline__ float kv_value_scale(uint32_t vtop, int ref) {
+    return kv_bits((uint32_t)min(max((int)vtop - ref + 127, 0), 254) << 23);
+}
+
+// First dim of a lane's eight in step s of the product with keys.
+template <int HD>
+__device__ __forceinline__ int kv_dim(int s, uint32_t g) {
+    return HD >= 128 ? 32 * (4 * (s >> 2) + (int)g) + 8 * (s & 3) : 16 * (int)g + 8 * s;
+}
+
+// A lane's part of a query row as it lies in memory: all of it requested at once.
+template <int HD, bool kF32>
+struct wh_kv4_query {
+    wh_u4 raw[HD / 32][kF32 ? 2 : 1];
+
+    // flip = 1: steps 2 i and 2 i + 1 change places
+    __device__ __forceinline__ void load(const void* base, uint64_t at, uint32_t g, uint32_t flip = 0) {
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s) {
+            const uint64_t d = at + kv_dim<HD>(s, g) + (s & 1 ? 0 : 8 * flip) - (s & 1 ? 8 * flip : 0);
+            if constexpr (kF32) {
+                raw[s][0] = *(const wh_u4*)((const float*)base + d);
+                raw[s][1] = *(const wh_u4*)((const float*)base + d + 4);
+            } else {
+                raw[s][0] = *(const wh_u4*)((const uint16_t*)base + d);
+            }
+        }
+    }
+
+    // Scaled, in one or two f16 parts; returns what a sum of products with it is to be multiplied by.
+    __device__ __forceinline__ float parts(wh_h8 (&q)[HD / 32][kF32 ? 2 : 1]) const {
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s)
+#pragma unroll
+            for (int p = 0; p < (kF32 ? 2 : 1); ++p)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t w = raw[s][p][k];
+                    top = max(top, kF32 ? w & 0x7fffffffu : max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
+                }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+        const int e = max((int)(top >> 23), 27);  // of the largest; 2^-100 at least, so that the factor is finite
+        const float up = kv_bits((uint32_t)(127 + 13 + 127 - e) << 23);
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s) {
+            wh_h8 hi, lo;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t w = kF32 ? raw[s][k >> 2][k & 3] : raw[s][0][k >> 1];
+                const float x = kv_bits(kF32 ? w : k & 1 ? w & 0xffff0000u : w << 16) * up;
+                hi[k] = (_Float16)x;
+                if constexpr (kF32) lo[k] = (_Float16)(x - (float)hi[k]);
+            }
+            q[s][0] = hi;
+            if constexpr (kF32) q[s][1] = lo;
+        }
+        return kv_bits((uint32_t)(e - 13) << 23);
+    }
+};
+
+// Four output values at `at`, in the type of the call.
+template <bool kF32>
+__device__ __forceinline__ void kv_store(void* out, uint64_t at, const wh_f4& x) {
+    if constexpr (kF32) {
+        *(wh_f4*)((float*)out + at) = x;
+    } else {
+        union {
+            __bf16 b[4];
+            wh_u2 u;
+        } y;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y.b[k] = (__bf16)x[k];
+        *(wh_u2*)((uint16_t*)out + at) = y.u;
+    }
 }
 
 // Four waves share a tile of 16 rows; wave w takes the blocks of 32 keys w,
@@ -437,49 +530,10 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
     const uint32_t token = min(tile.token0 + tok, a.n_tokens - 1);
     const int32_t pos = live ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
 
-    // the row's query, scaled, in one or two f16 parts
     wh_h8 q[D::kSteps][kParts];
-    float c_row;  // score = c_row * key scale * sum
-    {
-        auto dim = [&](int s) { return HD >= 128 ? 32 * (4 * (s >> 2) + (int)g) + 8 * (s & 3) : 16 * (int)g + 8 * s; };
-        const uint64_t at = (uint64_t)token * a.q_stride + (uint64_t)head * HD;
-        uint32_t top = 0;
-        float v[D::kSteps][8];
-#pragma unroll
-        for (int s = 0; s < D::kSteps; ++s) {
-            if constexpr (kF32) {
-                const wh_f4* p = (const wh_f4*)((const float*)a.q + at + dim(s));
-                const wh_f4 x = p[0], y = p[1];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[s][k] = x[k];
-                    v[s][4 + k] = y[k];
-                }
-            } else {
-                const wh_u4 w = *(const wh_u4*)((const uint16_t*)a.q + at + dim(s));
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[s][2 * k] = kv_bits(w[k] << 16);
-                    v[s][2 * k + 1] = kv_bits(w[k] & 0xffff0000u);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[s][k]) & 0x7fffffffu);
-        }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-        const int e = max((int)(top >> 23), 27);  // of the largest; 2^-100 at least, so that the factor is finite
-        const float up = kv_bits((uint32_t)(127 + 13 + 127 - e) << 23);
-        c_row = a.scale_log2 * kv_bits((uint32_t)max(e - 13, 1) << 23);
-#pragma unroll
-        for (int s = 0; s < D::kSteps; ++s)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float x = v[s][k] * up;
-                q[s][0][k] = (_Float16)x;
-                if constexpr (kF32) q[s][1][k] = (_Float16)(x - (float)q[s][0][k]);
-            }
-    }
+    wh_kv4_query<HD, kF32> query;
+    query.load(a.q, (uint64_t)token * a.q_stride + (uint64_t)head * HD, g);
+    const float c_row = a.scale_log2 * query.parts(q);
 
     wh_f4 acc[HD / 16];  // [dim 4g + i][row] of 16 dims each, times 2^(127 - ref)
 #pragma unroll
@@ -489,51 +543,53 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
 
     const uint32_t* const table = a.tables + tile.request * a.table_stride;
     const uint32_t pmask = (1u << a.s.shift) - 1u;
-    wh_kv4_raw<HD> kr, vr;
-    bool there[2];
+    // a block's rows are requested one block ahead, their pages two
+    wh_kv4_raw<HD, 2> kr, vr;
+    bool there[2], bad = false;
+    uint32_t page[2];
+    auto key_at = [&](uint32_t blk, int h, bool* in) {
+        const uint32_t v = blk * 32 + 16 * h + r16;
+        *in = blk < blk1 && v < tile.n_keys;
+        return *in ? wh_kv4_key(tile, v) : 0;
+    };
+    auto request_pages = [&](uint32_t blk) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            bool in;
+            const uint32_t key = key_at(blk, h, &in);
+            page[h] = in ? table[key >> a.s.shift] : 0;
+        }
+    };
     auto request = [&](uint32_t blk) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t v = blk * 32 + 16 * h + r16;
-            there[h] = blk < blk1 && v < tile.n_keys;
-            const uint32_t key = there[h] ? wh_kv4_key(tile, v) : 0;
-            uint32_t page = there[h] ? table[key >> a.s.shift] : 0;
-            if (page >= a.s.n_pages) {
-                atomicOr(a.status, WH_ST_NOT_RESIDENT);
-                there[h] = false;
-                page = 0;
-            }
-            const uint64_t line = wh_kv4_line(page, kvh, key & pmask, a.s.kv_heads, a.s.shift);
-            kv_load<HD>(kr, h, a.k, line, g);
-            if constexpr (!kLatent) kv_load<HD>(vr, h, a.v, line, g);
+            const uint32_t key = key_at(blk, h, &there[h]);
+            const bool out = page[h] >= a.s.n_pages;
+            bad |= out;
+            const uint64_t line = wh_kv4_line(out ? 0 : page[h], kvh, key & pmask, a.s.kv_heads, a.s.shift);
+            kv_load(kr, h, a.k, line, g);
+            if constexpr (!kLatent) kv_load(vr, h, a.v, line, g);
         }
+        request_pages(blk + 4);
     };
     _Float16* const stage = (_Float16*)(smem + wave * D::kStage);
-    auto put = [&](int h, int j, int w, const wh_h8& x) {
-        const int d = HD >= 128 ? 32 * (4 * j + (int)g) + 8 * w : 16 * (int)g + 8 * w;
-        *(wh_h8*)(stage + (16 * h + r16) * D::kLd + d) = x;
-    };
+    const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
+    const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
 
+    request_pages(blk0 + wave);
+    request(blk0 + wave);
     for (uint32_t blk = blk0 + wave; blk < blk1; blk += 4) {
-        request(blk);
         uint32_t ktop[2], vtop[2];
-        bool dead[2], vdead[2];
+        bool above = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            ktop[h] = kv_top_byte<HD>(kr, h);
-            dead[h] = !there[h] || ktop[h] == 255;
-            if constexpr (kLatent) {
-                vtop[h] = ktop[h];
-                vdead[h] = dead[h];
-            } else {
-                vtop[h] = kv_top_byte<HD>(vr, h);
-                vdead[h] = !there[h] || vtop[h] == 255;
-            }
+            ktop[h] = kv_top_byte(kr, h);
+            vtop[h] = kLatent ? ktop[h] : kv_top_byte(vr, h);
+            above |= there[h] && vtop[h] < 255 && (int)vtop[h] > ref;
         }
         // a value row above the reference: raise it, with room, and scale what is there
-        const bool above = (!vdead[0] && (int)vtop[0] > ref) || (!vdead[1] && (int)vtop[1] > ref);
         if (__ballot(above)) {
-            int top = max(vdead[0] ? 0 : (int)vtop[0], vdead[1] ? 0 : (int)vtop[1]);
+            int top = max(there[0] && vtop[0] < 255 ? (int)vtop[0] : 0, there[1] && vtop[1] < 255 ? (int)vtop[1] : 0);
             for (int off = 8; off >= 1; off >>= 1) top = max(top, __shfl_xor(top, off, 64));
             const int to = min(top + 3, 254);
             const float f = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
@@ -545,51 +601,51 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
         if (g == 0) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float nan = kv_bits(0x7fc00000u);
-                key_scale[wave][0][16 * h + r16] = ktop[h] == 255 ? nan : kv_bits(ktop[h] << 23);
-                key_scale[wave][1][16 * h + r16] =
-                    vtop[h] == 255 ? nan : kv_bits((uint32_t)max((int)vtop[h] - ref + 127, 0) << 23);
+                key_scale[wave][0][16 * h + r16] = kv_key_scale(ktop[h], vtop[h]);
+                key_scale[wave][1][16 * h + r16] = kv_value_scale(vtop[h], ref);
             }
         }
         wh_f4 s[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             s[h] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+            _Float16* const mine = stage + (16 * h + r16) * D::kLd;
 #pragma unroll
-            for (int j = 0; j < D::kPieces; ++j) {
-                const float rel = kv_rel<HD>(kr, h, j, g, ktop[h], dead[h]);
-#pragma unroll
-                for (int w = 0; w < D::kWords; ++w) {
-                    const wh_h8 x = kv_decode(kr.c[h][j][w], rel);
-                    if constexpr (kF32) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[j * D::kWords + w][1], s[h], 0, 0, 0);
-                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[j * D::kWords + w][0], s[h], 0, 0, 0);
-                    if constexpr (kLatent) put(h, j, w, x);
-                }
-            }
-            if constexpr (!kLatent) {
-#pragma unroll
-                for (int j = 0; j < D::kPieces; ++j) {
-                    const float rel = kv_rel<HD>(vr, h, j, g, vtop[h], vdead[h]);
-#pragma unroll
-                    for (int w = 0; w < D::kWords; ++w) put(h, j, w, kv_decode(vr.c[h][j][w], rel));
-                }
+            for (int k = 0; k < D::kSteps; ++k) {
+                const int j = k / D::kWords, w = k - j * D::kWords;
+                const wh_h8 x = kv_decode(kr.c[h][j][w], kv_rel(kr, h, j, g, ktop[h]));
+                if constexpr (kF32) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][1], s[h], 0, 0, 0);
+                s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][0], s[h], 0, 0, 0);
+                if constexpr (kLatent) *(wh_h8*)(mine + kv_dim<HD>(k, g)) = x;
+                else *(wh_h8*)(mine + kv_dim<HD>(k, g)) = kv_decode(vr.c[h][j][w], kv_rel(vr, h, j, g, vtop[h]));
             }
         }
         kv_wave_order();
-        // weights of keys 4g + i of each half, row r16
-        float p[2][4], top = kMinusBig;
-        bool seen[2][4];
+        request(blk + 4);
+        // scores of keys 4g + i of each half, row r16; -inf where it does not see them
+        const uint32_t last = blk * 32 + 31;
+        const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == 16 &&
+                         (!a.window || (int64_t)wh_kv4_key(tile, max(blk * 32, tile.n_first)) + a.window > pos_hi);
+        float top = kMinusBig;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const wh_f4 ks = *(const wh_f4*)&key_scale[wave][0][16 * h + 4 * g];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t v = blk * 32 + 16 * h + 4 * g + i;
-                seen[h][i] = v < tile.n_keys && wh_kv4_sees(pos, wh_kv4_key(tile, v), a.window, a.first);
-                p[h][i] = s[h][i] * (ks[i] * c_row);
-                top = fmaxf(top, seen[h][i] ? p[h][i] : kMinusBig);
-            }
+            s[h] *= ks * c_row;
         }
+        if (!all) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t v = blk * 32 + 16 * h + 4 * g + i;
+                    const bool see = v < tile.n_keys & wh_kv4_sees(pos, wh_kv4_key(tile, v), a.window, a.first);
+                    s[h][i] = see ? s[h][i] : kMinusInf;
+                }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         if (__ballot(top > m + kSlack)) {
@@ -600,14 +656,15 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
             m = to;
         }
         wh_h8 ph, pl;
+        const float up = kUp - m;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const wh_f4 vs = *(const wh_f4*)&key_scale[wave][1][16 * h + 4 * g];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float w = seen[h][i] ? __builtin_amdgcn_exp2f(p[h][i] - m + kUp) : 0.0f;
+                const float w = __builtin_amdgcn_exp2f(s[h][i] + up);
                 l += w;
-                const float x = seen[h][i] ? w * vs[i] : 0.0f;
+                const float x = w * vs[i];
                 ph[4 * h + i] = (_Float16)x;
                 if constexpr (kF32) pl[4 * h + i] = (_Float16)(x - (float)ph[4 * h + i]);
             }
@@ -628,6 +685,7 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
             acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.v, ph, acc[f], 0, 0, 0);
         }
     }
+    if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
 
     // join the four waves
     l += __shfl_xor(l, 16, 64);
@@ -671,16 +729,8 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
         if (!whole) {
             *(wh_f2*)(part + d) = (wh_f2){x[0], x[1]};
             *(wh_f2*)(part + d + 2) = (wh_f2){x[2], x[3]};
-        } else if constexpr (kF32) {
-            *(wh_f4*)((float*)a.out + (uint64_t)(tile.token0 + rtok) * a.out_stride + (uint64_t)rhead * HD + d) = x;
         } else {
-            union {
-                __bf16 b[4];
-                wh_u2 u;
-            } y;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y.b[k] = (__bf16)x[k];
-            *(wh_u2*)((uint16_t*)a.out + (uint64_t)(tile.token0 + rtok) * a.out_stride + (uint64_t)rhead * HD + d) = y.u;
+            kv_store<kF32>(a.out, (uint64_t)(tile.token0 + rtok) * a.out_stride + (uint64_t)rhead * HD + d, x);
         }
     }
     if (!whole && (t & 15) == 0) {
@@ -689,21 +739,326 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
     }
 }
 
-// Joins the splits of a tile: outputs weighted by their sums of weights, and
-// the sink.  16 threads a row.
+// A tile of 64 rows (32 in f32, whose queries and weights are two parts) for
+// the calls that have them: every decoded key serves four blocks of 16 rows.
+// Wave w scores keys 16 (w % 4) .. of each run of 64 against the rows of its
+// half (4 waves: all of them), its queries in registers, and leaves the value
+// rows it decoded and its weights in LDS; it adds the outputs of its share of
+// the dims for all rows and keys.  The two work on neighbouring runs at once, so
+// one barrier a run is enough and the matrix work of one covers the decoding
+// and the loads of the other.  Weights are taken against the running maximum as
+// it is; only a run with a score 2^5 above it (or a value row above the
+// reference) joins the waves' maxima and makes its weights again.
 template <int HD, bool kF32>
+struct wh_kv4_wide {
+    // rows of 256 and 512 dims: queries and outputs of 64 rows fill the registers
+    // of eight waves, the halves decoding the same keys
+    static constexpr int kHalves = HD >= 256 ? 2 : 1, kWaves = 4 * kHalves, kThreads = 64 * kWaves;
+    static constexpr int kParts = kF32 ? 2 : 1, kBlocks = kF32 ? 2 : 4, kRows = 16 * kBlocks;
+    static constexpr int kMine = kBlocks / kHalves;         // blocks of rows that a wave scores
+    static constexpr int kDims = HD / 16 / kWaves;          // blocks of dims that a wave adds up
+    static constexpr int kRun = 64 * wh_kv4_dims<HD>::kLd;  // f16 of a run's decoded rows
+    static constexpr int kPl = 72;                          // f16 between rows of weights
+    static constexpr int kPrun = kParts * kRows * kPl;
+    static constexpr size_t kLds = 2 * 2 * (size_t)(kRun + kPrun);
+};
+
+template <int HD, bool kF32, bool kLatent>
+__global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_attn_wide(wh_kv4_attn_args a) {
+    using D = wh_kv4_dims<HD>;
+    using W = wh_kv4_wide<HD, kF32>;
+    constexpr int kParts = W::kParts, kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kMine = W::kMine;
+    extern __shared__ __align__(16) uint8_t smem[];
+    _Float16* const vbuf = (_Float16*)smem;                      // [2][key][kLd]
+    _Float16* const pbuf = vbuf + 2 * W::kRun;                   // [2][part][row][kPl]
+    __shared__ __align__(16) float key_scale[W::kWaves][2][16];  // [wave][keys', values'][key]
+    __shared__ float wave_m[4][kRows], wave_l[4][kRows], row_m[kRows];
+    __shared__ uint32_t wave_top[4], raise[2];
+    const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
+    const uint32_t kvh = blockIdx.y, kq = wave & 3, half = wave >> 2;
+    const wh_kv4_tile tile = kv_tile<kRows>(a, blockIdx.x);
+    if (!tile.ok) return;
+    const uint32_t per = wh_kv4_per_split(tile.n_keys, 64, a.splits, a.min_blocks), runs = (tile.n_keys + 63) / 64;
+    const uint32_t run0 = blockIdx.z * per, run1 = min(runs, run0 + per);
+    if (blockIdx.z && run0 >= runs) return;
+    const bool whole = per >= runs;
+    if (t < 2) raise[t] = 0;
+    if (t < kRows) row_m[t] = kMinusBig;
+
+    // rows r16 of this wave's blocks
+    wh_h8 q[kMine][D::kSteps][kParts];
+    float c_row[kMine], m[kMine], l[kMine];
+    int32_t pos[kMine];
+    wh_kv4_query<HD, kF32> query[kMine];
+#pragma unroll
+    for (int b = 0; b < kMine; ++b) {
+        const uint32_t r = 16 * (half * kMine + b) + r16, flat = tile.row0 + min(r, tile.rows - 1), tok = flat / a.group;
+        const uint32_t head = kvh * a.group + (flat - tok * a.group);
+        pos[b] = r < tile.rows ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
+        query[b].load(a.q, (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD, g, half);
+        m[b] = kMinusBig;
+        l[b] = 0.0f;
+    }
+#pragma unroll
+    for (int b = 0; b < kMine; ++b) c_row[b] = a.scale_log2 * query[b].parts(q[b]);
+    const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
+    const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
+
+    wh_f4 acc[kDims][kBlocks];  // [dim 16 (kDims wave + f) + 4g + i][row]
+#pragma unroll
+    for (int f = 0; f < kDims; ++f)
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) acc[f][b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+    int ref = 0;
+
+    // a run's rows are requested one run ahead, their page two
+    const uint32_t* const table = a.tables + tile.request * a.table_stride;
+    const uint32_t pmask = (1u << a.s.shift) - 1u;
+    wh_kv4_raw<HD, 1> kr, vr;
+    bool there = false, bad = false;
+    uint32_t page = 0;
+    auto key_at = [&](uint32_t run, bool* in) {
+        const uint32_t v = run * 64 + 16 * kq + r16;
+        *in = run < run1 && v < tile.n_keys;
+        return *in ? wh_kv4_key(tile, v) : 0;
+    };
+    auto request_page = [&](uint32_t run) {
+        bool in;
+        const uint32_t key = key_at(run, &in);
+        page = in ? table[key >> a.s.shift] : 0;
+    };
+    auto request = [&](uint32_t run) {
+        const uint32_t key = key_at(run, &there);
+        const bool out = page >= a.s.n_pages;
+        bad |= out;
+        const uint64_t line = wh_kv4_line(out ? 0 : page, kvh, key & pmask, a.s.kv_heads, a.s.shift);
+        kv_load(kr, 0, a.k, line, g);
+        if constexpr (!kLatent) kv_load(vr, 0, a.v, line, g);
+        request_page(run + 1);
+    };
+
+    // a step of a run's outputs: 32 keys, a block of rows (f32: a part of one);
+    // the values of these keys stay in registers for all blocks
+    wh_h8 x[kDims];
+    auto values_step = [&](uint32_t at, int k) {
+        const int ks = k / (kBlocks * kParts), bp = k - ks * (kBlocks * kParts), b = bp / kParts, p = kParts - 1 - bp % kParts;
+        if (bp == 0) {
+            const _Float16* const vb = vbuf + at * W::kRun + (32 * ks + 4 * g + (r16 >> 2)) * D::kLd + 16 * kDims * wave +
+                                       4 * (r16 & 3);
+#pragma unroll
+            for (int f = 0; f < kDims; ++f) {
+                union {
+                    wh_s4 h[2];
+                    wh_h8 v;
+                } u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) wh_s4*)(vb + 16 * h * D::kLd + 16 * f));
+                x[f] = u.v;
+            }
+        }
+        const wh_h8 w = *(const wh_h8*)(pbuf + at * W::kPrun + (p * kRows + 16 * b + r16) * W::kPl + 32 * ks + 8 * g);
+#pragma unroll
+        for (int f = 0; f < kDims; ++f) acc[f][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[f], w, acc[f][b], 0, 0, 0);
+    };
+    constexpr int kValueSteps = 2 * kBlocks * kParts;
+    wh_f4 s[kMine];
+    auto pass = [&](uint32_t run, auto first) {
+        const uint32_t at = run & 1;
+        const uint32_t ktop = kv_top_byte(kr, 0), vtop = kLatent ? ktop : kv_top_byte(vr, 0);
+        const bool counts = there && vtop < 255;
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) s[b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+        _Float16* const mine = vbuf + at * W::kRun + (16 * kq + r16) * D::kLd + 8 * half;
+        kv_wave_order();
+        if (g == 0) {
+            key_scale[wave][0][r16] = kv_key_scale(ktop, vtop);
+            key_scale[wave][1][r16] = kv_value_scale(vtop, ref);
+        }
+        // scores, 32 dims a step, beside the outputs of the run before
+#pragma unroll
+        for (int k = 0; k < D::kSteps; ++k) {
+            // the second half takes the steps of a pair in the other order: both leave their first in LDS
+            const int j = k / D::kWords, w = k - j * D::kWords;
+            auto word = [&](const wh_kv4_raw<HD, 1>& r) { return W::kHalves == 2 && half ? r.c[0][j][w ^ 1] : r.c[0][j][w]; };
+            const wh_h8 y = kv_decode(word(kr), kv_rel(kr, 0, j, g, ktop));
+#pragma unroll
+            for (int b = 0; b < kMine; ++b)
+#pragma unroll
+                for (int p = kParts - 1; p >= 0; --p)
+                    s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[b][k][p], s[b], 0, 0, 0);
+            if (W::kHalves == 1 || !(k & 1)) {
+                if constexpr (kLatent) *(wh_h8*)(mine + kv_dim<HD>(k, g)) = y;
+                else *(wh_h8*)(mine + kv_dim<HD>(k, g)) = kv_decode(word(vr), kv_rel(vr, 0, j, g, vtop));
+            }
+            if constexpr (!decltype(first)::value) {
+#pragma unroll
+                for (int v = kValueSteps * k / D::kSteps; v < kValueSteps * (k + 1) / D::kSteps; ++v) values_step(at ^ 1, v);
+            }
+        }
+        request(run + 1);
+        kv_wave_order();
+        const wh_f4 ks = *(const wh_f4*)&key_scale[wave][0][4 * g];
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) s[b] *= ks * c_row[b];
+        // -inf where a row does not see this lane's keys
+        const uint32_t v0 = run * 64 + 16 * kq + 4 * g, last = run * 64 + 63;
+        const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == kRows &&
+                         (!a.window || (int64_t)wh_kv4_key(tile, max(run * 64, tile.n_first)) + a.window > pos_hi);
+        if (!all) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t key = wh_kv4_key(tile, v0 + i);
+                const bool in = v0 + i < tile.n_keys;
+#pragma unroll
+                for (int b = 0; b < kMine; ++b) {
+                    const bool see = in & wh_kv4_sees(pos[b], key, a.window, a.first);
+                    s[b][i] = see ? s[b][i] : kMinusInf;
+                }
+            }
+        }
+        float top[kMine], add[kMine];
+        bool over = counts && (int)vtop > ref;
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) {
+            top[b] = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
+            over |= top[b] > m[b] + kSlack;
+        }
+        auto weights = [&] {
+            const wh_f4 vs = *(const wh_f4*)&key_scale[wave][1][4 * g];
+            _Float16* const pw = pbuf + at * W::kPrun + (16 * half * kMine + r16) * W::kPl + 32 * (kq >> 1) + 8 * g + 4 * (kq & 1);
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+                union {
+                    _Float16 h[4];
+                    wh_u2 u;
+                } hi, lo;
+                const float up = kUp - m[b];
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = __builtin_amdgcn_exp2f(s[b][i] + up);
+                    const float x = w[i] * vs[i];
+                    hi.h[i] = (_Float16)x;
+                    lo.h[i] = (_Float16)(x - (float)hi.h[i]);
+                }
+                add[b] = (w[0] + w[1]) + (w[2] + w[3]);
+                *(wh_u2*)(pw + 16 * b * W::kPl) = hi.u;
+                if constexpr (kF32) *(wh_u2*)(pw + (kRows + 16 * b) * W::kPl) = lo.u;
+            }
+        };
+        weights();
+        if (__ballot(over) && lane == 0) raise[at] = run + 1;
+        kv_lds_barrier();
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(raise[at]) == run + 1, 0)) {  // the whole workgroup
+            uint32_t vmax = counts ? vtop : 0;
+            for (int off = 8; off >= 1; off >>= 1) vmax = max(vmax, (uint32_t)__shfl_xor((int)vmax, off, 64));
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+                top[b] = fmaxf(top[b], __shfl_xor(top[b], 16, 64));
+                top[b] = fmaxf(top[b], __shfl_xor(top[b], 32, 64));
+                if (g == 0) wave_m[kq][16 * (half * kMine + b) + r16] = top[b];
+            }
+            if (lane == 0 && half == 0) wave_top[kq] = vmax;
+            kv_lds_barrier();
+            vmax = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
+            const int to = (int)vmax > ref ? min((int)vmax + 3, 254) : ref;
+            const float f_ref = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
+            ref = to;
+            auto raised = [&](uint32_t row) {
+                return fmaxf(fmaxf(row_m[row], fmaxf(wave_m[0][row], wave_m[1][row])), fmaxf(wave_m[2][row], wave_m[3][row]));
+            };
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const uint32_t row = 16 * b + r16;
+                const float f = __builtin_amdgcn_exp2f(row_m[row] - raised(row)) * f_ref;
+#pragma unroll
+                for (int k = 0; k < kDims; ++k) acc[k][b] *= f;
+            }
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+                const float mm = raised(16 * (half * kMine + b) + r16);
+                l[b] *= __builtin_amdgcn_exp2f(m[b] - mm);
+                m[b] = mm;
+            }
+            if (g == 0) key_scale[wave][1][r16] = kv_value_scale(vtop, ref);
+            kv_wave_order();
+            weights();
+            kv_lds_barrier();
+#pragma unroll
+            for (int b = 0; b < kMine; ++b)
+                if (kq == 0 && g == 0) row_m[16 * (half * kMine + b) + r16] = m[b];
+        }
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) l[b] += add[b];
+    };
+
+    request_page(run0);
+    request(run0);
+    kv_lds_barrier();
+    if (run0 < run1) pass(run0, std::true_type());
+    for (uint32_t run = run0 + 1; run < run1; ++run) pass(run, std::false_type());
+    if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
+    if (run0 < run1) {
+#pragma unroll
+        for (int k = 0; k < kValueSteps; ++k) values_step((run1 - 1) & 1, k);
+    }
+
+#pragma unroll
+    for (int b = 0; b < kMine; ++b) {
+        l[b] += __shfl_xor(l[b], 16, 64);
+        l[b] += __shfl_xor(l[b], 32, 64);
+        if (g == 0) wave_l[kq][16 * (half * kMine + b) + r16] = l[b];
+    }
+    kv_lds_barrier();
+    const float up = kv_bits((uint32_t)ref << 23);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const uint32_t r = 16 * b + r16;
+        if (r >= tile.rows) continue;
+        const uint32_t flat = tile.row0 + r, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
+        const float L = (wave_l[0][r] + wave_l[1][r]) + (wave_l[2][r] + wave_l[3][r]), M = row_m[r];
+        float denom = L;
+        if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
+        const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
+        float* const part = a.part + ((((uint64_t)blockIdx.x * a.s.kv_heads + kvh) * a.splits + blockIdx.z) * kRows + r) * (HD + 2);
+        const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
+#pragma unroll
+        for (int f = 0; f < kDims; ++f) {
+            const uint32_t d = 16 * (kDims * wave + f) + 4 * g;
+            const wh_f4 y = acc[f][b] * up * inv;
+            if (!whole) {
+                *(wh_f2*)(part + d) = (wh_f2){y[0], y[1]};
+                *(wh_f2*)(part + d + 2) = (wh_f2){y[2], y[3]};
+            } else {
+                kv_store<kF32>(a.out, at + d, y);
+            }
+        }
+        if (!whole && wave == 0 && g == 0) {
+            part[HD] = M;
+            part[HD + 1] = L;
+        }
+    }
+}
+
+// Joins the splits of a tile of kRows rows, keys counted in blocks of kKeys:
+// outputs weighted by their sums of weights, and the sink.  16 threads a row,
+// 16 rows a workgroup.
+template <int HD, bool kF32, int kRows, int kKeys>
 __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
     const uint32_t t = threadIdx.x, kvh = blockIdx.y;
-    const wh_kv4_tile tile = kv_tile<16>(a, blockIdx.x);
+    const wh_kv4_tile tile = kv_tile<kRows>(a, blockIdx.x);
     if (!tile.ok) return;
-    const uint32_t per = kv_split_blocks(a, tile.n_keys), blocks = (tile.n_keys + 31) / 32;
+    const uint32_t per = wh_kv4_per_split(tile.n_keys, kKeys, a.splits, a.min_blocks);
+    const uint32_t blocks = (tile.n_keys + kKeys - 1) / kKeys;
     if (per >= blocks) return;
     const uint32_t n = (blocks + per - 1) / per;
-    const uint32_t row = t >> 4, d0 = (t & 15) * 4;
+    const uint32_t row = 16 * blockIdx.z + (t >> 4), d0 = (t & 15) * 4;
+    if (row >= tile.rows) return;
     const uint32_t flat = tile.row0 + row, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
-    if (row >= tile.rows || tile.token0 + tok >= a.n_tokens) return;
-    const float* const part = a.part + (((uint64_t)blockIdx.x * a.s.kv_heads + kvh) * a.splits * 16 + row) * (HD + 2);
-    constexpr uint64_t kNext = 16 * (HD + 2);
+    const float* const part = a.part + (((uint64_t)blockIdx.x * a.s.kv_heads + kvh) * a.splits * kRows + row) * (HD + 2);
+    constexpr uint64_t kNext = kRows * (HD + 2);
     float M = kMinusBig, L = 0.0f;
     for (uint32_t k = 0; k < n; ++k) M = fmaxf(M, part[k * kNext + HD]);
     wh_f4 x[HD / 64];
@@ -723,30 +1078,28 @@ __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i) {
-        const wh_f4 y = x[i] * inv;
-        if constexpr (kF32) {
-            *(wh_f4*)((float*)a.out + at + 64 * i + d0) = y;
-        } else {
-            union {
-                __bf16 b[4];
-                wh_u2 u;
-            } z;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) z.b[k] = (__bf16)y[k];
-            *(wh_u2*)((uint16_t*)a.out + at + 64 * i + d0) = z.u;
-        }
-    }
+    for (int i = 0; i < HD / 64; ++i) kv_store<kF32>(a.out, at + 64 * i + d0, x[i] * inv);
 }
 
 template <int HD, bool kF32, bool kLatent>
 hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
+    const dim3 grid(a.n_tiles, a.s.kv_heads, a.splits);
+    if (a.wide) {
+        using W = wh_kv4_wide<HD, kF32>;
+        static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_wide<HD, kF32, kLatent>,
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
+        if (set != hipSuccess) return set;
+        k_kv4_attn_wide<HD, kF32, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
+        if (a.splits > 1)
+            k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles, a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
+        return hipGetLastError();
+    }
     constexpr size_t lds = 4 * (size_t)wh_kv4_dims<HD>::kStage;
     static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn<HD, kF32, kLatent>,
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (set != hipSuccess) return set;
-    k_kv4_attn<HD, kF32, kLatent><<<dim3(a.n_tiles, a.s.kv_heads, a.splits), 256, lds, stream>>>(a);
-    if (a.splits > 1) k_kv4_join<HD, kF32><<<dim3(a.n_tiles, a.s.kv_heads), 256, 0, stream>>>(a);
+    k_kv4_attn<HD, kF32, kLatent><<<grid, 256, lds, stream>>>(a);
+    if (a.splits > 1) k_kv4_join<HD, kF32, 16, 32><<<dim3(a.n_tiles, a.s.kv_heads), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -784,17 +1137,22 @@ hipError_t wh_kv4_read_launch(const wh_kv4_rows_args& a, bool bf16, hipStream_t 
 }
 
 wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, bool latent, size_t max_len) {
-    (void)bf16;
     (void)latent;
     wh_kv4_attn_plan p{};
-    p.n_tiles = (uint32_t)((uint64_t)a.n_tokens * a.group / 16 + a.n_requests);
+    const uint64_t rows = (uint64_t)a.n_tokens * a.group;
+    const uint32_t wide_rows = bf16 ? 64 : 32;
+    p.wide = rows >= (uint64_t)a.n_requests * (wide_rows - 16);
+    const uint32_t tile_rows = p.wide ? wide_rows : 16, block = p.wide ? 64 : 32;
+    p.n_tiles = (uint32_t)wh_kv4_tile_slots(a.n_tokens, a.n_requests, a.group, tile_rows);
     const uint64_t wgs = (uint64_t)p.n_tiles * a.s.kv_heads;
+    const uint64_t busy = std::max<uint64_t>(rows / tile_rows, a.n_requests) * a.s.kv_heads;  // tiles that hold rows, about
     uint64_t keys = max_len;
     if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.first + a.n_tokens);
-    const uint64_t want = (512 + wgs - 1) / wgs, most = (keys + 127) / 128;
+    const uint64_t target = a.s.head_dim >= 256 ? 256 : 512;
+    const uint64_t want = target / busy, most = (keys + 127) / 128;
     p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, std::min<uint64_t>(most, 64)));
-    p.min_blocks = 4;
-    if (p.splits > 1) p.part_bytes = wgs * p.splits * 16 * (a.s.head_dim + 2) * sizeof(float);
+    p.min_blocks = 128 / block;
+    if (p.splits > 1) p.part_bytes = wgs * p.splits * tile_rows * (a.s.head_dim + 2) * sizeof(float);
     return p;
 }
 

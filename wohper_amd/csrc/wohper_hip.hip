@@ -4810,6 +4810,7 @@ int wh_kv4_attention_async(wh_ctx* c, const wh_kv4_cache* cache, const wh_kv4_at
     a.splits = p.splits;
     a.min_blocks = p.min_blocks;
     a.n_tiles = p.n_tiles;
+    a.wide = p.wide;
     WH_HIP(c->kv4_part.ensure(p.part_bytes, false));
     a.part = c->kv4_part.as<float>();
     WH_HIP(wh_kv4_attn_launch(a, d->is_bf16 != 0, !has_v, c->stream));
