@@ -5,11 +5,15 @@ they can go wrong.
 Tolerances are sums of half-step roundings, u = 2^-24 for f32:
   a score of d products added in f32, its query in two f16 parts (2^-22) and
   three factors: (d + 12) u of scale * sum |q||k|, and d u of the largest
-  |q| * |k| for what f16 drops 2^-24 below a row's largest;
+  |q| * |k| for what f16 drops 2^-24 below a row's largest; bf16 queries are
+  two E4M3 parts of 32 values each, the largest in [2^7, 2^8) and the second
+  part in steps of 2^-13 at least: half a step is 2^-21 = 8 u of the largest;
   a weight: twice the largest score error, 4 u of the largest score, and the
   rounding of the weight itself (f32 2^-22, bf16 one f16: 2^-11);
   sums of n weights and products: 2 n + 16 u, and f16's smallest step under
-  the largest weight: 2 n u of the largest |v|;
+  the largest weight: 2 n u of the largest |v|; bf16 also takes value rows
+  against the largest of all, in f16 steps of 2^-24 of at most 16 times the
+  largest |v|: 8 u of it;
   the output: 4 u, or half a step of bf16, 2^-8."""
 import math
 
@@ -416,9 +420,9 @@ class Case:
                 km = torch.where(see, k.abs().amax(1)[None], 0.0).amax(1)
                 vm = torch.where(see, v.abs().amax(1)[None], 0.0).amax(1)
                 cnt = see.sum(1)
-                delta = self.scale * ((d + 12) * U * ab + d * U * q[:, h].abs().amax(1) * km)
+                delta = self.scale * ((d + 12) * U * ab + (8 if self.bf16 else 1) * d * U * q[:, h].abs().amax(1) * km)
                 rel = 2 * delta + 4 * U * big + (2 * cnt + 16) * U + (2.0 ** -11 if self.bf16 else 2.0 ** -22)
-                tol[:, h] = rel[:, None] * W + (2 * cnt * U * vm)[:, None] + (2.0 ** -8 if self.bf16 else 4 * U) * out[:, h].abs()
+                tol[:, h] = rel[:, None] * W + ((2 * cnt + 8) * U * vm)[:, None] + (2.0 ** -8 if self.bf16 else 4 * U) * out[:, h].abs()
             outs.append(out.flatten(1))
             tols.append(tol.flatten(1))
         return torch.cat(outs), torch.cat(tols)

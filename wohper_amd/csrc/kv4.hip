@@ -371,6 +371,22 @@ struct wh_kv4_raw {
 };
 
 template <int HD, int kN>
+__device__ __forceinline__ void kv_load_scales(wh_kv4_raw<HD, kN>& r, int half, const wh_kv4_plane& p, uint64_t line) {
+    const uint8_t* s = p.scales + line * (HD / 32);
+    if constexpr (HD == 64) r.s[half][0] = *(const uint16_t*)s;
+    else if constexpr (HD == 128) r.s[half][0] = *(const uint32_t*)s;
+    else if constexpr (HD == 256) {
+        const wh_u2 w = *(const wh_u2*)s;
+        r.s[half][0] = w[0];
+        r.s[half][1] = w[1];
+    } else {
+        const wh_u4 w = *(const wh_u4*)s;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r.s[half][k] = w[k];
+    }
+}
+
+template <int HD, int kN>
 __device__ __forceinline__ void kv_load(wh_kv4_raw<HD, kN>& r, int half, const wh_kv4_plane& p, uint64_t line, uint32_t g) {
     using D = wh_kv4_dims<HD>;
     const uint8_t* c = p.codes + line * (HD / 2) + g * (4 * D::kWords);
@@ -386,20 +402,8 @@ __device__ __forceinline__ void kv_load(wh_kv4_raw<HD, kN>& r, int half, const w
             r.c[half][j][1] = w[1];
         }
     }
-    const uint8_t* s = p.scales + line * (HD / 32);
-    if constexpr (HD == 64) r.s[half][0] = *(const uint16_t*)s;
-    else if constexpr (HD == 128) r.s[half][0] = *(const uint32_t*)s;
-    else if constexpr (HD == 256) {
-        const wh_u2 w = *(const wh_u2*)s;
-        r.s[half][0] = w[0];
-        r.s[half][1] = w[1];
-    } else {
-        const wh_u4 w = *(const wh_u4*)s;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) r.s[half][k] = w[k];
-    }
+    kv_load_scales(r, half, p, line);
 }
-
 // The largest scale byte of a raw row.
 template <int HD, int kN>
 __device__ __forceinline__ uint32_t kv_top_byte(const wh_kv4_raw<HD, kN>& r, int half) {
@@ -407,6 +411,18 @@ __device__ __forceinline__ uint32_t kv_top_byte(const wh_kv4_raw<HD, kN>& r, int
 #pragma unroll
     for (int k = 0; k < wh_kv4_dims<HD>::kScaleWords; ++k) m = max(m, kv_max_bytes(r.s[half][k]));
     return m;
+}
+
+// Scale bytes of a lane's pieces, piece j in byte j.
+template <int HD, int kN>
+__device__ __forceinline__ uint32_t kv_piece_scales(const wh_kv4_raw<HD, kN>& r, uint32_t g) {
+    const uint32_t pick = g | (4 + g) << 8;
+    if constexpr (HD == 128) return r.s[0][0] >> (8 * g);
+    if constexpr (HD == 256) return __builtin_amdgcn_perm(r.s[0][1], r.s[0][0], pick);
+    if constexpr (HD == 512)
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(r.s[0][3], r.s[0][2], pick),
+                                     __builtin_amdgcn_perm(r.s[0][1], r.s[0][0], pick), 0x05040100u);
+    return 0;
 }
 
 // Scale of piece j relative to the row's largest byte: 2^0 at most, so that
@@ -772,7 +788,9 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
     _Float16* const vbuf = (_Float16*)smem;                      // [2][key][kLd]
     _Float16* const pbuf = vbuf + 2 * W::kRun;                   // [2][part][row][kPl]
     __shared__ __align__(16) float key_scale[W::kWaves][2][16];  // [wave][keys', values'][key]
-    __shared__ float wave_m[4][kRows], wave_l[4][kRows], row_m[kRows];
+    // of each row: the maximum, what its scores are multiplied by, its position
+    __shared__ float wave_m[4][kRows], wave_l[4][kRows], row_m[kRows], row_c[kRows];
+    __shared__ int32_t row_pos[kRows];
     __shared__ uint32_t wave_top[4], raise[2];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
     const uint32_t kvh = blockIdx.y, kq = wave & 3, half = wave >> 2;
@@ -785,22 +803,21 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
     if (t < 2) raise[t] = 0;
     if (t < kRows) row_m[t] = kMinusBig;
 
-    // rows r16 of this wave's blocks
+    // queries of rows r16 of this wave's blocks
     wh_h8 q[kMine][D::kSteps][kParts];
-    float c_row[kMine], m[kMine], l[kMine];
-    int32_t pos[kMine];
+    float l[kMine];
     wh_kv4_query<HD, kF32> query[kMine];
 #pragma unroll
     for (int b = 0; b < kMine; ++b) {
         const uint32_t r = 16 * (half * kMine + b) + r16, flat = tile.row0 + min(r, tile.rows - 1), tok = flat / a.group;
         const uint32_t head = kvh * a.group + (flat - tok * a.group);
-        pos[b] = r < tile.rows ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
         query[b].load(a.q, (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD, g, half);
-        m[b] = kMinusBig;
+        row_pos[r] = r < tile.rows ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
         l[b] = 0.0f;
     }
 #pragma unroll
-    for (int b = 0; b < kMine; ++b) c_row[b] = a.scale_log2 * query[b].parts(q[b]);
+    for (int b = 0; b < kMine; ++b) row_c[16 * (half * kMine + b) + r16] = a.scale_log2 * query[b].parts(q[b]);
+    const uint32_t row0 = 16 * half * kMine + r16;  // of block 0
     const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
     const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
 
@@ -839,14 +856,16 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
 
     // a step of a run's outputs: 32 keys, a block of rows (f32: a part of one);
     // the values of these keys stay in registers for all blocks
-    wh_h8 x[kDims];
+    constexpr int kTake = kDims < 2 ? kDims : 2;
+    wh_h8 x[kTake];
     auto values_step = [&](uint32_t at, int k) {
-        const int ks = k / (kBlocks * kParts), bp = k - ks * (kBlocks * kParts), b = bp / kParts, p = kParts - 1 - bp % kParts;
+        const int kf = k / (kBlocks * kParts), ks = kf / (kDims / kTake), f0 = kf % (kDims / kTake) * kTake;
+        const int bp = k - kf * (kBlocks * kParts), b = bp / kParts, p = kParts - 1 - bp % kParts;
         if (bp == 0) {
-            const _Float16* const vb = vbuf + at * W::kRun + (32 * ks + 4 * g + (r16 >> 2)) * D::kLd + 16 * kDims * wave +
-                                       4 * (r16 & 3);
+            const _Float16* const vb = vbuf + at * W::kRun + (32 * ks + 4 * g + (r16 >> 2)) * D::kLd +
+                                       16 * (kDims * wave + f0) + 4 * (r16 & 3);
 #pragma unroll
-            for (int f = 0; f < kDims; ++f) {
+            for (int f = 0; f < kTake; ++f) {
                 union {
                     wh_s4 h[2];
                     wh_h8 v;
@@ -860,9 +879,10 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
         }
         const wh_h8 w = *(const wh_h8*)(pbuf + at * W::kPrun + (p * kRows + 16 * b + r16) * W::kPl + 32 * ks + 8 * g);
 #pragma unroll
-        for (int f = 0; f < kDims; ++f) acc[f][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[f], w, acc[f][b], 0, 0, 0);
+        for (int f = 0; f < kTake; ++f)
+            acc[f0 + f][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[f], w, acc[f0 + f][b], 0, 0, 0);
     };
-    constexpr int kValueSteps = 2 * kBlocks * kParts;
+    constexpr int kValueSteps = 2 * kBlocks * kParts * (kDims / kTake);
     wh_f4 s[kMine];
     auto pass = [&](uint32_t run, auto first) {
         const uint32_t at = run & 1;
@@ -901,7 +921,7 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
         kv_wave_order();
         const wh_f4 ks = *(const wh_f4*)&key_scale[wave][0][4 * g];
 #pragma unroll
-        for (int b = 0; b < kMine; ++b) s[b] *= ks * c_row[b];
+        for (int b = 0; b < kMine; ++b) s[b] *= ks * row_c[row0 + 16 * b];
         // -inf where a row does not see this lane's keys
         const uint32_t v0 = run * 64 + 16 * kq + 4 * g, last = run * 64 + 63;
         const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == kRows &&
@@ -913,7 +933,7 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
                 const bool in = v0 + i < tile.n_keys;
 #pragma unroll
                 for (int b = 0; b < kMine; ++b) {
-                    const bool see = in & wh_kv4_sees(pos[b], key, a.window, a.first);
+                    const bool see = in & wh_kv4_sees(row_pos[row0 + 16 * b], key, a.window, a.first);
                     s[b][i] = see ? s[b][i] : kMinusInf;
                 }
             }
@@ -923,9 +943,9 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
 #pragma unroll
         for (int b = 0; b < kMine; ++b) {
             top[b] = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
-            over |= top[b] > m[b] + kSlack;
+            over |= top[b] > row_m[row0 + 16 * b] + kSlack;
         }
-        auto weights = [&] {
+        auto weights = [&](auto max_of) {
             const wh_f4 vs = *(const wh_f4*)&key_scale[wave][1][4 * g];
             _Float16* const pw = pbuf + at * W::kPrun + (16 * half * kMine + r16) * W::kPl + 32 * (kq >> 1) + 8 * g + 4 * (kq & 1);
 #pragma unroll
@@ -934,7 +954,7 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
                     _Float16 h[4];
                     wh_u2 u;
                 } hi, lo;
-                const float up = kUp - m[b];
+                const float up = kUp - max_of(b);
                 float w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -948,7 +968,7 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
                 if constexpr (kF32) *(wh_u2*)(pw + (kRows + 16 * b) * W::kPl) = lo.u;
             }
         };
-        weights();
+        weights([&](int b) { return row_m[row0 + 16 * b]; });
         if (__ballot(over) && lane == 0) raise[at] = run + 1;
         kv_lds_barrier();
         if (__builtin_expect(__builtin_amdgcn_readfirstlane(raise[at]) == run + 1, 0)) {  // the whole workgroup
@@ -976,19 +996,20 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
 #pragma unroll
                 for (int k = 0; k < kDims; ++k) acc[k][b] *= f;
             }
+            float m[kMine];
 #pragma unroll
             for (int b = 0; b < kMine; ++b) {
-                const float mm = raised(16 * (half * kMine + b) + r16);
-                l[b] *= __builtin_amdgcn_exp2f(m[b] - mm);
-                m[b] = mm;
+                m[b] = raised(row0 + 16 * b);
+                l[b] *= __builtin_amdgcn_exp2f(row_m[row0 + 16 * b] - m[b]);
             }
             if (g == 0) key_scale[wave][1][r16] = kv_value_scale(vtop, ref);
             kv_wave_order();
-            weights();
+            weights([&](int b) { return m[b]; });
             kv_lds_barrier();
 #pragma unroll
             for (int b = 0; b < kMine; ++b)
-                if (kq == 0 && g == 0) row_m[16 * (half * kMine + b) + r16] = m[b];
+                if (kq == 0 && g == 0) row_m[row0 + 16 * b] = m[b];
+            kv_lds_barrier();
         }
 #pragma unroll
         for (int b = 0; b < kMine; ++b) l[b] += add[b];
@@ -1042,6 +1063,422 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
     }
 }
 
+// The same tile for bf16 queries on rows of 128 dims and more, where the cached
+// codes are an operand of the scores as they lie: the block-scaled matrix
+// instruction takes E2M1 codes with a power of two for every 32 dims, which is
+// the cache's format, against a query of two E4M3 parts with powers of two of
+// their own (four significant bits each, so a bf16 is exact down to 2^-14 of the
+// largest of its 32).  Nothing of a key is decoded then but its value row, once,
+// into f16 relative to one reference byte `ref` (exact for scales down to 2^-20
+// of the largest seen).  Wave (kq, rq) scores its keys against its rows, adds
+// its dims of the run before for all rows, and decodes a share of the run's
+// value rows, which lie in LDS with the weights: one barrier a run.
+typedef int wh_i8 __attribute__((ext_vector_type(8)));
+typedef int wh_i4 __attribute__((ext_vector_type(4)));
+
+template <int HD, bool kLatent>
+struct wh_kv4_direct {
+    static constexpr int kRows = 64, kBlocks = 4;
+    static constexpr int kPieces = HD / 128;                      // products of 128 dims
+    static constexpr int kRowGroups = HD >= 256 ? 4 : 1;          // waves that score the same keys
+    static constexpr int kKeyGroups = HD >= 256 ? 2 : 4;
+    static constexpr int kWaves = kRowGroups * kKeyGroups, kThreads = 64 * kWaves;
+    static constexpr int kMine = kBlocks / kRowGroups;            // blocks of rows that a wave scores
+    static constexpr int kKeys = 4 / kKeyGroups;                  // blocks of 16 keys that a wave scores
+    static constexpr int kTasks = kKeys * kPieces / kRowGroups;   // pieces of value rows that a lane decodes
+    static constexpr int kDims = HD / 16 / kWaves;                // blocks of dims that a wave adds up
+    static constexpr int kRun = 64 * wh_kv4_dims<HD>::kLd;        // f16 of a run's decoded rows
+    static constexpr int kPl = 72;                                // f16 between rows of weights
+    static constexpr int kPrun = kRows * kPl;
+    static constexpr size_t kLds = 2 * 2 * (size_t)(kRun + kPrun);
+};
+
+// A lane's 32 of 128 bf16 values of a query as two E4M3 parts: dims 16g .. of
+// the first half and of the second, where the instruction wants 8-bit values (it
+// takes 4-bit ones and all scales as 32g ..).  Returns the first part's scale
+// byte for dims 32g .. (the second's is 4 less), 255 where one is not finite.
+__device__ __forceinline__ uint32_t kv_query_e4m3(const wh_u4 (&raw)[2][2], uint32_t flip, wh_i8& hi, wh_i8& lo) {
+    int e[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t w = raw[h][i][k];
+                top = max(top, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
+            }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));  // the other 16 of the 32
+        e[h] = max((int)(top >> 23), 20);
+        const float up = kv_bits((uint32_t)(127 + 127 + 7 - min(e[h], 254)) << 23);  // the largest to [2^7, 2^8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int a = 0, b = 0;
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t w = raw[h][i >> 1][2 * (i & 1) + (k >> 1)] ^ flip;
+                x[k] = kv_bits(k & 1 ? w & 0xffff0000u : w << 16) * up;
+            }
+            a = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], a, false);
+            a = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], a, true);
+            const wh_f2 u = __builtin_amdgcn_cvt_pk_f32_fp8(a, false), v = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
+            b = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - u.x) * 16.0f, (x[1] - u.y) * 16.0f, b, false);
+            b = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - v.x) * 16.0f, (x[3] - v.y) * 16.0f, b, true);
+            hi[4 * h + i] = a;
+            lo[4 * h + i] = b;
+        }
+    }
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, from = (lane & 15) + 32 * (g & 1);
+    const int e0 = __shfl(e[0], (int)from, 64), e1 = __shfl(e[1], (int)from, 64), w = g < 2 ? e0 : e1;
+    return w == 255 ? 255u : (uint32_t)(w - 7);
+}
+
+template <int HD, bool kLatent>
+__global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_kv4_attn_direct(wh_kv4_attn_args a) {
+    using D = wh_kv4_dims<HD>;
+    using W = wh_kv4_direct<HD, kLatent>;
+    constexpr int kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kMine = W::kMine, kKeys = W::kKeys,
+                  kPieces = W::kPieces, kTasks = W::kTasks;
+    extern __shared__ __align__(16) uint8_t smem[];
+    _Float16* const vbuf = (_Float16*)smem;     // [2][key][kLd]
+    _Float16* const pbuf = vbuf + 2 * W::kRun;  // [2][row][kPl]
+    __shared__ float wave_m[W::kKeyGroups][kRows], wave_l[W::kKeyGroups][kRows], row_m[kRows];
+    __shared__ int32_t row_pos[kRows];
+    __shared__ uint32_t wave_top[W::kWaves], raise[2];
+    __shared__ uint64_t nan_keys[2];
+    const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
+    const uint32_t kvh = blockIdx.y, kq = wave % W::kKeyGroups, rq = wave / W::kKeyGroups;
+    const wh_kv4_tile tile = kv_tile<kRows>(a, blockIdx.x);
+    if (!tile.ok) return;
+    const uint32_t per = wh_kv4_per_split(tile.n_keys, 64, a.splits, a.min_blocks), runs = (tile.n_keys + 63) / 64;
+    const uint32_t run0 = blockIdx.z * per, run1 = min(runs, run0 + per);
+    if (blockIdx.z && run0 >= runs) return;
+    const bool whole = per >= runs;
+    if (t < 2) raise[t] = 0;
+    if (t < 2) nan_keys[t] = 0;
+    if (t < kRows) row_m[t] = kMinusBig;
+
+    // a run's key rows are requested one run ahead, their pages two
+    const uint32_t* const table = a.tables + tile.request * a.table_stride;
+    const uint32_t pmask = (1u << a.s.shift) - 1u;
+    bool bad = false;
+    uint32_t page[kKeys];
+    uint64_t line[kKeys], vline[kKeys];  // of the requested run, of the run before
+    wh_u4 kc[kKeys][kPieces];
+    wh_kv4_raw<HD, 1> ks[kKeys];  // scale bytes only
+    auto key_at = [&](uint32_t run, int b, bool* in) {
+        const uint32_t v = run * 64 + 16 * (kKeys * kq + b) + r16;
+        *in = run < run1 && v < tile.n_keys;
+        return *in ? wh_kv4_key(tile, v) : 0;
+    };
+    auto request_pages = [&](uint32_t run) {
+#pragma unroll
+        for (int b = 0; b < kKeys; ++b) {
+            bool in;
+            const uint32_t key = key_at(run, b, &in);
+            page[b] = in ? table[key >> a.s.shift] : 0;
+        }
+    };
+    auto request = [&](uint32_t run) {
+#pragma unroll
+        for (int b = 0; b < kKeys; ++b) {
+            bool in;
+            const uint32_t key = key_at(run, b, &in);
+            const bool out = page[b] >= a.s.n_pages;
+            bad |= out;
+            line[b] = wh_kv4_line(out ? 0 : page[b], kvh, key & pmask, a.s.kv_heads, a.s.shift);
+            const uint8_t* const c = a.k.codes + line[b] * (HD / 2) + 16 * g;
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) kc[b][j] = *(const wh_u4*)(c + 64 * j);
+            kv_load_scales(ks[b], 0, a.k, line[b]);
+        }
+        request_pages(run + 1);
+    };
+
+    request_pages(run0);
+    // queries of rows r16 of this wave's blocks
+    wh_i8 q[kMine][kPieces][2];
+    uint32_t q_scale[kMine];
+    float l[kMine];
+#pragma unroll
+    for (int b = 0; b < kMine; ++b) {
+        const uint32_t r = 16 * (rq * kMine + b) + r16, flat = tile.row0 + min(r, tile.rows - 1), tok = flat / a.group;
+        const uint32_t head = kvh * a.group + (flat - tok * a.group);
+        const uint16_t* const p = (const uint16_t*)a.q + (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD + 16 * g;
+        wh_u4 raw[kPieces][2][2];
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[j][i >> 1][i & 1] = *(const wh_u4*)(p + 128 * j + 64 * (i >> 1) + 8 * (i & 1));
+        q_scale[b] = 0;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j)
+            q_scale[b] |= kv_query_e4m3(raw[j], a.scale_log2 < 0.0f ? 0x80008000u : 0u, q[b][j][0], q[b][j][1]) << (8 * j);
+        row_pos[r] = r < tile.rows ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
+        l[b] = 0.0f;
+    }
+    request(run0);
+    const uint32_t row0 = 16 * rq * kMine + r16;  // of block 0
+    // scores are taken times c > 0 (0 would hide what is masked), the sign is the query's
+    const float c = fmaxf(fabsf(a.scale_log2), 1.0e-37f);
+    const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
+    const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
+
+    wh_f4 acc[kDims][kBlocks];  // [dim 16 (kDims wave + f) + 4g + i][row]
+#pragma unroll
+    for (int f = 0; f < kDims; ++f)
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) acc[f][b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+    int ref = 0;
+
+    // outputs of the run in buffer `at`
+    auto values = [&](uint32_t at) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            wh_h8 x[kDims];
+            const _Float16* const vb = vbuf + at * W::kRun + (32 * h + 4 * g + (r16 >> 2)) * D::kLd + 16 * kDims * wave +
+                                       4 * (r16 & 3);
+#pragma unroll
+            for (int f = 0; f < kDims; ++f) {
+                union {
+                    wh_s4 s[2];
+                    wh_h8 v;
+                } u;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    u.s[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) wh_s4*)(vb + 16 * k * D::kLd + 16 * f));
+                x[f] = u.v;
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const wh_h8 w = *(const wh_h8*)(pbuf + at * W::kPrun + (16 * b + r16) * W::kPl + 32 * h + 8 * g);
+#pragma unroll
+                for (int f = 0; f < kDims; ++f) acc[f][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[f], w, acc[f][b], 0, 0, 0);
+            }
+        }
+    };
+
+    wh_u4 vc[kTasks];
+    uint32_t vb[kTasks];  // scale bytes
+    auto pass = [&](uint32_t run, auto first) {
+        const uint32_t at = run & 1;
+        // this run's value rows: for latent rows the lines that the keys came from
+#pragma unroll
+        for (int i = 0; i < kTasks; ++i) {
+            const int n0 = W::kRowGroups * i;  // task n = rq + n0: block n % kKeys, piece n / kKeys
+            const uint32_t n = rq + n0, j = n / kKeys;
+            const uint64_t ln = kKeys == 2 ? (n & 1 ? line[kKeys - 1] : line[0]) : line[0];
+            vc[i] = *(const wh_u4*)(a.v.codes + ln * (HD / 2) + 64 * j + 16 * g);
+            vb[i] = a.v.scales[ln * (HD / 32) + 4 * j + g];
+        }
+        wh_f4 s[kMine][kKeys];
+#pragma unroll
+        for (int kb = 0; kb < kKeys; ++kb) {
+            const uint32_t scale = kv_piece_scales(ks[kb], g);
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) s[b][kb] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+            wh_static_for<kPieces>([&](auto jc) {
+                constexpr int j = decltype(jc)::value;
+                wh_i8 x;
+                x[0] = kc[kb][j][0], x[1] = kc[kb][j][1], x[2] = kc[kb][j][2], x[3] = kc[kb][j][3];
+                x[4] = x[5] = x[6] = x[7] = 0;
+#pragma unroll
+                for (int b = 0; b < kMine; ++b) {
+                    s[b][kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, q[b][j][1], s[b][kb], 4, 0, j, scale, j,
+                                                                                q_scale[b] - 0x04040404u);
+                    s[b][kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, q[b][j][0], s[b][kb], 4, 0, j, scale, j,
+                                                                                q_scale[b]);
+                }
+            });
+        }
+        request(run + 1);
+        // -inf where a row does not see this lane's keys
+        const uint32_t v0 = run * 64 + 16 * kKeys * kq + 4 * g, last = run * 64 + 63;
+        const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == kRows &&
+                         (!a.window || (int64_t)wh_kv4_key(tile, max(run * 64, tile.n_first)) + a.window > pos_hi);
+        if (!all) {
+#pragma unroll
+            for (int kb = 0; kb < kKeys; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t v = v0 + 16 * kb + i, key = wh_kv4_key(tile, v);
+#pragma unroll
+                    for (int b = 0; b < kMine; ++b) {
+                        const bool see = (v < tile.n_keys) & wh_kv4_sees(row_pos[row0 + 16 * b], key, a.window, a.first);
+                        s[b][kb][i] = see ? s[b][kb][i] : kMinusInf;
+                    }
+                }
+        }
+        if constexpr (!decltype(first)::value) values(at ^ 1);
+        float top[kMine], add[kMine];
+        bool over = false;
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) {
+            top[b] = s[b][0][0];
+#pragma unroll
+            for (int kb = 0; kb < kKeys; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[b] = fmaxf(top[b], s[b][kb][i]);
+            over |= top[b] * c > row_m[row0 + 16 * b] + kSlack;
+        }
+        uint32_t vtop = 0;  // largest byte that counts
+        auto decode = [&] {
+#pragma unroll
+            for (int i = 0; i < kTasks; ++i) {
+                const uint32_t n = rq + W::kRowGroups * i, kb = n % kKeys, j = n / kKeys;
+                const float rel = kv_bits((uint32_t)min(max((int)vb[i] - ref + 127, 0), 127) << 23);
+                _Float16* const dst = vbuf + at * W::kRun + (16 * (kKeys * kq + kb) + r16) * D::kLd + 128 * j + 32 * g;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) *(wh_h8*)(dst + 8 * w) = kv_decode(vc[i][w], rel);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kTasks; ++i) {
+            const uint32_t n = rq + W::kRowGroups * i, kb = n % kKeys;
+            const bool counts = run * 64 + 16 * (kKeys * kq + kb) + r16 < tile.n_keys;
+            vtop = max(vtop, counts && vb[i] < 255 ? vb[i] : 0u);
+            over |= !kLatent && counts && vb[i] == 255;
+        }
+        over |= (int)vtop > ref;
+        decode();
+        auto weights = [&](auto max_of) {
+            _Float16* const pw = pbuf + at * W::kPrun + row0 * W::kPl + (kKeys == 2 ? 32 * kq : 32 * (kq >> 1) + 4 * (kq & 1)) + 8 * g;
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+                const float up = kUp - max_of(b);
+                union {
+                    _Float16 h[4 * kKeys];
+                    uint32_t u[2 * kKeys];
+                } x;
+                add[b] = 0.0f;
+#pragma unroll
+                for (int kb = 0; kb < kKeys; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float w = __builtin_amdgcn_exp2f(fmaf(s[b][kb][i], c, up));
+                        add[b] += w;
+                        x.h[4 * kb + i] = (_Float16)w;
+                    }
+                if constexpr (kKeys == 2) *(wh_u4*)(pw + 16 * b * W::kPl) = (wh_u4){x.u[0], x.u[1], x.u[2], x.u[3]};
+                else *(wh_u2*)(pw + 16 * b * W::kPl) = (wh_u2){x.u[0], x.u[1]};
+            }
+        };
+        weights([&](int b) { return row_m[row0 + 16 * b]; });
+        if (__ballot(over) && lane == 0) raise[at] = run + 1;
+        kv_lds_barrier();
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(raise[at]) == run + 1, 0)) {  // the whole workgroup
+            if constexpr (!kLatent) {  // keys whose value row holds NaN
+#pragma unroll
+                for (int i = 0; i < kTasks; ++i) {
+                    const uint32_t n = rq + W::kRowGroups * i, key = 16 * (kKeys * kq + n % kKeys) + r16;
+                    if (vb[i] == 255 && run * 64 + key < tile.n_keys) atomicOr((unsigned long long*)&nan_keys[at], 1ull << key);
+                }
+            }
+            for (int off = 32; off >= 1; off >>= 1) vtop = max(vtop, (uint32_t)__shfl_xor((int)vtop, off, 64));
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+                top[b] = fmaxf(top[b], __shfl_xor(top[b], 16, 64));
+                top[b] = fmaxf(top[b], __shfl_xor(top[b], 32, 64));
+                if (g == 0) wave_m[kq][row0 + 16 * b] = top[b] * c;
+            }
+            if (lane == 0) wave_top[wave] = vtop;
+            kv_lds_barrier();
+#pragma unroll
+            for (int w = 0; w < W::kWaves; ++w) vtop = max(vtop, wave_top[w]);
+            const int to = (int)vtop > ref ? min((int)vtop + 3, 254) : ref;
+            const float f_ref = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
+            ref = to;
+            auto raised = [&](uint32_t row) {
+                float mm = row_m[row];
+#pragma unroll
+                for (int w = 0; w < W::kKeyGroups; ++w) mm = fmaxf(mm, wave_m[w][row]);
+                return mm;
+            };
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const float f = __builtin_amdgcn_exp2f(row_m[16 * b + r16] - raised(16 * b + r16)) * f_ref;
+#pragma unroll
+                for (int k = 0; k < kDims; ++k) acc[k][b] *= f;
+            }
+            float m[kMine];
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+                m[b] = raised(row0 + 16 * b);
+                l[b] *= __builtin_amdgcn_exp2f(row_m[row0 + 16 * b] - m[b]);
+            }
+            if constexpr (!kLatent) {
+                const uint64_t nan = nan_keys[at];
+#pragma unroll
+                for (int kb = 0; kb < kKeys; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (nan >> (16 * (kKeys * kq + kb) + 4 * g + i) & 1)
+#pragma unroll
+                            for (int b = 0; b < kMine; ++b)
+                                if (s[b][kb][i] != kMinusInf) s[b][kb][i] = kv_bits(0x7fc00000u);
+            }
+            decode();
+            weights([&](int b) { return m[b]; });
+            kv_lds_barrier();
+#pragma unroll
+            for (int b = 0; b < kMine; ++b)
+                if (kq == 0 && g == 0) row_m[row0 + 16 * b] = m[b];
+            if (t == 0) nan_keys[at] = 0;
+            kv_lds_barrier();
+        }
+#pragma unroll
+        for (int b = 0; b < kMine; ++b) l[b] += add[b];
+    };
+
+    kv_lds_barrier();
+    if (run0 < run1) pass(run0, std::true_type());
+    for (uint32_t run = run0 + 1; run < run1; ++run) pass(run, std::false_type());
+    if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
+    if (run0 < run1) values((run1 - 1) & 1);
+
+#pragma unroll
+    for (int b = 0; b < kMine; ++b) {
+        l[b] += __shfl_xor(l[b], 16, 64);
+        l[b] += __shfl_xor(l[b], 32, 64);
+        if (g == 0) wave_l[kq][row0 + 16 * b] = l[b];
+    }
+    kv_lds_barrier();
+    const float up = kv_bits((uint32_t)ref << 23);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const uint32_t r = 16 * b + r16;
+        if (r >= tile.rows) continue;
+        const uint32_t flat = tile.row0 + r, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
+        float L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W::kKeyGroups; ++w) L += wave_l[w][r];
+        const float M = row_m[r];
+        float denom = L;
+        if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
+        const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
+        float* const part = a.part + ((((uint64_t)blockIdx.x * a.s.kv_heads + kvh) * a.splits + blockIdx.z) * kRows + r) * (HD + 2);
+        const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
+#pragma unroll
+        for (int f = 0; f < kDims; ++f) {
+            const uint32_t d = 16 * (kDims * wave + f) + 4 * g;
+            const wh_f4 y = acc[f][b] * up * inv;
+            if (!whole) {
+                *(wh_f2*)(part + d) = (wh_f2){y[0], y[1]};
+                *(wh_f2*)(part + d + 2) = (wh_f2){y[2], y[3]};
+            } else {
+                kv_store<false>(a.out, at + d, y);
+            }
+        }
+        if (!whole && wave == 0 && g == 0) {
+            part[HD] = M;
+            part[HD + 1] = L;
+        }
+    }
+}
+
 // Joins the splits of a tile of kRows rows, keys counted in blocks of kKeys:
 // outputs weighted by their sums of weights, and the sink.  16 threads a row,
 // 16 rows a workgroup.
@@ -1084,7 +1521,18 @@ __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
 template <int HD, bool kF32, bool kLatent>
 hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
     const dim3 grid(a.n_tiles, a.s.kv_heads, a.splits);
-    if (a.wide) {
+    if constexpr (!kF32 && HD >= 128) {
+        if (a.wide) {
+            using W = wh_kv4_direct<HD, kLatent>;
+            static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_direct<HD, kLatent>,
+                                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
+            if (set != hipSuccess) return set;
+            k_kv4_attn_direct<HD, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
+            if (a.splits > 1)
+                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles, a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
+            return hipGetLastError();
+        }
+    } else if (a.wide) {
         using W = wh_kv4_wide<HD, kF32>;
         static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_wide<HD, kF32, kLatent>,
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
