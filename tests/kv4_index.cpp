@@ -40,7 +40,7 @@ int main(int argc, char** argv) {
     const int n = std::atoi(argv[1]);
     for (int it = 0; it < n; ++it) {
         const bool garbage = it & 1;
-        const uint32_t tile_rows = 16u << upto(2), shift = upto(6), group = 1 + upto(it % 3 ? 8 : 70);
+        const uint32_t tile_rows = 16u << upto(2), shift = upto(6), group = it % 7 == 2 ? 16u << upto(3) : 1 + upto(it % 3 ? 8 : 70);
         const uint32_t requests = 1 + upto(it % 5 ? 6 : 150), n_tokens = upto(60);
         const uint32_t table_stride = upto(30), n_pages = 1 + upto(40), kv_heads = 1 + upto(3);
         const uint32_t window = upto(1) ? 0 : 1 + upto(20), first = upto(6);

@@ -20,6 +20,7 @@ typedef _Float16 wh_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 wh_h8 __attribute__((ext_vector_type(8)));
 typedef short wh_s4 __attribute__((ext_vector_type(4)));
 typedef __fp16 wh_hh4 __attribute__((ext_vector_type(4)));
+typedef int wh_i2 __attribute__((ext_vector_type(2)));
 typedef uint32_t wh_u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t wh_u4 __attribute__((ext_vector_type(4)));
 
@@ -316,6 +317,17 @@ __device__ __forceinline__ wh_kv4_tile kv_tile(const wh_kv4_attn_args& a, uint32
     return r;
 }
 
+// A workgroup's tile slot, key head and split: splits next to each other, then
+// heads, so that the slots that hold no rows are spread over the eight XCDs as
+// evenly as the others, and the tiles of one key head (of eight) meet in one L2.
+struct wh_kv4_place {
+    uint32_t slot, head, split;
+};
+__device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a) {
+    const uint32_t x = blockIdx.x / a.splits;
+    return {x / a.s.kv_heads, x % a.s.kv_heads, blockIdx.x % a.splits};
+}
+
 // Blocks of 32 keys of one split.
 __device__ __forceinline__ uint32_t kv_split_blocks(const wh_kv4_attn_args& a, uint32_t n_keys) {
     return wh_kv4_per_split(n_keys, 32, a.splits, a.min_blocks);
@@ -527,16 +539,17 @@ template <int HD, bool kF32, bool kLatent>
 __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
     using D = wh_kv4_dims<HD>;
     constexpr int kParts = kF32 ? 2 : 1;
+    const wh_kv4_place place = kv_place(a);
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(16) float key_scale[4][2][32];  // [wave][keys', values'][key]
     __shared__ float row_m[4][16], row_l[4][16];
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63, r16 = lane & 15, g = lane >> 4;
-    const uint32_t kvh = blockIdx.y;
-    const wh_kv4_tile tile = kv_tile<16>(a, blockIdx.x);
+    const uint32_t kvh = place.head;
+    const wh_kv4_tile tile = kv_tile<16>(a, place.slot);
     if (!tile.ok) return;
     const uint32_t per = kv_split_blocks(a, tile.n_keys), blocks = (tile.n_keys + 31) / 32;
-    const uint32_t blk0 = blockIdx.z * per, blk1 = min(blocks, blk0 + per);
-    if (blockIdx.z && blk0 >= blocks) return;
+    const uint32_t blk0 = place.split * per, blk1 = min(blocks, blk0 + per);
+    if (place.split && blk0 >= blocks) return;
     const bool whole = per >= blocks;  // the only split: the result is final
 
     // this lane's row
@@ -654,7 +667,7 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t v = blk * 32 + 16 * h + 4 * g + i;
-                    const bool see = v < tile.n_keys & wh_kv4_sees(pos, wh_kv4_key(tile, v), a.window, a.first);
+                    const bool see = (v < tile.n_keys) & wh_kv4_sees(pos, wh_kv4_key(tile, v), a.window, a.first);
                     s[h][i] = see ? s[h][i] : kMinusInf;
                 }
         }
@@ -734,7 +747,7 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
     float denom = L;
     if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[rhead] * 1.44269504088896340736f - M + kUp);
     const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-    float* const part = a.part + ((((uint64_t)blockIdx.x * a.s.kv_heads + kvh) * a.splits + blockIdx.z) * 16 + row) * (HD + 2);
+    float* const part = a.part + ((((uint64_t)place.slot * a.s.kv_heads + kvh) * a.splits + place.split) * 16 + row) * (HD + 2);
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i) {
         const uint32_t d = 64 * i + d0;
@@ -784,6 +797,7 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
     using D = wh_kv4_dims<HD>;
     using W = wh_kv4_wide<HD, kF32>;
     constexpr int kParts = W::kParts, kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kMine = W::kMine;
+    const wh_kv4_place place = kv_place(a);
     extern __shared__ __align__(16) uint8_t smem[];
     _Float16* const vbuf = (_Float16*)smem;                      // [2][key][kLd]
     _Float16* const pbuf = vbuf + 2 * W::kRun;                   // [2][part][row][kPl]
@@ -793,12 +807,12 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
     __shared__ int32_t row_pos[kRows];
     __shared__ uint32_t wave_top[4], raise[2];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
-    const uint32_t kvh = blockIdx.y, kq = wave & 3, half = wave >> 2;
-    const wh_kv4_tile tile = kv_tile<kRows>(a, blockIdx.x);
+    const uint32_t kvh = place.head, kq = wave & 3, half = wave >> 2;
+    const wh_kv4_tile tile = kv_tile<kRows>(a, place.slot);
     if (!tile.ok) return;
     const uint32_t per = wh_kv4_per_split(tile.n_keys, 64, a.splits, a.min_blocks), runs = (tile.n_keys + 63) / 64;
-    const uint32_t run0 = blockIdx.z * per, run1 = min(runs, run0 + per);
-    if (blockIdx.z && run0 >= runs) return;
+    const uint32_t run0 = place.split * per, run1 = min(runs, run0 + per);
+    if (place.split && run0 >= runs) return;
     const bool whole = per >= runs;
     if (t < 2) raise[t] = 0;
     if (t < kRows) row_m[t] = kMinusBig;
@@ -1043,7 +1057,7 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
         float denom = L;
         if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
         const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-        float* const part = a.part + ((((uint64_t)blockIdx.x * a.s.kv_heads + kvh) * a.splits + blockIdx.z) * kRows + r) * (HD + 2);
+        float* const part = a.part + ((((uint64_t)place.slot * a.s.kv_heads + kvh) * a.splits + place.split) * kRows + r) * (HD + 2);
         const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
         for (int f = 0; f < kDims; ++f) {
@@ -1141,6 +1155,7 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
     using W = wh_kv4_direct<HD, kLatent>;
     constexpr int kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kMine = W::kMine, kKeys = W::kKeys,
                   kPieces = W::kPieces, kTasks = W::kTasks;
+    const wh_kv4_place place = kv_place(a);
     extern __shared__ __align__(16) uint8_t smem[];
     _Float16* const vbuf = (_Float16*)smem;     // [2][key][kLd]
     _Float16* const pbuf = vbuf + 2 * W::kRun;  // [2][row][kPl]
@@ -1149,12 +1164,12 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
     __shared__ uint32_t wave_top[W::kWaves], raise[2];
     __shared__ uint64_t nan_keys[2];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
-    const uint32_t kvh = blockIdx.y, kq = wave % W::kKeyGroups, rq = wave / W::kKeyGroups;
-    const wh_kv4_tile tile = kv_tile<kRows>(a, blockIdx.x);
+    const uint32_t kvh = place.head, kq = wave % W::kKeyGroups, rq = wave / W::kKeyGroups;
+    const wh_kv4_tile tile = kv_tile<kRows>(a, place.slot);
     if (!tile.ok) return;
     const uint32_t per = wh_kv4_per_split(tile.n_keys, 64, a.splits, a.min_blocks), runs = (tile.n_keys + 63) / 64;
-    const uint32_t run0 = blockIdx.z * per, run1 = min(runs, run0 + per);
-    if (blockIdx.z && run0 >= runs) return;
+    const uint32_t run0 = place.split * per, run1 = min(runs, run0 + per);
+    if (place.split && run0 >= runs) return;
     const bool whole = per >= runs;
     if (t < 2) raise[t] = 0;
     if (t < 2) nan_keys[t] = 0;
@@ -1168,24 +1183,20 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
     uint64_t line[kKeys], vline[kKeys];  // of the requested run, of the run before
     wh_u4 kc[kKeys][kPieces];
     wh_kv4_raw<HD, 1> ks[kKeys];  // scale bytes only
-    auto key_at = [&](uint32_t run, int b, bool* in) {
+    const uint32_t end = min(tile.n_keys, run1 * 64);
+    // the tile's first key stands in for those past the last
+    auto key_at = [&](uint32_t run, int b) {
         const uint32_t v = run * 64 + 16 * (kKeys * kq + b) + r16;
-        *in = run < run1 && v < tile.n_keys;
-        return *in ? wh_kv4_key(tile, v) : 0;
+        return wh_kv4_key(tile, v < end ? v : 0);
     };
     auto request_pages = [&](uint32_t run) {
 #pragma unroll
-        for (int b = 0; b < kKeys; ++b) {
-            bool in;
-            const uint32_t key = key_at(run, b, &in);
-            page[b] = in ? table[key >> a.s.shift] : 0;
-        }
+        for (int b = 0; b < kKeys; ++b) page[b] = table[key_at(run, b) >> a.s.shift];
     };
     auto request = [&](uint32_t run) {
 #pragma unroll
         for (int b = 0; b < kKeys; ++b) {
-            bool in;
-            const uint32_t key = key_at(run, b, &in);
+            const uint32_t key = key_at(run, b);
             const bool out = page[b] >= a.s.n_pages;
             bad |= out;
             line[b] = wh_kv4_line(out ? 0 : page[b], kvh, key & pmask, a.s.kv_heads, a.s.shift);
@@ -1197,7 +1208,7 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
         request_pages(run + 1);
     };
 
-    request_pages(run0);
+    if (run0 < run1) request_pages(run0);
     // queries of rows r16 of this wave's blocks
     wh_i8 q[kMine][kPieces][2];
     uint32_t q_scale[kMine];
@@ -1219,7 +1230,7 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
         row_pos[r] = r < tile.rows ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
         l[b] = 0.0f;
     }
-    request(run0);
+    if (run0 < run1) request(run0);
     const uint32_t row0 = 16 * rq * kMine + r16;  // of block 0
     // scores are taken times c > 0 (0 would hide what is masked), the sign is the query's
     const float c = fmaxf(fabsf(a.scale_log2), 1.0e-37f);
@@ -1275,25 +1286,33 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
             vb[i] = a.v.scales[ln * (HD / 32) + 4 * j + g];
         }
         wh_f4 s[kMine][kKeys];
+        uint32_t scale[kKeys];
 #pragma unroll
         for (int kb = 0; kb < kKeys; ++kb) {
-            const uint32_t scale = kv_piece_scales(ks[kb], g);
+            scale[kb] = kv_piece_scales(ks[kb], g);
 #pragma unroll
             for (int b = 0; b < kMine; ++b) s[b][kb] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
-            wh_static_for<kPieces>([&](auto jc) {
-                constexpr int j = decltype(jc)::value;
-                wh_i8 x;
-                x[0] = kc[kb][j][0], x[1] = kc[kb][j][1], x[2] = kc[kb][j][2], x[3] = kc[kb][j][3];
-                x[4] = x[5] = x[6] = x[7] = 0;
-#pragma unroll
-                for (int b = 0; b < kMine; ++b) {
-                    s[b][kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, q[b][j][1], s[b][kb], 4, 0, j, scale, j,
-                                                                                q_scale[b] - 0x04040404u);
-                    s[b][kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, q[b][j][0], s[b][kb], 4, 0, j, scale, j,
-                                                                                q_scale[b]);
-                }
-            });
         }
+        wh_static_for<kPieces>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+#pragma unroll
+            for (int p = 1; p >= 0; --p)
+#pragma unroll
+                for (int kb = 0; kb < kKeys; ++kb) {
+                    wh_i8 x;
+                    x[0] = kc[kb][j][0], x[1] = kc[kb][j][1], x[2] = kc[kb][j][2], x[3] = kc[kb][j][3];
+                    x[4] = x[5] = x[6] = x[7] = 0;
+#pragma unroll
+                    for (int b = 0; b < kMine; ++b)
+                        s[b][kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                            x, q[b][j][p], s[b][kb], 4, 0, j, scale[kb], j, q_scale[b] - (p ? 0x04040404u : 0u));
+                }
+        });
+        // the next run's rows come into the registers of these: not before they are used
+#pragma unroll
+        for (int b = 0; b < kMine; ++b)
+#pragma unroll
+            for (int kb = 0; kb < kKeys; ++kb) asm volatile("" : "+v"(s[b][kb])::"memory");
         request(run + 1);
         // -inf where a row does not see this lane's keys
         const uint32_t v0 = run * 64 + 16 * kKeys * kq + 4 * g, last = run * 64 + 63;
@@ -1459,7 +1478,370 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
         float denom = L;
         if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
         const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-        float* const part = a.part + ((((uint64_t)blockIdx.x * a.s.kv_heads + kvh) * a.splits + blockIdx.z) * kRows + r) * (HD + 2);
+        float* const part = a.part + ((((uint64_t)place.slot * a.s.kv_heads + kvh) * a.splits + place.split) * kRows + r) * (HD + 2);
+        const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
+#pragma unroll
+        for (int f = 0; f < kDims; ++f) {
+            const uint32_t d = 16 * (kDims * wave + f) + 4 * g;
+            const wh_f4 y = acc[f][b] * up * inv;
+            if (!whole) {
+                *(wh_f2*)(part + d) = (wh_f2){y[0], y[1]};
+                *(wh_f2*)(part + d + 2) = (wh_f2){y[2], y[3]};
+            } else {
+                kv_store<false>(a.out, at + d, y);
+            }
+        }
+        if (!whole && wave == 0 && g == 0) {
+            part[HD] = M;
+            part[HD + 1] = L;
+        }
+    }
+}
+
+// The same for rows of 256 and 512 dims, where the value rows as f16 and the
+// requests of every wave for its own keys were too much: 153 KB of LDS, a third
+// of the time in the address unit (the four waves that score the same keys each
+// read them from memory) and registers for rows in flight.  Here the eight waves
+// bring a run's codes into LDS once, as they lie; the scores read them as
+// operands, and the values are read transposed, sixteen keys of one dim a lane
+// (the 4-bit transposing read), decoded to small f16 numbers and multiplied by
+// their keys' powers of two, which lie beside them relative to `ref`.
+template <int HD, bool kLatent>
+struct wh_kv4_packed {
+    static constexpr int kRows = 64, kBlocks = 4, kWaves = 8, kThreads = 512;
+    static constexpr int kPieces = HD / 128, kDims = HD / 128, kGroups = HD / 32;
+    static constexpr int kMine = HD / 256;            // 16-byte chunks, each a group of 32 dims, that a lane brings
+    static constexpr int kRow = HD / 2;               // bytes of a row's codes
+    static constexpr int kCodes = 64 * kRow;          // bytes of a run's codes
+    static constexpr int kKeyBufs = kLatent ? 3 : 2;  // latent codes are values one run later
+    static constexpr int kRel = 72;                   // f16 between groups of value scales
+    static constexpr int kPl = 72;                    // f16 between rows of weights
+    static constexpr int kAtValues = kKeyBufs * kCodes;                      // byte offsets in LDS
+    static constexpr int kAtScales = kAtValues + (kLatent ? 0 : 3 * kCodes);  // [2][g][key] dwords
+    static constexpr int kAtRel = kAtScales + 2 * 4 * 64 * 4;                // [3][group][key] f16
+    static constexpr int kAtWeights = kAtRel + 3 * kGroups * kRel * 2;       // [2][row][key] f16
+    static constexpr size_t kLds = kAtWeights + 2 * (size_t)kRows * kPl * 2;
+};
+
+template <int HD, bool kLatent>
+__global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) {
+    using W = wh_kv4_packed<HD, kLatent>;
+    constexpr int kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kPieces = W::kPieces;
+    const wh_kv4_place place = kv_place(a);
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float wave_m[2][kRows], wave_l[2][kRows], row_m[kRows];
+    __shared__ int32_t row_pos[kRows];
+    __shared__ uint32_t wave_top[8], raise[2];
+    __shared__ uint64_t nan_keys[3];
+    const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
+    const uint32_t kvh = place.head, kq = wave & 1, rq = wave >> 1;
+    const wh_kv4_tile tile = kv_tile<kRows>(a, place.slot);
+    if (!tile.ok) return;
+    const uint32_t per = wh_kv4_per_split(tile.n_keys, 64, a.splits, a.min_blocks), runs = (tile.n_keys + 63) / 64;
+    const uint32_t run0 = place.split * per, run1 = min(runs, run0 + per);
+    if (place.split && run0 >= runs) return;
+    const bool whole = per >= runs;
+    if (t < 2) raise[t] = 0;
+    if (t < 3) nan_keys[t] = 0;
+    if (t < kRows) row_m[t] = kMinusBig;
+
+    // 16-byte chunk c of a row lies at chunk c ^ swizzle(row): 16 rows of one chunk are on all banks
+    auto swizzle = [](uint32_t key) { return HD == 512 ? key & 15 : (key >> 1) & 7; };
+
+    // this lane's key of a run, and its chunks
+    const uint32_t* const table = a.tables + tile.request * a.table_stride;
+    const uint32_t pmask = (1u << a.s.shift) - 1u, end = min(tile.n_keys, run1 * 64);
+    const uint32_t my_key = 8 * wave + (lane >> 3), my_chunk = W::kMine * (lane & 7);
+    bool bad = false;
+    uint32_t page = 0;
+    wh_u4 kc[W::kMine], vc[W::kMine];
+    uint32_t kb = 0, vb = 0;  // their scale bytes
+    // the tile's first key stands in for those past the last
+    auto key_at = [&](uint32_t run) {
+        const uint32_t v = run * 64 + my_key;
+        return wh_kv4_key(tile, v < end ? v : 0);
+    };
+    auto request_page = [&](uint32_t run) { page = table[key_at(run) >> a.s.shift]; };
+    auto request_of = [&](const wh_kv4_plane& p, uint64_t line, wh_u4 (&c)[W::kMine], uint32_t& b) {
+        const uint8_t* const src = p.codes + line * (HD / 2) + 16 * my_chunk;
+#pragma unroll
+        for (int i = 0; i < W::kMine; ++i) c[i] = *(const wh_u4*)(src + 16 * i);
+        const uint8_t* const sc = p.scales + line * (HD / 32) + my_chunk;
+        b = W::kMine == 2 ? *(const uint16_t*)sc : *sc;
+    };
+    auto request = [&](uint32_t run) {
+        const uint32_t key = key_at(run);
+        const bool out = page >= a.s.n_pages;
+        bad |= out;
+        const uint64_t line = wh_kv4_line(out ? 0 : page, kvh, key & pmask, a.s.kv_heads, a.s.shift);
+        request_of(a.k, line, kc, kb);
+        if constexpr (!kLatent) request_of(a.v, line, vc, vb);
+        request_page(run + 1);
+    };
+    int ref = 0;
+    auto value_bytes = [&] { return kLatent ? kb : vb; };
+    auto counts = [&](uint32_t run) { return run * 64 + my_key < end; };
+    // largest value scale byte of this lane's chunks that counts
+    auto top_byte = [&](uint32_t run) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < W::kMine; ++i) {
+            const uint32_t b = (value_bytes() >> (8 * i)) & 0xff;
+            m = max(m, b < 255 ? b : 0u);
+        }
+        return counts(run) ? m : 0u;
+    };
+    auto stage_rel = [&](uint32_t run) {
+        _Float16* const rel = (_Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel);
+#pragma unroll
+        for (int i = 0; i < W::kMine; ++i) {
+            const int e = (int)((value_bytes() >> (8 * i)) & 0xff) - ref;  // above ref only where it does not count
+            rel[(my_chunk + i) * W::kRel + my_key] = (_Float16)kv_bits((uint32_t)max(min(e, 0) + 127, 0) << 23);
+        }
+    };
+    auto stage = [&](uint32_t run) {
+        uint8_t* const kd = smem + run % W::kKeyBufs * W::kCodes + my_key * W::kRow;
+#pragma unroll
+        for (int i = 0; i < W::kMine; ++i) *(wh_u4*)(kd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = kc[i];
+        uint8_t* const sc = smem + W::kAtScales + (run & 1) * 1024;
+#pragma unroll
+        for (int i = 0; i < W::kMine; ++i) {
+            const uint32_t n = my_chunk + i;
+            sc[((n & 3) * 64 + my_key) * 4 + (n >> 2)] = (uint8_t)(kb >> (8 * i));
+        }
+        if constexpr (!kLatent) {
+            uint8_t* const vd = smem + W::kAtValues + run % 3 * W::kCodes + my_key * W::kRow;
+#pragma unroll
+            for (int i = 0; i < W::kMine; ++i) *(wh_u4*)(vd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = vc[i];
+            bool nan = false;
+#pragma unroll
+            for (int i = 0; i < W::kMine; ++i) nan |= ((vb >> (8 * i)) & 0xff) == 255;
+            if (nan && counts(run)) atomicOr((unsigned long long*)&nan_keys[run % 3], 1ull << my_key);
+        }
+        stage_rel(run);
+    };
+
+    if (run0 < run1) request_page(run0);
+    // the query of row r16 of block rq
+    wh_i8 q[kPieces][2];
+    uint32_t q_scale = 0;
+    float l = 0.0f;
+    const uint32_t row0 = 16 * rq + r16;
+    {
+        const uint32_t flat = tile.row0 + min(row0, tile.rows - 1), tok = flat / a.group;
+        const uint32_t head = kvh * a.group + (flat - tok * a.group);
+        const uint16_t* const p = (const uint16_t*)a.q + (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD + 16 * g;
+        wh_u4 raw[kPieces][2][2];
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[j][i >> 1][i & 1] = *(const wh_u4*)(p + 128 * j + 64 * (i >> 1) + 8 * (i & 1));
+        if (run0 < run1) request(run0);
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j)
+            q_scale |= kv_query_e4m3(raw[j], a.scale_log2 < 0.0f ? 0x80008000u : 0u, q[j][0], q[j][1]) << (8 * j);
+        row_pos[row0] = row0 < tile.rows ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
+    }
+    // scores are taken times c > 0 (0 would hide what is masked), the sign is the query's
+    const float c = fmaxf(fabsf(a.scale_log2), 1.0e-37f);
+    const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
+    const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
+
+    wh_f4 acc[kDims][kBlocks];  // [dim 16 (kDims wave + f) + 4g + i][row]
+#pragma unroll
+    for (int f = 0; f < kDims; ++f)
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) acc[f][b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+
+    if (run0 < run1) {  // the first run's reference, with room
+        uint32_t top = top_byte(run0);
+        for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+        if (lane == 0) wave_top[wave] = top;
+        kv_lds_barrier();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) top = max(top, wave_top[w]);
+        ref = min((int)top + 3, 254);
+        stage(run0);
+    }
+    kv_lds_barrier();
+
+    // outputs of run x: 16 dims a step, all rows and keys
+    wh_h8 w[2][kBlocks];
+    auto read_weights = [&](uint32_t run) {
+        const _Float16* const pb = (const _Float16*)(smem + W::kAtWeights) + (run & 1) * (kRows * W::kPl) + r16 * W::kPl + 16 * g;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) w[h][b] = *(const wh_h8*)(pb + 16 * b * W::kPl + 8 * h);
+    };
+    wh_h8 rel[2];
+    auto values_step = [&](uint32_t run, int f) {
+        const uint32_t block = kDims * wave + f, key = 16 * g + r16;  // of the transposed read
+        if (f % 2 == 0) {
+            const _Float16* const rp =
+                (const _Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel) + (block >> 1) * W::kRel + 16 * g;
+            rel[0] = *(const wh_h8*)rp;
+            rel[1] = *(const wh_h8*)(rp + 8);
+        }
+        const uint8_t* const src = smem + (kLatent ? 0 : W::kAtValues) + run % 3 * W::kCodes + key * W::kRow +
+                                   16 * ((block >> 1) ^ swizzle(key)) + 8 * (block & 1);
+        const wh_i2 codes = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) wh_i2*)src);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const wh_h8 x = kv_decode((uint32_t)codes[h], 1.0f) * rel[h];
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) acc[f][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[h][b], acc[f][b], 0, 0, 0);
+        }
+    };
+
+    auto pass = [&](uint32_t run, auto first) {
+        constexpr bool kFirst = decltype(first)::value;
+        const uint32_t at = run & 1;
+        request(run + 1);
+        if constexpr (!kFirst) read_weights(run - 1);
+        if constexpr (!kLatent)
+            if (t == 0) nan_keys[(run + 2) % 3] = 0;
+        // scores of 32 keys
+        wh_f4 s[2];
+        uint32_t scale[2];
+        const uint8_t* krow[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t key = 32 * kq + 16 * i + r16;
+            krow[i] = smem + run % W::kKeyBufs * W::kCodes + key * W::kRow;
+            scale[i] = *(const uint32_t*)(smem + W::kAtScales + at * 1024 + (g * 64 + key) * 4);
+            s[i] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        wh_static_for<kPieces>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            wh_i8 x[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const wh_u4 v = *(const wh_u4*)(krow[i] + 16 * ((4 * j + g) ^ swizzle(32 * kq + 16 * i + r16)));
+                x[i][0] = v[0], x[i][1] = v[1], x[i][2] = v[2], x[i][3] = v[3];
+                x[i][4] = x[i][5] = x[i][6] = x[i][7] = 0;
+            }
+#pragma unroll
+            for (int p = 1; p >= 0; --p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    s[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[i], q[j][p], s[i], 4, 0, j, scale[i], j,
+                                                                            q_scale - (p ? 0x04040404u : 0u));
+        });
+        // -inf where a row does not see this lane's keys
+        const uint32_t v0 = run * 64 + 32 * kq + 4 * g, last = run * 64 + 63;
+        const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == kRows &&
+                         (!a.window || (int64_t)wh_kv4_key(tile, max(run * 64, tile.n_first)) + a.window > pos_hi);
+        if (!all) {
+            const int32_t pos = row_pos[row0];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t v = v0 + 16 * (i >> 2) + (i & 3), key = wh_kv4_key(tile, v);
+                const bool see = (v < tile.n_keys) & wh_kv4_sees(pos, key, a.window, a.first);
+                s[i >> 2][i & 3] = see ? s[i >> 2][i & 3] : kMinusInf;
+            }
+        }
+        if constexpr (!kLatent) {
+            const uint64_t nan = nan_keys[run % 3];
+            if (__builtin_expect(nan != 0, 0)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if ((nan >> (32 * kq + 16 * (i >> 2) + 4 * g + (i & 3)) & 1) && s[i >> 2][i & 3] != kMinusInf)
+                        s[i >> 2][i & 3] = kv_bits(0x7fc00000u);
+            }
+        }
+        if constexpr (!kFirst) {
+#pragma unroll
+            for (int f = 0; f < kDims; ++f) values_step(run - 1, f);
+        }
+        const float m0 = row_m[row0];
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        float add;
+        auto weights = [&](float m) {
+            const float up = kUp - m;
+            float e[8];
+            wh_h8 x;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], c, up));
+                x[i] = (_Float16)e[i];
+            }
+            add = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+            union {
+                wh_h8 h;
+                wh_u4 u;
+            } y;
+            y.h = x;
+            _Float16* const pw = (_Float16*)(smem + W::kAtWeights) + at * (kRows * W::kPl) + row0 * W::kPl + 32 * kq + 4 * g;
+            *(wh_u2*)pw = (wh_u2){y.u[0], y.u[1]};
+            *(wh_u2*)(pw + 16) = (wh_u2){y.u[2], y.u[3]};
+        };
+        weights(m0);
+        uint32_t vtop = top_byte(run + 1);
+        const bool over = top * c > m0 + kSlack || (int)vtop > ref;
+        stage(run + 1);
+        if (__ballot(over) && lane == 0) raise[at] = run + 1;
+        kv_lds_barrier();
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(raise[at]) == run + 1, 0)) {  // the whole workgroup
+            for (int off = 32; off >= 1; off >>= 1) vtop = max(vtop, (uint32_t)__shfl_xor((int)vtop, off, 64));
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            if (g == 0) wave_m[kq][row0] = top * c;
+            if (lane == 0) wave_top[wave] = vtop;
+            kv_lds_barrier();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) vtop = max(vtop, wave_top[i]);
+            const int to = (int)vtop > ref ? min((int)vtop + 3, 254) : ref;
+            const float f_ref = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
+            auto raised = [&](uint32_t row) { return fmaxf(row_m[row], fmaxf(wave_m[0][row], wave_m[1][row])); };
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const float f = __builtin_amdgcn_exp2f(row_m[16 * b + r16] - raised(16 * b + r16)) * f_ref;
+#pragma unroll
+                for (int k = 0; k < kDims; ++k) acc[k][b] *= f;
+            }
+            const float m = raised(row0);
+            l *= __builtin_amdgcn_exp2f(row_m[row0] - m);
+            if (to != ref) {  // this run's value scales are in LDS against the old one
+                _Float16* const r = (_Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel);
+#pragma unroll
+                for (int i = 0; i < W::kMine; ++i) r[(my_chunk + i) * W::kRel + my_key] *= (_Float16)f_ref;
+                ref = to;
+                stage_rel(run + 1);
+            }
+            weights(m);
+            kv_lds_barrier();
+            if (kq == 0 && g == 0) row_m[row0] = m;
+            kv_lds_barrier();
+        }
+        l += add;
+    };
+
+    if (run0 < run1) pass(run0, std::true_type());
+    for (uint32_t run = run0 + 1; run < run1; ++run) pass(run, std::false_type());
+    if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
+    if (run0 < run1) {
+        read_weights(run1 - 1);
+#pragma unroll
+        for (int f = 0; f < kDims; ++f) values_step(run1 - 1, f);
+    }
+
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (g == 0) wave_l[kq][row0] = l;
+    kv_lds_barrier();
+    const float up = kv_bits((uint32_t)ref << 23);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const uint32_t r = 16 * b + r16;
+        if (r >= tile.rows) continue;
+        const uint32_t flat = tile.row0 + r, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
+        const float L = wave_l[0][r] + wave_l[1][r], M = row_m[r];
+        float denom = L;
+        if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
+        const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
+        float* const part = a.part + ((((uint64_t)place.slot * a.s.kv_heads + kvh) * a.splits + place.split) * kRows + r) * (HD + 2);
         const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
         for (int f = 0; f < kDims; ++f) {
@@ -1484,17 +1866,17 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
 // 16 rows a workgroup.
 template <int HD, bool kF32, int kRows, int kKeys>
 __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
-    const uint32_t t = threadIdx.x, kvh = blockIdx.y;
-    const wh_kv4_tile tile = kv_tile<kRows>(a, blockIdx.x);
+    const uint32_t t = threadIdx.x, slot = blockIdx.x / a.s.kv_heads, kvh = blockIdx.x % a.s.kv_heads;
+    const wh_kv4_tile tile = kv_tile<kRows>(a, slot);
     if (!tile.ok) return;
     const uint32_t per = wh_kv4_per_split(tile.n_keys, kKeys, a.splits, a.min_blocks);
     const uint32_t blocks = (tile.n_keys + kKeys - 1) / kKeys;
     if (per >= blocks) return;
     const uint32_t n = (blocks + per - 1) / per;
-    const uint32_t row = 16 * blockIdx.z + (t >> 4), d0 = (t & 15) * 4;
+    const uint32_t row = 16 * blockIdx.y + (t >> 4), d0 = (t & 15) * 4;
     if (row >= tile.rows) return;
     const uint32_t flat = tile.row0 + row, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
-    const float* const part = a.part + (((uint64_t)blockIdx.x * a.s.kv_heads + kvh) * a.splits * kRows + row) * (HD + 2);
+    const float* const part = a.part + (((uint64_t)slot * a.s.kv_heads + kvh) * a.splits * kRows + row) * (HD + 2);
     constexpr uint64_t kNext = kRows * (HD + 2);
     float M = kMinusBig, L = 0.0f;
     for (uint32_t k = 0; k < n; ++k) M = fmaxf(M, part[k * kNext + HD]);
@@ -1520,8 +1902,19 @@ __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
 
 template <int HD, bool kF32, bool kLatent>
 hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
-    const dim3 grid(a.n_tiles, a.s.kv_heads, a.splits);
-    if constexpr (!kF32 && HD >= 128) {
+    const dim3 grid(a.n_tiles * a.s.kv_heads * a.splits);
+    if constexpr (!kF32 && HD >= 256) {
+        if (a.wide) {
+            using W = wh_kv4_packed<HD, kLatent>;
+            static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_packed<HD, kLatent>,
+                                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
+            if (set != hipSuccess) return set;
+            k_kv4_attn_packed<HD, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
+            if (a.splits > 1)
+                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
+            return hipGetLastError();
+        }
+    } else if constexpr (!kF32 && HD == 128) {
         if (a.wide) {
             using W = wh_kv4_direct<HD, kLatent>;
             static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_direct<HD, kLatent>,
@@ -1529,7 +1922,7 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
             if (set != hipSuccess) return set;
             k_kv4_attn_direct<HD, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
             if (a.splits > 1)
-                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles, a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
+                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
             return hipGetLastError();
         }
     } else if (a.wide) {
@@ -1539,7 +1932,7 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
         if (set != hipSuccess) return set;
         k_kv4_attn_wide<HD, kF32, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
         if (a.splits > 1)
-            k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles, a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
+            k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
         return hipGetLastError();
     }
     constexpr size_t lds = 4 * (size_t)wh_kv4_dims<HD>::kStage;
@@ -1547,7 +1940,7 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (set != hipSuccess) return set;
     k_kv4_attn<HD, kF32, kLatent><<<grid, 256, lds, stream>>>(a);
-    if (a.splits > 1) k_kv4_join<HD, kF32, 16, 32><<<dim3(a.n_tiles, a.s.kv_heads), 256, 0, stream>>>(a);
+    if (a.splits > 1) k_kv4_join<HD, kF32, 16, 32><<<dim3(a.n_tiles * a.s.kv_heads), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 

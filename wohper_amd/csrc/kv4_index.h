@@ -35,15 +35,16 @@ struct wh_kv4_tile {
 };
 
 // First tile slot of request b, whose first token is `start`: at least as many
-// slots before request b + 1's as b has tiles, and increasing with b, so that a
-// search finds a slot's request without a sum over the others.
+// slots before request b + 1's as b has tiles, and not falling with b, so that a
+// search for the last one at or before a slot finds its request without a sum
+// over the others.  Where a token fills whole tiles there is none between.
 WH_KV_HD uint64_t wh_kv4_tile_base(uint32_t start, uint32_t group, uint32_t b, uint32_t tile_rows) {
-    return (uint64_t)start * group / tile_rows + b;
+    return (uint64_t)start * group / tile_rows + (group % tile_rows ? b : 0);
 }
 
 // Tile slots of a call.
 WH_KV_HD uint64_t wh_kv4_tile_slots(uint64_t n_tokens, uint64_t n_requests, uint32_t group, uint32_t tile_rows) {
-    return n_tokens * group / tile_rows + n_requests;
+    return n_tokens * group / tile_rows + (group % tile_rows ? n_requests : 0);
 }
 
 // Slot x of request b with tokens [s0, s1) (both at most n_tokens) and len
