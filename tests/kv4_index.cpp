@@ -89,10 +89,26 @@ int main(int argc, char** argv) {
             }
             CHECK(got.size() == t.n_keys);  // each once
             for (uint32_t j : want) CHECK(got.count(j));
-            for (uint32_t splits : {1u, 2u, 3u, 64u}) {
-                const uint32_t per = wh_kv4_per_split(t.n_keys, 32, splits, 1 + upto(4));
-                CHECK((uint64_t)per * splits * 32 >= t.n_keys && per >= 1);
+            CHECK(t.n_keys <= 32 * (uint64_t)wh_kv4_blocks(t.n_q, lens[b], cap, window, first, 32));
+        }
+        uint64_t tiles = 0, blocks = 0;
+        for (uint32_t b = 0; b < requests; ++b) {
+            const uint32_t n_q = start(b + 1) > start(b) ? start(b + 1) - start(b) : 0, k = wh_kv4_tiles(n_q, group, tile_rows);
+            tiles += k;
+            blocks += (uint64_t)k * wh_kv4_blocks(n_q, lens[b], cap, window, first, 32);
+        }
+        if (!garbage) CHECK(tiles <= slots);
+        for (uint32_t units : {1u, 7u, 64u, 300u}) {
+            const uint32_t chunk = wh_kv4_chunk(blocks, tiles, units, 1 + upto(6));
+            CHECK(chunk >= 1);
+            uint64_t used = 0;
+            for (uint32_t b = 0; b < requests; ++b) {
+                const uint32_t n_q = start(b + 1) > start(b) ? start(b + 1) - start(b) : 0;
+                const uint32_t k = wh_kv4_blocks(n_q, lens[b], cap, window, first, 32), splits = wh_kv4_splits(k, chunk);
+                CHECK((uint64_t)splits * chunk >= k);
+                used += (uint64_t)wh_kv4_tiles(n_q, group, tile_rows) * splits;
             }
+            CHECK(used <= std::max<uint64_t>(units, tiles));
         }
         if (!garbage) {
             std::vector<int> all((size_t)n_tokens * group);

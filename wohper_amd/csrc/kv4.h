@@ -6,6 +6,7 @@
 
 #include "kv4_index.h"
 
+#define WH_KV_SPLIT_REQUESTS 256u  // requests of a call whose keys are cut up: each wave adds them up
 #define WH_KV_MAX_REQUESTS 4096u  // requests of one plan: three prefix sums of them lie in LDS
 
 // One step's plan (wh_kv_plan_async): device arrays as in the header.
@@ -49,16 +50,18 @@ struct wh_kv4_attn_args {
     const uint32_t *starts, *lens, *tables;
     uint64_t table_stride;
     const float* sink;
-    float* part;        // [tile][kv head][split][rows][head_dim + 2]: normalised outputs, maxima, sums
+    float* part;        // [unit][kv head][rows][head_dim + 2]: normalised outputs, maxima, sums
     uint32_t n_tokens, n_requests, group, window, first;
-    uint32_t splits, min_blocks, n_tiles;
+    uint32_t n_tiles;     // slots or tiles, at most
+    uint32_t units;       // workgroups of a key head, at most; > n_tiles: their keys are cut up
+    uint32_t min_blocks;  // that a workgroup takes
     bool wide;          // tiles of 64 (f32: 32) rows instead of 16
     float scale_log2;   // scale * log2(e)
     uint32_t* status;
 };
 // How a call is cut up: by sizes the host knows.
 struct wh_kv4_attn_plan {
-    uint32_t splits, min_blocks, n_tiles;
+    uint32_t n_tiles, units, min_blocks;
     bool wide;
     size_t part_bytes;  // scratch for partial results, 0 for one split
 };

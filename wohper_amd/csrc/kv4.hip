@@ -317,20 +317,94 @@ __device__ __forceinline__ wh_kv4_tile kv_tile(const wh_kv4_attn_args& a, uint32
     return r;
 }
 
-// A workgroup's tile slot, key head and split: splits next to each other, then
-// heads, so that the slots that hold no rows are spread over the eight XCDs as
-// evenly as the others, and the tiles of one key head (of eight) meet in one L2.
+// What a workgroup does: a tile of one key head, and which of its blocks of
+// keys.  Key heads lie next to each other in the grid, so that of eight each
+// has an XCD's L2 to itself.
 struct wh_kv4_place {
-    uint32_t slot, head, split;
+    wh_kv4_tile tile;
+    uint32_t head, unit;    // unit: where a partial result goes
+    uint32_t chunk, split;  // blocks [split * chunk, ...)
 };
-__device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a) {
-    const uint32_t x = blockIdx.x / a.splits;
-    return {x / a.s.kv_heads, x % a.s.kv_heads, blockIdx.x % a.splits};
-}
 
-// Blocks of 32 keys of one split.
-__device__ __forceinline__ uint32_t kv_split_blocks(const wh_kv4_attn_args& a, uint32_t n_keys) {
-    return wh_kv4_per_split(n_keys, 32, a.splits, a.min_blocks);
+// Where there are more workgroups than tiles, the requests' lengths decide how
+// many share one: every wave adds up all requests (at most WH_KV_SPLIT_REQUESTS)
+// and finds its own by the running sum.  by_tile: x counts tiles, and the place
+// is their first unit.
+template <int kRows, int kKeys>
+__device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a, bool by_tile) {
+    wh_kv4_place r;
+    const uint32_t x = blockIdx.x / a.s.kv_heads;
+    r.head = blockIdx.x % a.s.kv_heads;
+    r.unit = x;
+    r.split = 0;
+    r.chunk = 0x7fffffffu;
+    if (a.units <= a.n_tiles) {
+        r.tile = kv_tile<kRows>(a, x);
+        return r;
+    }
+    const uint32_t lane = threadIdx.x & 63, cap = (uint32_t)min(a.table_stride << a.s.shift, (uint64_t)0x7fffffff);
+    auto start = [&](uint32_t b) { return min(a.starts[b], a.n_tokens); };
+    auto request = [&](uint32_t b, uint32_t& tiles, uint32_t& blocks) {
+        tiles = blocks = 0;
+        if (b < a.n_requests) {
+            const uint32_t s0 = start(b), s1 = start(b + 1), n_q = s1 > s0 ? s1 - s0 : 0;
+            tiles = wh_kv4_tiles(n_q, a.group, kRows);
+            blocks = wh_kv4_blocks(n_q, a.lens[b], cap, a.window, a.first, kKeys);
+        }
+    };
+    uint64_t sum_tiles = 0, sum_blocks = 0;
+    uint32_t tiles, blocks;
+    for (uint32_t b = 0; b < a.n_requests; b += 64) {
+        request(b + lane, tiles, blocks);
+        sum_tiles += tiles;
+        sum_blocks += (uint64_t)tiles * blocks;
+    }
+    for (int off = 32; off >= 1; off >>= 1) {
+        sum_tiles += ((uint64_t)__shfl_xor((uint32_t)(sum_tiles >> 32), off, 64) << 32) | (uint32_t)__shfl_xor((uint32_t)sum_tiles, off, 64);
+        sum_blocks += ((uint64_t)__shfl_xor((uint32_t)(sum_blocks >> 32), off, 64) << 32) | (uint32_t)__shfl_xor((uint32_t)sum_blocks, off, 64);
+    }
+    r.chunk = wh_kv4_chunk(sum_blocks, sum_tiles, a.units, a.min_blocks);
+    uint32_t tile0 = 0, unit0 = 0;  // of the requests before these 64
+    r.tile = wh_kv4_tile_of(0, 0, 0, 0, 0, 0, a.group, 0, 0, kRows);  // none
+    for (uint32_t b = 0; b < a.n_requests; b += 64) {
+        if (a.n_requests > 64) request(b + lane, tiles, blocks);
+        const uint32_t splits = wh_kv4_splits(blocks, r.chunk);
+        uint32_t t = tiles, u = tiles * splits;
+        for (uint32_t d = 1; d < 64; d <<= 1) {
+            const uint32_t pt = __shfl_up(t, d, 64), pu = __shfl_up(u, d, 64);
+            if (lane >= d) t += pt, u += pu;
+        }
+        const uint64_t hit = __ballot((by_tile ? tile0 + t : unit0 + u) > x);
+        if (hit) {
+            const int src = __ffsll((unsigned long long)hit) - 1;
+            const uint32_t n = __shfl(splits, src, 64), before = __shfl(by_tile ? t - tiles : u - tiles * splits, src, 64);
+            const uint32_t at = x - (by_tile ? tile0 : unit0) - before, local = by_tile ? at : at / n;
+            if (by_tile) r.unit = unit0 + __shfl(u - tiles * splits, src, 64) + at * n;
+            r.split = by_tile ? 0 : at - local * n;
+            const uint32_t q = b + src, s0 = start(q);
+            r.tile = wh_kv4_tile_of(wh_kv4_tile_base(s0, a.group, q, kRows) + local, q, s0, start(q + 1), a.lens[q], cap, a.group,
+                                    a.window, a.first, kRows);
+            if (a.lens[q] > cap && threadIdx.x == 0) atomicOr(a.status, WH_ST_NOT_RESIDENT);
+            break;
+        }
+        tile0 += __shfl(t, 63, 64);
+        unit0 += __shfl(u, 63, 64);
+    }
+    // wave-uniform: in scalar registers from here
+    r.tile.request = __builtin_amdgcn_readfirstlane(r.tile.request);
+    r.tile.row0 = __builtin_amdgcn_readfirstlane(r.tile.row0);
+    r.tile.rows = __builtin_amdgcn_readfirstlane(r.tile.rows);
+    r.tile.n_q = __builtin_amdgcn_readfirstlane(r.tile.n_q);
+    r.tile.token0 = __builtin_amdgcn_readfirstlane(r.tile.token0);
+    r.tile.len = __builtin_amdgcn_readfirstlane(r.tile.len);
+    r.tile.n_first = __builtin_amdgcn_readfirstlane(r.tile.n_first);
+    r.tile.lo = __builtin_amdgcn_readfirstlane(r.tile.lo);
+    r.tile.n_keys = __builtin_amdgcn_readfirstlane(r.tile.n_keys);
+    r.tile.ok = __builtin_amdgcn_readfirstlane((int)r.tile.ok) != 0;
+    r.unit = __builtin_amdgcn_readfirstlane(r.unit);
+    r.split = __builtin_amdgcn_readfirstlane(r.split);
+    r.chunk = __builtin_amdgcn_readfirstlane(r.chunk);
+    return r;
 }
 
 // max over the bytes of w
@@ -539,18 +613,18 @@ template <int HD, bool kF32, bool kLatent>
 __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
     using D = wh_kv4_dims<HD>;
     constexpr int kParts = kF32 ? 2 : 1;
-    const wh_kv4_place place = kv_place(a);
+    const wh_kv4_place place = kv_place<16, 32>(a, false);
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(16) float key_scale[4][2][32];  // [wave][keys', values'][key]
     __shared__ float row_m[4][16], row_l[4][16];
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63, r16 = lane & 15, g = lane >> 4;
     const uint32_t kvh = place.head;
-    const wh_kv4_tile tile = kv_tile<16>(a, place.slot);
+    const wh_kv4_tile tile = place.tile;
     if (!tile.ok) return;
-    const uint32_t per = kv_split_blocks(a, tile.n_keys), blocks = (tile.n_keys + 31) / 32;
-    const uint32_t blk0 = place.split * per, blk1 = min(blocks, blk0 + per);
+    const uint32_t blocks = (tile.n_keys + 31) / 32;
+    const uint32_t blk0 = place.split ? place.split * place.chunk : 0, blk1 = min(blocks, blk0 + place.chunk);
     if (place.split && blk0 >= blocks) return;
-    const bool whole = per >= blocks;  // the only split: the result is final
+    const bool whole = place.chunk >= blocks;  // the only split: the result is final
 
     // this lane's row
     const uint32_t rr = min(r16, tile.rows - 1), flat = tile.row0 + rr, tok = flat / a.group;
@@ -747,7 +821,7 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
     float denom = L;
     if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[rhead] * 1.44269504088896340736f - M + kUp);
     const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-    float* const part = a.part + ((((uint64_t)place.slot * a.s.kv_heads + kvh) * a.splits + place.split) * 16 + row) * (HD + 2);
+    float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * 16 + row) * (HD + 2);
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i) {
         const uint32_t d = 64 * i + d0;
@@ -797,7 +871,7 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
     using D = wh_kv4_dims<HD>;
     using W = wh_kv4_wide<HD, kF32>;
     constexpr int kParts = W::kParts, kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kMine = W::kMine;
-    const wh_kv4_place place = kv_place(a);
+    const wh_kv4_place place = kv_place<W::kRows, 64>(a, false);
     extern __shared__ __align__(16) uint8_t smem[];
     _Float16* const vbuf = (_Float16*)smem;                      // [2][key][kLd]
     _Float16* const pbuf = vbuf + 2 * W::kRun;                   // [2][part][row][kPl]
@@ -808,12 +882,12 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
     __shared__ uint32_t wave_top[4], raise[2];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
     const uint32_t kvh = place.head, kq = wave & 3, half = wave >> 2;
-    const wh_kv4_tile tile = kv_tile<kRows>(a, place.slot);
+    const wh_kv4_tile tile = place.tile;
     if (!tile.ok) return;
-    const uint32_t per = wh_kv4_per_split(tile.n_keys, 64, a.splits, a.min_blocks), runs = (tile.n_keys + 63) / 64;
-    const uint32_t run0 = place.split * per, run1 = min(runs, run0 + per);
+    const uint32_t runs = (tile.n_keys + 63) / 64;
+    const uint32_t run0 = place.split ? place.split * place.chunk : 0, run1 = min(runs, run0 + place.chunk);
     if (place.split && run0 >= runs) return;
-    const bool whole = per >= runs;
+    const bool whole = place.chunk >= runs;
     if (t < 2) raise[t] = 0;
     if (t < kRows) row_m[t] = kMinusBig;
 
@@ -1057,7 +1131,7 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
         float denom = L;
         if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
         const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-        float* const part = a.part + ((((uint64_t)place.slot * a.s.kv_heads + kvh) * a.splits + place.split) * kRows + r) * (HD + 2);
+        float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * kRows + r) * (HD + 2);
         const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
         for (int f = 0; f < kDims; ++f) {
@@ -1155,7 +1229,7 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
     using W = wh_kv4_direct<HD, kLatent>;
     constexpr int kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kMine = W::kMine, kKeys = W::kKeys,
                   kPieces = W::kPieces, kTasks = W::kTasks;
-    const wh_kv4_place place = kv_place(a);
+    const wh_kv4_place place = kv_place<W::kRows, 64>(a, false);
     extern __shared__ __align__(16) uint8_t smem[];
     _Float16* const vbuf = (_Float16*)smem;     // [2][key][kLd]
     _Float16* const pbuf = vbuf + 2 * W::kRun;  // [2][row][kPl]
@@ -1165,12 +1239,12 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
     __shared__ uint64_t nan_keys[2];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
     const uint32_t kvh = place.head, kq = wave % W::kKeyGroups, rq = wave / W::kKeyGroups;
-    const wh_kv4_tile tile = kv_tile<kRows>(a, place.slot);
+    const wh_kv4_tile tile = place.tile;
     if (!tile.ok) return;
-    const uint32_t per = wh_kv4_per_split(tile.n_keys, 64, a.splits, a.min_blocks), runs = (tile.n_keys + 63) / 64;
-    const uint32_t run0 = place.split * per, run1 = min(runs, run0 + per);
+    const uint32_t runs = (tile.n_keys + 63) / 64;
+    const uint32_t run0 = place.split ? place.split * place.chunk : 0, run1 = min(runs, run0 + place.chunk);
     if (place.split && run0 >= runs) return;
-    const bool whole = per >= runs;
+    const bool whole = place.chunk >= runs;
     if (t < 2) raise[t] = 0;
     if (t < 2) nan_keys[t] = 0;
     if (t < kRows) row_m[t] = kMinusBig;
@@ -1478,7 +1552,7 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
         float denom = L;
         if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
         const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-        float* const part = a.part + ((((uint64_t)place.slot * a.s.kv_heads + kvh) * a.splits + place.split) * kRows + r) * (HD + 2);
+        float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * kRows + r) * (HD + 2);
         const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
         for (int f = 0; f < kDims; ++f) {
@@ -1527,7 +1601,7 @@ template <int HD, bool kLatent>
 __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) {
     using W = wh_kv4_packed<HD, kLatent>;
     constexpr int kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kPieces = W::kPieces;
-    const wh_kv4_place place = kv_place(a);
+    const wh_kv4_place place = kv_place<W::kRows, 64>(a, false);
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float wave_m[2][kRows], wave_l[2][kRows], row_m[kRows];
     __shared__ int32_t row_pos[kRows];
@@ -1535,12 +1609,12 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
     __shared__ uint64_t nan_keys[3];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
     const uint32_t kvh = place.head, kq = wave & 1, rq = wave >> 1;
-    const wh_kv4_tile tile = kv_tile<kRows>(a, place.slot);
+    const wh_kv4_tile tile = place.tile;
     if (!tile.ok) return;
-    const uint32_t per = wh_kv4_per_split(tile.n_keys, 64, a.splits, a.min_blocks), runs = (tile.n_keys + 63) / 64;
-    const uint32_t run0 = place.split * per, run1 = min(runs, run0 + per);
+    const uint32_t runs = (tile.n_keys + 63) / 64;
+    const uint32_t run0 = place.split ? place.split * place.chunk : 0, run1 = min(runs, run0 + place.chunk);
     if (place.split && run0 >= runs) return;
-    const bool whole = per >= runs;
+    const bool whole = place.chunk >= runs;
     if (t < 2) raise[t] = 0;
     if (t < 3) nan_keys[t] = 0;
     if (t < kRows) row_m[t] = kMinusBig;
@@ -1841,7 +1915,7 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
         float denom = L;
         if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
         const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-        float* const part = a.part + ((((uint64_t)place.slot * a.s.kv_heads + kvh) * a.splits + place.split) * kRows + r) * (HD + 2);
+        float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * kRows + r) * (HD + 2);
         const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
         for (int f = 0; f < kDims; ++f) {
@@ -1861,48 +1935,56 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
     }
 }
 
-// Joins the splits of a tile of kRows rows, keys counted in blocks of kKeys:
-// outputs weighted by their sums of weights, and the sink.  16 threads a row,
-// 16 rows a workgroup.
+// Joins the workgroups of a tile: outputs weighted by their sums of weights, and
+// the sink.  A wave a row, four rows a workgroup.
 template <int HD, bool kF32, int kRows, int kKeys>
 __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
-    const uint32_t t = threadIdx.x, slot = blockIdx.x / a.s.kv_heads, kvh = blockIdx.x % a.s.kv_heads;
-    const wh_kv4_tile tile = kv_tile<kRows>(a, slot);
-    if (!tile.ok) return;
-    const uint32_t per = wh_kv4_per_split(tile.n_keys, kKeys, a.splits, a.min_blocks);
-    const uint32_t blocks = (tile.n_keys + kKeys - 1) / kKeys;
-    if (per >= blocks) return;
-    const uint32_t n = (blocks + per - 1) / per;
-    const uint32_t row = 16 * blockIdx.y + (t >> 4), d0 = (t & 15) * 4;
-    if (row >= tile.rows) return;
+    constexpr int kPer = HD >= 256 ? 4 : HD / 64;  // values of a lane next to each other
+    const uint32_t lane = threadIdx.x & 63, row = 4 * blockIdx.y + (threadIdx.x >> 6);
+    const wh_kv4_place place = kv_place<kRows, kKeys>(a, true);
+    const wh_kv4_tile& tile = place.tile;
+    const uint32_t blocks = (tile.n_keys + kKeys - 1) / kKeys, kvh = place.head;
+    if (!tile.ok || row >= tile.rows || blocks <= place.chunk) return;
+    const uint32_t n = (blocks + place.chunk - 1) / place.chunk;
     const uint32_t flat = tile.row0 + row, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
-    const float* const part = a.part + (((uint64_t)slot * a.s.kv_heads + kvh) * a.splits * kRows + row) * (HD + 2);
-    constexpr uint64_t kNext = kRows * (HD + 2);
+    const uint64_t next = (uint64_t)a.s.kv_heads * kRows * (HD + 2);
+    const float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * kRows + row) * (HD + 2);
     float M = kMinusBig, L = 0.0f;
-    for (uint32_t k = 0; k < n; ++k) M = fmaxf(M, part[k * kNext + HD]);
-    wh_f4 x[HD / 64];
+    for (uint32_t k = lane; k < n; k += 64) M = fmaxf(M, part[k * next + HD]);
+    M = wh_wave_max(M);
+    float x[HD / 64];
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i) x[i] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < HD / 64; ++i) x[i] = 0.0f;
+#pragma unroll 4
     for (uint32_t k = 0; k < n; ++k) {
-        const float* const p = part + k * kNext;
+        const float* const p = part + k * next;
         const float w = p[HD + 1] * __builtin_amdgcn_exp2f(p[HD] - M);
         L += w;
 #pragma unroll
-        for (int i = 0; i < HD / 64; ++i) {
-            const wh_f2 u = *(const wh_f2*)(p + 64 * i + d0), v = *(const wh_f2*)(p + 64 * i + d0 + 2);
-            x[i] += (wh_f4){u[0], u[1], v[0], v[1]} * w;
-        }
+        for (int i = 0; i < HD / 64; i += 2)
+            if constexpr (kPer >= 2) {
+                const wh_f2 u = *(const wh_f2*)(p + 64 * kPer * (i / kPer) + kPer * lane + i % kPer);
+                x[i] += u[0] * w;
+                x[i + 1] += u[1] * w;
+            } else {
+                x[i] += p[lane] * w;
+            }
     }
     if (a.sink) L += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i) kv_store<kF32>(a.out, at + 64 * i + d0, x[i] * inv);
+    for (int i = 0; i < HD / 64; ++i) {
+        const uint64_t d = at + 64 * kPer * (i / kPer) + kPer * lane + i % kPer;
+        if constexpr (kF32) ((float*)a.out)[d] = x[i] * inv;
+        else ((__bf16*)a.out)[d] = (__bf16)(x[i] * inv);
+    }
 }
 
 template <int HD, bool kF32, bool kLatent>
 hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
-    const dim3 grid(a.n_tiles * a.s.kv_heads * a.splits);
+    const bool split = a.units > a.n_tiles;
+    const dim3 grid((split ? a.units : a.n_tiles) * a.s.kv_heads);
     if constexpr (!kF32 && HD >= 256) {
         if (a.wide) {
             using W = wh_kv4_packed<HD, kLatent>;
@@ -1910,8 +1992,8 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
                                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
             if (set != hipSuccess) return set;
             k_kv4_attn_packed<HD, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
-            if (a.splits > 1)
-                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
+            if (split)
+                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
             return hipGetLastError();
         }
     } else if constexpr (!kF32 && HD == 128) {
@@ -1921,8 +2003,8 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
                                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
             if (set != hipSuccess) return set;
             k_kv4_attn_direct<HD, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
-            if (a.splits > 1)
-                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
+            if (split)
+                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
             return hipGetLastError();
         }
     } else if (a.wide) {
@@ -1931,8 +2013,8 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
         if (set != hipSuccess) return set;
         k_kv4_attn_wide<HD, kF32, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
-        if (a.splits > 1)
-            k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 16), 256, 0, stream>>>(a);
+        if (split)
+            k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
         return hipGetLastError();
     }
     constexpr size_t lds = 4 * (size_t)wh_kv4_dims<HD>::kStage;
@@ -1940,7 +2022,7 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (set != hipSuccess) return set;
     k_kv4_attn<HD, kF32, kLatent><<<grid, 256, lds, stream>>>(a);
-    if (a.splits > 1) k_kv4_join<HD, kF32, 16, 32><<<dim3(a.n_tiles * a.s.kv_heads), 256, 0, stream>>>(a);
+    if (split) k_kv4_join<HD, kF32, 16, 32><<<dim3(a.n_tiles * a.s.kv_heads, 4), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -1985,15 +2067,16 @@ wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, bool 
     p.wide = rows >= (uint64_t)a.n_requests * (wide_rows - 16);
     const uint32_t tile_rows = p.wide ? wide_rows : 16, block = p.wide ? 64 : 32;
     p.n_tiles = (uint32_t)wh_kv4_tile_slots(a.n_tokens, a.n_requests, a.group, tile_rows);
-    const uint64_t wgs = (uint64_t)p.n_tiles * a.s.kv_heads;
-    const uint64_t busy = std::max<uint64_t>(rows / tile_rows, a.n_requests) * a.s.kv_heads;  // tiles that hold rows, about
+    // more workgroups than tiles: the keys are cut up by the lengths on the device
     uint64_t keys = max_len;
     if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.first + a.n_tokens);
-    const uint64_t target = a.s.head_dim >= 256 ? 256 : 512;
-    const uint64_t want = target / busy, most = (keys + 127) / 128;
-    p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(want, std::min<uint64_t>(most, 64)));
+    const uint64_t resident = p.wide && a.s.head_dim >= 256 ? 256 : a.s.head_dim >= 512 ? 256 : a.s.head_dim == 256 ? 512 : p.wide ? 512 : 1024;
     p.min_blocks = 128 / block;
-    if (p.splits > 1) p.part_bytes = wgs * p.splits * tile_rows * (a.s.head_dim + 2) * sizeof(float);
+    p.units = (uint32_t)(resident / a.s.kv_heads);
+    const uint64_t busy = std::max<uint64_t>(rows / tile_rows, 1);  // tiles that hold rows, at least
+    if (p.units < 2 * busy || a.n_requests > WH_KV_SPLIT_REQUESTS || keys <= 128) p.units = 0;
+    p.units = std::max(p.units, p.n_tiles);
+    if (p.units > p.n_tiles) p.part_bytes = (size_t)p.units * a.s.kv_heads * tile_rows * (a.s.head_dim + 2) * sizeof(float);
     return p;
 }
 

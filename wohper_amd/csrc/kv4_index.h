@@ -82,8 +82,27 @@ WH_KV_HD bool wh_kv4_sees(int32_t pos, uint32_t key, uint32_t window, uint32_t f
     return (int64_t)key <= pos && (!window || key < first || (int64_t)key + window > pos);
 }
 
-// Blocks of `block` keys that each of `splits` workgroups takes of n_keys.
-WH_KV_HD uint32_t wh_kv4_per_split(uint32_t n_keys, uint32_t block, uint32_t splits, uint32_t min_blocks) {
-    const uint32_t blocks = n_keys / block + (n_keys % block != 0), even = blocks / splits + (blocks % splits != 0);
-    return even > min_blocks ? even : min_blocks;
+// How a call whose tiles are fewer than its workgroups cuts up their keys.  Of
+// request b, n_q tokens on len rows: tiles, and at most how many blocks of
+// `block` keys each sees.
+WH_KV_HD uint32_t wh_kv4_tiles(uint32_t n_q, uint32_t group, uint32_t tile_rows) {
+    return (uint32_t)(((uint64_t)n_q * group + tile_rows - 1) / tile_rows);
+}
+WH_KV_HD uint32_t wh_kv4_blocks(uint32_t n_q, uint32_t len, uint32_t cap, uint32_t window, uint32_t first, uint32_t block) {
+    uint64_t keys = len < cap ? len : cap;
+    if (window && keys > (uint64_t)window + first + n_q) keys = (uint64_t)window + first + n_q;
+    return (uint32_t)((keys + block - 1) / block);
+}
+// Blocks a workgroup takes, for `tiles` tiles of `blocks` blocks in all and
+// `units` workgroups: then the workgroups that all tiles need, each its blocks
+// / chunk rounded up, are at most `units`.  Every key of a tile in one workgroup
+// where there are less than two for each.
+WH_KV_HD uint32_t wh_kv4_chunk(uint64_t blocks, uint64_t tiles, uint64_t units, uint32_t min_blocks) {
+    if (units < 2 * tiles) return 0x7fffffffu;
+    const uint64_t free = units - tiles, even = (blocks + free - 1) / free;
+    return even < min_blocks ? min_blocks : even > 0x7fffffffu ? 0x7fffffffu : (uint32_t)even;
+}
+// Workgroups of a tile of so many blocks.
+WH_KV_HD uint32_t wh_kv4_splits(uint32_t blocks, uint32_t chunk) {
+    return blocks <= chunk ? 1 : (blocks + chunk - 1) / chunk;
 }

@@ -4807,7 +4807,7 @@ int wh_kv4_attention_async(wh_ctx* c, const wh_kv4_cache* cache, const wh_kv4_at
     a.scale_log2 = d->scale * 1.44269504088896340736f;
     a.status = c->status;
     const wh_kv4_attn_plan p = wh_kv4_attn_plan_of(a, d->is_bf16 != 0, !has_v, d->max_len);
-    a.splits = p.splits;
+    a.units = p.units;
     a.min_blocks = p.min_blocks;
     a.n_tiles = p.n_tiles;
     a.wide = p.wide;
