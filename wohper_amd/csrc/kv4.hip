@@ -20,6 +20,7 @@ typedef _Float16 wh_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 wh_h8 __attribute__((ext_vector_type(8)));
 typedef short wh_s4 __attribute__((ext_vector_type(4)));
 typedef __fp16 wh_hh4 __attribute__((ext_vector_type(4)));
+typedef int wh_i8 __attribute__((ext_vector_type(8)));
 typedef int wh_i2 __attribute__((ext_vector_type(2)));
 typedef uint32_t wh_u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t wh_u4 __attribute__((ext_vector_type(4)));
@@ -446,7 +447,6 @@ struct wh_kv4_dims {
     static constexpr int kScaleWords = HD >= 128 ? HD / 128 : 1;
     static constexpr int kLd = HD + 16;                   // f16 between rows of a staged block: 16 rows of a
                                                           // transposed read start 32 bytes apart modulo 256
-    static constexpr int kStage = 32 * kLd * 2;           // bytes of a wave's block
 };
 
 // Raw rows of a lane: key lane % 16 of kN blocks of 16.
@@ -501,13 +501,13 @@ __device__ __forceinline__ uint32_t kv_top_byte(const wh_kv4_raw<HD, kN>& r, int
 
 // Scale bytes of a lane's pieces, piece j in byte j.
 template <int HD, int kN>
-__device__ __forceinline__ uint32_t kv_piece_scales(const wh_kv4_raw<HD, kN>& r, uint32_t g) {
+__device__ __forceinline__ uint32_t kv_piece_scales(const wh_kv4_raw<HD, kN>& r, int half, uint32_t g) {
     const uint32_t pick = g | (4 + g) << 8;
-    if constexpr (HD == 128) return r.s[0][0] >> (8 * g);
-    if constexpr (HD == 256) return __builtin_amdgcn_perm(r.s[0][1], r.s[0][0], pick);
+    if constexpr (HD == 128) return (r.s[half][0] >> (8 * g)) & 0xff;
+    if constexpr (HD == 256) return __builtin_amdgcn_perm(r.s[half][1], r.s[half][0], pick) & 0xffff;
     if constexpr (HD == 512)
-        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(r.s[0][3], r.s[0][2], pick),
-                                     __builtin_amdgcn_perm(r.s[0][1], r.s[0][0], pick), 0x05040100u);
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(r.s[half][3], r.s[half][2], pick),
+                                     __builtin_amdgcn_perm(r.s[half][1], r.s[half][0], pick), 0x05040100u);
     return 0;
 }
 
@@ -603,154 +603,341 @@ __device__ __forceinline__ void kv_store(void* out, uint64_t at, const wh_f4& x)
     }
 }
 
-// Four waves share a tile of 16 rows; wave w takes the blocks of 32 keys w,
-// w + 4, ... of the workgroup's run with a softmax of its own, and the four
-// are joined at the end.  Scores are formed as [key][row], so a lane's eight
-// weights of a row are already the operand of the product with the values,
-// whose rows pass through the wave's own LDS for the transposed read: no
-// barrier between waves before the end.
+// A lane's 32 of 128 bf16 values of a query as two E4M3 parts: dims 16g .. of
+// the first half and of the second, where the instruction wants 8-bit values (it
+// takes 4-bit ones and all scales as 32g ..).  Returns the first part's scale
+// byte for dims 32g .. (the second's is 4 less), 255 where one is not finite.
+__device__ __forceinline__ uint32_t kv_query_e4m3(const wh_u4 (&raw)[2][2], uint32_t flip, wh_i8& hi, wh_i8& lo) {
+    int e[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t w = raw[h][i][k];
+                top = max(top, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
+            }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));  // the other 16 of the 32
+        e[h] = max((int)(top >> 23), 20);
+        const float up = kv_bits((uint32_t)(127 + 127 + 7 - min(e[h], 254)) << 23);  // the largest to [2^7, 2^8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int a = 0, b = 0;
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t w = raw[h][i >> 1][2 * (i & 1) + (k >> 1)] ^ flip;
+                x[k] = kv_bits(k & 1 ? w & 0xffff0000u : w << 16) * up;
+            }
+            a = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], a, false);
+            a = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], a, true);
+            const wh_f2 u = __builtin_amdgcn_cvt_pk_f32_fp8(a, false), v = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
+            b = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - u.x) * 16.0f, (x[1] - u.y) * 16.0f, b, false);
+            b = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - v.x) * 16.0f, (x[3] - v.y) * 16.0f, b, true);
+            hi[4 * h + i] = a;
+            lo[4 * h + i] = b;
+        }
+    }
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, from = (lane & 15) + 32 * (g & 1);
+    const int e0 = __shfl(e[0], (int)from, 64), e1 = __shfl(e[1], (int)from, 64), w = g < 2 ? e0 : e1;
+    return w == 255 ? 255u : (uint32_t)(w - 7);
+}
+
+// Max and sum over the four lanes of a row (lane % 16), in all of them.
+__device__ __forceinline__ float kv_max_groups(float v) {
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    u2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float kv_sum_groups(float v) {
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    u2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// Four waves share a tile of 16 rows; wave w takes the blocks of 64 keys w, w +
+// 4, ... of the workgroup's run with a softmax of its own, and the four are
+// joined at the end: no barrier between waves before that.  Scores are formed as
+// [key][row]: lane (row, g) holds the keys 16 b + 4 g + i of four blocks b.  The
+// value rows' codes go through the wave's own LDS as they lie and come back
+// transposed, sixteen keys of one dim a lane (the 4-bit transposing read), whose
+// source rows are chosen to be just these keys: a lane's weights are the operand
+// of the product with the values as they are.
+template <int HD, bool kF32>
+struct wh_kv4_narrow {
+    static constexpr bool kDirect = !kF32 && HD >= 128;      // scores on codes as they lie
+    static constexpr int kParts = kF32 ? 2 : 1;
+    static constexpr int kPieces = HD / 128 ? HD / 128 : 1;
+    static constexpr int kHold = HD >= 256 ? 2 : 4;          // blocks of 16 keys whose rows are held at once
+    static constexpr int kRow = HD / 2;                      // bytes of a row's codes
+    static constexpr int kGroups = HD / 32, kRel = 72;       // f16 between groups of value scales
+    static constexpr int kAtRel = 64 * kRow;                 // byte offsets in a wave's LDS
+    static constexpr int kAtKeys = kAtRel + kGroups * kRel * 2;
+    static constexpr int kWave = kAtKeys + (kDirect ? 0 : 2 * 64 * 4);
+    static constexpr size_t kLds = 4 * (size_t)kWave > 2 * 64 * (size_t)HD ? 4 * (size_t)kWave : 2 * 64 * (size_t)HD;
+};
+
 template <int HD, bool kF32, bool kLatent>
 __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
     using D = wh_kv4_dims<HD>;
-    constexpr int kParts = kF32 ? 2 : 1;
-    const wh_kv4_place place = kv_place<16, 32>(a, false);
+    using W = wh_kv4_narrow<HD, kF32>;
+    constexpr int kParts = W::kParts, kHold = W::kHold, kPieces = W::kPieces;
+    constexpr bool kDirect = W::kDirect;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ __align__(16) float key_scale[4][2][32];  // [wave][keys', values'][key]
-    __shared__ float row_m[4][16], row_l[4][16];
-    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63, r16 = lane & 15, g = lane >> 4;
+    __shared__ float wave_m[4][16], wave_l[4][16];
+    const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
+    const wh_kv4_place place = kv_place<16, 64>(a, false);
     const uint32_t kvh = place.head;
     const wh_kv4_tile tile = place.tile;
     if (!tile.ok) return;
-    const uint32_t blocks = (tile.n_keys + 31) / 32;
+    const uint32_t blocks = (tile.n_keys + 63) / 64;
     const uint32_t blk0 = place.split ? place.split * place.chunk : 0, blk1 = min(blocks, blk0 + place.chunk);
     if (place.split && blk0 >= blocks) return;
-    const bool whole = place.chunk >= blocks;  // the only split: the result is final
+    const bool whole = place.chunk >= blocks;
 
     // this lane's row
-    const uint32_t rr = min(r16, tile.rows - 1), flat = tile.row0 + rr, tok = flat / a.group;
+    const uint32_t flat = tile.row0 + min(r16, tile.rows - 1), tok = flat / a.group;
     const uint32_t head = kvh * a.group + (flat - tok * a.group);
-    const bool live = r16 < tile.rows && tile.token0 + tok < a.n_tokens;
-    const uint32_t token = min(tile.token0 + tok, a.n_tokens - 1);
+    const bool live = r16 < tile.rows;
+    const uint32_t token = tile.token0 + tok;
     const int32_t pos = live ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
+    const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
+    const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
 
-    wh_h8 q[D::kSteps][kParts];
-    wh_kv4_query<HD, kF32> query;
-    query.load(a.q, (uint64_t)token * a.q_stride + (uint64_t)head * HD, g);
-    const float c_row = a.scale_log2 * query.parts(q);
-
-    wh_f4 acc[HD / 16];  // [dim 4g + i][row] of 16 dims each, times 2^(127 - ref)
-#pragma unroll
-    for (int f = 0; f < HD / 16; ++f) acc[f] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
-    float m = kMinusBig, l = 0.0f;
-    int ref = 0;  // values are taken relative to this scale byte
-
+    // rows are requested kHold blocks of 16 ahead, their pages twice that
     const uint32_t* const table = a.tables + tile.request * a.table_stride;
-    const uint32_t pmask = (1u << a.s.shift) - 1u;
-    // a block's rows are requested one block ahead, their pages two
-    wh_kv4_raw<HD, 2> kr, vr;
-    bool there[2], bad = false;
-    uint32_t page[2];
-    auto key_at = [&](uint32_t blk, int h, bool* in) {
-        const uint32_t v = blk * 32 + 16 * h + r16;
-        *in = blk < blk1 && v < tile.n_keys;
-        return *in ? wh_kv4_key(tile, v) : 0;
+    const uint32_t pmask = (1u << a.s.shift) - 1u, end = min(tile.n_keys, blk1 * 64);
+    wh_kv4_raw<HD, kHold> kr, vr;
+    uint32_t page[kHold];
+    bool bad = false;
+    // the tile's first key stands in for those past the last; n counts parts of kHold blocks
+    constexpr uint32_t kParts64 = 4 / kHold;
+    auto key_at = [&](uint32_t n, int h) {
+        const uint32_t v = (n / kParts64) * 64 + 16 * (kHold * (n % kParts64) + h) + r16;
+        return wh_kv4_key(tile, v < end ? v : 0);
     };
-    auto request_pages = [&](uint32_t blk) {
+    // the part after part n of this wave
+    auto after = [&](uint32_t n) { return n % kParts64 == kParts64 - 1 ? n + 1 + 3 * kParts64 : n + 1; };
+    auto request_pages = [&](uint32_t n) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            bool in;
-            const uint32_t key = key_at(blk, h, &in);
-            page[h] = in ? table[key >> a.s.shift] : 0;
-        }
+        for (int h = 0; h < kHold; ++h) page[h] = table[key_at(n, h) >> a.s.shift];
     };
-    auto request = [&](uint32_t blk) {
+    auto request = [&](uint32_t n) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t key = key_at(blk, h, &there[h]);
+        for (int h = 0; h < kHold; ++h) {
+            const uint32_t key = key_at(n, h);
             const bool out = page[h] >= a.s.n_pages;
             bad |= out;
             const uint64_t line = wh_kv4_line(out ? 0 : page[h], kvh, key & pmask, a.s.kv_heads, a.s.shift);
             kv_load(kr, h, a.k, line, g);
             if constexpr (!kLatent) kv_load(vr, h, a.v, line, g);
         }
-        request_pages(blk + 4);
+        request_pages(after(n));
     };
-    _Float16* const stage = (_Float16*)(smem + wave * D::kStage);
-    const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
-    const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
+    const uint32_t part0 = (blk0 + wave) * kParts64;
+    const bool any = blk0 + wave < blk1;
+    if (any) request_pages(part0);
 
-    request_pages(blk0 + wave);
-    request(blk0 + wave);
+    // the row's query
+    wh_h8 qd[kDirect ? 1 : D::kSteps][kParts];
+    wh_i8 qx[kDirect ? kPieces : 1][2];
+    uint32_t q_scale = 0;
+    float c;  // a score is its sum times this (and its key's power of two, unless direct)
+    {
+        const uint64_t at = (uint64_t)token * a.q_stride + (uint64_t)head * HD;
+        if constexpr (kDirect) {
+            const uint16_t* const p = (const uint16_t*)a.q + at + 16 * g;
+            wh_u4 raw[kPieces][2][2];
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[j][i >> 1][i & 1] = *(const wh_u4*)(p + 128 * j + 64 * (i >> 1) + 8 * (i & 1));
+            if (any) request(part0);
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j)
+                q_scale |= kv_query_e4m3(raw[j], a.scale_log2 < 0.0f ? 0x80008000u : 0u, qx[j][0], qx[j][1]) << (8 * j);
+            c = fmaxf(fabsf(a.scale_log2), 1.0e-37f);
+        } else {
+            wh_kv4_query<HD, kF32> query;
+            query.load(a.q, at, g);
+            if (any) request(part0);
+            c = a.scale_log2 * query.parts(qd);
+        }
+    }
+
+    wh_f4 acc[HD / 16];  // [dim 16 f + 4g + i][row], times 2^(127 - ref)
+#pragma unroll
+    for (int f = 0; f < HD / 16; ++f) acc[f] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+    float m = kMinusBig, l = 0.0f;
+    int ref = 0;
+    auto raise_ref = [&](uint32_t top) {  // top: of this lane
+        for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+        const int to = min((int)top + 3, 254);
+        const float f = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) acc[i] *= f;
+        ref = to;
+    };
+
+    uint8_t* const mine = smem + wave * W::kWave;
+    _Float16* const rel = (_Float16*)(mine + W::kAtRel);  // [group][16 g + 4 b + i of key 16 b + 4 g + i]
+    float* const key_s = (float*)(mine + W::kAtKeys);     // [keys', values'][key]
+    // 16-byte chunk c of key's row lies at chunk c ^ swizzle: neither the rows that a store
+    // meets (b fixed) nor those of a transposed read (g fixed) share banks
+    auto swizzle = [](uint32_t key) {
+        const uint32_t i = key & 3, b = ((key >> 4) + (key >> 2)) & 3;
+        return HD == 512 ? i | b << 2 : HD == 256 ? i >> 1 | b << 1 : HD == 128 ? b : b & 1;
+    };
+    const uint32_t tkey = 16 * (r16 >> 2) + 4 * g + (r16 & 3);  // this lane's source row of a transposed read
+
     for (uint32_t blk = blk0 + wave; blk < blk1; blk += 4) {
-        uint32_t ktop[2], vtop[2];
-        bool above = false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            ktop[h] = kv_top_byte(kr, h);
-            vtop[h] = kLatent ? ktop[h] : kv_top_byte(vr, h);
-            above |= there[h] && vtop[h] < 255 && (int)vtop[h] > ref;
-        }
-        // a value row above the reference: raise it, with room, and scale what is there
-        if (__ballot(above)) {
-            int top = max(there[0] && vtop[0] < 255 ? (int)vtop[0] : 0, there[1] && vtop[1] < 255 ? (int)vtop[1] : 0);
-            for (int off = 8; off >= 1; off >>= 1) top = max(top, __shfl_xor(top, off, 64));
-            const int to = min(top + 3, 254);
-            const float f = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
-#pragma unroll
-            for (int i = 0; i < HD / 16; ++i) acc[i] *= f;
-            ref = to;
-        }
+        wh_f4 s[4];
         kv_wave_order();
-        if (g == 0) {
+        wh_static_for<(int)kParts64>([&](auto pc) {
+            constexpr int part = decltype(pc)::value;
+            uint32_t ktop[kHold], vtop[kHold];
+            uint32_t above = 0;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                key_scale[wave][0][16 * h + r16] = kv_key_scale(ktop[h], vtop[h]);
-                key_scale[wave][1][16 * h + r16] = kv_value_scale(vtop[h], ref);
+            for (int h = 0; h < kHold; ++h) {
+                const uint32_t v = blk * 64 + 16 * (kHold * part + h) + r16;
+                if constexpr (kDirect) {
+                    const uint32_t b = kv_piece_scales(kLatent ? kr : vr, h, g);
+#pragma unroll
+                    for (int j = 0; j < kPieces; ++j) {
+                        const uint32_t e = (b >> (8 * j)) & 0xff;
+                        above = max(above, v < end && e < 255 ? e : 0u);
+                    }
+                    ktop[h] = vtop[h] = b;
+                } else {
+                    ktop[h] = kv_top_byte(kr, h);
+                    vtop[h] = kLatent ? ktop[h] : kv_top_byte(vr, h);
+                    above = max(above, v < end && vtop[h] < 255 ? vtop[h] : 0u);
+                }
             }
-        }
-        wh_f4 s[2];
+            if (__ballot((int)above > ref)) {
+                const int old = ref;
+                raise_ref(above);
+                if constexpr (part > 0) {  // what the earlier part left is against the old one
+                    const float f = kv_bits((uint32_t)max(old - ref + 127, 0) << 23);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            s[h] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
-            _Float16* const mine = stage + (16 * h + r16) * D::kLd;
+                    for (int h = 0; h < kHold * part; ++h)
+                        if constexpr (kDirect) {
 #pragma unroll
-            for (int k = 0; k < D::kSteps; ++k) {
-                const int j = k / D::kWords, w = k - j * D::kWords;
-                const wh_h8 x = kv_decode(kr.c[h][j][w], kv_rel(kr, h, j, g, ktop[h]));
-                if constexpr (kF32) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][1], s[h], 0, 0, 0);
-                s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][0], s[h], 0, 0, 0);
-                if constexpr (kLatent) *(wh_h8*)(mine + kv_dim<HD>(k, g)) = x;
-                else *(wh_h8*)(mine + kv_dim<HD>(k, g)) = kv_decode(vr.c[h][j][w], kv_rel(vr, h, j, g, vtop[h]));
+                            for (int j = 0; j < kPieces; ++j)
+                                rel[(4 * j + g) * W::kRel + 16 * (r16 >> 2) + 4 * h + (r16 & 3)] *= (_Float16)f;
+                        } else if (g == 0) {
+                            key_s[64 + 16 * h + r16] *= f;
+                        }
+                }
             }
-        }
+#pragma unroll
+            for (int h = 0; h < kHold; ++h) {
+                const int b = kHold * part + h;
+                const uint32_t key = 16 * b + r16, at = 16 * (r16 >> 2) + 4 * b + (r16 & 3);
+                // value scales, and the powers of two of keys and value rows where those are against their largest
+                if constexpr (kDirect) {
+#pragma unroll
+                    for (int j = 0; j < kPieces; ++j) {
+                        const int e = (int)((vtop[h] >> (8 * j)) & 0xff) - ref;  // above ref only where it does not count
+                        rel[(4 * j + g) * W::kRel + at] = (_Float16)kv_bits((uint32_t)max(min(e, 0) + 127, 0) << 23);
+                    }
+                } else {
+                    if (g == 0) {
+                        key_s[key] = kv_key_scale(ktop[h], vtop[h]);
+                        key_s[64 + key] = kv_value_scale(vtop[h], ref);
+                    }
+                    if constexpr (HD == 64) {
+                        if ((g & 1) == 0) rel[(g >> 1) * W::kRel + at] = (_Float16)kv_rel(kLatent ? kr : vr, h, 0, g, vtop[h]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kPieces; ++j)
+                            rel[(4 * j + g) * W::kRel + at] = (_Float16)kv_rel(kLatent ? kr : vr, h, j, g, vtop[h]);
+                    }
+                }
+                // the value row's codes
+                uint8_t* const row = mine + key * W::kRow;
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    const uint32_t* const cw = kLatent ? kr.c[h][j] : vr.c[h][j];
+                    if constexpr (HD == 64) *(wh_u2*)(row + 16 * ((g >> 1) ^ swizzle(key)) + 8 * (g & 1)) = (wh_u2){cw[0], cw[1]};
+                    else *(wh_u4*)(row + 16 * ((4 * j + g) ^ swizzle(key))) = (wh_u4){cw[0], cw[1], cw[2], cw[3]};
+                }
+                // scores
+                s[b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (kDirect) {
+                    const uint32_t scale = kLatent ? vtop[h] : kv_piece_scales(kr, h, g);
+                    wh_static_for<kPieces>([&](auto jc) {
+                        constexpr int j = decltype(jc)::value;
+                        wh_i8 x;
+                        x[0] = kr.c[h][j][0], x[1] = kr.c[h][j][1], x[2] = kr.c[h][j][2], x[3] = kr.c[h][j][3];
+                        x[4] = x[5] = x[6] = x[7] = 0;
+#pragma unroll
+                        for (int p = 1; p >= 0; --p)
+                            s[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, qx[j][p], s[b], 4, 0, j, scale, j,
+                                                                                    q_scale - (p ? 0x04040404u : 0u));
+                    });
+                } else {
+#pragma unroll
+                    for (int k = 0; k < D::kSteps; ++k) {
+                        const int j = k / D::kWords, w = k - j * D::kWords;
+                        const wh_h8 x = kv_decode(kr.c[h][j][w], kv_rel(kr, h, j, g, ktop[h]));
+#pragma unroll
+                        for (int p = kParts - 1; p >= 0; --p)
+                            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qd[k][p], s[b], 0, 0, 0);
+                    }
+                }
+                // direct: a value row that holds NaN beside keys that do not
+                if constexpr (kDirect && !kLatent) {
+                    bool nan = false;
+#pragma unroll
+                    for (int j = 0; j < kPieces; ++j) nan |= ((vtop[h] >> (8 * j)) & 0xff) == 255;
+                    if (__builtin_expect(__ballot(nan) != 0, 0)) {
+                        uint64_t hit = __ballot(nan);
+                        hit |= hit >> 32;
+                        hit |= hit >> 16;  // bit r16: key 16 b + r16
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (hit >> (4 * g + i) & 1) s[b][i] = kv_bits(0x7fc00000u);
+                    }
+                }
+            }
+            // the next rows come into the registers of these: not before they are used
+#pragma unroll
+            for (int h = 0; h < kHold; ++h) asm volatile("" : "+v"(s[kHold * part + h])::"memory");
+            request(after(blk * kParts64 + part));
+        });
         kv_wave_order();
-        request(blk + 4);
-        // scores of keys 4g + i of each half, row r16; -inf where it does not see them
-        const uint32_t last = blk * 32 + 31;
+        // -inf where the row does not see a key
+        if constexpr (!kDirect) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) s[b] *= *(const wh_f4*)&key_s[16 * b + 4 * g] * c;
+        }
+        const uint32_t last = blk * 64 + 63;
         const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == 16 &&
-                         (!a.window || (int64_t)wh_kv4_key(tile, max(blk * 32, tile.n_first)) + a.window > pos_hi);
-        float top = kMinusBig;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const wh_f4 ks = *(const wh_f4*)&key_scale[wave][0][16 * h + 4 * g];
-            s[h] *= ks * c_row;
-        }
+                         (!a.window || (int64_t)wh_kv4_key(tile, max(blk * 64, tile.n_first)) + a.window > pos_hi);
         if (!all) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int b = 0; b < 4; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t v = blk * 32 + 16 * h + 4 * g + i;
+                    const uint32_t v = blk * 64 + 16 * b + 4 * g + i;
                     const bool see = (v < tile.n_keys) & wh_kv4_sees(pos, wh_kv4_key(tile, v), a.window, a.first);
-                    s[h][i] = see ? s[h][i] : kMinusInf;
+                    s[b][i] = see ? s[b][i] : kMinusInf;
                 }
         }
+        float top = kMinusInf;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int b = 0; b < 4; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][i]);
+        top = kv_max_groups(top);
+        if constexpr (kDirect) top *= c;
         if (__ballot(top > m + kSlack)) {
             const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
             l *= f;
@@ -758,85 +945,90 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
             for (int i = 0; i < HD / 16; ++i) acc[i] *= f;
             m = to;
         }
-        wh_h8 ph, pl;
+        wh_h8 ph[2], pl[2];
         const float up = kUp - m;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const wh_f4 vs = *(const wh_f4*)&key_scale[wave][1][16 * h + 4 * g];
+        for (int b = 0; b < 4; ++b) {
+            wh_f4 vs;
+            if constexpr (!kDirect) vs = *(const wh_f4*)&key_s[64 + 16 * b + 4 * g];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float w = __builtin_amdgcn_exp2f(s[h][i] + up);
+                const float w = __builtin_amdgcn_exp2f(kDirect ? fmaf(s[b][i], c, up) : s[b][i] + up);
                 l += w;
-                const float x = w * vs[i];
-                ph[4 * h + i] = (_Float16)x;
-                if constexpr (kF32) pl[4 * h + i] = (_Float16)(x - (float)ph[4 * h + i]);
+                float x = w;
+                if constexpr (!kDirect) x *= vs[i];
+                const int n = 4 * (b & 1) + i;
+                ph[b >> 1][n] = (_Float16)x;
+                if constexpr (kF32) pl[b >> 1][n] = (_Float16)(x - (float)ph[b >> 1][n]);
             }
         }
-        // values: lane row = dim r16 of 16, keys 4g + i of each half
+        // values: 16 dims a step, keys of half h in blocks 2 h and 2 h + 1
+        wh_h8 rv[2];
 #pragma unroll
         for (int f = 0; f < HD / 16; ++f) {
-            union {
-                wh_s4 s[2];
-                wh_h8 v;
-            } x;
+            if (f % 2 == 0) {
+                const _Float16* const rp = rel + (f >> 1) * W::kRel + 16 * g;
+                rv[0] = *(const wh_h8*)rp;
+                rv[1] = *(const wh_h8*)(rp + 8);
+            }
+            const uint8_t* const src = mine + tkey * W::kRow + 16 * ((f >> 1) ^ swizzle(tkey)) + 8 * (f & 1);
+            const wh_i2 codes = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) wh_i2*)src);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                x.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) wh_s4*)(stage + (16 * h + 4 * g + (r16 >> 2)) * D::kLd + 16 * f +
-                                                               4 * (r16 & 3)));
-            if constexpr (kF32) acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.v, pl, acc[f], 0, 0, 0);
-            acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.v, ph, acc[f], 0, 0, 0);
+            for (int h = 0; h < 2; ++h) {
+                const wh_h8 x = kv_decode((uint32_t)codes[h], 1.0f) * rv[h];
+                if constexpr (kF32) acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[h], acc[f], 0, 0, 0);
+                acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph[h], acc[f], 0, 0, 0);
+            }
         }
     }
     if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
 
-    // join the four waves
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    // join the four waves: 2 and 3 into 0 and 1, then 1 into 0
+    l = kv_sum_groups(l);
     if (g == 0) {
-        row_m[wave][r16] = m;
-        row_l[wave][r16] = l;
+        wave_m[wave][r16] = m;
+        wave_l[wave][r16] = l;
     }
-    __syncthreads();
-    constexpr int kOld = HD + 4;  // floats between rows of a wave's outputs
-    float* const o = (float*)smem;
-    float mm = row_m[0][r16];
+    kv_lds_barrier();
+    float M = wave_m[0][r16], L = 0.0f;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) mm = fmaxf(mm, row_m[w][r16]);
-    {
-        const float f = __builtin_amdgcn_exp2f(m - mm) * kv_bits((uint32_t)ref << 23);
+    for (int w = 1; w < 4; ++w) M = fmaxf(M, wave_m[w][r16]);
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) *(wh_f4*)(o + (wave * 16 + r16) * kOld + 16 * i + 4 * g) = acc[i] * f;
+    for (int w = 0; w < 4; ++w) L += wave_l[w][r16] * __builtin_amdgcn_exp2f(wave_m[w][r16] - M);
+    const float f0 = __builtin_amdgcn_exp2f(m - M) * kv_bits((uint32_t)ref << 23);
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) acc[i] *= f0;
+    wh_f4* const o = (wh_f4*)smem;  // [wave of a pair][block of dims][lane]
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {
+        if (wave >= (uint32_t)half && wave < 2 * (uint32_t)half) {
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) o[((wave - half) * (HD / 16) + i) * 64 + lane] = acc[i];
+        }
+        kv_lds_barrier();
+        if (wave < (uint32_t)half) {
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) acc[i] += o[(wave * (HD / 16) + i) * 64 + lane];
+        }
+        kv_lds_barrier();
     }
-    __syncthreads();
-    // 16 threads a row
-    const uint32_t row = t >> 4, d0 = (t & 15) * 4;
-    float M = row_m[0][row], L = 0.0f;
-#pragma unroll
-    for (int w = 1; w < 4; ++w) M = fmaxf(M, row_m[w][row]);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) L += row_l[w][row] * __builtin_amdgcn_exp2f(row_m[w][row] - M);
-    const uint32_t rflat = tile.row0 + row, rtok = rflat / a.group, rhead = kvh * a.group + (rflat - rtok * a.group);
-    if (row >= tile.rows || tile.token0 + rtok >= a.n_tokens) return;
+    if (wave || !live) return;
     float denom = L;
-    if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[rhead] * 1.44269504088896340736f - M + kUp);
+    if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
     const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-    float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * 16 + row) * (HD + 2);
+    float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * 16 + r16) * (HD + 2);
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i) {
-        const uint32_t d = 64 * i + d0;
-        wh_f4 x = *(const wh_f4*)(o + row * kOld + d);
-#pragma unroll
-        for (int w = 1; w < 4; ++w) x += *(const wh_f4*)(o + (w * 16 + row) * kOld + d);
-        x *= inv;
+    for (int f = 0; f < HD / 16; ++f) {
+        const uint32_t d = 16 * f + 4 * g;
+        const wh_f4 x = acc[f] * inv;
         if (!whole) {
             *(wh_f2*)(part + d) = (wh_f2){x[0], x[1]};
             *(wh_f2*)(part + d + 2) = (wh_f2){x[2], x[3]};
         } else {
-            kv_store<kF32>(a.out, (uint64_t)(tile.token0 + rtok) * a.out_stride + (uint64_t)rhead * HD + d, x);
+            kv_store<kF32>(a.out, (uint64_t)token * a.out_stride + (uint64_t)head * HD + d, x);
         }
     }
-    if (!whole && (t & 15) == 0) {
+    if (!whole && g == 0) {
         part[HD] = M;
         part[HD + 1] = L;
     }
@@ -1161,9 +1353,6 @@ __global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_at
 // of the largest seen).  Wave (kq, rq) scores its keys against its rows, adds
 // its dims of the run before for all rows, and decodes a share of the run's
 // value rows, which lie in LDS with the weights: one barrier a run.
-typedef int wh_i8 __attribute__((ext_vector_type(8)));
-typedef int wh_i4 __attribute__((ext_vector_type(4)));
-
 template <int HD, bool kLatent>
 struct wh_kv4_direct {
     static constexpr int kRows = 64, kBlocks = 4;
@@ -1180,48 +1369,6 @@ struct wh_kv4_direct {
     static constexpr int kPrun = kRows * kPl;
     static constexpr size_t kLds = 2 * 2 * (size_t)(kRun + kPrun);
 };
-
-// A lane's 32 of 128 bf16 values of a query as two E4M3 parts: dims 16g .. of
-// the first half and of the second, where the instruction wants 8-bit values (it
-// takes 4-bit ones and all scales as 32g ..).  Returns the first part's scale
-// byte for dims 32g .. (the second's is 4 less), 255 where one is not finite.
-__device__ __forceinline__ uint32_t kv_query_e4m3(const wh_u4 (&raw)[2][2], uint32_t flip, wh_i8& hi, wh_i8& lo) {
-    int e[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t w = raw[h][i][k];
-                top = max(top, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
-            }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));  // the other 16 of the 32
-        e[h] = max((int)(top >> 23), 20);
-        const float up = kv_bits((uint32_t)(127 + 127 + 7 - min(e[h], 254)) << 23);  // the largest to [2^7, 2^8)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            int a = 0, b = 0;
-            float x[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t w = raw[h][i >> 1][2 * (i & 1) + (k >> 1)] ^ flip;
-                x[k] = kv_bits(k & 1 ? w & 0xffff0000u : w << 16) * up;
-            }
-            a = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], a, false);
-            a = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], a, true);
-            const wh_f2 u = __builtin_amdgcn_cvt_pk_f32_fp8(a, false), v = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
-            b = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - u.x) * 16.0f, (x[1] - u.y) * 16.0f, b, false);
-            b = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - v.x) * 16.0f, (x[3] - v.y) * 16.0f, b, true);
-            hi[4 * h + i] = a;
-            lo[4 * h + i] = b;
-        }
-    }
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, from = (lane & 15) + 32 * (g & 1);
-    const int e0 = __shfl(e[0], (int)from, 64), e1 = __shfl(e[1], (int)from, 64), w = g < 2 ? e0 : e1;
-    return w == 255 ? 255u : (uint32_t)(w - 7);
-}
 
 template <int HD, bool kLatent>
 __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_kv4_attn_direct(wh_kv4_attn_args a) {
@@ -1363,7 +1510,7 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
         uint32_t scale[kKeys];
 #pragma unroll
         for (int kb = 0; kb < kKeys; ++kb) {
-            scale[kb] = kv_piece_scales(ks[kb], g);
+            scale[kb] = kv_piece_scales(ks[kb], 0, g);
 #pragma unroll
             for (int b = 0; b < kMine; ++b) s[b][kb] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -2017,12 +2164,12 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
             k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
         return hipGetLastError();
     }
-    constexpr size_t lds = 4 * (size_t)wh_kv4_dims<HD>::kStage;
+    constexpr size_t lds = wh_kv4_narrow<HD, kF32>::kLds;
     static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn<HD, kF32, kLatent>,
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (set != hipSuccess) return set;
     k_kv4_attn<HD, kF32, kLatent><<<grid, 256, lds, stream>>>(a);
-    if (split) k_kv4_join<HD, kF32, 16, 32><<<dim3(a.n_tiles * a.s.kv_heads, 4), 256, 0, stream>>>(a);
+    if (split) k_kv4_join<HD, kF32, 16, 64><<<dim3(a.n_tiles * a.s.kv_heads, 4), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -2065,7 +2212,7 @@ wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, bool 
     const uint64_t rows = (uint64_t)a.n_tokens * a.group;
     const uint32_t wide_rows = bf16 ? 64 : 32;
     p.wide = rows >= (uint64_t)a.n_requests * (wide_rows - 16);
-    const uint32_t tile_rows = p.wide ? wide_rows : 16, block = p.wide ? 64 : 32;
+    const uint32_t tile_rows = p.wide ? wide_rows : 16, block = 64;
     p.n_tiles = (uint32_t)wh_kv4_tile_slots(a.n_tokens, a.n_requests, a.group, tile_rows);
     // more workgroups than tiles: the keys are cut up by the lengths on the device
     uint64_t keys = max_len;
@@ -2073,7 +2220,7 @@ wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, bool 
     const uint64_t resident = p.wide && a.s.head_dim >= 256 ? 256 : a.s.head_dim >= 512 ? 256 : a.s.head_dim == 256 ? 512 : p.wide ? 512 : 1024;
     p.min_blocks = 128 / block;
     p.units = (uint32_t)(resident / a.s.kv_heads);
-    const uint64_t busy = std::max<uint64_t>(rows / tile_rows, 1);  // tiles that hold rows, at least
+    const uint64_t busy = std::max<uint64_t>(rows / tile_rows, a.n_requests);  // tiles, where every request has rows
     if (p.units < 2 * busy || a.n_requests > WH_KV_SPLIT_REQUESTS || keys <= 128) p.units = 0;
     p.units = std::max(p.units, p.n_tiles);
     if (p.units > p.n_tiles) p.part_bytes = (size_t)p.units * a.s.kv_heads * tile_rows * (a.s.head_dim + 2) * sizeof(float);
