@@ -22,6 +22,7 @@ typedef short wh_s4 __attribute__((ext_vector_type(4)));
 typedef __fp16 wh_hh4 __attribute__((ext_vector_type(4)));
 typedef int wh_i8 __attribute__((ext_vector_type(8)));
 typedef int wh_i2 __attribute__((ext_vector_type(2)));
+typedef int wh_i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t wh_u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t wh_u4 __attribute__((ext_vector_type(4)));
 
@@ -380,6 +381,7 @@ __device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a, bool
             const int src = __ffsll((unsigned long long)hit) - 1;
             const uint32_t n = __shfl(splits, src, 64), before = __shfl(by_tile ? t - tiles : u - tiles * splits, src, 64);
             const uint32_t at = x - (by_tile ? tile0 : unit0) - before, local = by_tile ? at : at / n;
+            r.chunk = wh_kv4_even(__shfl(blocks, src, 64), n);
             if (by_tile) r.unit = unit0 + __shfl(u - tiles * splits, src, 64) + at * n;
             r.split = by_tile ? 0 : at - local * n;
             const uint32_t q = b + src, s0 = start(q);
@@ -645,6 +647,16 @@ __device__ __forceinline__ uint32_t kv_query_e4m3(const wh_u4 (&raw)[2][2], uint
     return w == 255 ? 255u : (uint32_t)(w - 7);
 }
 
+// Max over groups of 2, 4 or 8 lanes next to each other, in all of them.
+template <int kN>
+__device__ __forceinline__ uint32_t kv_near_max(uint32_t v) {
+    auto with = [&](uint32_t other) { v = max(v, other); };
+    with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));                  // lanes 1 0 3 2 of a quad
+    if constexpr (kN >= 4) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));   // 2 3 0 1
+    if constexpr (kN >= 8) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));  // 7 - lane of eight
+    return v;
+}
+
 // Max and sum over the four lanes of a row (lane % 16), in all of them.
 __device__ __forceinline__ float kv_max_groups(float v) {
     typedef unsigned u2 __attribute__((ext_vector_type(2)));
@@ -684,7 +696,7 @@ struct wh_kv4_narrow {
 };
 
 template <int HD, bool kF32, bool kLatent>
-__global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
+__global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn_args a) {
     using D = wh_kv4_dims<HD>;
     using W = wh_kv4_narrow<HD, kF32>;
     constexpr int kParts = W::kParts, kHold = W::kHold, kPieces = W::kPieces;
@@ -1035,355 +1047,56 @@ __global__ void __launch_bounds__(256) k_kv4_attn(wh_kv4_attn_args a) {
 }
 
 // A tile of 64 rows (32 in f32, whose queries and weights are two parts) for
-// the calls that have them: every decoded key serves four blocks of 16 rows.
-// Wave w scores keys 16 (w % 4) .. of each run of 64 against the rows of its
-// half (4 waves: all of them), its queries in registers, and leaves the value
-// rows it decoded and its weights in LDS; it adds the outputs of its share of
-// the dims for all rows and keys.  The two work on neighbouring runs at once, so
-// one barrier a run is enough and the matrix work of one covers the decoding
-// and the loads of the other.  Weights are taken against the running maximum as
-// it is; only a run with a score 2^5 above it (or a value row above the
-// reference) joins the waves' maxima and makes its weights again.
-template <int HD, bool kF32>
-struct wh_kv4_wide {
-    // rows of 256 and 512 dims: queries and outputs of 64 rows fill the registers
-    // of eight waves, the halves decoding the same keys
-    static constexpr int kHalves = HD >= 256 ? 2 : 1, kWaves = 4 * kHalves, kThreads = 64 * kWaves;
-    static constexpr int kParts = kF32 ? 2 : 1, kBlocks = kF32 ? 2 : 4, kRows = 16 * kBlocks;
-    static constexpr int kMine = kBlocks / kHalves;         // blocks of rows that a wave scores
-    static constexpr int kDims = HD / 16 / kWaves;          // blocks of dims that a wave adds up
-    static constexpr int kRun = 64 * wh_kv4_dims<HD>::kLd;  // f16 of a run's decoded rows
-    static constexpr int kPl = 72;                          // f16 between rows of weights
-    static constexpr int kPrun = kParts * kRows * kPl;
-    static constexpr size_t kLds = 2 * 2 * (size_t)(kRun + kPrun);
+// the calls that have them.  Eight waves bring a run of 64 keys' codes into LDS
+// once, as they lie, and the powers of two beside them.  Wave (kq, rq) scores its
+// keys against 16 rows, whose queries stay in its registers, and leaves their
+// weights in LDS; for the run before it adds up its share of the dims for all
+// rows: the codes are read transposed, sixteen keys of one dim a lane (the 4-bit
+// transposing read), decoded to small f16 numbers and multiplied by their powers
+// of two.  The two work on neighbouring runs at once, so one barrier a run is
+// enough and the matrix work of one covers the loads and exponentials of the
+// other.  Weights are taken against the running maximum as it is; only a run with
+// a score 2^5 above it (or a value row above the reference) joins the waves'
+// maxima and makes its weights again.
+template <int HD, bool kF32, bool kLatent>
+struct wh_kv4_packed {
+    static constexpr int kRows = kF32 ? 32 : 64, kBlocks = kRows / 16;
+    static constexpr int kWaves = HD >= 256 ? 8 : 4, kThreads = 64 * kWaves, kPerSimd = HD >= 256 ? 2 : 3;
+    static constexpr int kParts = kF32 ? 2 : 1;
+    static constexpr int kRowGroups = kBlocks, kKeyGroups = kWaves / kRowGroups;
+    static constexpr int kKeyBlocks = 4 / kKeyGroups;    // blocks of 16 keys a wave scores
+    static constexpr int kPieces = HD >= 128 ? HD / 128 : 1;
+    static constexpr int kGroups = HD / 32;
+    static constexpr int kDims = HD / 16 / kWaves;       // blocks of 16 dims whose outputs a wave adds up
+    static constexpr bool kBoth = HD >= 128 || kLatent;  // a lane brings chunks of keys and of values
+    static constexpr int kMine = HD >= 256 ? HD / 256 : 1;  // 16-byte chunks, each a group of 32 dims, that a lane brings
+    static constexpr int kLanes = kGroups / kMine;       // lanes of a row
+    static constexpr int kBring = kLanes;                // waves that bring a plane's 64 rows
+    static constexpr int kRow = HD / 2;                  // bytes of a row's codes
+    static constexpr int kCodes = 64 * kRow;             // bytes of a run's codes
+    static constexpr int kKeyBufs = kLatent ? 3 : 2;     // latent codes are values one run later
+    static constexpr int kRel = 72;                      // f16 between groups of value scales
+    static constexpr int kPl = 72;                       // f16 between rows of weights
+    static constexpr int kAtValues = kKeyBufs * kCodes;                       // byte offsets in LDS
+    static constexpr int kAtScales = kAtValues + (kLatent ? 0 : 3 * kCodes);  // [2][g][key] dwords
+    static constexpr int kAtKeys = kAtScales + 2 * 4 * 64 * 4;                // f32: [2][key] power of two of keys
+    static constexpr int kAtTops = kAtKeys + (kF32 ? 2 * 64 * 4 : 0);         // f32: [2][key] exponent of value rows
+    static constexpr int kAtRel = kAtTops + (kF32 ? 2 * 64 * 4 : 0);          // [3][group][key] f16
+    static constexpr int kAtWeights = kAtRel + 3 * kGroups * kRel * 2;        // [2][part][row][key] f16
+    static constexpr size_t kLds = kAtWeights + 2 * (size_t)kParts * kRows * kPl * 2;
 };
 
 template <int HD, bool kF32, bool kLatent>
-__global__ void __launch_bounds__((wh_kv4_wide<HD, kF32>::kThreads), 2) k_kv4_attn_wide(wh_kv4_attn_args a) {
-    using D = wh_kv4_dims<HD>;
-    using W = wh_kv4_wide<HD, kF32>;
-    constexpr int kParts = W::kParts, kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kMine = W::kMine;
+__global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), (wh_kv4_packed<HD, kF32, kLatent>::kPerSimd)) k_kv4_attn_packed(wh_kv4_attn_args a) {
+    using W = wh_kv4_packed<HD, kF32, kLatent>;
+    constexpr int kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kPieces = W::kPieces, kParts = W::kParts;
+    constexpr int kKeyBlocks = W::kKeyBlocks, kWaves = W::kWaves;
     const wh_kv4_place place = kv_place<W::kRows, 64>(a, false);
     extern __shared__ __align__(16) uint8_t smem[];
-    _Float16* const vbuf = (_Float16*)smem;                      // [2][key][kLd]
-    _Float16* const pbuf = vbuf + 2 * W::kRun;                   // [2][part][row][kPl]
-    __shared__ __align__(16) float key_scale[W::kWaves][2][16];  // [wave][keys', values'][key]
-    // of each row: the maximum, what its scores are multiplied by, its position
-    __shared__ float wave_m[4][kRows], wave_l[4][kRows], row_m[kRows], row_c[kRows];
-    __shared__ int32_t row_pos[kRows];
-    __shared__ uint32_t wave_top[4], raise[2];
-    const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
-    const uint32_t kvh = place.head, kq = wave & 3, half = wave >> 2;
-    const wh_kv4_tile tile = place.tile;
-    if (!tile.ok) return;
-    const uint32_t runs = (tile.n_keys + 63) / 64;
-    const uint32_t run0 = place.split ? place.split * place.chunk : 0, run1 = min(runs, run0 + place.chunk);
-    if (place.split && run0 >= runs) return;
-    const bool whole = place.chunk >= runs;
-    if (t < 2) raise[t] = 0;
-    if (t < kRows) row_m[t] = kMinusBig;
-
-    // queries of rows r16 of this wave's blocks
-    wh_h8 q[kMine][D::kSteps][kParts];
-    float l[kMine];
-    wh_kv4_query<HD, kF32> query[kMine];
-#pragma unroll
-    for (int b = 0; b < kMine; ++b) {
-        const uint32_t r = 16 * (half * kMine + b) + r16, flat = tile.row0 + min(r, tile.rows - 1), tok = flat / a.group;
-        const uint32_t head = kvh * a.group + (flat - tok * a.group);
-        query[b].load(a.q, (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD, g, half);
-        row_pos[r] = r < tile.rows ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
-        l[b] = 0.0f;
-    }
-#pragma unroll
-    for (int b = 0; b < kMine; ++b) row_c[16 * (half * kMine + b) + r16] = a.scale_log2 * query[b].parts(q[b]);
-    const uint32_t row0 = 16 * half * kMine + r16;  // of block 0
-    const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
-    const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
-
-    wh_f4 acc[kDims][kBlocks];  // [dim 16 (kDims wave + f) + 4g + i][row]
-#pragma unroll
-    for (int f = 0; f < kDims; ++f)
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) acc[f][b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
-    int ref = 0;
-
-    // a run's rows are requested one run ahead, their page two
-    const uint32_t* const table = a.tables + tile.request * a.table_stride;
-    const uint32_t pmask = (1u << a.s.shift) - 1u;
-    wh_kv4_raw<HD, 1> kr, vr;
-    bool there = false, bad = false;
-    uint32_t page = 0;
-    auto key_at = [&](uint32_t run, bool* in) {
-        const uint32_t v = run * 64 + 16 * kq + r16;
-        *in = run < run1 && v < tile.n_keys;
-        return *in ? wh_kv4_key(tile, v) : 0;
-    };
-    auto request_page = [&](uint32_t run) {
-        bool in;
-        const uint32_t key = key_at(run, &in);
-        page = in ? table[key >> a.s.shift] : 0;
-    };
-    auto request = [&](uint32_t run) {
-        const uint32_t key = key_at(run, &there);
-        const bool out = page >= a.s.n_pages;
-        bad |= out;
-        const uint64_t line = wh_kv4_line(out ? 0 : page, kvh, key & pmask, a.s.kv_heads, a.s.shift);
-        kv_load(kr, 0, a.k, line, g);
-        if constexpr (!kLatent) kv_load(vr, 0, a.v, line, g);
-        request_page(run + 1);
-    };
-
-    // a step of a run's outputs: 32 keys, a block of rows (f32: a part of one);
-    // the values of these keys stay in registers for all blocks
-    constexpr int kTake = kDims < 2 ? kDims : 2;
-    wh_h8 x[kTake];
-    auto values_step = [&](uint32_t at, int k) {
-        const int kf = k / (kBlocks * kParts), ks = kf / (kDims / kTake), f0 = kf % (kDims / kTake) * kTake;
-        const int bp = k - kf * (kBlocks * kParts), b = bp / kParts, p = kParts - 1 - bp % kParts;
-        if (bp == 0) {
-            const _Float16* const vb = vbuf + at * W::kRun + (32 * ks + 4 * g + (r16 >> 2)) * D::kLd +
-                                       16 * (kDims * wave + f0) + 4 * (r16 & 3);
-#pragma unroll
-            for (int f = 0; f < kTake; ++f) {
-                union {
-                    wh_s4 h[2];
-                    wh_h8 v;
-                } u;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) wh_s4*)(vb + 16 * h * D::kLd + 16 * f));
-                x[f] = u.v;
-            }
-        }
-        const wh_h8 w = *(const wh_h8*)(pbuf + at * W::kPrun + (p * kRows + 16 * b + r16) * W::kPl + 32 * ks + 8 * g);
-#pragma unroll
-        for (int f = 0; f < kTake; ++f)
-            acc[f0 + f][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[f], w, acc[f0 + f][b], 0, 0, 0);
-    };
-    constexpr int kValueSteps = 2 * kBlocks * kParts * (kDims / kTake);
-    wh_f4 s[kMine];
-    auto pass = [&](uint32_t run, auto first) {
-        const uint32_t at = run & 1;
-        const uint32_t ktop = kv_top_byte(kr, 0), vtop = kLatent ? ktop : kv_top_byte(vr, 0);
-        const bool counts = there && vtop < 255;
-#pragma unroll
-        for (int b = 0; b < kMine; ++b) s[b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
-        _Float16* const mine = vbuf + at * W::kRun + (16 * kq + r16) * D::kLd + 8 * half;
-        kv_wave_order();
-        if (g == 0) {
-            key_scale[wave][0][r16] = kv_key_scale(ktop, vtop);
-            key_scale[wave][1][r16] = kv_value_scale(vtop, ref);
-        }
-        // scores, 32 dims a step, beside the outputs of the run before
-#pragma unroll
-        for (int k = 0; k < D::kSteps; ++k) {
-            // the second half takes the steps of a pair in the other order: both leave their first in LDS
-            const int j = k / D::kWords, w = k - j * D::kWords;
-            auto word = [&](const wh_kv4_raw<HD, 1>& r) { return W::kHalves == 2 && half ? r.c[0][j][w ^ 1] : r.c[0][j][w]; };
-            const wh_h8 y = kv_decode(word(kr), kv_rel(kr, 0, j, g, ktop));
-#pragma unroll
-            for (int b = 0; b < kMine; ++b)
-#pragma unroll
-                for (int p = kParts - 1; p >= 0; --p)
-                    s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[b][k][p], s[b], 0, 0, 0);
-            if (W::kHalves == 1 || !(k & 1)) {
-                if constexpr (kLatent) *(wh_h8*)(mine + kv_dim<HD>(k, g)) = y;
-                else *(wh_h8*)(mine + kv_dim<HD>(k, g)) = kv_decode(word(vr), kv_rel(vr, 0, j, g, vtop));
-            }
-            if constexpr (!decltype(first)::value) {
-#pragma unroll
-                for (int v = kValueSteps * k / D::kSteps; v < kValueSteps * (k + 1) / D::kSteps; ++v) values_step(at ^ 1, v);
-            }
-        }
-        request(run + 1);
-        kv_wave_order();
-        const wh_f4 ks = *(const wh_f4*)&key_scale[wave][0][4 * g];
-#pragma unroll
-        for (int b = 0; b < kMine; ++b) s[b] *= ks * row_c[row0 + 16 * b];
-        // -inf where a row does not see this lane's keys
-        const uint32_t v0 = run * 64 + 16 * kq + 4 * g, last = run * 64 + 63;
-        const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == kRows &&
-                         (!a.window || (int64_t)wh_kv4_key(tile, max(run * 64, tile.n_first)) + a.window > pos_hi);
-        if (!all) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t key = wh_kv4_key(tile, v0 + i);
-                const bool in = v0 + i < tile.n_keys;
-#pragma unroll
-                for (int b = 0; b < kMine; ++b) {
-                    const bool see = in & wh_kv4_sees(row_pos[row0 + 16 * b], key, a.window, a.first);
-                    s[b][i] = see ? s[b][i] : kMinusInf;
-                }
-            }
-        }
-        float top[kMine], add[kMine];
-        bool over = counts && (int)vtop > ref;
-#pragma unroll
-        for (int b = 0; b < kMine; ++b) {
-            top[b] = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
-            over |= top[b] > row_m[row0 + 16 * b] + kSlack;
-        }
-        auto weights = [&](auto max_of) {
-            const wh_f4 vs = *(const wh_f4*)&key_scale[wave][1][4 * g];
-            _Float16* const pw = pbuf + at * W::kPrun + (16 * half * kMine + r16) * W::kPl + 32 * (kq >> 1) + 8 * g + 4 * (kq & 1);
-#pragma unroll
-            for (int b = 0; b < kMine; ++b) {
-                union {
-                    _Float16 h[4];
-                    wh_u2 u;
-                } hi, lo;
-                const float up = kUp - max_of(b);
-                float w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(s[b][i] + up);
-                    const float x = w[i] * vs[i];
-                    hi.h[i] = (_Float16)x;
-                    lo.h[i] = (_Float16)(x - (float)hi.h[i]);
-                }
-                add[b] = (w[0] + w[1]) + (w[2] + w[3]);
-                *(wh_u2*)(pw + 16 * b * W::kPl) = hi.u;
-                if constexpr (kF32) *(wh_u2*)(pw + (kRows + 16 * b) * W::kPl) = lo.u;
-            }
-        };
-        weights([&](int b) { return row_m[row0 + 16 * b]; });
-        if (__ballot(over) && lane == 0) raise[at] = run + 1;
-        kv_lds_barrier();
-        if (__builtin_expect(__builtin_amdgcn_readfirstlane(raise[at]) == run + 1, 0)) {  // the whole workgroup
-            uint32_t vmax = counts ? vtop : 0;
-            for (int off = 8; off >= 1; off >>= 1) vmax = max(vmax, (uint32_t)__shfl_xor((int)vmax, off, 64));
-#pragma unroll
-            for (int b = 0; b < kMine; ++b) {
-                top[b] = fmaxf(top[b], __shfl_xor(top[b], 16, 64));
-                top[b] = fmaxf(top[b], __shfl_xor(top[b], 32, 64));
-                if (g == 0) wave_m[kq][16 * (half * kMine + b) + r16] = top[b];
-            }
-            if (lane == 0 && half == 0) wave_top[kq] = vmax;
-            kv_lds_barrier();
-            vmax = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
-            const int to = (int)vmax > ref ? min((int)vmax + 3, 254) : ref;
-            const float f_ref = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
-            ref = to;
-            auto raised = [&](uint32_t row) {
-                return fmaxf(fmaxf(row_m[row], fmaxf(wave_m[0][row], wave_m[1][row])), fmaxf(wave_m[2][row], wave_m[3][row]));
-            };
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                const uint32_t row = 16 * b + r16;
-                const float f = __builtin_amdgcn_exp2f(row_m[row] - raised(row)) * f_ref;
-#pragma unroll
-                for (int k = 0; k < kDims; ++k) acc[k][b] *= f;
-            }
-            float m[kMine];
-#pragma unroll
-            for (int b = 0; b < kMine; ++b) {
-                m[b] = raised(row0 + 16 * b);
-                l[b] *= __builtin_amdgcn_exp2f(row_m[row0 + 16 * b] - m[b]);
-            }
-            if (g == 0) key_scale[wave][1][r16] = kv_value_scale(vtop, ref);
-            kv_wave_order();
-            weights([&](int b) { return m[b]; });
-            kv_lds_barrier();
-#pragma unroll
-            for (int b = 0; b < kMine; ++b)
-                if (kq == 0 && g == 0) row_m[row0 + 16 * b] = m[b];
-            kv_lds_barrier();
-        }
-#pragma unroll
-        for (int b = 0; b < kMine; ++b) l[b] += add[b];
-    };
-
-    request_page(run0);
-    request(run0);
-    kv_lds_barrier();
-    if (run0 < run1) pass(run0, std::true_type());
-    for (uint32_t run = run0 + 1; run < run1; ++run) pass(run, std::false_type());
-    if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
-    if (run0 < run1) {
-#pragma unroll
-        for (int k = 0; k < kValueSteps; ++k) values_step((run1 - 1) & 1, k);
-    }
-
-#pragma unroll
-    for (int b = 0; b < kMine; ++b) {
-        l[b] += __shfl_xor(l[b], 16, 64);
-        l[b] += __shfl_xor(l[b], 32, 64);
-        if (g == 0) wave_l[kq][16 * (half * kMine + b) + r16] = l[b];
-    }
-    kv_lds_barrier();
-    const float up = kv_bits((uint32_t)ref << 23);
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-        const uint32_t r = 16 * b + r16;
-        if (r >= tile.rows) continue;
-        const uint32_t flat = tile.row0 + r, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
-        const float L = (wave_l[0][r] + wave_l[1][r]) + (wave_l[2][r] + wave_l[3][r]), M = row_m[r];
-        float denom = L;
-        if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
-        const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-        float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * kRows + r) * (HD + 2);
-        const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
-#pragma unroll
-        for (int f = 0; f < kDims; ++f) {
-            const uint32_t d = 16 * (kDims * wave + f) + 4 * g;
-            const wh_f4 y = acc[f][b] * up * inv;
-            if (!whole) {
-                *(wh_f2*)(part + d) = (wh_f2){y[0], y[1]};
-                *(wh_f2*)(part + d + 2) = (wh_f2){y[2], y[3]};
-            } else {
-                kv_store<kF32>(a.out, at + d, y);
-            }
-        }
-        if (!whole && wave == 0 && g == 0) {
-            part[HD] = M;
-            part[HD + 1] = L;
-        }
-    }
-}
-
-// The same tile for bf16 queries on rows of 128 dims and more, where the cached
-// codes are an operand of the scores as they lie: the block-scaled matrix
-// instruction takes E2M1 codes with a power of two for every 32 dims, which is
-// the cache's format, against a query of two E4M3 parts with powers of two of
-// their own (four significant bits each, so a bf16 is exact down to 2^-14 of the
-// largest of its 32).  Nothing of a key is decoded then but its value row, once,
-// into f16 relative to one reference byte `ref` (exact for scales down to 2^-20
-// of the largest seen).  Wave (kq, rq) scores its keys against its rows, adds
-// its dims of the run before for all rows, and decodes a share of the run's
-// value rows, which lie in LDS with the weights: one barrier a run.
-template <int HD, bool kLatent>
-struct wh_kv4_direct {
-    static constexpr int kRows = 64, kBlocks = 4;
-    static constexpr int kPieces = HD / 128;                      // products of 128 dims
-    static constexpr int kRowGroups = HD >= 256 ? 4 : 1;          // waves that score the same keys
-    static constexpr int kKeyGroups = HD >= 256 ? 2 : 4;
-    static constexpr int kWaves = kRowGroups * kKeyGroups, kThreads = 64 * kWaves;
-    static constexpr int kMine = kBlocks / kRowGroups;            // blocks of rows that a wave scores
-    static constexpr int kKeys = 4 / kKeyGroups;                  // blocks of 16 keys that a wave scores
-    static constexpr int kTasks = kKeys * kPieces / kRowGroups;   // pieces of value rows that a lane decodes
-    static constexpr int kDims = HD / 16 / kWaves;                // blocks of dims that a wave adds up
-    static constexpr int kRun = 64 * wh_kv4_dims<HD>::kLd;        // f16 of a run's decoded rows
-    static constexpr int kPl = 72;                                // f16 between rows of weights
-    static constexpr int kPrun = kRows * kPl;
-    static constexpr size_t kLds = 2 * 2 * (size_t)(kRun + kPrun);
-};
-
-template <int HD, bool kLatent>
-__global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_kv4_attn_direct(wh_kv4_attn_args a) {
-    using D = wh_kv4_dims<HD>;
-    using W = wh_kv4_direct<HD, kLatent>;
-    constexpr int kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kMine = W::kMine, kKeys = W::kKeys,
-                  kPieces = W::kPieces, kTasks = W::kTasks;
-    const wh_kv4_place place = kv_place<W::kRows, 64>(a, false);
-    extern __shared__ __align__(16) uint8_t smem[];
-    _Float16* const vbuf = (_Float16*)smem;     // [2][key][kLd]
-    _Float16* const pbuf = vbuf + 2 * W::kRun;  // [2][row][kPl]
     __shared__ float wave_m[W::kKeyGroups][kRows], wave_l[W::kKeyGroups][kRows], row_m[kRows];
     __shared__ int32_t row_pos[kRows];
-    __shared__ uint32_t wave_top[W::kWaves], raise[2];
-    __shared__ uint64_t nan_keys[2];
+    __shared__ uint32_t wave_top[kWaves], raise[2];
+    __shared__ uint64_t nan_keys[3];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
     const uint32_t kvh = place.head, kq = wave % W::kKeyGroups, rq = wave / W::kKeyGroups;
     const wh_kv4_tile tile = place.tile;
@@ -1393,397 +1106,37 @@ __global__ void __launch_bounds__((wh_kv4_direct<HD, kLatent>::kThreads), 2) k_k
     if (place.split && run0 >= runs) return;
     const bool whole = place.chunk >= runs;
     if (t < 2) raise[t] = 0;
-    if (t < 2) nan_keys[t] = 0;
-    if (t < kRows) row_m[t] = kMinusBig;
-
-    // a run's key rows are requested one run ahead, their pages two
-    const uint32_t* const table = a.tables + tile.request * a.table_stride;
-    const uint32_t pmask = (1u << a.s.shift) - 1u;
-    bool bad = false;
-    uint32_t page[kKeys];
-    uint64_t line[kKeys], vline[kKeys];  // of the requested run, of the run before
-    wh_u4 kc[kKeys][kPieces];
-    wh_kv4_raw<HD, 1> ks[kKeys];  // scale bytes only
-    const uint32_t end = min(tile.n_keys, run1 * 64);
-    // the tile's first key stands in for those past the last
-    auto key_at = [&](uint32_t run, int b) {
-        const uint32_t v = run * 64 + 16 * (kKeys * kq + b) + r16;
-        return wh_kv4_key(tile, v < end ? v : 0);
-    };
-    auto request_pages = [&](uint32_t run) {
-#pragma unroll
-        for (int b = 0; b < kKeys; ++b) page[b] = table[key_at(run, b) >> a.s.shift];
-    };
-    auto request = [&](uint32_t run) {
-#pragma unroll
-        for (int b = 0; b < kKeys; ++b) {
-            const uint32_t key = key_at(run, b);
-            const bool out = page[b] >= a.s.n_pages;
-            bad |= out;
-            line[b] = wh_kv4_line(out ? 0 : page[b], kvh, key & pmask, a.s.kv_heads, a.s.shift);
-            const uint8_t* const c = a.k.codes + line[b] * (HD / 2) + 16 * g;
-#pragma unroll
-            for (int j = 0; j < kPieces; ++j) kc[b][j] = *(const wh_u4*)(c + 64 * j);
-            kv_load_scales(ks[b], 0, a.k, line[b]);
-        }
-        request_pages(run + 1);
-    };
-
-    if (run0 < run1) request_pages(run0);
-    // queries of rows r16 of this wave's blocks
-    wh_i8 q[kMine][kPieces][2];
-    uint32_t q_scale[kMine];
-    float l[kMine];
-#pragma unroll
-    for (int b = 0; b < kMine; ++b) {
-        const uint32_t r = 16 * (rq * kMine + b) + r16, flat = tile.row0 + min(r, tile.rows - 1), tok = flat / a.group;
-        const uint32_t head = kvh * a.group + (flat - tok * a.group);
-        const uint16_t* const p = (const uint16_t*)a.q + (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD + 16 * g;
-        wh_u4 raw[kPieces][2][2];
-#pragma unroll
-        for (int j = 0; j < kPieces; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) raw[j][i >> 1][i & 1] = *(const wh_u4*)(p + 128 * j + 64 * (i >> 1) + 8 * (i & 1));
-        q_scale[b] = 0;
-#pragma unroll
-        for (int j = 0; j < kPieces; ++j)
-            q_scale[b] |= kv_query_e4m3(raw[j], a.scale_log2 < 0.0f ? 0x80008000u : 0u, q[b][j][0], q[b][j][1]) << (8 * j);
-        row_pos[r] = r < tile.rows ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
-        l[b] = 0.0f;
-    }
-    if (run0 < run1) request(run0);
-    const uint32_t row0 = 16 * rq * kMine + r16;  // of block 0
-    // scores are taken times c > 0 (0 would hide what is masked), the sign is the query's
-    const float c = fmaxf(fabsf(a.scale_log2), 1.0e-37f);
-    const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
-    const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
-
-    wh_f4 acc[kDims][kBlocks];  // [dim 16 (kDims wave + f) + 4g + i][row]
-#pragma unroll
-    for (int f = 0; f < kDims; ++f)
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) acc[f][b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
-    int ref = 0;
-
-    // outputs of the run in buffer `at`
-    auto values = [&](uint32_t at) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            wh_h8 x[kDims];
-            const _Float16* const vb = vbuf + at * W::kRun + (32 * h + 4 * g + (r16 >> 2)) * D::kLd + 16 * kDims * wave +
-                                       4 * (r16 & 3);
-#pragma unroll
-            for (int f = 0; f < kDims; ++f) {
-                union {
-                    wh_s4 s[2];
-                    wh_h8 v;
-                } u;
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    u.s[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) wh_s4*)(vb + 16 * k * D::kLd + 16 * f));
-                x[f] = u.v;
-            }
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                const wh_h8 w = *(const wh_h8*)(pbuf + at * W::kPrun + (16 * b + r16) * W::kPl + 32 * h + 8 * g);
-#pragma unroll
-                for (int f = 0; f < kDims; ++f) acc[f][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[f], w, acc[f][b], 0, 0, 0);
-            }
-        }
-    };
-
-    wh_u4 vc[kTasks];
-    uint32_t vb[kTasks];  // scale bytes
-    auto pass = [&](uint32_t run, auto first) {
-        const uint32_t at = run & 1;
-        // this run's value rows: for latent rows the lines that the keys came from
-#pragma unroll
-        for (int i = 0; i < kTasks; ++i) {
-            const int n0 = W::kRowGroups * i;  // task n = rq + n0: block n % kKeys, piece n / kKeys
-            const uint32_t n = rq + n0, j = n / kKeys;
-            const uint64_t ln = kKeys == 2 ? (n & 1 ? line[kKeys - 1] : line[0]) : line[0];
-            vc[i] = *(const wh_u4*)(a.v.codes + ln * (HD / 2) + 64 * j + 16 * g);
-            vb[i] = a.v.scales[ln * (HD / 32) + 4 * j + g];
-        }
-        wh_f4 s[kMine][kKeys];
-        uint32_t scale[kKeys];
-#pragma unroll
-        for (int kb = 0; kb < kKeys; ++kb) {
-            scale[kb] = kv_piece_scales(ks[kb], 0, g);
-#pragma unroll
-            for (int b = 0; b < kMine; ++b) s[b][kb] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        wh_static_for<kPieces>([&](auto jc) {
-            constexpr int j = decltype(jc)::value;
-#pragma unroll
-            for (int p = 1; p >= 0; --p)
-#pragma unroll
-                for (int kb = 0; kb < kKeys; ++kb) {
-                    wh_i8 x;
-                    x[0] = kc[kb][j][0], x[1] = kc[kb][j][1], x[2] = kc[kb][j][2], x[3] = kc[kb][j][3];
-                    x[4] = x[5] = x[6] = x[7] = 0;
-#pragma unroll
-                    for (int b = 0; b < kMine; ++b)
-                        s[b][kb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                            x, q[b][j][p], s[b][kb], 4, 0, j, scale[kb], j, q_scale[b] - (p ? 0x04040404u : 0u));
-                }
-        });
-        // the next run's rows come into the registers of these: not before they are used
-#pragma unroll
-        for (int b = 0; b < kMine; ++b)
-#pragma unroll
-            for (int kb = 0; kb < kKeys; ++kb) asm volatile("" : "+v"(s[b][kb])::"memory");
-        request(run + 1);
-        // -inf where a row does not see this lane's keys
-        const uint32_t v0 = run * 64 + 16 * kKeys * kq + 4 * g, last = run * 64 + 63;
-        const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == kRows &&
-                         (!a.window || (int64_t)wh_kv4_key(tile, max(run * 64, tile.n_first)) + a.window > pos_hi);
-        if (!all) {
-#pragma unroll
-            for (int kb = 0; kb < kKeys; ++kb)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t v = v0 + 16 * kb + i, key = wh_kv4_key(tile, v);
-#pragma unroll
-                    for (int b = 0; b < kMine; ++b) {
-                        const bool see = (v < tile.n_keys) & wh_kv4_sees(row_pos[row0 + 16 * b], key, a.window, a.first);
-                        s[b][kb][i] = see ? s[b][kb][i] : kMinusInf;
-                    }
-                }
-        }
-        if constexpr (!decltype(first)::value) values(at ^ 1);
-        float top[kMine], add[kMine];
-        bool over = false;
-#pragma unroll
-        for (int b = 0; b < kMine; ++b) {
-            top[b] = s[b][0][0];
-#pragma unroll
-            for (int kb = 0; kb < kKeys; ++kb)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top[b] = fmaxf(top[b], s[b][kb][i]);
-            over |= top[b] * c > row_m[row0 + 16 * b] + kSlack;
-        }
-        uint32_t vtop = 0;  // largest byte that counts
-        auto decode = [&] {
-#pragma unroll
-            for (int i = 0; i < kTasks; ++i) {
-                const uint32_t n = rq + W::kRowGroups * i, kb = n % kKeys, j = n / kKeys;
-                const float rel = kv_bits((uint32_t)min(max((int)vb[i] - ref + 127, 0), 127) << 23);
-                _Float16* const dst = vbuf + at * W::kRun + (16 * (kKeys * kq + kb) + r16) * D::kLd + 128 * j + 32 * g;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) *(wh_h8*)(dst + 8 * w) = kv_decode(vc[i][w], rel);
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < kTasks; ++i) {
-            const uint32_t n = rq + W::kRowGroups * i, kb = n % kKeys;
-            const bool counts = run * 64 + 16 * (kKeys * kq + kb) + r16 < tile.n_keys;
-            vtop = max(vtop, counts && vb[i] < 255 ? vb[i] : 0u);
-            over |= !kLatent && counts && vb[i] == 255;
-        }
-        over |= (int)vtop > ref;
-        decode();
-        auto weights = [&](auto max_of) {
-            _Float16* const pw = pbuf + at * W::kPrun + row0 * W::kPl + (kKeys == 2 ? 32 * kq : 32 * (kq >> 1) + 4 * (kq & 1)) + 8 * g;
-#pragma unroll
-            for (int b = 0; b < kMine; ++b) {
-                const float up = kUp - max_of(b);
-                union {
-                    _Float16 h[4 * kKeys];
-                    uint32_t u[2 * kKeys];
-                } x;
-                add[b] = 0.0f;
-#pragma unroll
-                for (int kb = 0; kb < kKeys; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float w = __builtin_amdgcn_exp2f(fmaf(s[b][kb][i], c, up));
-                        add[b] += w;
-                        x.h[4 * kb + i] = (_Float16)w;
-                    }
-                if constexpr (kKeys == 2) *(wh_u4*)(pw + 16 * b * W::kPl) = (wh_u4){x.u[0], x.u[1], x.u[2], x.u[3]};
-                else *(wh_u2*)(pw + 16 * b * W::kPl) = (wh_u2){x.u[0], x.u[1]};
-            }
-        };
-        weights([&](int b) { return row_m[row0 + 16 * b]; });
-        if (__ballot(over) && lane == 0) raise[at] = run + 1;
-        kv_lds_barrier();
-        if (__builtin_expect(__builtin_amdgcn_readfirstlane(raise[at]) == run + 1, 0)) {  // the whole workgroup
-            if constexpr (!kLatent) {  // keys whose value row holds NaN
-#pragma unroll
-                for (int i = 0; i < kTasks; ++i) {
-                    const uint32_t n = rq + W::kRowGroups * i, key = 16 * (kKeys * kq + n % kKeys) + r16;
-                    if (vb[i] == 255 && run * 64 + key < tile.n_keys) atomicOr((unsigned long long*)&nan_keys[at], 1ull << key);
-                }
-            }
-            for (int off = 32; off >= 1; off >>= 1) vtop = max(vtop, (uint32_t)__shfl_xor((int)vtop, off, 64));
-#pragma unroll
-            for (int b = 0; b < kMine; ++b) {
-                top[b] = fmaxf(top[b], __shfl_xor(top[b], 16, 64));
-                top[b] = fmaxf(top[b], __shfl_xor(top[b], 32, 64));
-                if (g == 0) wave_m[kq][row0 + 16 * b] = top[b] * c;
-            }
-            if (lane == 0) wave_top[wave] = vtop;
-            kv_lds_barrier();
-#pragma unroll
-            for (int w = 0; w < W::kWaves; ++w) vtop = max(vtop, wave_top[w]);
-            const int to = (int)vtop > ref ? min((int)vtop + 3, 254) : ref;
-            const float f_ref = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
-            ref = to;
-            auto raised = [&](uint32_t row) {
-                float mm = row_m[row];
-#pragma unroll
-                for (int w = 0; w < W::kKeyGroups; ++w) mm = fmaxf(mm, wave_m[w][row]);
-                return mm;
-            };
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                const float f = __builtin_amdgcn_exp2f(row_m[16 * b + r16] - raised(16 * b + r16)) * f_ref;
-#pragma unroll
-                for (int k = 0; k < kDims; ++k) acc[k][b] *= f;
-            }
-            float m[kMine];
-#pragma unroll
-            for (int b = 0; b < kMine; ++b) {
-                m[b] = raised(row0 + 16 * b);
-                l[b] *= __builtin_amdgcn_exp2f(row_m[row0 + 16 * b] - m[b]);
-            }
-            if constexpr (!kLatent) {
-                const uint64_t nan = nan_keys[at];
-#pragma unroll
-                for (int kb = 0; kb < kKeys; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (nan >> (16 * (kKeys * kq + kb) + 4 * g + i) & 1)
-#pragma unroll
-                            for (int b = 0; b < kMine; ++b)
-                                if (s[b][kb][i] != kMinusInf) s[b][kb][i] = kv_bits(0x7fc00000u);
-            }
-            decode();
-            weights([&](int b) { return m[b]; });
-            kv_lds_barrier();
-#pragma unroll
-            for (int b = 0; b < kMine; ++b)
-                if (kq == 0 && g == 0) row_m[row0 + 16 * b] = m[b];
-            if (t == 0) nan_keys[at] = 0;
-            kv_lds_barrier();
-        }
-#pragma unroll
-        for (int b = 0; b < kMine; ++b) l[b] += add[b];
-    };
-
-    kv_lds_barrier();
-    if (run0 < run1) pass(run0, std::true_type());
-    for (uint32_t run = run0 + 1; run < run1; ++run) pass(run, std::false_type());
-    if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
-    if (run0 < run1) values((run1 - 1) & 1);
-
-#pragma unroll
-    for (int b = 0; b < kMine; ++b) {
-        l[b] += __shfl_xor(l[b], 16, 64);
-        l[b] += __shfl_xor(l[b], 32, 64);
-        if (g == 0) wave_l[kq][row0 + 16 * b] = l[b];
-    }
-    kv_lds_barrier();
-    const float up = kv_bits((uint32_t)ref << 23);
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-        const uint32_t r = 16 * b + r16;
-        if (r >= tile.rows) continue;
-        const uint32_t flat = tile.row0 + r, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
-        float L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W::kKeyGroups; ++w) L += wave_l[w][r];
-        const float M = row_m[r];
-        float denom = L;
-        if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
-        const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
-        float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * kRows + r) * (HD + 2);
-        const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
-#pragma unroll
-        for (int f = 0; f < kDims; ++f) {
-            const uint32_t d = 16 * (kDims * wave + f) + 4 * g;
-            const wh_f4 y = acc[f][b] * up * inv;
-            if (!whole) {
-                *(wh_f2*)(part + d) = (wh_f2){y[0], y[1]};
-                *(wh_f2*)(part + d + 2) = (wh_f2){y[2], y[3]};
-            } else {
-                kv_store<false>(a.out, at + d, y);
-            }
-        }
-        if (!whole && wave == 0 && g == 0) {
-            part[HD] = M;
-            part[HD + 1] = L;
-        }
-    }
-}
-
-// The same for rows of 256 and 512 dims, where the value rows as f16 and the
-// requests of every wave for its own keys were too much: 153 KB of LDS, a third
-// of the time in the address unit (the four waves that score the same keys each
-// read them from memory) and registers for rows in flight.  Here the eight waves
-// bring a run's codes into LDS once, as they lie; the scores read them as
-// operands, and the values are read transposed, sixteen keys of one dim a lane
-// (the 4-bit transposing read), decoded to small f16 numbers and multiplied by
-// their keys' powers of two, which lie beside them relative to `ref`.
-template <int HD, bool kLatent>
-struct wh_kv4_packed {
-    static constexpr int kRows = 64, kBlocks = 4, kWaves = 8, kThreads = 512;
-    static constexpr int kPieces = HD / 128, kDims = HD / 128, kGroups = HD / 32;
-    static constexpr int kMine = HD / 256;            // 16-byte chunks, each a group of 32 dims, that a lane brings
-    static constexpr int kRow = HD / 2;               // bytes of a row's codes
-    static constexpr int kCodes = 64 * kRow;          // bytes of a run's codes
-    static constexpr int kKeyBufs = kLatent ? 3 : 2;  // latent codes are values one run later
-    static constexpr int kRel = 72;                   // f16 between groups of value scales
-    static constexpr int kPl = 72;                    // f16 between rows of weights
-    static constexpr int kAtValues = kKeyBufs * kCodes;                      // byte offsets in LDS
-    static constexpr int kAtScales = kAtValues + (kLatent ? 0 : 3 * kCodes);  // [2][g][key] dwords
-    static constexpr int kAtRel = kAtScales + 2 * 4 * 64 * 4;                // [3][group][key] f16
-    static constexpr int kAtWeights = kAtRel + 3 * kGroups * kRel * 2;       // [2][row][key] f16
-    static constexpr size_t kLds = kAtWeights + 2 * (size_t)kRows * kPl * 2;
-};
-
-template <int HD, bool kLatent>
-__global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) {
-    using W = wh_kv4_packed<HD, kLatent>;
-    constexpr int kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kPieces = W::kPieces;
-    const wh_kv4_place place = kv_place<W::kRows, 64>(a, false);
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float wave_m[2][kRows], wave_l[2][kRows], row_m[kRows];
-    __shared__ int32_t row_pos[kRows];
-    __shared__ uint32_t wave_top[8], raise[2];
-    __shared__ uint64_t nan_keys[3];
-    const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
-    const uint32_t kvh = place.head, kq = wave & 1, rq = wave >> 1;
-    const wh_kv4_tile tile = place.tile;
-    if (!tile.ok) return;
-    const uint32_t runs = (tile.n_keys + 63) / 64;
-    const uint32_t run0 = place.split ? place.split * place.chunk : 0, run1 = min(runs, run0 + place.chunk);
-    if (place.split && run0 >= runs) return;
-    const bool whole = place.chunk >= runs;
-    if (t < 2) raise[t] = 0;
     if (t < 3) nan_keys[t] = 0;
     if (t < kRows) row_m[t] = kMinusBig;
+    // what the first run finds in place of an earlier one's: no weights, and finite value scales
+    for (uint32_t i = 16 * t; i < W::kLds - W::kAtRel; i += 16 * W::kThreads) *(wh_u4*)(smem + W::kAtRel + i) = (wh_u4){0, 0, 0, 0};
 
     // 16-byte chunk c of a row lies at chunk c ^ swizzle(row): 16 rows of one chunk are on all banks
-    auto swizzle = [](uint32_t key) { return HD == 512 ? key & 15 : (key >> 1) & 7; };
+    auto swizzle = [](uint32_t key) {
+        return HD == 512 ? key & 15 : HD == 256 ? (key >> 1) & 7 : HD == 128 ? (key >> 2) & 3 : (key >> 3) & 1;
+    };
 
-    // this lane's key of a run, and its chunks
+    // this lane's key of a run, and its chunks: of the key and the value row, or
+    // (short rows apart) of keys in the first waves, of values in the next
+    const bool brings = wave < W::kBring * (W::kBoth ? 1u : 2u);
+    const bool has_values = W::kBoth ? brings : brings && wave >= W::kBring, has_keys = W::kBoth ? brings : wave < W::kBring;
     const uint32_t* const table = a.tables + tile.request * a.table_stride;
     const uint32_t pmask = (1u << a.s.shift) - 1u, end = min(tile.n_keys, run1 * 64);
-    const uint32_t my_key = 8 * wave + (lane >> 3), my_chunk = W::kMine * (lane & 7);
+    const uint32_t my_key = 64 / W::kLanes * (wave % W::kBring) + lane / W::kLanes, my_chunk = W::kMine * (lane % W::kLanes);
     bool bad = false;
     uint32_t page = 0;
-    wh_u4 kc[W::kMine], vc[W::kMine];
+    constexpr bool kTwo = W::kBoth && !kLatent;  // chunks of values are held beside those of keys
+    wh_u4 kc[W::kMine], vc[kTwo ? W::kMine : 1];
     uint32_t kb = 0, vb = 0;  // their scale bytes
     // the tile's first key stands in for those past the last
     auto key_at = [&](uint32_t run) {
         const uint32_t v = run * 64 + my_key;
         return wh_kv4_key(tile, v < end ? v : 0);
     };
-    auto request_page = [&](uint32_t run) { page = table[key_at(run) >> a.s.shift]; };
-    auto request_of = [&](const wh_kv4_plane& p, uint64_t line, wh_u4 (&c)[W::kMine], uint32_t& b) {
+    auto request_page = [&](uint32_t run) {
+        if (W::kBring == kWaves || brings) page = table[key_at(run) >> a.s.shift];
+    };
+    auto request_of = [&](const wh_kv4_plane& p, uint64_t line, wh_u4* c, uint32_t& b) {
         const uint8_t* const src = p.codes + line * (HD / 2) + 16 * my_chunk;
 #pragma unroll
         for (int i = 0; i < W::kMine; ++i) c[i] = *(const wh_u4*)(src + 16 * i);
@@ -1791,16 +1144,17 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
         b = W::kMine == 2 ? *(const uint16_t*)sc : *sc;
     };
     auto request = [&](uint32_t run) {
+        if (W::kBring < kWaves && !brings) return;
         const uint32_t key = key_at(run);
         const bool out = page >= a.s.n_pages;
         bad |= out;
         const uint64_t line = wh_kv4_line(out ? 0 : page, kvh, key & pmask, a.s.kv_heads, a.s.shift);
-        request_of(a.k, line, kc, kb);
-        if constexpr (!kLatent) request_of(a.v, line, vc, vb);
+        request_of(W::kBoth || has_keys ? a.k : a.v, line, kc, kb);
+        if constexpr (kTwo) request_of(a.v, line, vc, vb);
         request_page(run + 1);
     };
     int ref = 0;
-    auto value_bytes = [&] { return kLatent ? kb : vb; };
+    auto value_bytes = [&] { return kTwo ? vb : kb; };
     auto counts = [&](uint32_t run) { return run * 64 + my_key < end; };
     // largest value scale byte of this lane's chunks that counts
     auto top_byte = [&](uint32_t run) {
@@ -1810,65 +1164,95 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
             const uint32_t b = (value_bytes() >> (8 * i)) & 0xff;
             m = max(m, b < 255 ? b : 0u);
         }
-        return counts(run) ? m : 0u;
+        return has_values && counts(run) ? m : 0u;
     };
-    auto stage_rel = [&](uint32_t run) {
+    // a row's largest byte, from its lanes
+    auto row_top = [&](uint32_t b) { return kv_near_max<W::kLanes>(W::kMine == 2 ? max(b & 0xff, b >> 8) : b); };
+    auto stage_rel = [&](uint32_t run, uint32_t against) {
         _Float16* const rel = (_Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel);
 #pragma unroll
         for (int i = 0; i < W::kMine; ++i) {
-            const int e = (int)((value_bytes() >> (8 * i)) & 0xff) - ref;  // above ref only where it does not count
+            const int e = (int)((value_bytes() >> (8 * i)) & 0xff) - (int)against;  // above only where it does not count
             rel[(my_chunk + i) * W::kRel + my_key] = (_Float16)kv_bits((uint32_t)max(min(e, 0) + 127, 0) << 23);
         }
     };
     auto stage = [&](uint32_t run) {
-        uint8_t* const kd = smem + run % W::kKeyBufs * W::kCodes + my_key * W::kRow;
+        if (W::kBring < kWaves && !brings) return;
+        uint32_t top = 0;
+        if constexpr (kF32) top = row_top(kb);
+        if (W::kBoth || has_keys) {
+            uint8_t* const kd = smem + run % W::kKeyBufs * W::kCodes + my_key * W::kRow;
 #pragma unroll
-        for (int i = 0; i < W::kMine; ++i) *(wh_u4*)(kd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = kc[i];
-        uint8_t* const sc = smem + W::kAtScales + (run & 1) * 1024;
+            for (int i = 0; i < W::kMine; ++i) *(wh_u4*)(kd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = kc[i];
+            uint8_t* const sc = smem + W::kAtScales + (run & 1) * 1024;
 #pragma unroll
-        for (int i = 0; i < W::kMine; ++i) {
-            const uint32_t n = my_chunk + i;
-            sc[((n & 3) * 64 + my_key) * 4 + (n >> 2)] = (uint8_t)(kb >> (8 * i));
+            for (int i = 0; i < W::kMine; ++i) {
+                const uint32_t n = my_chunk + i, b = (kb >> (8 * i)) & 0xff;
+                // f32: against the row's largest, so that decoded values are finite f16 whatever the bytes are
+                sc[((n & 3) * 64 + my_key) * 4 + (n >> 2)] = (uint8_t)(kF32 ? (uint32_t)max((int)b - (int)top + 127, 0) : b);
+            }
+            if constexpr (kF32)
+                if (my_chunk == 0) ((float*)(smem + W::kAtKeys))[(run & 1) * 64 + my_key] = kv_key_scale(top, 0);
         }
-        if constexpr (!kLatent) {
+        if constexpr (kLatent) {
+            if constexpr (kF32)
+                if (my_chunk == 0) ((int*)(smem + W::kAtTops))[(run & 1) * 64 + my_key] = (int)top;
+            stage_rel(run, kF32 ? top : (uint32_t)ref);
+        } else if (W::kBoth || has_values) {
+            if constexpr (kF32 && kTwo) top = row_top(vb);
             uint8_t* const vd = smem + W::kAtValues + run % 3 * W::kCodes + my_key * W::kRow;
-#pragma unroll
-            for (int i = 0; i < W::kMine; ++i) *(wh_u4*)(vd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = vc[i];
+            const uint32_t bytes = value_bytes();
             bool nan = false;
 #pragma unroll
-            for (int i = 0; i < W::kMine; ++i) nan |= ((vb >> (8 * i)) & 0xff) == 255;
+            for (int i = 0; i < W::kMine; ++i) {
+                *(wh_u4*)(vd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = kTwo ? vc[kTwo ? i : 0] : kc[i];
+                nan |= ((bytes >> (8 * i)) & 0xff) == 255;
+            }
             if (nan && counts(run)) atomicOr((unsigned long long*)&nan_keys[run % 3], 1ull << my_key);
+            if constexpr (kF32)
+                if (my_chunk == 0) ((int*)(smem + W::kAtTops))[(run & 1) * 64 + my_key] = (int)top;
+            stage_rel(run, kF32 ? top : (uint32_t)ref);
         }
-        stage_rel(run);
     };
 
     if (run0 < run1) request_page(run0);
     // the query of row r16 of block rq
-    wh_i8 q[kPieces][2];
+    wh_i8 qx[kF32 ? 1 : kPieces][2];
+    wh_h8 qd[kF32 ? HD / 32 : 1][kParts];
     uint32_t q_scale = 0;
+    float c;  // scores are sums times this
     float l = 0.0f;
     const uint32_t row0 = 16 * rq + r16;
     {
         const uint32_t flat = tile.row0 + min(row0, tile.rows - 1), tok = flat / a.group;
         const uint32_t head = kvh * a.group + (flat - tok * a.group);
-        const uint16_t* const p = (const uint16_t*)a.q + (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD + 16 * g;
-        wh_u4 raw[kPieces][2][2];
+        const uint64_t at = (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD;
+        if constexpr (kF32) {
+            wh_kv4_query<HD, true> query;
+            query.load(a.q, at, g);
+            if (run0 < run1) request(run0);
+            c = a.scale_log2 * query.parts(qd);
+        } else {
+            const uint16_t* const p = (const uint16_t*)a.q + at + 16 * g;
+            wh_u4 raw[kPieces][2][2];
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j)
+            for (int j = 0; j < kPieces; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) raw[j][i >> 1][i & 1] = *(const wh_u4*)(p + 128 * j + 64 * (i >> 1) + 8 * (i & 1));
-        if (run0 < run1) request(run0);
+                for (int i = 0; i < 4; ++i)
+                    raw[j][i >> 1][i & 1] = HD == 64 && i >= 2 ? (wh_u4){0, 0, 0, 0} : *(const wh_u4*)(p + 128 * j + 64 * (i >> 1) + 8 * (i & 1));
+            if (run0 < run1) request(run0);
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j)
-            q_scale |= kv_query_e4m3(raw[j], a.scale_log2 < 0.0f ? 0x80008000u : 0u, q[j][0], q[j][1]) << (8 * j);
+            for (int j = 0; j < kPieces; ++j)
+                q_scale |= kv_query_e4m3(raw[j], a.scale_log2 < 0.0f ? 0x80008000u : 0u, qx[j][0], qx[j][1]) << (8 * j);
+            c = fmaxf(fabsf(a.scale_log2), 1.0e-37f);  // above 0, which would hide what is masked; the sign is the query's
+        }
         row_pos[row0] = row0 < tile.rows ? tile.len - (int32_t)tile.n_q + (int32_t)tok : -1;
     }
-    // scores are taken times c > 0 (0 would hide what is masked), the sign is the query's
-    const float c = fmaxf(fabsf(a.scale_log2), 1.0e-37f);
     const int32_t pos_lo = tile.len - (int32_t)tile.n_q + (int32_t)(tile.row0 / a.group);
     const int32_t pos_hi = tile.len - (int32_t)tile.n_q + (int32_t)((tile.row0 + tile.rows - 1) / a.group);
 
-    wh_f4 acc[kDims][kBlocks];  // [dim 16 (kDims wave + f) + 4g + i][row]
+    const uint32_t dim0 = kDims * wave;
+    wh_f4 acc[kDims][kBlocks];  // [dim 16 (dim0 + f) + 4g + i][row 16 b + r16]
 #pragma unroll
     for (int f = 0; f < kDims; ++f)
 #pragma unroll
@@ -1880,24 +1264,27 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
         if (lane == 0) wave_top[wave] = top;
         kv_lds_barrier();
 #pragma unroll
-        for (int w = 0; w < 8; ++w) top = max(top, wave_top[w]);
+        for (int i = 0; i < kWaves; ++i) top = max(top, wave_top[i]);
         ref = min((int)top + 3, 254);
         stage(run0);
     }
     kv_lds_barrier();
 
-    // outputs of run x: 16 dims a step, all rows and keys
-    wh_h8 w[2][kBlocks];
+    // outputs of the run whose weights lie at `run` modulo 2, its values and their scales modulo 3: 16 dims a step
+    wh_h8 w[2][kBlocks][kParts];
     auto read_weights = [&](uint32_t run) {
-        const _Float16* const pb = (const _Float16*)(smem + W::kAtWeights) + (run & 1) * (kRows * W::kPl) + r16 * W::kPl + 16 * g;
+        const _Float16* const pb =
+            (const _Float16*)(smem + W::kAtWeights) + (run & 1) * (kParts * kRows * W::kPl) + r16 * W::kPl + 16 * g;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) w[h][b] = *(const wh_h8*)(pb + 16 * b * W::kPl + 8 * h);
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) w[h][b][p] = *(const wh_h8*)(pb + p * (kRows * W::kPl) + 16 * b * W::kPl + 8 * h);
     };
     wh_h8 rel[2];
     auto values_step = [&](uint32_t run, int f) {
-        const uint32_t block = kDims * wave + f, key = 16 * g + r16;  // of the transposed read
+        const uint32_t block = dim0 + f, key = 16 * g + r16;  // of the transposed read
         if (f % 2 == 0) {
             const _Float16* const rp =
                 (const _Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel) + (block >> 1) * W::kRel + 16 * g;
@@ -1911,52 +1298,85 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
         for (int h = 0; h < 2; ++h) {
             const wh_h8 x = kv_decode((uint32_t)codes[h], 1.0f) * rel[h];
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) acc[f][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[h][b], acc[f][b], 0, 0, 0);
+            for (int p = kParts - 1; p >= 0; --p)
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) acc[f][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[h][b][p], acc[f][b], 0, 0, 0);
         }
     };
 
-    auto pass = [&](uint32_t run, auto first) {
-        constexpr bool kFirst = decltype(first)::value;
+    for (uint32_t run = run0; run < run1; ++run) {
         const uint32_t at = run & 1;
         request(run + 1);
-        if constexpr (!kFirst) read_weights(run - 1);
+        read_weights(run + 1);
         if constexpr (!kLatent)
             if (t == 0) nan_keys[(run + 2) % 3] = 0;
-        // scores of 32 keys
-        wh_f4 s[2];
-        uint32_t scale[2];
-        const uint8_t* krow[2];
+        // scores
+        wh_f4 s[kKeyBlocks];
+        uint32_t scale[kKeyBlocks];
+        const uint8_t* krow[kKeyBlocks];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t key = 32 * kq + 16 * i + r16;
+        for (int i = 0; i < kKeyBlocks; ++i) {
+            const uint32_t key = 16 * (kKeyBlocks * kq + i) + r16;
             krow[i] = smem + run % W::kKeyBufs * W::kCodes + key * W::kRow;
-            scale[i] = *(const uint32_t*)(smem + W::kAtScales + at * 1024 + (g * 64 + key) * 4);
+            scale[i] = *(const uint32_t*)(smem + W::kAtScales + at * 1024 + ((HD == 64 ? kF32 ? g >> 1 : g & 1 : g) * 64 + key) * 4);
             s[i] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
         }
-        wh_static_for<kPieces>([&](auto jc) {
-            constexpr int j = decltype(jc)::value;
-            wh_i8 x[2];
+        if constexpr (kF32) {
+            // keys decoded against their row's power of two
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const wh_u4 v = *(const wh_u4*)(krow[i] + 16 * ((4 * j + g) ^ swizzle(32 * kq + 16 * i + r16)));
-                x[i][0] = v[0], x[i][1] = v[1], x[i][2] = v[2], x[i][3] = v[3];
-                x[i][4] = x[i][5] = x[i][6] = x[i][7] = 0;
-            }
+            for (int j = 0; j < kPieces; ++j)
 #pragma unroll
-            for (int p = 1; p >= 0; --p)
+                for (int i = 0; i < kKeyBlocks; ++i) {
+                    const uint32_t key = 16 * (kKeyBlocks * kq + i) + r16;
+                    const float against = kv_bits((scale[i] >> (8 * j) & 0xff) << 23);
+                    uint32_t v[4];
+                    if constexpr (HD == 64) {
+                        const wh_u2 u = *(const wh_u2*)(krow[i] + 16 * ((g >> 1) ^ swizzle(key)) + 8 * (g & 1));
+                        v[0] = u[0], v[1] = u[1];
+                    } else {
+                        const wh_u4 u = *(const wh_u4*)(krow[i] + 16 * ((4 * j + g) ^ swizzle(key)));
+                        v[0] = u[0], v[1] = u[1], v[2] = u[2], v[3] = u[3];
+                    }
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    s[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[i], q[j][p], s[i], 4, 0, j, scale[i], j,
-                                                                            q_scale - (p ? 0x04040404u : 0u));
-        });
+                    for (int k = 0; k < (HD == 64 ? 2 : 4); ++k) {
+                        const wh_h8 x = kv_decode(v[k], against);
+#pragma unroll
+                        for (int p = kParts - 1; p >= 0; --p)
+                            s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qd[4 * j + k][p], s[i], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < kKeyBlocks; ++i)
+                s[i] = s[i] * c * *(const wh_f4*)(smem + W::kAtKeys + (at * 64 + 16 * (kKeyBlocks * kq + i) + 4 * g) * 4);
+        } else {
+            // codes as they lie, which takes scales by 32 dims
+            wh_static_for<kPieces>([&](auto jc) {
+                constexpr int j = decltype(jc)::value;
+                wh_i8 x[kKeyBlocks];
+#pragma unroll
+                for (int i = 0; i < kKeyBlocks; ++i) {
+                    const uint32_t key = 16 * (kKeyBlocks * kq + i) + r16;
+                    const wh_u4 v = *(const wh_u4*)(krow[i] + 16 * ((HD == 64 ? g & 1 : 4 * j + g) ^ swizzle(key)));
+                    // 64 dims: the other 64 of the product are zeros of the query
+                    x[i][0] = v[0], x[i][1] = v[1], x[i][2] = v[2], x[i][3] = v[3];
+                    x[i][4] = x[i][5] = x[i][6] = x[i][7] = 0;
+                }
+#pragma unroll
+                for (int p = 1; p >= 0; --p)
+#pragma unroll
+                    for (int i = 0; i < kKeyBlocks; ++i)
+                        s[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[i], qx[j][p], s[i], 4, 0, j, scale[i], j,
+                                                                                q_scale - (p ? 0x04040404u : 0u));
+            });
+        }
         // -inf where a row does not see this lane's keys
-        const uint32_t v0 = run * 64 + 32 * kq + 4 * g, last = run * 64 + 63;
+        const uint32_t v0 = run * 64 + 16 * kKeyBlocks * kq + 4 * g, last = run * 64 + 63;
         const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == kRows &&
                          (!a.window || (int64_t)wh_kv4_key(tile, max(run * 64, tile.n_first)) + a.window > pos_hi);
         if (!all) {
             const int32_t pos = row_pos[row0];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4 * kKeyBlocks; ++i) {
                 const uint32_t v = v0 + 16 * (i >> 2) + (i & 3), key = wh_kv4_key(tile, v);
                 const bool see = (v < tile.n_keys) & wh_kv4_sees(pos, key, a.window, a.first);
                 s[i >> 2][i & 3] = see ? s[i >> 2][i & 3] : kMinusInf;
@@ -1966,70 +1386,89 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
             const uint64_t nan = nan_keys[run % 3];
             if (__builtin_expect(nan != 0, 0)) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if ((nan >> (32 * kq + 16 * (i >> 2) + 4 * g + (i & 3)) & 1) && s[i >> 2][i & 3] != kMinusInf)
+                for (int i = 0; i < 4 * kKeyBlocks; ++i)
+                    if ((nan >> (16 * (kKeyBlocks * kq + (i >> 2)) + 4 * g + (i & 3)) & 1) && s[i >> 2][i & 3] != kMinusInf)
                         s[i >> 2][i & 3] = kv_bits(0x7fc00000u);
             }
         }
-        if constexpr (!kFirst) {
 #pragma unroll
-            for (int f = 0; f < kDims; ++f) values_step(run - 1, f);
-        }
+        for (int f = 0; f < kDims; ++f) values_step(run + 2, f);
         const float m0 = row_m[row0];
-        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        float top = kMinusInf;
+#pragma unroll
+        for (int i = 0; i < kKeyBlocks; ++i) top = fmaxf(top, fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
+        if constexpr (!kF32) top *= c;
         float add;
         auto weights = [&](float m) {
             const float up = kUp - m;
-            float e[8];
-            wh_h8 x;
+            add = 0.0f;
+            _Float16* const pw =
+                (_Float16*)(smem + W::kAtWeights) + at * (kParts * kRows * W::kPl) + row0 * W::kPl + 16 * kKeyBlocks * kq + 4 * g;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], c, up));
-                x[i] = (_Float16)e[i];
+            for (int i = 0; i < kKeyBlocks; ++i) {
+                float e[4];
+                union {
+                    _Float16 h[4];
+                    wh_u2 u;
+                } hi, lo;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(kF32 ? s[i][k] + up : fmaf(s[i][k], c, up));
+                add += (e[0] + e[1]) + (e[2] + e[3]);
+                if constexpr (kF32) {
+                    const wh_i4 tops = *(const wh_i4*)(smem + W::kAtTops + (at * 64 + 16 * (kKeyBlocks * kq + i) + 4 * g) * 4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_ldexpf(e[k], tops[k] - ref);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    hi.h[k] = (_Float16)e[k];
+                    if constexpr (kF32) lo.h[k] = (_Float16)(e[k] - (float)hi.h[k]);
+                }
+                *(wh_u2*)(pw + 16 * i) = hi.u;
+                if constexpr (kF32) *(wh_u2*)(pw + kRows * W::kPl + 16 * i) = lo.u;
             }
-            add = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-            union {
-                wh_h8 h;
-                wh_u4 u;
-            } y;
-            y.h = x;
-            _Float16* const pw = (_Float16*)(smem + W::kAtWeights) + at * (kRows * W::kPl) + row0 * W::kPl + 32 * kq + 4 * g;
-            *(wh_u2*)pw = (wh_u2){y.u[0], y.u[1]};
-            *(wh_u2*)(pw + 16) = (wh_u2){y.u[2], y.u[3]};
         };
         weights(m0);
         uint32_t vtop = top_byte(run + 1);
-        const bool over = top * c > m0 + kSlack || (int)vtop > ref;
+        const bool over = top > m0 + kSlack || (int)vtop > ref;
         stage(run + 1);
         if (__ballot(over) && lane == 0) raise[at] = run + 1;
         kv_lds_barrier();
         if (__builtin_expect(__builtin_amdgcn_readfirstlane(raise[at]) == run + 1, 0)) {  // the whole workgroup
             for (int off = 32; off >= 1; off >>= 1) vtop = max(vtop, (uint32_t)__shfl_xor((int)vtop, off, 64));
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (g == 0) wave_m[kq][row0] = top * c;
+            top = kv_max_groups(top);
+            if (g == 0) wave_m[kq][row0] = top;
             if (lane == 0) wave_top[wave] = vtop;
             kv_lds_barrier();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) vtop = max(vtop, wave_top[i]);
+            for (int i = 0; i < kWaves; ++i) vtop = max(vtop, wave_top[i]);
             const int to = (int)vtop > ref ? min((int)vtop + 3, 254) : ref;
             const float f_ref = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
-            auto raised = [&](uint32_t row) { return fmaxf(row_m[row], fmaxf(wave_m[0][row], wave_m[1][row])); };
+            auto raised = [&](uint32_t row) {
+                float m = row_m[row];
+#pragma unroll
+                for (int i = 0; i < W::kKeyGroups; ++i) m = fmaxf(m, wave_m[i][row]);
+                return m;
+            };
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
-                const float f = __builtin_amdgcn_exp2f(row_m[16 * b + r16] - raised(16 * b + r16)) * f_ref;
+                const uint32_t row = 16 * b + r16;
+                const float f = __builtin_amdgcn_exp2f(row_m[row] - raised(row)) * f_ref;
 #pragma unroll
                 for (int k = 0; k < kDims; ++k) acc[k][b] *= f;
             }
             const float m = raised(row0);
             l *= __builtin_amdgcn_exp2f(row_m[row0] - m);
-            if (to != ref) {  // this run's value scales are in LDS against the old one
-                _Float16* const r = (_Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel);
-#pragma unroll
-                for (int i = 0; i < W::kMine; ++i) r[(my_chunk + i) * W::kRel + my_key] *= (_Float16)f_ref;
+            if (to != ref) {
                 ref = to;
-                stage_rel(run + 1);
+                if constexpr (!kF32) {  // this run's value scales are in LDS against the old one
+                    if (has_values) {
+                        _Float16* const r = (_Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel);
+#pragma unroll
+                        for (int i = 0; i < W::kMine; ++i) r[(my_chunk + i) * W::kRel + my_key] *= (_Float16)f_ref;
+                        stage_rel(run + 1, (uint32_t)ref);
+                    }
+                }
             }
             weights(m);
             kv_lds_barrier();
@@ -2037,19 +1476,15 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
             kv_lds_barrier();
         }
         l += add;
-    };
-
-    if (run0 < run1) pass(run0, std::true_type());
-    for (uint32_t run = run0 + 1; run < run1; ++run) pass(run, std::false_type());
+    }
     if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
     if (run0 < run1) {
-        read_weights(run1 - 1);
+        read_weights(run1 + 1);
 #pragma unroll
-        for (int f = 0; f < kDims; ++f) values_step(run1 - 1, f);
+        for (int f = 0; f < kDims; ++f) values_step(run1 + 2, f);
     }
 
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = kv_sum_groups(l);
     if (g == 0) wave_l[kq][row0] = l;
     kv_lds_barrier();
     const float up = kv_bits((uint32_t)ref << 23);
@@ -2058,7 +1493,10 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
         const uint32_t r = 16 * b + r16;
         if (r >= tile.rows) continue;
         const uint32_t flat = tile.row0 + r, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
-        const float L = wave_l[0][r] + wave_l[1][r], M = row_m[r];
+        const float M = row_m[r];
+        float L = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W::kKeyGroups; ++i) L += wave_l[i][r];
         float denom = L;
         if (whole && a.sink) denom += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
         const float inv = denom == 0.0f ? 0.0f : 1.0f / denom;
@@ -2066,16 +1504,16 @@ __global__ void __launch_bounds__(512, 2) k_kv4_attn_packed(wh_kv4_attn_args a) 
         const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
         for (int f = 0; f < kDims; ++f) {
-            const uint32_t d = 16 * (kDims * wave + f) + 4 * g;
+            const uint32_t d = 16 * (dim0 + f) + 4 * g;
             const wh_f4 y = acc[f][b] * up * inv;
             if (!whole) {
                 *(wh_f2*)(part + d) = (wh_f2){y[0], y[1]};
                 *(wh_f2*)(part + d + 2) = (wh_f2){y[2], y[3]};
             } else {
-                kv_store<false>(a.out, at + d, y);
+                kv_store<kF32>(a.out, at + d, y);
             }
         }
-        if (!whole && wave == 0 && g == 0) {
+        if (!whole && dim0 == 0 && g == 0) {
             part[HD] = M;
             part[HD + 1] = L;
         }
@@ -2132,34 +1570,12 @@ template <int HD, bool kF32, bool kLatent>
 hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
     const bool split = a.units > a.n_tiles;
     const dim3 grid((split ? a.units : a.n_tiles) * a.s.kv_heads);
-    if constexpr (!kF32 && HD >= 256) {
-        if (a.wide) {
-            using W = wh_kv4_packed<HD, kLatent>;
-            static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_packed<HD, kLatent>,
-                                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
-            if (set != hipSuccess) return set;
-            k_kv4_attn_packed<HD, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
-            if (split)
-                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
-            return hipGetLastError();
-        }
-    } else if constexpr (!kF32 && HD == 128) {
-        if (a.wide) {
-            using W = wh_kv4_direct<HD, kLatent>;
-            static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_direct<HD, kLatent>,
-                                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
-            if (set != hipSuccess) return set;
-            k_kv4_attn_direct<HD, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
-            if (split)
-                k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
-            return hipGetLastError();
-        }
-    } else if (a.wide) {
-        using W = wh_kv4_wide<HD, kF32>;
-        static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_wide<HD, kF32, kLatent>,
+    if (a.wide) {
+        using W = wh_kv4_packed<HD, kF32, kLatent>;
+        static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_packed<HD, kF32, kLatent>,
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
         if (set != hipSuccess) return set;
-        k_kv4_attn_wide<HD, kF32, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
+        k_kv4_attn_packed<HD, kF32, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
         if (split)
             k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
         return hipGetLastError();

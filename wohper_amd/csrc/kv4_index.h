@@ -106,3 +106,7 @@ WH_KV_HD uint32_t wh_kv4_chunk(uint64_t blocks, uint64_t tiles, uint64_t units, 
 WH_KV_HD uint32_t wh_kv4_splits(uint32_t blocks, uint32_t chunk) {
     return blocks <= chunk ? 1 : (blocks + chunk - 1) / chunk;
 }
+// And blocks of each of those when they share alike: so many that at most `splits` have any.
+WH_KV_HD uint32_t wh_kv4_even(uint32_t blocks, uint32_t splits) {
+    return splits <= 1 ? 0x7fffffffu : (blocks + splits - 1) / splits;
+}
