@@ -657,6 +657,17 @@ __device__ __forceinline__ uint32_t kv_near_max(uint32_t v) {
     return v;
 }
 
+// Max over the wave, in all lanes.
+__device__ __forceinline__ uint32_t kv_wave_max(uint32_t v) {
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    v = kv_near_max<8>(v);
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true));  // 15 - lane of sixteen
+    u2 p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(p[0], p[1]);
+    p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(p[0], p[1]);
+}
+
 // Max and sum over the four lanes of a row (lane % 16), in all of them.
 __device__ __forceinline__ float kv_max_groups(float v) {
     typedef unsigned u2 __attribute__((ext_vector_type(2)));
@@ -789,7 +800,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
     float m = kMinusBig, l = 0.0f;
     int ref = 0;
     auto raise_ref = [&](uint32_t top) {  // top: of this lane
-        for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+        top = kv_wave_max(top);
         const int to = min((int)top + 3, 254);
         const float f = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
 #pragma unroll
@@ -1260,7 +1271,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
 
     if (run0 < run1) {  // the first run's reference, with room
         uint32_t top = top_byte(run0);
-        for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+        top = kv_wave_max(top);
         if (lane == 0) wave_top[wave] = top;
         kv_lds_barrier();
 #pragma unroll
@@ -1307,18 +1318,18 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     for (uint32_t run = run0; run < run1; ++run) {
         const uint32_t at = run & 1;
         request(run + 1);
-        read_weights(run + 1);
         if constexpr (!kLatent)
             if (t == 0) nan_keys[(run + 2) % 3] = 0;
         // scores
         wh_f4 s[kKeyBlocks];
         uint32_t scale[kKeyBlocks];
-        const uint8_t* krow[kKeyBlocks];
+        const uint8_t* const krow = smem + run % W::kKeyBufs * W::kCodes + (16 * kKeyBlocks * kq + r16) * W::kRow;
+        const uint8_t* const krow_s =
+            smem + W::kAtScales + at * 1024 + ((HD == 64 ? kF32 ? g >> 1 : g & 1 : g) * 64 + 16 * kKeyBlocks * kq + r16) * 4;
+        const uint32_t flip = swizzle(r16);  // of all this lane's keys
 #pragma unroll
         for (int i = 0; i < kKeyBlocks; ++i) {
-            const uint32_t key = 16 * (kKeyBlocks * kq + i) + r16;
-            krow[i] = smem + run % W::kKeyBufs * W::kCodes + key * W::kRow;
-            scale[i] = *(const uint32_t*)(smem + W::kAtScales + at * 1024 + ((HD == 64 ? kF32 ? g >> 1 : g & 1 : g) * 64 + key) * 4);
+            scale[i] = *(const uint32_t*)(krow_s + 64 * i);
             s[i] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
         }
         if constexpr (kF32) {
@@ -1327,14 +1338,13 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
             for (int j = 0; j < kPieces; ++j)
 #pragma unroll
                 for (int i = 0; i < kKeyBlocks; ++i) {
-                    const uint32_t key = 16 * (kKeyBlocks * kq + i) + r16;
                     const float against = kv_bits((scale[i] >> (8 * j) & 0xff) << 23);
                     uint32_t v[4];
                     if constexpr (HD == 64) {
-                        const wh_u2 u = *(const wh_u2*)(krow[i] + 16 * ((g >> 1) ^ swizzle(key)) + 8 * (g & 1));
+                        const wh_u2 u = *(const wh_u2*)(krow + 16 * ((g >> 1) ^ flip) + 8 * (g & 1) + i * 16 * W::kRow);
                         v[0] = u[0], v[1] = u[1];
                     } else {
-                        const wh_u4 u = *(const wh_u4*)(krow[i] + 16 * ((4 * j + g) ^ swizzle(key)));
+                        const wh_u4 u = *(const wh_u4*)(krow + 16 * ((4 * j + g) ^ flip) + i * 16 * W::kRow);
                         v[0] = u[0], v[1] = u[1], v[2] = u[2], v[3] = u[3];
                     }
 #pragma unroll
@@ -1355,8 +1365,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
                 wh_i8 x[kKeyBlocks];
 #pragma unroll
                 for (int i = 0; i < kKeyBlocks; ++i) {
-                    const uint32_t key = 16 * (kKeyBlocks * kq + i) + r16;
-                    const wh_u4 v = *(const wh_u4*)(krow[i] + 16 * ((HD == 64 ? g & 1 : 4 * j + g) ^ swizzle(key)));
+                    const wh_u4 v = *(const wh_u4*)(krow + 16 * ((HD == 64 ? g & 1 : 4 * j + g) ^ flip) + i * 16 * W::kRow);
                     // 64 dims: the other 64 of the product are zeros of the query
                     x[i][0] = v[0], x[i][1] = v[1], x[i][2] = v[2], x[i][3] = v[3];
                     x[i][4] = x[i][5] = x[i][6] = x[i][7] = 0;
@@ -1369,6 +1378,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
                                                                                 q_scale - (p ? 0x04040404u : 0u));
             });
         }
+        read_weights(run + 1);
         // -inf where a row does not see this lane's keys
         const uint32_t v0 = run * 64 + 16 * kKeyBlocks * kq + 4 * g, last = run * 64 + 63;
         const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == kRows &&
@@ -1385,9 +1395,10 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         if constexpr (!kLatent) {
             const uint64_t nan = nan_keys[run % 3];
             if (__builtin_expect(nan != 0, 0)) {
+const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
 #pragma unroll
                 for (int i = 0; i < 4 * kKeyBlocks; ++i)
-                    if ((nan >> (16 * (kKeyBlocks * kq + (i >> 2)) + 4 * g + (i & 3)) & 1) && s[i >> 2][i & 3] != kMinusInf)
+                    if ((mine >> (16 * (i >> 2) + (i & 3)) & 1) && s[i >> 2][i & 3] != kMinusInf)
                         s[i >> 2][i & 3] = kv_bits(0x7fc00000u);
             }
         }
@@ -1435,7 +1446,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         if (__ballot(over) && lane == 0) raise[at] = run + 1;
         kv_lds_barrier();
         if (__builtin_expect(__builtin_amdgcn_readfirstlane(raise[at]) == run + 1, 0)) {  // the whole workgroup
-            for (int off = 32; off >= 1; off >>= 1) vtop = max(vtop, (uint32_t)__shfl_xor((int)vtop, off, 64));
+            vtop = kv_wave_max(vtop);
             top = kv_max_groups(top);
             if (g == 0) wave_m[kq][row0] = top;
             if (lane == 0) wave_top[wave] = vtop;
