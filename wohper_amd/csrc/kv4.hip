@@ -441,26 +441,25 @@ __device__ __forceinline__ void kv_lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <int HD>
-struct wh_kv4_dims {
-    static constexpr int kSteps = HD / 32;                // products of 32 dims
-    static constexpr int kPieces = HD >= 128 ? HD / 128 : 1;  // loads a lane makes of a row
-    static constexpr int kWords = HD >= 128 ? 4 : 2;      // dwords of a load: 32 (16) dims
-    static constexpr int kScaleWords = HD >= 128 ? HD / 128 : 1;
-    static constexpr int kLd = HD + 16;                   // f16 between rows of a staged block: 16 rows of a
-                                                          // transposed read start 32 bytes apart modulo 256
-};
-
-// Raw rows of a lane: key lane % 16 of kN blocks of 16.
+// Raw rows of a lane: key lane % 16 of kN blocks of 16, of each 128 dims the 32
+// that are chunk g (of 64 the 32 that are chunk g % 2), and all its scale bytes.
 template <int HD, int kN>
 struct wh_kv4_raw {
-    uint32_t c[kN][wh_kv4_dims<HD>::kPieces][wh_kv4_dims<HD>::kWords];
-    uint32_t s[kN][wh_kv4_dims<HD>::kScaleWords];
+    static constexpr int kPieces = HD >= 128 ? HD / 128 : 1;
+    uint32_t c[kN][kPieces][4];
+    uint32_t s[kN][kPieces];
 };
 
 template <int HD, int kN>
-__device__ __forceinline__ void kv_load_scales(wh_kv4_raw<HD, kN>& r, int half, const wh_kv4_plane& p, uint64_t line) {
-    const uint8_t* s = p.scales + line * (HD / 32);
+__device__ __forceinline__ void kv_load(wh_kv4_raw<HD, kN>& r, int half, const wh_kv4_plane& p, uint64_t line, uint32_t g) {
+    const uint8_t* const c = p.codes + line * (HD / 2) + 16 * (HD == 64 ? g & 1 : g);
+#pragma unroll
+    for (int j = 0; j < r.kPieces; ++j) {
+        const wh_u4 w = *(const wh_u4*)(c + 64 * j);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r.c[half][j][k] = w[k];
+    }
+    const uint8_t* const s = p.scales + line * (HD / 32);
     if constexpr (HD == 64) r.s[half][0] = *(const uint16_t*)s;
     else if constexpr (HD == 128) r.s[half][0] = *(const uint32_t*)s;
     else if constexpr (HD == 256) {
@@ -473,31 +472,12 @@ __device__ __forceinline__ void kv_load_scales(wh_kv4_raw<HD, kN>& r, int half, 
         for (int k = 0; k < 4; ++k) r.s[half][k] = w[k];
     }
 }
-
-template <int HD, int kN>
-__device__ __forceinline__ void kv_load(wh_kv4_raw<HD, kN>& r, int half, const wh_kv4_plane& p, uint64_t line, uint32_t g) {
-    using D = wh_kv4_dims<HD>;
-    const uint8_t* c = p.codes + line * (HD / 2) + g * (4 * D::kWords);
-#pragma unroll
-    for (int j = 0; j < D::kPieces; ++j) {
-        if constexpr (D::kWords == 4) {
-            const wh_u4 w = *(const wh_u4*)(c + 64 * j);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) r.c[half][j][k] = w[k];
-        } else {
-            const wh_u2 w = *(const wh_u2*)c;
-            r.c[half][j][0] = w[0];
-            r.c[half][j][1] = w[1];
-        }
-    }
-    kv_load_scales(r, half, p, line);
-}
 // The largest scale byte of a raw row.
 template <int HD, int kN>
 __device__ __forceinline__ uint32_t kv_top_byte(const wh_kv4_raw<HD, kN>& r, int half) {
     uint32_t m = 0;
 #pragma unroll
-    for (int k = 0; k < wh_kv4_dims<HD>::kScaleWords; ++k) m = max(m, kv_max_bytes(r.s[half][k]));
+    for (int k = 0; k < r.kPieces; ++k) m = max(m, kv_max_bytes(r.s[half][k]));
     return m;
 }
 
@@ -505,6 +485,7 @@ __device__ __forceinline__ uint32_t kv_top_byte(const wh_kv4_raw<HD, kN>& r, int
 template <int HD, int kN>
 __device__ __forceinline__ uint32_t kv_piece_scales(const wh_kv4_raw<HD, kN>& r, int half, uint32_t g) {
     const uint32_t pick = g | (4 + g) << 8;
+    if constexpr (HD == 64) return (r.s[half][0] >> (8 * (g & 1))) & 0xff;
     if constexpr (HD == 128) return (r.s[half][0] >> (8 * g)) & 0xff;
     if constexpr (HD == 256) return __builtin_amdgcn_perm(r.s[half][1], r.s[half][0], pick) & 0xffff;
     if constexpr (HD == 512)
@@ -517,7 +498,7 @@ __device__ __forceinline__ uint32_t kv_piece_scales(const wh_kv4_raw<HD, kN>& r,
 // decoded values are finite whatever the bytes are.
 template <int HD, int kN>
 __device__ __forceinline__ float kv_rel(const wh_kv4_raw<HD, kN>& r, int half, int j, uint32_t g, uint32_t top) {
-    const uint32_t b = HD == 64 ? (r.s[half][0] >> (8 * (g >> 1))) & 0xff : (r.s[half][j] >> (8 * g)) & 0xff;
+    const uint32_t b = HD == 64 ? (r.s[half][0] >> (8 * (g & 1))) & 0xff : (r.s[half][j] >> (8 * g)) & 0xff;
     return kv_bits((uint32_t)max((int)b - (int)top + 127, 0) << 23);
 }
 
@@ -534,58 +515,95 @@ __device__ __forceinline__ float kv_value_scale(uint32_t vtop, int ref) {
 // First dim of a lane's eight in step s of the product with keys.
 template <int HD>
 __device__ __forceinline__ int kv_dim(int s, uint32_t g) {
-    return HD >= 128 ? 32 * (4 * (s >> 2) + (int)g) + 8 * (s & 3) : 16 * (int)g + 8 * s;
+    return HD >= 128 ? 32 * (4 * (s >> 2) + (int)g) + 8 * (s & 3) : 32 * ((int)g & 1) + 16 * ((int)g >> 1) + 8 * s;
 }
 
-// A lane's part of a query row as it lies in memory: all of it requested at once.
-template <int HD, bool kF32>
-struct wh_kv4_query {
-    wh_u4 raw[HD / 32][kF32 ? 2 : 1];
+// Max over groups of 2, 4 or 8 lanes next to each other, in all of them.
+template <int kN>
+__device__ __forceinline__ uint32_t kv_near_max(uint32_t v) {
+    auto with = [&](uint32_t other) { v = max(v, other); };
+    with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));                  // lanes 1 0 3 2 of a quad
+    if constexpr (kN >= 4) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));   // 2 3 0 1
+    if constexpr (kN >= 8) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));  // 7 - lane of eight
+    return v;
+}
 
-    // flip = 1: steps 2 i and 2 i + 1 change places
-    __device__ __forceinline__ void load(const void* base, uint64_t at, uint32_t g, uint32_t flip = 0) {
+// Max over groups of sixteen lanes, in all of them.
+__device__ __forceinline__ uint32_t kv_row_max(uint32_t v) {
+    v = kv_near_max<8>(v);
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true));  // 15 - lane
+}
+// Max over the wave, in all lanes.
+__device__ __forceinline__ uint32_t kv_wave_max(uint32_t v) {
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    v = kv_row_max(v);
+    u2 p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(p[0], p[1]);
+    p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(p[0], p[1]);
+}
+
+// Queries in f32: the waves share a tile's rows, sixteen lanes a row, and leave
+// each in LDS as two f16 parts against its largest exponent.
+template <int HD, int kRows, int kWaves>
+struct wh_kv4_query {
+    static constexpr int kLd = HD + 8;                        // f16 between rows
+    static constexpr int kEach = kRows / kWaves / 4;          // rows of a lane
+    static constexpr int kBytes = 2 * kRows * kLd * 2;
+    wh_u4 raw[kEach][HD / 64];
+
+    __device__ __forceinline__ static uint32_t row(int i, uint32_t wave, uint32_t lane) { return 4 * (kEach * wave + i) + (lane >> 4); }
+
+    // at(row): the row's first value
+    template <class At>
+    __device__ __forceinline__ void load(uint32_t wave, uint32_t lane, At at) {
 #pragma unroll
-        for (int s = 0; s < HD / 32; ++s) {
-            const uint64_t d = at + kv_dim<HD>(s, g) + (s & 1 ? 0 : 8 * flip) - (s & 1 ? 8 * flip : 0);
-            if constexpr (kF32) {
-                raw[s][0] = *(const wh_u4*)((const float*)base + d);
-                raw[s][1] = *(const wh_u4*)((const float*)base + d + 4);
-            } else {
-                raw[s][0] = *(const wh_u4*)((const uint16_t*)base + d);
-            }
+        for (int i = 0; i < kEach; ++i) {
+            const float* const p = at(row(i, wave, lane)) + 4 * (lane & 15);
+#pragma unroll
+            for (int k = 0; k < HD / 64; ++k) raw[i][k] = *(const wh_u4*)(p + 64 * k);
         }
     }
 
-    // Scaled, in one or two f16 parts; returns what a sum of products with it is to be multiplied by.
-    __device__ __forceinline__ float parts(wh_h8 (&q)[HD / 32][kF32 ? 2 : 1]) const {
-        uint32_t top = 0;
+    // factor[row]: what a sum of products with the row is to be multiplied by
+    __device__ __forceinline__ void put(uint32_t wave, uint32_t lane, _Float16* lds, float* factor) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int k = 0; k < HD / 64; ++k)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) top = max(top, raw[i][k][n] & 0x7fffffffu);
+            top = kv_row_max(top);
+            const int e = max((int)(top >> 23), 27);  // of the largest; 2^-100 at least, so that the factor is finite
+            const float up = kv_bits((uint32_t)(127 + 13 + 127 - e) << 23);
+            const uint32_t r = row(i, wave, lane);
+            _Float16* const dst = lds + r * kLd + 4 * (lane & 15);
+#pragma unroll
+            for (int k = 0; k < HD / 64; ++k) {
+                union {
+                    _Float16 h[4];
+                    wh_u2 u;
+                } hi, lo;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const float x = kv_bits(raw[i][k][n]) * up;
+                    hi.h[n] = (_Float16)x;
+                    lo.h[n] = (_Float16)(x - (float)hi.h[n]);
+                }
+                *(wh_u2*)(dst + 64 * k) = hi.u;
+                *(wh_u2*)(dst + kRows * kLd + 64 * k) = lo.u;
+            }
+            if ((lane & 15) == 0) factor[r] = kv_bits((uint32_t)(e - 13) << 23);
+        }
+    }
+
+    // A lane's operands: the parts of a row's dims kv_dim(step, g) ..
+    __device__ __forceinline__ static void get(wh_h8 (&q)[HD / 32][2], const _Float16* lds, uint32_t row, uint32_t g) {
 #pragma unroll
         for (int s = 0; s < HD / 32; ++s)
 #pragma unroll
-            for (int p = 0; p < (kF32 ? 2 : 1); ++p)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t w = raw[s][p][k];
-                    top = max(top, kF32 ? w & 0x7fffffffu : max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
-                }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-        const int e = max((int)(top >> 23), 27);  // of the largest; 2^-100 at least, so that the factor is finite
-        const float up = kv_bits((uint32_t)(127 + 13 + 127 - e) << 23);
-#pragma unroll
-        for (int s = 0; s < HD / 32; ++s) {
-            wh_h8 hi, lo;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t w = kF32 ? raw[s][k >> 2][k & 3] : raw[s][0][k >> 1];
-                const float x = kv_bits(kF32 ? w : k & 1 ? w & 0xffff0000u : w << 16) * up;
-                hi[k] = (_Float16)x;
-                if constexpr (kF32) lo[k] = (_Float16)(x - (float)hi[k]);
-            }
-            q[s][0] = hi;
-            if constexpr (kF32) q[s][1] = lo;
-        }
-        return kv_bits((uint32_t)(e - 13) << 23);
+            for (int p = 0; p < 2; ++p) q[s][p] = *(const wh_h8*)(lds + (p * kRows + row) * kLd + kv_dim<HD>(s, g));
     }
 };
 
@@ -647,27 +665,6 @@ __device__ __forceinline__ uint32_t kv_query_e4m3(const wh_u4 (&raw)[2][2], uint
     return w == 255 ? 255u : (uint32_t)(w - 7);
 }
 
-// Max over groups of 2, 4 or 8 lanes next to each other, in all of them.
-template <int kN>
-__device__ __forceinline__ uint32_t kv_near_max(uint32_t v) {
-    auto with = [&](uint32_t other) { v = max(v, other); };
-    with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));                  // lanes 1 0 3 2 of a quad
-    if constexpr (kN >= 4) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));   // 2 3 0 1
-    if constexpr (kN >= 8) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));  // 7 - lane of eight
-    return v;
-}
-
-// Max over the wave, in all lanes.
-__device__ __forceinline__ uint32_t kv_wave_max(uint32_t v) {
-    typedef unsigned u2 __attribute__((ext_vector_type(2)));
-    v = kv_near_max<8>(v);
-    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true));  // 15 - lane of sixteen
-    u2 p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max(p[0], p[1]);
-    p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return max(p[0], p[1]);
-}
-
 // Max and sum over the four lanes of a row (lane % 16), in all of them.
 __device__ __forceinline__ float kv_max_groups(float v) {
     typedef unsigned u2 __attribute__((ext_vector_type(2)));
@@ -694,7 +691,7 @@ __device__ __forceinline__ float kv_sum_groups(float v) {
 // of the product with the values as they are.
 template <int HD, bool kF32>
 struct wh_kv4_narrow {
-    static constexpr bool kDirect = !kF32 && HD >= 128;      // scores on codes as they lie
+    static constexpr bool kDirect = !kF32;                   // scores on codes as they lie
     static constexpr int kParts = kF32 ? 2 : 1;
     static constexpr int kPieces = HD / 128 ? HD / 128 : 1;
     static constexpr int kHold = HD >= 256 ? 2 : 4;          // blocks of 16 keys whose rows are held at once
@@ -704,16 +701,17 @@ struct wh_kv4_narrow {
     static constexpr int kAtKeys = kAtRel + kGroups * kRel * 2;
     static constexpr int kWave = kAtKeys + (kDirect ? 0 : 2 * 64 * 4);
     static constexpr size_t kLds = 4 * (size_t)kWave > 2 * 64 * (size_t)HD ? 4 * (size_t)kWave : 2 * 64 * (size_t)HD;
+    using Query = wh_kv4_query<HD, 16, 4>;  // f32: as parts in LDS before the first block
+    static_assert(!kF32 || (size_t)Query::kBytes <= kLds, "queries fit");
 };
 
 template <int HD, bool kF32, bool kLatent>
 __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn_args a) {
-    using D = wh_kv4_dims<HD>;
     using W = wh_kv4_narrow<HD, kF32>;
     constexpr int kParts = W::kParts, kHold = W::kHold, kPieces = W::kPieces;
     constexpr bool kDirect = W::kDirect;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float wave_m[4][16], wave_l[4][16];
+    __shared__ float wave_m[4][16], wave_l[4][16], row_c[kF32 ? 16 : 1];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
     const wh_kv4_place place = kv_place<16, 64>(a, false);
     const uint32_t kvh = place.head;
@@ -768,29 +766,36 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
     if (any) request_pages(part0);
 
     // the row's query
-    wh_h8 qd[kDirect ? 1 : D::kSteps][kParts];
+    wh_h8 qd[kDirect ? 1 : HD / 32][kParts];
     wh_i8 qx[kDirect ? kPieces : 1][2];
     uint32_t q_scale = 0;
     float c;  // a score is its sum times this (and its key's power of two, unless direct)
     {
-        const uint64_t at = (uint64_t)token * a.q_stride + (uint64_t)head * HD;
         if constexpr (kDirect) {
-            const uint16_t* const p = (const uint16_t*)a.q + at + 16 * g;
+            const uint16_t* const p = (const uint16_t*)a.q + (uint64_t)token * a.q_stride + (uint64_t)head * HD + 16 * g;
             wh_u4 raw[kPieces][2][2];
 #pragma unroll
             for (int j = 0; j < kPieces; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) raw[j][i >> 1][i & 1] = *(const wh_u4*)(p + 128 * j + 64 * (i >> 1) + 8 * (i & 1));
+                for (int i = 0; i < 4; ++i)
+                    raw[j][i >> 1][i & 1] = HD == 64 && i >= 2 ? (wh_u4){0, 0, 0, 0} : *(const wh_u4*)(p + 128 * j + 64 * (i >> 1) + 8 * (i & 1));
             if (any) request(part0);
 #pragma unroll
             for (int j = 0; j < kPieces; ++j)
                 q_scale |= kv_query_e4m3(raw[j], a.scale_log2 < 0.0f ? 0x80008000u : 0u, qx[j][0], qx[j][1]) << (8 * j);
             c = fmaxf(fabsf(a.scale_log2), 1.0e-37f);
         } else {
-            wh_kv4_query<HD, kF32> query;
-            query.load(a.q, at, g);
+            typename W::Query query;
+            query.load(wave, lane, [&](uint32_t r) {
+                const uint32_t f = tile.row0 + min(r, tile.rows - 1), n = f / a.group;
+                return (const float*)a.q + (uint64_t)(tile.token0 + n) * a.q_stride + (uint64_t)(kvh * a.group + f - n * a.group) * HD;
+            });
             if (any) request(part0);
-            c = a.scale_log2 * query.parts(qd);
+            query.put(wave, lane, (_Float16*)smem, row_c);
+            kv_lds_barrier();
+            W::Query::get(qd, (const _Float16*)smem, r16, g);
+            c = a.scale_log2 * row_c[r16];
+            kv_lds_barrier();
         }
     }
 
@@ -853,7 +858,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                         if constexpr (kDirect) {
 #pragma unroll
                             for (int j = 0; j < kPieces; ++j)
-                                rel[(4 * j + g) * W::kRel + 16 * (r16 >> 2) + 4 * h + (r16 & 3)] *= (_Float16)f;
+                                if (HD > 64 || g < 2) rel[(4 * j + g) * W::kRel + 16 * (r16 >> 2) + 4 * h + (r16 & 3)] *= (_Float16)f;
                         } else if (g == 0) {
                             key_s[64 + 16 * h + r16] *= f;
                         }
@@ -868,28 +873,23 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
 #pragma unroll
                     for (int j = 0; j < kPieces; ++j) {
                         const int e = (int)((vtop[h] >> (8 * j)) & 0xff) - ref;  // above ref only where it does not count
-                        rel[(4 * j + g) * W::kRel + at] = (_Float16)kv_bits((uint32_t)max(min(e, 0) + 127, 0) << 23);
+                        if (HD > 64 || g < 2) rel[(4 * j + g) * W::kRel + at] = (_Float16)kv_bits((uint32_t)max(min(e, 0) + 127, 0) << 23);
                     }
                 } else {
                     if (g == 0) {
                         key_s[key] = kv_key_scale(ktop[h], vtop[h]);
                         key_s[64 + key] = kv_value_scale(vtop[h], ref);
                     }
-                    if constexpr (HD == 64) {
-                        if ((g & 1) == 0) rel[(g >> 1) * W::kRel + at] = (_Float16)kv_rel(kLatent ? kr : vr, h, 0, g, vtop[h]);
-                    } else {
 #pragma unroll
-                        for (int j = 0; j < kPieces; ++j)
-                            rel[(4 * j + g) * W::kRel + at] = (_Float16)kv_rel(kLatent ? kr : vr, h, j, g, vtop[h]);
-                    }
+                    for (int j = 0; j < kPieces; ++j)
+                        if (HD > 64 || g < 2) rel[(4 * j + g) * W::kRel + at] = (_Float16)kv_rel(kLatent ? kr : vr, h, j, g, vtop[h]);
                 }
                 // the value row's codes
                 uint8_t* const row = mine + key * W::kRow;
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
                     const uint32_t* const cw = kLatent ? kr.c[h][j] : vr.c[h][j];
-                    if constexpr (HD == 64) *(wh_u2*)(row + 16 * ((g >> 1) ^ swizzle(key)) + 8 * (g & 1)) = (wh_u2){cw[0], cw[1]};
-                    else *(wh_u4*)(row + 16 * ((4 * j + g) ^ swizzle(key))) = (wh_u4){cw[0], cw[1], cw[2], cw[3]};
+                    if (HD > 64 || g < 2) *(wh_u4*)(row + 16 * ((4 * j + g) ^ swizzle(key))) = (wh_u4){cw[0], cw[1], cw[2], cw[3]};
                 }
                 // scores
                 s[b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -907,9 +907,10 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                     });
                 } else {
 #pragma unroll
-                    for (int k = 0; k < D::kSteps; ++k) {
-                        const int j = k / D::kWords, w = k - j * D::kWords;
-                        const wh_h8 x = kv_decode(kr.c[h][j][w], kv_rel(kr, h, j, g, ktop[h]));
+                    for (int k = 0; k < HD / 32; ++k) {
+                        const int j = k / 4, w = k - j * 4;
+                        const uint32_t codes = HD == 64 && g >= 2 ? kr.c[h][j][w + 2] : kr.c[h][j][w];
+                        const wh_h8 x = kv_decode(codes, kv_rel(kr, h, j, g, ktop[h]));
 #pragma unroll
                         for (int p = kParts - 1; p >= 0; --p)
                             s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qd[k][p], s[b], 0, 0, 0);
@@ -1095,6 +1096,8 @@ struct wh_kv4_packed {
     static constexpr int kAtRel = kAtTops + (kF32 ? 2 * 64 * 4 : 0);          // [3][group][key] f16
     static constexpr int kAtWeights = kAtRel + 3 * kGroups * kRel * 2;        // [2][part][row][key] f16
     static constexpr size_t kLds = kAtWeights + 2 * (size_t)kParts * kRows * kPl * 2;
+    using Query = wh_kv4_query<HD, kRows, kF32 ? kWaves : 4>;  // f32: as parts in LDS before the first run
+    static_assert(!kF32 || (size_t)Query::kBytes <= kLds, "queries fit");
 };
 
 template <int HD, bool kF32, bool kLatent>
@@ -1104,7 +1107,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     constexpr int kKeyBlocks = W::kKeyBlocks, kWaves = W::kWaves;
     const wh_kv4_place place = kv_place<W::kRows, 64>(a, false);
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float wave_m[W::kKeyGroups][kRows], wave_l[W::kKeyGroups][kRows], row_m[kRows];
+    __shared__ float wave_m[W::kKeyGroups][kRows], wave_l[W::kKeyGroups][kRows], row_m[kRows], row_c[kF32 ? kRows : 1];
     __shared__ int32_t row_pos[kRows];
     __shared__ uint32_t wave_top[kWaves], raise[2];
     __shared__ uint64_t nan_keys[3];
@@ -1119,8 +1122,6 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     if (t < 2) raise[t] = 0;
     if (t < 3) nan_keys[t] = 0;
     if (t < kRows) row_m[t] = kMinusBig;
-    // what the first run finds in place of an earlier one's: no weights, and finite value scales
-    for (uint32_t i = 16 * t; i < W::kLds - W::kAtRel; i += 16 * W::kThreads) *(wh_u4*)(smem + W::kAtRel + i) = (wh_u4){0, 0, 0, 0};
 
     // 16-byte chunk c of a row lies at chunk c ^ swizzle(row): 16 rows of one chunk are on all banks
     auto swizzle = [](uint32_t key) {
@@ -1236,14 +1237,20 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     const uint32_t row0 = 16 * rq + r16;
     {
         const uint32_t flat = tile.row0 + min(row0, tile.rows - 1), tok = flat / a.group;
-        const uint32_t head = kvh * a.group + (flat - tok * a.group);
-        const uint64_t at = (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD;
         if constexpr (kF32) {
-            wh_kv4_query<HD, true> query;
-            query.load(a.q, at, g);
+            typename W::Query query;
+            query.load(wave, lane, [&](uint32_t r) {
+                const uint32_t f = tile.row0 + min(r, tile.rows - 1), n = f / a.group;
+                return (const float*)a.q + (uint64_t)(tile.token0 + n) * a.q_stride + (uint64_t)(kvh * a.group + f - n * a.group) * HD;
+            });
             if (run0 < run1) request(run0);
-            c = a.scale_log2 * query.parts(qd);
+            query.put(wave, lane, (_Float16*)smem, row_c);
+            kv_lds_barrier();
+            W::Query::get(qd, (const _Float16*)smem, row0, g);
+            c = a.scale_log2 * row_c[row0];
+            kv_lds_barrier();
         } else {
+            const uint64_t at = (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)(kvh * a.group + flat - tok * a.group) * HD;
             const uint16_t* const p = (const uint16_t*)a.q + at + 16 * g;
             wh_u4 raw[kPieces][2][2];
 #pragma unroll
@@ -1269,6 +1276,8 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) acc[f][b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
 
+    // what the first run finds in place of an earlier one's: no weights, and finite value scales
+    for (uint32_t i = 16 * t; i < W::kLds - W::kAtRel; i += 16 * W::kThreads) *(wh_u4*)(smem + W::kAtRel + i) = (wh_u4){0, 0, 0, 0};
     if (run0 < run1) {  // the first run's reference, with room
         uint32_t top = top_byte(run0);
         top = kv_wave_max(top);
@@ -1325,7 +1334,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         uint32_t scale[kKeyBlocks];
         const uint8_t* const krow = smem + run % W::kKeyBufs * W::kCodes + (16 * kKeyBlocks * kq + r16) * W::kRow;
         const uint8_t* const krow_s =
-            smem + W::kAtScales + at * 1024 + ((HD == 64 ? kF32 ? g >> 1 : g & 1 : g) * 64 + 16 * kKeyBlocks * kq + r16) * 4;
+            smem + W::kAtScales + at * 1024 + ((HD == 64 ? g & 1 : g) * 64 + 16 * kKeyBlocks * kq + r16) * 4;
         const uint32_t flip = swizzle(r16);  // of all this lane's keys
 #pragma unroll
         for (int i = 0; i < kKeyBlocks; ++i) {
@@ -1341,7 +1350,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
                     const float against = kv_bits((scale[i] >> (8 * j) & 0xff) << 23);
                     uint32_t v[4];
                     if constexpr (HD == 64) {
-                        const wh_u2 u = *(const wh_u2*)(krow + 16 * ((g >> 1) ^ flip) + 8 * (g & 1) + i * 16 * W::kRow);
+                        const wh_u2 u = *(const wh_u2*)(krow + 16 * ((g & 1) ^ flip) + 8 * (g >> 1) + i * 16 * W::kRow);
                         v[0] = u[0], v[1] = u[1];
                     } else {
                         const wh_u4 u = *(const wh_u4*)(krow + 16 * ((4 * j + g) ^ flip) + i * 16 * W::kRow);
