@@ -99,12 +99,13 @@ int main(int argc, char** argv) {
         }
         if (!garbage) CHECK(tiles <= slots);
         for (uint32_t units : {1u, 7u, 64u, 300u}) {
-            const uint32_t chunk = wh_kv4_chunk(blocks, tiles, units, 1 + upto(6));
-            CHECK(chunk >= 1);
+            const uint32_t least = 1 + upto(6);
             uint64_t used = 0;
             for (uint32_t b = 0; b < requests; ++b) {
                 const uint32_t n_q = start(b + 1) > start(b) ? start(b + 1) - start(b) : 0;
-                const uint32_t k = wh_kv4_blocks(n_q, lens[b], cap, window, first, 32), splits = wh_kv4_splits(k, chunk);
+                const uint32_t k = wh_kv4_blocks(n_q, lens[b], cap, window, first, 32), splits = wh_kv4_splits(k, blocks, tiles, units, least);
+                const uint32_t chunk = wh_kv4_even(k, splits);
+                CHECK(splits >= 1 && (splits == 1 || splits * least <= k));
                 CHECK((uint64_t)splits * chunk >= k);
                 used += (uint64_t)wh_kv4_tiles(n_q, group, tile_rows) * splits;
             }

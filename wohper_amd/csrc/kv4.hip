@@ -365,12 +365,11 @@ __device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a, bool
         sum_tiles += ((uint64_t)__shfl_xor((uint32_t)(sum_tiles >> 32), off, 64) << 32) | (uint32_t)__shfl_xor((uint32_t)sum_tiles, off, 64);
         sum_blocks += ((uint64_t)__shfl_xor((uint32_t)(sum_blocks >> 32), off, 64) << 32) | (uint32_t)__shfl_xor((uint32_t)sum_blocks, off, 64);
     }
-    r.chunk = wh_kv4_chunk(sum_blocks, sum_tiles, a.units, a.min_blocks);
     uint32_t tile0 = 0, unit0 = 0;  // of the requests before these 64
     r.tile = wh_kv4_tile_of(0, 0, 0, 0, 0, 0, a.group, 0, 0, kRows);  // none
     for (uint32_t b = 0; b < a.n_requests; b += 64) {
         if (a.n_requests > 64) request(b + lane, tiles, blocks);
-        const uint32_t splits = wh_kv4_splits(blocks, r.chunk);
+        const uint32_t splits = wh_kv4_splits(blocks, sum_blocks, sum_tiles, a.units, a.min_blocks);
         uint32_t t = tiles, u = tiles * splits;
         for (uint32_t d = 1; d < 64; d <<= 1) {
             const uint32_t pt = __shfl_up(t, d, 64), pu = __shfl_up(u, d, 64);
@@ -1095,9 +1094,15 @@ struct wh_kv4_packed {
     static constexpr int kAtTops = kAtKeys + (kF32 ? 2 * 64 * 4 : 0);         // f32: [2][key] exponent of value rows
     static constexpr int kAtRel = kAtTops + (kF32 ? 2 * 64 * 4 : 0);          // [3][group][key] f16
     static constexpr int kAtWeights = kAtRel + 3 * kGroups * kRel * 2;        // [2][part][row][key] f16
-    static constexpr size_t kLds = kAtWeights + 2 * (size_t)kParts * kRows * kPl * 2;
-    using Query = wh_kv4_query<HD, kRows, kF32 ? kWaves : 4>;  // f32: as parts in LDS before the first run
-    static_assert(!kF32 || (size_t)Query::kBytes <= kLds, "queries fit");
+    static constexpr int kEnd = kAtWeights + 2 * kParts * kRows * kPl * 2;
+    // f32: queries lie as parts in LDS before the first run.  At 512 dims registers do not hold all of them (what
+    // the compiler moves to memory instead waits for the rows in flight): the last kFromLds steps' second parts
+    // stay there, behind the rest, and are read again each run.
+    using Query = wh_kv4_query<HD, kRows, kF32 ? kWaves : 4>;
+    static constexpr int kFromLds = kF32 && HD == 512 ? kLatent ? 4 : 8 : 0;
+    static constexpr int kAtQuery = kFromLds ? kEnd - Query::kBytes / 2 : 0;
+    static constexpr size_t kLds = kFromLds ? kEnd + Query::kBytes / 2 : kEnd;
+    static_assert(!kF32 || (size_t)(kAtQuery + Query::kBytes) <= kLds, "queries fit");
 };
 
 template <int HD, bool kF32, bool kLatent>
@@ -1244,9 +1249,9 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
                 return (const float*)a.q + (uint64_t)(tile.token0 + n) * a.q_stride + (uint64_t)(kvh * a.group + f - n * a.group) * HD;
             });
             if (run0 < run1) request(run0);
-            query.put(wave, lane, (_Float16*)smem, row_c);
+            query.put(wave, lane, (_Float16*)(smem + W::kAtQuery), row_c);
             kv_lds_barrier();
-            W::Query::get(qd, (const _Float16*)smem, row0, g);
+            W::Query::get(qd, (const _Float16*)(smem + W::kAtQuery), row0, g);
             c = a.scale_log2 * row_c[row0];
             kv_lds_barrier();
         } else {
@@ -1277,7 +1282,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         for (int b = 0; b < kBlocks; ++b) acc[f][b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
 
     // what the first run finds in place of an earlier one's: no weights, and finite value scales
-    for (uint32_t i = 16 * t; i < W::kLds - W::kAtRel; i += 16 * W::kThreads) *(wh_u4*)(smem + W::kAtRel + i) = (wh_u4){0, 0, 0, 0};
+    for (uint32_t i = 16 * t; i < W::kEnd - W::kAtRel; i += 16 * W::kThreads) *(wh_u4*)(smem + W::kAtRel + i) = (wh_u4){0, 0, 0, 0};
     if (run0 < run1) {  // the first run's reference, with room
         uint32_t top = top_byte(run0);
         top = kv_wave_max(top);
@@ -1342,7 +1347,11 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
             s[i] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
         }
         if constexpr (kF32) {
+            wh_f4 s_low[kKeyBlocks];  // of the second parts: a chain of products of its own
+#pragma unroll
+            for (int i = 0; i < kKeyBlocks; ++i) s_low[i] = s[i];
             // keys decoded against their row's power of two
+            const _Float16* const low = (const _Float16*)(smem + W::kEnd) + row0 * W::Query::kLd;
 #pragma unroll
             for (int j = 0; j < kPieces; ++j)
 #pragma unroll
@@ -1360,13 +1369,20 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
                     for (int k = 0; k < (HD == 64 ? 2 : 4); ++k) {
                         const wh_h8 x = kv_decode(v[k], against);
 #pragma unroll
-                        for (int p = kParts - 1; p >= 0; --p)
-                            s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qd[4 * j + k][p], s[i], 0, 0, 0);
+                        for (int p = kParts - 1; p >= 0; --p) {
+                            constexpr int kSteps = HD / 32;
+                            const int step = 4 * j + k;
+                            const wh_h8 y = p == 1 && step >= kSteps - W::kFromLds
+                                                ? *(const wh_h8*)(low + kv_dim<HD>(step, g))
+                                                : qd[step][p];
+                            wh_f4& to = p ? s_low[i] : s[i];
+                            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, to, 0, 0, 0);
+                        }
                     }
                 }
 #pragma unroll
             for (int i = 0; i < kKeyBlocks; ++i)
-                s[i] = s[i] * c * *(const wh_f4*)(smem + W::kAtKeys + (at * 64 + 16 * (kKeyBlocks * kq + i) + 4 * g) * 4);
+                s[i] = (s[i] + s_low[i]) * c * *(const wh_f4*)(smem + W::kAtKeys + (at * 64 + 16 * (kKeyBlocks * kq + i) + 4 * g) * 4);
         } else {
             // codes as they lie, which takes scales by 32 dims
             wh_static_for<kPieces>([&](auto jc) {

@@ -93,18 +93,16 @@ WH_KV_HD uint32_t wh_kv4_blocks(uint32_t n_q, uint32_t len, uint32_t cap, uint32
     if (window && keys > (uint64_t)window + first + n_q) keys = (uint64_t)window + first + n_q;
     return (uint32_t)((keys + block - 1) / block);
 }
-// Blocks a workgroup takes, for `tiles` tiles of `blocks` blocks in all and
-// `units` workgroups: then the workgroups that all tiles need, each its blocks
-// / chunk rounded up, are at most `units`.  Every key of a tile in one workgroup
-// where there are less than two for each.
-WH_KV_HD uint32_t wh_kv4_chunk(uint64_t blocks, uint64_t tiles, uint64_t units, uint32_t min_blocks) {
-    if (units < 2 * tiles) return 0x7fffffffu;
-    const uint64_t free = units - tiles, even = (blocks + free - 1) / free;
-    return even < min_blocks ? min_blocks : even > 0x7fffffffu ? 0x7fffffffu : (uint32_t)even;
-}
-// Workgroups of a tile of so many blocks.
-WH_KV_HD uint32_t wh_kv4_splits(uint32_t blocks, uint32_t chunk) {
-    return blocks <= chunk ? 1 : (blocks + chunk - 1) / chunk;
+// Workgroups of a tile of `blocks` blocks: one, and its part of the `units` that
+// are more than there are tiles (by all their blocks, `sum`), rounded down: all
+// tiles together have max(units, tiles) at most.  No less than min_blocks each.
+// The quotient of whole numbers below 2^53 is rounded to the nearest double, which
+// does not reach a whole number that it is less than (by 1 / sum at least).
+WH_KV_HD uint32_t wh_kv4_splits(uint32_t blocks, uint64_t sum, uint64_t tiles, uint32_t units, uint32_t min_blocks) {
+    const uint32_t most = blocks / min_blocks;
+    if (units <= tiles || !sum || most <= 1) return 1;
+    const double share = (double)((uint64_t)blocks * (units - (uint32_t)tiles)) / (double)sum;
+    return share + 1.0 < (double)most ? 1 + (uint32_t)share : most;
 }
 // And blocks of each of those when they share alike: so many that at most `splits` have any.
 WH_KV_HD uint32_t wh_kv4_even(uint32_t blocks, uint32_t splits) {
