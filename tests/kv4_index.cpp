@@ -40,10 +40,10 @@ int main(int argc, char** argv) {
     const int n = std::atoi(argv[1]);
     for (int it = 0; it < n; ++it) {
         const bool garbage = it & 1;
-        const uint32_t tile_rows = 16u << upto(2), shift = upto(6), group = it % 7 == 2 ? 16u << upto(3) : 1 + upto(it % 3 ? 8 : 70);
+        const uint32_t tile_rows = 16u << upto(2), shift = upto(8), group = it % 7 == 2 ? 16u << upto(3) : 1 + upto(it % 3 ? 8 : 70);
         const uint32_t requests = 1 + upto(it % 5 ? 6 : 150), n_tokens = upto(60);
         const uint32_t table_stride = upto(30), n_pages = 1 + upto(40), kv_heads = 1 + upto(3);
-        const uint32_t window = upto(1) ? 0 : 1 + upto(20), first = upto(6);
+        const uint32_t window = upto(1) ? 0 : 1 + upto(it % 8 ? 20 : 300), first = upto(it % 4 ? 6 : 200);
         std::vector<uint32_t> starts(requests + 1), lens(requests);
         for (auto& s : starts) s = garbage && upto(1) ? (uint32_t)next() : upto(n_tokens);
         std::sort(starts.begin(), starts.end());
@@ -62,7 +62,7 @@ int main(int argc, char** argv) {
                 while (b + 1 < requests && wh_kv4_tile_base(start(b + 1), group, b + 1, tile_rows) <= x) ++b;
             const wh_kv4_tile t = wh_kv4_tile_of(x, b, start(b), start(b + 1), lens[b], cap, group, window, first, tile_rows);
             if (!t.ok) {
-                CHECK(t.n_keys == 0 && t.rows == 0);
+                CHECK(t.runs == 0 && t.rows == 0);
                 continue;
             }
             CHECK(t.rows >= 1 && t.rows <= tile_rows && (uint64_t)t.row0 + t.rows <= (uint64_t)t.n_q * group);
@@ -80,22 +80,26 @@ int main(int argc, char** argv) {
                 CHECK(!wh_kv4_sees((int32_t)pos, (uint32_t)std::max<int64_t>(pos + 1, 0), window, first));
             }
             std::set<uint32_t> got;
-            for (uint32_t v = 0; v < t.n_keys; ++v) {
-                const uint32_t key = wh_kv4_key(t, v);
-                CHECK(key < cap && (key >> shift) < table_stride);
-                got.insert(key);
-                const uint32_t page = upto(n_pages - 1), head = upto(kv_heads - 1), row = key & ((1u << shift) - 1u);
-                CHECK(wh_kv4_line(page, head, row, kv_heads, shift) < ((uint64_t)n_pages * kv_heads << shift));
+            for (uint32_t run = 0; run < t.runs; ++run) {
+                const uint32_t key0 = wh_kv4_run(t, run);
+                CHECK(key0 % 64 == 0);
+                for (uint32_t key = key0; key < key0 + 64; ++key) {
+                    const uint32_t some = wh_kv4_seen(t, key0, key);
+                    CHECK(some >= key0 && some < key0 + 64 && some < cap && (some >> shift) < table_stride);
+                    if (some != key) continue;
+                    CHECK(got.insert(key).second);  // each once
+                    const uint32_t page = upto(n_pages - 1), head = upto(kv_heads - 1), row = key & ((1u << shift) - 1u);
+                    CHECK(wh_kv4_line(page, head, row, kv_heads, shift) < ((uint64_t)n_pages * kv_heads << shift));
+                }
             }
-            CHECK(got.size() == t.n_keys);  // each once
             for (uint32_t j : want) CHECK(got.count(j));
-            CHECK(t.n_keys <= 32 * (uint64_t)wh_kv4_blocks(t.n_q, lens[b], cap, window, first, 32));
+            CHECK(t.runs <= wh_kv4_runs(t.n_q, lens[b], cap, window, first));
         }
         uint64_t tiles = 0, blocks = 0;
         for (uint32_t b = 0; b < requests; ++b) {
             const uint32_t n_q = start(b + 1) > start(b) ? start(b + 1) - start(b) : 0, k = wh_kv4_tiles(n_q, group, tile_rows);
             tiles += k;
-            blocks += (uint64_t)k * wh_kv4_blocks(n_q, lens[b], cap, window, first, 32);
+            blocks += (uint64_t)k * wh_kv4_runs(n_q, lens[b], cap, window, first);
         }
         if (!garbage) CHECK(tiles <= slots);
         for (uint32_t units : {1u, 7u, 64u, 300u}) {
@@ -103,7 +107,7 @@ int main(int argc, char** argv) {
             uint64_t used = 0;
             for (uint32_t b = 0; b < requests; ++b) {
                 const uint32_t n_q = start(b + 1) > start(b) ? start(b + 1) - start(b) : 0;
-                const uint32_t k = wh_kv4_blocks(n_q, lens[b], cap, window, first, 32), splits = wh_kv4_splits(k, blocks, tiles, units, least);
+                const uint32_t k = wh_kv4_runs(n_q, lens[b], cap, window, first), splits = wh_kv4_splits(k, blocks, tiles, units, least);
                 const uint32_t chunk = wh_kv4_even(k, splits);
                 CHECK(splits >= 1 && (splits == 1 || splits * least <= k));
                 CHECK((uint64_t)splits * chunk >= k);

@@ -54,14 +54,14 @@ struct wh_kv4_attn_args {
     uint32_t n_tokens, n_requests, group, window, first;
     uint32_t n_tiles;     // slots or tiles, at most
     uint32_t units;       // workgroups of a key head, at most; > n_tiles: their keys are cut up
-    uint32_t min_blocks;  // that a workgroup takes
+    uint32_t min_runs;  // that a workgroup takes
     bool wide;          // tiles of 64 (f32: 32) rows instead of 16
     float scale_log2;   // scale * log2(e)
     uint32_t* status;
 };
 // How a call is cut up: by sizes the host knows.
 struct wh_kv4_attn_plan {
-    uint32_t n_tiles, units, min_blocks;
+    uint32_t n_tiles, units, min_runs;
     bool wide;
     size_t part_bytes;  // scratch for partial results, 0 for one split
 };

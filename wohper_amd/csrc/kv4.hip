@@ -332,7 +332,7 @@ struct wh_kv4_place {
 // many share one: every wave adds up all requests (at most WH_KV_SPLIT_REQUESTS)
 // and finds its own by the running sum.  by_tile: x counts tiles, and the place
 // is their first unit.
-template <int kRows, int kKeys>
+template <int kRows>
 __device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a, bool by_tile) {
     wh_kv4_place r;
     const uint32_t x = blockIdx.x / a.s.kv_heads;
@@ -351,7 +351,7 @@ __device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a, bool
         if (b < a.n_requests) {
             const uint32_t s0 = start(b), s1 = start(b + 1), n_q = s1 > s0 ? s1 - s0 : 0;
             tiles = wh_kv4_tiles(n_q, a.group, kRows);
-            blocks = wh_kv4_blocks(n_q, a.lens[b], cap, a.window, a.first, kKeys);
+            blocks = wh_kv4_runs(n_q, a.lens[b], cap, a.window, a.first);
         }
     };
     uint64_t sum_tiles = 0, sum_blocks = 0;
@@ -369,7 +369,7 @@ __device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a, bool
     r.tile = wh_kv4_tile_of(0, 0, 0, 0, 0, 0, a.group, 0, 0, kRows);  // none
     for (uint32_t b = 0; b < a.n_requests; b += 64) {
         if (a.n_requests > 64) request(b + lane, tiles, blocks);
-        const uint32_t splits = wh_kv4_splits(blocks, sum_blocks, sum_tiles, a.units, a.min_blocks);
+        const uint32_t splits = wh_kv4_splits(blocks, sum_blocks, sum_tiles, a.units, a.min_runs);
         uint32_t t = tiles, u = tiles * splits;
         for (uint32_t d = 1; d < 64; d <<= 1) {
             const uint32_t pt = __shfl_up(t, d, 64), pu = __shfl_up(u, d, 64);
@@ -399,9 +399,12 @@ __device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a, bool
     r.tile.n_q = __builtin_amdgcn_readfirstlane(r.tile.n_q);
     r.tile.token0 = __builtin_amdgcn_readfirstlane(r.tile.token0);
     r.tile.len = __builtin_amdgcn_readfirstlane(r.tile.len);
-    r.tile.n_first = __builtin_amdgcn_readfirstlane(r.tile.n_first);
+    r.tile.first = __builtin_amdgcn_readfirstlane(r.tile.first);
+    r.tile.from = __builtin_amdgcn_readfirstlane(r.tile.from);
+    r.tile.end = __builtin_amdgcn_readfirstlane(r.tile.end);
+    r.tile.first_runs = __builtin_amdgcn_readfirstlane(r.tile.first_runs);
     r.tile.lo = __builtin_amdgcn_readfirstlane(r.tile.lo);
-    r.tile.n_keys = __builtin_amdgcn_readfirstlane(r.tile.n_keys);
+    r.tile.runs = __builtin_amdgcn_readfirstlane(r.tile.runs);
     r.tile.ok = __builtin_amdgcn_readfirstlane((int)r.tile.ok) != 0;
     r.unit = __builtin_amdgcn_readfirstlane(r.unit);
     r.split = __builtin_amdgcn_readfirstlane(r.split);
@@ -712,11 +715,11 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float wave_m[4][16], wave_l[4][16], row_c[kF32 ? 16 : 1];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
-    const wh_kv4_place place = kv_place<16, 64>(a, false);
+    const wh_kv4_place place = kv_place<16>(a, false);
     const uint32_t kvh = place.head;
     const wh_kv4_tile tile = place.tile;
     if (!tile.ok) return;
-    const uint32_t blocks = (tile.n_keys + 63) / 64;
+    const uint32_t blocks = tile.runs;
     const uint32_t blk0 = place.split ? place.split * place.chunk : 0, blk1 = min(blocks, blk0 + place.chunk);
     if (place.split && blk0 >= blocks) return;
     const bool whole = place.chunk >= blocks;
@@ -732,29 +735,26 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
 
     // rows are requested kHold blocks of 16 ahead, their pages twice that
     const uint32_t* const table = a.tables + tile.request * a.table_stride;
-    const uint32_t pmask = (1u << a.s.shift) - 1u, end = min(tile.n_keys, blk1 * 64);
+    const uint32_t pmask = (1u << a.s.shift) - 1u;
     wh_kv4_raw<HD, kHold> kr, vr;
     uint32_t page[kHold];
     bool bad = false;
-    // the tile's first key stands in for those past the last; n counts parts of kHold blocks
+    // n counts parts of kHold blocks of 16
     constexpr uint32_t kParts64 = 4 / kHold;
-    auto key_at = [&](uint32_t n, int h) {
-        const uint32_t v = (n / kParts64) * 64 + 16 * (kHold * (n % kParts64) + h) + r16;
-        return wh_kv4_key(tile, v < end ? v : 0);
-    };
+    auto run_of = [&](uint32_t n) { return wh_kv4_run(tile, min(n / kParts64, blk1 - 1)); };
+    auto key_of = [&](uint32_t n, int h) { return run_of(n) + 16 * (kHold * (n % kParts64) + h) + r16; };
     // the part after part n of this wave
     auto after = [&](uint32_t n) { return n % kParts64 == kParts64 - 1 ? n + 1 + 3 * kParts64 : n + 1; };
     auto request_pages = [&](uint32_t n) {
 #pragma unroll
-        for (int h = 0; h < kHold; ++h) page[h] = table[key_at(n, h) >> a.s.shift];
+        for (int h = 0; h < kHold; ++h) page[h] = table[wh_kv4_seen(tile, run_of(n), key_of(n, h)) >> a.s.shift];
     };
     auto request = [&](uint32_t n) {
 #pragma unroll
         for (int h = 0; h < kHold; ++h) {
-            const uint32_t key = key_at(n, h);
             const bool out = page[h] >= a.s.n_pages;
             bad |= out;
-            const uint64_t line = wh_kv4_line(out ? 0 : page[h], kvh, key & pmask, a.s.kv_heads, a.s.shift);
+            const uint64_t line = wh_kv4_line(out ? 0 : page[h], kvh, key_of(n, h) & pmask, a.s.kv_heads, a.s.shift);
             kv_load(kr, h, a.k, line, g);
             if constexpr (!kLatent) kv_load(vr, h, a.v, line, g);
         }
@@ -825,6 +825,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
 
     for (uint32_t blk = blk0 + wave; blk < blk1; blk += 4) {
         wh_f4 s[4];
+        const uint32_t key0 = wh_kv4_run(tile, blk);
         kv_wave_order();
         wh_static_for<(int)kParts64>([&](auto pc) {
             constexpr int part = decltype(pc)::value;
@@ -832,19 +833,20 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
             uint32_t above = 0;
 #pragma unroll
             for (int h = 0; h < kHold; ++h) {
-                const uint32_t v = blk * 64 + 16 * (kHold * part + h) + r16;
+                const uint32_t my_key = key0 + 16 * (kHold * part + h) + r16;
+                const bool counts = wh_kv4_seen(tile, key0, my_key) == my_key;
                 if constexpr (kDirect) {
                     const uint32_t b = kv_piece_scales(kLatent ? kr : vr, h, g);
 #pragma unroll
                     for (int j = 0; j < kPieces; ++j) {
                         const uint32_t e = (b >> (8 * j)) & 0xff;
-                        above = max(above, v < end && e < 255 ? e : 0u);
+                        above = max(above, counts && e < 255 ? e : 0u);
                     }
                     ktop[h] = vtop[h] = b;
                 } else {
                     ktop[h] = kv_top_byte(kr, h);
                     vtop[h] = kLatent ? ktop[h] : kv_top_byte(vr, h);
-                    above = max(above, v < end && vtop[h] < 255 ? vtop[h] : 0u);
+                    above = max(above, counts && vtop[h] < 255 ? vtop[h] : 0u);
                 }
             }
             if (__ballot((int)above > ref)) {
@@ -941,18 +943,13 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
 #pragma unroll
             for (int b = 0; b < 4; ++b) s[b] *= *(const wh_f4*)&key_s[16 * b + 4 * g] * c;
         }
-        const uint32_t last = blk * 64 + 63;
-        const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == 16 &&
-                         (!a.window || (int64_t)wh_kv4_key(tile, max(blk * 64, tile.n_first)) + a.window > pos_hi);
+        const bool all = (int32_t)key0 + 63 <= pos_lo && tile.rows == 16 && (!a.window || (int64_t)key0 + a.window > pos_hi);
         if (!all) {
 #pragma unroll
             for (int b = 0; b < 4; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t v = blk * 64 + 16 * b + 4 * g + i;
-                    const bool see = (v < tile.n_keys) & wh_kv4_sees(pos, wh_kv4_key(tile, v), a.window, a.first);
-                    s[b][i] = see ? s[b][i] : kMinusInf;
-                }
+                for (int i = 0; i < 4; ++i)
+                    s[b][i] = wh_kv4_sees(pos, key0 + 16 * b + 4 * g + i, a.window, a.first) ? s[b][i] : kMinusInf;
         }
         float top = kMinusInf;
 #pragma unroll
@@ -1110,7 +1107,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     using W = wh_kv4_packed<HD, kF32, kLatent>;
     constexpr int kBlocks = W::kBlocks, kRows = W::kRows, kDims = W::kDims, kPieces = W::kPieces, kParts = W::kParts;
     constexpr int kKeyBlocks = W::kKeyBlocks, kWaves = W::kWaves;
-    const wh_kv4_place place = kv_place<W::kRows, 64>(a, false);
+    const wh_kv4_place place = kv_place<W::kRows>(a, false);
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float wave_m[W::kKeyGroups][kRows], wave_l[W::kKeyGroups][kRows], row_m[kRows], row_c[kF32 ? kRows : 1];
     __shared__ int32_t row_pos[kRows];
@@ -1120,7 +1117,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     const uint32_t kvh = place.head, kq = wave % W::kKeyGroups, rq = wave / W::kKeyGroups;
     const wh_kv4_tile tile = place.tile;
     if (!tile.ok) return;
-    const uint32_t runs = (tile.n_keys + 63) / 64;
+    const uint32_t runs = tile.runs;
     const uint32_t run0 = place.split ? place.split * place.chunk : 0, run1 = min(runs, run0 + place.chunk);
     if (place.split && run0 >= runs) return;
     const bool whole = place.chunk >= runs;
@@ -1138,20 +1135,18 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     const bool brings = wave < W::kBring * (W::kBoth ? 1u : 2u);
     const bool has_values = W::kBoth ? brings : brings && wave >= W::kBring, has_keys = W::kBoth ? brings : wave < W::kBring;
     const uint32_t* const table = a.tables + tile.request * a.table_stride;
-    const uint32_t pmask = (1u << a.s.shift) - 1u, end = min(tile.n_keys, run1 * 64);
+    const uint32_t pmask = (1u << a.s.shift) - 1u;
     const uint32_t my_key = 64 / W::kLanes * (wave % W::kBring) + lane / W::kLanes, my_chunk = W::kMine * (lane % W::kLanes);
     bool bad = false;
     uint32_t page = 0;
     constexpr bool kTwo = W::kBoth && !kLatent;  // chunks of values are held beside those of keys
     wh_u4 kc[W::kMine], vc[kTwo ? W::kMine : 1];
     uint32_t kb = 0, vb = 0;  // their scale bytes
-    // the tile's first key stands in for those past the last
-    auto key_at = [&](uint32_t run) {
-        const uint32_t v = run * 64 + my_key;
-        return wh_kv4_key(tile, v < end ? v : 0);
-    };
+    auto run_at = [&](uint32_t run) { return wh_kv4_run(tile, min(run, run1 - 1)); };
     auto request_page = [&](uint32_t run) {
-        if (W::kBring == kWaves || brings) page = table[key_at(run) >> a.s.shift];
+        if (W::kBring < kWaves && !brings) return;
+        const uint32_t key0 = run_at(run);
+        page = table[wh_kv4_seen(tile, key0, key0 + my_key) >> a.s.shift];
     };
     auto request_of = [&](const wh_kv4_plane& p, uint64_t line, wh_u4* c, uint32_t& b) {
         const uint8_t* const src = p.codes + line * (HD / 2) + 16 * my_chunk;
@@ -1162,17 +1157,19 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     };
     auto request = [&](uint32_t run) {
         if (W::kBring < kWaves && !brings) return;
-        const uint32_t key = key_at(run);
         const bool out = page >= a.s.n_pages;
         bad |= out;
-        const uint64_t line = wh_kv4_line(out ? 0 : page, kvh, key & pmask, a.s.kv_heads, a.s.shift);
+        const uint64_t line = wh_kv4_line(out ? 0 : page, kvh, (run_at(run) + my_key) & pmask, a.s.kv_heads, a.s.shift);
         request_of(W::kBoth || has_keys ? a.k : a.v, line, kc, kb);
         if constexpr (kTwo) request_of(a.v, line, vc, vb);
         request_page(run + 1);
     };
     int ref = 0;
     auto value_bytes = [&] { return kTwo ? vb : kb; };
-    auto counts = [&](uint32_t run) { return run * 64 + my_key < end; };
+    auto counts = [&](uint32_t run) {  // whether some row may see this lane's key; so too of the last run's once more
+        const uint32_t key0 = run_at(run);
+        return wh_kv4_seen(tile, key0, key0 + my_key) == key0 + my_key;
+    };
     // largest value scale byte of this lane's chunks that counts
     auto top_byte = [&](uint32_t run) {
         uint32_t m = 0;
@@ -1405,16 +1402,14 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         }
         read_weights(run + 1);
         // -inf where a row does not see this lane's keys
-        const uint32_t v0 = run * 64 + 16 * kKeyBlocks * kq + 4 * g, last = run * 64 + 63;
-        const bool all = last < tile.n_keys && (int32_t)wh_kv4_key(tile, last) <= pos_lo && tile.rows == kRows &&
-                         (!a.window || (int64_t)wh_kv4_key(tile, max(run * 64, tile.n_first)) + a.window > pos_hi);
+        const uint32_t key0 = wh_kv4_run(tile, run);
+        const bool all = (int32_t)key0 + 63 <= pos_lo && tile.rows == kRows && (!a.window || (int64_t)key0 + a.window > pos_hi);
         if (!all) {
             const int32_t pos = row_pos[row0];
 #pragma unroll
             for (int i = 0; i < 4 * kKeyBlocks; ++i) {
-                const uint32_t v = v0 + 16 * (i >> 2) + (i & 3), key = wh_kv4_key(tile, v);
-                const bool see = (v < tile.n_keys) & wh_kv4_sees(pos, key, a.window, a.first);
-                s[i >> 2][i & 3] = see ? s[i >> 2][i & 3] : kMinusInf;
+                const uint32_t key = key0 + 16 * (kKeyBlocks * kq + (i >> 2)) + 4 * g + (i & 3);
+                s[i >> 2][i & 3] = wh_kv4_sees(pos, key, a.window, a.first) ? s[i >> 2][i & 3] : kMinusInf;
             }
         }
         if constexpr (!kLatent) {
@@ -1558,13 +1553,13 @@ const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
 
 // Joins the workgroups of a tile: outputs weighted by their sums of weights, and
 // the sink.  A wave a row, four rows a workgroup.
-template <int HD, bool kF32, int kRows, int kKeys>
+template <int HD, bool kF32, int kRows>
 __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
     constexpr int kPer = HD >= 256 ? 4 : HD / 64;  // values of a lane next to each other
     const uint32_t lane = threadIdx.x & 63, row = 4 * blockIdx.y + (threadIdx.x >> 6);
-    const wh_kv4_place place = kv_place<kRows, kKeys>(a, true);
+    const wh_kv4_place place = kv_place<kRows>(a, true);
     const wh_kv4_tile& tile = place.tile;
-    const uint32_t blocks = (tile.n_keys + kKeys - 1) / kKeys, kvh = place.head;
+    const uint32_t blocks = tile.runs, kvh = place.head;
     if (!tile.ok || row >= tile.rows || blocks <= place.chunk) return;
     const uint32_t n = (blocks + place.chunk - 1) / place.chunk;
     const uint32_t flat = tile.row0 + row, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
@@ -1613,7 +1608,7 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
         if (set != hipSuccess) return set;
         k_kv4_attn_packed<HD, kF32, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
         if (split)
-            k_kv4_join<HD, kF32, W::kRows, 64><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
+            k_kv4_join<HD, kF32, W::kRows><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
         return hipGetLastError();
     }
     constexpr size_t lds = wh_kv4_narrow<HD, kF32>::kLds;
@@ -1621,7 +1616,7 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (set != hipSuccess) return set;
     k_kv4_attn<HD, kF32, kLatent><<<grid, 256, lds, stream>>>(a);
-    if (split) k_kv4_join<HD, kF32, 16, 64><<<dim3(a.n_tiles * a.s.kv_heads, 4), 256, 0, stream>>>(a);
+    if (split) k_kv4_join<HD, kF32, 16><<<dim3(a.n_tiles * a.s.kv_heads, 4), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -1670,7 +1665,7 @@ wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, bool 
     uint64_t keys = max_len;
     if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.first + a.n_tokens);
     const uint64_t resident = p.wide && a.s.head_dim >= 256 ? 256 : a.s.head_dim >= 512 ? 256 : a.s.head_dim == 256 ? 512 : p.wide ? 512 : 1024;
-    p.min_blocks = 128 / block;
+    p.min_runs = 128 / block;
     p.units = (uint32_t)(resident / a.s.kv_heads);
     const uint64_t busy = std::max<uint64_t>(rows / tile_rows, a.n_requests);  // tiles, where every request has rows
     if (p.units < 2 * busy || a.n_requests > WH_KV_SPLIT_REQUESTS || keys <= 128) p.units = 0;

@@ -30,7 +30,8 @@ struct wh_kv4_tile {
     uint32_t request, row0, rows, n_q;  // first row of the request's n_q * group and how many
     uint32_t token0;                    // the request's first row of q and out
     int32_t len;                        // its cached rows
-    uint32_t n_first, lo, n_keys;       // keys [0, n_first) and [lo, lo + n_keys - n_first)
+    uint32_t first, from, end;          // its rows see keys [0, first) and [from, end) at most
+    uint32_t first_runs, lo, runs;      // runs of 64 keys that hold those: first_runs from key 0, the others from lo
     bool ok;                            // holds rows
 };
 
@@ -61,21 +62,33 @@ WH_KV_HD wh_kv4_tile wh_kv4_tile_of(uint64_t x, uint32_t b, uint32_t s0, uint32_
     r.row0 = r.ok ? (uint32_t)row0 : 0;
     r.rows = r.ok ? (uint32_t)(all - row0 < tile_rows ? all - row0 : tile_rows) : 0;
     r.len = (int32_t)(len < cap ? len : cap);
-    r.n_first = r.lo = r.n_keys = 0;
+    r.first = r.from = r.end = r.first_runs = r.lo = r.runs = 0;
     if (!r.ok) return r;
     // positions of the first and the last row; negative where there are more tokens than rows
     const int64_t p0 = (int64_t)r.len - r.n_q + r.row0 / group;
     const int64_t p1 = (int64_t)r.len - r.n_q + (r.row0 + r.rows - 1) / group;
     if (p1 < 0) return r;
     const int64_t from = window && p0 + 1 > (int64_t)window ? p0 + 1 - (int64_t)window : 0;
-    r.lo = (uint32_t)from;
-    r.n_first = first < r.lo ? first : r.lo;
-    r.n_keys = r.n_first + (uint32_t)(p1 + 1 - from);
+    r.from = (uint32_t)from;
+    r.end = (uint32_t)(p1 + 1);
+    r.lo = r.from & ~63u;
+    r.first = first < r.from ? first : r.from;
+    r.first_runs = r.first < r.lo ? (r.first + 63) / 64 : r.lo / 64;
+    r.runs = r.first_runs + (r.end - r.lo + 63) / 64;
     return r;
 }
 
-// The v-th key of a tile, v < n_keys.
-WH_KV_HD uint32_t wh_kv4_key(const wh_kv4_tile& t, uint32_t v) { return v < t.n_first ? v : v - t.n_first + t.lo; }
+// First key of run x, a multiple of 64: where a page has 64 rows or more, a run
+// lies in one, and some row sees a key of it.
+WH_KV_HD uint32_t wh_kv4_run(const wh_kv4_tile& t, uint32_t x) { return x < t.first_runs ? 64 * x : t.lo + 64 * (x - t.first_runs); }
+
+// A key of a run that some row may see: `key` itself or, where no row does, one
+// that stands in for it.  Keys that no row sees need not have pages.
+WH_KV_HD uint32_t wh_kv4_seen(const wh_kv4_tile& t, uint32_t key0, uint32_t key) {
+    const uint32_t low = key0 < t.lo ? t.first - 1 : t.from, high = key0 < t.lo ? t.first - 1 : t.end - 1;
+    const uint32_t in = key < low ? low : key < high ? key : high;
+    return key < t.first ? key : in;
+}
 
 // Whether a token at position pos (negative: none) sees a key.
 WH_KV_HD bool wh_kv4_sees(int32_t pos, uint32_t key, uint32_t window, uint32_t first) {
@@ -83,28 +96,28 @@ WH_KV_HD bool wh_kv4_sees(int32_t pos, uint32_t key, uint32_t window, uint32_t f
 }
 
 // How a call whose tiles are fewer than its workgroups cuts up their keys.  Of
-// request b, n_q tokens on len rows: tiles, and at most how many blocks of
-// `block` keys each sees.
+// request b, n_q tokens on len rows: tiles, and at most how many runs each has.
 WH_KV_HD uint32_t wh_kv4_tiles(uint32_t n_q, uint32_t group, uint32_t tile_rows) {
     return (uint32_t)(((uint64_t)n_q * group + tile_rows - 1) / tile_rows);
 }
-WH_KV_HD uint32_t wh_kv4_blocks(uint32_t n_q, uint32_t len, uint32_t cap, uint32_t window, uint32_t first, uint32_t block) {
-    uint64_t keys = len < cap ? len : cap;
-    if (window && keys > (uint64_t)window + first + n_q) keys = (uint64_t)window + first + n_q;
-    return (uint32_t)((keys + block - 1) / block);
+WH_KV_HD uint32_t wh_kv4_runs(uint32_t n_q, uint32_t len, uint32_t cap, uint32_t window, uint32_t first) {
+    const uint64_t keys = len < cap ? len : cap, all = (keys + 63) / 64;
+    if (!window) return (uint32_t)all;
+    const uint64_t seen = ((uint64_t)first + 63) / 64 + ((uint64_t)window + n_q + 125) / 64;  // from a multiple of 64
+    return (uint32_t)(seen < all ? seen : all);
 }
-// Workgroups of a tile of `blocks` blocks: one, and its part of the `units` that
-// are more than there are tiles (by all their blocks, `sum`), rounded down: all
-// tiles together have max(units, tiles) at most.  No less than min_blocks each.
+// Workgroups of a tile of so many runs: one, and its part of the `units` that
+// are more than there are tiles (by all their runs, `sum`), rounded down: all
+// tiles together have max(units, tiles) at most.  No less than min_runs each.
 // The quotient of whole numbers below 2^53 is rounded to the nearest double, which
 // does not reach a whole number that it is less than (by 1 / sum at least).
-WH_KV_HD uint32_t wh_kv4_splits(uint32_t blocks, uint64_t sum, uint64_t tiles, uint32_t units, uint32_t min_blocks) {
-    const uint32_t most = blocks / min_blocks;
+WH_KV_HD uint32_t wh_kv4_splits(uint32_t runs, uint64_t sum, uint64_t tiles, uint32_t units, uint32_t min_runs) {
+    const uint32_t most = runs / min_runs;
     if (units <= tiles || !sum || most <= 1) return 1;
-    const double share = (double)((uint64_t)blocks * (units - (uint32_t)tiles)) / (double)sum;
+    const double share = (double)((uint64_t)runs * (units - (uint32_t)tiles)) / (double)sum;
     return share + 1.0 < (double)most ? 1 + (uint32_t)share : most;
 }
-// And blocks of each of those when they share alike: so many that at most `splits` have any.
-WH_KV_HD uint32_t wh_kv4_even(uint32_t blocks, uint32_t splits) {
-    return splits <= 1 ? 0x7fffffffu : (blocks + splits - 1) / splits;
+// And runs of each of those when they share alike: so many that at most `splits` have any.
+WH_KV_HD uint32_t wh_kv4_even(uint32_t runs, uint32_t splits) {
+    return splits <= 1 ? 0x7fffffffu : (runs + splits - 1) / splits;
 }

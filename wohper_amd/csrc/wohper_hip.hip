@@ -4808,7 +4808,7 @@ int wh_kv4_attention_async(wh_ctx* c, const wh_kv4_cache* cache, const wh_kv4_at
     a.status = c->status;
     const wh_kv4_attn_plan p = wh_kv4_attn_plan_of(a, d->is_bf16 != 0, !has_v, d->max_len);
     a.units = p.units;
-    a.min_blocks = p.min_blocks;
+    a.min_runs = p.min_runs;
     a.n_tiles = p.n_tiles;
     a.wide = p.wide;
     WH_HIP(c->kv4_part.ensure(p.part_bytes, false));
