@@ -319,6 +319,26 @@ __device__ __forceinline__ wh_kv4_tile kv_tile(const wh_kv4_attn_args& a, uint32
     return r;
 }
 
+// Sum over this lane and those before it: within rows of 16, then over the rows.
+template <int kFrom, int kRows>
+__device__ __forceinline__ uint64_t kv_scan_step(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kFrom, kRows, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), kFrom, kRows, 0xf, false);
+    return v + ((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ uint64_t kv_scan(uint64_t v) {
+    v = kv_scan_step<0x111, 0xf>(v);  // 1, 2, 4, 8 lanes before
+    v = kv_scan_step<0x112, 0xf>(v);
+    v = kv_scan_step<0x114, 0xf>(v);
+    v = kv_scan_step<0x118, 0xf>(v);
+    v = kv_scan_step<0x142, 0xa>(v);  // the end of the row before
+    return kv_scan_step<0x143, 0xc>(v);  // the end of the first half
+}
+__device__ __forceinline__ uint64_t kv_lane(uint64_t v, uint32_t lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+
 // What a workgroup does: a tile of one key head, and which of its blocks of
 // keys.  Key heads lie next to each other in the grid, so that of eight each
 // has an XCD's L2 to itself.
@@ -341,56 +361,56 @@ __device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a, bool
     r.split = 0;
     r.chunk = 0x7fffffffu;
     if (a.units <= a.n_tiles) {
-        r.tile = kv_tile<kRows>(a, x);
+        r.tile = kv_tile<kRows>(a, a.n_tiles - 1 - x);  // a prompt's last tiles, which see the most keys, first
         return r;
     }
     const uint32_t lane = threadIdx.x & 63, cap = (uint32_t)min(a.table_stride << a.s.shift, (uint64_t)0x7fffffff);
     auto start = [&](uint32_t b) { return min(a.starts[b], a.n_tokens); };
-    auto request = [&](uint32_t b, uint32_t& tiles, uint32_t& blocks) {
-        tiles = blocks = 0;
-        if (b < a.n_requests) {
-            const uint32_t s0 = start(b), s1 = start(b + 1), n_q = s1 > s0 ? s1 - s0 : 0;
-            tiles = wh_kv4_tiles(n_q, a.group, kRows);
-            blocks = wh_kv4_runs(n_q, a.lens[b], cap, a.window, a.first);
-        }
+    uint32_t s0, s1, len, tiles, blocks;  // of this lane's request
+    auto request = [&](uint32_t b) {
+        const bool ok = b < a.n_requests;
+        s0 = ok ? start(b) : 0;
+        s1 = ok ? start(b + 1) : 0;
+        len = ok ? a.lens[b] : 0;
+        const uint32_t n_q = s1 > s0 ? s1 - s0 : 0;
+        tiles = wh_kv4_tiles(n_q, a.group, kRows);
+        blocks = wh_kv4_runs(n_q, len, cap, a.window, a.first);
     };
     uint64_t sum_tiles = 0, sum_blocks = 0;
-    uint32_t tiles, blocks;
     for (uint32_t b = 0; b < a.n_requests; b += 64) {
-        request(b + lane, tiles, blocks);
+        request(b + lane);
         sum_tiles += tiles;
         sum_blocks += (uint64_t)tiles * blocks;
     }
-    for (int off = 32; off >= 1; off >>= 1) {
-        sum_tiles += ((uint64_t)__shfl_xor((uint32_t)(sum_tiles >> 32), off, 64) << 32) | (uint32_t)__shfl_xor((uint32_t)sum_tiles, off, 64);
-        sum_blocks += ((uint64_t)__shfl_xor((uint32_t)(sum_blocks >> 32), off, 64) << 32) | (uint32_t)__shfl_xor((uint32_t)sum_blocks, off, 64);
-    }
+    sum_tiles = kv_lane(kv_scan(sum_tiles), 63);
+    sum_blocks = kv_lane(kv_scan(sum_blocks), 63);
     uint32_t tile0 = 0, unit0 = 0;  // of the requests before these 64
     r.tile = wh_kv4_tile_of(0, 0, 0, 0, 0, 0, a.group, 0, 0, kRows);  // none
     for (uint32_t b = 0; b < a.n_requests; b += 64) {
-        if (a.n_requests > 64) request(b + lane, tiles, blocks);
+        if (a.n_requests > 64) request(b + lane);
         const uint32_t splits = wh_kv4_splits(blocks, sum_blocks, sum_tiles, a.units, a.min_runs);
-        uint32_t t = tiles, u = tiles * splits;
-        for (uint32_t d = 1; d < 64; d <<= 1) {
-            const uint32_t pt = __shfl_up(t, d, 64), pu = __shfl_up(u, d, 64);
-            if (lane >= d) t += pt, u += pu;
-        }
-        const uint64_t hit = __ballot((by_tile ? tile0 + t : unit0 + u) > x);
+        // tiles below, their units above
+        const uint64_t mine = (uint64_t)(tiles * splits) << 32 | tiles, sum = kv_scan(mine), past = sum - mine;
+        const uint64_t hit = __ballot((by_tile ? tile0 + (uint32_t)sum : unit0 + (uint32_t)(sum >> 32)) > x);
         if (hit) {
-            const int src = __ffsll((unsigned long long)hit) - 1;
-            const uint32_t n = __shfl(splits, src, 64), before = __shfl(by_tile ? t - tiles : u - tiles * splits, src, 64);
+            const uint32_t src = (uint32_t)__ffsll((unsigned long long)hit) - 1;
+            const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)splits, src);
+            const uint64_t all_before = kv_lane(past, src);
+            const uint32_t before = by_tile ? (uint32_t)all_before : (uint32_t)(all_before >> 32);
             const uint32_t at = x - (by_tile ? tile0 : unit0) - before, local = by_tile ? at : at / n;
-            r.chunk = wh_kv4_even(__shfl(blocks, src, 64), n);
-            if (by_tile) r.unit = unit0 + __shfl(u - tiles * splits, src, 64) + at * n;
+            r.chunk = wh_kv4_even((uint32_t)__builtin_amdgcn_readlane((int)blocks, src), n);
+            if (by_tile) r.unit = unit0 + (uint32_t)(all_before >> 32) + at * n;
             r.split = by_tile ? 0 : at - local * n;
-            const uint32_t q = b + src, s0 = start(q);
-            r.tile = wh_kv4_tile_of(wh_kv4_tile_base(s0, a.group, q, kRows) + local, q, s0, start(q + 1), a.lens[q], cap, a.group,
-                                    a.window, a.first, kRows);
-            if (a.lens[q] > cap && threadIdx.x == 0) atomicOr(a.status, WH_ST_NOT_RESIDENT);
+            const uint32_t q = b + src, from = (uint32_t)__builtin_amdgcn_readlane((int)s0, src);
+            const uint32_t rows = (uint32_t)__builtin_amdgcn_readlane((int)len, src);
+            r.tile = wh_kv4_tile_of(wh_kv4_tile_base(from, a.group, q, kRows) + local, q, from,
+                                    (uint32_t)__builtin_amdgcn_readlane((int)s1, src), rows, cap, a.group, a.window, a.first, kRows);
+            if (rows > cap && threadIdx.x == 0) atomicOr(a.status, WH_ST_NOT_RESIDENT);
             break;
         }
-        tile0 += __shfl(t, 63, 64);
-        unit0 += __shfl(u, 63, 64);
+        const uint64_t last = kv_lane(sum, 63);
+        tile0 += (uint32_t)last;
+        unit0 += (uint32_t)(last >> 32);
     }
     // wave-uniform: in scalar registers from here
     r.tile.request = __builtin_amdgcn_readfirstlane(r.tile.request);
@@ -410,6 +430,26 @@ __device__ __forceinline__ wh_kv4_place kv_place(const wh_kv4_attn_args& a, bool
     r.split = __builtin_amdgcn_readfirstlane(r.split);
     r.chunk = __builtin_amdgcn_readfirstlane(r.chunk);
     return r;
+}
+
+// -inf for the keys key + 16 b + i that position pos (-1: none) does not see.  A
+// branch (the empty asm) and not a part of what every run does: the compiler
+// would otherwise compare for all of them.
+template <int kN>
+__device__ __forceinline__ void kv_mask(wh_f4 (&s)[kN], int32_t pos, uint32_t key, uint32_t window, uint32_t first) {
+    asm volatile("");
+    const int32_t past = pos - (int32_t)key;  // the last offset that is not past pos
+#pragma unroll
+    for (int b = 0; b < kN; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[b][i] = 16 * b + i <= past ? s[b][i] : kMinusInf;
+    if (window) {
+        const int32_t near = past - (int32_t)window, early = (int32_t)first - (int32_t)key;
+#pragma unroll
+        for (int b = 0; b < kN; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][i] = (16 * b + i > near) | (16 * b + i < early) ? s[b][i] : kMinusInf;
+    }
 }
 
 // max over the bytes of w
@@ -944,13 +984,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
             for (int b = 0; b < 4; ++b) s[b] *= *(const wh_f4*)&key_s[16 * b + 4 * g] * c;
         }
         const bool all = (int32_t)key0 + 63 <= pos_lo && tile.rows == 16 && (!a.window || (int64_t)key0 + a.window > pos_hi);
-        if (!all) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[b][i] = wh_kv4_sees(pos, key0 + 16 * b + 4 * g + i, a.window, a.first) ? s[b][i] : kMinusInf;
-        }
+        if (!all) kv_mask(s, pos, key0 + 4 * g, a.window, a.first);
         float top = kMinusInf;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
@@ -1404,14 +1438,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         // -inf where a row does not see this lane's keys
         const uint32_t key0 = wh_kv4_run(tile, run);
         const bool all = (int32_t)key0 + 63 <= pos_lo && tile.rows == kRows && (!a.window || (int64_t)key0 + a.window > pos_hi);
-        if (!all) {
-            const int32_t pos = row_pos[row0];
-#pragma unroll
-            for (int i = 0; i < 4 * kKeyBlocks; ++i) {
-                const uint32_t key = key0 + 16 * (kKeyBlocks * kq + (i >> 2)) + 4 * g + (i & 3);
-                s[i >> 2][i & 3] = wh_kv4_sees(pos, key, a.window, a.first) ? s[i >> 2][i & 3] : kMinusInf;
-            }
-        }
+        if (!all) kv_mask(s, row_pos[row0], key0 + 16 * kKeyBlocks * kq + 4 * g, a.window, a.first);
         if constexpr (!kLatent) {
             const uint64_t nan = nan_keys[run % 3];
             if (__builtin_expect(nan != 0, 0)) {

@@ -90,11 +90,6 @@ WH_KV_HD uint32_t wh_kv4_seen(const wh_kv4_tile& t, uint32_t key0, uint32_t key)
     return key < t.first ? key : in;
 }
 
-// Whether a token at position pos (negative: none) sees a key.
-WH_KV_HD bool wh_kv4_sees(int32_t pos, uint32_t key, uint32_t window, uint32_t first) {
-    return (int64_t)key <= pos && (!window || key < first || (int64_t)key + window > pos);
-}
-
 // How a call whose tiles are fewer than its workgroups cuts up their keys.  Of
 // request b, n_q tokens on len rows: tiles, and at most how many runs each has.
 WH_KV_HD uint32_t wh_kv4_tiles(uint32_t n_q, uint32_t group, uint32_t tile_rows) {
