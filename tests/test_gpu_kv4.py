@@ -420,7 +420,7 @@ class Case:
                 km = torch.where(see, k.abs().amax(1)[None], 0.0).amax(1)
                 vm = torch.where(see, v.abs().amax(1)[None], 0.0).amax(1)
                 cnt = see.sum(1)
-                delta = self.scale * ((d + 12) * U * ab + (8 if self.bf16 else 1) * d * U * q[:, h].abs().amax(1) * km)
+                delta = abs(self.scale) * ((d + 12) * U * ab + (8 if self.bf16 else 1) * d * U * q[:, h].abs().amax(1) * km)
                 rel = 2 * delta + 4 * U * big + (2 * cnt + 16) * U + (2.0 ** -11 if self.bf16 else 2.0 ** -22)
                 tol[:, h] = rel[:, None] * W + ((2 * cnt + 8) * U * vm)[:, None] + (2.0 ** -8 if self.bf16 else 4 * U) * out[:, h].abs()
             outs.append(out.flatten(1))
@@ -621,6 +621,127 @@ def test_results_repeat_bit_for_bit(ctx):
         for _ in range(5):
             c.out.fill_(7.0)
             assert torch.equal(c.run(ctx), first)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layout,q", [("latent", [1]), ("latent", [40]), ("group_8", [3]), ("group_8", [90]), ("latent_64", [50])])
+def test_keys_that_are_not_finite_in_long_lists(ctx, layout, q, bf16):
+    """The same past the first run of keys, in both kinds of tile: NaN reaches
+    the tokens whose window holds the key and no others."""
+    n, window = 400, 100
+    for key in (150, 310, 396):
+        for plane in (0, -1):
+            c = Case(q, [n], *LAYOUTS[layout], bf16, window=window, page=64)
+            ref = c.run(ctx).clone()
+            slot = int(c.slots[0][key])
+            c.cache.planes[plane][1][slot // c.page, 0, slot % c.page, -1] = 255
+            c.out.fill_(7.0)
+            got = c.run(ctx)
+            pos = n - q[0] + torch.arange(q[0], device="cuda")
+            sees = (pos >= key) & (pos - window < key)
+            g = c.heads // c.kv_heads
+            nan = torch.isnan(got.reshape(q[0], c.heads, c.d))
+            assert bool(nan[sees, :g].all()) and not bool(nan[~sees].any()) and not bool(nan[:, g:].any())
+            assert torch.equal(got[~sees], ref[~sees])
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layout,q", [("group_8", [1]), ("group_8", [60]), ("pairs", [2]), ("group_5", [30]), ("wide", [1]), ("group_40", [4])])
+def test_value_scales_that_rise(ctx, layout, q, bf16):
+    """Values that grow with the key by 2^40 over the list, so that what was
+    added up is taken against a new reference many times."""
+    c = Case(q, [500], *LAYOUTS[layout], bf16, page=64, sink=True)
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((500, c.kv_heads * c.d)) * np.exp2(np.arange(500) * 40 // 500 - 20.0)[:, None]
+    c.cache.fill(1, c.slots[0], x)
+    c.check(ctx)
+
+
+@pytest.mark.parametrize("requests", [70, 200, 300])
+def test_many_requests_with_none_between(ctx, requests):
+    """Lengths from 0 to some thousands, tokens from none to three, over and
+    under the number of requests that a split counts."""
+    rng = np.random.default_rng(requests)
+    q = [int(v) for v in rng.integers(0, 4, requests)]
+    q[0], q[-1] = 0, 0
+    lens = [max(n, int(v)) for n, v in zip(q, np.exp2(rng.uniform(0, 9, requests)))]
+    lens[requests // 2] = 4000
+    q[requests // 2] = 2
+    for layout in ("group_8", "latent_64"):
+        Case(q, lens, *LAYOUTS[layout], True, page=32, behind=3).check(ctx)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30])
+@pytest.mark.parametrize("layout,q", [("latent", [2]), ("group_8", [1]), ("group_8", [70])])
+def test_other_scales(ctx, layout, q, scale):
+    for bf16 in (False, True):
+        c = Case(q, [200], *LAYOUTS[layout], bf16, window=150, first=3, sink=True)
+        c.scale = float(np.float32(scale))
+        c.check(ctx)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layout,q,lens,window,first", [
+    ("group_8", [1], [6000], 3000, 0), ("group_8", [3, 1], [6000, 100], 2500, 130), ("latent", [1], [3000], 1000, 64),
+    ("latent", [2], [3000], 1500, 7), ("latent_16", [1, 1], [5000, 64], 4095, 1)])
+def test_windows_of_split_lists(ctx, layout, q, lens, window, first, bf16):
+    Case(q, lens, *LAYOUTS[layout], bf16, page=64, window=window, first=first).check(ctx)
+
+
+@pytest.mark.parametrize("page", [8, 64, 256])
+@pytest.mark.parametrize("layout,q", [("group_8", [1]), ("group_8", [70]), ("latent", [1, 3]), ("latent", [1])])
+@pytest.mark.parametrize("window,first", [(100, 0), (100, 5), (300, 70), (65, 64)])
+def test_pages_that_no_token_sees_need_no_entry(ctx, layout, q, page, window, first):
+    lens = [1111, 700][:len(q)]
+    c = Case(q, lens, *LAYOUTS[layout], False, page=page, window=window, first=first)
+    tables = u32(c.tables).reshape(len(q), -1)
+    for b, (nq, n) in enumerate(zip(q, lens)):
+        seen = np.zeros(n, bool)
+        seen[:first] = True
+        seen[max(0, n - nq + 1 - window):] = True
+        for p in range(-(-n // page)):
+            if not seen[p * page:(p + 1) * page].any():
+                tables[b, p] = 0xFFFFFFFF - p
+    c.tables = i32(tables)
+    c.check(ctx)
+
+
+def test_graphs_that_share_scratch(ctx):
+    """Two captured calls whose key lists are split use the same scratch: in
+    any order, with an eager one between, each gives its own result."""
+    cases = [Case([1], [5000], *LAYOUTS["group_8"], True, page=64), Case([1, 1], [3000, 900], *LAYOUTS["latent"], False, page=16),
+             Case([2], [2500], *LAYOUTS["group_5"], False, page=64)]
+    want = [c.run(ctx).clone() for c in cases]
+    graphs = [ctx.graph_capture(lambda c=c: ctx.kv4_attention_async(c.cache.c, c.d_)) for c in cases[:2]]
+    for order in ((0, 1), (1, 0), (0, 0), (1, 1)):
+        for c in cases:
+            c.out.fill_(7.0)
+        torch.cuda.synchronize()
+        for k in order:
+            ctx.graph_launch(graphs[k])
+        ctx.kv4_attention_async(cases[2].cache.c, cases[2].d_)
+        done(ctx)
+        assert torch.equal(cases[2].out, want[2])
+        for k in set(order):
+            assert torch.equal(cases[k].out, want[k])
+    for g in graphs:
+        ctx.graph_release(g)
+
+
+def test_two_contexts_at_once():
+    """Each context has its own stream and scratch."""
+    with wa.Context(0) as one, wa.Context(0) as two:
+        cases = [Case([1], [5000], *LAYOUTS["group_8"], True, page=64), Case([1], [4000], *LAYOUTS["latent"], True, page=64)]
+        want = [c.run(one).clone() for c in cases]
+        for _ in range(4):
+            for c in cases:
+                c.out.fill_(7.0)
+            torch.cuda.synchronize()
+            for c, k in zip(cases, (one, two)):
+                k.kv4_attention_async(c.cache.c, c.d_)
+            done(one)
+            done(two)
+            assert all(torch.equal(c.out, w) for c, w in zip(cases, want))
 
 
 # ------------------------------------------------------- the calls together

@@ -54,8 +54,8 @@ struct wh_kv4_attn_args {
     uint32_t n_tokens, n_requests, group, window, first;
     uint32_t n_tiles;     // slots or tiles, at most
     uint32_t units;       // workgroups of a key head, at most; > n_tiles: their keys are cut up
-    uint32_t min_runs;  // that a workgroup takes
-    bool wide;          // tiles of 64 (f32: 32) rows instead of 16
+    uint32_t min_runs;    // runs of 64 keys that a part of a tile has at least
+    bool wide;            // tiles of 64 (f32: 32) rows instead of 16
     float scale_log2;   // scale * log2(e)
     uint32_t* status;
 };
@@ -65,5 +65,6 @@ struct wh_kv4_attn_plan {
     bool wide;
     size_t part_bytes;  // scratch for partial results, 0 for one split
 };
-wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, bool latent, size_t max_len);
+wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, size_t max_len);
+hipError_t wh_kv4_setup();  // once for each device, before the first launch there
 hipError_t wh_kv4_attn_launch(const wh_kv4_attn_args& a, bool bf16, bool latent, hipStream_t stream);

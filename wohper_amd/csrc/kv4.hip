@@ -16,10 +16,7 @@
 namespace {
 
 typedef _Float16 wh_h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 wh_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 wh_h8 __attribute__((ext_vector_type(8)));
-typedef short wh_s4 __attribute__((ext_vector_type(4)));
-typedef __fp16 wh_hh4 __attribute__((ext_vector_type(4)));
 typedef int wh_i8 __attribute__((ext_vector_type(8)));
 typedef int wh_i2 __attribute__((ext_vector_type(2)));
 typedef int wh_i4 __attribute__((ext_vector_type(4)));
@@ -165,9 +162,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
 
 // ------------------------------------------------------------- rows in, out
 
-__device__ __forceinline__ uint32_t kv_quad_max(uint32_t v) {
-    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, false));
-    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, false));
+// Max over groups of 2, 4 or 8 lanes next to each other, in all of them.
+template <int kN>
+__device__ __forceinline__ uint32_t kv_near_max(uint32_t v) {
+    auto with = [&](uint32_t other) { v = max(v, other); };
+    with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));                  // lanes 1 0 3 2 of a quad
+    if constexpr (kN >= 4) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));   // 2 3 0 1
+    if constexpr (kN >= 8) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));  // 7 - lane of eight
+    return v;
 }
 
 // Where 8 values of a row lie in a plane: piece of 8 within the row of a slot.
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(256) k_kv4_write(wh_kv4_rows_args a) {
     uint32_t top = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
-    top = kv_quad_max(top);
+    top = kv_near_max<4>(top);
     // 1.m * 2^(E - 127) <= 6 * 2^e = 1.5 * 2^(e + 2): e = E - 129, one more when 1.m > 1.5
     const uint32_t exp = top >> 23;
     uint32_t byte = exp < 3 ? 1 : exp - 2 + ((top & 0x7fffffu) > 0x400000u);
@@ -277,20 +279,20 @@ __global__ void __launch_bounds__(256) k_kv4_read(wh_kv4_rows_args a) {
 // -------------------------------------------------------------- attention
 //
 // A request's queries are rows (token, head of the group) of one key head,
-// flattened; a workgroup takes a tile of 16 of them and a run of the keys that
-// any of them sees, and adds weights and values in one pass with the running
-// maximum.  Softmax in powers of two: w = 2^(s * scale * log2(e) - m).
+// flattened; a workgroup takes a tile of them and a part of the keys that any of
+// them sees, and adds weights and values in one pass with the running maximum.
+// Softmax in powers of two: w = 2^(s * scale * log2(e) - m).
 //
-// Numbers: both factors of every product go to f16 matrix instructions, whose
-// products are exact in their f32 sums.  A cached row is taken relative to its
-// largest scale byte (code * 2^(byte - largest): exact in f16 down to 2^-23 of
-// that, below which f32 would lose it too), the power of two returns to the
-// score in f32.  A query row is scaled by a power of two so that its largest
-// value is 2^13..2^14: a bf16 query is exact in one f16 unless 2^-28 of that,
-// an f32 query takes two (22 bits, and 2^-38 of the largest).  A weight times
-// its value row's power of two is rounded to one f16 (11 bits, one more than
-// a bf16 output keeps beside its sign) or, for f32, split into two.  Maxima,
-// sums of weights and outputs are f32.
+// Numbers.  Scores, bf16: the codes as they lie and the query as two E4M3 parts
+// with a power of two for every 32 values (together 2^-9 of a value, and 8 u of
+// the largest of the 32), in the scaled matrix instruction; products are exact in
+// its f32 sums.  f32: keys decoded to f16 against their row's largest scale byte
+// (exact down to 2^-23 of that, below which f32 would lose them too) and the
+// query as two f16 parts (22 bits, and 2^-38 of its largest value).  Outputs, bf16:
+// values against the largest scale byte so far (f16 down to 2^-24 of it), weights
+// as one f16 (11 bits, one more than a bf16 output keeps beside its sign).  f32:
+// values against their row's largest byte, weights times that row's power of two
+// in two f16 parts.  Maxima, sums of weights and outputs are f32.
 
 #define kMinusInf (-__builtin_inff())
 constexpr float kMinusBig = -1.0e30f;  // the maximum of no key: finite, so that differences are
@@ -448,7 +450,7 @@ __device__ __forceinline__ void kv_mask(wh_f4 (&s)[kN], int32_t pos, uint32_t ke
 #pragma unroll
         for (int b = 0; b < kN; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][i] = (16 * b + i > near) | (16 * b + i < early) ? s[b][i] : kMinusInf;
+            for (int i = 0; i < 4; ++i) s[b][i] = ((16 * b + i > near) | (16 * b + i < early)) ? s[b][i] : kMinusInf;
     }
 }
 
@@ -558,16 +560,6 @@ __device__ __forceinline__ float kv_value_scale(uint32_t vtop, int ref) {
 template <int HD>
 __device__ __forceinline__ int kv_dim(int s, uint32_t g) {
     return HD >= 128 ? 32 * (4 * (s >> 2) + (int)g) + 8 * (s & 3) : 32 * ((int)g & 1) + 16 * ((int)g >> 1) + 8 * s;
-}
-
-// Max over groups of 2, 4 or 8 lanes next to each other, in all of them.
-template <int kN>
-__device__ __forceinline__ uint32_t kv_near_max(uint32_t v) {
-    auto with = [&](uint32_t other) { v = max(v, other); };
-    with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));                  // lanes 1 0 3 2 of a quad
-    if constexpr (kN >= 4) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));   // 2 3 0 1
-    if constexpr (kN >= 8) with((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));  // 7 - lane of eight
-    return v;
 }
 
 // Max over groups of sixteen lanes, in all of them.
@@ -1630,21 +1622,32 @@ hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
     const dim3 grid((split ? a.units : a.n_tiles) * a.s.kv_heads);
     if (a.wide) {
         using W = wh_kv4_packed<HD, kF32, kLatent>;
-        static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn_packed<HD, kF32, kLatent>,
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)W::kLds);
-        if (set != hipSuccess) return set;
         k_kv4_attn_packed<HD, kF32, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
         if (split)
             k_kv4_join<HD, kF32, W::kRows><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
         return hipGetLastError();
     }
     constexpr size_t lds = wh_kv4_narrow<HD, kF32>::kLds;
-    static const hipError_t set = hipFuncSetAttribute((const void*)k_kv4_attn<HD, kF32, kLatent>,
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (set != hipSuccess) return set;
     k_kv4_attn<HD, kF32, kLatent><<<grid, 256, lds, stream>>>(a);
     if (split) k_kv4_join<HD, kF32, 16><<<dim3(a.n_tiles * a.s.kv_heads, 4), 256, 0, stream>>>(a);
     return hipGetLastError();
+}
+
+// Dynamic LDS above the default.
+template <int HD, bool kF32, bool kLatent>
+hipError_t attn_setup_of() {
+    const hipError_t e = hipFuncSetAttribute((const void*)k_kv4_attn_packed<HD, kF32, kLatent>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)wh_kv4_packed<HD, kF32, kLatent>::kLds);
+    if (e != hipSuccess) return e;
+    return hipFuncSetAttribute((const void*)k_kv4_attn<HD, kF32, kLatent>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)wh_kv4_narrow<HD, kF32>::kLds);
+}
+template <int HD>
+hipError_t attn_setup_hd() {
+    for (const hipError_t e : {attn_setup_of<HD, false, false>(), attn_setup_of<HD, false, true>(), attn_setup_of<HD, true, false>(),
+                               attn_setup_of<HD, true, true>()})
+        if (e != hipSuccess) return e;
+    return hipSuccess;
 }
 
 template <int HD>
@@ -1654,6 +1657,12 @@ hipError_t attn_launch_hd(const wh_kv4_attn_args& a, bool bf16, bool latent, hip
 }
 
 }  // namespace
+
+hipError_t wh_kv4_setup() {
+    for (const hipError_t e : {attn_setup_hd<64>(), attn_setup_hd<128>(), attn_setup_hd<256>(), attn_setup_hd<512>()})
+        if (e != hipSuccess) return e;
+    return hipSuccess;
+}
 
 hipError_t wh_kv_plan_launch(const wh_kv_plan_args& a, hipStream_t stream) {
     const size_t lds = 3 * ((size_t)a.n + 1) * sizeof(uint32_t);
@@ -1680,20 +1689,27 @@ hipError_t wh_kv4_read_launch(const wh_kv4_rows_args& a, bool bf16, hipStream_t 
     return hipGetLastError();
 }
 
-wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, bool latent, size_t max_len) {
-    (void)latent;
+// Tiles of 64 rows (f32: 32) where requests have 48 rows (16) on average, else of
+// 16, whose product wastes less and whose waves wait for nobody.  @@RULE@@
+//
+// Where there are less than half as many tiles as workgroups the chip holds, keys
+// are cut up.  Workgroups aimed at: one for each that is resident at once (LDS and
+// registers allow one a CU from 256 dims on), but two rounds for narrow tiles of
+// up to 128 dims, which even out what requests of different lengths leave over:
+// 32 requests of up to 8192 keys, 8 key heads of 128: 79, 74, 73 and 83 us for
+// 512, 768, 1024 and 2048.
+wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, size_t max_len) {
     wh_kv4_attn_plan p{};
     const uint64_t rows = (uint64_t)a.n_tokens * a.group;
     const uint32_t wide_rows = bf16 ? 64 : 32;
     p.wide = rows >= (uint64_t)a.n_requests * (wide_rows - 16);
-    const uint32_t tile_rows = p.wide ? wide_rows : 16, block = 64;
+    const uint32_t tile_rows = p.wide ? wide_rows : 16;
     p.n_tiles = (uint32_t)wh_kv4_tile_slots(a.n_tokens, a.n_requests, a.group, tile_rows);
-    // more workgroups than tiles: the keys are cut up by the lengths on the device
     uint64_t keys = max_len;
     if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.first + a.n_tokens);
-    const uint64_t resident = p.wide && a.s.head_dim >= 256 ? 256 : a.s.head_dim >= 512 ? 256 : a.s.head_dim == 256 ? 512 : p.wide ? 512 : 1024;
-    p.min_runs = 128 / block;
-    p.units = (uint32_t)(resident / a.s.kv_heads);
+    const uint32_t aim = a.s.head_dim >= 512 || (p.wide && a.s.head_dim >= 256) ? 256 : p.wide || a.s.head_dim >= 256 ? 512 : 1024;
+    p.min_runs = 2;  // a workgroup's start and end cost as much
+    p.units = aim / a.s.kv_heads;
     const uint64_t busy = std::max<uint64_t>(rows / tile_rows, a.n_requests);  // tiles, where every request has rows
     if (p.units < 2 * busy || a.n_requests > WH_KV_SPLIT_REQUESTS || keys <= 128) p.units = 0;
     p.units = std::max(p.units, p.n_tiles);

@@ -2102,6 +2102,7 @@ int wh_init(int device, wh_ctx** out) {
     if (e == hipSuccess) e = hipEventCreate(&c->timer[1]);
     if (e == hipSuccess)
         e = c->attn_max.ensure((size_t)WH_POS_BATCH * WH_ATTN_MX_HEADS * WH_ATTN_MX_TILES * sizeof(float), false);
+    if (e == hipSuccess) e = wh_kv4_setup();
     if (e == hipSuccess) e = c->kv4_ticket.ensure(sizeof(uint32_t), true);
     if (e != hipSuccess) {
         delete c;
@@ -4806,7 +4807,7 @@ int wh_kv4_attention_async(wh_ctx* c, const wh_kv4_cache* cache, const wh_kv4_at
     a.first = (uint32_t)std::min<size_t>(d->first, 0x7fffffffu);
     a.scale_log2 = d->scale * 1.44269504088896340736f;
     a.status = c->status;
-    const wh_kv4_attn_plan p = wh_kv4_attn_plan_of(a, d->is_bf16 != 0, !has_v, d->max_len);
+    const wh_kv4_attn_plan p = wh_kv4_attn_plan_of(a, d->is_bf16 != 0, d->max_len);
     a.units = p.units;
     a.min_runs = p.min_runs;
     a.n_tiles = p.n_tiles;
