@@ -1620,16 +1620,18 @@ template <int HD, bool kF32, bool kLatent>
 hipError_t attn_launch_of(const wh_kv4_attn_args& a, hipStream_t stream) {
     const bool split = a.units > a.n_tiles;
     const dim3 grid((split ? a.units : a.n_tiles) * a.s.kv_heads);
-    if (a.wide) {
+    constexpr bool kAlways = kF32 && HD == 512;  // wide, as wh_kv4_attn_plan_of has it
+    if (kAlways || a.wide) {
         using W = wh_kv4_packed<HD, kF32, kLatent>;
         k_kv4_attn_packed<HD, kF32, kLatent><<<grid, W::kThreads, W::kLds, stream>>>(a);
         if (split)
             k_kv4_join<HD, kF32, W::kRows><<<dim3(a.n_tiles * a.s.kv_heads, W::kRows / 4), 256, 0, stream>>>(a);
         return hipGetLastError();
     }
-    constexpr size_t lds = wh_kv4_narrow<HD, kF32>::kLds;
-    k_kv4_attn<HD, kF32, kLatent><<<grid, 256, lds, stream>>>(a);
-    if (split) k_kv4_join<HD, kF32, 16><<<dim3(a.n_tiles * a.s.kv_heads, 4), 256, 0, stream>>>(a);
+    if constexpr (!kAlways) {
+        k_kv4_attn<HD, kF32, kLatent><<<grid, 256, wh_kv4_narrow<HD, kF32>::kLds, stream>>>(a);
+        if (split) k_kv4_join<HD, kF32, 16><<<dim3(a.n_tiles * a.s.kv_heads, 4), 256, 0, stream>>>(a);
+    }
     return hipGetLastError();
 }
 
@@ -1638,9 +1640,11 @@ template <int HD, bool kF32, bool kLatent>
 hipError_t attn_setup_of() {
     const hipError_t e = hipFuncSetAttribute((const void*)k_kv4_attn_packed<HD, kF32, kLatent>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)wh_kv4_packed<HD, kF32, kLatent>::kLds);
-    if (e != hipSuccess) return e;
-    return hipFuncSetAttribute((const void*)k_kv4_attn<HD, kF32, kLatent>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)wh_kv4_narrow<HD, kF32>::kLds);
+    if constexpr (!(kF32 && HD == 512))
+        if (e == hipSuccess)
+            return hipFuncSetAttribute((const void*)k_kv4_attn<HD, kF32, kLatent>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)wh_kv4_narrow<HD, kF32>::kLds);
+    return e;
 }
 template <int HD>
 hipError_t attn_setup_hd() {
@@ -1689,29 +1693,42 @@ hipError_t wh_kv4_read_launch(const wh_kv4_rows_args& a, bool bf16, hipStream_t 
     return hipGetLastError();
 }
 
-// Tiles of 64 rows (f32: 32) where requests have 48 rows (16) on average, else of
-// 16, whose product wastes less and whose waves wait for nobody.  @@RULE@@
+// Wide tiles, of 64 rows (f32: 32), against narrow ones of 16, whose product wastes
+// less where a request has few rows and whose waves wait for nobody; by the rows
+// (tokens x heads of a key head) that requests have on average.  us, 16 requests of
+// one token and up to 6000 keys, narrow against wide:
+//  - f32, 512 dims: always wide.  8 rows 40.0 and 31.3, 64 rows 73.3 and 47.3;
+//  - from 256 dims on: over 16 rows.  bf16, 4 key heads of 256: 16 rows 35.8 and
+//    55.8, 24 rows 61.0 and 57.2, 64 rows 79.2 and 57.4; f32: 42.0 and 57.3, 73.6
+//    and 58.3, 102.6 and 102.4; bf16, one of 512: 34.4 and 33.5, 36.8 and 36.4,
+//    49.7 and 41.2;
+//  - up to 128 dims: bf16 over 48 rows, f32 over 64.  bf16, 8 key heads of 128: 48
+//    rows 53.5 and 58.2, 64 rows 57.7 and 56.0; f32: 48 rows 81.6 and 102.0, 64
+//    rows 86.4 and 92.9.  4 prompts of 2000 tokens, 4 rows a token: bf16 298 and
+//    161, f32 381 and 300.
 //
-// Where there are less than half as many tiles as workgroups the chip holds, keys
-// are cut up.  Workgroups aimed at: one for each that is resident at once (LDS and
-// registers allow one a CU from 256 dims on), but two rounds for narrow tiles of
-// up to 128 dims, which even out what requests of different lengths leave over:
-// 32 requests of up to 8192 keys, 8 key heads of 128: 79, 74, 73 and 83 us for
-// 512, 768, 1024 and 2048.
+// With few tiles their keys are cut up.  Workgroups aimed at: those that the chip
+// holds at once; twice as many where that is less than four a tile, since whole
+// parts of requests of different lengths do not come out even (32 requests of up to
+// 8192 keys, 8 key heads of 128: 79, 74, 73 and 83 us for one, one and a half, two
+// and four rounds; 16 of up to 6000 with two wide tiles each, f32: 153 and 102 for
+// one and two); none where two rounds are less than three a tile (96 windows of
+// 1024 keys, 8 key heads: 41 us a workgroup a tile, 67 us cut up).
 wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, size_t max_len) {
     wh_kv4_attn_plan p{};
     const uint64_t rows = (uint64_t)a.n_tokens * a.group;
     const uint32_t wide_rows = bf16 ? 64 : 32;
-    p.wide = rows >= (uint64_t)a.n_requests * (wide_rows - 16);
+    const uint32_t narrow_rows = a.s.head_dim >= 512 && !bf16 ? 0 : a.s.head_dim >= 256 ? 16 : bf16 ? 48 : 64;
+    p.wide = rows > (uint64_t)a.n_requests * narrow_rows;
     const uint32_t tile_rows = p.wide ? wide_rows : 16;
     p.n_tiles = (uint32_t)wh_kv4_tile_slots(a.n_tokens, a.n_requests, a.group, tile_rows);
     uint64_t keys = max_len;
     if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.first + a.n_tokens);
-    const uint32_t aim = a.s.head_dim >= 512 || (p.wide && a.s.head_dim >= 256) ? 256 : p.wide || a.s.head_dim >= 256 ? 512 : 1024;
+    const uint32_t resident = (p.wide ? a.s.head_dim >= 256 ? 256 : 768 : a.s.head_dim >= 256 ? 256 : 512) / a.s.kv_heads;
     p.min_runs = 2;  // a workgroup's start and end cost as much
-    p.units = aim / a.s.kv_heads;
     const uint64_t busy = std::max<uint64_t>(rows / tile_rows, a.n_requests);  // tiles, where every request has rows
-    if (p.units < 2 * busy || a.n_requests > WH_KV_SPLIT_REQUESTS || keys <= 128) p.units = 0;
+    p.units = resident < 4 * busy ? 2 * resident : resident;
+    if (p.units < 3 * busy || a.n_requests > WH_KV_SPLIT_REQUESTS || keys <= 64 * (2 * p.min_runs - 1)) p.units = 0;
     p.units = std::max(p.units, p.n_tiles);
     if (p.units > p.n_tiles) p.part_bytes = (size_t)p.units * a.s.kv_heads * tile_rows * (a.s.head_dim + 2) * sizeof(float);
     return p;
