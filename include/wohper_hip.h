@@ -910,7 +910,8 @@ int wh_kv4_read_async(wh_ctx* ctx, const wh_kv4_cache* cache, const uint32_t* sl
  * max_len: at least the largest of lens_dev; it only sizes the split of long
  * key lists and the context's scratch for it, not the result.  A table entry
  * of n_pages or more, or a length above table_stride * page_size, reports
- * WH_NOT_RESIDENT.  A visible row that holds NaN makes its heads' outputs NaN;
+ * WH_NOT_RESIDENT; entries of pages that no token sees a row of are not looked
+ * at, so pages behind a window can be given back.  A visible row that holds NaN makes its heads' outputs NaN;
  * rows that are not visible do nothing, whatever their bytes.
  * Sums are f32 in both types and in both numerics modes; an f32 result is
  * within a few units of f32 rounding of the sums' size. */

@@ -19,6 +19,11 @@ include/wohper_hip.h (libwohper_hip.so, built from wohper_amd/csrc):
   load_optional_expert_pack        model_format.rs:458         model_format.load_optional_expert_pack
   route_experts_from_dense_block   compute.rs:2129             Context.store_router + Context.route_experts
 
+The paged 4-bit attention cache has no counterpart there: Context.kv_plan_async
+(lengths to pages and slots), kv4_write_async and kv4_read_async (rows in and
+out) and kv4_attention_async (decode, verify and prefill over the cached rows)
+with the descriptors WhKvPlan, WhKv4Cache and WhKv4Attention.
+
 The slice-based functions upload the weights for the call, as the reference
 reads them from its I/O buffers; the resident path (Context.store_* plus the
 handle-based methods) keeps them in HBM.  There is no CPU fallback: without
