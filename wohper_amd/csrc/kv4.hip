@@ -27,9 +27,24 @@ __device__ __forceinline__ float kv_bits(uint32_t u) { return __uint_as_float(u)
 
 // ------------------------------------------------------------------- plan
 
-__device__ __forceinline__ uint64_t kv_shfl_up64(uint64_t v, uint32_t d) {
-    const uint32_t lo = __shfl_up((uint32_t)v, d, 64), hi = __shfl_up((uint32_t)(v >> 32), d, 64);
-    return ((uint64_t)hi << 32) | lo;
+// Sum over this lane and those before it: within rows of 16, then over the rows.
+template <int kFrom, int kRows>
+__device__ __forceinline__ uint64_t kv_scan_step(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kFrom, kRows, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), kFrom, kRows, 0xf, false);
+    return v + ((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ uint64_t kv_scan(uint64_t v) {
+    v = kv_scan_step<0x111, 0xf>(v);  // 1, 2, 4, 8 lanes before
+    v = kv_scan_step<0x112, 0xf>(v);
+    v = kv_scan_step<0x114, 0xf>(v);
+    v = kv_scan_step<0x118, 0xf>(v);
+    v = kv_scan_step<0x142, 0xa>(v);  // the end of the row before
+    return kv_scan_step<0x143, 0xc>(v);  // the end of the first half
+}
+__device__ __forceinline__ uint64_t kv_lane(uint64_t v, uint32_t lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
 
 // Last index i with prefix[i] <= x (prefix ascending, prefix[0] = 0 <= x).
@@ -50,8 +65,8 @@ constexpr uint32_t kPlanThreads = 1024;
 // of the outputs, so a plan is one launch whose workgroups wait for nobody.  A
 // page that a request takes is worked out where it is needed (its table entry,
 // each slot on it) instead of being read back from another workgroup's store.
-// Bound by latency: the prefix sums and one chain of dependent loads (8.7 us for
-// 64 requests, 14.5 for 512).
+// Bound by latency: the prefix sums and one chain of dependent loads (7.2 us for
+// 64 requests, 13.0 for 512).
 __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
     extern __shared__ __align__(16) uint32_t lds[];
     uint32_t* const tok = lds;                  // [n + 1]
@@ -59,7 +74,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
     uint32_t* const give = take + a.n + 1;      // [n + 1]
     __shared__ uint64_t wave_sum[3][kPlanThreads / 64];
     __shared__ uint32_t bad;
-    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint32_t count_in = *a.free_count, mask = (1u << a.shift) - 1u;
     if (t == 0) bad = 0;
     __syncthreads();
@@ -83,23 +98,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
     uint64_t incl[3];
 #pragma unroll
     for (int s = 0; s < 3; ++s) {
-        uint64_t v = run[s];
-        for (uint32_t d = 1; d < 64; d <<= 1) {
-            const uint64_t u = kv_shfl_up64(v, d);
-            if (lane >= d) v += u;
-        }
-        incl[s] = v;
-        if (lane == 63) wave_sum[s][wave] = v;
+        incl[s] = kv_scan(run[s]);
+        if (lane == 63) wave_sum[s][wave] = incl[s];
     }
     __syncthreads();
     uint64_t total[3];
 #pragma unroll
     for (int s = 0; s < 3; ++s) {
-        uint64_t before = 0, all = 0;
-        for (uint32_t w = 0; w < kPlanThreads / 64; ++w) {
-            if (w < wave) before += wave_sum[s][w];
-            all += wave_sum[s][w];
-        }
+        const uint64_t sum = lane < kPlanThreads / 64 ? wave_sum[s][lane] : 0, upto = kv_scan(sum);
+        const uint64_t all = kv_lane(upto, 63), before = kv_lane(upto - sum, wave);
         total[s] = all;
         uint32_t* const dst = s == 0 ? tok : s == 1 ? take : give;
         const uint64_t base = before + incl[s] - run[s];
@@ -322,26 +329,6 @@ __device__ __forceinline__ wh_kv4_tile kv_tile(const wh_kv4_attn_args& a, uint32
     const wh_kv4_tile r = wh_kv4_tile_of(x, lo, s0, s1, len, cap, a.group, a.window, a.first, kRows);
     if (r.ok && len > cap && threadIdx.x == 0) atomicOr(a.status, WH_ST_NOT_RESIDENT);
     return r;
-}
-
-// Sum over this lane and those before it: within rows of 16, then over the rows.
-template <int kFrom, int kRows>
-__device__ __forceinline__ uint64_t kv_scan_step(uint64_t v) {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kFrom, kRows, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), kFrom, kRows, 0xf, false);
-    return v + ((uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ uint64_t kv_scan(uint64_t v) {
-    v = kv_scan_step<0x111, 0xf>(v);  // 1, 2, 4, 8 lanes before
-    v = kv_scan_step<0x112, 0xf>(v);
-    v = kv_scan_step<0x114, 0xf>(v);
-    v = kv_scan_step<0x118, 0xf>(v);
-    v = kv_scan_step<0x142, 0xa>(v);  // the end of the row before
-    return kv_scan_step<0x143, 0xc>(v);  // the end of the first half
-}
-__device__ __forceinline__ uint64_t kv_lane(uint64_t v, uint32_t lane) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
 
 // What a workgroup does: a tile of one key head, and which of its blocks of
