@@ -911,10 +911,14 @@ int wh_kv4_read_async(wh_ctx* ctx, const wh_kv4_cache* cache, const uint32_t* sl
  * key lists and the context's scratch for it, not the result.  A table entry
  * of n_pages or more, or a length above table_stride * page_size, reports
  * WH_NOT_RESIDENT; entries of pages that no token sees a row of are not looked
- * at, so pages behind a window can be given back.  A visible row that holds NaN makes its heads' outputs NaN;
- * rows that are not visible do nothing, whatever their bytes.
- * Sums are f32 in both types and in both numerics modes; an f32 result is
- * within a few units of f32 rounding of the sums' size. */
+ * at, so pages behind a window can be given back.  A visible row that holds
+ * NaN makes its heads' outputs NaN.  A row that a token does not see takes
+ * nothing from that token's output, whatever its bytes, nor does one of no
+ * weight, nor do other dims: sums are f32 in both types and in both numerics
+ * modes, and an f32 result is within f32 rounding of the sums of w |v|, |v|
+ * being the largest of the value's group of 32 dims.  A tile of tokens some of
+ * which see a row whose groups are more than 2^9 apart, or whose largest is not
+ * within 2^40 of 1, takes many times as long. */
 typedef struct {
     const void* q_dev;
     size_t q_stride;

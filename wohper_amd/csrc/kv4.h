@@ -50,7 +50,7 @@ struct wh_kv4_attn_args {
     const uint32_t *starts, *lens, *tables;
     uint64_t table_stride;
     const float* sink;
-    float* part;        // [unit][kv head][rows][head_dim + 2]: normalised outputs, maxima, sums
+    float* part;        // [unit][kv head][rows][head_dim + 2]: normalised outputs, sums of weights (kv_put_sum)
     uint32_t n_tokens, n_requests, group, window, first;
     uint32_t n_tiles;     // slots or tiles, at most
     uint32_t units;       // workgroups of a key head, at most; > n_tiles: their keys are cut up

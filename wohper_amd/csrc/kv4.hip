@@ -19,7 +19,6 @@ typedef _Float16 wh_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 wh_h8 __attribute__((ext_vector_type(8)));
 typedef int wh_i8 __attribute__((ext_vector_type(8)));
 typedef int wh_i2 __attribute__((ext_vector_type(2)));
-typedef int wh_i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t wh_u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t wh_u4 __attribute__((ext_vector_type(4)));
 
@@ -298,16 +297,33 @@ __global__ void __launch_bounds__(256) k_kv4_read(wh_kv4_rows_args a) {
 // the largest of the 32), in the scaled matrix instruction; products are exact in
 // its f32 sums.  f32: keys decoded to f16 against their row's largest scale byte
 // (exact down to 2^-23 of that, below which f32 would lose them too) and the
-// query as two f16 parts (22 bits, and 2^-38 of its largest value).  Outputs, bf16:
-// values against the largest scale byte so far (f16 down to 2^-24 of it), weights
-// as one f16 (11 bits, one more than a bf16 output keeps beside its sign).  f32:
-// values against their row's largest byte, weights times that row's power of two
-// in two f16 parts.  Maxima, sums of weights and outputs are f32.
+// query as two f16 parts (22 bits, and 2^-38 of its largest value).  Outputs:
+// values are f16 against their row's largest scale byte, exact down to 2^-23 of it,
+// and that byte's power of two goes into the weight.  Weights are f16, times 2^8,
+// against a reference of each query row: the largest score plus value exponent of
+// the keys that this row sees.  So what a row does not see, or sees with no weight,
+// takes no bits from it.  bf16 calls take one f16 (11 bits, one more than a bf16
+// output keeps beside its sign), f32 calls two.  Sums of weights and of products
+// and references are f32.
+//
+// f16 ends 2^-33 below the reference.  A group of 32 dims that lies as high as its
+// row keeps 2^-33 of its largest term, one that lies 2^9 below it 2^-24, which is
+// what an f32 sum rounds a term by too.  Values past that (kNear), or whose powers
+// of two are too far from 1 for f32 sums of weights under such references (kLow,
+// kHigh), are left to kv_plain_part, which takes the workgroup's part in f32: ten
+// to thirty times as long, for rows no model is known to make.
 
 #define kMinusInf (-__builtin_inff())
-constexpr float kMinusBig = -1.0e30f;  // the maximum of no key: finite, so that differences are
-constexpr float kUp = 10.0f;           // weights are held times 2^10: f16 keeps small ones
-constexpr float kSlack = 5.0f;         // the maximum is raised once a score is 2^5 above it
+constexpr float kMinusBig = -1.0e30f;  // the reference of no key: finite, so that differences are
+// Weights are held times 2^kUp: f16 keeps small ones.  A row's reference is raised
+// to its largest score once a weight is past f16, 2^8 above: with 2^5 the prompts of
+// k_kv4_attn_packed took 290 us for 243.  Rows raise theirs by themselves: that
+// another one does changes nothing in a row's rounding.
+constexpr float kUp = 8.0f;
+constexpr float kMost = 65504.0f;
+constexpr uint32_t kApart = 0xffffffffu;  // past every run
+constexpr int kNear = 9;                  // a value group's scale byte is at most so far below its row's
+constexpr uint32_t kLow = 127 - 40, kHigh = 127 + 40;  // and the row's in here
 
 // The tile of slot x: a search over the requests, 64 candidates a step.
 template <int kRows>
@@ -541,9 +557,23 @@ __device__ __forceinline__ float kv_rel(const wh_kv4_raw<HD, kN>& r, int half, i
 __device__ __forceinline__ float kv_key_scale(uint32_t ktop, uint32_t vtop) {
     return ktop == 255 || vtop == 255 ? kv_bits(0x7fc00000u) : kv_bits(ktop << 23);
 }
-// A value row's power of two against the reference; finite.
-__device__ __forceinline__ float kv_value_scale(uint32_t vtop, int ref) {
-    return kv_bits((uint32_t)min(max((int)vtop - ref + 127, 0), 254) << 23);
+// The exponent byte that a value row's weights take, from its largest scale byte
+// (0: a row of zeros; 255: NaN, whose weights are NaN or 0).
+__device__ __forceinline__ uint32_t kv_value_top(uint32_t top) { return min(max(top, kLow), kHigh); }
+// A value group's scale against that: a power of two of at most 1, as f16, and 0
+// from 2^-15 on (kNear is less).
+__device__ __forceinline__ _Float16 kv_value_rel(uint32_t b, uint32_t vexp) {
+    union {
+        uint16_t u;
+        _Float16 h;
+    } x;
+    x.u = (uint16_t)((min(max((int)b - (int)vexp, -15), 0) + 15) << 10);
+    return x.h;
+}
+// Whether a group of a value row (top: its largest byte) is NaN or not held by f16
+// products.  Not where the group is zeros: byte 0.
+__device__ __forceinline__ bool kv_value_odd(uint32_t b, uint32_t top, uint32_t vexp) {
+    return (((int)b - (int)vexp < -kNear) | (vexp != top)) & (b != 0);
 }
 
 // First dim of a lane's eight in step s of the product with keys.
@@ -697,12 +727,138 @@ __device__ __forceinline__ float kv_max_groups(float v) {
     p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
 }
+// Sum over the wave, in all lanes.
+__device__ __forceinline__ float kv_wave_sum(float v) {
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) v += __shfl_xor(v, k, 64);
+    return v;
+}
 __device__ __forceinline__ float kv_sum_groups(float v) {
     typedef unsigned u2 __attribute__((ext_vector_type(2)));
     u2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
     p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// A power of two's exponent.
+__device__ __forceinline__ int kv_exponent(float power) { return (int)(__float_as_uint(power) >> 23) - 127; }
+
+// A part's sum of weights, l * 2^m, as a power of two and a factor in [.5, 1): by
+// it parts are compared, since references include the values' exponents.
+__device__ __forceinline__ void kv_put_sum(float* to, float m, float l) {
+    to[0] = m + (float)__builtin_amdgcn_frexp_expf(l);
+    to[1] = __builtin_amdgcn_frexp_mantf(l);
+}
+
+// A workgroup's part of a tile in plain f32: for values, or in f32 calls keys, that
+// f16 products do not hold (above).  A wave takes a row at a time, a lane a key of
+// its score and HD / 64 dims of its output.  The output is kept divided by the sum
+// of weights so far, so it stays within the values' size whatever that is.  Bound by
+// instruction issue: some 1.5 HD instructions of scores and 10 of outputs for a row
+// and 64 keys, where the tiles above decode a key once for all their rows.
+template <int HD, bool kF32, bool kLatent, int kRows>
+__device__ __forceinline__ void kv_plain_part(const wh_kv4_attn_args& a, const wh_kv4_place& place, uint32_t wave, uint32_t waves) {
+    constexpr int kPer = HD / 64;  // dims of a lane
+    const uint32_t lane = threadIdx.x & 63, kvh = place.head, pmask = (1u << a.s.shift) - 1u;
+    const wh_kv4_tile& tile = place.tile;
+    const uint32_t run0 = place.split ? place.split * place.chunk : 0, run1 = min(tile.runs, run0 + place.chunk);
+    const uint32_t* const table = a.tables + tile.request * a.table_stride;
+    bool bad = false;
+    for (uint32_t row = wave; row < tile.rows; row += waves) {
+        const uint32_t flat = tile.row0 + row, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
+        const int32_t pos = tile.len - (int32_t)tile.n_q + (int32_t)tok;
+        const uint64_t at_q = (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD;
+        float m = kMinusBig, l = 0.0f, o[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) o[i] = 0.0f;
+        for (uint32_t run = run0; run < run1; ++run) {
+            const uint32_t key0 = wh_kv4_run(tile, run), key = key0 + lane;
+            const bool sees = (int64_t)key <= pos && (!a.window || (int64_t)key > (int64_t)pos - a.window || key < a.first);
+            const uint32_t page = table[wh_kv4_seen(tile, key0, key) >> a.s.shift];
+            const bool out = page >= a.s.n_pages;
+            bad |= out;
+            const uint64_t line = wh_kv4_line(out ? 0 : page, kvh, key & pmask, a.s.kv_heads, a.s.shift);
+            float s = 0.0f;
+#pragma unroll 1
+            for (int n = 0; n < HD / 32; ++n) {
+                const wh_u4 codes = *(const wh_u4*)(a.k.codes + line * (HD / 2) + 16 * n);
+                const float scale = kv_bits((uint32_t)a.k.scales[line * (HD / 32) + n] << 23);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const wh_f2 k[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 0),
+                                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 1),
+                                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 2),
+                                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 3)};
+                    float q[8];
+                    if constexpr (kF32) {
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            const wh_f4 x = *(const wh_f4*)((const float*)a.q + at_q + 32 * n + 8 * i + 4 * d);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) q[4 * d + e] = x[e];
+                        }
+                    } else {
+                        const wh_u4 x = *(const wh_u4*)((const uint16_t*)a.q + at_q + 32 * n + 8 * i);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) q[e] = kv_bits(e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s = fmaf(q[e], e & 1 ? k[e >> 1].y : k[e >> 1].x, s);
+                }
+            }
+            if constexpr (!kLatent) {  // a value row that holds NaN makes all of the output NaN
+                bool nan = false;
+#pragma unroll 1
+                for (int n = 0; n < HD / 32; ++n) nan |= a.v.scales[line * (HD / 32) + n] == 255;
+                if (nan) s = kv_bits(0x7fc00000u);
+            }
+            s = sees ? s * a.scale_log2 : kMinusInf;
+            const float to = fmaxf(m, wh_wave_max(s)), f = l * __builtin_amdgcn_exp2f(m - to), w = __builtin_amdgcn_exp2f(s - to);
+            l = f + kv_wave_sum(w);
+            m = to;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l, p = w * inv;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) o[i] *= f * inv;
+            const uint64_t seen = __ballot(sees);
+#pragma unroll 8
+            for (int j = 0; j < 64; ++j) {  // rows that are not seen count as zeros
+                const uint64_t at = kv_lane(line, j);
+                const float pj = kv_bits((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(p), j));
+                const uint8_t* const codes = a.v.codes + at * (HD / 2) + lane * kPer / 2;
+                uint32_t code;
+                if constexpr (kPer == 8) code = *(const uint32_t*)codes;
+                else if constexpr (kPer == 4) code = *(const uint16_t*)codes;
+                else code = *codes;
+                const uint32_t byte = a.v.scales[at * (HD / 32) + lane * kPer / 32];
+                const float scale = kv_bits(seen >> j & 1 ? byte << 23 : 0u);
+                if constexpr (kPer == 1) {
+                    const wh_f2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 0);
+                    o[0] = fmaf(pj, lane & 1 ? v.y : v.x, o[0]);
+                } else {
+                    wh_static_for<kPer / 2>([&](auto ic) {
+                        constexpr int i = decltype(ic)::value;
+                        const wh_f2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, i);
+                        o[2 * i] = fmaf(pj, v.x, o[2 * i]);
+                        o[2 * i + 1] = fmaf(pj, v.y, o[2 * i + 1]);
+                    });
+                }
+            }
+        }
+        float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * kRows + row) * (HD + 2);
+        const bool whole = place.chunk >= tile.runs;
+        float f = 1.0f;
+        if (whole && a.sink && l > 0.0f) f = l / (l + __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - m));
+        const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD + lane * kPer;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (!whole) part[lane * kPer + i] = o[i];
+            else if constexpr (kF32) ((float*)a.out)[at + i] = o[i] * f;
+            else ((__bf16*)a.out)[at + i] = (__bf16)(o[i] * f);
+        }
+        if (!whole && lane == 0) kv_put_sum(part + HD, m, l);
+    }
+    if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
 }
 
 // Four waves share a tile of 16 rows; wave w takes the blocks of 64 keys w, w +
@@ -729,7 +885,8 @@ struct wh_kv4_narrow {
     static constexpr int kGroups = HD / 32, kRel = 72;       // f16 between groups of value scales
     static constexpr int kAtRel = 64 * kRow;                 // byte offsets in a wave's LDS
     static constexpr int kAtKeys = kAtRel + kGroups * kRel * 2;
-    static constexpr int kWave = kAtKeys + (kDirect ? 0 : 2 * 64 * 4);
+    static constexpr int kAtPow = kAtKeys + (kDirect ? 0 : 64 * 4);
+    static constexpr int kWave = kAtPow + 64 * 4;
     static constexpr size_t kLds = 4 * (size_t)kWave > 2 * 64 * (size_t)HD ? 4 * (size_t)kWave : 2 * 64 * (size_t)HD;
     using Query = wh_kv4_query<HD, 16, 4>;  // f32: as parts in LDS before the first block
     static_assert(!kF32 || (size_t)Query::kBytes <= kLds, "queries fit");
@@ -742,6 +899,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
     constexpr bool kDirect = W::kDirect;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float wave_m[4][16], wave_l[4][16], row_c[kF32 ? 16 : 1];
+    __shared__ uint32_t wave_apart[4];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
     const wh_kv4_place place = kv_place<16>(a, false);
     const uint32_t kvh = place.head;
@@ -826,23 +984,16 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
         }
     }
 
-    wh_f4 acc[HD / 16];  // [dim 16 f + 4g + i][row], times 2^(127 - ref)
+    wh_f4 acc[HD / 16];  // [dim 16 f + 4g + i][row]
 #pragma unroll
     for (int f = 0; f < HD / 16; ++f) acc[f] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
-    float m = kMinusBig, l = 0.0f;
-    int ref = 0;
-    auto raise_ref = [&](uint32_t top) {  // top: of this lane
-        top = kv_wave_max(top);
-        const int to = min((int)top + 3, 254);
-        const float f = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) acc[i] *= f;
-        ref = to;
-    };
+    float m = kMinusBig, l = 0.0f;  // of the row, in all its lanes: the reference, and this lane's sum of weights
+    bool apart = false;
 
     uint8_t* const mine = smem + wave * W::kWave;
     _Float16* const rel = (_Float16*)(mine + W::kAtRel);  // [group][16 g + 4 b + i of key 16 b + 4 g + i]
-    float* const key_s = (float*)(mine + W::kAtKeys);     // [keys', values'][key]
+    float* const key_s = (float*)(mine + W::kAtKeys);     // powers of two of keys
+    float* const pow_s = (float*)(mine + W::kAtPow);      // and of value rows
     // 16-byte chunk c of key's row lies at chunk c ^ swizzle: neither the rows that a store
     // meets (b fixed) nor those of a transposed read (g fixed) share banks
     auto swizzle = [](uint32_t key) {
@@ -851,67 +1002,34 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
     };
     const uint32_t tkey = 16 * (r16 >> 2) + 4 * g + (r16 & 3);  // this lane's source row of a transposed read
 
-    for (uint32_t blk = blk0 + wave; blk < blk1; blk += 4) {
+    uint32_t end = blk1;  // 0 once the values are apart: not a second way out, which costs registers
+    for (uint32_t blk = blk0 + wave; blk < end; blk += 4) {
         wh_f4 s[4];
         const uint32_t key0 = wh_kv4_run(tile, blk);
         kv_wave_order();
         wh_static_for<(int)kParts64>([&](auto pc) {
             constexpr int part = decltype(pc)::value;
-            uint32_t ktop[kHold], vtop[kHold];
-            uint32_t above = 0;
-#pragma unroll
-            for (int h = 0; h < kHold; ++h) {
-                const uint32_t my_key = key0 + 16 * (kHold * part + h) + r16;
-                const bool counts = wh_kv4_seen(tile, key0, my_key) == my_key;
-                if constexpr (kDirect) {
-                    const uint32_t b = kv_piece_scales(kLatent ? kr : vr, h, g);
-#pragma unroll
-                    for (int j = 0; j < kPieces; ++j) {
-                        const uint32_t e = (b >> (8 * j)) & 0xff;
-                        above = max(above, counts && e < 255 ? e : 0u);
-                    }
-                    ktop[h] = vtop[h] = b;
-                } else {
-                    ktop[h] = kv_top_byte(kr, h);
-                    vtop[h] = kLatent ? ktop[h] : kv_top_byte(vr, h);
-                    above = max(above, counts && vtop[h] < 255 ? vtop[h] : 0u);
-                }
-            }
-            if (__ballot((int)above > ref)) {
-                const int old = ref;
-                raise_ref(above);
-                if constexpr (part > 0) {  // what the earlier part left is against the old one
-                    const float f = kv_bits((uint32_t)max(old - ref + 127, 0) << 23);
-#pragma unroll
-                    for (int h = 0; h < kHold * part; ++h)
-                        if constexpr (kDirect) {
-#pragma unroll
-                            for (int j = 0; j < kPieces; ++j)
-                                if (HD > 64 || g < 2) rel[(4 * j + g) * W::kRel + 16 * (r16 >> 2) + 4 * h + (r16 & 3)] *= (_Float16)f;
-                        } else if (g == 0) {
-                            key_s[64 + 16 * h + r16] *= f;
-                        }
-                }
-            }
 #pragma unroll
             for (int h = 0; h < kHold; ++h) {
                 const int b = kHold * part + h;
                 const uint32_t key = 16 * b + r16, at = 16 * (r16 >> 2) + 4 * b + (r16 & 3);
-                // value scales, and the powers of two of keys and value rows where those are against their largest
-                if constexpr (kDirect) {
+                const auto& raw_v = kLatent ? kr : vr;
+                const uint32_t kbytes = kDirect ? kv_piece_scales(kr, h, g) : kv_top_byte(kr, h);
+                const uint32_t vbytes = kLatent && kDirect ? kbytes : kv_piece_scales(raw_v, h, g);
+                const uint32_t vtop = kLatent && !kDirect ? kbytes : kv_top_byte(raw_v, h), vexp = kv_value_top(vtop);
+                // value scales, and the powers of two of keys and value rows
+                bool odd = false;
 #pragma unroll
-                    for (int j = 0; j < kPieces; ++j) {
-                        const int e = (int)((vtop[h] >> (8 * j)) & 0xff) - ref;  // above ref only where it does not count
-                        if (HD > 64 || g < 2) rel[(4 * j + g) * W::kRel + at] = (_Float16)kv_bits((uint32_t)max(min(e, 0) + 127, 0) << 23);
-                    }
-                } else {
-                    if (g == 0) {
-                        key_s[key] = kv_key_scale(ktop[h], vtop[h]);
-                        key_s[64 + key] = kv_value_scale(vtop[h], ref);
-                    }
-#pragma unroll
-                    for (int j = 0; j < kPieces; ++j)
-                        if (HD > 64 || g < 2) rel[(4 * j + g) * W::kRel + at] = (_Float16)kv_rel(kLatent ? kr : vr, h, j, g, vtop[h]);
+                for (int j = 0; j < kPieces; ++j) {
+                    const uint32_t e = (vbytes >> (8 * j)) & 0xff;
+                    odd |= kv_value_odd(e, vtop, vexp);
+                    if (HD > 64 || g < 2) rel[(4 * j + g) * W::kRel + at] = kv_value_rel(e, vexp);
+                }
+                const uint64_t odds = __ballot(odd);
+                if (__builtin_expect(odds != 0, 0)) apart |= odd && vtop != 255 && wh_kv4_seen(tile, key0, key0 + key) == key0 + key;
+                if (g == 0) {
+                    pow_s[key] = kv_bits(vexp << 23);
+                    if constexpr (!kDirect) key_s[key] = kv_key_scale(kbytes, vtop);
                 }
                 // the value row's codes
                 uint8_t* const row = mine + key * W::kRow;
@@ -923,7 +1041,6 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                 // scores
                 s[b] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
                 if constexpr (kDirect) {
-                    const uint32_t scale = kLatent ? vtop[h] : kv_piece_scales(kr, h, g);
                     wh_static_for<kPieces>([&](auto jc) {
                         constexpr int j = decltype(jc)::value;
                         wh_i8 x;
@@ -931,7 +1048,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                         x[4] = x[5] = x[6] = x[7] = 0;
 #pragma unroll
                         for (int p = 1; p >= 0; --p)
-                            s[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, qx[j][p], s[b], 4, 0, j, scale, j,
+                            s[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, qx[j][p], s[b], 4, 0, j, kbytes, j,
                                                                                     q_scale - (p ? 0x04040404u : 0u));
                     });
                 } else {
@@ -939,7 +1056,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                     for (int k = 0; k < HD / 32; ++k) {
                         const int j = k / 4, w = k - j * 4;
                         const uint32_t codes = HD == 64 && g >= 2 ? kr.c[h][j][w + 2] : kr.c[h][j][w];
-                        const wh_h8 x = kv_decode(codes, kv_rel(kr, h, j, g, ktop[h]));
+                        const wh_h8 x = kv_decode(codes, kv_rel(kr, h, j, g, kbytes));
 #pragma unroll
                         for (int p = kParts - 1; p >= 0; --p)
                             s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qd[k][p], s[b], 0, 0, 0);
@@ -947,13 +1064,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                 }
                 // direct: a value row that holds NaN beside keys that do not
                 if constexpr (kDirect && !kLatent) {
-                    bool nan = false;
-#pragma unroll
-                    for (int j = 0; j < kPieces; ++j) nan |= ((vtop[h] >> (8 * j)) & 0xff) == 255;
-                    if (__builtin_expect(__ballot(nan) != 0, 0)) {
-                        uint64_t hit = __ballot(nan);
-                        hit |= hit >> 32;
-                        hit |= hit >> 16;  // bit r16: key 16 b + r16
+                    if (__builtin_expect(odds != 0, 0)) {
+                        const uint64_t hit = __ballot(vtop == 255);  // bit r16: key 16 b + r16, by every g
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (hit >> (4 * g + i) & 1) s[b][i] = kv_bits(0x7fc00000u);
@@ -973,37 +1085,43 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
         }
         const bool all = (int32_t)key0 + 63 <= pos_lo && tile.rows == 16 && (!a.window || (int64_t)key0 + a.window > pos_hi);
         if (!all) kv_mask(s, pos, key0 + 4 * g, a.window, a.first);
-        float top = kMinusInf;
+        wh_h8 ph[2], pl[2];
+        float add, most;
+        auto weights = [&] {
+            const float up = kUp - m;
+            add = most = 0.0f;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+            for (int b = 0; b < 4; ++b) {
+                const wh_f4 power = *(const wh_f4*)&pow_s[16 * b + 4 * g];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][i]);
-        top = kv_max_groups(top);
-        if constexpr (kDirect) top *= c;
-        if (__ballot(top > m + kSlack)) {
-            const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
+                for (int i = 0; i < 4; ++i) {
+                    const float w = __builtin_amdgcn_exp2f(kDirect ? fmaf(s[b][i], c, up) : s[b][i] + up), x = w * power[i];
+                    add += w;
+                    most = fmaxf(most, x);
+                    const int n = 4 * (b & 1) + i;
+                    ph[b >> 1][n] = (_Float16)x;
+                    if constexpr (kF32) pl[b >> 1][n] = (_Float16)(x - (float)ph[b >> 1][n]);
+                }
+            }
+        };
+        weights();
+        if (__ballot(most > kMost)) {  // rows with such a weight take their largest score plus exponent as the reference
+            float top = kMinusInf;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    top = fmaxf(top, s[b][i] * (kDirect ? c : 1.0f) + (float)kv_exponent(pow_s[16 * b + 4 * g + i]));
+            top = kv_max_groups(top);
+            const float to = kv_max_groups(most) > kMost ? fmaxf(m, top) : m, f = __builtin_amdgcn_exp2f(m - to);
             l *= f;
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) acc[i] *= f;
             m = to;
+            weights();
         }
-        wh_h8 ph[2], pl[2];
-        const float up = kUp - m;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            wh_f4 vs;
-            if constexpr (!kDirect) vs = *(const wh_f4*)&key_s[64 + 16 * b + 4 * g];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float w = __builtin_amdgcn_exp2f(kDirect ? fmaf(s[b][i], c, up) : s[b][i] + up);
-                l += w;
-                float x = w;
-                if constexpr (!kDirect) x *= vs[i];
-                const int n = 4 * (b & 1) + i;
-                ph[b >> 1][n] = (_Float16)x;
-                if constexpr (kF32) pl[b >> 1][n] = (_Float16)(x - (float)ph[b >> 1][n]);
-            }
-        }
+        l += add;
+        if (__ballot(apart)) end = 0;
         // values: 16 dims a step, keys of half h in blocks 2 h and 2 h + 1
         wh_h8 rv[2];
 #pragma unroll
@@ -1031,13 +1149,19 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
         wave_m[wave][r16] = m;
         wave_l[wave][r16] = l;
     }
+    const bool wave_is_apart = __ballot(apart) != 0;
+    if (lane == 0) wave_apart[wave] = wave_is_apart;
     kv_lds_barrier();
+    if (__builtin_expect(wave_apart[0] | wave_apart[1] | wave_apart[2] | wave_apart[3], 0)) {
+        kv_plain_part<HD, kF32, kLatent, 16>(a, place, wave, 4);
+        return;
+    }
     float M = wave_m[0][r16], L = 0.0f;
 #pragma unroll
     for (int w = 1; w < 4; ++w) M = fmaxf(M, wave_m[w][r16]);
 #pragma unroll
     for (int w = 0; w < 4; ++w) L += wave_l[w][r16] * __builtin_amdgcn_exp2f(wave_m[w][r16] - M);
-    const float f0 = __builtin_amdgcn_exp2f(m - M) * kv_bits((uint32_t)ref << 23);
+    const float f0 = __builtin_amdgcn_exp2f(m - M);
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) acc[i] *= f0;
     wh_f4* const o = (wh_f4*)smem;  // [wave of a pair][block of dims][lane]
@@ -1070,10 +1194,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
             kv_store<kF32>(a.out, (uint64_t)token * a.out_stride + (uint64_t)head * HD + d, x);
         }
     }
-    if (!whole && g == 0) {
-        part[HD] = M;
-        part[HD + 1] = L;
-    }
+    if (!whole && g == 0) kv_put_sum(part + HD, M - kUp, L);
 }
 
 // A tile of 64 rows (32 in f32, whose queries and weights are two parts) for
@@ -1119,8 +1240,8 @@ struct wh_kv4_packed {
     static constexpr int kAtValues = kKeyBufs * kCodes;                       // byte offsets in LDS
     static constexpr int kAtScales = kAtValues + (kLatent ? 0 : 3 * kCodes);  // [2][g][key] dwords
     static constexpr int kAtKeys = kAtScales + 2 * 4 * 64 * 4;                // f32: [2][key] power of two of keys
-    static constexpr int kAtTops = kAtKeys + (kF32 ? 2 * 64 * 4 : 0);         // f32: [2][key] exponent of value rows
-    static constexpr int kAtRel = kAtTops + (kF32 ? 2 * 64 * 4 : 0);          // [3][group][key] f16
+    static constexpr int kAtPow = kAtKeys + (kF32 ? 2 * 64 * 4 : 0);          // [2][key] power of two of value rows
+    static constexpr int kAtRel = kAtPow + 2 * 64 * 4;                        // [3][group][key] f16
     static constexpr int kAtWeights = kAtRel + 3 * kGroups * kRel * 2;        // [2][part][row][key] f16
     static constexpr int kEnd = kAtWeights + 2 * kParts * kRows * kPl * 2;
     // f32: queries lie as parts in LDS before the first run.  At 512 dims registers do not hold all of them (what
@@ -1142,7 +1263,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float wave_m[W::kKeyGroups][kRows], wave_l[W::kKeyGroups][kRows], row_m[kRows], row_c[kF32 ? kRows : 1];
     __shared__ int32_t row_pos[kRows];
-    __shared__ uint32_t wave_top[kWaves], raise[2];
+    __shared__ uint32_t raise[2];
     __shared__ uint64_t nan_keys[3];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r16 = lane & 15, g = lane >> 4;
     const uint32_t kvh = place.head, kq = wave % W::kKeyGroups, rq = wave / W::kKeyGroups;
@@ -1195,36 +1316,14 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         if constexpr (kTwo) request_of(a.v, line, vc, vb);
         request_page(run + 1);
     };
-    int ref = 0;
     auto value_bytes = [&] { return kTwo ? vb : kb; };
-    auto counts = [&](uint32_t run) {  // whether some row may see this lane's key; so too of the last run's once more
-        const uint32_t key0 = run_at(run);
-        return wh_kv4_seen(tile, key0, key0 + my_key) == key0 + my_key;
-    };
-    // largest value scale byte of this lane's chunks that counts
-    auto top_byte = [&](uint32_t run) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < W::kMine; ++i) {
-            const uint32_t b = (value_bytes() >> (8 * i)) & 0xff;
-            m = max(m, b < 255 ? b : 0u);
-        }
-        return has_values && counts(run) ? m : 0u;
-    };
     // a row's largest byte, from its lanes
     auto row_top = [&](uint32_t b) { return kv_near_max<W::kLanes>(W::kMine == 2 ? max(b & 0xff, b >> 8) : b); };
-    auto stage_rel = [&](uint32_t run, uint32_t against) {
-        _Float16* const rel = (_Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel);
-#pragma unroll
-        for (int i = 0; i < W::kMine; ++i) {
-            const int e = (int)((value_bytes() >> (8 * i)) & 0xff) - (int)against;  // above only where it does not count
-            rel[(my_chunk + i) * W::kRel + my_key] = (_Float16)kv_bits((uint32_t)max(min(e, 0) + 127, 0) << 23);
-        }
-    };
-    auto stage = [&](uint32_t run) {
+    // rows of a run to LDS; now: the run that the workgroup is at
+    auto stage = [&](uint32_t run, uint32_t now) {
         if (W::kBring < kWaves && !brings) return;
-        uint32_t top = 0;
-        if constexpr (kF32) top = row_top(kb);
+        uint32_t ktop = 0;
+        if constexpr (kF32) ktop = row_top(kb);
         if (W::kBoth || has_keys) {
             uint8_t* const kd = smem + run % W::kKeyBufs * W::kCodes + my_key * W::kRow;
 #pragma unroll
@@ -1234,29 +1333,35 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
             for (int i = 0; i < W::kMine; ++i) {
                 const uint32_t n = my_chunk + i, b = (kb >> (8 * i)) & 0xff;
                 // f32: against the row's largest, so that decoded values are finite f16 whatever the bytes are
-                sc[((n & 3) * 64 + my_key) * 4 + (n >> 2)] = (uint8_t)(kF32 ? (uint32_t)max((int)b - (int)top + 127, 0) : b);
+                sc[((n & 3) * 64 + my_key) * 4 + (n >> 2)] = (uint8_t)(kF32 ? (uint32_t)max((int)b - (int)ktop + 127, 0) : b);
             }
             if constexpr (kF32)
-                if (my_chunk == 0) ((float*)(smem + W::kAtKeys))[(run & 1) * 64 + my_key] = kv_key_scale(top, 0);
+                if (my_chunk == 0) ((float*)(smem + W::kAtKeys))[(run & 1) * 64 + my_key] = kv_key_scale(ktop, 0);
         }
-        if constexpr (kLatent) {
-            if constexpr (kF32)
-                if (my_chunk == 0) ((int*)(smem + W::kAtTops))[(run & 1) * 64 + my_key] = (int)top;
-            stage_rel(run, kF32 ? top : (uint32_t)ref);
-        } else if (W::kBoth || has_values) {
-            if constexpr (kF32 && kTwo) top = row_top(vb);
-            uint8_t* const vd = smem + W::kAtValues + run % 3 * W::kCodes + my_key * W::kRow;
-            const uint32_t bytes = value_bytes();
-            bool nan = false;
+        if (W::kBoth || has_values) {
+            const uint32_t bytes = value_bytes(), top = kTwo || !kF32 ? row_top(bytes) : ktop, vexp = kv_value_top(top);
+            _Float16* const rel = (_Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel);
+            bool odd = false;
 #pragma unroll
             for (int i = 0; i < W::kMine; ++i) {
-                *(wh_u4*)(vd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = kTwo ? vc[kTwo ? i : 0] : kc[i];
-                nan |= ((bytes >> (8 * i)) & 0xff) == 255;
+                const uint32_t b = (bytes >> (8 * i)) & 0xff;
+                rel[(my_chunk + i) * W::kRel + my_key] = kv_value_rel(b, vexp);
+                odd |= kv_value_odd(b, top, vexp);
             }
-            if (nan && counts(run)) atomicOr((unsigned long long*)&nan_keys[run % 3], 1ull << my_key);
-            if constexpr (kF32)
-                if (my_chunk == 0) ((int*)(smem + W::kAtTops))[(run & 1) * 64 + my_key] = (int)top;
-            stage_rel(run, kF32 ? top : (uint32_t)ref);
+            ((float*)(smem + W::kAtPow))[(run & 1) * 64 + my_key] = kv_bits(vexp << 23);
+            if constexpr (!kLatent) {
+                uint8_t* const vd = smem + W::kAtValues + run % 3 * W::kCodes + my_key * W::kRow;
+#pragma unroll
+                for (int i = 0; i < W::kMine; ++i) *(wh_u4*)(vd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = kTwo ? vc[kTwo ? i : 0] : kc[i];
+            }
+            if (__builtin_expect(__ballot(odd) != 0, 0)) {
+                asm volatile("");
+                const uint32_t key0 = run_at(run);  // the last run's once more: so too its keys
+                if (odd && wh_kv4_seen(tile, key0, key0 + my_key) == key0 + my_key) {  // some row may see this lane's key
+                    if (top != 255) atomicMax(&raise[now & 1], kApart);
+                    else if constexpr (!kLatent) atomicOr((unsigned long long*)&nan_keys[run % 3], 1ull << my_key);
+                }
+            }
         }
     };
 
@@ -1311,16 +1416,8 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
 
     // what the first run finds in place of an earlier one's: no weights, and finite value scales
     for (uint32_t i = 16 * t; i < W::kEnd - W::kAtRel; i += 16 * W::kThreads) *(wh_u4*)(smem + W::kAtRel + i) = (wh_u4){0, 0, 0, 0};
-    if (run0 < run1) {  // the first run's reference, with room
-        uint32_t top = top_byte(run0);
-        top = kv_wave_max(top);
-        if (lane == 0) wave_top[wave] = top;
-        kv_lds_barrier();
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) top = max(top, wave_top[i]);
-        ref = min((int)top + 3, 254);
-        stage(run0);
-    }
+    kv_lds_barrier();
+    if (run0 < run1) stage(run0, run0);
     kv_lds_barrier();
 
     // outputs of the run whose weights lie at `run` modulo 2, its values and their scales modulo 3: 16 dims a step
@@ -1357,7 +1454,8 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         }
     };
 
-    for (uint32_t run = run0; run < run1; ++run) {
+    uint32_t end = run1;  // 0 once the values are apart: not a second way out, which costs registers
+    for (uint32_t run = run0; run < end; ++run) {
         const uint32_t at = run & 1;
         request(run + 1);
         if constexpr (!kLatent)
@@ -1439,24 +1537,24 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         if constexpr (!kLatent) {
             const uint64_t nan = nan_keys[run % 3];
             if (__builtin_expect(nan != 0, 0)) {
-const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
+                const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
 #pragma unroll
                 for (int i = 0; i < 4 * kKeyBlocks; ++i)
                     if ((mine >> (16 * (i >> 2) + (i & 3)) & 1) && s[i >> 2][i & 3] != kMinusInf)
                         s[i >> 2][i & 3] = kv_bits(0x7fc00000u);
             }
         }
+        const float* const power_of = (const float*)(smem + W::kAtPow) + at * 64 + 16 * kKeyBlocks * kq + 4 * g;
+        wh_f4 power[kKeyBlocks];
+#pragma unroll
+        for (int i = 0; i < kKeyBlocks; ++i) power[i] = *(const wh_f4*)(power_of + 16 * i);
 #pragma unroll
         for (int f = 0; f < kDims; ++f) values_step(run + 2, f);
         const float m0 = row_m[row0];
-        float top = kMinusInf;
-#pragma unroll
-        for (int i = 0; i < kKeyBlocks; ++i) top = fmaxf(top, fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
-        if constexpr (!kF32) top *= c;
-        float add;
+        float add, most;
         auto weights = [&](float m) {
             const float up = kUp - m;
-            add = 0.0f;
+            add = most = 0.0f;
             _Float16* const pw =
                 (_Float16*)(smem + W::kAtWeights) + at * (kParts * kRows * W::kPl) + row0 * W::kPl + 16 * kKeyBlocks * kq + 4 * g;
 #pragma unroll
@@ -1469,10 +1567,10 @@ const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(kF32 ? s[i][k] + up : fmaf(s[i][k], c, up));
                 add += (e[0] + e[1]) + (e[2] + e[3]);
-                if constexpr (kF32) {
-                    const wh_i4 tops = *(const wh_i4*)(smem + W::kAtTops + (at * 64 + 16 * (kKeyBlocks * kq + i) + 4 * g) * 4);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_ldexpf(e[k], tops[k] - ref);
+                for (int k = 0; k < 4; ++k) {
+                    e[k] *= power[i][k];
+                    most = fmaxf(most, e[k]);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -1483,22 +1581,24 @@ const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
                 if constexpr (kF32) *(wh_u2*)(pw + kRows * W::kPl + 16 * i) = lo.u;
             }
         };
+        stage(run + 1, run);
         weights(m0);
-        uint32_t vtop = top_byte(run + 1);
-        const bool over = top > m0 + kSlack || (int)vtop > ref;
-        stage(run + 1);
-        if (__ballot(over) && lane == 0) raise[at] = run + 1;
+        if (__ballot(most > kMost) && lane == 0) atomicMax(&raise[at], run + 1);
         kv_lds_barrier();
-        if (__builtin_expect(__builtin_amdgcn_readfirstlane(raise[at]) == run + 1, 0)) {  // the whole workgroup
-            vtop = kv_wave_max(vtop);
-            top = kv_max_groups(top);
-            if (g == 0) wave_m[kq][row0] = top;
-            if (lane == 0) wave_top[wave] = vtop;
-            kv_lds_barrier();
+        const uint32_t raises = __builtin_amdgcn_readfirstlane(raise[at]);
+        if (__builtin_expect(raises > run, 0)) {  // the whole workgroup
+            if (raises == kApart) end = 0;
+            // rows with such a weight take their largest score plus exponent as the reference
+            float top = kMinusInf;
 #pragma unroll
-            for (int i = 0; i < kWaves; ++i) vtop = max(vtop, wave_top[i]);
-            const int to = (int)vtop > ref ? min((int)vtop + 3, 254) : ref;
-            const float f_ref = kv_bits((uint32_t)max(ref - to + 127, 0) << 23);
+            for (int i = 0; i < kKeyBlocks; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    top = fmaxf(top, s[i][k] * (kF32 ? 1.0f : c) + (float)kv_exponent(power[i][k]));
+            top = kv_max_groups(top);
+            if (!(kv_max_groups(most) > kMost)) top = kMinusBig;
+            if (g == 0) wave_m[kq][row0] = top;
+            kv_lds_barrier();
             auto raised = [&](uint32_t row) {
                 float m = row_m[row];
 #pragma unroll
@@ -1508,23 +1608,12 @@ const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const uint32_t row = 16 * b + r16;
-                const float f = __builtin_amdgcn_exp2f(row_m[row] - raised(row)) * f_ref;
+                const float f = __builtin_amdgcn_exp2f(row_m[row] - raised(row));
 #pragma unroll
                 for (int k = 0; k < kDims; ++k) acc[k][b] *= f;
             }
             const float m = raised(row0);
             l *= __builtin_amdgcn_exp2f(row_m[row0] - m);
-            if (to != ref) {
-                ref = to;
-                if constexpr (!kF32) {  // this run's value scales are in LDS against the old one
-                    if (has_values) {
-                        _Float16* const r = (_Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel);
-#pragma unroll
-                        for (int i = 0; i < W::kMine; ++i) r[(my_chunk + i) * W::kRel + my_key] *= (_Float16)f_ref;
-                        stage_rel(run + 1, (uint32_t)ref);
-                    }
-                }
-            }
             weights(m);
             kv_lds_barrier();
             if (kq == 0 && g == 0) row_m[row0] = m;
@@ -1533,6 +1622,10 @@ const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
         l += add;
     }
     if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
+    if (__builtin_expect(end < run1, 0)) {
+        kv_plain_part<HD, kF32, kLatent, kRows>(a, place, wave, kWaves);
+        return;
+    }
     if (run0 < run1) {
         read_weights(run1 + 1);
 #pragma unroll
@@ -1542,7 +1635,6 @@ const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
     l = kv_sum_groups(l);
     if (g == 0) wave_l[kq][row0] = l;
     kv_lds_barrier();
-    const float up = kv_bits((uint32_t)ref << 23);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
         const uint32_t r = 16 * b + r16;
@@ -1560,7 +1652,7 @@ const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
 #pragma unroll
         for (int f = 0; f < kDims; ++f) {
             const uint32_t d = 16 * (dim0 + f) + 4 * g;
-            const wh_f4 y = acc[f][b] * up * inv;
+            const wh_f4 y = acc[f][b] * inv;
             if (!whole) {
                 *(wh_f2*)(part + d) = (wh_f2){y[0], y[1]};
                 *(wh_f2*)(part + d + 2) = (wh_f2){y[2], y[3]};
@@ -1568,10 +1660,7 @@ const uint64_t mine = nan >> (16 * kKeyBlocks * kq + 4 * g);
                 kv_store<kF32>(a.out, at + d, y);
             }
         }
-        if (!whole && dim0 == 0 && g == 0) {
-            part[HD] = M;
-            part[HD + 1] = L;
-        }
+        if (!whole && dim0 == 0 && g == 0) kv_put_sum(part + HD, M - kUp, L);
     }
 }
 
@@ -1612,7 +1701,7 @@ __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
                 x[i] += p[lane] * w;
             }
     }
-    if (a.sink) L += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M + kUp);
+    if (a.sink) L += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
