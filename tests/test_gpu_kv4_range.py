@@ -175,3 +175,27 @@ def test_f32_sums_keep_f32(ctx, layout, q, lens):
     got = c.run(ctx).double()
     want, _ = c.expect()
     assert float((got - want).square().mean().sqrt() / want.square().mean().sqrt()) < 2e-6
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layout,q,n", [("group_8", [2], 130), ("group_8", [70], 130), ("group_8", [1], 4000), ("group_5", [2], 2500),
+                                        ("group_5", [40], 2500), ("pairs", [1], 1), ("pairs", [1], 6000), ("wide", [1], 3000)])
+def test_values_at_the_upper_end(ctx, layout, q, n, bf16):
+    """Finite values of up to 1.5 * 2^127 give finite outputs, in one part and
+    joined from many."""
+    for power in (125, 127.58):
+        c = Case([min(q[0], n)], [n], *LAYOUTS[layout], bf16, page=64, q_scale=0.1, sink=n == 130)
+        x = np.abs(rows(c)) if n > 130 else rows(c)  # of one sign, the sums stay that large
+        c.cache.fill(1, c.slots[0], x * 2.0 ** power)
+        check(c, ctx)
+        assert bool(torch.isfinite(c.out).all())
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layout,q,n", [("group_8", [2], 130), ("group_8", [70], 130), ("group_8", [1], 4000), ("group_5", [2], 2500)])
+def test_values_at_the_lower_end(ctx, layout, q, n, bf16):
+    """Values of some 2^-100: outputs keep f32's relative precision down to
+    products of 2^-126 (n roundings of 2^-149 below)."""
+    c = Case(q, [n], *LAYOUTS[layout], bf16, page=64, q_scale=0.1)
+    c.cache.fill(1, c.slots[0], rows(c) * 2.0 ** -100)
+    check(c, ctx, tiny=2 * n * 2.0 ** -149)

@@ -1683,14 +1683,17 @@ __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
     float M = kMinusBig, L = 0.0f;
     for (uint32_t k = lane; k < n; k += 64) M = fmaxf(M, part[k * next + HD]);
     M = wh_wave_max(M);
+    for (uint32_t k = lane; k < n; k += 64) L += part[k * next + HD + 1] * __builtin_amdgcn_exp2f(part[k * next + HD] - M);
+    L = kv_wave_sum(L);
+    if (a.sink) L += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // before the sum, which then stays within the parts' size
     float x[HD / 64];
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i) x[i] = 0.0f;
 #pragma unroll 4
     for (uint32_t k = 0; k < n; ++k) {
         const float* const p = part + k * next;
-        const float w = p[HD + 1] * __builtin_amdgcn_exp2f(p[HD] - M);
-        L += w;
+        const float w = p[HD + 1] * __builtin_amdgcn_exp2f(p[HD] - M) * inv;
 #pragma unroll
         for (int i = 0; i < HD / 64; i += 2)
             if constexpr (kPer >= 2) {
@@ -1701,14 +1704,12 @@ __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
                 x[i] += p[lane] * w;
             }
     }
-    if (a.sink) L += __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - M);
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i) {
         const uint64_t d = at + 64 * kPer * (i / kPer) + kPer * lane + i % kPer;
-        if constexpr (kF32) ((float*)a.out)[d] = x[i] * inv;
-        else ((__bf16*)a.out)[d] = (__bf16)(x[i] * inv);
+        if constexpr (kF32) ((float*)a.out)[d] = x[i];
+        else ((__bf16*)a.out)[d] = (__bf16)x[i];
     }
 }
 
