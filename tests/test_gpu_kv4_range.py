@@ -7,7 +7,8 @@ it bits.  So the tolerance has no term of the largest |v|:
   u = 2^-24.  |error| <= (2 delta + 4 u S + (2 n + 16) u + r) sum w g + o |out|
   g: the largest |v| of the value's own group of 32 dims
   delta: a score's error, (d + 12) u scale sum |q||k| for d f32 products, the
-    query's two f16 parts and three factors; bf16 queries (two E4M3 parts of 32
+    query's two f16 parts and three factors (the second part ends 2^-48 below the
+    query's largest value, 2^-25 where keys are 2^23 the other way); bf16 queries (two E4M3 parts of 32
     values) add 8 d u of the largest |q||k|
   S: the largest score, whose rounding in the exponent the weights carry; where
     the weight's reference includes a value's exponent, at most 40 and 6 more of
@@ -199,3 +200,22 @@ def test_values_at_the_lower_end(ctx, layout, q, n, bf16):
     c = Case(q, [n], *LAYOUTS[layout], bf16, page=64, q_scale=0.1)
     c.cache.fill(1, c.slots[0], rows(c) * 2.0 ** -100)
     check(c, ctx, tiny=2 * n * 2.0 ** -149)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("power", [14, 23, 30, 60, 100])
+@pytest.mark.parametrize("layout,q", [f for f in FORMS if not f[0].startswith("latent")])
+def test_keys_and_queries_far_apart(ctx, layout, q, power, bf16):
+    """Queries that are small where keys are large: a score's terms are of one
+    size, whatever the factors' are.  Queries' groups are 2^power apart, keys'
+    the other way round, in every third key."""
+    c = Case(q, [130], *LAYOUTS[layout], bf16, page=64, q_scale=1.0)
+    G, d = c.heads // c.kv_heads, c.d
+    big = np.zeros(d // 32, bool)
+    big[::2] = True
+    up = torch.from_numpy(np.where(big, 2.0 ** -power, 1.0).repeat(32)).cuda()
+    x = (c.q.double().reshape(-1, c.heads, d) * up).to(c.q.dtype)
+    c.q.copy_(x.reshape(c.q.shape))
+    sizes = np.where(big[None] & (np.arange(130) % 3 == 0)[:, None], 2.0 ** power, 1.0)
+    c.cache.fill(0, c.slots[0], rows(c, seed=9, sizes=sizes))
+    check(c, ctx)

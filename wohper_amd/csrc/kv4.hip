@@ -296,8 +296,10 @@ __global__ void __launch_bounds__(256) k_kv4_read(wh_kv4_rows_args a) {
 // with a power of two for every 32 values (together 2^-9 of a value, and 8 u of
 // the largest of the 32), in the scaled matrix instruction; products are exact in
 // its f32 sums.  f32: keys decoded to f16 against their row's largest scale byte
-// (exact down to 2^-23 of that, below which f32 would lose them too) and the
-// query as two f16 parts (22 bits, and 2^-38 of its largest value).  Outputs:
+// (exact down to 2^-23 of that, kKeyNear; what lies further apart kv_plain_part
+// takes, as below) and the query as two f16 parts, the second times 2^10: 22 bits,
+// and 2^-48 of its largest value, which times 2^23 is 2^-25 of a term again where
+// queries are small and keys large.  Outputs:
 // values are f16 against their row's largest scale byte, exact down to 2^-23 of it,
 // and that byte's power of two goes into the weight.  Weights are f16, times 2^8,
 // against a reference of each query row: the largest score plus value exponent of
@@ -322,6 +324,8 @@ constexpr float kMinusBig = -1.0e30f;  // the reference of no key: finite, so th
 constexpr float kUp = 8.0f;
 constexpr float kMost = 65504.0f;
 constexpr uint32_t kApart = 0xffffffffu;  // past every run
+constexpr int kKeyNear = 23;              // f32: a key group's scale byte is at most so far below its row's
+constexpr float kLowPart = 1024.0f;       // f32: what a query's second f16 part is multiplied by
 constexpr int kNear = 9;                  // a value group's scale byte is at most so far below its row's
 constexpr uint32_t kLow = 127 - 40, kHigh = 127 + 40;  // and the row's in here
 
@@ -570,6 +574,8 @@ __device__ __forceinline__ _Float16 kv_value_rel(uint32_t b, uint32_t vexp) {
     x.u = (uint16_t)((min(max((int)b - (int)vexp, -15), 0) + 15) << 10);
     return x.h;
 }
+// Whether a group of a key row (top: its largest byte) is not held by f16.
+__device__ __forceinline__ bool kv_key_odd(uint32_t b, uint32_t top) { return ((int)top - (int)b > kKeyNear) & (b != 0) & (top != 255); }
 // Whether a group of a value row (top: its largest byte) is NaN or not held by f16
 // products.  Not where the group is zeros: byte 0.
 __device__ __forceinline__ bool kv_value_odd(uint32_t b, uint32_t top, uint32_t vexp) {
@@ -643,7 +649,7 @@ struct wh_kv4_query {
                 for (int n = 0; n < 4; ++n) {
                     const float x = kv_bits(raw[i][k][n]) * up;
                     hi.h[n] = (_Float16)x;
-                    lo.h[n] = (_Float16)(x - (float)hi.h[n]);
+                    lo.h[n] = (_Float16)((x - (float)hi.h[n]) * kLowPart);
                 }
                 *(wh_u2*)(dst + 64 * k) = hi.u;
                 *(wh_u2*)(dst + kRows * kLd + 64 * k) = lo.u;
@@ -1019,6 +1025,11 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                 const uint32_t vtop = kLatent && !kDirect ? kbytes : kv_top_byte(raw_v, h), vexp = kv_value_top(vtop);
                 // value scales, and the powers of two of keys and value rows
                 bool odd = false;
+                if constexpr (!kDirect && !kLatent) {  // a latent row's groups are values too, and kNear is less
+                    const uint32_t pieces = kv_piece_scales(kr, h, g);
+#pragma unroll
+                    for (int j = 0; j < kPieces; ++j) odd |= kv_key_odd((pieces >> (8 * j)) & 0xff, kbytes);
+                }
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
                     const uint32_t e = (vbytes >> (8 * j)) & 0xff;
@@ -1052,15 +1063,17 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                                                                                     q_scale - (p ? 0x04040404u : 0u));
                     });
                 } else {
+                    wh_f4 s_low = s[b];  // of the second parts
 #pragma unroll
                     for (int k = 0; k < HD / 32; ++k) {
                         const int j = k / 4, w = k - j * 4;
                         const uint32_t codes = HD == 64 && g >= 2 ? kr.c[h][j][w + 2] : kr.c[h][j][w];
                         const wh_h8 x = kv_decode(codes, kv_rel(kr, h, j, g, kbytes));
-#pragma unroll
-                        for (int p = kParts - 1; p >= 0; --p)
-                            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qd[k][p], s[b], 0, 0, 0);
+                        s_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qd[k][kParts - 1], s_low, 0, 0, 0);
+                        s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qd[k][0], s[b], 0, 0, 0);
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[b][i] = fmaf(s_low[i], 1.0f / kLowPart, s[b][i]);
                 }
                 // direct: a value row that holds NaN beside keys that do not
                 if constexpr (kDirect && !kLatent) {
@@ -1322,7 +1335,8 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     // rows of a run to LDS; now: the run that the workgroup is at
     auto stage = [&](uint32_t run, uint32_t now) {
         if (W::kBring < kWaves && !brings) return;
-        uint32_t ktop = 0;
+        uint32_t ktop = 0, vtop = 0;
+        bool odd = false;
         if constexpr (kF32) ktop = row_top(kb);
         if (W::kBoth || has_keys) {
             uint8_t* const kd = smem + run % W::kKeyBufs * W::kCodes + my_key * W::kRow;
@@ -1335,18 +1349,23 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
                 // f32: against the row's largest, so that decoded values are finite f16 whatever the bytes are
                 sc[((n & 3) * 64 + my_key) * 4 + (n >> 2)] = (uint8_t)(kF32 ? (uint32_t)max((int)b - (int)ktop + 127, 0) : b);
             }
-            if constexpr (kF32)
+            if constexpr (kF32) {
                 if (my_chunk == 0) ((float*)(smem + W::kAtKeys))[(run & 1) * 64 + my_key] = kv_key_scale(ktop, 0);
+                if constexpr (!kLatent)  // a latent row's groups are values too, and kNear is less
+#pragma unroll
+                    for (int i = 0; i < W::kMine; ++i) odd |= kv_key_odd((kb >> (8 * i)) & 0xff, ktop);
+            }
         }
         if (W::kBoth || has_values) {
-            const uint32_t bytes = value_bytes(), top = kTwo || !kF32 ? row_top(bytes) : ktop, vexp = kv_value_top(top);
+            const uint32_t bytes = value_bytes();
+            vtop = kTwo || !kF32 ? row_top(bytes) : ktop;
+            const uint32_t vexp = kv_value_top(vtop);
             _Float16* const rel = (_Float16*)(smem + W::kAtRel) + run % 3 * (W::kGroups * W::kRel);
-            bool odd = false;
 #pragma unroll
             for (int i = 0; i < W::kMine; ++i) {
                 const uint32_t b = (bytes >> (8 * i)) & 0xff;
                 rel[(my_chunk + i) * W::kRel + my_key] = kv_value_rel(b, vexp);
-                odd |= kv_value_odd(b, top, vexp);
+                odd |= kv_value_odd(b, vtop, vexp);
             }
             ((float*)(smem + W::kAtPow))[(run & 1) * 64 + my_key] = kv_bits(vexp << 23);
             if constexpr (!kLatent) {
@@ -1354,13 +1373,13 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
 #pragma unroll
                 for (int i = 0; i < W::kMine; ++i) *(wh_u4*)(vd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = kTwo ? vc[kTwo ? i : 0] : kc[i];
             }
-            if (__builtin_expect(__ballot(odd) != 0, 0)) {
-                asm volatile("");
-                const uint32_t key0 = run_at(run);  // the last run's once more: so too its keys
-                if (odd && wh_kv4_seen(tile, key0, key0 + my_key) == key0 + my_key) {  // some row may see this lane's key
-                    if (top != 255) atomicMax(&raise[now & 1], kApart);
-                    else if constexpr (!kLatent) atomicOr((unsigned long long*)&nan_keys[run % 3], 1ull << my_key);
-                }
+        }
+        if (__builtin_expect(__ballot(odd) != 0, 0)) {
+            asm volatile("");
+            const uint32_t key0 = run_at(run);  // the last run's once more: so too its keys
+            if (odd && wh_kv4_seen(tile, key0, key0 + my_key) == key0 + my_key) {  // some row may see this lane's key
+                if (vtop != 255) atomicMax(&raise[now & 1], kApart);
+                else if constexpr (!kLatent) atomicOr((unsigned long long*)&nan_keys[run % 3], 1ull << my_key);
             }
         }
     };
@@ -1508,7 +1527,11 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
                 }
 #pragma unroll
             for (int i = 0; i < kKeyBlocks; ++i)
-                s[i] = (s[i] + s_low[i]) * c * *(const wh_f4*)(smem + W::kAtKeys + (at * 64 + 16 * (kKeyBlocks * kq + i) + 4 * g) * 4);
+            {
+                const wh_f4 k_scale = *(const wh_f4*)(smem + W::kAtKeys + (at * 64 + 16 * (kKeyBlocks * kq + i) + 4 * g) * 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[i][k] = fmaf(s_low[i][k], 1.0f / kLowPart, s[i][k]) * c * k_scale[k];
+            }
         } else {
             // codes as they lie, which takes scales by 32 dims
             wh_static_for<kPieces>([&](auto jc) {
