@@ -219,3 +219,28 @@ def test_keys_and_queries_far_apart(ctx, layout, q, power, bf16):
     sizes = np.where(big[None] & (np.arange(130) % 3 == 0)[:, None], 2.0 ** power, 1.0)
     c.cache.fill(0, c.slots[0], rows(c, seed=9, sizes=sizes))
     check(c, ctx)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("power", [-122, -110, 110, 124])
+@pytest.mark.parametrize("layout,q", [f for f in FORMS if not f[0].startswith("latent")])
+def test_queries_at_both_ends(ctx, layout, q, power, bf16):
+    """Queries of 2^power and keys of 2^-power: scores of order one and ten."""
+    c = Case(q, [130], *LAYOUTS[layout], bf16, page=64, q_scale=1.0)
+    c.q[-1] = c.q[-1].abs()  # a query that all keys with it are large for
+    c.q.copy_((c.q.double() * 2.0 ** power).to(c.q.dtype))
+    k = rows(c, seed=9)
+    k[::5] = np.abs(k[::5])
+    c.cache.fill(0, c.slots[0], k * 2.0 ** -power)
+    check(c, ctx)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 90, 2.0 ** -60])
+@pytest.mark.parametrize("layout,q", [("pairs", [3]), ("group_8", [2]), ("group_8", [70]), ("wide", [3])])
+def test_scales_that_undo_the_sizes(ctx, layout, q, scale):
+    """Queries, keys and the scale far from one, scores not, in f32."""
+    c = Case(q, [130], *LAYOUTS[layout], False, page=64, q_scale=1.0)
+    c.q.mul_(2.0 ** (-30 if scale > 1 else -58))
+    c.cache.fill(0, c.slots[0], rows(c, seed=9) * 2.0 ** (-60 if scale > 1 else 116))
+    c.scale = scale
+    check(c, ctx)

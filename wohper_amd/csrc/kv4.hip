@@ -625,8 +625,11 @@ struct wh_kv4_query {
         }
     }
 
-    // factor[row]: what a sum of products with the row is to be multiplied by
-    __device__ __forceinline__ void put(uint32_t wave, uint32_t lane, _Float16* lds, float* factor) const {
+    // factor[row]: what a sum of products with the row is to be multiplied by,
+    // `scale` included.  Sums are below 2^26: whether that takes finite ones past
+    // f32 before the key's power of two brings them back, or is subnormal itself.
+    __device__ __forceinline__ bool put(uint32_t wave, uint32_t lane, _Float16* lds, float* factor, float scale) const {
+        bool far = false;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             uint32_t top = 0;
@@ -654,8 +657,11 @@ struct wh_kv4_query {
                 *(wh_u2*)(dst + 64 * k) = hi.u;
                 *(wh_u2*)(dst + kRows * kLd + 64 * k) = lo.u;
             }
-            if ((lane & 15) == 0) factor[r] = kv_bits((uint32_t)(e - 13) << 23);
+            const float c = scale * kv_bits((uint32_t)(e - 13) << 23), size = fabsf(c);
+            if ((lane & 15) == 0) factor[r] = c;
+            far |= e < 255 && scale != 0.0f && !(size >= 0x1p-126f && size < 0x1p102f);
         }
+        return far;
     }
 
     // A lane's operands: the parts of a row's dims kv_dim(step, g) ..
@@ -700,7 +706,7 @@ __device__ __forceinline__ uint32_t kv_query_e4m3(const wh_u4 (&raw)[2][2], uint
                 top = max(top, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
             }
         top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));  // the other 16 of the 32
-        e[h] = max((int)(top >> 23), 20);
+        e[h] = max((int)(top >> 23), 11);  // the second part's byte is 11 less
         const float up = kv_bits((uint32_t)(127 + 127 + 7 - min(e[h], 254)) << 23);  // the largest to [2^7, 2^8)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -957,6 +963,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
     if (any) request_pages(part0);
 
     // the row's query
+    bool apart = false;  // what f16 products do not hold
     wh_h8 qd[kDirect ? 1 : HD / 32][kParts];
     wh_i8 qx[kDirect ? kPieces : 1][2];
     uint32_t q_scale = 0;
@@ -982,10 +989,10 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                 return (const float*)a.q + (uint64_t)(tile.token0 + n) * a.q_stride + (uint64_t)(kvh * a.group + f - n * a.group) * HD;
             });
             if (any) request(part0);
-            query.put(wave, lane, (_Float16*)smem, row_c);
+            apart = query.put(wave, lane, (_Float16*)smem, row_c, a.scale_log2);
             kv_lds_barrier();
             W::Query::get(qd, (const _Float16*)smem, r16, g);
-            c = a.scale_log2 * row_c[r16];
+            c = row_c[r16];
             kv_lds_barrier();
         }
     }
@@ -994,7 +1001,6 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
 #pragma unroll
     for (int f = 0; f < HD / 16; ++f) acc[f] = (wh_f4){0.0f, 0.0f, 0.0f, 0.0f};
     float m = kMinusBig, l = 0.0f;  // of the row, in all its lanes: the reference, and this lane's sum of weights
-    bool apart = false;
 
     uint8_t* const mine = smem + wave * W::kWave;
     _Float16* const rel = (_Float16*)(mine + W::kAtRel);  // [group][16 g + 4 b + i of key 16 b + 4 g + i]
@@ -1388,6 +1394,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     // the query of row r16 of block rq
     wh_i8 qx[kF32 ? 1 : kPieces][2];
     wh_h8 qd[kF32 ? HD / 32 : 1][kParts];
+    bool apart = false;  // f32: what f16 products do not hold
     uint32_t q_scale = 0;
     float c;  // scores are sums times this
     float l = 0.0f;
@@ -1401,10 +1408,10 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
                 return (const float*)a.q + (uint64_t)(tile.token0 + n) * a.q_stride + (uint64_t)(kvh * a.group + f - n * a.group) * HD;
             });
             if (run0 < run1) request(run0);
-            query.put(wave, lane, (_Float16*)(smem + W::kAtQuery), row_c);
+            apart = query.put(wave, lane, (_Float16*)(smem + W::kAtQuery), row_c, a.scale_log2);
             kv_lds_barrier();
             W::Query::get(qd, (const _Float16*)(smem + W::kAtQuery), row0, g);
-            c = a.scale_log2 * row_c[row0];
+            c = row_c[row0];
             kv_lds_barrier();
         } else {
             const uint64_t at = (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)(kvh * a.group + flat - tok * a.group) * HD;
@@ -1436,7 +1443,10 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     // what the first run finds in place of an earlier one's: no weights, and finite value scales
     for (uint32_t i = 16 * t; i < W::kEnd - W::kAtRel; i += 16 * W::kThreads) *(wh_u4*)(smem + W::kAtRel + i) = (wh_u4){0, 0, 0, 0};
     kv_lds_barrier();
-    if (run0 < run1) stage(run0, run0);
+    if (run0 < run1) {
+        stage(run0, run0);
+        if (kF32 && apart) atomicMax(&raise[run0 & 1], kApart);
+    }
     kv_lds_barrier();
 
     // outputs of the run whose weights lie at `run` modulo 2, its values and their scales modulo 3: 16 dims a step
