@@ -244,3 +244,22 @@ def test_scales_that_undo_the_sizes(ctx, layout, q, scale):
     c.cache.fill(0, c.slots[0], rows(c, seed=9) * 2.0 ** (-60 if scale > 1 else 116))
     c.scale = scale
     check(c, ctx)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layout,q,n", [("pairs", [3], 130), ("group_8", [2], 130), ("group_8", [70], 130), ("group_5", [30], 130),
+                                        ("wide", [3], 130), ("group_8", [1], 4000), ("group_5", [40], 2500)])
+def test_scores_at_the_lower_end(ctx, layout, q, n, bf16):
+    """Scores of some -2^122 are scores: the key that has the largest takes all
+    of the weight."""
+    c = Case(q, [n], *LAYOUTS[layout], bf16, page=64, q_scale=0.0)
+    c.scale = 1.0
+    c.q[:, :c.heads * c.d] = 2.0 ** 60
+    k = np.full((n, c.kv_heads * c.d), -2.0 ** 56)
+    k[17] = -2.0 ** 55
+    c.cache.fill(0, c.slots[0], k)
+    c.cache.fill(1, c.slots[0], rows(c))
+    got = c.run(ctx).double()
+    v = torch.from_numpy(c.cache.rows(1, c.slots[0][17:18])[0]).cuda()
+    want = v.repeat_interleave(c.heads // c.kv_heads, 0).reshape(1, -1)
+    assert bool(((got - want).abs() <= 4 * U * want.abs()).all())

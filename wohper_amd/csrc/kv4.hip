@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(256) k_kv4_read(wh_kv4_rows_args a) {
 // to thirty times as long, for rows no model is known to make.
 
 #define kMinusInf (-__builtin_inff())
-constexpr float kMinusBig = -1.0e30f;  // the reference of no key: finite, so that differences are
+constexpr float kMinusBig = -3.402823466e38f;  // the reference of no key: finite, so that differences are, and below every score
 // Weights are held times 2^kUp: f16 keeps small ones.  A row's reference is raised
 // to its largest score once a weight is past f16, 2^8 above: with 2^5 the prompts of
 // k_kv4_attn_packed took 290 us for 243.  Rows raise theirs by themselves: that
