@@ -856,9 +856,12 @@ typedef struct {
  * A plan that does not fit takes, gives and numbers nothing: starts are 0, no
  * token has a slot, the stack is as before, and wh_stream_status reports
  * WH_OUT_OF_MEMORY (not enough pages) or WH_OUTPUT_TOO_SMALL (max_tokens,
- * table_stride).  A page id of n_pages or more reports WH_NOT_RESIDENT and
- * its tokens get no slot.  At most 4096 requests; apart from the stack no
- * output may overlap an input. */
+ * table_stride).  A table entry of 0xFFFFFFFF holds no page (one behind a window,
+ * say, that the caller has put onto the stack itself): it is passed over when a
+ * request shrinks.  Any other page id of n_pages or more reports WH_NOT_RESIDENT;
+ * it does not get onto the stack, and tokens on it or on an entry of no page get
+ * no slot.  At most 4096 requests; apart from the stack no output may overlap an
+ * input. */
 typedef struct {
     size_t n_requests;
     const uint32_t* old_lens_dev;
@@ -911,14 +914,14 @@ int wh_kv4_read_async(wh_ctx* ctx, const wh_kv4_cache* cache, const uint32_t* sl
  * key lists and the context's scratch for it, not the result.  A table entry
  * of n_pages or more, or a length above table_stride * page_size, reports
  * WH_NOT_RESIDENT; entries of pages that no token sees a row of are not looked
- * at, so pages behind a window can be given back.  A visible row that holds
- * NaN makes its heads' outputs NaN.  A row that a token does not see takes
- * nothing from that token's output, whatever its bytes, nor does one of no
- * weight, nor do other dims: sums are f32 in both types and in both numerics
- * modes, and an f32 result is within f32 rounding of the sums of w |v|, |v|
- * being the largest of the value's group of 32 dims.  A tile of tokens some of
- * which see a row whose groups are more than 2^9 apart, or whose largest is not
- * within 2^40 of 1, takes many times as long. */
+ * at, so pages behind a window can be given back (0xFFFFFFFF in their place).
+ * A visible row that holds NaN makes its heads' outputs NaN.  A row that a
+ * token does not see takes nothing from that token's output, whatever its
+ * bytes, nor does one of no weight, nor do other dims: sums are f32 in both
+ * types and in both numerics modes, and an f32 result is within f32 rounding
+ * of the sums of w |v|, |v| being the largest of the value's group of 32 dims.
+ * A tile of tokens some of which see a row whose groups are more than 2^9
+ * apart, or whose largest is not within 2^40 of 1, takes many times as long. */
 typedef struct {
     const void* q_dev;
     size_t q_stride;

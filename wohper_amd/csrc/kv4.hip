@@ -46,31 +46,48 @@ __device__ __forceinline__ uint64_t kv_lane(uint64_t v, uint32_t lane) {
            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
 
-// Last index i with prefix[i] <= x (prefix ascending, prefix[0] = 0 <= x).
-__device__ __forceinline__ uint32_t kv_find(const uint32_t* prefix, uint32_t n, uint32_t x) {
-    uint32_t lo = 0, hi = n;  // prefix[lo] <= x, answer in [lo, hi)
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (prefix[mid] <= x) lo = mid;
-        else hi = mid;
+// Last indexes i with prefix[i] <= x (prefix ascending, prefix[0] = 0 <= x), kN
+// searches in step.
+template <int kN>
+__device__ __forceinline__ void kv_find(const uint32_t* prefix, uint32_t n, const uint32_t (&x)[kN], uint32_t (&at)[kN]) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) at[i] = 0;  // the answer is in [at, at + n)
+    while (n > 1) {
+        const uint32_t half = n >> 1;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) at[i] += prefix[at[i] + half] <= x[i] ? half : 0;
+        n -= half;
     }
-    return lo;
+}
+__device__ __forceinline__ uint32_t kv_find(const uint32_t* prefix, uint32_t n, uint32_t x) {
+    const uint32_t xs[1] = {x};
+    uint32_t at[1];
+    kv_find<1>(prefix, n, xs, at);
+    return at[0];
 }
 
 constexpr uint32_t kPlanThreads = 1024;
+constexpr uint32_t kPlanStage = 8192;  // table entries given back that lie in LDS
+constexpr size_t plan_lds(uint32_t n) { return (4 * ((size_t)n + 1) + kPlanStage) * sizeof(uint32_t); }
 
 // Every workgroup adds up all requests (three prefix sums of n <= 4096 numbers
-// in LDS: new tokens, pages taken, pages given back) and then fills its share
+// in LDS: new tokens, pages taken, table entries given back) and then fills its share
 // of the outputs, so a plan is one launch whose workgroups wait for nobody.  A
 // page that a request takes is worked out where it is needed (its table entry,
 // each slot on it) instead of being read back from another workgroup's store.
-// Bound by latency: the prefix sums and one chain of dependent loads (7.2 us for
-// 64 requests, 13.0 for 512).
+// Entries given back that are no pages (behind a window, and given back before)
+// are not numbered: a workgroup that finds one counts the pages of every request
+// that shrinks and lays all of them out on the stack, each for itself, as the
+// same values.
+// Bound by latency: the prefix sums and one chain of dependent loads (7.5 us for
+// 64 requests, 12.6 for 512).
 __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
     extern __shared__ __align__(16) uint32_t lds[];
     uint32_t* const tok = lds;                  // [n + 1]
     uint32_t* const take = tok + a.n + 1;       // [n + 1]
     uint32_t* const give = take + a.n + 1;      // [n + 1]
+    uint32_t* const kept = give + a.n + 1;      // [n + 1] pages of a request after the step
+    uint32_t* const stage = kept + a.n + 1;     // [kPlanStage]
     __shared__ uint64_t wave_sum[3][kPlanThreads / 64];
     __shared__ uint32_t bad;
     const uint32_t t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -79,6 +96,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
     __syncthreads();
     constexpr uint32_t kPer = WH_KV_MAX_REQUESTS / kPlanThreads;
     const uint32_t per = (a.n + kPlanThreads - 1) / kPlanThreads, b0 = t * per;
+    auto pages = [&](uint64_t len) { return (len + mask) >> a.shift; };
     uint64_t mine[kPer][3], run[3] = {0, 0, 0};
 #pragma unroll
     for (uint32_t k = 0; k < kPer; ++k) {
@@ -87,47 +105,108 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
         for (int s = 0; s < 3; ++s) mine[k][s] = run[s];
         if (k < per && b < a.n) {
             const uint64_t o = a.old_lens[b], w = a.new_lens[b];
-            const uint64_t po = (o + mask) >> a.shift, pw = (w + mask) >> a.shift;
+            const uint64_t po = pages(o), pw = pages(w);
+            kept[b] = (uint32_t)pw;
             if (po > a.table_stride || pw > a.table_stride) bad = 1;
             run[0] += w > o ? w - o : 0;
             run[1] += pw > po ? pw - po : 0;
             run[2] += po > pw ? po - pw : 0;
         }
     }
-    uint64_t incl[3];
-#pragma unroll
-    for (int s = 0; s < 3; ++s) {
-        incl[s] = kv_scan(run[s]);
-        if (lane == 63) wave_sum[s][wave] = incl[s];
-    }
-    __syncthreads();
+    // the sums over all threads, and of each request's share those before it
     uint64_t total[3];
+    auto prefix = [&](auto from) {
+        constexpr int kFrom = decltype(from)::value;
+        uint64_t incl[3];
 #pragma unroll
-    for (int s = 0; s < 3; ++s) {
-        const uint64_t sum = lane < kPlanThreads / 64 ? wave_sum[s][lane] : 0, upto = kv_scan(sum);
-        const uint64_t all = kv_lane(upto, 63), before = kv_lane(upto - sum, wave);
-        total[s] = all;
-        uint32_t* const dst = s == 0 ? tok : s == 1 ? take : give;
-        const uint64_t base = before + incl[s] - run[s];
+        for (int s = kFrom; s < 3; ++s) {
+            incl[s] = kv_scan(run[s]);
+            if (lane == 63) wave_sum[s][wave] = incl[s];
+        }
+        __syncthreads();
 #pragma unroll
-        for (uint32_t k = 0; k < kPer; ++k)
-            if (k < per && b0 + k < a.n) dst[b0 + k] = (uint32_t)(base + mine[k][s]);
-        if (t == 0) dst[a.n] = (uint32_t)all;
-    }
-    __syncthreads();
-    // a plan that does not fit is none: nothing is taken, given or numbered
+        for (int s = kFrom; s < 3; ++s) {
+            const uint64_t sum = lane < kPlanThreads / 64 ? wave_sum[s][lane] : 0, upto = kv_scan(sum);
+            const uint64_t all = kv_lane(upto, 63), before = kv_lane(upto - sum, wave);
+            total[s] = all;
+            uint32_t* const dst = s == 0 ? tok : s == 1 ? take : give;
+            const uint64_t base = before + incl[s] - run[s];
+#pragma unroll
+            for (uint32_t k = 0; k < kPer; ++k)
+                if (k < per && b0 + k < a.n) dst[b0 + k] = (uint32_t)(base + mine[k][s]);
+            if (t == 0) dst[a.n] = (uint32_t)all;
+        }
+        __syncthreads();
+    };
+    prefix(std::integral_constant<int, 0>());
     const bool narrow = bad || total[0] > a.max_tokens;
+    auto entry = [&](uint32_t j) {  // the j-th table entry given back
+        const uint32_t b = kv_find(give, a.n, j);
+        return a.tables[b * a.table_stride + kept[b] + (j - give[b])];
+    };
+    bool odd = false;  // whether some of them are no pages
+    const bool staged = total[2] <= kPlanStage;
+    if (!narrow && staged) {
+        const uint32_t n = (uint32_t)total[2];
+        for (uint32_t j0 = t; j0 < n; j0 += 4 * kPlanThreads) {
+            uint32_t j[4], b[4], page[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) j[i] = min(j0 + i * kPlanThreads, n - 1);
+            kv_find<4>(give, a.n, j, b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) page[i] = a.tables[b[i] * a.table_stride + kept[b[i]] + (j[i] - give[b[i]])];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                stage[j[i]] = page[i];
+                odd |= page[i] >= a.n_pages;
+            }
+        }
+    } else if (!narrow && total[2] <= 0xffffffffu) {
+        for (uint64_t j = t; j < total[2]; j += kPlanThreads) odd |= entry((uint32_t)j) >= a.n_pages;
+    }
+    const bool holes = total[2] && __syncthreads_or(odd);
+    if (holes) {
+        // pages of each request, counted by a wave, in the place of its entries
+        for (uint32_t b = wave; b < a.n; b += kPlanThreads / 64) {
+            const uint32_t po = (uint32_t)pages(a.old_lens[b]), pw = kept[b];
+            uint32_t n = 0;
+            for (uint64_t i = pw; i < po; i += 64) {
+                const uint32_t page = i + lane < po ? a.tables[b * a.table_stride + i + lane] : WH_KV_NONE;
+                if (page >= a.n_pages && page != WH_KV_NONE && blockIdx.x == 0) atomicOr(a.status, WH_ST_NOT_RESIDENT);
+                n += (uint32_t)__popcll(__ballot(page < a.n_pages));
+            }
+            if (lane == 0) give[b] = n;
+        }
+        __syncthreads();
+        run[2] = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k) {
+            mine[k][2] = run[2];
+            if (k < per && b0 + k < a.n) run[2] += give[b0 + k];
+        }
+        prefix(std::integral_constant<int, 2>());
+    }
+    // a plan that does not fit is none: nothing is taken, given or numbered
     const bool empty = count_in > a.n_pages || count_in + total[2] > a.n_pages || total[1] > count_in + total[2];
     const bool ok = !narrow && !empty;
     const uint32_t n_tok = ok ? (uint32_t)total[0] : 0, n_take = ok ? (uint32_t)total[1] : 0,
                    n_give = ok ? (uint32_t)total[2] : 0;
     const uint32_t top = count_in + n_give;
+    if (holes && ok) {
+        for (uint32_t b = wave; b < a.n; b += kPlanThreads / 64) {
+            const uint32_t po = (uint32_t)pages(a.old_lens[b]), pw = kept[b];
+            uint32_t to = count_in + give[b];
+            for (uint64_t i = pw; i < po; i += 64) {
+                const uint32_t page = i + lane < po ? a.tables[b * a.table_stride + i + lane] : WH_KV_NONE;
+                const uint64_t real = __ballot(page < a.n_pages);
+                if (page < a.n_pages) a.free_out[to + (uint32_t)__popcll(real & ((1ull << lane) - 1))] = page;
+                to += (uint32_t)__popcll(real);
+            }
+        }
+        __syncthreads();
+    }
     const uint32_t first = blockIdx.x * kPlanThreads + t, step = gridDim.x * kPlanThreads;
-    auto given = [&](uint32_t j) {  // the j-th page given back
-        const uint32_t b = kv_find(give, a.n, j);
-        const uint32_t at = (uint32_t)(((uint64_t)a.new_lens[b] + mask) >> a.shift) + (j - give[b]);
-        return a.tables[b * a.table_stride + at];
-    };
+    auto given = [&](uint32_t j) { return holes ? a.free_out[count_in + j] : staged ? stage[j] : entry(j); };  // the j-th page given back
     auto taken = [&](uint32_t k) {  // the k-th page off the stack
         const uint32_t at = top - 1 - k;
         return at < count_in ? a.free_in[at] : given(at - count_in);
@@ -138,7 +217,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
             const uint32_t b = kv_find(tok, a.n, i);
             const uint32_t old = a.old_lens[b];
             pos = old + (i - tok[b]);
-            const uint32_t po = (uint32_t)(((uint64_t)old + mask) >> a.shift), pi = pos >> a.shift;
+            const uint32_t po = (uint32_t)pages(old), pi = pos >> a.shift;
             const uint32_t page = pi < po ? a.tables[b * a.table_stride + pi] : taken(take[b] + (pi - po));
             if (page < a.n_pages) slot = (page << a.shift) + (pos & mask);
             else atomicOr(a.status, WH_ST_NOT_RESIDENT);
@@ -148,10 +227,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
     }
     for (uint32_t k = first; k < n_take; k += step) {
         const uint32_t b = kv_find(take, a.n, k);
-        const uint32_t po = (uint32_t)(((uint64_t)a.old_lens[b] + mask) >> a.shift);
-        a.tables[b * a.table_stride + po + (k - take[b])] = taken(k);
+        a.tables[b * a.table_stride + (uint32_t)pages(a.old_lens[b]) + (k - take[b])] = taken(k);
     }
-    for (uint32_t j = first; j < n_give; j += step) a.free_out[count_in + j] = given(j);
+    if (!holes)
+        for (uint32_t j = first; j < n_give; j += step) a.free_out[count_in + j] = given(j);
     if (a.free_out != a.free_in)
         for (uint32_t k = first; k < min(count_in, a.n_pages); k += step) a.free_out[k] = a.free_in[k];
     for (uint32_t b = first; b <= a.n; b += step) a.starts[b] = ok ? tok[b] : 0;
@@ -1793,17 +1872,20 @@ hipError_t attn_launch_hd(const wh_kv4_attn_args& a, bool bf16, bool latent, hip
 }  // namespace
 
 hipError_t wh_kv4_setup() {
+    if (const hipError_t e = hipFuncSetAttribute((const void*)k_kv_plan, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)plan_lds(WH_KV_MAX_REQUESTS));
+        e != hipSuccess)
+        return e;
     for (const hipError_t e : {attn_setup_hd<64>(), attn_setup_hd<128>(), attn_setup_hd<256>(), attn_setup_hd<512>()})
         if (e != hipSuccess) return e;
     return hipSuccess;
 }
 
 hipError_t wh_kv_plan_launch(const wh_kv_plan_args& a, hipStream_t stream) {
-    const size_t lds = 3 * ((size_t)a.n + 1) * sizeof(uint32_t);
     const uint64_t copy = a.free_out != a.free_in ? a.n_pages : 0;
     const uint64_t items = std::max<uint64_t>(std::max<uint64_t>(a.max_tokens, copy), 1);
     const uint32_t grid = (uint32_t)std::min<uint64_t>((items + 4 * kPlanThreads - 1) / (4 * kPlanThreads), 256);
-    k_kv_plan<<<grid, kPlanThreads, lds, stream>>>(a);
+    k_kv_plan<<<grid, kPlanThreads, plan_lds(a.n), stream>>>(a);
     return hipGetLastError();
 }
 
