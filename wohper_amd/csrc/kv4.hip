@@ -205,13 +205,13 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
         }
         __syncthreads();
     }
-    const uint32_t first = blockIdx.x * kPlanThreads + t, step = gridDim.x * kPlanThreads;
     auto given = [&](uint32_t j) { return holes ? a.free_out[count_in + j] : staged ? stage[j] : entry(j); };  // the j-th page given back
     auto taken = [&](uint32_t k) {  // the k-th page off the stack
         const uint32_t at = top - 1 - k;
         return at < count_in ? a.free_in[at] : given(at - count_in);
     };
-    for (uint32_t i = first; i < a.max_tokens; i += step) {
+    auto share = [&](uint32_t n, auto f) { wh_kv_share(blockIdx.x * kPlanThreads + t, gridDim.x * kPlanThreads, n, f); };
+    share(a.max_tokens, [&](uint32_t i) {
         uint32_t slot = WH_KV_NONE, pos = 0;
         if (i < n_tok) {
             const uint32_t b = kv_find(tok, a.n, i);
@@ -224,16 +224,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(wh_kv_plan_args a) {
         }
         a.slots[i] = slot;
         a.positions[i] = pos;
-    }
-    for (uint32_t k = first; k < n_take; k += step) {
+    });
+    share(n_take, [&](uint32_t k) {
         const uint32_t b = kv_find(take, a.n, k);
         a.tables[b * a.table_stride + (uint32_t)pages(a.old_lens[b]) + (k - take[b])] = taken(k);
-    }
-    if (!holes)
-        for (uint32_t j = first; j < n_give; j += step) a.free_out[count_in + j] = given(j);
-    if (a.free_out != a.free_in)
-        for (uint32_t k = first; k < min(count_in, a.n_pages); k += step) a.free_out[k] = a.free_in[k];
-    for (uint32_t b = first; b <= a.n; b += step) a.starts[b] = ok ? tok[b] : 0;
+    });
+    if (!holes) share(n_give, [&](uint32_t j) { a.free_out[count_in + j] = given(j); });
+    if (a.free_out != a.free_in) share(min(count_in, a.n_pages), [&](uint32_t k) { a.free_out[k] = a.free_in[k]; });
+    share(a.n + 1, [&](uint32_t b) { a.starts[b] = ok ? tok[b] : 0; });
     if (t == 0 && blockIdx.x == 0 && !ok) atomicOr(a.status, narrow ? WH_ST_KV_NARROW : WH_ST_KV_PAGES);
     // free_count_out may be free_count: it is written once every workgroup has read it
     if (t == 0) {

@@ -12,6 +12,13 @@
 
 #define WH_KV_NONE 0xffffffffu  // a slot or page that is none
 
+// f(i) for a thread's share of n things: first, first + step, ..; 64 bits, since a
+// cache may have 2^32 - 2 pages, past which a step would start over.
+template <class F>
+WH_KV_HD void wh_kv_share(uint64_t first, uint64_t step, uint64_t n, F f) {
+    for (uint64_t i = first; i < n; i += step) f((uint32_t)i);
+}
+
 // Line of a row in a plane: codes start at line * head_dim / 2, scale bytes at
 // line * head_dim / 32.
 WH_KV_HD uint64_t wh_kv4_line(uint32_t page, uint32_t head, uint32_t row, uint32_t kv_heads, uint32_t shift) {
