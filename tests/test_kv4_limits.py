@@ -14,6 +14,7 @@ def build_and_run(tmp_path, source):
 
 
 SHARE = r"""
+#include <initializer_list>
 #include "kv4_index.h"
 int main() {
     // a cache of pages of one row may have 2^32 - 2 of them; a 32-bit counter that
