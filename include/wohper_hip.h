@@ -921,7 +921,9 @@ int wh_kv4_read_async(wh_ctx* ctx, const wh_kv4_cache* cache, const uint32_t* sl
  * types and in both numerics modes, and an f32 result is within f32 rounding
  * of the sums of w |v|, |v| being the largest of the value's group of 32 dims.
  * A tile of tokens some of which see a row whose groups are more than 2^9
- * apart, or whose largest is not within 2^40 of 1, takes many times as long. */
+ * apart, or whose largest is not within 2^40 of 1, takes many times as long.
+ * A call whose tiles (of 16 rows of a key head at least) times kv_heads may be
+ * 2^23 or more is WH_UNSUPPORTED. */
 typedef struct {
     const void* q_dev;
     size_t q_stride;

@@ -1887,20 +1887,35 @@ hipError_t wh_kv_plan_launch(const wh_kv_plan_args& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+namespace {
+// Launches for all rows of a call; launch(grid, a) takes some.
+template <class F>
+hipError_t kv_rows_launch(wh_kv4_rows_args a, bool bf16, F launch) {
+    const uint64_t pieces = (uint64_t)a.s.kv_heads * (a.s.head_dim / 8);
+    for (uint64_t left = a.n; left;) {
+        a.n = (uint32_t)wh_kv4_rows_of_launch(left, pieces);
+        launch(dim3((uint32_t)((a.n * pieces + 255) / 256), a.planes), a);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        left -= a.n;
+        a.slots += a.n;
+        for (uint32_t p = 0; p < a.planes; ++p) a.rows[p] = (uint8_t*)a.rows[p] + a.n * a.stride[p] * (bf16 ? 2 : 4);
+    }
+    return hipSuccess;
+}
+}  // namespace
+
 hipError_t wh_kv4_write_launch(const wh_kv4_rows_args& a, bool bf16, hipStream_t stream) {
-    const uint64_t units = (uint64_t)a.n * a.s.kv_heads * (a.s.head_dim / 8);
-    const dim3 grid((uint32_t)((units + 255) / 256), a.planes);
-    if (bf16) k_kv4_write<true><<<grid, 256, 0, stream>>>(a);
-    else k_kv4_write<false><<<grid, 256, 0, stream>>>(a);
-    return hipGetLastError();
+    return kv_rows_launch(a, bf16, [&](dim3 grid, const wh_kv4_rows_args& b) {
+        if (bf16) k_kv4_write<true><<<grid, 256, 0, stream>>>(b);
+        else k_kv4_write<false><<<grid, 256, 0, stream>>>(b);
+    });
 }
 
 hipError_t wh_kv4_read_launch(const wh_kv4_rows_args& a, bool bf16, hipStream_t stream) {
-    const uint64_t units = (uint64_t)a.n * a.s.kv_heads * (a.s.head_dim / 8);
-    const dim3 grid((uint32_t)((units + 255) / 256), a.planes);
-    if (bf16) k_kv4_read<true><<<grid, 256, 0, stream>>>(a);
-    else k_kv4_read<false><<<grid, 256, 0, stream>>>(a);
-    return hipGetLastError();
+    return kv_rows_launch(a, bf16, [&](dim3 grid, const wh_kv4_rows_args& b) {
+        if (bf16) k_kv4_read<true><<<grid, 256, 0, stream>>>(b);
+        else k_kv4_read<false><<<grid, 256, 0, stream>>>(b);
+    });
 }
 
 // Wide tiles, of 64 rows (f32: 32), against narrow ones of 16, whose product wastes

@@ -25,6 +25,13 @@ WH_KV_HD uint64_t wh_kv4_line(uint32_t page, uint32_t head, uint32_t row, uint32
     return ((((uint64_t)page * kv_heads) + head) << shift) + row;
 }
 
+// Rows of a call that one launch takes, of `pieces` work-items each (at most 65535
+// heads of 64): 2^31 items, well below the 2^32 of a grid dimension.
+WH_KV_HD uint64_t wh_kv4_rows_of_launch(uint64_t n, uint64_t pieces) {
+    const uint64_t most = (1ull << 31) / pieces;
+    return n < most ? n : most;
+}
+
 // A slot's page, or false when the slot is none or behind the cache.
 WH_KV_HD bool wh_kv4_slot_page(uint32_t slot, uint32_t shift, uint32_t n_pages, uint32_t* page, uint32_t* row) {
     *page = slot >> shift;

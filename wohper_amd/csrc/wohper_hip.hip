@@ -4690,7 +4690,7 @@ int kv4_rows_args(const wh_kv4_cache* cache, void* k, size_t k_stride, void* v, 
     if (out ? !k && !v : !k || (has_v && !v)) return WH_INVALID_ARGUMENT;
     if (n && !slots) return WH_INVALID_ARGUMENT;
     const size_t width = cache->kv_heads * cache->head_dim;
-    if (n > 0x7fffffffu || n * (width / 8) > (size_t)0x7fffffff * 256) return WH_UNSUPPORTED;
+    if (n > 0x7fffffffu) return WH_UNSUPPORTED;
     if (k) {
         WH_TRY(kv4_row_check(k, k_stride, width, bf16));
         a->plane[0] = {cache->k_codes, cache->k_scales};
@@ -4786,8 +4786,6 @@ int wh_kv4_attention_async(wh_ctx* c, const wh_kv4_cache* cache, const wh_kv4_at
     if (d->n_tokens > 0x3fffffffu || d->n_requests > 0x3fffffffu || d->heads > 65536 ||
         d->n_tokens * group > 0x3fffffffu || d->table_stride > 0xffffffffu)
         return WH_UNSUPPORTED;
-    std::lock_guard<std::recursive_mutex> lk(c->mu);
-    WH_HIP(hipSetDevice(c->device));
     a.k = {cache->k_codes, cache->k_scales};
     a.v = has_v ? wh_kv4_plane{cache->v_codes, cache->v_scales} : a.k;
     a.q = d->q_dev;
@@ -4806,8 +4804,12 @@ int wh_kv4_attention_async(wh_ctx* c, const wh_kv4_cache* cache, const wh_kv4_at
     a.window = d->window > 0x7fffffffu ? 0 : (uint32_t)d->window;
     a.first = (uint32_t)std::min<size_t>(d->first, 0x7fffffffu);
     a.scale_log2 = d->scale * 1.44269504088896340736f;
-    a.status = c->status;
     const wh_kv4_attn_plan p = wh_kv4_attn_plan_of(a, d->is_bf16 != 0, d->max_len);
+    // a grid has less than 2^32 threads, up to 512 a workgroup
+    if ((uint64_t)p.units * cache->kv_heads > 0x7fffffu) return WH_UNSUPPORTED;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    WH_HIP(hipSetDevice(c->device));
+    a.status = c->status;
     a.units = p.units;
     a.min_runs = p.min_runs;
     a.n_tiles = p.n_tiles;
