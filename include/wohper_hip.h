@@ -937,7 +937,7 @@ typedef struct {
     size_t table_stride;
     size_t max_len;
     size_t heads;
-    float scale;
+    float scale;        /* finite, below 2^127 */
     size_t window;      /* 0: none */
     size_t first;
     const float* sink;  /* device [heads] or NULL */

@@ -1,5 +1,5 @@
-"""CPU checks of how large a call of the paged 4-bit cache may be: a grid
-dimension times its workgroup's threads stays below 2^32."""
+"""CPU checks of how large a call of the paged 4-bit cache may be (a grid
+dimension times its workgroup's threads stays below 2^32), and of its scale."""
 import ctypes
 import subprocess
 from pathlib import Path
@@ -7,7 +7,7 @@ from pathlib import Path
 import pytest
 
 import wohper_amd as wa
-from test_kv4_host import DEV, UNSUPPORTED, attention, cache, lib_and_ctx  # noqa: F401
+from test_kv4_host import ARGUMENT, UNSUPPORTED, attention, cache, lib_and_ctx  # noqa: F401
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -30,6 +30,14 @@ def test_too_many_workgroups_are_refused(lib_and_ctx, n_tokens, n_requests, kv_h
     a = attention(n_tokens=n_tokens, n_requests=n_requests, heads=kv_heads * group, q_stride=width, out_stride=width,
                   is_bf16=bf16, max_len=1 << 20)
     assert lib.wh_kv4_attention_async(ctx, ctypes.byref(c), ctypes.byref(a)) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3.4e38])
+def test_scales_that_are_not_finite_are_refused(lib_and_ctx, scale, bf16):  # noqa: F811
+    lib, ctx = lib_and_ctx
+    a = attention(scale=scale, is_bf16=bf16)
+    assert lib.wh_kv4_attention_async(ctx, ctypes.byref(cache()), ctypes.byref(a)) == ARGUMENT
 
 
 SOURCE = r"""

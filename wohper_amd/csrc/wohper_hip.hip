@@ -4779,7 +4779,7 @@ int wh_kv4_attention_async(wh_ctx* c, const wh_kv4_cache* cache, const wh_kv4_at
     if (d->heads == 0) return WH_EMPTY_SHAPE;
     if (d->heads % cache->kv_heads) return WH_INVALID_SHAPE;
     if (d->n_tokens == 0 || d->n_requests == 0) return WH_OK;
-    if (!d->starts_dev || !d->lens_dev || !d->tables_dev) return WH_INVALID_ARGUMENT;
+    if (!d->starts_dev || !d->lens_dev || !d->tables_dev || !std::isfinite(d->scale * 1.5f)) return WH_INVALID_ARGUMENT;
     const size_t width = d->heads * cache->head_dim, group = d->heads / cache->kv_heads;
     WH_TRY(kv4_row_check(d->q_dev, d->q_stride, width, d->is_bf16));
     WH_TRY(kv4_row_check(d->out_dev, d->out_stride, width, d->is_bf16));
