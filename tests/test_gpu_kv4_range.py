@@ -263,3 +263,27 @@ def test_scores_at_the_lower_end(ctx, layout, q, n, bf16):
     v = torch.from_numpy(c.cache.rows(1, c.slots[0][17:18])[0]).cuda()
     want = v.repeat_interleave(c.heads // c.kv_heads, 0).reshape(1, -1)
     assert bool(((got - want).abs() <= 4 * U * want.abs()).all())
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("layout,q", FORMS)
+def test_queries_that_are_not_finite(ctx, layout, q, value, bf16):
+    """They make their own head of their own token NaN."""
+    c = Case(q, [300], *LAYOUTS[layout], bf16, page=64, sink=True)
+    want = c.run(ctx).clone().reshape(-1, c.heads, c.d)
+    c.q[-1, (c.heads // 2) * c.d + 5] = value
+    c.out.fill_(7.0)
+    got = c.run(ctx).reshape(-1, c.heads, c.d)
+    nan = torch.zeros(len(got), c.heads, dtype=torch.bool, device="cuda")
+    nan[-1, c.heads // 2] = True
+    assert bool(torch.isnan(got[nan]).all()) and torch.equal(got[~nan], want[~nan])
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layout", ["group_8", "latent_64"])
+def test_a_prompt_among_single_tokens(ctx, layout, bf16):
+    """One prompt of 2000 tokens beside 95 requests of one: one call, any mix."""
+    q = [1] * 50 + [2000] + [1] * 45
+    lens = [1 + (b * 37) % 900 for b in range(50)] + [2100] + [1 + (b * 53) % 700 for b in range(45)]
+    Case(q, lens, *LAYOUTS[layout], bf16, page=16, behind=5).check(ctx)
