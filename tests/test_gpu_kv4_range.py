@@ -9,7 +9,7 @@ it bits.  So the tolerance has no term of the largest |v|:
   delta: a score's error, (d + 12) u scale sum |q||k| for d f32 products, the
     query's two f16 parts and three factors (the second part ends 2^-48 below the
     query's largest value, 2^-25 where keys are 2^23 the other way); bf16 queries (two E4M3 parts of 32
-    values) add 8 d u of the largest |q||k|
+    values) add 8 u of the largest |q| times the largest |k| for each of a group's dims
   S: the largest score, whose rounding in the exponent the weights carry; where
     the weight's reference includes a value's exponent, at most 40 and 6 more of
     such powers of two: 48 u
@@ -56,8 +56,9 @@ def bound(c, tiny=0.0):
             w = torch.exp(s - top[:, None])
             w = w / (w.sum(1) + torch.exp(sink - top))[:, None]
             ab = torch.where(see, q[:, h].abs() @ k.abs().T, 0.0).amax(1)
-            km = torch.where(see, k.abs().amax(1)[None], 0.0).amax(1)
-            delta = abs(c.scale) * ((d + 12) * U * ab + (8 * d * U * q[:, h].abs().amax(1) * km if c.bf16 else 0.0))
+            qg, kg = q[:, h].abs().reshape(nq, -1, 32).amax(2), k.abs().reshape(n, -1, 32).amax(2)
+            by_group = torch.where(see, 32 * (qg @ kg.T), 0.0).amax(1)
+            delta = abs(c.scale) * ((d + 12) * U * ab + (8 * U * by_group if c.bf16 else 0.0))
             big = torch.where(see, s.abs(), 0.0).amax(1)
             rel = 2 * delta + 4 * U * big + 48 * U + (2 * see.sum(1) + 16) * U + (2.0 ** -11 if c.bf16 else 2.0 ** -22)
             out[:, h] = w @ v
@@ -287,3 +288,17 @@ def test_a_prompt_among_single_tokens(ctx, layout, bf16):
     q = [1] * 50 + [2000] + [1] * 45
     lens = [1 + (b * 37) % 900 for b in range(50)] + [2100] + [1 + (b * 53) % 700 for b in range(45)]
     Case(q, lens, *LAYOUTS[layout], bf16, page=16, behind=5).check(ctx)
+
+
+@pytest.mark.parametrize("layout,q", [("pairs", [3]), ("group_8", [2]), ("group_8", [70]), ("group_5", [30]), ("wide", [3]), ("latent", [1])])
+def test_query_groups_far_apart(ctx, layout, q):
+    """f32 queries that are 2^40 larger in a group of 32 dims where the keys are
+    zero: the other groups make the scores."""
+    c = Case(q, [130], *LAYOUTS[layout], False, page=64, q_scale=1.0)
+    up = torch.ones(c.heads * c.d, device="cuda").reshape(c.heads, c.d)
+    up[:, 32:64] = 2.0 ** 40
+    c.q.mul_(up.reshape(-1))
+    sizes = np.ones((130, c.d // 32))
+    sizes[:, 1] = 0.0
+    c.cache.fill(0, c.slots[0], rows(c, seed=9, sizes=sizes))
+    check(c, ctx)

@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(256) k_kv4_read(wh_kv4_rows_args a) {
 // its f32 sums.  f32: keys decoded to f16 against their row's largest scale byte
 // (exact down to 2^-23 of that, kKeyNear; what lies further apart kv_plain_part
 // takes, as below) and the query as two f16 parts, the second times 2^10: 22 bits,
-// and 2^-48 of its largest value, which times 2^23 is 2^-25 of a term again where
-// queries are small and keys large.  Outputs:
+// and 2^-48 of its largest value, which is 2^-24 of that of a group of 32 dims up to
+// 2^24 below (kQueryNear).  Outputs:
 // values are f16 against their row's largest scale byte, exact down to 2^-23 of it,
 // and that byte's power of two goes into the weight.  Weights are f16, times 2^8,
 // against a reference of each query row: the largest score plus value exponent of
@@ -402,6 +402,7 @@ constexpr float kUp = 8.0f;
 constexpr float kMost = 65504.0f;
 constexpr uint32_t kApart = 0xffffffffu;  // past every run
 constexpr int kKeyNear = 23;              // f32: a key group's scale byte is at most so far below its row's
+constexpr int kQueryNear = 24;            // f32: a query's group's exponent is at most so far below the row's
 constexpr float kLowPart = 1024.0f;       // f32: what a query's second f16 part is multiplied by
 constexpr int kNear = 9;                  // a value group's scale byte is at most so far below its row's
 constexpr uint32_t kLow = 127 - 40, kHigh = 127 + 40;  // and the row's in here
@@ -704,17 +705,25 @@ struct wh_kv4_query {
 
     // factor[row]: what a sum of products with the row is to be multiplied by,
     // `scale` included.  Sums are below 2^26: whether that takes finite ones past
-    // f32 before the key's power of two brings them back, or is subnormal itself.
+    // f32 before the key's power of two brings them back, or is subnormal itself;
+    // or a group of 32 dims lies too far below the row's largest value.
     __device__ __forceinline__ bool put(uint32_t wave, uint32_t lane, _Float16* lds, float* factor, float scale) const {
         bool far = false;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            uint32_t top = 0;
+            // the largest of each group of 32 dims, eight lanes, and of the row
+            uint32_t top = 0, low = 0x7fffffffu;
 #pragma unroll
-            for (int k = 0; k < HD / 64; ++k)
+            for (int k = 0; k < HD / 64; ++k) {
+                uint32_t group = 0;
 #pragma unroll
-                for (int n = 0; n < 4; ++n) top = max(top, raw[i][k][n] & 0x7fffffffu);
+                for (int n = 0; n < 4; ++n) group = max(group, raw[i][k][n] & 0x7fffffffu);
+                group = kv_near_max<8>(group);
+                top = max(top, group);
+                low = min(low, group - 1);  // zeros are of no size
+            }
             top = kv_row_max(top);
+            far |= top < 0x7f800000u && (int)(top >> 23) - (int)((low + 1) >> 23) > kQueryNear;
             const int e = max((int)(top >> 23), 27);  // of the largest; 2^-100 at least, so that the factor is finite
             const float up = kv_bits((uint32_t)(127 + 13 + 127 - e) << 23);
             const uint32_t r = row(i, wave, lane);
