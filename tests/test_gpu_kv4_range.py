@@ -302,3 +302,28 @@ def test_query_groups_far_apart(ctx, layout, q):
     sizes[:, 1] = 0.0
     c.cache.fill(0, c.slots[0], rows(c, seed=9, sizes=sizes))
     check(c, ctx)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("layout,q", [("pairs", [3]), ("group_8", [2]), ("group_8", [70]), ("group_5", [30]), ("wide", [3]), ("latent", [1]),
+                                      ("latent_16", [1]), ("latent_256", [3]), ("latent_64", [50])])
+def test_scale_byte_0(ctx, layout, q, bf16):
+    """A group whose byte is 0 stands for zeros, whatever its codes: in rows
+    read, in scores of queries of 2^125, in values."""
+    for size in (1.0, 2.0 ** -60):  # products of f16, and the plain way
+        c = Case(q, [100], *LAYOUTS[layout], bf16, page=64, q_scale=1.0)
+        for k in range(len(c.cache.planes)):
+            c.cache.fill(k, c.slots[0], rows(c, seed=k) * (size if k else 1.0))
+        for codes, scales in c.cache.planes:
+            scales[..., 1] = 0
+        up = torch.ones(c.heads, c.d, device="cuda")
+        up[:, 32:64] = 2.0 ** 123
+        c.q.copy_((c.q.double() * up.reshape(-1)).to(c.q.dtype))
+        check(c, ctx)
+    slots = torch.from_numpy(c.slots[0].astype(np.int32)).cuda()
+    width = c.kv_heads * c.d
+    out = torch.full((100, width), 7.0, dtype=c.dt, device="cuda")
+    torch.cuda.synchronize()
+    ctx.kv4_read_async(c.cache.c, ptr(slots), 100, ptr(out), width, None, 0, bf16)
+    ctx.synchronize()
+    assert np.array_equal(out.double().cpu().numpy(), c.cache.rows(0, c.slots[0]).reshape(100, -1))

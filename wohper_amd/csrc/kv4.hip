@@ -342,9 +342,9 @@ __global__ void __launch_bounds__(256) k_kv4_read(wh_kv4_rows_args a) {
     const uint32_t i = (uint32_t)(unit / per), piece = (uint32_t)(unit - (uint64_t)i * per);
     const wh_kv4_at at = kv_at(a, a.slots[i], piece);
     if (!at.ok) return;
-    const uint32_t c = ((const uint32_t*)a.plane[pl].codes)[at.code];
     const uint32_t byte = a.plane[pl].scales[at.scale];
-    const float scale = kv_bits(byte << 23);  // 0 -> 0.0; 255 -> the conversion gives NaN
+    const uint32_t codes = ((const uint32_t*)a.plane[pl].codes)[at.code], c = byte ? codes : 0;
+    const float scale = kv_bits(byte << 23);  // of 0 the conversion makes 2^-127, of 255 NaN
     wh_f2 v[4];
     v[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 0);
     v[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 1);
@@ -652,12 +652,12 @@ __device__ __forceinline__ _Float16 kv_value_rel(uint32_t b, uint32_t vexp) {
     x.u = (uint16_t)((min(max((int)b - (int)vexp, -15), 0) + 15) << 10);
     return x.h;
 }
-// Whether a group of a key row (top: its largest byte) is not held by f16.
-__device__ __forceinline__ bool kv_key_odd(uint32_t b, uint32_t top) { return ((int)top - (int)b > kKeyNear) & (b != 0) & (top != 255); }
-// Whether a group of a value row (top: its largest byte) is NaN or not held by f16
-// products.  Not where the group is zeros: byte 0.
+// The same of a key row's group, in f32.
+__device__ __forceinline__ bool kv_key_odd(uint32_t b, uint32_t top) { return (int)top - (int)b > kKeyNear; }
+// Whether a group of a value row (top: its largest byte) is to be looked at: not held
+// by f16 products, or NaN, or zeros.
 __device__ __forceinline__ bool kv_value_odd(uint32_t b, uint32_t top, uint32_t vexp) {
-    return (((int)b - (int)vexp < -kNear) | (vexp != top)) & (b != 0);
+    return ((int)b - (int)vexp < -kNear) | (vexp != top);
 }
 
 // First dim of a lane's eight in step s of the product with keys.
@@ -880,8 +880,10 @@ __device__ __forceinline__ void kv_plain_part(const wh_kv4_attn_args& a, const w
             float s = 0.0f;
 #pragma unroll 1
             for (int n = 0; n < HD / 32; ++n) {
-                const wh_u4 codes = *(const wh_u4*)(a.k.codes + line * (HD / 2) + 16 * n);
-                const float scale = kv_bits((uint32_t)a.k.scales[line * (HD / 32) + n] << 23);
+                const uint32_t byte = a.k.scales[line * (HD / 32) + n];
+                const float scale = kv_bits(byte << 23);
+                wh_u4 codes = *(const wh_u4*)(a.k.codes + line * (HD / 2) + 16 * n);
+                if (byte == 0) codes = (wh_u4){0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const wh_f2 k[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 0),
@@ -930,6 +932,7 @@ __device__ __forceinline__ void kv_plain_part(const wh_kv4_attn_args& a, const w
                 else code = *codes;
                 const uint32_t byte = a.v.scales[at * (HD / 32) + lane * kPer / 32];
                 const float scale = kv_bits(seen >> j & 1 ? byte << 23 : 0u);
+                if (byte == 0) code = 0;
                 if constexpr (kPer == 1) {
                     const wh_f2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 0);
                     o[0] = fmaf(pj, lane & 1 ? v.y : v.x, o[0]);
@@ -1117,10 +1120,13 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                 const uint32_t vtop = kLatent && !kDirect ? kbytes : kv_top_byte(raw_v, h), vexp = kv_value_top(vtop);
                 // value scales, and the powers of two of keys and value rows
                 bool odd = false;
-                if constexpr (!kDirect && !kLatent) {  // a latent row's groups are values too, and kNear is less
-                    const uint32_t pieces = kv_piece_scales(kr, h, g);
+                const uint32_t kpieces = kDirect ? kbytes : kv_piece_scales(kr, h, g);
+                if constexpr (!kLatent) {  // a latent row's groups are values too, and kNear is less
 #pragma unroll
-                    for (int j = 0; j < kPieces; ++j) odd |= kv_key_odd((pieces >> (8 * j)) & 0xff, kbytes);
+                    for (int j = 0; j < kPieces; ++j) {
+                        const uint32_t b = (kpieces >> (8 * j)) & 0xff;
+                        odd |= kDirect ? b == 0 : kv_key_odd(b, kbytes);
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
@@ -1129,7 +1135,19 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                     if (HD > 64 || g < 2) rel[(4 * j + g) * W::kRel + at] = kv_value_rel(e, vexp);
                 }
                 const uint64_t odds = __ballot(odd);
-                if (__builtin_expect(odds != 0, 0)) apart |= odd && vtop != 255 && wh_kv4_seen(tile, key0, key0 + key) == key0 + key;
+                if (__builtin_expect(odds != 0, 0)) {
+                    bool far = false;  // a group of a row without NaN, not zeros
+#pragma unroll
+                    for (int j = 0; j < kPieces; ++j) {
+                        const uint32_t kb = (kpieces >> (8 * j)) & 0xff, vb = (vbytes >> (8 * j)) & 0xff;
+                        if constexpr (kDirect)  // the instruction takes a byte of 0 as 2^-127
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) kr.c[h][j][k] = kb ? kr.c[h][j][k] : 0;
+                        far |= vb != 0 && vtop != 255 && kv_value_odd(vb, vtop, vexp);
+                        if constexpr (!kDirect && !kLatent) far |= kb != 0 && kbytes != 255 && kv_key_odd(kb, kbytes);
+                    }
+                    apart |= far && wh_kv4_seen(tile, key0, key0 + key) == key0 + key;
+                }
                 if (g == 0) {
                     pow_s[key] = kv_bits(vexp << 23);
                     if constexpr (!kDirect) key_s[key] = kv_key_scale(kbytes, vtop);
@@ -1431,6 +1449,11 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         bool odd = false;
         if constexpr (kF32) ktop = row_top(kb);
         if (W::kBoth || has_keys) {
+            if constexpr (!kF32)  // the instruction takes a byte of 0 as 2^-127
+#pragma unroll
+                for (int i = 0; i < W::kMine; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) kc[i][k] = (kb >> (8 * i)) & 0xff ? kc[i][k] : 0;
             uint8_t* const kd = smem + run % W::kKeyBufs * W::kCodes + my_key * W::kRow;
 #pragma unroll
             for (int i = 0; i < W::kMine; ++i) *(wh_u4*)(kd + 16 * ((my_chunk + i) ^ swizzle(my_key))) = kc[i];
@@ -1443,10 +1466,10 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
             }
             if constexpr (kF32) {
                 if (my_chunk == 0) ((float*)(smem + W::kAtKeys))[(run & 1) * 64 + my_key] = kv_key_scale(ktop, 0);
-                if constexpr (!kLatent)  // a latent row's groups are values too, and kNear is less
-#pragma unroll
-                    for (int i = 0; i < W::kMine; ++i) odd |= kv_key_odd((kb >> (8 * i)) & 0xff, ktop);
             }
+            if constexpr (kF32 && !kLatent)  // a latent row's groups are values too, and kNear is less
+#pragma unroll
+                for (int i = 0; i < W::kMine; ++i) odd |= kv_key_odd((kb >> (8 * i)) & 0xff, ktop);
         }
         if (W::kBoth || has_values) {
             const uint32_t bytes = value_bytes();
@@ -1468,10 +1491,20 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
         }
         if (__builtin_expect(__ballot(odd) != 0, 0)) {
             asm volatile("");
+            bool far = false;  // a group of a row without NaN, not zeros
+#pragma unroll
+            for (int i = 0; i < W::kMine; ++i) {
+                const uint32_t k = (kb >> (8 * i)) & 0xff, v = (value_bytes() >> (8 * i)) & 0xff;
+                if (W::kBoth || has_keys) {
+                    if constexpr (kF32 && !kLatent) far |= k != 0 && ktop != 255 && kv_key_odd(k, ktop);
+                }
+                if (W::kBoth || has_values) far |= v != 0 && vtop != 255 && kv_value_odd(v, vtop, kv_value_top(vtop));
+            }
             const uint32_t key0 = run_at(run);  // the last run's once more: so too its keys
-            if (odd && wh_kv4_seen(tile, key0, key0 + my_key) == key0 + my_key) {  // some row may see this lane's key
-                if (vtop != 255) atomicMax(&raise[now & 1], kApart);
-                else if constexpr (!kLatent) atomicOr((unsigned long long*)&nan_keys[run % 3], 1ull << my_key);
+            if (wh_kv4_seen(tile, key0, key0 + my_key) == key0 + my_key) {  // some row may see this lane's key
+                if (far) atomicMax(&raise[now & 1], kApart);
+                if constexpr (!kLatent)
+                    if (vtop == 255) atomicOr((unsigned long long*)&nan_keys[run % 3], 1ull << my_key);
             }
         }
     };
