@@ -910,20 +910,27 @@ int wh_kv4_read_async(wh_ctx* ctx, const wh_kv4_cache* cache, const uint32_t* sl
  * 16-byte aligned with strides of a multiple of 16 bytes; rows from
  * starts_dev[n_requests] on are left as they are.  q and out must not
  * overlap.
- * max_len: at least the largest of lens_dev; it only sizes the split of long
- * key lists and the context's scratch for it, not the result.  A table entry
- * of n_pages or more, or a length above table_stride * page_size, reports
- * WH_NOT_RESIDENT; entries of pages that no token sees a row of are not looked
- * at, so pages behind a window can be given back (0xFFFFFFFF in their place).
+ * max_len: at least the largest of lens_dev.  It and n_tokens, where starts_dev
+ * ends before it, only size the call: which kernel runs, how long key lists are
+ * split and the context's scratch for that.  So with other bounds a result may
+ * differ by the rounding of its f32 sums, and with loose ones take longer.  The
+ * same call repeats bit for bit.
+ * A table entry of n_pages or more, or a length above table_stride * page_size,
+ * reports WH_NOT_RESIDENT; entries of pages that no token sees a row of are not
+ * looked at, so pages behind a window can be given back (0xFFFFFFFF in their
+ * place).
  * A visible row that holds NaN makes its heads' outputs NaN.  A row that a
  * token does not see takes nothing from that token's output, whatever its
- * bytes, nor does one of no weight, nor do other dims: sums are f32 in both
+ * bytes, nor does one of no weight, nor do other dims.  Sums are f32 in both
  * types and in both numerics modes, and an f32 result is within f32 rounding
- * of the sums of w |v|, |v| being the largest of the value's group of 32 dims.
- * A tile of tokens some of which see a row whose groups are more than 2^9
- * apart, or whose largest is not within 2^40 of 1, takes many times as long.
- * A call whose tiles (of 16 rows of a key head at least) times kv_heads may be
- * 2^23 or more is WH_UNSUPPORTED. */
+ * of the sums of w |v| and of |q| |k|, each |x| being the largest of the
+ * value's group of 32 dims; bf16 calls round a weight to 11 bits.
+ * Rows of ordinary sizes are taken by matrix instructions.  A tile of tokens
+ * takes 5 to 30 times as long if one of them sees a value row whose largest
+ * value is not within 2^40 of 1 or whose groups of 32 are more than 2^9 apart
+ * (bf16: 2^12), or, in f32, a key row with groups 2^23 or a query with groups
+ * 2^24 apart.  A call whose tiles (of 16 rows of a key head at least) times
+ * kv_heads may be 2^23 or more is WH_UNSUPPORTED. */
 typedef struct {
     const void* q_dev;
     size_t q_stride;

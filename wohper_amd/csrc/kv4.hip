@@ -387,13 +387,15 @@ __global__ void __launch_bounds__(256) k_kv4_read(wh_kv4_rows_args a) {
 //
 // f16 ends 2^-33 below the reference.  A group of 32 dims that lies as high as its
 // row keeps 2^-33 of its largest term, one that lies 2^9 below it 2^-24, which is
-// what an f32 sum rounds a term by too.  Values past that (kNear), or whose powers
-// of two are too far from 1 for f32 sums of weights under such references (kLow,
-// kHigh), are left to kv_plain_part, which takes the workgroup's part in f32: ten
-// to thirty times as long, for rows no model is known to make.
+// what an f32 sum rounds a term by too; bf16 calls, whose outputs round by 2^-9, allow
+// 2^12.  Values past that (kNear), or whose powers of two are too far from 1 for f32
+// sums of weights under such references (kLow, kHigh), are left to kv_plain_part,
+// which takes the workgroup's part in f32.  That takes five (one short list) to thirty
+// times as long (a chunk of 384 tokens, all of whose tiles see such a row).
 
 #define kMinusInf (-__builtin_inff())
-constexpr float kMinusBig = -3.402823466e38f;  // the reference of no key: finite, so that differences are, and below every score
+constexpr float kMaxFloat = 3.402823466e38f;
+constexpr float kMinusBig = -kMaxFloat;  // the reference of no key: finite, so that differences are, and below every score
 // Weights are held times 2^kUp: f16 keeps small ones.  A row's reference is raised
 // to its largest score once a weight is past f16, 2^8 above: with 2^5 the prompts of
 // k_kv4_attn_packed took 290 us for 243.  Rows raise theirs by themselves: that
@@ -404,7 +406,8 @@ constexpr uint32_t kApart = 0xffffffffu;  // past every run
 constexpr int kKeyNear = 23;              // f32: a key group's scale byte is at most so far below its row's
 constexpr int kQueryNear = 24;            // f32: a query's group's exponent is at most so far below the row's
 constexpr float kLowPart = 1024.0f;       // f32: what a query's second f16 part is multiplied by
-constexpr int kNear = 9;                  // a value group's scale byte is at most so far below its row's
+template <bool kF32>
+constexpr int kNear = kF32 ? 9 : 12;      // a value group's scale byte is at most so far below its row's
 constexpr uint32_t kLow = 127 - 40, kHigh = 127 + 40;  // and the row's in here
 
 // The tile of slot x: a search over the requests, 64 candidates a step.
@@ -656,8 +659,9 @@ __device__ __forceinline__ _Float16 kv_value_rel(uint32_t b, uint32_t vexp) {
 __device__ __forceinline__ bool kv_key_odd(uint32_t b, uint32_t top) { return (int)top - (int)b > kKeyNear; }
 // Whether a group of a value row (top: its largest byte) is to be looked at: not held
 // by f16 products, or NaN, or zeros.
+template <bool kF32>
 __device__ __forceinline__ bool kv_value_odd(uint32_t b, uint32_t top, uint32_t vexp) {
-    return ((int)b - (int)vexp < -kNear) | (vexp != top);
+    return ((int)b - (int)vexp < -kNear<kF32>) | (vexp != top);
 }
 
 // First dim of a lane's eight in step s of the product with keys.
@@ -849,115 +853,156 @@ __device__ __forceinline__ void kv_put_sum(float* to, float m, float l) {
     to[1] = __builtin_amdgcn_frexp_mantf(l);
 }
 
-// A workgroup's part of a tile in plain f32: for values, or in f32 calls keys, that
-// f16 products do not hold (above).  A wave takes a row at a time, a lane a key of
-// its score and HD / 64 dims of its output.  The output is kept divided by the sum
-// of weights so far, so it stays within the values' size whatever that is.  Bound by
-// instruction issue: some 1.5 HD instructions of scores and 10 of outputs for a row
-// and 64 keys, where the tiles above decode a key once for all their rows.
-template <int HD, bool kF32, bool kLatent, int kRows>
-__device__ __forceinline__ void kv_plain_part(const wh_kv4_attn_args& a, const wh_kv4_place& place, uint32_t wave, uint32_t waves) {
+// A workgroup's part of a tile in plain f32: for values, or in f32 calls queries and
+// keys, that f16 products do not hold (above).  A wave takes up to eight rows, a lane
+// a key of their scores and HD / 64 dims of their outputs.  Outputs are kept divided
+// by the sum of weights so far, so they stay within the values' size whatever that
+// is.  Bound by instruction issue: HD products a row and key, without the matrix
+// instructions.
+template <int HD, bool kF32, bool kLatent, int kRows, int kWaves>
+__device__ __forceinline__ void kv_plain_part(const wh_kv4_attn_args& a, const wh_kv4_place& place, uint32_t wave) {
     constexpr int kPer = HD / 64;  // dims of a lane
+    constexpr int kMany = kRows / kWaves < 8 ? kRows / kWaves : 8;
     const uint32_t lane = threadIdx.x & 63, kvh = place.head, pmask = (1u << a.s.shift) - 1u;
     const wh_kv4_tile& tile = place.tile;
     const uint32_t run0 = place.split ? place.split * place.chunk : 0, run1 = min(tile.runs, run0 + place.chunk);
+    const bool whole = place.chunk >= tile.runs;
     const uint32_t* const table = a.tables + tile.request * a.table_stride;
     bool bad = false;
-    for (uint32_t row = wave; row < tile.rows; row += waves) {
-        const uint32_t flat = tile.row0 + row, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
-        const int32_t pos = tile.len - (int32_t)tile.n_q + (int32_t)tok;
-        const uint64_t at_q = (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)head * HD;
-        float m = kMinusBig, l = 0.0f, o[kPer];
+    for (uint32_t first = kMany * wave; first < tile.rows; first += kMany * kWaves) {
+        uint64_t at_q[kMany];
+        int32_t pos[kMany];
+        float m[kMany], l[kMany], o[kMany][kPer];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) o[i] = 0.0f;
+        for (int r = 0; r < kMany; ++r) {
+            const uint32_t flat = tile.row0 + min(first + r, tile.rows - 1), tok = flat / a.group;
+            pos[r] = tile.len - (int32_t)tile.n_q + (int32_t)tok;
+            at_q[r] = (uint64_t)(tile.token0 + tok) * a.q_stride + (uint64_t)(kvh * a.group + (flat - tok * a.group)) * HD;
+            m[r] = kMinusBig;
+            l[r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) o[r][i] = 0.0f;
+        }
         for (uint32_t run = run0; run < run1; ++run) {
             const uint32_t key0 = wh_kv4_run(tile, run), key = key0 + lane;
-            const bool sees = (int64_t)key <= pos && (!a.window || (int64_t)key > (int64_t)pos - a.window || key < a.first);
+            const bool some = wh_kv4_seen(tile, key0, key) == key;
             const uint32_t page = table[wh_kv4_seen(tile, key0, key) >> a.s.shift];
             const bool out = page >= a.s.n_pages;
             bad |= out;
             const uint64_t line = wh_kv4_line(out ? 0 : page, kvh, key & pmask, a.s.kv_heads, a.s.shift);
-            float s = 0.0f;
+            float s[kMany];
+#pragma unroll
+            for (int r = 0; r < kMany; ++r) s[r] = 0.0f;
+            uint32_t n0 = 0;
+            asm volatile("" : "+s"(n0));  // queries are not to be held over the runs: there are no registers
 #pragma unroll 1
-            for (int n = 0; n < HD / 32; ++n) {
+            for (uint32_t n = n0; n < HD / 32; ++n) {
                 const uint32_t byte = a.k.scales[line * (HD / 32) + n];
                 const float scale = kv_bits(byte << 23);
                 wh_u4 codes = *(const wh_u4*)(a.k.codes + line * (HD / 2) + 16 * n);
                 if (byte == 0) codes = (wh_u4){0, 0, 0, 0};
+                float k[32];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const wh_f2 k[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 0),
+                    const wh_f2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 0),
                                         __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 1),
                                         __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 2),
                                         __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], scale, 3)};
-                    float q[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) k[8 * i + e] = e & 1 ? v[e >> 1].y : v[e >> 1].x;
+                }
+#pragma unroll
+                for (int r = 0; r < kMany; ++r) {
+                    __builtin_amdgcn_sched_barrier(0);  // nor all rows' at once
+                    // sixteen bytes that all lanes read
                     if constexpr (kF32) {
 #pragma unroll
-                        for (int d = 0; d < 2; ++d) {
-                            const wh_f4 x = *(const wh_f4*)((const float*)a.q + at_q + 32 * n + 8 * i + 4 * d);
+                        for (int h = 0; h < 8; ++h) {
+                            const wh_f4 q = *(const wh_f4*)((const float*)a.q + at_q[r] + 32 * n + 4 * h);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) q[4 * d + e] = x[e];
+                            for (int e = 0; e < 4; ++e) s[r] = fmaf(q[e], k[4 * h + e], s[r]);
                         }
                     } else {
-                        const wh_u4 x = *(const wh_u4*)((const uint16_t*)a.q + at_q + 32 * n + 8 * i);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) q[e] = kv_bits(e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
+                        for (int h = 0; h < 4; ++h) {
+                            const wh_u4 q = *(const wh_u4*)((const uint16_t*)a.q + at_q[r] + 32 * n + 8 * h);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                s[r] = fmaf(kv_bits(e & 1 ? q[e >> 1] & 0xffff0000u : q[e >> 1] << 16), k[8 * h + e], s[r]);
+                        }
                     }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s = fmaf(q[e], e & 1 ? k[e >> 1].y : k[e >> 1].x, s);
                 }
             }
-            if constexpr (!kLatent) {  // a value row that holds NaN makes all of the output NaN
-                bool nan = false;
+            bool nan = false;  // a value row that holds NaN makes all of the output NaN
+            if constexpr (!kLatent)
 #pragma unroll 1
                 for (int n = 0; n < HD / 32; ++n) nan |= a.v.scales[line * (HD / 32) + n] == 255;
-                if (nan) s = kv_bits(0x7fc00000u);
-            }
-            s = sees ? s * a.scale_log2 : kMinusInf;
-            const float to = fmaxf(m, wh_wave_max(s)), f = l * __builtin_amdgcn_exp2f(m - to), w = __builtin_amdgcn_exp2f(s - to);
-            l = f + kv_wave_sum(w);
-            m = to;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l, p = w * inv;
+            float p[kMany];
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) o[i] *= f * inv;
-            const uint64_t seen = __ballot(sees);
+            for (int r = 0; r < kMany; ++r) {
+                const bool sees = (int64_t)key <= pos[r] && (!a.window || (int64_t)key > (int64_t)pos[r] - a.window || key < a.first);
+                const float x = !sees ? kMinusInf : nan ? kv_bits(0x7fc00000u) : s[r] * a.scale_log2;
+                const float to = fmaxf(m[r], wh_wave_max(x)), f = l[r] * __builtin_amdgcn_exp2f(m[r] - to), w = __builtin_amdgcn_exp2f(x - to);
+                l[r] = f + kv_wave_sum(w);
+                m[r] = to;
+                const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+                p[r] = w * inv;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) o[r][i] *= f * inv;
+            }
+            const uint64_t seen = __ballot(some);
 #pragma unroll 8
-            for (int j = 0; j < 64; ++j) {  // rows that are not seen count as zeros
+            for (int j = 0; j < 64; ++j) {
                 const uint64_t at = kv_lane(line, j);
-                const float pj = kv_bits((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(p), j));
                 const uint8_t* const codes = a.v.codes + at * (HD / 2) + lane * kPer / 2;
                 uint32_t code;
                 if constexpr (kPer == 8) code = *(const uint32_t*)codes;
                 else if constexpr (kPer == 4) code = *(const uint16_t*)codes;
                 else code = *codes;
-                const uint32_t byte = a.v.scales[at * (HD / 32) + lane * kPer / 32];
-                const float scale = kv_bits(seen >> j & 1 ? byte << 23 : 0u);
+                uint32_t byte = a.v.scales[at * (HD / 32) + lane * kPer / 32];
+                // finite for the rows that do not see it: their weight is 0
+                if (!(seen >> j & 1) || byte == 255) byte = 0;
                 if (byte == 0) code = 0;
+                const float scale = kv_bits(byte << 23);
+                float v[kPer];
                 if constexpr (kPer == 1) {
-                    const wh_f2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 0);
-                    o[0] = fmaf(pj, lane & 1 ? v.y : v.x, o[0]);
+                    const wh_f2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 0);
+                    v[0] = lane & 1 ? x.y : x.x;
                 } else {
                     wh_static_for<kPer / 2>([&](auto ic) {
                         constexpr int i = decltype(ic)::value;
-                        const wh_f2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, i);
-                        o[2 * i] = fmaf(pj, v.x, o[2 * i]);
-                        o[2 * i + 1] = fmaf(pj, v.y, o[2 * i + 1]);
+                        const wh_f2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, i);
+                        v[2 * i] = x.x;
+                        v[2 * i + 1] = x.y;
                     });
+                }
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) v[i] = fminf(fmaxf(v[i], -kMaxFloat), kMaxFloat);
+#pragma unroll
+                for (int r = 0; r < kMany; ++r) {
+                    const float pj = kv_bits((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(p[r]), j));
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) o[r][i] = fmaf(pj, v[i], o[r][i]);
                 }
             }
         }
-        float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * kRows + row) * (HD + 2);
-        const bool whole = place.chunk >= tile.runs;
-        float f = 1.0f;
-        if (whole && a.sink && l > 0.0f) f = l / (l + __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - m));
-        const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD + lane * kPer;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (!whole) part[lane * kPer + i] = o[i];
-            else if constexpr (kF32) ((float*)a.out)[at + i] = o[i] * f;
-            else ((__bf16*)a.out)[at + i] = (__bf16)(o[i] * f);
+        for (int r = 0; r < kMany; ++r) {
+            const uint32_t row = first + r;
+            if (row >= tile.rows) continue;
+            const uint32_t flat = tile.row0 + row, tok = flat / a.group, head = kvh * a.group + (flat - tok * a.group);
+            float* const part = a.part + (((uint64_t)place.unit * a.s.kv_heads + kvh) * kRows + row) * (HD + 2);
+            float f = 1.0f;
+            if (whole && a.sink && l[r] > 0.0f) f = l[r] / (l[r] + __builtin_amdgcn_exp2f(a.sink[head] * 1.44269504088896340736f - m[r]));
+            const uint64_t at = (uint64_t)(tile.token0 + tok) * a.out_stride + (uint64_t)head * HD + lane * kPer;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (!whole) part[lane * kPer + i] = o[r][i];
+                else if constexpr (kF32) ((float*)a.out)[at + i] = o[r][i] * f;
+                else ((__bf16*)a.out)[at + i] = (__bf16)(o[r][i] * f);
+            }
+            if (!whole && lane == 0) kv_put_sum(part + HD, m[r], l[r]);
         }
-        if (!whole && lane == 0) kv_put_sum(part + HD, m, l);
     }
     if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
 }
@@ -1131,7 +1176,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
                     const uint32_t e = (vbytes >> (8 * j)) & 0xff;
-                    odd |= kv_value_odd(e, vtop, vexp);
+                    odd |= kv_value_odd<kF32>(e, vtop, vexp);
                     if (HD > 64 || g < 2) rel[(4 * j + g) * W::kRel + at] = kv_value_rel(e, vexp);
                 }
                 const uint64_t odds = __ballot(odd);
@@ -1143,7 +1188,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
                         if constexpr (kDirect)  // the instruction takes a byte of 0 as 2^-127
 #pragma unroll
                             for (int k = 0; k < 4; ++k) kr.c[h][j][k] = kb ? kr.c[h][j][k] : 0;
-                        far |= vb != 0 && vtop != 255 && kv_value_odd(vb, vtop, vexp);
+                        far |= vb != 0 && vtop != 255 && kv_value_odd<kF32>(vb, vtop, vexp);
                         if constexpr (!kDirect && !kLatent) far |= kb != 0 && kbytes != 255 && kv_key_odd(kb, kbytes);
                     }
                     apart |= far && wh_kv4_seen(tile, key0, key0 + key) == key0 + key;
@@ -1276,7 +1321,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
     if (lane == 0) wave_apart[wave] = wave_is_apart;
     kv_lds_barrier();
     if (__builtin_expect(wave_apart[0] | wave_apart[1] | wave_apart[2] | wave_apart[3], 0)) {
-        kv_plain_part<HD, kF32, kLatent, 16>(a, place, wave, 4);
+        kv_plain_part<HD, kF32, kLatent, 16, 4>(a, place, wave);
         return;
     }
     float M = wave_m[0][r16], L = 0.0f;
@@ -1480,7 +1525,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
             for (int i = 0; i < W::kMine; ++i) {
                 const uint32_t b = (bytes >> (8 * i)) & 0xff;
                 rel[(my_chunk + i) * W::kRel + my_key] = kv_value_rel(b, vexp);
-                odd |= kv_value_odd(b, vtop, vexp);
+                odd |= kv_value_odd<kF32>(b, vtop, vexp);
             }
             ((float*)(smem + W::kAtPow))[(run & 1) * 64 + my_key] = kv_bits(vexp << 23);
             if constexpr (!kLatent) {
@@ -1498,7 +1543,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
                 if (W::kBoth || has_keys) {
                     if constexpr (kF32 && !kLatent) far |= k != 0 && ktop != 255 && kv_key_odd(k, ktop);
                 }
-                if (W::kBoth || has_values) far |= v != 0 && vtop != 255 && kv_value_odd(v, vtop, kv_value_top(vtop));
+                if (W::kBoth || has_values) far |= v != 0 && vtop != 255 && kv_value_odd<kF32>(v, vtop, kv_value_top(vtop));
             }
             const uint32_t key0 = run_at(run);  // the last run's once more: so too its keys
             if (wh_kv4_seen(tile, key0, key0 + my_key) == key0 + my_key) {  // some row may see this lane's key
@@ -1775,7 +1820,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
     }
     if (bad) atomicOr(a.status, WH_ST_NOT_RESIDENT);
     if (__builtin_expect(end < run1, 0)) {
-        kv_plain_part<HD, kF32, kLatent, kRows>(a, place, wave, kWaves);
+        kv_plain_part<HD, kF32, kLatent, kRows, kWaves>(a, place, wave);
         return;
     }
     if (run0 < run1) {
