@@ -1014,13 +1014,13 @@ __device__ __forceinline__ void kv_plain_part(const wh_kv4_attn_args& a, const w
 // value rows' codes go through the wave's own LDS as they lie and come back
 // transposed, sixteen keys of one dim a lane (the 4-bit transposing read), whose
 // source rows are chosen to be just these keys: a lane's weights are the operand
-// of the product with the values as they are.  Bound by instruction issue, which
-// is what few rows leave: a key's codes are decoded for 16 rows at most.  32 tokens,
-// up to 8192 keys, 8 heads on each of 8 key heads of 128, bf16: 54 us and 6 for the
-// join, vector instructions 41 % and matrix ones 17 % of the cycles, 3.6 TB/s of
-// cache (a copy: 4.9); 96 windows, 4 heads a key head, f32: 40 us.  Up to 128 dims
-// two waves a SIMD with all registers as vector ones: with accumulators aside, 32
-// copies a block, the first took 73 instead of 70 us.
+// of the product with the values as they are.  A key's codes are decoded for 16 rows
+// at most, which keeps every unit short of full: 32 tokens, up to 8192 keys, 8 heads
+// on each of 8 key heads of 128, bf16: 57 us and 6 for the join, 3.4 TB/s of cache (a
+// copy: 4.9), vector instructions 43 % and matrix ones 8 % of the cycles, waves
+// waiting for 35 % of theirs; 96 windows, 4 heads a key head, f32: 41 us.  Up to 128
+// dims two waves a SIMD with all registers as vector ones: one a SIMD, which puts
+// accumulators aside, takes 58.6 us in all instead of 56.5 and 41.5 instead of 40.4.
 template <int HD, bool kF32>
 struct wh_kv4_narrow {
     static constexpr bool kDirect = !kF32;                   // scores on codes as they lie
@@ -1374,18 +1374,19 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_kv4_attn(wh_kv4_attn
 // transposing read), decoded to small f16 numbers and multiplied by their powers
 // of two.  The two work on neighbouring runs at once, so one barrier a run is
 // enough and the matrix work of one covers the loads and exponentials of the
-// other.  Weights are taken against the running maximum as it is; only a run with
-// a score 2^5 above it (or a value row above the reference) joins the waves'
-// maxima and makes its weights again.
+// other.  Weights are taken against a row's reference as it is; only a run with a
+// weight past f16 joins the waves' maxima and makes its weights again.
 //
 // Four waves up to 128 dims, three a SIMD (prompts of up to 2500 tokens, 4 heads
-// on each of 8 key heads of 128, bf16: 264 us; in turn 288 and, with two a SIMD,
-// 334), eight above, where one workgroup takes a CU's registers.  Bound by
-// instruction issue: in those prompts vector instructions take 66 % of the cycles
-// and matrix ones 25 %, and LDS is busy for 44 %.  A chunk of 384 tokens, 64 heads
-// on one key head of 512, up to 4384 keys, bf16: 175 us, 0.71 PFLOP/s; 3 requests
-// of 5 tokens there, f32: 36 us and 7 for the join.  Value rows as f16 in LDS
-// instead of codes (each wave decoding what it scores) took 384 us for the prompts.
+// on each of 8 key heads of 128, bf16: 247 us; with tiles in the order of their
+// tokens 267 and, with two waves a SIMD, 305), eight above, where one workgroup takes
+// a CU's registers.  In those prompts vector instructions take 67 % of the cycles,
+// matrix ones 27 %, LDS 47 %, and waves wait for 27 % of theirs: instruction issue is
+// what is fullest.  Not so at 512 dims: a chunk of 384 tokens, 64 heads on one key
+// head, up to 2676 keys, bf16: 169 us, 0.73 PFLOP/s, vector instructions 38 % and
+// matrix ones 28 %, waves waiting for a third of their cycles, and 384 workgroups
+// are one and a half rounds; 12 tokens there, up to 40000 keys: 62 us and 11 for the
+// join, the same shares; 3 requests of 5 tokens, f32: 34 us and 7 for the join.
 template <int HD, bool kF32, bool kLatent>
 struct wh_kv4_packed {
     static constexpr int kRows = kF32 ? 32 : 64, kBlocks = kRows / 16;
@@ -1863,7 +1864,7 @@ __global__ void __launch_bounds__((wh_kv4_packed<HD, kF32, kLatent>::kThreads), 
 
 // Joins the workgroups of a tile: outputs weighted by their sums of weights, and
 // the sink.  A wave a row, four rows a workgroup.  Bound by latency (lengths, the
-// parts' maxima, the parts): 6 us for 4 parts of 256 tiles of 16 rows of 128, 10 us
+// parts' maxima, the parts): 6 us for 4 parts of 256 tiles of 16 rows of 128, 11 us
 // for 33 MB of 22 parts of 12 tiles of 64 rows of 512.
 template <int HD, bool kF32, int kRows>
 __global__ void __launch_bounds__(256) k_kv4_join(wh_kv4_attn_args a) {
@@ -2009,23 +2010,30 @@ hipError_t wh_kv4_read_launch(const wh_kv4_rows_args& a, bool bf16, hipStream_t 
 // less where a request has few rows and whose waves wait for nobody; by the rows
 // (tokens x heads of a key head) that requests have on average.  us, 16 requests of
 // one token and up to 6000 keys, narrow against wide:
-//  - f32, 512 dims: always wide.  8 rows 40.0 and 31.3, 64 rows 73.3 and 47.3;
-//  - from 256 dims on: over 16 rows.  bf16, 4 key heads of 256: 16 rows 35.8 and
-//    55.8, 24 rows 61.0 and 57.2, 64 rows 79.2 and 57.4; f32: 42.0 and 57.3, 73.6
-//    and 58.3, 102.6 and 102.4; bf16, one of 512: 34.4 and 33.5, 36.8 and 36.4,
-//    49.7 and 41.2;
-//  - up to 128 dims: bf16 over 48 rows, f32 over 64.  bf16, 8 key heads of 128: 48
-//    rows 53.5 and 58.2, 64 rows 57.7 and 56.0; f32: 48 rows 81.6 and 102.0, 64
-//    rows 86.4 and 92.9.  4 prompts of 2000 tokens, 4 rows a token: bf16 298 and
-//    161, f32 381 and 300.
+//  - f32, 512 dims: always wide (the narrow kernel, which is not kept, took 40 to 73
+//    for 8 to 64 rows, this one 30 to 45);
+//  - from 256 dims on: over 16 rows.  bf16, 4 key heads of 256: 16 rows 33 and 53, 24
+//    rows 59 and 53, 64 rows 74 and 54; f32: 39 and 55, 70 and 55, 97 and 95; bf16,
+//    one of 512: 35 and 33, 36 and 35, 50 and 40;
+//  - up to 128 dims: bf16 over 48 rows, f32 over 64.  bf16, 8 key heads of 128: 16
+//    rows 29 and 51, 32 rows 45 and 54, 48 rows 54 and 56, 64 rows 60 and 54; f32: 16
+//    rows 35 and 53, 24 rows 56 and 54, 32 rows 55 and 54, 48 rows 77 and 98, 64 rows
+//    79 and 88.  4 prompts of 2000 tokens, 4 rows a token: bf16 297 and 143, f32 363
+//    and 275.
+// Rows alone do not tell short prompts, where there are few tiles and few keys to
+// cut up.  16 of 20 to 40 tokens, 8 rows each, up to 1000 rows before them, narrow
+// against the wide tiles that they get: bf16, 8 key heads of 128: 60 and 74, 4 of 64:
+// 30 and 48; f32, 4 of 64: 36 and 51; but 8 of 128 in f32: 73 and 65, 4 of 256: 88
+// and 57 in bf16, 101 and 73 in f32.  Nor does an average tell one prompt among
+// single tokens, all of which get its tiles.
 //
 // With few tiles their keys are cut up.  Workgroups aimed at: those that the chip
 // holds at once; twice as many where that is less than four a tile, since whole
 // parts of requests of different lengths do not come out even (32 requests of up to
-// 8192 keys, 8 key heads of 128: 79, 74, 73 and 83 us for one, one and a half, two
-// and four rounds; 16 of up to 6000 with two wide tiles each, f32: 153 and 102 for
-// one and two); none where two rounds are less than three a tile (96 windows of
-// 1024 keys, 8 key heads: 41 us a workgroup a tile, 67 us cut up).
+// 8192 keys, 8 key heads of 128: 73, 61, 59 and 67 us for one, one and a half, two
+// and four rounds; 16 of up to 6000 with two wide tiles each, f32: 103, 98, 94 and
+// 107); none where two rounds are less than three a tile (96 windows of 1024 keys, 8
+// key heads: 40 us a workgroup a tile, 55 cut up in two rounds, 67 in four).
 wh_kv4_attn_plan wh_kv4_attn_plan_of(const wh_kv4_attn_args& a, bool bf16, size_t max_len) {
     wh_kv4_attn_plan p{};
     const uint64_t rows = (uint64_t)a.n_tokens * a.group;
