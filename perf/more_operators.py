@@ -96,7 +96,7 @@ class _State:
 
     def __del__(self):
         if self.weight is not None and _kept:
-            _kept["ctx"].store_release(self.weight)
+            _kept["ctx"].release(self.weight)
 
 
 def _float(bf16):
