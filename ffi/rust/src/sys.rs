@@ -185,6 +185,15 @@ pub struct WhKvPlan {
 
 /// Attention of new tokens over a 4-bit cache.
 #[repr(C)]
+#[derive(Clone, Copy)]
+pub struct WhFp8Rows {
+    pub codes: *mut u8,
+    pub stride: usize,
+    pub scales: *mut u8,
+    pub scale_stride: usize,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy, Debug)]
 pub struct WhKv4Attention {
     pub q_dev: *const c_void,
@@ -368,4 +377,26 @@ extern "C" {
                              is_bf16: c_int) -> c_int;
     pub fn wh_kv4_attention_async(ctx: *mut WhCtx, cache: *const WhKv4Cache,
                                   attention: *const WhKv4Attention) -> c_int;
+    pub fn wh_store_fp8_device(ctx: *mut WhCtx, weight_dev: *const u8, rows: usize, cols: usize,
+                               scales_dev: *const c_void, scale_rows: usize, scale_cols: usize,
+                               scale_format: c_int, out_: *mut WhTensor) -> c_int;
+    pub fn wh_fp8_quant_rows_async(ctx: *mut WhCtx, x_dev: *const c_void, x_stride: usize, is_bf16: c_int, n: usize,
+                                   cols: usize, out_: *const WhFp8Rows) -> c_int;
+    pub fn wh_fp8_swiglu_rows_async(ctx: *mut WhCtx, gate_dev: *const c_void, up_dev: *const c_void, stride: usize,
+                                    is_bf16: c_int, n: usize, cols: usize, limit: f32,
+                                    out_: *const WhFp8Rows) -> c_int;
+    pub fn wh_fp8_read_rows_async(ctx: *mut WhCtx, rows: *const WhFp8Rows, n: usize, cols: usize,
+                                  out_dev: *mut c_void, out_stride: usize, is_bf16: c_int) -> c_int;
+    pub fn wh_fp8_rows_mm_async(ctx: *mut WhCtx, w: WhTensor, row_start: usize, row_end: usize, x: *const WhFp8Rows,
+                                n: usize, y_dev: *mut c_void, y_stride: usize, is_bf16: c_int) -> c_int;
+    pub fn wh_fp8_rows_mm_groups_async(ctx: *mut WhCtx, w: WhTensor, row_start: usize, group_rows: usize,
+                                       n_groups: usize, x: *const WhFp8Rows, n_x: usize, rows_dev: *const u32,
+                                       starts_dev: *const u32, n: usize, y_dev: *mut c_void, y_stride: usize,
+                                       is_bf16: c_int) -> c_int;
+    pub fn wh_expert_plan_async(ctx: *mut WhCtx, ids_dev: *const u32, npos: usize, topk: usize, n_experts: usize,
+                                starts_dev: *mut u32, rows_dev: *mut u32, slots_dev: *mut u32) -> c_int;
+    pub fn wh_expert_combine_async(ctx: *mut WhCtx, y_dev: *const c_void, y_stride: usize, is_bf16: c_int,
+                                   n_rows: usize, slots_dev: *const u32, weights_dev: *const f32, npos: usize,
+                                   topk: usize, hidden: usize, add_dev: *const f32, add_stride: usize,
+                                   out_dev: *mut f32, out_stride: usize) -> c_int;
 }

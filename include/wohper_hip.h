@@ -256,6 +256,13 @@ void wh_synth_fp8_host(uint64_t seed, uint64_t stream, uint8_t* weight, size_t n
 void wh_synth_fp4_host(uint64_t seed, uint64_t stream, uint8_t* packed, size_t packed_len,
                        uint8_t* scales, size_t scales_len, uint32_t scale_lo, uint32_t scale_hi);
 
+/* wh_store_fp8 of a weight and scales in device memory, whole when the call is
+ * made: no counterpart in the reference.  128-column scale groups only (cols /
+ * scale_cols == 128, else WH_INVALID_SHAPE), f32 scales 4-byte aligned.  Waits
+ * for its copy, so the caller may reuse the memory; not inside a graph capture. */
+int wh_store_fp8_device(wh_ctx* ctx, const uint8_t* weight_dev, size_t rows, size_t cols, const void* scales_dev,
+                        size_t scale_rows, size_t scale_cols, int scale_format, wh_tensor* out);
+
 int wh_store_release(wh_ctx* ctx, wh_tensor t);
 int wh_store_usage(wh_ctx* ctx, size_t* device_bytes, size_t* tensors, size_t* experts);
 
@@ -950,6 +957,90 @@ typedef struct {
     const float* sink;  /* device [heads] or NULL */
 } wh_kv4_attention;
 int wh_kv4_attention_async(wh_ctx* ctx, const wh_kv4_cache* cache, const wh_kv4_attention* attention);
+
+/* ------------------------------------------------------------------
+ * Products of 8-bit rows, no counterpart in the reference (its products take
+ * f32 inputs, as wh_fp8_gemv_multi does): for prompts and large batches, where
+ * both sides in 8 bits take a sixth of the matrix instructions.
+ *
+ * A row of cols values (a multiple of 128) is E4M3 codes and a UE8M0 scale byte
+ * for every 128 columns: value = code * 2^(byte - 127); code 0x7F / 0xFF and
+ * byte 255 stand for NaN.  Codes lie in the weight store's order: byte 16 l + i
+ * of a block is its column 16 (i % 8) + 8 (i / 8) + l (l < 8, i < 16).
+ *
+ * An MoE layer's step: wh_fp8_quant_rows_async of the positions,
+ * wh_expert_plan_async of their routes, wh_fp8_rows_mm_groups_async with gate
+ * and up stacked, wh_fp8_swiglu_rows_async, wh_fp8_rows_mm_groups_async with
+ * down, wh_expert_combine_async.  Lists are device arrays, so one captured
+ * graph serves every step of the same sizes.
+ * ------------------------------------------------------------------ */
+
+/* Device pointers, the caller's: row r's codes at codes + r * stride (16-byte
+ * aligned, stride a multiple of 16), its scale bytes at scales + r *
+ * scale_stride (4-byte aligned, a multiple of 4; whole words are read, so
+ * scale_stride is at least cols / 128 rounded up to 4). */
+typedef struct {
+    uint8_t* codes;
+    size_t stride;
+    uint8_t* scales;
+    size_t scale_stride;
+} wh_fp8_rows;
+
+/* Rounds n rows of cols values (f32, or bf16 with is_bf16) to 8 bits.  A block
+ * of 128 gets the least power of two, at least 2^-126, under which its largest
+ * finite magnitude is at most 448, and each value the nearest code, ties to
+ * even; infinities and NaN become NaN.  The swiglu form rounds silu(min(gate,
+ * limit)) * clamp(up, -limit, limit), in f32 (E/deepseek_v4.rs:590-594 with
+ * limit 10; INFINITY: no clamp); a product beyond f32 becomes NaN. */
+int wh_fp8_quant_rows_async(wh_ctx* ctx, const void* x_dev, size_t x_stride, int is_bf16, size_t n, size_t cols,
+                            const wh_fp8_rows* out);
+int wh_fp8_swiglu_rows_async(wh_ctx* ctx, const void* gate_dev, const void* up_dev, size_t stride, int is_bf16, size_t n,
+                             size_t cols, float limit, const wh_fp8_rows* out);
+/* The values that n rows stand for (bf16: rounded only below 2^-126). */
+int wh_fp8_read_rows_async(wh_ctx* ctx, const wh_fp8_rows* rows, size_t n, size_t cols, void* out_dev, size_t out_stride,
+                           int is_bf16);
+
+/* y row i = rows [row_start, row_end) of w times x row i, f32 or bf16
+ * (is_bf16), for n rows of w's columns.  w: an FP8 tensor of 128-column scale
+ * groups.  Products of codes are exact; a block's sum times both scales, and the
+ * sum over blocks, are f32 in any order, in both numerics modes: within
+ * 1e-6 * sqrt(cols) * ||w_row||_2 * ||x_i||_2, then rounded once to bf16.  A NaN
+ * in an x row makes its y row NaN and no other.  Weight codes 0x7F / 0xFF are
+ * +-480 and UE8M0 bytes 0 and 255 are 0.0 and infinity, as in every product
+ * here; tensors with such codes, and ranges or scale rows that are no multiples
+ * of 16 rows, take a kernel without matrix instructions, many times as long.
+ * y must not overlap x. */
+int wh_fp8_rows_mm_async(wh_ctx* ctx, wh_tensor w, size_t row_start, size_t row_end, const wh_fp8_rows* x, size_t n,
+                         void* y_dev, size_t y_stride, int is_bf16);
+
+/* The same grouped by expert: y row j, starts_dev[g] <= j < starts_dev[g + 1],
+ * is x row rows_dev[j] (NULL: j) times w's rows row_start + g * group_rows +
+ * [0, group_rows).  starts_dev [n_groups + 1] ascends (not checked; groups that
+ * overlap leave either one's result) and is cut off at n, the rows of y;
+ * y rows in no group are left as they are.  rows_dev [n] entries of n_x or more
+ * are no row: their y rows are 0.  At most 1024 groups. */
+int wh_fp8_rows_mm_groups_async(wh_ctx* ctx, wh_tensor w, size_t row_start, size_t group_rows, size_t n_groups,
+                                const wh_fp8_rows* x, size_t n_x, const uint32_t* rows_dev, const uint32_t* starts_dev,
+                                size_t n, void* y_dev, size_t y_stride, int is_bf16);
+
+/* Expert lists of npos positions' routes ids_dev [npos][topk]: an id of
+ * n_experts or more is no expert (padding, an expert elsewhere).  Expert e's
+ * list is starts_dev[e] .. starts_dev[e + 1] (starts_dev [n_experts + 1]), its
+ * routes in order; rows_dev [npos * topk] gets each listed route's position
+ * and 0xFFFFFFFF behind the last list, slots_dev [npos][topk] each route's
+ * place in the lists or 0xFFFFFFFF.  At most 1024 experts; outputs overlap
+ * neither each other nor ids_dev. */
+int wh_expert_plan_async(wh_ctx* ctx, const uint32_t* ids_dev, size_t npos, size_t topk, size_t n_experts,
+                         uint32_t* starts_dev, uint32_t* rows_dev, uint32_t* slots_dev);
+
+/* out row p = sum over k of weights_dev[p][k] * y row slots_dev[p][k], in f32
+ * in the order of k, plus add row p (add_dev NULL: none; the shared expert's, it
+ * may be out).  Slots of n_rows or more are passed over, whatever their weight; a
+ * position of no slots gets 0 or its add row.  y is f32 or bf16; hidden and all
+ * strides are multiples of 4 values, rows aligned to 4 values. */
+int wh_expert_combine_async(wh_ctx* ctx, const void* y_dev, size_t y_stride, int is_bf16, size_t n_rows,
+                            const uint32_t* slots_dev, const float* weights_dev, size_t npos, size_t topk, size_t hidden,
+                            const float* add_dev, size_t add_stride, float* out_dev, size_t out_stride);
 
 #ifdef __cplusplus
 }

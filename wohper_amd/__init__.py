@@ -22,7 +22,10 @@ include/wohper_hip.h (libwohper_hip.so, built from wohper_amd/csrc):
 The paged 4-bit attention cache has no counterpart there: Context.kv_plan_async
 (lengths to pages and slots), kv4_write_async and kv4_read_async (rows in and
 out) and kv4_attention_async (decode, verify and prefill over the cached rows)
-with the descriptors WhKvPlan, WhKv4Cache and WhKv4Attention.
+with the descriptors WhKvPlan, WhKv4Cache and WhKv4Attention.  Nor have the
+products of 8-bit rows: Context.fp8_quant_rows_async, fp8_swiglu_rows_async and
+fp8_read_rows_async (WhFp8Rows), fp8_rows_mm_async, fp8_rows_mm_groups_async,
+expert_plan_async and expert_combine_async.
 
 The slice-based functions upload the weights for the call, as the reference
 reads them from its I/O buffers; the resident path (Context.store_* plus the
@@ -100,6 +103,8 @@ EXPORTED = (
     "wh_graph_begin", "wh_graph_end", "wh_graph_launch", "wh_graph_release",
     "wh_routed_and_shared_experts_dev_async", "wh_deepseek_mhc_layer_async", "wh_deepseek_mhc_layer_batch_async",
     "wh_kv_plan_async", "wh_kv4_write_async", "wh_kv4_read_async", "wh_kv4_attention_async",
+    "wh_store_fp8_device", "wh_fp8_quant_rows_async", "wh_fp8_swiglu_rows_async", "wh_fp8_read_rows_async",
+    "wh_fp8_rows_mm_async", "wh_fp8_rows_mm_groups_async", "wh_expert_plan_async", "wh_expert_combine_async",
 )
 
 ROUTER_RAW_LOGITS = 0
@@ -193,6 +198,12 @@ class WhKv4Attention(ctypes.Structure):
                 ("tables_dev", ctypes.c_void_p), ("table_stride", ctypes.c_size_t), ("max_len", ctypes.c_size_t),
                 ("heads", ctypes.c_size_t), ("scale", ctypes.c_float), ("window", ctypes.c_size_t),
                 ("first", ctypes.c_size_t), ("sink", ctypes.c_void_p)]
+
+
+class WhFp8Rows(ctypes.Structure):
+    """8-bit rows by their device buffers (wh_fp8_rows)."""
+    _fields_ = [("codes", ctypes.c_void_p), ("stride", ctypes.c_size_t), ("scales", ctypes.c_void_p),
+                ("scale_stride", ctypes.c_size_t)]
 
 
 class WhExpertPackEntry(ctypes.Structure):
@@ -315,6 +326,15 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         "wh_kv4_write_async": (c.c_int, [vp, c.POINTER(WhKv4Cache), vp, sz, vp, sz, c.c_int, vp, sz]),
         "wh_kv4_read_async": (c.c_int, [vp, c.POINTER(WhKv4Cache), vp, sz, vp, sz, vp, sz, c.c_int]),
         "wh_kv4_attention_async": (c.c_int, [vp, c.POINTER(WhKv4Cache), c.POINTER(WhKv4Attention)]),
+        "wh_store_fp8_device": (c.c_int, [vp, vp, sz, sz, vp, sz, sz, c.c_int, c.POINTER(c.c_uint64)]),
+        "wh_fp8_quant_rows_async": (c.c_int, [vp, vp, sz, c.c_int, sz, sz, c.POINTER(WhFp8Rows)]),
+        "wh_fp8_swiglu_rows_async": (c.c_int, [vp, vp, vp, sz, c.c_int, sz, sz, c.c_float, c.POINTER(WhFp8Rows)]),
+        "wh_fp8_read_rows_async": (c.c_int, [vp, c.POINTER(WhFp8Rows), sz, sz, vp, sz, c.c_int]),
+        "wh_fp8_rows_mm_async": (c.c_int, [vp, c.c_uint64, sz, sz, c.POINTER(WhFp8Rows), sz, vp, sz, c.c_int]),
+        "wh_fp8_rows_mm_groups_async": (c.c_int, [vp, c.c_uint64, sz, sz, sz, c.POINTER(WhFp8Rows), sz, vp, vp, sz, vp,
+                                                  sz, c.c_int]),
+        "wh_expert_plan_async": (c.c_int, [vp, vp, sz, sz, sz, vp, vp, vp]),
+        "wh_expert_combine_async": (c.c_int, [vp, vp, sz, c.c_int, sz, vp, vp, sz, sz, sz, vp, sz, vp, sz]),
         "wh_route_experts_async": (c.c_int, [vp, c.c_uint32, vp, sz, sz, vp, sz, c.POINTER(WhRouteOptions), vp, vp,
                                              vp]),
     }
@@ -914,6 +934,59 @@ class Context:
         """Attention of new tokens over their requests' cached rows."""
         _check(self.lib.wh_kv4_attention_async(self._h, ctypes.byref(cache), ctypes.byref(attention)),
                "kv4_attention_async")
+
+    # ------------------------------------------------------------- 8-bit rows
+    def store_fp8_device(self, weight_ptr: int, rows: int, cols: int, scales_ptr: int, scale_rows: int, scale_cols: int,
+                         scale_format: int = SCALE_UE8M0) -> int:
+        """store_fp8 of a weight and scales in device memory."""
+        out = ctypes.c_uint64()
+        _check(self.lib.wh_store_fp8_device(self._h, weight_ptr, rows, cols, scales_ptr, scale_rows, scale_cols,
+                                            scale_format, ctypes.byref(out)), "store_fp8_device")
+        return out.value
+
+    def fp8_quant_rows_async(self, x_ptr: int, x_stride: int, is_bf16: bool, n: int, cols: int, rows: WhFp8Rows):
+        """Rounds n rows of cols values to 8 bits."""
+        _check(self.lib.wh_fp8_quant_rows_async(self._h, x_ptr, x_stride, is_bf16, n, cols, ctypes.byref(rows)),
+               "fp8_quant_rows_async")
+
+    def fp8_swiglu_rows_async(self, gate_ptr: int, up_ptr: int, stride: int, is_bf16: bool, n: int, cols: int,
+                              limit: float, rows: WhFp8Rows):
+        """Rounds SwiGLU of n gate and up rows to 8 bits."""
+        _check(self.lib.wh_fp8_swiglu_rows_async(self._h, gate_ptr, up_ptr, stride, is_bf16, n, cols, limit,
+                                                 ctypes.byref(rows)), "fp8_swiglu_rows_async")
+
+    def fp8_read_rows_async(self, rows: WhFp8Rows, n: int, cols: int, out_ptr: int, out_stride: int, is_bf16: bool):
+        """The values that n 8-bit rows stand for."""
+        _check(self.lib.wh_fp8_read_rows_async(self._h, ctypes.byref(rows), n, cols, out_ptr, out_stride, is_bf16),
+               "fp8_read_rows_async")
+
+    def fp8_rows_mm_async(self, w: int, row_start: int, row_end: int, x: WhFp8Rows, n: int, y_ptr: int, y_stride: int,
+                          is_bf16: bool):
+        """n 8-bit rows times rows [row_start, row_end) of a resident FP8 weight."""
+        _check(self.lib.wh_fp8_rows_mm_async(self._h, w, row_start, row_end, ctypes.byref(x), n, y_ptr, y_stride,
+                                             is_bf16), "fp8_rows_mm_async")
+
+    def fp8_rows_mm_groups_async(self, w: int, row_start: int, group_rows: int, n_groups: int, x: WhFp8Rows, n_x: int,
+                                 rows_ptr: Optional[int], starts_ptr: int, n: int, y_ptr: int, y_stride: int,
+                                 is_bf16: bool):
+        """8-bit rows grouped by expert times each expert's rows of the weight."""
+        _check(self.lib.wh_fp8_rows_mm_groups_async(self._h, w, row_start, group_rows, n_groups, ctypes.byref(x), n_x,
+                                                    rows_ptr, starts_ptr, n, y_ptr, y_stride, is_bf16),
+               "fp8_rows_mm_groups_async")
+
+    def expert_plan_async(self, ids_ptr: int, npos: int, topk: int, n_experts: int, starts_ptr: int, rows_ptr: int,
+                          slots_ptr: int):
+        """Expert lists of a batch of routes."""
+        _check(self.lib.wh_expert_plan_async(self._h, ids_ptr, npos, topk, n_experts, starts_ptr, rows_ptr, slots_ptr),
+               "expert_plan_async")
+
+    def expert_combine_async(self, y_ptr: int, y_stride: int, is_bf16: bool, n_rows: int, slots_ptr: int,
+                             weights_ptr: int, npos: int, topk: int, hidden: int, out_ptr: int, out_stride: int,
+                             add_ptr: Optional[int] = None, add_stride: int = 0):
+        """Each position's weighted sum of its experts' rows."""
+        _check(self.lib.wh_expert_combine_async(self._h, y_ptr, y_stride, is_bf16, n_rows, slots_ptr, weights_ptr, npos,
+                                                topk, hidden, add_ptr, add_stride, out_ptr, out_stride),
+               "expert_combine_async")
 
     def debug_eval(self, fn: int, x) -> np.ndarray:
         x = _f32(x)

@@ -30,7 +30,7 @@ HIP_FLAGS = [
 
 
 # the HIP translation units of the library
-UNITS = ("wohper_hip", "kv4")
+UNITS = ("wohper_hip", "kv4", "fp8_rows")
 
 
 def _hipcc() -> str:

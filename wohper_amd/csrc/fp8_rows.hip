@@ -1,0 +1,516 @@
+// 8-bit rows (gfx950): activations to E4M3 codes and back, their products with
+// resident FP8 weights, plain and grouped by expert, expert lists from routes
+// and the sum over a position's experts.
+//
+// A row holds one code a column and one UE8M0 scale byte for every 128 columns:
+// value = code * 2^(byte - 127).  Inside a block of 128 the codes lie in the
+// weight store's lane order (byte 16 l + i is column 16 (i % 8) + 8 (i / 8) + l,
+// kernels.h), so a product multiplies both sides' bytes as they lie: which
+// column a byte is does not matter to a sum over the whole block.
+#include "fp8_rows.h"
+
+#include <algorithm>
+
+#include "wh_device.h"
+
+namespace {
+
+typedef uint32_t wh_u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t wh_u4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kNone = WH_ROWS_NONE;
+
+// Largest over a row of 16 lanes, in all of them.
+__device__ __forceinline__ uint32_t rows_max16(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, false));  // rotated by 8, 4, 2, 1
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x124, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x122, 0xf, 0xf, false));
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x121, 0xf, 0xf, false));
+}
+
+// A row's scale byte, as the matrix instructions read it: 255 is NaN, 0 is 2^-127.
+__device__ __forceinline__ float rows_scale(uint32_t byte) {
+    return __uint_as_float(byte == 255 ? 0x7fc00000u : byte ? byte << 23 : 0x00400000u);
+}
+
+// ------------------------------------------------------------------- rows
+
+// Rows to 8 bits.  Sixteen lanes take a block of 128 columns, lane q the codes
+// of bytes 8 q .. 8 q + 7: columns 16 i + q' with q' = 8 (q % 2) + q / 2, so that
+// each of its eight loads is 16 consecutive columns of the block over the lanes
+// and its store is consecutive bytes.  The scale is the least power of two, 2^-126
+// at least, under which the block's largest finite magnitude is at most 448: from
+// its bits, since 448 is 1.75 * 2^8.  Values times its inverse are exact (or round
+// to code 0), so each code is rounded once, to nearest even.  Infinities and NaN
+// become NaN and do not count for the scale.
+template <bool kBf16, bool kSwiglu>
+__global__ void __launch_bounds__(256) k_rows_quant(wh_rows_quant_args a) {
+    const uint64_t unit = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    const uint32_t q = threadIdx.x & 15;
+    const uint64_t row = unit / a.blocks;
+    const uint32_t block = (uint32_t)(unit - row * a.blocks);
+    if (row >= a.n) return;
+    const uint64_t at = row * a.x_stride + block * 128u + 8 * (q & 1) + (q >> 1);
+    auto load = [&](const void* p, uint32_t i) {
+        if constexpr (kBf16) return __uint_as_float((uint32_t)((const uint16_t*)p)[at + 16 * i] << 16);
+        else return ((const float*)p)[at + 16 * i];
+    };
+    float v[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v[i] = load(a.x, i);
+    if constexpr (kSwiglu) {
+        float u[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) u[i] = load(a.up, i);
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            // NaN stays NaN through both clamps
+            const float g = v[i] > a.limit ? a.limit : v[i];
+            const float p = u[i] > a.limit ? a.limit : u[i] < -a.limit ? -a.limit : u[i];
+            // from exp(-|g|), which leaves no result behind that f32 has
+            const float z = expf(-fabsf(g));
+            v[i] = g * ((g < 0.0f ? z : 1.0f) / (1.0f + z)) * p;
+        }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+        top = max(top, b < 0x7f800000u ? b : 0);
+    }
+    top = rows_max16(top);
+    int e = (int)(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    e = max(e, -126);
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    uint32_t codes[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const bool finite = (__float_as_uint(v[i]) & 0x7fffffffu) < 0x7f800000u;
+        const uint32_t c = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(finite ? v[i] * inv : 0.0f, 0.0f, 0, false) & 0xffu;
+        codes[i] = finite ? c : 0x7fu;
+    }
+    wh_u2 out;
+    out.x = codes[0] | codes[1] << 8 | codes[2] << 16 | codes[3] << 24;
+    out.y = codes[4] | codes[5] << 8 | codes[6] << 16 | codes[7] << 24;
+    *(wh_u2*)(a.out.codes + row * a.out.stride + block * 128u + 8 * q) = out;
+    if (q == 0) a.out.scales[row * a.out.scale_stride + block] = top ? (uint8_t)(e + 127) : 0;
+}
+
+// 8-bit rows as the values they stand for: the same lanes the other way.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) k_rows_read(wh_rows_read_args a) {
+    const uint64_t unit = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    const uint32_t q = threadIdx.x & 15;
+    const uint64_t row = unit / a.blocks;
+    const uint32_t block = (uint32_t)(unit - row * a.blocks);
+    if (row >= a.n) return;
+    const wh_u2 codes = *(const wh_u2*)(a.in.codes + row * a.in.stride + block * 128u + 8 * q);
+    const float scale = rows_scale(a.in.scales[row * a.in.scale_stride + block]);
+    const uint64_t at = row * a.out_stride + block * 128u + 8 * (q & 1) + (q >> 1);
+#pragma unroll
+    for (uint32_t h = 0; h < 4; ++h) {
+        const uint32_t w = h < 2 ? codes.x : codes.y;
+        const wh_f2 v = h & 1 ? wh_fp8x2<false, true>(w) : wh_fp8x2<false, false>(w);
+#pragma unroll
+        for (uint32_t j = 0; j < 2; ++j) {
+            const float x = (j ? v.y : v.x) * scale;
+            if constexpr (kBf16) ((__bf16*)a.out)[at + 16 * (2 * h + j)] = (__bf16)x;
+            else ((float*)a.out)[at + 16 * (2 * h + j)] = x;
+        }
+    }
+}
+
+// --------------------------------------------------------------- products
+
+// The t-th tile of at most kRows listed rows [r0, r1) of one group g.  With
+// groups, tiles are numbered group by group: every wave adds up the groups' tiles
+// 64 at a time.  False behind the last tile.  Starts that do not ascend, or pass
+// n, are cut off.
+template <uint32_t kRows>
+__device__ __forceinline__ bool rows_tile(const wh_rows_mm_args& a, uint32_t t, uint32_t& g, uint32_t& r0, uint32_t& r1) {
+    if (!a.starts) {
+        g = 0;
+        r0 = t * kRows;
+        r1 = min(a.n, r0 + kRows);
+        return r0 < a.n;
+    }
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < a.n_groups; base += 64) {
+        const uint32_t at = base + lane;
+        uint32_t s = 0, e = 0;
+        if (at < a.n_groups) {
+            s = min(a.starts[at], a.n);
+            e = max(s, min(a.starts[at + 1], a.n));
+        }
+        const uint32_t tiles = (e - s + kRows - 1) / kRows;
+        uint32_t upto = tiles;
+#pragma unroll
+        for (uint32_t off = 1; off < 64; off <<= 1) {
+            const uint32_t y = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += y;
+        }
+        const uint64_t past = __ballot(before + upto > t);
+        if (past) {
+            const uint32_t first = (uint32_t)__builtin_ctzll(past);
+            const uint32_t own = __shfl(before + upto - tiles, first, 64);
+            g = base + first;
+            r0 = __shfl(s, first, 64) + (t - own) * kRows;
+            r1 = min(__shfl(e, first, 64), r0 + kRows);
+            return true;
+        }
+        before += __shfl(upto, 63, 64);
+    }
+    return false;
+}
+
+// Scale of weight row `row` in block b as mantissa * 2^exponent, so that its
+// product with a row's power of two leaves f32's range only where the result does.
+__device__ __forceinline__ float rows_w_scale(const wh_rows_mm_args& a, uint64_t row, uint32_t b, int* e) {
+    const uint64_t at = row / a.row_block * (a.cols / 128u) + b;
+    *e = 0;
+    if (a.scale_f32) {
+        const float s = ((const float*)a.w_scales)[at];
+        if (!(fabsf(s) <= 3.4028235e38f)) return s;
+        return frexpf(s, e);
+    }
+    const uint32_t byte = ((const uint8_t*)a.w_scales)[at];
+    if (byte == 0 || byte == 255) return wh_ue8m0(byte);
+    *e = (int)byte - 127;
+    return 1.0f;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void rows_put(const wh_rows_mm_args& a, uint64_t row, uint32_t col, float v) {
+    if constexpr (kBf16) ((__bf16*)a.y)[row * a.y_stride + col] = (__bf16)v;
+    else ((float*)a.y)[row * a.y_stride + col] = v;
+}
+
+// Any product: 16 x 16 outputs a workgroup, one a thread, the block's values of
+// both sides decoded into LDS.  For what the matrix instructions read otherwise or
+// do not take: weight codes 0x7F / 0xFF (+-480 here, NaN there) and scales shared
+// by a number of rows that is no multiple of 16.
+constexpr uint32_t kAnyRows = 16;
+template <bool kBf16>
+__global__ void __launch_bounds__(256) k_rows_mm_any(wh_rows_mm_args a) {
+    __shared__ float xs[kAnyRows][132], ws[16][132];
+    const uint32_t n_cols = (a.out_rows + 15) / 16, t = threadIdx.x, lane16 = t & 15, row16 = t >> 4;
+    uint32_t g = 0, r0 = 0, r1 = 0;
+    if (!rows_tile<kAnyRows>(a, blockIdx.x / n_cols, g, r0, r1)) return;
+    const uint32_t c0 = (blockIdx.x % n_cols) * 16;
+    const uint64_t w0 = a.row_start + (uint64_t)g * a.out_rows;
+    // staging: thread (row16, lane16) brings 8 codes of row row16 of both sides
+    uint32_t src = 0;
+    bool have = r0 + row16 < r1;
+    if (have) {
+        src = a.rows ? a.rows[r0 + row16] : r0 + row16;
+        have = src < a.n_x;
+    }
+    const bool have_w = c0 + row16 < a.out_rows;
+    const uint64_t w_row = w0 + c0 + row16, my_w = w0 + min(c0 + lane16, a.out_rows - 1);
+    float acc = 0.0f;
+    for (uint32_t b = 0; b < a.cols / 128u; ++b) {
+        wh_u2 xc = {0, 0}, wc = {0, 0};
+        if (have) xc = *(const wh_u2*)(a.x.codes + (uint64_t)src * a.x.stride + b * 128u + 8 * lane16);
+        if (have_w) wc = *(const wh_u2*)(a.w + w_row * a.cols + b * 128u + 8 * lane16);
+        __syncthreads();
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t xw = h ? xc.y : xc.x, ww = h ? wc.y : wc.x;
+            const wh_f2 x0 = wh_fp8x2<false, false>(xw), x1 = wh_fp8x2<false, true>(xw);
+            const wh_f2 w0v = wh_fp8x2<true, false>(ww), w1v = wh_fp8x2<true, true>(ww);
+            float* const xd = &xs[row16][8 * lane16 + 4 * h];
+            float* const wd = &ws[row16][8 * lane16 + 4 * h];
+            xd[0] = x0.x, xd[1] = x0.y, xd[2] = x1.x, xd[3] = x1.y;
+            wd[0] = w0v.x, wd[1] = w0v.y, wd[2] = w1v.x, wd[3] = w1v.y;
+        }
+        __syncthreads();
+        float sum = 0.0f;
+        for (uint32_t k = 0; k < 128; ++k) sum = fmaf(xs[row16][k], ws[lane16][k], sum);
+        int e = 0;
+        const float m = rows_w_scale(a, my_w, b, &e);
+        if (have) {
+            const int byte = a.x.scales[(uint64_t)src * a.x.scale_stride + b];
+            acc += byte == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(sum * m, byte - 127 + e);
+        }
+    }
+    if (r0 + row16 < r1 && c0 + lane16 < a.out_rows) rows_put<kBf16>(a, r0 + row16, c0 + lane16, acc);
+}
+
+// Most tiles of kRows listed rows that a call can have.
+uint64_t rows_tiles(const wh_rows_mm_args& a, uint32_t rows) {
+    const uint64_t full = ((uint64_t)a.n + rows - 1) / rows;
+    // each group may end in a tile that is not full, and has at least a row then
+    return a.starts ? full + std::min<uint64_t>(a.n_groups, a.n) : full;
+}
+
+// ------------------------------------------------------------------ store
+
+// Row-major codes into the store's order, and whether one is 0x7F or 0xFF.
+__global__ void __launch_bounds__(256) k_rows_store(const uint8_t* in, uint8_t* out, uint64_t blocks, uint32_t* flags) {
+    const uint64_t unit = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    const uint32_t q = threadIdx.x & 15;
+    if (unit >= blocks) return;
+    const uint8_t* const p = in + unit * 128 + 8 * (q & 1) + (q >> 1);
+    uint32_t c[8], special = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        c[i] = p[16 * i];
+        special |= (c[i] & 0x7fu) == 0x7fu;
+    }
+    wh_u2 o;
+    o.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+    o.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
+    *(wh_u2*)(out + unit * 128 + 8 * q) = o;
+    if (special) atomicOr(flags, 1u);
+}
+
+__global__ void __launch_bounds__(256) k_rows_scales(const uint8_t* scales, uint64_t n, uint32_t* flags) {
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n && (scales[i] == 0 || scales[i] == 255)) atomicOr(flags, 2u);
+}
+
+// ------------------------------------------------------------ expert lists
+
+constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr uint32_t kPlanChunk = 4096;                      // routes of a workgroup
+constexpr uint32_t kPlanPerWave = kPlanChunk / kPlanWaves;  // consecutive ones of a wave
+
+// What a wave's lanes have stored to LDS is there for its other lanes.
+__device__ __forceinline__ void plan_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Lanes with this lane's id (< 2^bits).
+__device__ __forceinline__ uint64_t plan_same(uint32_t id, uint32_t bits) {
+    uint64_t same = ~0ull;
+    for (uint32_t b = 0; b < bits; ++b) {
+        const bool set = id >> b & 1;
+        const uint64_t with = __ballot(set);
+        same &= set ? with : ~with;
+    }
+    return same;
+}
+
+// How many routes of each expert a chunk has.
+__global__ void __launch_bounds__(kPlanThreads) k_expert_count(wh_expert_plan_args a) {
+    __shared__ uint32_t count[WH_ROWS_MAX_GROUPS];
+    for (uint32_t e = threadIdx.x; e < a.n_groups; e += kPlanThreads) count[e] = 0;
+    __syncthreads();
+    const uint32_t from = blockIdx.x * kPlanChunk, to = min(a.n, from + kPlanChunk);
+    for (uint32_t i = from + threadIdx.x; i < to; i += kPlanThreads) {
+        const uint32_t id = a.ids[i];
+        if (id < a.n_groups) atomicAdd(&count[id], 1u);
+    }
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < a.n_groups; e += kPlanThreads) a.counts[(uint64_t)blockIdx.x * a.n_groups + e] = count[e];
+}
+
+// Expert lists: a counting sort that keeps the order of routes.  A workgroup
+// takes 4096 routes, a wave 256 consecutive ones 64 at a time; lanes of the same
+// expert find each other by ballots over the id's bits, so a route's place is
+// the expert's start, its routes of chunks and waves before, of this wave so far,
+// and of lanes before.  With one chunk this is the only launch.
+__global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_args a, uint32_t chunks, uint32_t bits) {
+    extern __shared__ uint32_t lds[];
+    uint32_t* const at = lds;  // [kPlanWaves][n_groups]: counts, then next places of a wave
+    __shared__ uint32_t wave_sum[kPlanWaves];
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, E = a.n_groups;
+    for (uint32_t i = t; i < kPlanWaves * E; i += kPlanThreads) at[i] = 0;
+    __syncthreads();
+    const uint32_t from = blockIdx.x * kPlanChunk + wave * kPlanPerWave;
+    uint32_t id[kPlanPerWave / 64];
+    uint64_t same[kPlanPerWave / 64];
+#pragma unroll
+    for (uint32_t k = 0; k < kPlanPerWave / 64; ++k) {
+        const uint32_t i = from + 64 * k + lane;
+        id[k] = i < a.n ? a.ids[i] : kNone;
+        if (id[k] >= E) id[k] = E;  // no expert: a number of its own, E < 2^bits
+        same[k] = plan_same(id[k], bits);
+        const bool leads = __builtin_ctzll(same[k]) == lane;
+        if (leads && id[k] < E) at[wave * E + id[k]] += (uint32_t)__popcll(same[k]);
+        plan_wave_sync();
+    }
+    __syncthreads();
+    // this chunk's and all chunks' routes of expert t, those before this chunk
+    uint32_t all = 0, before = 0;
+    if (t < E) {
+        if (chunks == 1) {
+            for (uint32_t w = 0; w < kPlanWaves; ++w) all += at[w * E + t];
+        } else {
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t v = a.counts[(uint64_t)c * E + t];
+                before += c < blockIdx.x ? v : 0;
+                all += v;
+            }
+        }
+    }
+    uint32_t upto = all;
+    for (uint32_t off = 1; off < 64; off <<= 1) {
+        const uint32_t y = __shfl_up(upto, off, 64);
+        if (lane >= off) upto += y;
+    }
+    if (lane == 63) wave_sum[wave] = upto;
+    __syncthreads();
+    uint32_t total = 0, waves_before = 0;
+    for (uint32_t w = 0; w < kPlanWaves; ++w) {
+        if (w < wave) waves_before += wave_sum[w];
+        total += wave_sum[w];
+    }
+    if (t < E) {
+        const uint32_t start = waves_before + upto - all;
+        uint32_t next = start + before;
+        for (uint32_t w = 0; w < kPlanWaves; ++w) {
+            const uint32_t v = at[w * E + t];
+            at[w * E + t] = next;
+            next += v;
+        }
+        if (blockIdx.x == 0) {
+            a.starts[t] = start;
+            if (t == E - 1) a.starts[E] = start + all;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < kPlanPerWave / 64; ++k) {
+        const uint32_t i = from + 64 * k + lane;
+        const bool some = id[k] < E;
+        uint32_t place = kNone;
+        if (some) place = at[wave * E + id[k]] + (uint32_t)__popcll(same[k] & ((1ull << lane) - 1));
+        plan_wave_sync();
+        if (some && __builtin_ctzll(same[k]) == lane) at[wave * E + id[k]] += (uint32_t)__popcll(same[k]);
+        plan_wave_sync();
+        if (i < a.n) {
+            a.slots[i] = place;
+            if (some) a.rows[place] = i / a.topk;
+            if (i >= total) a.rows[i] = kNone;  // behind the lists
+        }
+    }
+}
+
+// A position's weighted sum over its experts' rows, four columns a thread, its
+// routes in order; rows of no slot are passed over.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) k_expert_combine(wh_expert_combine_args a, uint32_t units) {
+    const uint32_t p = blockIdx.x / units, col = ((blockIdx.x % units) * 256 + threadIdx.x) * 4;
+    if (col >= a.hidden) return;
+    wh_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t k = 0; k < a.topk; ++k) {
+        const uint32_t slot = a.slots[(uint64_t)p * a.topk + k];
+        if (slot >= a.n_rows) continue;
+        const float w = a.weights[(uint64_t)p * a.topk + k];
+        wh_f4 v;
+        if constexpr (kBf16) {
+            const wh_u2 b = *(const wh_u2*)((const uint16_t*)a.y + slot * a.y_stride + col);
+            v = wh_f4{__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16),
+                      __uint_as_float(b.y & 0xffff0000u)};
+        } else {
+            v = *(const wh_f4*)((const float*)a.y + slot * a.y_stride + col);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = fmaf(v[j], w, acc[j]);
+    }
+    if (a.add) {
+        const wh_f4 s = *(const wh_f4*)(a.add + p * a.add_stride + col);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += s[j];
+    }
+    *(wh_f4*)(a.out + p * a.out_stride + col) = acc;
+}
+
+// A grid has less than 2^32 threads.
+constexpr uint64_t kMaxGrid256 = 0xffffffull;
+
+}  // namespace
+
+constexpr size_t plan_lds(uint32_t n_groups) { return kPlanWaves * (size_t)n_groups * sizeof(uint32_t); }
+
+hipError_t wh_rows_setup() {
+    return hipFuncSetAttribute((const void*)k_expert_place, hipFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)plan_lds(WH_ROWS_MAX_GROUPS));
+}
+
+hipError_t wh_rows_quant_launch(const wh_rows_quant_args& a, bool bf16, hipStream_t stream) {
+    const uint64_t grid = ((uint64_t)a.n * a.blocks + 15) / 16;
+    if (grid > kMaxGrid256) return hipErrorInvalidValue;
+    if (a.up) {
+        if (bf16) k_rows_quant<true, true><<<(unsigned)grid, 256, 0, stream>>>(a);
+        else k_rows_quant<false, true><<<(unsigned)grid, 256, 0, stream>>>(a);
+    } else {
+        if (bf16) k_rows_quant<true, false><<<(unsigned)grid, 256, 0, stream>>>(a);
+        else k_rows_quant<false, false><<<(unsigned)grid, 256, 0, stream>>>(a);
+    }
+    return hipGetLastError();
+}
+
+hipError_t wh_rows_read_launch(const wh_rows_read_args& a, bool bf16, hipStream_t stream) {
+    const uint64_t grid = ((uint64_t)a.n * a.blocks + 15) / 16;
+    if (grid > kMaxGrid256) return hipErrorInvalidValue;
+    if (bf16) k_rows_read<true><<<(unsigned)grid, 256, 0, stream>>>(a);
+    else k_rows_read<false><<<(unsigned)grid, 256, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
+bool wh_rows_mm_fits(const wh_rows_mm_args& a) {
+    return rows_tiles(a, kAnyRows) * ((a.out_rows + 15) / 16) <= kMaxGrid256;
+}
+
+hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, bool bf16, hipStream_t stream) {
+    const unsigned grid = (unsigned)(rows_tiles(a, kAnyRows) * ((a.out_rows + 15) / 16));
+    if (bf16) k_rows_mm_any<true><<<grid, 256, 0, stream>>>(a);
+    else k_rows_mm_any<false><<<grid, 256, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
+hipError_t wh_rows_store_launch(const uint8_t* weight, uint8_t* out, uint64_t rows, uint32_t cols, uint32_t* flags,
+                                hipStream_t stream) {
+    // pieces of rows whose grids are within a launch's limits
+    const uint64_t per = std::max<uint64_t>(1, (kMaxGrid256 * 16) / (cols / 128u));
+    for (uint64_t r = 0; r < rows; r += per) {
+        const uint64_t blocks = std::min(per, rows - r) * (cols / 128u);
+        k_rows_store<<<(unsigned)((blocks + 15) / 16), 256, 0, stream>>>(weight + r * cols, out + r * cols, blocks, flags);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+hipError_t wh_rows_scales_launch(const uint8_t* scales, uint64_t n, uint32_t* flags, hipStream_t stream) {
+    const uint64_t per = kMaxGrid256 * 256;
+    for (uint64_t i = 0; i < n; i += per) {
+        const uint64_t m = std::min(per, n - i);
+        k_rows_scales<<<(unsigned)((m + 255) / 256), 256, 0, stream>>>(scales + i, m, flags);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+size_t wh_expert_plan_scratch(size_t n, size_t n_groups) {
+    const size_t chunks = (n + kPlanChunk - 1) / kPlanChunk;
+    return chunks > 1 ? chunks * n_groups * sizeof(uint32_t) : 0;
+}
+
+hipError_t wh_expert_plan_launch(const wh_expert_plan_args& a, hipStream_t stream) {
+    const uint32_t chunks = std::max(1u, (a.n + kPlanChunk - 1) / kPlanChunk);
+    uint32_t bits = 1;
+    while ((a.n_groups >> bits) != 0) ++bits;
+    if (chunks > 1) {
+        k_expert_count<<<chunks, kPlanThreads, 0, stream>>>(a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    k_expert_place<<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
+    return hipGetLastError();
+}
+
+hipError_t wh_expert_combine_launch(const wh_expert_combine_args& a, bool bf16, hipStream_t stream) {
+    const uint32_t units = (a.hidden / 4 + 255) / 256;
+    const uint64_t grid = (uint64_t)a.npos * units;
+    if (grid > kMaxGrid256) return hipErrorInvalidValue;
+    if (bf16) k_expert_combine<true><<<(unsigned)grid, 256, 0, stream>>>(a, units);
+    else k_expert_combine<false><<<(unsigned)grid, 256, 0, stream>>>(a, units);
+    return hipGetLastError();
+}

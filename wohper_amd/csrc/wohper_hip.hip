@@ -31,6 +31,7 @@
 #include "fp8_exact_mm.h"
 #include "fp8_multi.h"
 #include "kv4.h"
+#include "fp8_rows.h"
 #include "moe_bmx.h"
 #include "probe.h"
 #include "quant_block.h"
@@ -62,6 +63,7 @@ struct Tensor {
     bool fast = false;     // resident lane layout (else original row-major)
     bool special = false;  // FP8 codes 0x7F/0xFF present
     bool zero_scale = false;  // FP4: some UE8M0 scale byte is 0 (the MFMA kernels would read it as 2^-127)
+    bool odd_scale = false;   // FP8: some UE8M0 scale byte is 0 or 255 (0.0 and inf; matrix instructions: 2^-127, NaN)
     size_t bytes = 0;
     size_t w_alloc = 0, s_alloc = 0;  // arena bytes behind w and s
 };
@@ -302,6 +304,7 @@ struct wh_ctx {
     Scratch moe_dyn;                        // a device route list resolved for the experts (wh_moe_dyn)
     Scratch attn_max;                       // attn_mx.h: the score tiles' maxima, of a fixed size
     Scratch kv4_part, kv4_ticket;           // the 4-bit cache: partial outputs of split attention, a plan's arrivals
+    Scratch rows_counts;                    // expert lists: routes of each expert by chunk
     Scratch layer;                          // the decode layer's state and activations between its steps
     bool exact = true;                      // routed experts in the reference's summation order
     int token_kernels = 1;                  // MFMA token kernels: bit 0 gate/up, bit 1 down on k_*_tok (else k_*_px)
@@ -321,7 +324,7 @@ struct wh_ctx {
     hipStream_t base_stream = nullptr, cap_stream = nullptr;
     std::vector<Scratch*> scratch() {
         return {&x_in, &y_out, &h, &ybuf, &cnt_y, &tmp, &batch, &routes, &bout, &gu, &relayout, &rtr, &rtr_cnt,
-                &mla, &hcs, &fp8mm_ws, &fp8mm_cnt, &moe_dyn, &attn_max, &kv4_part, &kv4_ticket, &layer};
+                &mla, &hcs, &fp8mm_ws, &fp8mm_cnt, &moe_dyn, &attn_max, &kv4_part, &kv4_ticket, &rows_counts, &layer};
     }
 };
 
@@ -2103,6 +2106,7 @@ int wh_init(int device, wh_ctx** out) {
     if (e == hipSuccess)
         e = c->attn_max.ensure((size_t)WH_POS_BATCH * WH_ATTN_MX_HEADS * WH_ATTN_MX_TILES * sizeof(float), false);
     if (e == hipSuccess) e = wh_kv4_setup();
+    if (e == hipSuccess) e = wh_rows_setup();
     if (e == hipSuccess) e = c->kv4_ticket.ensure(sizeof(uint32_t), true);
     if (e != hipSuccess) {
         delete c;
@@ -2248,6 +2252,9 @@ int wh_store_fp8(wh_ctx* c, const uint8_t* weight, size_t weight_len, size_t row
     t.scale_fmt = scale_format;
     t.fast = (cols / scale_cols == 128) && cols * 4 <= g_max_lds;
     for (size_t i = 0; i < rows * cols && !t.special; ++i) t.special = (weight[i] & 0x7f) == 0x7f;
+    if (scale_format == WH_SCALE_UE8M0)
+        for (size_t i = 0; i < sbytes && !t.odd_scale; ++i)
+            t.odd_scale = ((const uint8_t*)scales)[i] == 0 || ((const uint8_t*)scales)[i] == 255;
     t.bytes = rows * cols + sbytes;
     WH_TRY(alloc_tensor(c, t, rows * cols, sbytes));
     const size_t chunk_rows = std::max<size_t>(1, (size_t(64) << 20) / cols);
@@ -2724,6 +2731,50 @@ int wh_store_fp8_synthetic(wh_ctx* c, size_t rows, size_t cols, uint64_t seed, u
     k_synth_fp8<<<(unsigned)((n + 255) / 256), 256, 0, c->stream>>>(t.w, (uint32_t)rows, (uint32_t)cols, seed, stream);
     WH_HIP(hipGetLastError());
     WH_TRY(upload(c, t.s, scales, sbytes));
+    return store_tensor_common(c, std::move(t), out);
+}
+
+int wh_store_fp8_device(wh_ctx* c, const uint8_t* weight_dev, size_t rows, size_t cols, const void* scales_dev,
+                        size_t scale_rows, size_t scale_cols, int scale_format, wh_tensor* out) {
+    if (!c || !out || !weight_dev || !scales_dev) return WH_INVALID_ARGUMENT;
+    if (scale_format != WH_SCALE_UE8M0 && scale_format != WH_SCALE_F32) return WH_INVALID_QUANT_FORMAT;
+    if (scale_format == WH_SCALE_F32 && ((uintptr_t)scales_dev & 3)) return WH_INVALID_ARGUMENT;
+    if (rows == 0 || cols == 0 || scale_rows == 0 || scale_cols == 0 || rows % scale_rows || cols % scale_cols ||
+        cols / scale_cols != 128 || cols % 128)
+        return WH_INVALID_SHAPE;
+    if (rows > 0xffffffffu || cols * 4 > g_max_lds) return WH_UNSUPPORTED;  // the lane layout's widths
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    if (c->capturing) return WH_INVALID_ARGUMENT;  // a store waits for the device
+    WH_HIP(hipSetDevice(c->device));
+    Tensor t;
+    t.kind = kFp8;
+    t.rows = rows;
+    t.cols = cols;
+    t.scale_rows = scale_rows;
+    t.scale_cols = scale_cols;
+    t.scale_fmt = scale_format;
+    t.fast = true;
+    const size_t n_scales = scale_rows * scale_cols, sbytes = n_scales * (scale_format == WH_SCALE_F32 ? 4 : 1);
+    t.bytes = rows * cols + sbytes;
+    WH_HIP(c->rows_counts.ensure(sizeof(uint32_t), false));
+    WH_TRY(alloc_tensor(c, t, rows * cols, sbytes));
+    uint32_t* const flags = c->rows_counts.as<uint32_t>();
+    uint32_t seen = 0;
+    hipError_t e = hipMemsetAsync(flags, 0, sizeof seen, c->stream);
+    if (e == hipSuccess) e = wh_rows_store_launch(weight_dev, t.w, rows, (uint32_t)cols, flags, c->stream);
+    if (e == hipSuccess && scale_format == WH_SCALE_UE8M0)
+        e = wh_rows_scales_launch((const uint8_t*)scales_dev, n_scales, flags, c->stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(t.s, scales_dev, sbytes, hipMemcpyDeviceToDevice, c->stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(c->status_host, flags, sizeof seen, hipMemcpyDeviceToHost, c->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+    if (e != hipSuccess) {
+        c->arena.free(t.w, t.w_alloc);
+        c->arena.free(t.s, t.s_alloc);
+        return hip_status(e);
+    }
+    seen = *c->status_host;
+    t.special = seen & 1;
+    t.odd_scale = seen & 2;
     return store_tensor_common(c, std::move(t), out);
 }
 
@@ -4817,5 +4868,208 @@ int wh_kv4_attention_async(wh_ctx* c, const wh_kv4_cache* cache, const wh_kv4_at
     WH_HIP(c->kv4_part.ensure(p.part_bytes, false));
     a.part = c->kv4_part.as<float>();
     WH_HIP(wh_kv4_attn_launch(a, d->is_bf16 != 0, !has_v, c->stream));
+    return WH_OK;
+}
+
+// ------------------------------------------------------------ 8-bit rows
+
+namespace {
+constexpr size_t kMaxStride = (size_t)1 << 40;
+
+// An 8-bit rows descriptor for n rows of cols columns.
+int rows8_check(const wh_fp8_rows* r, size_t n, size_t cols, wh_rows8* out) {
+    if (!r) return WH_INVALID_ARGUMENT;
+    if (cols == 0) return WH_EMPTY_SHAPE;
+    if (cols % 128) return WH_INVALID_SHAPE;
+    if (n > 0x7fffffffu || cols > 0xffffff80u || r->stride > kMaxStride || r->scale_stride > kMaxStride) return WH_UNSUPPORTED;
+    if (n && (!r->codes || !r->scales || ((uintptr_t)r->codes & 15) || ((uintptr_t)r->scales & 3) || r->stride % 16 ||
+              r->scale_stride % 4))
+        return WH_INVALID_ARGUMENT;
+    if (n && (r->stride < cols || r->scale_stride < (cols / 128 + 3) / 4 * 4)) return WH_INVALID_SHAPE;
+    *out = wh_rows8{r->codes, r->stride, r->scales, r->scale_stride};
+    return WH_OK;
+}
+
+// Rows of f32 or bf16 values on boundaries of `unit` values.
+int rows_float_check(const void* p, size_t stride, size_t width, int bf16, size_t unit) {
+    if (!p || ((uintptr_t)p & (unit * (bf16 ? 2 : 4) - 1)) || stride % unit) return WH_INVALID_ARGUMENT;
+    if (stride > kMaxStride) return WH_UNSUPPORTED;
+    return stride < width ? WH_INVALID_SHAPE : WH_OK;
+}
+
+int rows_quant(wh_ctx* c, const void* x, const void* up, size_t x_stride, int bf16, size_t n, size_t cols, float limit,
+               const wh_fp8_rows* out) {
+    if (!c) return WH_INVALID_ARGUMENT;
+    wh_rows_quant_args a{};
+    WH_TRY(rows8_check(out, n, cols, &a.out));
+    if (n == 0) return WH_OK;
+    WH_TRY(rows_float_check(x, x_stride, cols, bf16, 1));
+    if (up) WH_TRY(rows_float_check(up, x_stride, cols, bf16, 1));
+    if (n * (cols / 128) > 0xffffff0u) return WH_UNSUPPORTED;  // a grid has less than 2^32 threads
+    a.x = x;
+    a.up = up;
+    a.x_stride = x_stride;
+    a.n = (uint32_t)n;
+    a.blocks = (uint32_t)(cols / 128);
+    a.limit = limit;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    WH_HIP(hipSetDevice(c->device));
+    WH_HIP(wh_rows_quant_launch(a, bf16 != 0, c->stream));
+    return WH_OK;
+}
+
+// A product's arguments but for the tensor's.
+int rows_mm_args(const wh_fp8_rows* x, size_t n_x, const uint32_t* rows, const uint32_t* starts, size_t n_groups,
+                 size_t n, void* y, size_t y_stride, int bf16, size_t cols, size_t out_rows, wh_rows_mm_args* a) {
+    WH_TRY(rows8_check(x, n_x, cols, &a->x));
+    WH_TRY(rows_float_check(y, y_stride, out_rows, bf16, 1));
+    a->rows = rows;
+    a->starts = starts;
+    a->y = y;
+    a->y_stride = y_stride;
+    a->n = (uint32_t)n;
+    a->n_x = (uint32_t)n_x;
+    a->n_groups = (uint32_t)n_groups;
+    a->out_rows = (uint32_t)out_rows;
+    a->cols = (uint32_t)cols;
+    a->y_vec = y_stride % 4 == 0 && ((uintptr_t)y & (bf16 ? 7 : 15)) == 0;
+    return WH_OK;
+}
+
+int rows_mm_go(wh_ctx* c, const Tensor& t, size_t row_start, wh_rows_mm_args& a, int bf16) {
+    a.w = t.w;
+    a.w_scales = t.s;
+    a.row_start = row_start;
+    a.row_block = (uint32_t)(t.rows / t.scale_rows);
+    a.scale_f32 = t.scale_fmt == WH_SCALE_F32;
+    a.special = t.special;
+    a.odd_scale = t.odd_scale;
+    if (!wh_rows_mm_fits(a)) return WH_UNSUPPORTED;
+    WH_HIP(hipSetDevice(c->device));
+    WH_HIP(wh_rows_mm_launch(a, bf16 != 0, c->stream));
+    return WH_OK;
+}
+
+// A tensor that products of 8-bit rows take.
+int rows_mm_tensor(const Tensor* t) {
+    if (!t) return WH_NOT_RESIDENT;
+    if (t->kind != kFp8) return WH_INVALID_QUANT_FORMAT;
+    return t->fast && t->rows <= 0xffffffffu ? WH_OK : WH_UNSUPPORTED;
+}
+}  // namespace
+
+int wh_fp8_quant_rows_async(wh_ctx* c, const void* x_dev, size_t x_stride, int is_bf16, size_t n, size_t cols,
+                            const wh_fp8_rows* out) {
+    return rows_quant(c, x_dev, nullptr, x_stride, is_bf16, n, cols, 0.0f, out);
+}
+
+int wh_fp8_swiglu_rows_async(wh_ctx* c, const void* gate_dev, const void* up_dev, size_t stride, int is_bf16, size_t n,
+                             size_t cols, float limit, const wh_fp8_rows* out) {
+    if (!(limit > 0.0f) || (n && !up_dev)) return WH_INVALID_ARGUMENT;
+    return rows_quant(c, gate_dev, up_dev, stride, is_bf16, n, cols, limit, out);
+}
+
+int wh_fp8_read_rows_async(wh_ctx* c, const wh_fp8_rows* rows, size_t n, size_t cols, void* out_dev, size_t out_stride,
+                           int is_bf16) {
+    if (!c) return WH_INVALID_ARGUMENT;
+    wh_rows_read_args a{};
+    WH_TRY(rows8_check(rows, n, cols, &a.in));
+    if (n == 0) return WH_OK;
+    WH_TRY(rows_float_check(out_dev, out_stride, cols, is_bf16, 1));
+    if (n * (cols / 128) > 0xffffff0u) return WH_UNSUPPORTED;  // a grid has less than 2^32 threads
+    a.out = out_dev;
+    a.out_stride = out_stride;
+    a.n = (uint32_t)n;
+    a.blocks = (uint32_t)(cols / 128);
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    WH_HIP(hipSetDevice(c->device));
+    WH_HIP(wh_rows_read_launch(a, is_bf16 != 0, c->stream));
+    return WH_OK;
+}
+
+int wh_fp8_rows_mm_async(wh_ctx* c, wh_tensor w, size_t row_start, size_t row_end, const wh_fp8_rows* x, size_t n,
+                         void* y_dev, size_t y_stride, int is_bf16) {
+    if (!c || !x) return WH_INVALID_ARGUMENT;
+    if (row_start >= row_end) return WH_INVALID_SHAPE;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    const Tensor* t = find_tensor(c, w);
+    WH_TRY(rows_mm_tensor(t));
+    if (row_end > t->rows) return WH_INVALID_SHAPE;
+    wh_rows_mm_args a{};
+    if (n == 0) return WH_OK;
+    WH_TRY(rows_mm_args(x, n, nullptr, nullptr, 1, n, y_dev, y_stride, is_bf16, t->cols, row_end - row_start, &a));
+    return rows_mm_go(c, *t, row_start, a, is_bf16);
+}
+
+int wh_fp8_rows_mm_groups_async(wh_ctx* c, wh_tensor w, size_t row_start, size_t group_rows, size_t n_groups,
+                                const wh_fp8_rows* x, size_t n_x, const uint32_t* rows_dev, const uint32_t* starts_dev,
+                                size_t n, void* y_dev, size_t y_stride, int is_bf16) {
+    if (!c || !x || !starts_dev || ((uintptr_t)starts_dev & 3) || ((uintptr_t)rows_dev & 3)) return WH_INVALID_ARGUMENT;
+    if (group_rows == 0 || n_groups == 0) return WH_EMPTY_SHAPE;
+    if (n_groups > WH_ROWS_MAX_GROUPS || n > 0x7fffffffu) return WH_UNSUPPORTED;
+    if (!rows_dev && n_x < n) return WH_INPUT_TOO_SMALL;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    const Tensor* t = find_tensor(c, w);
+    WH_TRY(rows_mm_tensor(t));
+    if (row_start > t->rows || group_rows > (t->rows - row_start) / n_groups) return WH_INVALID_SHAPE;
+    wh_rows_mm_args a{};
+    if (n == 0) return WH_OK;
+    WH_TRY(rows_mm_args(x, n_x, rows_dev, starts_dev, n_groups, n, y_dev, y_stride, is_bf16, t->cols, group_rows, &a));
+    return rows_mm_go(c, *t, row_start, a, is_bf16);
+}
+
+int wh_expert_plan_async(wh_ctx* c, const uint32_t* ids_dev, size_t npos, size_t topk, size_t n_experts,
+                         uint32_t* starts_dev, uint32_t* rows_dev, uint32_t* slots_dev) {
+    if (!c || !starts_dev) return WH_INVALID_ARGUMENT;
+    if (topk == 0 || n_experts == 0) return WH_EMPTY_SHAPE;
+    if (n_experts > WH_ROWS_MAX_GROUPS || topk > 65536 || npos > 0x7fffffffu / topk) return WH_UNSUPPORTED;
+    if (npos && (!ids_dev || !rows_dev || !slots_dev)) return WH_INVALID_ARGUMENT;
+    for (const void* p : {(const void*)ids_dev, (const void*)starts_dev, (const void*)rows_dev, (const void*)slots_dev})
+        if ((uintptr_t)p & 3) return WH_INVALID_ARGUMENT;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    WH_HIP(hipSetDevice(c->device));
+    wh_expert_plan_args a{};
+    WH_HIP(c->rows_counts.ensure(wh_expert_plan_scratch(npos * topk, n_experts), false));
+    a.ids = ids_dev;
+    a.starts = starts_dev;
+    a.rows = rows_dev;
+    a.slots = slots_dev;
+    a.counts = c->rows_counts.as<uint32_t>();
+    a.n = (uint32_t)(npos * topk);
+    a.topk = (uint32_t)topk;
+    a.n_groups = (uint32_t)n_experts;
+    WH_HIP(wh_expert_plan_launch(a, c->stream));
+    return WH_OK;
+}
+
+int wh_expert_combine_async(wh_ctx* c, const void* y_dev, size_t y_stride, int is_bf16, size_t n_rows,
+                            const uint32_t* slots_dev, const float* weights_dev, size_t npos, size_t topk, size_t hidden,
+                            const float* add_dev, size_t add_stride, float* out_dev, size_t out_stride) {
+    if (!c) return WH_INVALID_ARGUMENT;
+    if (hidden == 0 || topk == 0) return WH_EMPTY_SHAPE;
+    if (hidden % 4) return WH_INVALID_SHAPE;
+    if (hidden > 0x7fffffffu || topk > 65536 || npos > 0x7fffffffu / topk || n_rows > 0x7fffffffu) return WH_UNSUPPORTED;
+    if (npos == 0) return WH_OK;
+    if (!slots_dev || !weights_dev || ((uintptr_t)slots_dev & 3) || ((uintptr_t)weights_dev & 3)) return WH_INVALID_ARGUMENT;
+    if (n_rows) WH_TRY(rows_float_check(y_dev, y_stride, hidden, is_bf16, 4));
+    if (add_dev) WH_TRY(rows_float_check(add_dev, add_stride, hidden, 0, 4));
+    WH_TRY(rows_float_check(out_dev, out_stride, hidden, 0, 4));
+    if (npos * ((hidden / 4 + 255) / 256) > 0xffffffu) return WH_UNSUPPORTED;  // a grid has less than 2^32 threads
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    WH_HIP(hipSetDevice(c->device));
+    wh_expert_combine_args a{};
+    a.y = y_dev;
+    a.y_stride = y_stride;
+    a.out_stride = out_stride;
+    a.add_stride = add_stride;
+    a.slots = slots_dev;
+    a.weights = weights_dev;
+    a.add = add_dev;
+    a.out = out_dev;
+    a.n_rows = (uint32_t)n_rows;
+    a.npos = (uint32_t)npos;
+    a.topk = (uint32_t)topk;
+    a.hidden = (uint32_t)hidden;
+    WH_HIP(wh_expert_combine_launch(a, is_bf16 != 0, c->stream));
     return WH_OK;
 }
