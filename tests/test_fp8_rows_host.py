@@ -81,7 +81,7 @@ def test_products_refused(lib_and_ctx):
     assert groups(rp=None) == groups(starts=None) == groups(starts=DEV + 2) == groups(rows_ptr=DEV + 1) == ARGUMENT
     assert groups(gr=0) == groups(ng=0) == EMPTY
     assert groups(ng=1025) == groups(n=1 << 31) == UNSUPPORTED
-    assert groups(n_x=3) == SMALL
+    assert groups(n_x=3) == groups(rows_ptr=DEV, n_x=0) == SMALL
 
 
 def test_plans_refused(lib_and_ctx):

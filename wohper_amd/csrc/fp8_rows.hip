@@ -237,6 +237,248 @@ __global__ void __launch_bounds__(256) k_rows_mm_any(wh_rows_mm_args a) {
     if (r0 + row16 < r1 && c0 + lane16 < a.out_rows) rows_put<kBf16>(a, r0 + row16, c0 + lane16, acc);
 }
 
+// ------------------------------------------------- matrix instructions
+//
+// Weights are the first operand and x rows the second, so a lane of a 16 x 16
+// result holds four consecutive columns of one y row.  A lane brings 32 bytes of a
+// 128-byte block, its 16-byte chunks q and 4 + q (q = lane / 16): which columns
+// those are is the same for both sides.
+//
+// bf16 results take the 8-bit instruction with both scales as its block scales.
+// It aligns the products of eight bytes to the largest of them and keeps 13 bits
+// under it, so an f32 result would be 2e-5 to 6e-5 off (of the results' norm, rows
+// of 4096): a hundredth of what rounding to bf16 does, and a hundred times what an
+// f32 sum does.  So f32 results decode both sides to f16, which holds every E4M3
+// value, and add a block up in the f16 instruction (8e-8 to 4e-7 off), scaled
+// after it.
+
+typedef int wh_i8 __attribute__((ext_vector_type(8)));
+typedef _Float16 wh_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 wh_h8 __attribute__((ext_vector_type(8)));
+
+struct rows_frag {
+    wh_u4 a, b;
+};
+
+__device__ __forceinline__ wh_i8 rows_codes(const rows_frag& f) {
+    return wh_i8{(int)f.a.x, (int)f.a.y, (int)f.a.z, (int)f.a.w, (int)f.b.x, (int)f.b.y, (int)f.b.z, (int)f.b.w};
+}
+
+// Eight codes as f16.
+__device__ __forceinline__ wh_h8 rows_f16(uint32_t lo, uint32_t hi) {
+    const wh_h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+    const wh_h2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+    const wh_h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+    const wh_h2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+    return wh_h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+struct rows_f16x4 {
+    wh_h8 v[4];
+};
+__device__ __forceinline__ rows_f16x4 rows_decode(const rows_frag& f) {
+    return rows_f16x4{{rows_f16(f.a.x, f.a.y), rows_f16(f.a.z, f.a.w), rows_f16(f.b.x, f.b.y), rows_f16(f.b.z, f.b.w)}};
+}
+
+// acc + (block of codes) * 2^e * m.
+__device__ __forceinline__ wh_f4 rows_scaled(wh_f4 acc, wh_f4 block, int e, float m) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(ldexpf(block[i], e), m, acc[i]);
+    return acc;
+}
+
+// A weight scale as the byte of a power of two and a factor: 1 for ordinary UE8M0
+// bytes, else in [1, 2), or the scale itself where it is no normal number.
+__device__ __forceinline__ uint32_t rows_split_scale(const wh_rows_mm_args& a, uint64_t at, float* m) {
+    *m = 1.0f;
+    if (!a.scale_f32) {
+        const uint32_t byte = ((const uint8_t*)a.w_scales)[at];
+        if (byte != 0 && byte != 255) return byte;
+        *m = wh_ue8m0(byte);
+        return 127;
+    }
+    const float s = ((const float*)a.w_scales)[at];
+    const uint32_t u = __float_as_uint(s), e = u >> 23 & 0xff;
+    if (e == 255 || (u & 0x7fffffffu) == 0) {
+        *m = s;
+        return 127;
+    }
+    if (e == 0) {
+        *m = s * 1.70141183460469231732e38f;  // 2^127
+        return 0;
+    }
+    *m = __uint_as_float((u & 0x807fffffu) | 0x3f800000u);
+    return e;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void rows_put4(const wh_rows_mm_args& a, uint64_t row, uint32_t col, wh_f4 v) {
+    if (a.y_vec && col + 4 <= a.out_rows) {
+        if constexpr (kBf16) {
+            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+            *(b4*)((__bf16*)a.y + row * a.y_stride + col) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        } else {
+            *(wh_f4*)((float*)a.y + row * a.y_stride + col) = v;
+        }
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+        if (col + i < a.out_rows) rows_put<kBf16>(a, row, col + i, v[i]);
+}
+
+// The x row of listed row j, and whether it is one.
+__device__ __forceinline__ uint32_t rows_source(const wh_rows_mm_args& a, uint32_t j, bool* is) {
+    const uint32_t r = a.rows ? a.rows[j] : j;
+    *is = r < a.n_x;
+    return *is ? r : 0;
+}
+
+// Few rows a group: bound by the weights' bytes.  A wave takes 16 weight rows and
+// every kS-th block of their columns for up to 16 kMt x rows, straight from memory
+// into registers; the kS waves of the same weight rows join in LDS.  Blocks come
+// kU at a time, all their loads before the first product.
+constexpr uint32_t kThinWaves = 8;
+template <int kMt, bool kBf16, bool kMant>
+__device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part)[64][4], uint32_t ks_n, uint32_t g, uint32_t j0,
+                                          uint32_t j1, uint32_t c0) {
+    constexpr int kU = kMt == 1 ? 4 : kMt == 2 ? 2 : 1;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t ks = wave & (ks_n - 1), l16 = lane & 15, q = lane >> 4;
+    const uint32_t blocks = a.cols / 128u, col0 = c0 + 16 * (wave / ks_n);
+    const bool works = col0 < a.out_rows;
+    wh_f4 acc[kMt];
+    const uint8_t *xp[kMt], *xs[kMt];
+    bool have[kMt], nan[kMt];
+#pragma unroll
+    for (int t = 0; t < kMt; ++t) {
+        const uint32_t src = rows_source(a, min(j0 + 16 * t + l16, j1 - 1), &have[t]);
+        xp[t] = a.x.codes + (uint64_t)src * a.x.stride + 16 * q;
+        xs[t] = a.x.scales + (uint64_t)src * a.x.scale_stride;
+        acc[t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        nan[t] = false;
+    }
+    if (works) {
+        const uint64_t w_row = a.row_start + (uint64_t)g * a.out_rows + col0;
+        const uint8_t* const wp = a.w + (w_row + min(l16, a.out_rows - 1 - col0)) * a.cols + 16 * q;
+        // scales of this wave's blocks, one a lane: 16 rows share one
+        float wm = 1.0f;
+        uint32_t wb = 127;
+        if (ks + ks_n * lane < blocks) wb = rows_split_scale(a, w_row / a.row_block * blocks + ks + ks_n * lane, &wm);
+        const uint32_t mine = (blocks - ks + ks_n - 1) / ks_n;  // 64 at most
+        for (uint32_t i0 = 0; i0 < mine; i0 += kU) {
+            rows_frag w[kU], x[kU][kMt];
+            uint32_t xb[kU][kMt];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const uint32_t b = min(ks + ks_n * (i0 + u), blocks - 1);
+                w[u].a = *(const wh_u4*)(wp + b * 128u);
+                w[u].b = *(const wh_u4*)(wp + b * 128u + 64);
+#pragma unroll
+                for (int t = 0; t < kMt; ++t) {
+                    x[u][t].a = *(const wh_u4*)(xp[t] + b * 128u);
+                    x[u][t].b = *(const wh_u4*)(xp[t] + b * 128u + 64);
+                    xb[u][t] = xs[t][b];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                if (i0 + u < mine) {
+                    const int byte = __builtin_amdgcn_readlane((int)wb, i0 + u);
+                    const float m = kMant ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wm), i0 + u)) : 1.0f;
+                    if constexpr (kBf16) {
+                        const wh_i8 wc = rows_codes(w[u]);
+#pragma unroll
+                        for (int t = 0; t < kMt; ++t) {
+                            const wh_f4 from = kMant ? wh_f4{0.0f, 0.0f, 0.0f, 0.0f} : acc[t];
+                            const wh_f4 s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wc, rows_codes(x[u][t]), from, 0,
+                                                                                             0, 0, byte, 0, (int)xb[u][t]);
+                            if constexpr (kMant) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(s[i], m, acc[t][i]);
+                            } else {
+                                acc[t] = s;
+                            }
+                        }
+                    } else {
+                        const rows_f16x4 wv = rows_decode(w[u]);
+#pragma unroll
+                        for (int t = 0; t < kMt; ++t) {
+                            const rows_f16x4 xv = rows_decode(x[u][t]);
+                            wh_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv.v[j], xv.v[j], s, 0, 0, 0);
+                            acc[t] = rows_scaled(acc[t], s, (int)xb[u][t] + byte - 254, m);
+                            nan[t] |= xb[u][t] == 255;
+                        }
+                    }
+                }
+            }
+        }
+        if constexpr (!kBf16) {
+#pragma unroll
+            for (int t = 0; t < kMt; ++t)
+                if (nan[t]) acc[t] = wh_f4{1.0f, 1.0f, 1.0f, 1.0f} * __uint_as_float(0x7fc00000u);
+        }
+    }
+    if (ks_n > 1) {
+        __syncthreads();  // the parts of the rows before have been read
+#pragma unroll
+        for (int t = 0; t < kMt; ++t) *(wh_f4*)part[wave * kMt + t][lane] = acc[t];
+        __syncthreads();
+    }
+    if (!works) return;
+#pragma unroll
+    for (int t = 0; t < kMt; ++t) {
+        if ((t & (ks_n - 1)) != ks) continue;
+        wh_f4 v = acc[t];
+        if (ks_n > 1) {
+            const uint32_t first = wave - ks;
+            v = *(const wh_f4*)part[first * kMt + t][lane];
+            for (uint32_t s = 1; s < ks_n; ++s) v += *(const wh_f4*)part[(first + s) * kMt + t][lane];
+        }
+        const uint32_t j = j0 + 16 * t + l16;
+        if (j < j1) rows_put4<kBf16>(a, j, col0 + 4 * q, have[t] ? v : wh_f4{0.0f, 0.0f, 0.0f, 0.0f});
+    }
+}
+
+template <bool kBf16, bool kMant>
+__global__ void __launch_bounds__(64 * kThinWaves) k_rows_mm_thin(wh_rows_mm_args a, uint32_t ks_n) {
+    __shared__ __align__(16) float part[kThinWaves * 4][64][4];
+    const uint32_t g = blockIdx.y, c0 = blockIdx.x * 16 * (kThinWaves / ks_n);
+    uint32_t j0 = 0, j1 = a.n;
+    if (a.starts) {
+        j0 = min(a.starts[g], a.n);
+        j1 = min(a.starts[g + 1], a.n);
+    }
+    while (j0 < j1) {
+        const uint32_t left = j1 - j0;
+        if (left <= 16) {
+            rows_thin<1, kBf16, kMant>(a, part, ks_n, g, j0, j1, c0);
+            return;
+        }
+        if (left <= 32) {
+            rows_thin<2, kBf16, kMant>(a, part, ks_n, g, j0, j1, c0);
+            return;
+        }
+        rows_thin<4, kBf16, kMant>(a, part, ks_n, g, j0, j1, c0);
+        j0 += 64;
+    }
+}
+
+// The waves that share weight rows in the thin kernel: as many as leave each four
+// blocks of columns, whose loads are in flight together.
+uint32_t rows_thin_split(uint32_t cols) {
+    uint32_t ks = 1;
+    while (ks < kThinWaves && cols / 128u >= 8 * ks) ks *= 2;
+    return ks;
+}
+
+// Whether the matrix instructions take a call: every 16 rows of a tile share a
+// scale, and codes mean the same.
+bool rows_mm_matrix(const wh_rows_mm_args& a) {
+    return !a.special && a.row_block % 16 == 0 && a.row_start % 16 == 0 && (a.out_rows % 16 == 0 || a.n_groups == 1);
+}
+
 // Most tiles of kRows listed rows that a call can have.
 uint64_t rows_tiles(const wh_rows_mm_args& a, uint32_t rows) {
     const uint64_t full = ((uint64_t)a.n + rows - 1) / rows;
@@ -458,6 +700,20 @@ bool wh_rows_mm_fits(const wh_rows_mm_args& a) {
 }
 
 hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, bool bf16, hipStream_t stream) {
+    const bool mant = a.scale_f32 || a.odd_scale;
+    if (rows_mm_matrix(a)) {
+        const uint32_t ks = rows_thin_split(a.cols), per = 16 * (kThinWaves / ks);
+        const dim3 grid((a.out_rows + per - 1) / per, a.n_groups);
+        auto go = [&](auto kern) { kern<<<grid, 64 * kThinWaves, 0, stream>>>(a, ks); };
+        if (bf16) {
+            if (mant) go(k_rows_mm_thin<true, true>);
+            else go(k_rows_mm_thin<true, false>);
+        } else {
+            if (mant) go(k_rows_mm_thin<false, true>);
+            else go(k_rows_mm_thin<false, false>);
+        }
+        return hipGetLastError();
+    }
     const unsigned grid = (unsigned)(rows_tiles(a, kAnyRows) * ((a.out_rows + 15) / 16));
     if (bf16) k_rows_mm_any<true><<<grid, 256, 0, stream>>>(a);
     else k_rows_mm_any<false><<<grid, 256, 0, stream>>>(a);

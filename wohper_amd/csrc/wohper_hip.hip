@@ -5007,7 +5007,7 @@ int wh_fp8_rows_mm_groups_async(wh_ctx* c, wh_tensor w, size_t row_start, size_t
     if (!c || !x || !starts_dev || ((uintptr_t)starts_dev & 3) || ((uintptr_t)rows_dev & 3)) return WH_INVALID_ARGUMENT;
     if (group_rows == 0 || n_groups == 0) return WH_EMPTY_SHAPE;
     if (n_groups > WH_ROWS_MAX_GROUPS || n > 0x7fffffffu) return WH_UNSUPPORTED;
-    if (!rows_dev && n_x < n) return WH_INPUT_TOO_SMALL;
+    if (rows_dev ? n && !n_x : n_x < n) return WH_INPUT_TOO_SMALL;
     std::lock_guard<std::recursive_mutex> lk(c->mu);
     const Tensor* t = find_tensor(c, w);
     WH_TRY(rows_mm_tensor(t));
