@@ -465,6 +465,244 @@ __global__ void __launch_bounds__(64 * kThinWaves) k_rows_mm_thin(wh_rows_mm_arg
     }
 }
 
+// LDS byte address of a pointer into __shared__ memory.
+__device__ __forceinline__ uint32_t rows_lds(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
+}
+// One 16-byte load a lane straight into LDS: lane l's bytes land at lds + 16 l.  The
+// compiler does not see them, so its own waits do not empty the queue: rows_arrived
+// waits for them.
+__device__ __forceinline__ void rows_dma(const uint8_t* p, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void rows_dma(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+}
+// All of this wave's loads have landed and its LDS reads are done, and every wave's.
+__device__ __forceinline__ void rows_arrived() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// A workgroup's tile: listed rows [r0, r1) of group g and columns from c0 on.  Tiles
+// are numbered group by group, in bands of kBand tiles of rows, columns outside rows,
+// and every XCD (workgroup id mod 8) takes a run of consecutive ones, so that those
+// in flight on one L2 share rows and weights.  False behind the last tile.
+constexpr uint32_t kBand = 8;
+template <uint32_t kM, uint32_t kN>
+__device__ __forceinline__ bool rows_place(const wh_rows_mm_args& a, uint32_t& g, uint32_t& r0, uint32_t& r1, uint32_t& c0) {
+    const uint32_t n_tiles = (a.out_rows + kN - 1) / kN, lane = threadIdx.x & 63;
+    auto group = [&](uint32_t at, uint32_t& s, uint32_t& e) {
+        s = e = 0;
+        if (at < a.n_groups) {
+            s = a.starts ? min(a.starts[at], a.n) : 0;
+            e = a.starts ? max(s, min(a.starts[at + 1], a.n)) : a.n;
+        }
+        return (e - s + kM - 1) / kM;
+    };
+    // 64 bits: starts that do not ascend may count rows more than once
+    uint32_t s, e;
+    uint64_t total = 0;
+    for (uint32_t base = 0; base < a.n_groups; base += 64) {
+        uint32_t sum = group(base + lane, s, e);
+        for (uint32_t off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        total += (uint32_t)__builtin_amdgcn_readfirstlane(sum);
+    }
+    total *= n_tiles;
+    const uint64_t per = (total + 7) / 8;
+    const uint32_t slot = blockIdx.x / 8;
+    uint64_t t = (blockIdx.x & 7) * per + slot;
+    if (slot >= per || t >= total) return false;
+    for (uint32_t base = 0; base < a.n_groups; base += 64) {
+        const uint32_t tiles = group(base + lane, s, e);
+        uint32_t upto = tiles;
+#pragma unroll
+        for (uint32_t off = 1; off < 64; off <<= 1) {
+            const uint32_t y = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += y;
+        }
+        const uint64_t past = __ballot((uint64_t)upto * n_tiles > t);
+        if (past) {
+            const uint32_t first = (uint32_t)__builtin_ctzll(past);
+            const uint32_t mine = __builtin_amdgcn_readlane((int)tiles, first);
+            const uint64_t own = t - (uint64_t)((uint32_t)__builtin_amdgcn_readlane((int)upto, first) - mine) * n_tiles;
+            g = base + first;
+            const uint32_t band = (uint32_t)(own / (kBand * n_tiles)), in = (uint32_t)(own % (kBand * n_tiles));
+            const uint32_t high = min(kBand, mine - band * kBand);
+            const uint32_t end = __builtin_amdgcn_readlane((int)e, first);
+            r0 = __builtin_amdgcn_readlane((int)s, first) + (band * kBand + in % high) * kM;
+            r1 = min(end, r0 + kM);
+            c0 = in / high * kN;
+            return true;
+        }
+        t -= (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * n_tiles;
+    }
+    return false;
+}
+
+// Many rows a group: tiles of kM x kN outputs in LDS.  Both sides' blocks of 128 bytes
+// go straight from memory into LDS, one step ahead, 16-byte chunk c of row r at place
+// c ^ (r % 8), so that the 16-byte reads of a column of chunks hit all banks.  Scales lie
+// in LDS too, kScaleBlocks blocks at a time, four rows' bytes (16 apart) in a word,
+// as the scaled instruction takes them.
+constexpr uint32_t kScaleBlocks = 64;
+template <int kMt, int kNt, int kWm, int kWn>
+struct rows_tile_shape {
+    static constexpr uint32_t kM = 16 * kMt * kWm, kN = 16 * kNt * kWn, kThreads = 64 * kWm * kWn;
+    static constexpr uint32_t kStage = (kM + kN) * 128, kXs = 2 * kStage, kWs = kXs + kScaleBlocks * kM;
+    static constexpr uint32_t kWm0 = kWs + kScaleBlocks * kN / 16, kNan = kWm0 + kScaleBlocks * kN / 4, kLds = kNan + kM;
+};
+
+// Brings the scales of blocks [b0, b0 + kScaleBlocks) into LDS.
+template <class S>
+__device__ __forceinline__ void rows_tile_scales(const wh_rows_mm_args& a, uint8_t* lds, uint32_t b0, uint32_t r0, uint32_t r1,
+                                                 uint64_t w0, uint32_t c0) {
+    const uint32_t blocks = a.cols / 128u, count = min(kScaleBlocks, blocks - b0), words = (count + 3) / 4;
+    for (uint32_t i = threadIdx.x; i < S::kM * (kScaleBlocks / 4); i += S::kThreads) {
+        const uint32_t r = i / (kScaleBlocks / 4), k = i % (kScaleBlocks / 4);
+        if (k >= words || r0 + r >= r1) continue;
+        bool is;
+        const uint32_t src = rows_source(a, r0 + r, &is);
+        const uint32_t v = *(const uint32_t*)(a.x.scales + (uint64_t)src * a.x.scale_stride + b0 + 4 * k);
+        uint8_t* const to = lds + S::kXs + ((4 * k * (S::kM / 64) + r / 64) * 16 + r % 16) * 4 + r % 64 / 16;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            to[j * S::kM] = (uint8_t)(v >> 8 * j);
+            if (4 * k + j < count && (v >> 8 * j & 0xff) == 255) lds[S::kNan + r] = 1;
+        }
+    }
+    for (uint32_t i = threadIdx.x; i < S::kN / 16 * kScaleBlocks; i += S::kThreads) {
+        const uint32_t k = i / (S::kN / 16), t = i % (S::kN / 16);
+        if (k >= count) continue;
+        const uint64_t row = w0 + min(c0 + 16 * t, a.out_rows - 1);
+        float m;
+        lds[S::kWs + k * (S::kN / 16) + t] = (uint8_t)rows_split_scale(a, row / a.row_block * blocks + b0 + k, &m);
+        *(float*)(lds + S::kWm0 + 4 * (k * (S::kN / 16) + t)) = m;
+    }
+}
+
+template <int kMt, int kNt, int kWm, int kWn, bool kBf16, bool kMant>
+__global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads), 2) k_rows_mm_tile(wh_rows_mm_args a) {
+    typedef rows_tile_shape<kMt, kNt, kWm, kWn> S;
+    static_assert(kMt == 4 && kNt == 4, "a word of scale bytes is four tiles");
+    extern __shared__ __align__(128) uint8_t tile_lds[];
+    uint8_t* const lds = tile_lds;
+    uint32_t g = 0, r0 = 0, r1 = 0, c0 = 0;
+    if (!rows_place<S::kM, S::kN>(a, g, r0, r1, c0)) return;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t l16 = lane & 15, q = lane >> 4, wm = wave % kWm, wn = wave / kWm, blocks = a.cols / 128u;
+    const uint64_t w0 = a.row_start + (uint64_t)g * a.out_rows;
+    constexpr uint32_t kWaves = kWm * kWn, kXd = S::kM / 8 / kWaves, kWd = S::kN / 8 / kWaves;
+    // this wave's loads: eight rows each, a lane one chunk
+    const uint8_t* xp[kXd];
+    uint32_t wo[kWd];
+    const uint32_t chunk = 16 * ((lane & 7) ^ (lane >> 3));
+#pragma unroll
+    for (uint32_t i = 0; i < kXd; ++i) {
+        bool is;
+        const uint32_t src = rows_source(a, min(r0 + (wave + i * kWaves) * 8 + (lane >> 3), r1 - 1), &is);
+        xp[i] = a.x.codes + (uint64_t)src * a.x.stride + chunk;
+    }
+    const uint8_t* wp = a.w + (w0 + c0) * a.cols;
+#pragma unroll
+    for (uint32_t i = 0; i < kWd; ++i)
+        wo[i] = min((wave + i * kWaves) * 8 + (lane >> 3), a.out_rows - 1 - c0) * a.cols + chunk;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rows_lds(lds));
+    auto bring = [&](uint32_t b) {
+        const uint32_t to = lds0 + (b & 1) * S::kStage + wave * 1024;
+#pragma unroll
+        for (uint32_t i = 0; i < kXd; ++i) rows_dma(xp[i] + b * 128u, to + i * kWaves * 1024);
+#pragma unroll
+        for (uint32_t i = 0; i < kWd; ++i) rows_dma(wp + b * 128u, wo[i], to + S::kM * 128 + i * kWaves * 1024);
+    };
+    if constexpr (!kBf16) {
+        for (uint32_t i = threadIdx.x; i < S::kM; i += S::kThreads) lds[S::kNan + i] = 0;
+    }
+    wh_f4 acc[kNt][kMt];
+#pragma unroll
+    for (int i = 0; i < kNt; ++i)
+#pragma unroll
+        for (int t = 0; t < kMt; ++t) acc[i][t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    bring(0);
+    const uint32_t at = l16 * 128 + ((q ^ (l16 & 7)) << 4);  // the lane's first chunk in a tile of 16 rows
+    for (uint32_t b = 0; b < blocks; ++b) {
+        if (b % kScaleBlocks == 0) {
+            __syncthreads();
+            rows_tile_scales<S>(a, lds, b, r0, r1, w0, c0);
+        }
+        rows_arrived();
+        if (b + 1 < blocks) bring(b + 1);
+        const uint8_t* const stage = lds + (b & 1) * S::kStage;
+        const uint8_t* const xt = stage + wm * (16 * kMt * 128);
+        const uint8_t* const wt = stage + S::kM * 128 + wn * (16 * kNt * 128);
+        const uint32_t k = b % kScaleBlocks;
+        const uint32_t xb = *(const uint32_t*)(lds + S::kXs + ((k * (S::kM / 64) + wm) * 16 + l16) * 4);
+        const uint32_t wb = *(const uint32_t*)(lds + S::kWs + (k * (S::kN / 64) + wn) * 4);
+        wh_f4 m = {1.0f, 1.0f, 1.0f, 1.0f};
+        if constexpr (kMant) m = *(const wh_f4*)(lds + S::kWm0 + (k * (S::kN / 64) + wn) * 16);
+        auto frag = [&](const uint8_t* p, int i) {
+            rows_frag f;
+            f.a = *(const wh_u4*)(p + i * 2048 + at);
+            f.b = *(const wh_u4*)(p + i * 2048 + (at ^ 64));
+            return f;
+        };
+        if constexpr (kBf16) {
+            wh_i8 x[kMt];
+#pragma unroll
+            for (int t = 0; t < kMt; ++t) x[t] = rows_codes(frag(xt, t));
+            wh_static_for<kNt>([&](auto iv) {
+                constexpr int i = decltype(iv)::value;
+                const wh_i8 w = rows_codes(frag(wt, i));
+                wh_static_for<kMt>([&](auto tv) {
+                    constexpr int t = decltype(tv)::value;
+                    if constexpr (kMant) {
+                        const wh_f4 s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                            w, x[t], wh_f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, i, (int)wb, t, (int)xb);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[i][t][j] = fmaf(s[j], m[i], acc[i][t][j]);
+                    } else {
+                        acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x[t], acc[i][t], 0, 0, i, (int)wb, t, (int)xb);
+                    }
+                });
+            });
+        } else {
+            rows_f16x4 w[kNt];
+#pragma unroll
+            for (int i = 0; i < kNt; ++i) w[i] = rows_decode(frag(wt, i));
+#pragma unroll
+            for (int t = 0; t < kMt; ++t) {
+                const rows_f16x4 x = rows_decode(frag(xt, t));
+                wh_f4 s[kNt];
+#pragma unroll
+                for (int i = 0; i < kNt; ++i) s[i] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < kNt; ++i) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i].v[j], x.v[j], s[i], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < kNt; ++i)
+                    acc[i][t] = rows_scaled(acc[i][t], s[i], (int)(xb >> 8 * t & 0xff) + (int)(wb >> 8 * i & 0xff) - 254, m[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kMt; ++t) {
+        const uint32_t r = wm * 16 * kMt + 16 * t + l16, j = r0 + r;
+        if (j >= r1) continue;
+        bool is = true;
+        if (a.rows) rows_source(a, j, &is);
+        bool nan = false;
+        if constexpr (!kBf16) nan = lds[S::kNan + r];
+#pragma unroll
+        for (int i = 0; i < kNt; ++i) {
+            wh_f4 v = acc[i][t];
+            if (nan) v = wh_f4{1.0f, 1.0f, 1.0f, 1.0f} * __uint_as_float(0x7fc00000u);
+            if (!is) v = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            const uint32_t col = c0 + (wn * kNt + i) * 16 + 4 * q;
+            if (col < a.out_rows) rows_put4<kBf16>(a, j, col, v);
+        }
+    }
+}
+
 // The waves that share weight rows in the thin kernel: as many as leave each four
 // blocks of columns, whose loads are in flight together.
 uint32_t rows_thin_split(uint32_t cols) {
@@ -670,8 +908,17 @@ constexpr uint64_t kMaxGrid256 = 0xffffffull;
 constexpr size_t plan_lds(uint32_t n_groups) { return kPlanWaves * (size_t)n_groups * sizeof(uint32_t); }
 
 hipError_t wh_rows_setup() {
-    return hipFuncSetAttribute((const void*)k_expert_place, hipFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)plan_lds(WH_ROWS_MAX_GROUPS));
+    hipError_t e = hipFuncSetAttribute((const void*)k_expert_place, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)plan_lds(WH_ROWS_MAX_GROUPS));
+    auto tile = [&](const void* f, size_t lds) {
+        if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    };
+    constexpr size_t lds = rows_tile_shape<4, 4, 2, 2>::kLds;
+    tile((const void*)k_rows_mm_tile<4, 4, 2, 2, true, true>, lds);
+    tile((const void*)k_rows_mm_tile<4, 4, 2, 2, true, false>, lds);
+    tile((const void*)k_rows_mm_tile<4, 4, 2, 2, false, true>, lds);
+    tile((const void*)k_rows_mm_tile<4, 4, 2, 2, false, false>, lds);
+    return e;
 }
 
 hipError_t wh_rows_quant_launch(const wh_rows_quant_args& a, bool bf16, hipStream_t stream) {
@@ -701,6 +948,20 @@ bool wh_rows_mm_fits(const wh_rows_mm_args& a) {
 
 hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, bool bf16, hipStream_t stream) {
     const bool mant = a.scale_f32 || a.odd_scale;
+    if (rows_mm_matrix(a) && a.n > 48 * a.n_groups) {
+        typedef rows_tile_shape<4, 4, 2, 2> S;
+        const uint64_t tiles = rows_tiles(a, S::kM) * ((a.out_rows + S::kN - 1) / S::kN);
+        const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);
+        auto go = [&](auto kern) { kern<<<grid, S::kThreads, S::kLds, stream>>>(a); };
+        if (bf16) {
+            if (mant) go(k_rows_mm_tile<4, 4, 2, 2, true, true>);
+            else go(k_rows_mm_tile<4, 4, 2, 2, true, false>);
+        } else {
+            if (mant) go(k_rows_mm_tile<4, 4, 2, 2, false, true>);
+            else go(k_rows_mm_tile<4, 4, 2, 2, false, false>);
+        }
+        return hipGetLastError();
+    }
     if (rows_mm_matrix(a)) {
         const uint32_t ks = rows_thin_split(a.cols), per = 16 * (kThinWaves / ks);
         const dim3 grid((a.out_rows + per - 1) / per, a.n_groups);
