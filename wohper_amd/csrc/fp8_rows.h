@@ -50,7 +50,7 @@ struct wh_rows_mm_args {
     uint32_t scale_f32;  // scales are f32, else UE8M0 bytes
     uint32_t special;    // weight codes 0x7F / 0xFF are there, +-480
     uint32_t odd_scale;  // UE8M0 scale bytes 0 or 255 are there
-    uint32_t y_vec;      // y takes stores of four values
+    uint32_t y_vec;      // y takes stores of four values (1), of 16 bytes (2)
 };
 // Whether a call's grid is within the limits of a launch.
 bool wh_rows_mm_fits(const wh_rows_mm_args& a);

@@ -552,32 +552,46 @@ struct rows_tile_shape {
     static constexpr uint32_t kWm0 = kWs + kScaleBlocks * kN / 16, kNan = kWm0 + kScaleBlocks * kN / 4, kLds = kNan + kM;
 };
 
-// Brings the scales of blocks [b0, b0 + kScaleBlocks) into LDS.
-template <class S>
+// Brings the scales of blocks [b0, b0 + kScaleBlocks) into LDS; a block behind the
+// last gets bytes 0, whose product of 2^-254 with any sum of codes is 0.  One row a
+// thread, its words all in flight.
+template <class S, bool kNanFlags>
 __device__ __forceinline__ void rows_tile_scales(const wh_rows_mm_args& a, uint8_t* lds, uint32_t b0, uint32_t r0, uint32_t r1,
-                                                 uint64_t w0, uint32_t c0) {
-    const uint32_t blocks = a.cols / 128u, count = min(kScaleBlocks, blocks - b0), words = (count + 3) / 4;
-    for (uint32_t i = threadIdx.x; i < S::kM * (kScaleBlocks / 4); i += S::kThreads) {
-        const uint32_t r = i / (kScaleBlocks / 4), k = i % (kScaleBlocks / 4);
-        if (k >= words || r0 + r >= r1) continue;
-        bool is;
-        const uint32_t src = rows_source(a, r0 + r, &is);
-        const uint32_t v = *(const uint32_t*)(a.x.scales + (uint64_t)src * a.x.scale_stride + b0 + 4 * k);
-        uint8_t* const to = lds + S::kXs + ((4 * k * (S::kM / 64) + r / 64) * 16 + r % 16) * 4 + r % 64 / 16;
+                                                 uint32_t w0, uint32_t c0) {
+    const uint32_t blocks = a.cols / 128u, count = min(kScaleBlocks, blocks - b0);
+    constexpr uint32_t kParts = S::kThreads / S::kM, kWords = kScaleBlocks / 4 / kParts;
+    const uint32_t r = threadIdx.x % S::kM, from = threadIdx.x / S::kM * kWords;
+    bool is;
+    const uint32_t src = rows_source(a, min(r0 + r, r1 - 1), &is);
+    const uint32_t* const xs = (const uint32_t*)(a.x.scales + (uint64_t)src * a.x.scale_stride + b0);
+    uint32_t v[kWords];
+#pragma unroll
+    for (uint32_t k = 0; k < kWords; ++k) v[k] = 4 * (from + k) < count ? xs[from + k] : 0;
+    constexpr uint32_t kTiles = S::kN / 16, kStep = S::kThreads / kTiles, kEach = kScaleBlocks / kStep;
+    const uint32_t t = threadIdx.x % kTiles, k0 = threadIdx.x / kTiles;
+    const uint32_t row = (w0 + min(c0 + 16 * t, a.out_rows - 1)) / a.row_block;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t k = k0 + i * kStep;
+        float m = 1.0f;
+        const uint32_t byte = k < count ? rows_split_scale(a, (uint64_t)row * blocks + b0 + k, &m) : 0;
+        lds[S::kWs + k * kTiles + t] = (uint8_t)byte;
+        if (a.scale_f32 || a.odd_scale) *(float*)(lds + S::kWm0 + 4 * (k * kTiles + t)) = m;
+    }
+    uint8_t* const to = lds + S::kXs + r / 64 * 64 + r % 16 * 4 + r % 64 / 16;
+    bool nan = false;
+#pragma unroll
+    for (uint32_t k = 0; k < kWords; ++k) {
+        const uint32_t b = 4 * (from + k);
+        if (b < count && count - b < 4) v[k] &= (1u << 8 * (count - b)) - 1;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-            to[j * S::kM] = (uint8_t)(v >> 8 * j);
-            if (4 * k + j < count && (v >> 8 * j & 0xff) == 255) lds[S::kNan + r] = 1;
+            const uint32_t byte = v[k] >> 8 * j & 0xff;
+            to[(b + j) * S::kM] = (uint8_t)byte;
+            if (kNanFlags) nan |= byte == 255;
         }
     }
-    for (uint32_t i = threadIdx.x; i < S::kN / 16 * kScaleBlocks; i += S::kThreads) {
-        const uint32_t k = i / (S::kN / 16), t = i % (S::kN / 16);
-        if (k >= count) continue;
-        const uint64_t row = w0 + min(c0 + 16 * t, a.out_rows - 1);
-        float m;
-        lds[S::kWs + k * (S::kN / 16) + t] = (uint8_t)rows_split_scale(a, row / a.row_block * blocks + b0 + k, &m);
-        *(float*)(lds + S::kWm0 + 4 * (k * (S::kN / 16) + t)) = m;
-    }
+    if (kNanFlags && nan) lds[S::kNan + r] = 1;
 }
 
 template <int kMt, int kNt, int kWm, int kWn, bool kBf16, bool kMant>
@@ -627,7 +641,7 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
     for (uint32_t b = 0; b < blocks; ++b) {
         if (b % kScaleBlocks == 0) {
             __syncthreads();
-            rows_tile_scales<S>(a, lds, b, r0, r1, w0, c0);
+            rows_tile_scales<S, !kBf16>(a, lds, b, r0, r1, (uint32_t)w0, c0);
         }
         rows_arrived();
         if (b + 1 < blocks) bring(b + 1);
@@ -699,6 +713,149 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
             if (!is) v = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
             const uint32_t col = c0 + (wn * kNt + i) * 16 + 4 * q;
             if (col < a.out_rows) rows_put4<kBf16>(a, j, col, v);
+        }
+    }
+}
+
+// Tiles of 256 x 256 for bf16 results, four waves of 128 x 128, where there are enough
+// of them.  A block's 64 products a wave go in quarters of four by four tiles, in the
+// order (w0 x0) (w0 x1) (w1 x1) (w1 x0), the next block's with x0 and x1 changed over:
+// so each half of the operands dies in time to take the next block's behind products
+// that do not need it, and 128 registers hold both blocks.  The middle of a block is
+// where every wave has read all of it: there the block after the next goes into its
+// buffer, a whole block ahead of its first use, behind the only barrier.
+__global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
+    typedef rows_tile_shape<8, 8, 2, 2> S;
+    extern __shared__ __align__(128) uint8_t tile_lds[];
+    uint8_t* const lds = tile_lds;
+    uint32_t g = 0, r0 = 0, r1 = 0, c0 = 0;
+    if (!rows_place<S::kM, S::kN>(a, g, r0, r1, c0)) return;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t l16 = lane & 15, q = lane >> 4, wm = wave & 1, wn = wave >> 1, blocks = a.cols / 128u;
+    const uint64_t w0 = a.row_start + (uint64_t)g * a.out_rows;
+    const uint8_t* xp[8];
+    uint32_t wo[8];
+    const uint32_t chunk = 16 * ((lane & 7) ^ (lane >> 3));
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        bool is;
+        const uint32_t src = rows_source(a, min(r0 + (wave + i * 4) * 8 + (lane >> 3), r1 - 1), &is);
+        xp[i] = a.x.codes + (uint64_t)src * a.x.stride + chunk;
+        wo[i] = min((wave + i * 4) * 8 + (lane >> 3), a.out_rows - 1 - c0) * a.cols + chunk;
+    }
+    const uint8_t* const wp = a.w + (w0 + c0) * a.cols;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rows_lds(lds)) + wave * 1024;
+    wh_f4 acc[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) acc[i][t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t at = l16 * 128 + ((q ^ (l16 & 7)) << 4);
+    const uint32_t xt = wm * 16384 + at, wt = 32768 + wn * 16384 + at;
+    // load i of 16 of block b into a buffer
+    auto bring = [&](uint32_t b, uint32_t buffer, uint32_t i) {
+        const uint32_t to = lds0 + buffer + i * 4096;
+        if (i < 8) rows_dma(xp[i] + b * 128u, to);
+        else rows_dma(wp + b * 128u, wo[i - 8], to);
+    };
+    auto frag = [&](uint32_t off) {
+        rows_frag f;
+        f.a = *(const wh_u4*)(lds + off);
+        f.b = *(const wh_u4*)(lds + (off ^ 64));
+        return rows_codes(f);
+    };
+    wh_i8 x[8], w[8];
+    uint32_t xb[2], wb[2];  // scale bytes of the halves
+    auto scales = [&](uint32_t k) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            wb[h] = *(const uint32_t*)(lds + S::kWs + k * 16 + wn * 8 + 4 * h);
+            xb[h] = *(const uint32_t*)(lds + S::kXs + ((k * 4 + wm * 2 + h) * 16 + l16) * 4);
+        }
+    };
+    // a quarter's 16 products, f(n) behind the n-th
+    auto quarter = [&](auto wv, auto xv, auto&& f) {
+        constexpr int kW = decltype(wv)::value, kX = decltype(xv)::value;
+        wh_static_for<16>([&](auto nv) {
+            constexpr int n = decltype(nv)::value, i = 4 * kW + n / 4, t = 4 * kX + n % 4;
+            acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[t], acc[i][t], 0, 0, n / 4, (int)wb[kW], n % 4,
+                                                                         (int)xb[kX]);
+            f(nv);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    using std::integral_constant;
+    constexpr integral_constant<int, 0> first;
+    constexpr integral_constant<int, 1> last;
+    wh_static_for<16>([&](auto iv) { bring(0, 0, decltype(iv)::value); });
+    wh_static_for<16>([&](auto iv) { bring(min(1u, blocks - 1), S::kStage, decltype(iv)::value); });
+    rows_arrived();
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[t] = frag(xt + t * 2048);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = frag(wt + i * 2048);
+    // block b of buffer kBuffer, first with x half kBuffer.  There is always a next block
+    // and one after it: behind the last they are the last again, and not used, or
+    // (blocks go in pairs) multiplied by scales of 0.
+    auto step = [&](auto bv, uint32_t b, uint32_t k) {
+        constexpr int kX = decltype(bv)::value;
+        constexpr integral_constant<int, 1 - kX> other;
+        constexpr uint32_t here = kX * S::kStage, next = S::kStage - here;
+        const uint32_t after = min(b + 2, blocks - 1);
+        scales(k);
+        quarter(first, bv, [&](auto nv) {
+            constexpr int n = decltype(nv)::value;
+            if constexpr (n < 4) x[4 * (1 - kX) + n] = frag(here + xt + (4 * (1 - kX) + n) * 2048);
+            else if constexpr (n < 8) w[n] = frag(here + wt + n * 2048);
+        });
+        quarter(first, other, [&](auto) {});
+        rows_arrived();
+        quarter(last, other, [&](auto nv) {
+            constexpr int n = decltype(nv)::value;
+            bring(after, here, n);
+            if constexpr (n < 4) w[n] = frag(next + wt + n * 2048);
+        });
+        quarter(last, bv, [&](auto nv) {
+            constexpr int n = decltype(nv)::value;
+            if constexpr (n < 4) x[4 * (1 - kX) + n] = frag(next + xt + (4 * (1 - kX) + n) * 2048);
+        });
+    };
+    for (uint32_t b0 = 0; b0 < blocks; b0 += kScaleBlocks) {
+        rows_tile_scales<S, false>(a, lds, b0, r0, r1, (uint32_t)w0, c0);
+        __syncthreads();
+        const uint32_t count = min(kScaleBlocks, blocks - b0);
+        for (uint32_t k = 0; k < count; k += 2) {
+            step(first, b0 + k, k);
+            step(last, b0 + k + 1, k + 1);
+        }
+    }
+    rows_arrived();  // also the loads behind the last block
+    // through LDS, so that rows go out in whole lines and by a short loop
+    constexpr uint32_t kPitch = 2 * S::kN + 16;
+    static_assert(kPitch * S::kM <= S::kLds, "a tile of results");
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+            const wh_f4 v = acc[i][t];
+            *(b4*)(lds + (wm * 128 + 16 * t + l16) * kPitch + ((wn * 8 + i) * 16 + 4 * q) * 2) =
+                b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        }
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t u = threadIdx.x; u < S::kM * S::kN / 8; u += S::kThreads) {
+        const uint32_t r = u / (S::kN / 8), col = c0 + u % (S::kN / 8) * 8, j = r0 + r;
+        if (j >= r1 || col >= a.out_rows) continue;
+        wh_u4 v = *(const wh_u4*)(lds + r * kPitch + (col - c0) * 2);
+        bool is = true;
+        if (a.rows) rows_source(a, j, &is);
+        if (!is) v = wh_u4{0, 0, 0, 0};
+        uint16_t* const to = (uint16_t*)a.y + (uint64_t)j * a.y_stride + col;
+        if (a.y_vec == 2 && col + 8 <= a.out_rows) {
+            *(wh_u4*)to = v;
+        } else {
+            for (uint32_t e = 0; e < 8 && col + e < a.out_rows; ++e) to[e] = (uint16_t)(v[e / 2] >> 16 * (e & 1));
         }
     }
 }
@@ -918,6 +1075,7 @@ hipError_t wh_rows_setup() {
     tile((const void*)k_rows_mm_tile<4, 4, 2, 2, true, false>, lds);
     tile((const void*)k_rows_mm_tile<4, 4, 2, 2, false, true>, lds);
     tile((const void*)k_rows_mm_tile<4, 4, 2, 2, false, false>, lds);
+    tile((const void*)k_rows_mm_big, rows_tile_shape<8, 8, 2, 2>::kLds);
     return e;
 }
 
@@ -948,6 +1106,13 @@ bool wh_rows_mm_fits(const wh_rows_mm_args& a) {
 
 hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, bool bf16, hipStream_t stream) {
     const bool mant = a.scale_f32 || a.odd_scale;
+    if (rows_mm_matrix(a) && bf16 && !mant && a.n >= 256 * a.n_groups) {
+        typedef rows_tile_shape<8, 8, 2, 2> S;
+        const uint64_t tiles = rows_tiles(a, S::kM) * ((a.out_rows + S::kN - 1) / S::kN);
+        const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);
+        k_rows_mm_big<<<grid, S::kThreads, S::kLds, stream>>>(a);
+        return hipGetLastError();
+    }
     if (rows_mm_matrix(a) && a.n > 48 * a.n_groups) {
         typedef rows_tile_shape<4, 4, 2, 2> S;
         const uint64_t tiles = rows_tiles(a, S::kM) * ((a.out_rows + S::kN - 1) / S::kN);
