@@ -483,6 +483,12 @@ __device__ __forceinline__ void rows_arrived() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// The same for all but the last kLeft of this wave's loads.
+template <int kLeft>
+__device__ __forceinline__ void rows_arrived_but() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+}
+
 // A workgroup's tile: listed rows [r0, r1) of group g and columns from c0 on.  Tiles
 // are numbered group by group, in bands of kBand tiles of rows, columns outside rows,
 // and every XCD (workgroup id mod 8) takes a run of consecutive ones, so that those
@@ -721,9 +727,10 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
 // of them.  A block's 64 products a wave go in quarters of four by four tiles, in the
 // order (w0 x0) (w0 x1) (w1 x1) (w1 x0), the next block's with x0 and x1 changed over:
 // so each half of the operands dies in time to take the next block's behind products
-// that do not need it, and 128 registers hold both blocks.  The middle of a block is
-// where every wave has read all of it: there the block after the next goes into its
-// buffer, a whole block ahead of its first use, behind the only barrier.
+// that do not need it, and 128 registers hold both blocks.  In LDS the halves of a block
+// are free, and filled with the block after the next, as soon as every wave has read
+// them: the first ones a block before the end, the others half a block later, so loads
+// run a whole block ahead and come evenly.
 __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
     typedef rows_tile_shape<8, 8, 2, 2> S;
     extern __shared__ __align__(128) uint8_t tile_lds[];
@@ -733,18 +740,25 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t l16 = lane & 15, q = lane >> 4, wm = wave & 1, wn = wave >> 1, blocks = a.cols / 128u;
     const uint64_t w0 = a.row_start + (uint64_t)g * a.out_rows;
+    // this wave's loads: eight rows each, a lane one chunk; half h of a side is 64 of each
+    // wave's 128 rows
+    auto at_row = [&](uint32_t h, uint32_t j) {
+        const uint32_t e = wave + 4 * j;
+        return 8 * (e % 8) + 128 * (e / 8) + 64 * h;
+    };
     const uint8_t* xp[8];
     uint32_t wo[8];
     const uint32_t chunk = 16 * ((lane & 7) ^ (lane >> 3));
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t row = at_row(i / 4, i % 4) + (lane >> 3);
         bool is;
-        const uint32_t src = rows_source(a, min(r0 + (wave + i * 4) * 8 + (lane >> 3), r1 - 1), &is);
+        const uint32_t src = rows_source(a, min(r0 + row, r1 - 1), &is);
         xp[i] = a.x.codes + (uint64_t)src * a.x.stride + chunk;
-        wo[i] = min((wave + i * 4) * 8 + (lane >> 3), a.out_rows - 1 - c0) * a.cols + chunk;
+        wo[i] = min(row, a.out_rows - 1 - c0) * a.cols + chunk;
     }
     const uint8_t* const wp = a.w + (w0 + c0) * a.cols;
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rows_lds(lds)) + wave * 1024;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rows_lds(lds));
     wh_f4 acc[8][8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -752,11 +766,10 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
         for (int t = 0; t < 8; ++t) acc[i][t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
     const uint32_t at = l16 * 128 + ((q ^ (l16 & 7)) << 4);
     const uint32_t xt = wm * 16384 + at, wt = 32768 + wn * 16384 + at;
-    // load i of 16 of block b into a buffer
-    auto bring = [&](uint32_t b, uint32_t buffer, uint32_t i) {
-        const uint32_t to = lds0 + buffer + i * 4096;
-        if (i < 8) rows_dma(xp[i] + b * 128u, to);
-        else rows_dma(wp + b * 128u, wo[i - 8], to);
+    // load j of 8 of x half kH and weight half kW of block b into a buffer
+    auto bring = [&](uint32_t b, uint32_t buffer, uint32_t xh, uint32_t wh, uint32_t j) {
+        if (j < 4) rows_dma(xp[4 * xh + j] + b * 128u, lds0 + buffer + at_row(xh, j) * 128);
+        else rows_dma(wp + b * 128u, wo[4 * wh + j - 4], lds0 + buffer + 32768 + at_row(wh, j - 4) * 128);
     };
     auto frag = [&](uint32_t off) {
         rows_frag f;
@@ -764,22 +777,29 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
         f.b = *(const wh_u4*)(lds + (off ^ 64));
         return rows_codes(f);
     };
+    // half h of it
+    auto half = [&](wh_i8& to, uint32_t off, int h) {
+        const wh_u4 v = *(const wh_u4*)(lds + (off ^ 64 * h));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[4 * h + j] = (int)v[j];
+    };
     wh_i8 x[8], w[8];
-    uint32_t xb[2], wb[2];  // scale bytes of the halves
-    auto scales = [&](uint32_t k) {
+    uint32_t xb[2][2], wb[2][2];  // scale bytes of the halves, of even and odd blocks
+    auto scales = [&](auto bv, uint32_t k) {
+        constexpr int kB = decltype(bv)::value;
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
-            wb[h] = *(const uint32_t*)(lds + S::kWs + k * 16 + wn * 8 + 4 * h);
-            xb[h] = *(const uint32_t*)(lds + S::kXs + ((k * 4 + wm * 2 + h) * 16 + l16) * 4);
+            wb[kB][h] = *(const uint32_t*)(lds + S::kWs + k * 16 + wn * 8 + 4 * h);
+            xb[kB][h] = *(const uint32_t*)(lds + S::kXs + ((k * 4 + wm * 2 + h) * 16 + l16) * 4);
         }
     };
     // a quarter's 16 products, f(n) behind the n-th
-    auto quarter = [&](auto wv, auto xv, auto&& f) {
-        constexpr int kW = decltype(wv)::value, kX = decltype(xv)::value;
+    auto quarter = [&](auto bv, auto wv, auto xv, auto&& f) {
+        constexpr int kB = decltype(bv)::value, kW = decltype(wv)::value, kX = decltype(xv)::value;
         wh_static_for<16>([&](auto nv) {
             constexpr int n = decltype(nv)::value, i = 4 * kW + n / 4, t = 4 * kX + n % 4;
-            acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[t], acc[i][t], 0, 0, n / 4, (int)wb[kW], n % 4,
-                                                                         (int)xb[kX]);
+            acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[t], acc[i][t], 0, 0, n / 4, (int)wb[kB][kW], n % 4,
+                                                                         (int)xb[kB][kX]);
             f(nv);
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -787,42 +807,54 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
     using std::integral_constant;
     constexpr integral_constant<int, 0> first;
     constexpr integral_constant<int, 1> last;
-    wh_static_for<16>([&](auto iv) { bring(0, 0, decltype(iv)::value); });
-    wh_static_for<16>([&](auto iv) { bring(min(1u, blocks - 1), S::kStage, decltype(iv)::value); });
-    rows_arrived();
-#pragma unroll
-    for (int t = 0; t < 4; ++t) x[t] = frag(xt + t * 2048);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = frag(wt + i * 2048);
-    // block b of buffer kBuffer, first with x half kBuffer.  There is always a next block
-    // and one after it: behind the last they are the last again, and not used, or
-    // (blocks go in pairs) multiplied by scales of 0.
+    wh_static_for<2>([&](auto bv) {
+        constexpr int kB = decltype(bv)::value;
+        wh_static_for<8>([&](auto iv) { bring(min((uint32_t)kB, blocks - 1), kB * S::kStage, kB, 0, decltype(iv)::value); });
+        wh_static_for<8>([&](auto iv) { bring(min((uint32_t)kB, blocks - 1), kB * S::kStage, 1 - kB, 1, decltype(iv)::value); });
+    });
+    // block b of buffer kB, first with x half kB.  There is always a next block and one
+    // after it: behind the last they are the last again, and not used, or (blocks go in
+    // pairs) multiplied by scales of 0.  Loads and 16-byte LDS reads are spread over the
+    // products: a CU takes one load of 64 lanes in 16 cycles, one read in 8.
     auto step = [&](auto bv, uint32_t b, uint32_t k) {
-        constexpr int kX = decltype(bv)::value;
-        constexpr integral_constant<int, 1 - kX> other;
-        constexpr uint32_t here = kX * S::kStage, next = S::kStage - here;
+        constexpr int kB = decltype(bv)::value;
+        constexpr integral_constant<int, 1 - kB> other;
+        constexpr uint32_t here = kB * S::kStage, next = S::kStage - here;
         const uint32_t after = min(b + 2, blocks - 1);
-        scales(k);
-        quarter(first, bv, [&](auto nv) {
-            constexpr int n = decltype(nv)::value;
-            if constexpr (n < 4) x[4 * (1 - kX) + n] = frag(here + xt + (4 * (1 - kX) + n) * 2048);
-            else if constexpr (n < 8) w[n] = frag(here + wt + n * 2048);
+        rows_arrived_but<16>();  // every wave has b's first halves in registers, its second halves are there
+        quarter(bv, first, bv, [&](auto nv) {
+            constexpr int n = decltype(nv)::value, t = 4 * (1 - kB) + n / 2;
+            if constexpr (n % 4 == 3) bring(after, here, kB, 0, n / 4);
+            if constexpr (n < 8) half(x[t], here + xt + t % 8 * 2048, n % 2);
+            else if constexpr (n % 2 == 0) half(w[n / 4 + 2], here + wt + (n / 4 + 2) * 2048, n / 2 % 2);
         });
-        quarter(first, other, [&](auto) {});
-        rows_arrived();
-        quarter(last, other, [&](auto nv) {
+        quarter(bv, first, other, [&](auto nv) {
             constexpr int n = decltype(nv)::value;
-            bring(after, here, n);
-            if constexpr (n < 4) w[n] = frag(next + wt + n * 2048);
+            if constexpr (n % 4 == 3) bring(after, here, kB, 0, 4 + n / 4);
+            if constexpr (n < 8 && n % 2 == 0) half(w[n / 4 + 6], here + wt + (n / 4 + 6) * 2048, n / 2 % 2);
         });
-        quarter(last, bv, [&](auto nv) {
+        rows_arrived_but<16>();  // every wave has all of b in registers, b + 1's first halves are there
+        quarter(bv, last, other, [&](auto nv) {
             constexpr int n = decltype(nv)::value;
-            if constexpr (n < 4) x[4 * (1 - kX) + n] = frag(next + xt + (4 * (1 - kX) + n) * 2048);
+            if constexpr (n % 4 == 3) bring(after, here, 1 - kB, 1, n / 4);
+            if constexpr (n % 2 == 0) half(w[n / 4], next + wt + n / 4 * 2048, n / 2 % 2);
+        });
+        quarter(bv, last, bv, [&](auto nv) {
+            constexpr int n = decltype(nv)::value, t = 4 * (1 - kB) + n / 2;
+            if constexpr (n % 4 == 3) bring(after, here, 1 - kB, 1, 4 + n / 4);
+            if constexpr (n < 8) half(x[t], next + xt + t % 8 * 2048, n % 2);
+            if constexpr (n == 8) scales(other, (k + 1) % kScaleBlocks);  // behind a chunk's last: read again
         });
     };
     for (uint32_t b0 = 0; b0 < blocks; b0 += kScaleBlocks) {
         rows_tile_scales<S, false>(a, lds, b0, r0, r1, (uint32_t)w0, c0);
-        __syncthreads();
+        rows_arrived_but<16>();
+        // the first block's (a later chunk's are there already)
+        scales(first, 0);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = frag(xt + t * 2048);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = frag(wt + i * 2048);
         const uint32_t count = min(kScaleBlocks, blocks - b0);
         for (uint32_t k = 0; k < count; k += 2) {
             step(first, b0 + k, k);
