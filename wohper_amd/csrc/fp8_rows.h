@@ -7,6 +7,8 @@
 #define WH_ROWS_NONE 0xFFFFFFFFu     // a route to no expert, a slot of no row
 #define WH_ROWS_MAX_GROUPS 1024u     // experts of a grouped product or a plan
 
+#define WH_ROWS_TICKETS 16u          // counters that a context's products share
+
 // 8-bit rows in device memory (wh_fp8_rows).
 struct wh_rows8 {
     uint8_t* codes;
@@ -50,10 +52,11 @@ struct wh_rows_mm_args {
     uint32_t scale_f32;  // scales are f32, else UE8M0 bytes
     uint32_t special;    // weight codes 0x7F / 0xFF are there, +-480
     uint32_t odd_scale;  // UE8M0 scale bytes 0 or 255 are there
+    uint32_t* tickets;   // [WH_ROWS_TICKETS], 0 between launches
     uint32_t y_vec;      // y takes stores of four values (1), of 16 bytes (2)
 };
 // Whether a call's grid is within the limits of a launch.
-bool wh_rows_mm_fits(const wh_rows_mm_args& a);
+bool wh_rows_mm_fits(const wh_rows_mm_args& a, bool bf16);
 hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, bool bf16, hipStream_t stream);
 hipError_t wh_rows_setup();  // once for each device, before the first launch there
 

@@ -489,61 +489,69 @@ __device__ __forceinline__ void rows_arrived_but() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
 
-// A workgroup's tile: listed rows [r0, r1) of group g and columns from c0 on.  Tiles
-// are numbered group by group, in bands of kBand tiles of rows, columns outside rows,
-// and every XCD (workgroup id mod 8) takes a run of consecutive ones, so that those
-// in flight on one L2 share rows and weights.  False behind the last tile.
+// Tiles of at most kM listed rows [r0, r1) of one group g and kN columns from c0 on.
+// They are numbered group by group, in bands of kBand tiles of rows, columns outside
+// rows, and every XCD (workgroup id mod 8) takes a run of consecutive ones, so that those
+// in flight on one L2 share rows and weights.
 constexpr uint32_t kBand = 8;
 template <uint32_t kM, uint32_t kN>
-__device__ __forceinline__ bool rows_place(const wh_rows_mm_args& a, uint32_t& g, uint32_t& r0, uint32_t& r1, uint32_t& c0) {
-    const uint32_t n_tiles = (a.out_rows + kN - 1) / kN, lane = threadIdx.x & 63;
-    auto group = [&](uint32_t at, uint32_t& s, uint32_t& e) {
+struct rows_tiling {
+    const wh_rows_mm_args& a;
+    uint32_t n_tiles;    // of columns
+    uint64_t total, per;  // tiles, and of them an XCD's
+
+    // Tiles of rows of the group at, and its rows.  64 bits over groups: starts that do
+    // not ascend may count rows more than once.
+    __device__ __forceinline__ uint32_t group(uint32_t at, uint32_t& s, uint32_t& e) const {
         s = e = 0;
         if (at < a.n_groups) {
             s = a.starts ? min(a.starts[at], a.n) : 0;
             e = a.starts ? max(s, min(a.starts[at + 1], a.n)) : a.n;
         }
         return (e - s + kM - 1) / kM;
-    };
-    // 64 bits: starts that do not ascend may count rows more than once
-    uint32_t s, e;
-    uint64_t total = 0;
-    for (uint32_t base = 0; base < a.n_groups; base += 64) {
-        uint32_t sum = group(base + lane, s, e);
-        for (uint32_t off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-        total += (uint32_t)__builtin_amdgcn_readfirstlane(sum);
     }
-    total *= n_tiles;
-    const uint64_t per = (total + 7) / 8;
-    const uint32_t slot = blockIdx.x / 8;
-    uint64_t t = (blockIdx.x & 7) * per + slot;
-    if (slot >= per || t >= total) return false;
-    for (uint32_t base = 0; base < a.n_groups; base += 64) {
-        const uint32_t tiles = group(base + lane, s, e);
-        uint32_t upto = tiles;
+    __device__ __forceinline__ explicit rows_tiling(const wh_rows_mm_args& args) : a(args), n_tiles((args.out_rows + kN - 1) / kN), total(0) {
+        for (uint32_t base = 0; base < a.n_groups; base += 64) {
+            uint32_t s, e, sum = group(base + (threadIdx.x & 63), s, e);
+            for (uint32_t off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+            total += (uint32_t)__builtin_amdgcn_readfirstlane(sum);
+        }
+        total *= n_tiles;
+        per = (total + 7) / 8;
+    }
+    __device__ __forceinline__ uint64_t count(uint32_t xcd) const { return xcd * per >= total ? 0 : min(per, total - xcd * per); }
+    // The t-th tile of an XCD, t < count.
+    __device__ __forceinline__ void at(uint32_t xcd, uint64_t t, uint32_t& g, uint32_t& r0, uint32_t& r1, uint32_t& c0) const {
+        const uint32_t lane = threadIdx.x & 63;
+        t += xcd * per;
+        g = r0 = r1 = c0 = 0;
+        for (uint32_t base = 0; base < a.n_groups; base += 64) {
+            uint32_t s, e;
+            const uint32_t tiles = group(base + lane, s, e);
+            uint32_t upto = tiles;
 #pragma unroll
-        for (uint32_t off = 1; off < 64; off <<= 1) {
-            const uint32_t y = __shfl_up(upto, off, 64);
-            if (lane >= off) upto += y;
+            for (uint32_t off = 1; off < 64; off <<= 1) {
+                const uint32_t y = __shfl_up(upto, off, 64);
+                if (lane >= off) upto += y;
+            }
+            const uint64_t past = __ballot((uint64_t)upto * n_tiles > t);
+            if (past) {
+                const uint32_t lead = (uint32_t)__builtin_ctzll(past);
+                const uint32_t mine = __builtin_amdgcn_readlane((int)tiles, lead);
+                const uint64_t own = t - (uint64_t)((uint32_t)__builtin_amdgcn_readlane((int)upto, lead) - mine) * n_tiles;
+                g = base + lead;
+                const uint32_t band = (uint32_t)(own / (kBand * n_tiles)), in = (uint32_t)(own % (kBand * n_tiles));
+                const uint32_t high = min(kBand, mine - band * kBand);
+                const uint32_t end = __builtin_amdgcn_readlane((int)e, lead);
+                r0 = __builtin_amdgcn_readlane((int)s, lead) + (band * kBand + in % high) * kM;
+                r1 = min(end, r0 + kM);
+                c0 = __builtin_amdgcn_readfirstlane(in / high * kN);
+                return;
+            }
+            t -= (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * n_tiles;
         }
-        const uint64_t past = __ballot((uint64_t)upto * n_tiles > t);
-        if (past) {
-            const uint32_t first = (uint32_t)__builtin_ctzll(past);
-            const uint32_t mine = __builtin_amdgcn_readlane((int)tiles, first);
-            const uint64_t own = t - (uint64_t)((uint32_t)__builtin_amdgcn_readlane((int)upto, first) - mine) * n_tiles;
-            g = base + first;
-            const uint32_t band = (uint32_t)(own / (kBand * n_tiles)), in = (uint32_t)(own % (kBand * n_tiles));
-            const uint32_t high = min(kBand, mine - band * kBand);
-            const uint32_t end = __builtin_amdgcn_readlane((int)e, first);
-            r0 = __builtin_amdgcn_readlane((int)s, first) + (band * kBand + in % high) * kM;
-            r1 = min(end, r0 + kM);
-            c0 = in / high * kN;
-            return true;
-        }
-        t -= (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * n_tiles;
     }
-    return false;
-}
+};
 
 // Many rows a group: tiles of kM x kN outputs in LDS.  Both sides' blocks of 128 bytes
 // go straight from memory into LDS, one step ahead, 16-byte chunk c of row r at place
@@ -560,15 +568,15 @@ struct rows_tile_shape {
 
 // Brings the scales of blocks [b0, b0 + kScaleBlocks) into LDS; a block behind the
 // last gets bytes 0, whose product of 2^-254 with any sum of codes is 0.  One row a
-// thread, its words all in flight.
-template <class S, bool kNanFlags>
+// thread, its words all in flight.  kHalf: place r is row r / 128 * 64 + r % 64.
+template <class S, bool kNanFlags, bool kHalf = false>
 __device__ __forceinline__ void rows_tile_scales(const wh_rows_mm_args& a, uint8_t* lds, uint32_t b0, uint32_t r0, uint32_t r1,
                                                  uint32_t w0, uint32_t c0) {
     const uint32_t blocks = a.cols / 128u, count = min(kScaleBlocks, blocks - b0);
     constexpr uint32_t kParts = S::kThreads / S::kM, kWords = kScaleBlocks / 4 / kParts;
     const uint32_t r = threadIdx.x % S::kM, from = threadIdx.x / S::kM * kWords;
     bool is;
-    const uint32_t src = rows_source(a, min(r0 + r, r1 - 1), &is);
+    const uint32_t src = rows_source(a, min(r0 + (kHalf ? r / 128 * 64 + r % 64 : r), r1 - 1), &is);
     const uint32_t* const xs = (const uint32_t*)(a.x.scales + (uint64_t)src * a.x.scale_stride + b0);
     uint32_t v[kWords];
 #pragma unroll
@@ -607,7 +615,9 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
     extern __shared__ __align__(128) uint8_t tile_lds[];
     uint8_t* const lds = tile_lds;
     uint32_t g = 0, r0 = 0, r1 = 0, c0 = 0;
-    if (!rows_place<S::kM, S::kN>(a, g, r0, r1, c0)) return;
+    const rows_tiling<S::kM, S::kN> tiles(a);
+    if (blockIdx.x / 8 >= tiles.count(blockIdx.x & 7)) return;
+    tiles.at(blockIdx.x & 7, blockIdx.x / 8, g, r0, r1, c0);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t l16 = lane & 15, q = lane >> 4, wm = wave % kWm, wn = wave / kWm, blocks = a.cols / 128u;
     const uint64_t w0 = a.row_start + (uint64_t)g * a.out_rows;
@@ -731,53 +741,50 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
 // are free, and filled with the block after the next, as soon as every wave has read
 // them: the first ones a block before the end, the others half a block later, so loads
 // run a whole block ahead and come evenly.
-__global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
+// kHalf: a tile of 128 rows, 64 a wave: x0 alone, in two sets of registers.
+template <bool kHalf, bool kMant>
+__device__ __forceinline__ void rows_big(const wh_rows_mm_args& a, uint8_t* lds, uint32_t g, uint32_t r0, uint32_t r1, uint32_t c0) {
+    static_assert(kHalf || !kMant, "factors take results through vector registers: 64 rows a wave at most");
     typedef rows_tile_shape<8, 8, 2, 2> S;
-    extern __shared__ __align__(128) uint8_t tile_lds[];
-    uint8_t* const lds = tile_lds;
-    uint32_t g = 0, r0 = 0, r1 = 0, c0 = 0;
-    if (!rows_place<S::kM, S::kN>(a, g, r0, r1, c0)) return;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t l16 = lane & 15, q = lane >> 4, wm = wave & 1, wn = wave >> 1, blocks = a.cols / 128u;
     const uint64_t w0 = a.row_start + (uint64_t)g * a.out_rows;
+    constexpr int kXt = kHalf ? 4 : 8;                   // tiles of 16 rows a wave
+    constexpr uint32_t kLoads = kHalf ? 12 : 16;         // of a wave for a block
     // this wave's loads: eight rows each, a lane one chunk; half h of a side is 64 of each
-    // wave's 128 rows
-    auto at_row = [&](uint32_t h, uint32_t j) {
+    // wave's 128 places
+    auto place = [&](uint32_t h, uint32_t j) {
         const uint32_t e = wave + 4 * j;
         return 8 * (e % 8) + 128 * (e / 8) + 64 * h;
     };
-    const uint8_t* xp[8];
+    const uint8_t* xp[kXt];
     uint32_t wo[8];
     const uint32_t chunk = 16 * ((lane & 7) ^ (lane >> 3));
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
-        const uint32_t row = at_row(i / 4, i % 4) + (lane >> 3);
-        bool is;
-        const uint32_t src = rows_source(a, min(r0 + row, r1 - 1), &is);
-        xp[i] = a.x.codes + (uint64_t)src * a.x.stride + chunk;
-        wo[i] = min(row, a.out_rows - 1 - c0) * a.cols + chunk;
+        const uint32_t at = place(i / 4, i % 4), row = (kHalf ? at / 128 * 64 + at % 64 : at) + (lane >> 3);
+        if (i < kXt) {
+            bool is;
+            const uint32_t src = rows_source(a, min(r0 + row, r1 - 1), &is);
+            xp[i] = a.x.codes + (uint64_t)src * a.x.stride + chunk;
+        }
+        wo[i] = min(at + (lane >> 3), a.out_rows - 1 - c0) * a.cols + chunk;
     }
     const uint8_t* const wp = a.w + (w0 + c0) * a.cols;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rows_lds(lds));
-    wh_f4 acc[8][8];
+    wh_f4 acc[8][kXt];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int t = 0; t < 8; ++t) acc[i][t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < kXt; ++t) acc[i][t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
     const uint32_t at = l16 * 128 + ((q ^ (l16 & 7)) << 4);
     const uint32_t xt = wm * 16384 + at, wt = 32768 + wn * 16384 + at;
-    // load j of 8 of x half kH and weight half kW of block b into a buffer
+    // load j of 8 of x half xh and weight half wh of block b into a buffer
     auto bring = [&](uint32_t b, uint32_t buffer, uint32_t xh, uint32_t wh, uint32_t j) {
-        if (j < 4) rows_dma(xp[4 * xh + j] + b * 128u, lds0 + buffer + at_row(xh, j) * 128);
-        else rows_dma(wp + b * 128u, wo[4 * wh + j - 4], lds0 + buffer + 32768 + at_row(wh, j - 4) * 128);
+        if (j < 4) rows_dma(xp[4 * xh + j] + b * 128u, lds0 + buffer + place(xh, j) * 128);
+        else rows_dma(wp + b * 128u, wo[4 * wh + j - 4], lds0 + buffer + 32768 + place(wh, j - 4) * 128);
     };
-    auto frag = [&](uint32_t off) {
-        rows_frag f;
-        f.a = *(const wh_u4*)(lds + off);
-        f.b = *(const wh_u4*)(lds + (off ^ 64));
-        return rows_codes(f);
-    };
-    // half h of it
+    // half h of an operand of 16 rows
     auto half = [&](wh_i8& to, uint32_t off, int h) {
         const wh_u4 v = *(const wh_u4*)(lds + (off ^ 64 * h));
 #pragma unroll
@@ -785,22 +792,36 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
     };
     wh_i8 x[8], w[8];
     uint32_t xb[2][2], wb[2][2];  // scale bytes of the halves, of even and odd blocks
+    wh_f4 m[2][2] = {};           // factors of the weights' scales
     auto scales = [&](auto bv, uint32_t k) {
         constexpr int kB = decltype(bv)::value;
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
             wb[kB][h] = *(const uint32_t*)(lds + S::kWs + k * 16 + wn * 8 + 4 * h);
-            xb[kB][h] = *(const uint32_t*)(lds + S::kXs + ((k * 4 + wm * 2 + h) * 16 + l16) * 4);
+            xb[kB][h] = kHalf && h ? 0 : *(const uint32_t*)(lds + S::kXs + ((k * 4 + wm * 2 + h) * 16 + l16) * 4);
+            if constexpr (kMant) m[kB][h] = *(const wh_f4*)(lds + S::kWm0 + (k * 16 + wn * 8 + 4 * h) * 4);
         }
     };
-    // a quarter's 16 products, f(n) behind the n-th
+    // the 16 products of weight half kW and x half kX (kHalf: set kX), f(n) behind the n-th
     auto quarter = [&](auto bv, auto wv, auto xv, auto&& f) {
         constexpr int kB = decltype(bv)::value, kW = decltype(wv)::value, kX = decltype(xv)::value;
-        wh_static_for<16>([&](auto nv) {
-            constexpr int n = decltype(nv)::value, i = 4 * kW + n / 4, t = 4 * kX + n % 4;
-            acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[t], acc[i][t], 0, 0, n / 4, (int)wb[kB][kW], n % 4,
-                                                                         (int)xb[kB][kX]);
-            f(nv);
+        wh_f4 s[16];
+        wh_static_for<18>([&](auto nv) {
+            constexpr int n = decltype(nv)::value;
+            if constexpr (n < 16) {
+                constexpr int i = 4 * kW + n / 4, t = n % 4, at_t = kHalf ? t : 4 * kX + t;
+                const wh_f4 from = kMant ? wh_f4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][at_t];
+                s[n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[4 * kX + t], from, 0, 0, n / 4, (int)wb[kB][kW], t,
+                                                                        (int)xb[kB][kHalf ? 0 : kX]);
+                if constexpr (!kMant) acc[i][at_t] = s[n];
+                f(nv);
+            }
+            if constexpr (kMant && n >= 2) {  // two products behind, whose result is there
+                constexpr int p = n - 2;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[4 * kW + p / 4][p % 4][j] = fmaf(s[p][j], m[kB][kW][p / 4], acc[4 * kW + p / 4][p % 4][j]);
+            }
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -809,19 +830,39 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
     constexpr integral_constant<int, 1> last;
     wh_static_for<2>([&](auto bv) {
         constexpr int kB = decltype(bv)::value;
-        wh_static_for<8>([&](auto iv) { bring(min((uint32_t)kB, blocks - 1), kB * S::kStage, kB, 0, decltype(iv)::value); });
-        wh_static_for<8>([&](auto iv) { bring(min((uint32_t)kB, blocks - 1), kB * S::kStage, 1 - kB, 1, decltype(iv)::value); });
+        const uint32_t b = min((uint32_t)kB, blocks - 1);
+        wh_static_for<8>([&](auto iv) { bring(b, kB * S::kStage, kHalf ? 0 : kB, 0, decltype(iv)::value); });
+        wh_static_for<8>([&](auto iv) {
+            constexpr int j = decltype(iv)::value;
+            if constexpr (!kHalf || j >= 4) bring(b, kB * S::kStage, 1 - kB, 1, j);
+        });
     });
-    // block b of buffer kB, first with x half kB.  There is always a next block and one
-    // after it: behind the last they are the last again, and not used, or (blocks go in
-    // pairs) multiplied by scales of 0.  Loads and 16-byte LDS reads are spread over the
-    // products: a CU takes one load of 64 lanes in 16 cycles, one read in 8.
+    // block b of buffer kB, first with x half kB (kHalf: in x set kB).  There is always a
+    // next block and one after it: behind the last they are the last again, and not used,
+    // or (blocks go in pairs) multiplied by scales of 0.  Loads and 16-byte LDS reads are
+    // spread over the products: a CU takes one load of 64 lanes in 16 cycles, one read in 8.
     auto step = [&](auto bv, uint32_t b, uint32_t k) {
         constexpr int kB = decltype(bv)::value;
         constexpr integral_constant<int, 1 - kB> other;
         constexpr uint32_t here = kB * S::kStage, next = S::kStage - here;
         const uint32_t after = min(b + 2, blocks - 1);
-        rows_arrived_but<16>();  // every wave has b's first halves in registers, its second halves are there
+        rows_arrived_but<kLoads>();  // every wave has b's first halves in registers, its second halves are there
+        if constexpr (kHalf) {
+            quarter(bv, first, bv, [&](auto nv) {
+                constexpr int n = decltype(nv)::value;
+                if constexpr (n % 2 == 1) bring(after, here, 0, 0, n / 2);
+                if constexpr (n % 2 == 0) half(w[n / 4 + 4], here + wt + (n / 4 + 4) * 2048, n / 2 % 2);
+            });
+            rows_arrived_but<kLoads>();  // every wave has all of b in registers, b + 1's x and first half are there
+            quarter(bv, last, bv, [&](auto nv) {
+                constexpr int n = decltype(nv)::value;
+                if constexpr (n % 4 == 3) bring(after, here, 0, 1, 4 + n / 4);
+                if constexpr (n < 8) half(x[4 * (1 - kB) + n / 2], next + xt + n / 2 * 2048, n % 2);
+                else half(w[(n - 8) / 2], next + wt + (n - 8) / 2 * 2048, n % 2);
+                if constexpr (n == 12) scales(other, (k + 1) % kScaleBlocks);  // behind a chunk's last: read again
+            });
+            return;
+        }
         quarter(bv, first, bv, [&](auto nv) {
             constexpr int n = decltype(nv)::value, t = 4 * (1 - kB) + n / 2;
             if constexpr (n % 4 == 3) bring(after, here, kB, 0, n / 4);
@@ -833,7 +874,7 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
             if constexpr (n % 4 == 3) bring(after, here, kB, 0, 4 + n / 4);
             if constexpr (n < 8 && n % 2 == 0) half(w[n / 4 + 6], here + wt + (n / 4 + 6) * 2048, n / 2 % 2);
         });
-        rows_arrived_but<16>();  // every wave has all of b in registers, b + 1's first halves are there
+        rows_arrived_but<kLoads>();  // every wave has all of b in registers, b + 1's first halves are there
         quarter(bv, last, other, [&](auto nv) {
             constexpr int n = decltype(nv)::value;
             if constexpr (n % 4 == 3) bring(after, here, 1 - kB, 1, n / 4);
@@ -847,14 +888,17 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
         });
     };
     for (uint32_t b0 = 0; b0 < blocks; b0 += kScaleBlocks) {
-        rows_tile_scales<S, false>(a, lds, b0, r0, r1, (uint32_t)w0, c0);
-        rows_arrived_but<16>();
+        rows_tile_scales<S, false, kHalf>(a, lds, b0, r0, r1, (uint32_t)w0, c0);
+        rows_arrived_but<kLoads>();
         // the first block's (a later chunk's are there already)
         scales(first, 0);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = frag(xt + t * 2048);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = frag(wt + i * 2048);
+            for (int h = 0; h < 2; ++h) {
+                half(x[i], xt + i * 2048, h);
+                half(w[i], wt + i * 2048, h);
+            }
         const uint32_t count = min(kScaleBlocks, blocks - b0);
         for (uint32_t k = 0; k < count; k += 2) {
             step(first, b0 + k, k);
@@ -866,17 +910,17 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
     constexpr uint32_t kPitch = 2 * S::kN + 16;
     static_assert(kPitch * S::kM <= S::kLds, "a tile of results");
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
+    for (int t = 0; t < kXt; ++t)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             typedef __bf16 b4 __attribute__((ext_vector_type(4)));
             const wh_f4 v = acc[i][t];
-            *(b4*)(lds + (wm * 128 + 16 * t + l16) * kPitch + ((wn * 8 + i) * 16 + 4 * q) * 2) =
+            *(b4*)(lds + (wm * 16 * kXt + 16 * t + l16) * kPitch + ((wn * 8 + i) * 16 + 4 * q) * 2) =
                 b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
         }
     __syncthreads();
 #pragma unroll 4
-    for (uint32_t u = threadIdx.x; u < S::kM * S::kN / 8; u += S::kThreads) {
+    for (uint32_t u = threadIdx.x; u < 32 * kXt * S::kN / 8; u += S::kThreads) {
         const uint32_t r = u / (S::kN / 8), col = c0 + u % (S::kN / 8) * 8, j = r0 + r;
         if (j >= r1 || col >= a.out_rows) continue;
         wh_u4 v = *(const wh_u4*)(lds + r * kPitch + (col - c0) * 2);
@@ -889,6 +933,60 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
         } else {
             for (uint32_t e = 0; e < 8 && col + e < a.out_rows; ++e) to[e] = (uint16_t)(v[e / 2] >> 16 * (e & 1));
         }
+    }
+}
+
+// kTall: tiles of 256 rows, those with at most 128 as half tiles; else of 128.  A
+// workgroup a CU takes its XCD's tiles until there are none left (half tiles take half
+// as long), then other XCDs': the first by its id, the next from a counter that it asks a
+// tile ahead.  tickets: [8] tiles taken, workgroups done; 0 between launches.
+template <bool kTall, bool kMant>
+__global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
+    extern __shared__ __align__(128) uint8_t tile_lds[];
+    __shared__ uint32_t upcoming[2];  // the next tile's XCD (8: none) and number
+    const rows_tiling<kTall ? 256 : 128, 256> tiles(a);
+    const uint32_t mates = gridDim.x / 8, lane = threadIdx.x & 63;
+    const bool once = tiles.total <= gridDim.x;  // then nobody takes a second one (XCDs have equal shares)
+    uint32_t xcd = blockIdx.x & 7;
+    uint64_t t = blockIdx.x / 8;
+    if (once && t >= tiles.count(xcd)) return;
+    while (xcd < 8) {
+        uint32_t taken = 0;
+        if (!once && threadIdx.x == 0) taken = atomicAdd(&a.tickets[xcd], 1u);
+        if (t < tiles.count(xcd)) {
+            uint32_t g, r0, r1, c0;
+            tiles.at(xcd, t, g, r0, r1, c0);
+            if (kTall && r1 - r0 > 128) rows_big<false, false>(a, tile_lds, g, r0, r1, c0);
+            else rows_big<true, kMant>(a, tile_lds, g, r0, r1, c0);
+        }
+        if (once) return;
+        if (threadIdx.x < 64) {  // one wave's view of who has tiles left
+            uint32_t x = xcd;
+            uint64_t n = (uint64_t)mates + (uint32_t)__builtin_amdgcn_readfirstlane((int)taken);
+            while (x < 8 && n >= tiles.count(x)) {
+                const uint32_t other = (x + 1 + lane) & 7;
+                const uint32_t is = __hip_atomic_load(&a.tickets[other], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const uint64_t left = __ballot(lane < 8 && (uint64_t)mates + is < tiles.count(other));
+                if (!left) {
+                    x = 8;
+                } else {
+                    x = (x + 1 + (uint32_t)__builtin_ctzll(left)) & 7;
+                    if (lane == 0) taken = atomicAdd(&a.tickets[x], 1u);
+                    n = (uint64_t)mates + (uint32_t)__builtin_amdgcn_readfirstlane((int)taken);
+                }
+            }
+            if (lane == 0) {
+                upcoming[0] = x;
+                upcoming[1] = (uint32_t)n;
+            }
+        }
+        __syncthreads();
+        xcd = __builtin_amdgcn_readfirstlane((int)upcoming[0]);
+        t = (uint32_t)__builtin_amdgcn_readfirstlane((int)upcoming[1]);
+        __syncthreads();
+    }
+    if (threadIdx.x == 0 && atomicAdd(&a.tickets[8], 1u) == gridDim.x - 1) {
+        for (uint32_t i = 0; i < 9; ++i) a.tickets[i] = 0;
     }
 }
 
@@ -1094,9 +1192,17 @@ constexpr uint64_t kMaxGrid256 = 0xffffffull;
 
 }  // namespace
 
+// ------------------------------------------------------------------- host
+
 constexpr size_t plan_lds(uint32_t n_groups) { return kPlanWaves * (size_t)n_groups * sizeof(uint32_t); }
 
+uint32_t g_workgroups = 256;  // a multiple of 8, one a CU
+
 hipError_t wh_rows_setup() {
+    int device = 0, cus = 0;
+    if (hipGetDevice(&device) == hipSuccess &&
+        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) == hipSuccess && cus >= 8)
+        g_workgroups = (uint32_t)cus / 8 * 8;
     hipError_t e = hipFuncSetAttribute((const void*)k_expert_place, hipFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)plan_lds(WH_ROWS_MAX_GROUPS));
     auto tile = [&](const void* f, size_t lds) {
@@ -1107,7 +1213,10 @@ hipError_t wh_rows_setup() {
     tile((const void*)k_rows_mm_tile<4, 4, 2, 2, true, false>, lds);
     tile((const void*)k_rows_mm_tile<4, 4, 2, 2, false, true>, lds);
     tile((const void*)k_rows_mm_tile<4, 4, 2, 2, false, false>, lds);
-    tile((const void*)k_rows_mm_big, rows_tile_shape<8, 8, 2, 2>::kLds);
+    constexpr size_t big = rows_tile_shape<8, 8, 2, 2>::kLds;
+    tile((const void*)k_rows_mm_big<true, false>, big);
+    tile((const void*)k_rows_mm_big<false, false>, big);
+    tile((const void*)k_rows_mm_big<false, true>, big);
     return e;
 }
 
@@ -1132,49 +1241,80 @@ hipError_t wh_rows_read_launch(const wh_rows_read_args& a, bool bf16, hipStream_
     return hipGetLastError();
 }
 
-bool wh_rows_mm_fits(const wh_rows_mm_args& a) {
-    return rows_tiles(a, kAnyRows) * ((a.out_rows + 15) / 16) <= kMaxGrid256;
+// The kernel of a product.
+enum class rows_kind { kAny, kThin, kTile, kHalf, kTall };
+rows_kind rows_kind_of(const wh_rows_mm_args& a, bool bf16) {
+    if (!rows_mm_matrix(a)) return rows_kind::kAny;
+    const bool mant = a.scale_f32 || a.odd_scale;
+    rows_kind kind = rows_kind::kThin;
+    if (a.n > 48 * a.n_groups) kind = rows_kind::kTile;
+    if (bf16 && !mant && a.n >= 256 * a.n_groups) kind = rows_kind::kTall;
+    return kind;
+}
+
+// Workgroups of a call, and threads of each.
+uint64_t rows_grid(const wh_rows_mm_args& a, rows_kind kind, uint32_t* threads) {
+    auto tiles = [&](uint32_t m, uint32_t n) { return rows_tiles(a, m) * ((a.out_rows + n - 1) / n); };
+    *threads = 256;
+    switch (kind) {
+        case rows_kind::kAny: return tiles(kAnyRows, 16);
+        case rows_kind::kThin: {
+            *threads = 64 * kThinWaves;
+            const uint32_t per = 16 * (kThinWaves / rows_thin_split(a.cols));
+            return (uint64_t)((a.out_rows + per - 1) / per) * a.n_groups;
+        }
+        case rows_kind::kTile: return (tiles(128, 128) + 7) / 8 * 8;
+        case rows_kind::kHalf: return std::min<uint64_t>((tiles(128, 256) + 7) / 8 * 8, g_workgroups);
+        default: return std::min<uint64_t>((tiles(256, 256) + 7) / 8 * 8, g_workgroups);
+    }
+}
+
+bool wh_rows_mm_fits(const wh_rows_mm_args& a, bool bf16) {
+    uint32_t threads;
+    const uint64_t grid = rows_grid(a, rows_kind_of(a, bf16), &threads);
+    return grid * threads <= 0xffffffffull;
 }
 
 hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, bool bf16, hipStream_t stream) {
     const bool mant = a.scale_f32 || a.odd_scale;
-    if (rows_mm_matrix(a) && bf16 && !mant && a.n >= 256 * a.n_groups) {
-        typedef rows_tile_shape<8, 8, 2, 2> S;
-        const uint64_t tiles = rows_tiles(a, S::kM) * ((a.out_rows + S::kN - 1) / S::kN);
-        const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);
-        k_rows_mm_big<<<grid, S::kThreads, S::kLds, stream>>>(a);
-        return hipGetLastError();
-    }
-    if (rows_mm_matrix(a) && a.n > 48 * a.n_groups) {
-        typedef rows_tile_shape<4, 4, 2, 2> S;
-        const uint64_t tiles = rows_tiles(a, S::kM) * ((a.out_rows + S::kN - 1) / S::kN);
-        const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);
-        auto go = [&](auto kern) { kern<<<grid, S::kThreads, S::kLds, stream>>>(a); };
-        if (bf16) {
-            if (mant) go(k_rows_mm_tile<4, 4, 2, 2, true, true>);
-            else go(k_rows_mm_tile<4, 4, 2, 2, true, false>);
-        } else {
-            if (mant) go(k_rows_mm_tile<4, 4, 2, 2, false, true>);
-            else go(k_rows_mm_tile<4, 4, 2, 2, false, false>);
+    const rows_kind kind = rows_kind_of(a, bf16);
+    uint32_t threads;
+    const uint32_t grid = (uint32_t)rows_grid(a, kind, &threads);
+    auto go = [&](size_t lds, auto kern) { kern<<<grid, threads, lds, stream>>>(a); };
+    constexpr size_t tile = rows_tile_shape<4, 4, 2, 2>::kLds, big = rows_tile_shape<8, 8, 2, 2>::kLds;
+    switch (kind) {
+        case rows_kind::kAny:
+            if (bf16) go(0, k_rows_mm_any<true>);
+            else go(0, k_rows_mm_any<false>);
+            break;
+        case rows_kind::kThin: {
+            const uint32_t ks = rows_thin_split(a.cols);
+            const dim3 by_group(grid / a.n_groups, a.n_groups);
+            auto thin = [&](auto kern) { kern<<<by_group, threads, 0, stream>>>(a, ks); };
+            if (bf16) {
+                if (mant) thin(k_rows_mm_thin<true, true>);
+                else thin(k_rows_mm_thin<true, false>);
+            } else {
+                if (mant) thin(k_rows_mm_thin<false, true>);
+                else thin(k_rows_mm_thin<false, false>);
+            }
+            break;
         }
-        return hipGetLastError();
+        case rows_kind::kTile:
+            if (bf16) {
+                if (mant) go(tile, k_rows_mm_tile<4, 4, 2, 2, true, true>);
+                else go(tile, k_rows_mm_tile<4, 4, 2, 2, true, false>);
+            } else {
+                if (mant) go(tile, k_rows_mm_tile<4, 4, 2, 2, false, true>);
+                else go(tile, k_rows_mm_tile<4, 4, 2, 2, false, false>);
+            }
+            break;
+        case rows_kind::kHalf:
+            if (mant) go(big, k_rows_mm_big<false, true>);
+            else go(big, k_rows_mm_big<false, false>);
+            break;
+        case rows_kind::kTall: go(big, k_rows_mm_big<true, false>); break;
     }
-    if (rows_mm_matrix(a)) {
-        const uint32_t ks = rows_thin_split(a.cols), per = 16 * (kThinWaves / ks);
-        const dim3 grid((a.out_rows + per - 1) / per, a.n_groups);
-        auto go = [&](auto kern) { kern<<<grid, 64 * kThinWaves, 0, stream>>>(a, ks); };
-        if (bf16) {
-            if (mant) go(k_rows_mm_thin<true, true>);
-            else go(k_rows_mm_thin<true, false>);
-        } else {
-            if (mant) go(k_rows_mm_thin<false, true>);
-            else go(k_rows_mm_thin<false, false>);
-        }
-        return hipGetLastError();
-    }
-    const unsigned grid = (unsigned)(rows_tiles(a, kAnyRows) * ((a.out_rows + 15) / 16));
-    if (bf16) k_rows_mm_any<true><<<grid, 256, 0, stream>>>(a);
-    else k_rows_mm_any<false><<<grid, 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 

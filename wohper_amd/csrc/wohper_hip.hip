@@ -305,6 +305,7 @@ struct wh_ctx {
     Scratch attn_max;                       // attn_mx.h: the score tiles' maxima, of a fixed size
     Scratch kv4_part, kv4_ticket;           // the 4-bit cache: partial outputs of split attention, a plan's arrivals
     Scratch rows_counts;                    // expert lists: routes of each expert by chunk
+    Scratch rows_tickets;                   // 8-bit rows: which tiles of a product are taken
     Scratch layer;                          // the decode layer's state and activations between its steps
     bool exact = true;                      // routed experts in the reference's summation order
     int token_kernels = 1;                  // MFMA token kernels: bit 0 gate/up, bit 1 down on k_*_tok (else k_*_px)
@@ -324,7 +325,7 @@ struct wh_ctx {
     hipStream_t base_stream = nullptr, cap_stream = nullptr;
     std::vector<Scratch*> scratch() {
         return {&x_in, &y_out, &h, &ybuf, &cnt_y, &tmp, &batch, &routes, &bout, &gu, &relayout, &rtr, &rtr_cnt,
-                &mla, &hcs, &fp8mm_ws, &fp8mm_cnt, &moe_dyn, &attn_max, &kv4_part, &kv4_ticket, &rows_counts, &layer};
+                &mla, &hcs, &fp8mm_ws, &fp8mm_cnt, &moe_dyn, &attn_max, &kv4_part, &kv4_ticket, &rows_counts, &rows_tickets, &layer};
     }
 };
 
@@ -2107,6 +2108,7 @@ int wh_init(int device, wh_ctx** out) {
         e = c->attn_max.ensure((size_t)WH_POS_BATCH * WH_ATTN_MX_HEADS * WH_ATTN_MX_TILES * sizeof(float), false);
     if (e == hipSuccess) e = wh_kv4_setup();
     if (e == hipSuccess) e = wh_rows_setup();
+    if (e == hipSuccess) e = c->rows_tickets.ensure(WH_ROWS_TICKETS * sizeof(uint32_t), true);
     if (e == hipSuccess) e = c->kv4_ticket.ensure(sizeof(uint32_t), true);
     if (e != hipSuccess) {
         delete c;
@@ -4945,7 +4947,8 @@ int rows_mm_go(wh_ctx* c, const Tensor& t, size_t row_start, wh_rows_mm_args& a,
     a.scale_f32 = t.scale_fmt == WH_SCALE_F32;
     a.special = t.special;
     a.odd_scale = t.odd_scale;
-    if (!wh_rows_mm_fits(a)) return WH_UNSUPPORTED;
+    a.tickets = c->rows_tickets.as<uint32_t>();
+    if (!wh_rows_mm_fits(a, bf16 != 0)) return WH_UNSUPPORTED;
     WH_HIP(hipSetDevice(c->device));
     WH_HIP(wh_rows_mm_launch(a, bf16 != 0, c->stream));
     return WH_OK;
