@@ -456,6 +456,97 @@ def test_f32_products_keep_what_is_far_below_the_largest(ctx, n):
     ctx.release(h)
 
 
+# Large calls: references on the GPU, in 64 bits.
+
+E4M3_DEV = {}
+
+
+def gpu_values(codes, scales, rows_each):
+    """f64 of codes [n, cols] (uint8, on the GPU, column order) whose scales [n / rows_each, cols / 128] are f64."""
+    if "t" not in E4M3_DEV:
+        E4M3_DEV["t"] = torch.from_numpy(E4M3).cuda()
+    v = E4M3_DEV["t"][codes.int()]
+    return v * scales.repeat_interleave(rows_each, 0).repeat_interleave(BLOCK, 1)
+
+
+class Large:
+    """A weight and rows whose bytes are made on the GPU."""
+
+    def __init__(self, ctx, seed, n, rows, cols, f32):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        self.ctx, self.n, self.cols = ctx, n, cols
+
+        def codes(m):
+            v = (torch.randn(m, cols, generator=g, device="cuda") * 110).clamp_(-448, 448)
+            return v.to(torch.float8_e4m3fn).view(torch.uint8)
+
+        w, x = codes(rows), codes(n)
+        block = 16 if rows % 128 else 128
+        ws = torch.exp2(6 * torch.rand(rows // block, cols // 128, generator=g, device="cuda") - 10)
+        if not f32:
+            ws = torch.randint(117, 124, ws.shape, generator=g, device="cuda", dtype=torch.uint8)
+        xs = torch.randint(115, 126, (n, cols // 128), generator=g, device="cuda", dtype=torch.uint8)
+        self.w = gpu_values(w, ws.double() if f32 else torch.exp2(ws.double() - 127), block)
+        self.x = gpu_values(x, torch.exp2(xs.double() - 127), 1)
+        self.rows = Rows(n, cols)
+        self.rows.codes.copy_(x.reshape(n, -1, BLOCK)[:, :, torch.from_numpy(COLUMN).cuda()].reshape(n, cols))
+        self.rows.scales[:, :cols // 128] = xs
+        self.h = ctx.store_fp8_device(w.data_ptr(), rows, cols, ws.data_ptr(), *ws.shape, int(f32))
+
+
+def gpu_near(got, x, w, bf16, cols):
+    got = got.double()
+    want, size = x @ w.T, x.abs() @ w.abs().T
+    err = (got - want).abs()
+    if bf16:
+        assert bool((err <= 2.0 ** -8 * want.abs() + 1.01 * 2.0 ** -10 * size).all())
+        assert float(err.norm()) <= 2.0 ** -8 * float(want.norm())
+    else:
+        assert bool((err <= (cols + 8) * U * size).all())
+        assert float(err.norm()) <= (cols ** 0.5 + 2) * U * float(want.norm())
+
+
+@pytest.mark.parametrize("n,rows,cols", [(4096, 4096, 1280), (2048, 4096, 4096), (4100, 2112, 8320), (300, 704, 10240), (5000, 1008, 128),
+                                         (700, 512, 8192), (1024, 32768, 256), (33, 4096, 10240), (100, 16384, 4096)])
+@pytest.mark.parametrize("bf16,f32", [(False, False), (False, True), (True, False), (True, True)])
+def test_large_products(ctx, n, rows, cols, bf16, f32):
+    c = Large(ctx, n, n, rows, cols, f32)
+    last = rows - 5  # an odd range
+    y = torch.full((n + 1, last), 5.0, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    ctx.fp8_rows_mm_async(c.h, 0, last, c.rows.c, n, y.data_ptr(), last, bf16)
+    ctx.synchronize()
+    gpu_near(y[:n], c.x, c.w[:last], bf16, cols)
+    assert bool((y[n] == 5.0).all())
+    ctx.release(c.h)
+
+
+@pytest.mark.parametrize("n_groups,n,rows,cols", [(64, 6000, 512, 1152), (5, 9000, 1024, 640), (16, 3000, 272, 8448), (300, 2000, 256, 256),
+                                                  (3, 500, 512, 4096), (1024, 3000, 16, 128)])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_large_groups(ctx, n_groups, n, rows, cols, bf16):
+    rng = np.random.default_rng(n)
+    n_x = 900
+    c = Large(ctx, n, n_x, n_groups * rows, cols, n_groups == 5)
+    starts = lists(rng, n_groups, n, "ragged")
+    at = rng.integers(0, n_x, n)
+    at[rng.integers(0, n, 20)] = NONE
+    s, r = i32(starts), i32(at)
+    y = torch.full((n + 1, rows + 4), 5.0, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    for _ in range(2):
+        ctx.fp8_rows_mm_groups_async(c.h, 0, rows, n_groups, c.rows.c, n_x, r.data_ptr(), s.data_ptr(), n, y.data_ptr(), rows + 4, bf16)
+    ctx.synchronize()
+    assert bool((y[starts[-1]:] == 5.0).all()) and bool((y[:, rows:] == 5.0).all())
+    at_dev = torch.from_numpy(at).cuda()
+    for g in range(n_groups):
+        a, b = int(starts[g]), int(starts[g + 1])
+        if b > a:
+            take = at_dev[a:b]
+            v = torch.where((take < n_x)[:, None], c.x[take.clamp(max=n_x - 1)], 0.0)
+            gpu_near(y[a:b, :rows], v, c.w[g * rows:(g + 1) * rows], bf16, cols)
+    ctx.release(c.h)
+
+
 # --------------------------------------------------------------- groups
 
 def lists(rng, n_groups, n, kind):

@@ -52,12 +52,21 @@ struct wh_rows_mm_args {
     uint32_t scale_f32;  // scales are f32, else UE8M0 bytes
     uint32_t special;    // weight codes 0x7F / 0xFF are there, +-480
     uint32_t odd_scale;  // UE8M0 scale bytes 0 or 255 are there
+    float* part;         // the plan's part_bytes
     uint32_t* tickets;   // [WH_ROWS_TICKETS], 0 between launches
     uint32_t y_vec;      // y takes stores of four values (1), of 16 bytes (2)
 };
-// Whether a call's grid is within the limits of a launch.
-bool wh_rows_mm_fits(const wh_rows_mm_args& a, bool bf16);
-hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, bool bf16, hipStream_t stream);
+// How a product is done: by sizes that the host knows.
+struct wh_rows_mm_plan {
+    enum kind_t { kAny, kThin, kTile, kHalf, kTall } kind;
+    uint32_t splits, per;  // ranges that its columns are cut into, and blocks of each
+    uint32_t threads;
+    uint64_t grid;         // workgroups for each range
+    size_t part_bytes;     // scratch for the ranges' parts
+    bool fits;             // within the limits of a launch
+};
+wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16);
+hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, const wh_rows_mm_plan& p, bool bf16, hipStream_t stream);
 hipError_t wh_rows_setup();  // once for each device, before the first launch there
 
 // The store's lane layout of a tensor that is on the device, and which of its

@@ -10,6 +10,7 @@
 #include "fp8_rows.h"
 
 #include <algorithm>
+#include <cmath>
 
 #include "wh_device.h"
 
@@ -465,6 +466,9 @@ __global__ void __launch_bounds__(64 * kThinWaves) k_rows_mm_thin(wh_rows_mm_arg
     }
 }
 
+// Values between rows of a part.
+__host__ __device__ __forceinline__ uint32_t rows_part_stride(const wh_rows_mm_args& a) { return (a.out_rows + 3) / 4 * 4; }
+
 // LDS byte address of a pointer into __shared__ memory.
 __device__ __forceinline__ uint32_t rows_lds(const void* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
@@ -566,13 +570,13 @@ struct rows_tile_shape {
     static constexpr uint32_t kWm0 = kWs + kScaleBlocks * kN / 16, kNan = kWm0 + kScaleBlocks * kN / 4, kLds = kNan + kM;
 };
 
-// Brings the scales of blocks [b0, b0 + kScaleBlocks) into LDS; a block behind the
-// last gets bytes 0, whose product of 2^-254 with any sum of codes is 0.  One row a
+// Brings the scales of blocks [b0, b0 + kScaleBlocks) below b1 into LDS (b0 a multiple
+// of 4); a block behind the last gets bytes 0, whose product of 2^-254 with any sum of codes is 0.  One row a
 // thread, its words all in flight.  kHalf: place r is row r / 128 * 64 + r % 64.
 template <class S, bool kNanFlags, bool kHalf = false>
-__device__ __forceinline__ void rows_tile_scales(const wh_rows_mm_args& a, uint8_t* lds, uint32_t b0, uint32_t r0, uint32_t r1,
-                                                 uint32_t w0, uint32_t c0) {
-    const uint32_t blocks = a.cols / 128u, count = min(kScaleBlocks, blocks - b0);
+__device__ __forceinline__ void rows_tile_scales(const wh_rows_mm_args& a, uint8_t* lds, uint32_t b0, uint32_t b1, uint32_t r0,
+                                                 uint32_t r1, uint32_t w0, uint32_t c0) {
+    const uint32_t blocks = a.cols / 128u, count = min(kScaleBlocks, b1 - b0);
     constexpr uint32_t kParts = S::kThreads / S::kM, kWords = kScaleBlocks / 4 / kParts;
     const uint32_t r = threadIdx.x % S::kM, from = threadIdx.x / S::kM * kWords;
     bool is;
@@ -608,8 +612,11 @@ __device__ __forceinline__ void rows_tile_scales(const wh_rows_mm_args& a, uint8
     if (kNanFlags && nan) lds[S::kNan + r] = 1;
 }
 
-template <int kMt, int kNt, int kWm, int kWn, bool kBf16, bool kMant>
-__global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads), 2) k_rows_mm_tile(wh_rows_mm_args a) {
+// Where there are few tiles, their columns are cut into gridDim.y ranges of `per` blocks (a
+// multiple of 4), whose parts go to a.part in f32 and k_rows_join adds up.
+template <bool kBf16, bool kMant>
+__global__ void __launch_bounds__(256, 2) k_rows_mm_tile(wh_rows_mm_args a, uint32_t per) {
+    constexpr int kMt = 4, kNt = 4, kWm = 2, kWn = 2;
     typedef rows_tile_shape<kMt, kNt, kWm, kWn> S;
     static_assert(kMt == 4 && kNt == 4, "a word of scale bytes is four tiles");
     extern __shared__ __align__(128) uint8_t tile_lds[];
@@ -619,7 +626,8 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
     if (blockIdx.x / 8 >= tiles.count(blockIdx.x & 7)) return;
     tiles.at(blockIdx.x & 7, blockIdx.x / 8, g, r0, r1, c0);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t l16 = lane & 15, q = lane >> 4, wm = wave % kWm, wn = wave / kWm, blocks = a.cols / 128u;
+    const uint32_t l16 = lane & 15, q = lane >> 4, wm = wave % kWm, wn = wave / kWm;
+    const uint32_t first = blockIdx.y * per, end = min(a.cols / 128u, first + per);
     const uint64_t w0 = a.row_start + (uint64_t)g * a.out_rows;
     constexpr uint32_t kWaves = kWm * kWn, kXd = S::kM / 8 / kWaves, kWd = S::kN / 8 / kWaves;
     // this wave's loads: eight rows each, a lane one chunk
@@ -638,7 +646,7 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
         wo[i] = min((wave + i * kWaves) * 8 + (lane >> 3), a.out_rows - 1 - c0) * a.cols + chunk;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rows_lds(lds));
     auto bring = [&](uint32_t b) {
-        const uint32_t to = lds0 + (b & 1) * S::kStage + wave * 1024;
+        const uint32_t to = lds0 + (b - first) % 2 * S::kStage + wave * 1024;
 #pragma unroll
         for (uint32_t i = 0; i < kXd; ++i) rows_dma(xp[i] + b * 128u, to + i * kWaves * 1024);
 #pragma unroll
@@ -652,19 +660,19 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
     for (int i = 0; i < kNt; ++i)
 #pragma unroll
         for (int t = 0; t < kMt; ++t) acc[i][t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    bring(0);
+    bring(first);
     const uint32_t at = l16 * 128 + ((q ^ (l16 & 7)) << 4);  // the lane's first chunk in a tile of 16 rows
-    for (uint32_t b = 0; b < blocks; ++b) {
-        if (b % kScaleBlocks == 0) {
+    for (uint32_t b = first; b < end; ++b) {
+        const uint32_t k = (b - first) % kScaleBlocks;
+        if (k == 0) {
             __syncthreads();
-            rows_tile_scales<S, !kBf16>(a, lds, b, r0, r1, (uint32_t)w0, c0);
+            rows_tile_scales<S, !kBf16>(a, lds, b, end, r0, r1, (uint32_t)w0, c0);
         }
         rows_arrived();
-        if (b + 1 < blocks) bring(b + 1);
-        const uint8_t* const stage = lds + (b & 1) * S::kStage;
+        if (b + 1 < end) bring(b + 1);
+        const uint8_t* const stage = lds + (b - first) % 2 * S::kStage;
         const uint8_t* const xt = stage + wm * (16 * kMt * 128);
         const uint8_t* const wt = stage + S::kM * 128 + wn * (16 * kNt * 128);
-        const uint32_t k = b % kScaleBlocks;
         const uint32_t xb = *(const uint32_t*)(lds + S::kXs + ((k * (S::kM / 64) + wm) * 16 + l16) * 4);
         const uint32_t wb = *(const uint32_t*)(lds + S::kWs + (k * (S::kN / 64) + wn) * 4);
         wh_f4 m = {1.0f, 1.0f, 1.0f, 1.0f};
@@ -728,13 +736,29 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
             if (nan) v = wh_f4{1.0f, 1.0f, 1.0f, 1.0f} * __uint_as_float(0x7fc00000u);
             if (!is) v = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
             const uint32_t col = c0 + (wn * kNt + i) * 16 + 4 * q;
-            if (col < a.out_rows) rows_put4<kBf16>(a, j, col, v);
+            if (col >= a.out_rows) continue;
+            if (gridDim.y > 1) *(wh_f4*)(a.part + (blockIdx.y * (uint64_t)a.n + j) * rows_part_stride(a) + col) = v;
+            else rows_put4<kBf16>(a, j, col, v);
         }
     }
 }
 
+// Adds up the parts of listed rows, in order, four columns a thread.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) k_rows_join(wh_rows_mm_args a, uint32_t splits) {
+    const uint32_t units = rows_part_stride(a) / 4;
+    const uint64_t u = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t j = u / units;
+    const uint32_t col = (uint32_t)(u - j * units) * 4;
+    if (j >= a.n || (a.starts && (j < a.starts[0] || j >= a.starts[a.n_groups]))) return;
+    const float* p = a.part + j * rows_part_stride(a) + col;
+    wh_f4 v = *(const wh_f4*)p;
+    for (uint32_t s = 1; s < splits; ++s) v += *(const wh_f4*)(p + s * (uint64_t)a.n * rows_part_stride(a));
+    rows_put4<kBf16>(a, j, col, v);
+}
+
 // Tiles of 256 x 256 for bf16 results, four waves of 128 x 128, where there are enough
-// of them.  A block's 64 products a wave go in quarters of four by four tiles, in the
+// of them (and no factors of scales, which would take results through vector registers).  A block's 64 products a wave go in quarters of four by four tiles, in the
 // order (w0 x0) (w0 x1) (w1 x1) (w1 x0), the next block's with x0 and x1 changed over:
 // so each half of the operands dies in time to take the next block's behind products
 // that do not need it, and 128 registers hold both blocks.  In LDS the halves of a block
@@ -742,9 +766,8 @@ __global__ void __launch_bounds__((rows_tile_shape<kMt, kNt, kWm, kWn>::kThreads
 // them: the first ones a block before the end, the others half a block later, so loads
 // run a whole block ahead and come evenly.
 // kHalf: a tile of 128 rows, 64 a wave: x0 alone, in two sets of registers.
-template <bool kHalf, bool kMant>
+template <bool kHalf>
 __device__ __forceinline__ void rows_big(const wh_rows_mm_args& a, uint8_t* lds, uint32_t g, uint32_t r0, uint32_t r1, uint32_t c0) {
-    static_assert(kHalf || !kMant, "factors take results through vector registers: 64 rows a wave at most");
     typedef rows_tile_shape<8, 8, 2, 2> S;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t l16 = lane & 15, q = lane >> 4, wm = wave & 1, wn = wave >> 1, blocks = a.cols / 128u;
@@ -792,36 +815,22 @@ __device__ __forceinline__ void rows_big(const wh_rows_mm_args& a, uint8_t* lds,
     };
     wh_i8 x[8], w[8];
     uint32_t xb[2][2], wb[2][2];  // scale bytes of the halves, of even and odd blocks
-    wh_f4 m[2][2] = {};           // factors of the weights' scales
     auto scales = [&](auto bv, uint32_t k) {
         constexpr int kB = decltype(bv)::value;
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
             wb[kB][h] = *(const uint32_t*)(lds + S::kWs + k * 16 + wn * 8 + 4 * h);
             xb[kB][h] = kHalf && h ? 0 : *(const uint32_t*)(lds + S::kXs + ((k * 4 + wm * 2 + h) * 16 + l16) * 4);
-            if constexpr (kMant) m[kB][h] = *(const wh_f4*)(lds + S::kWm0 + (k * 16 + wn * 8 + 4 * h) * 4);
         }
     };
     // the 16 products of weight half kW and x half kX (kHalf: set kX), f(n) behind the n-th
     auto quarter = [&](auto bv, auto wv, auto xv, auto&& f) {
         constexpr int kB = decltype(bv)::value, kW = decltype(wv)::value, kX = decltype(xv)::value;
-        wh_f4 s[16];
-        wh_static_for<18>([&](auto nv) {
-            constexpr int n = decltype(nv)::value;
-            if constexpr (n < 16) {
-                constexpr int i = 4 * kW + n / 4, t = n % 4, at_t = kHalf ? t : 4 * kX + t;
-                const wh_f4 from = kMant ? wh_f4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][at_t];
-                s[n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[4 * kX + t], from, 0, 0, n / 4, (int)wb[kB][kW], t,
-                                                                        (int)xb[kB][kHalf ? 0 : kX]);
-                if constexpr (!kMant) acc[i][at_t] = s[n];
-                f(nv);
-            }
-            if constexpr (kMant && n >= 2) {  // two products behind, whose result is there
-                constexpr int p = n - 2;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[4 * kW + p / 4][p % 4][j] = fmaf(s[p][j], m[kB][kW][p / 4], acc[4 * kW + p / 4][p % 4][j]);
-            }
+        wh_static_for<16>([&](auto nv) {
+            constexpr int n = decltype(nv)::value, i = 4 * kW + n / 4, t = n % 4, at_t = kHalf ? t : 4 * kX + t;
+            acc[i][at_t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[4 * kX + t], acc[i][at_t], 0, 0, n / 4,
+                                                                            (int)wb[kB][kW], t, (int)xb[kB][kHalf ? 0 : kX]);
+            f(nv);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -888,7 +897,7 @@ __device__ __forceinline__ void rows_big(const wh_rows_mm_args& a, uint8_t* lds,
         });
     };
     for (uint32_t b0 = 0; b0 < blocks; b0 += kScaleBlocks) {
-        rows_tile_scales<S, false, kHalf>(a, lds, b0, r0, r1, (uint32_t)w0, c0);
+        rows_tile_scales<S, false, kHalf>(a, lds, b0, blocks, r0, r1, (uint32_t)w0, c0);
         rows_arrived_but<kLoads>();
         // the first block's (a later chunk's are there already)
         scales(first, 0);
@@ -940,7 +949,7 @@ __device__ __forceinline__ void rows_big(const wh_rows_mm_args& a, uint8_t* lds,
 // workgroup a CU takes its XCD's tiles until there are none left (half tiles take half
 // as long), then other XCDs': the first by its id, the next from a counter that it asks a
 // tile ahead.  tickets: [8] tiles taken, workgroups done; 0 between launches.
-template <bool kTall, bool kMant>
+template <bool kTall>
 __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
     extern __shared__ __align__(128) uint8_t tile_lds[];
     __shared__ uint32_t upcoming[2];  // the next tile's XCD (8: none) and number
@@ -956,8 +965,8 @@ __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
         if (t < tiles.count(xcd)) {
             uint32_t g, r0, r1, c0;
             tiles.at(xcd, t, g, r0, r1, c0);
-            if (kTall && r1 - r0 > 128) rows_big<false, false>(a, tile_lds, g, r0, r1, c0);
-            else rows_big<true, kMant>(a, tile_lds, g, r0, r1, c0);
+            if (kTall && r1 - r0 > 128) rows_big<false>(a, tile_lds, g, r0, r1, c0);
+            else rows_big<true>(a, tile_lds, g, r0, r1, c0);
         }
         if (once) return;
         if (threadIdx.x < 64) {  // one wave's view of who has tiles left
@@ -1209,14 +1218,13 @@ hipError_t wh_rows_setup() {
         if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     };
     constexpr size_t lds = rows_tile_shape<4, 4, 2, 2>::kLds;
-    tile((const void*)k_rows_mm_tile<4, 4, 2, 2, true, true>, lds);
-    tile((const void*)k_rows_mm_tile<4, 4, 2, 2, true, false>, lds);
-    tile((const void*)k_rows_mm_tile<4, 4, 2, 2, false, true>, lds);
-    tile((const void*)k_rows_mm_tile<4, 4, 2, 2, false, false>, lds);
+    tile((const void*)k_rows_mm_tile<true, true>, lds);
+    tile((const void*)k_rows_mm_tile<true, false>, lds);
+    tile((const void*)k_rows_mm_tile<false, true>, lds);
+    tile((const void*)k_rows_mm_tile<false, false>, lds);
     constexpr size_t big = rows_tile_shape<8, 8, 2, 2>::kLds;
-    tile((const void*)k_rows_mm_big<true, false>, big);
-    tile((const void*)k_rows_mm_big<false, false>, big);
-    tile((const void*)k_rows_mm_big<false, true>, big);
+    tile((const void*)k_rows_mm_big<true>, big);
+    tile((const void*)k_rows_mm_big<false>, big);
     return e;
 }
 
@@ -1241,56 +1249,93 @@ hipError_t wh_rows_read_launch(const wh_rows_read_args& a, bool bf16, hipStream_
     return hipGetLastError();
 }
 
-// The kernel of a product.
-enum class rows_kind { kAny, kThin, kTile, kHalf, kTall };
-rows_kind rows_kind_of(const wh_rows_mm_args& a, bool bf16) {
-    if (!rows_mm_matrix(a)) return rows_kind::kAny;
+// Which kernel takes a product, and how many ranges its columns are cut into: the least
+// of these estimates of its time in us, fitted to 400 measured calls (one MI355X; 1 to
+// 4096 rows, 1 to 64 groups, weights from 1408 x 512 to 32768 x 1024 and 4096 x 8192).
+//  - thin: a wave's block of columns takes 0.95, 1.6 and 3 us for up to 16, 32 and 64
+//    rows, workgroups in rounds of 256: 4096 x 4096 with 16, 64 and 128 rows 7.7, 15.6 and
+//    29, where tiles take 23 to 25, cut up 13 to 18;
+//  - tile: a block 0.56 us in bf16 (0.95 with factors of scales), 1.1 in f32, in rounds of
+//    256 workgroups; ranges divide that and add a launch and their parts' bytes: 4096 x
+//    4096 with 128 rows in 1, 2 and 4 ranges 24.6, 19.9 and 18.1, with 1024 27, 34 and 48;
+//  - half and tall tiles (bf16): 5 and 9 us, and 0.85 and 1.45 a block, by rounds that need
+//    not be whole, since workgroups take tiles until there are none: 4096 x 4096 with
+//    1024, 2048 and 4096 rows 28, 35 and 71 in half tiles, 44, 49 and 59 in tall ones, 27, 40
+//    and 80 in tiles of 128.
+wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
+    const uint32_t blocks = a.cols / 128u;
     const bool mant = a.scale_f32 || a.odd_scale;
-    rows_kind kind = rows_kind::kThin;
-    if (a.n > 48 * a.n_groups) kind = rows_kind::kTile;
-    if (bf16 && !mant && a.n >= 256 * a.n_groups) kind = rows_kind::kTall;
-    return kind;
-}
-
-// Workgroups of a call, and threads of each.
-uint64_t rows_grid(const wh_rows_mm_args& a, rows_kind kind, uint32_t* threads) {
-    auto tiles = [&](uint32_t m, uint32_t n) { return rows_tiles(a, m) * ((a.out_rows + n - 1) / n); };
-    *threads = 256;
-    switch (kind) {
-        case rows_kind::kAny: return tiles(kAnyRows, 16);
-        case rows_kind::kThin: {
-            *threads = 64 * kThinWaves;
-            const uint32_t per = 16 * (kThinWaves / rows_thin_split(a.cols));
-            return (uint64_t)((a.out_rows + per - 1) / per) * a.n_groups;
+    wh_rows_mm_plan p{wh_rows_mm_plan::kAny, 1, blocks, 256, 0, 0, false};
+    const double groups = std::min(a.n_groups, a.n), rows = a.n / groups;
+    // tiles, of groups that end in a tile half full on average
+    auto tiles = [&](double m, uint32_t n) {
+        return (a.n_groups == 1 ? std::ceil(a.n / m) : std::max(groups, a.n / m + groups / 2)) * ((a.out_rows + n - 1) / n);
+    };
+    auto most = [&](uint32_t m, uint32_t n) { return rows_tiles(a, m) * ((a.out_rows + n - 1) / n); };
+    if (rows_mm_matrix(a)) {
+        const uint32_t each = 16 * (kThinWaves / rows_thin_split(a.cols));
+        const double left = rows - 64 * std::floor(rows / 64);
+        const double chunk = 3.0 * std::floor(rows / 64) + (left == 0 ? 0 : left <= 16 ? 0.95 : left <= 32 ? 1.6 : 3.0);
+        double best = 3.5 + std::max(1.0, groups * ((a.out_rows + each - 1) / each) / 256) *
+                                std::ceil((double)blocks / rows_thin_split(a.cols)) * chunk;
+        p.kind = wh_rows_mm_plan::kThin;
+        auto offer = [&](double us, wh_rows_mm_plan::kind_t kind, uint32_t splits, uint32_t per) {
+            if (us >= best) return;
+            best = us;
+            p.kind = kind;
+            p.splits = splits;
+            p.per = per;
+        };
+        const double block = bf16 ? (mant ? 0.95 : 0.56) : 1.1, n_tiles = tiles(128, 128);
+        for (uint32_t want = 1; want <= 16; want *= 2) {
+            uint32_t per = blocks, splits = 1;
+            if (want > 1) {  // ranges of a multiple of 4 blocks, whose scales lie in whole words
+                per = (blocks + want * 4 - 1) / (want * 4) * 4;
+                splits = (blocks + per - 1) / per;
+                if (splits == 1) continue;
+            }
+            const double join = splits == 1 ? 0 : 3 + 8.0 * splits * a.n * a.out_rows / 6.5e6;
+            offer(7 + std::max(1.0, n_tiles * splits / 256) * per * block + join, wh_rows_mm_plan::kTile, splits, per);
         }
-        case rows_kind::kTile: return (tiles(128, 128) + 7) / 8 * 8;
-        case rows_kind::kHalf: return std::min<uint64_t>((tiles(128, 256) + 7) / 8 * 8, g_workgroups);
-        default: return std::min<uint64_t>((tiles(256, 256) + 7) / 8 * 8, g_workgroups);
+        if (bf16 && !mant) {
+            const double half = tiles(128, 256) / 256, tall = (tiles(256, 256) - (a.n_groups == 1 ? 0 : 0.2 * groups * ((a.out_rows + 255) / 256))) / 256;
+            offer(5 + std::max(1.0, half > 1 ? half + 0.25 : half) * (5 + blocks * (0.5 + 0.35 * std::min(1.0, half))),
+                  wh_rows_mm_plan::kHalf, 1, blocks);
+            offer(4 + std::max(1.0, tall > 1 ? tall + 0.25 : tall) * (9 + blocks * (0.9 + 0.55 * std::min(1.0, tall))),
+                  wh_rows_mm_plan::kTall, 1, blocks);
+        }
     }
+    /*force*/
+    switch (p.kind) {
+        case wh_rows_mm_plan::kAny: p.grid = most(kAnyRows, 16); break;
+        case wh_rows_mm_plan::kThin: {
+            p.threads = 64 * kThinWaves;
+            const uint32_t each = 16 * (kThinWaves / rows_thin_split(a.cols));
+            p.grid = (uint64_t)((a.out_rows + each - 1) / each) * a.n_groups;
+            break;
+        }
+        case wh_rows_mm_plan::kTile: p.grid = (most(128, 128) + 7) / 8 * 8; break;
+        case wh_rows_mm_plan::kHalf: p.grid = std::min<uint64_t>((most(128, 256) + 7) / 8 * 8, g_workgroups); break;
+        case wh_rows_mm_plan::kTall: p.grid = std::min<uint64_t>((most(256, 256) + 7) / 8 * 8, g_workgroups); break;
+    }
+    if (p.splits > 1) p.part_bytes = (size_t)p.splits * a.n * rows_part_stride(a) * sizeof(float);
+    p.fits = p.grid * p.threads * p.splits <= 0xffffffffull;  // a grid's threads
+    return p;
 }
 
-bool wh_rows_mm_fits(const wh_rows_mm_args& a, bool bf16) {
-    uint32_t threads;
-    const uint64_t grid = rows_grid(a, rows_kind_of(a, bf16), &threads);
-    return grid * threads <= 0xffffffffull;
-}
-
-hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, bool bf16, hipStream_t stream) {
+hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, const wh_rows_mm_plan& p, bool bf16, hipStream_t stream) {
     const bool mant = a.scale_f32 || a.odd_scale;
-    const rows_kind kind = rows_kind_of(a, bf16);
-    uint32_t threads;
-    const uint32_t grid = (uint32_t)rows_grid(a, kind, &threads);
-    auto go = [&](size_t lds, auto kern) { kern<<<grid, threads, lds, stream>>>(a); };
-    constexpr size_t tile = rows_tile_shape<4, 4, 2, 2>::kLds, big = rows_tile_shape<8, 8, 2, 2>::kLds;
-    switch (kind) {
-        case rows_kind::kAny:
+    const uint32_t grid = (uint32_t)p.grid;
+    constexpr size_t small = rows_tile_shape<4, 4, 2, 2>::kLds, big = rows_tile_shape<8, 8, 2, 2>::kLds;
+    auto go = [&](size_t lds, auto kern) { kern<<<grid, p.threads, lds, stream>>>(a); };
+    switch (p.kind) {
+        case wh_rows_mm_plan::kAny:
             if (bf16) go(0, k_rows_mm_any<true>);
             else go(0, k_rows_mm_any<false>);
             break;
-        case rows_kind::kThin: {
+        case wh_rows_mm_plan::kThin: {
             const uint32_t ks = rows_thin_split(a.cols);
-            const dim3 by_group(grid / a.n_groups, a.n_groups);
-            auto thin = [&](auto kern) { kern<<<by_group, threads, 0, stream>>>(a, ks); };
+            auto thin = [&](auto kern) { kern<<<dim3(grid / a.n_groups, a.n_groups), p.threads, 0, stream>>>(a, ks); };
             if (bf16) {
                 if (mant) thin(k_rows_mm_thin<true, true>);
                 else thin(k_rows_mm_thin<true, false>);
@@ -1300,20 +1345,26 @@ hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, bool bf16, hipStream_t st
             }
             break;
         }
-        case rows_kind::kTile:
+        case wh_rows_mm_plan::kTile: {
+            auto tile = [&](auto kern) { kern<<<dim3(grid, p.splits), p.threads, small, stream>>>(a, p.per); };
             if (bf16) {
-                if (mant) go(tile, k_rows_mm_tile<4, 4, 2, 2, true, true>);
-                else go(tile, k_rows_mm_tile<4, 4, 2, 2, true, false>);
+                if (mant) tile(k_rows_mm_tile<true, true>);
+                else tile(k_rows_mm_tile<true, false>);
             } else {
-                if (mant) go(tile, k_rows_mm_tile<4, 4, 2, 2, false, true>);
-                else go(tile, k_rows_mm_tile<4, 4, 2, 2, false, false>);
+                if (mant) tile(k_rows_mm_tile<false, true>);
+                else tile(k_rows_mm_tile<false, false>);
+            }
+            if (p.splits > 1) {
+                const hipError_t e = hipGetLastError();
+                if (e != hipSuccess) return e;
+                const uint32_t join = (uint32_t)(((uint64_t)a.n * (rows_part_stride(a) / 4) + 255) / 256);
+                if (bf16) k_rows_join<true><<<join, 256, 0, stream>>>(a, p.splits);
+                else k_rows_join<false><<<join, 256, 0, stream>>>(a, p.splits);
             }
             break;
-        case rows_kind::kHalf:
-            if (mant) go(big, k_rows_mm_big<false, true>);
-            else go(big, k_rows_mm_big<false, false>);
-            break;
-        case rows_kind::kTall: go(big, k_rows_mm_big<true, false>); break;
+        }
+        case wh_rows_mm_plan::kHalf: go(big, k_rows_mm_big<false>); break;
+        case wh_rows_mm_plan::kTall: go(big, k_rows_mm_big<true>); break;
     }
     return hipGetLastError();
 }

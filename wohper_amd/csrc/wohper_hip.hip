@@ -305,6 +305,7 @@ struct wh_ctx {
     Scratch attn_max;                       // attn_mx.h: the score tiles' maxima, of a fixed size
     Scratch kv4_part, kv4_ticket;           // the 4-bit cache: partial outputs of split attention, a plan's arrivals
     Scratch rows_counts;                    // expert lists: routes of each expert by chunk
+    Scratch rows_part;                      // 8-bit rows: parts of products whose columns are cut up
     Scratch rows_tickets;                   // 8-bit rows: which tiles of a product are taken
     Scratch layer;                          // the decode layer's state and activations between its steps
     bool exact = true;                      // routed experts in the reference's summation order
@@ -325,7 +326,7 @@ struct wh_ctx {
     hipStream_t base_stream = nullptr, cap_stream = nullptr;
     std::vector<Scratch*> scratch() {
         return {&x_in, &y_out, &h, &ybuf, &cnt_y, &tmp, &batch, &routes, &bout, &gu, &relayout, &rtr, &rtr_cnt,
-                &mla, &hcs, &fp8mm_ws, &fp8mm_cnt, &moe_dyn, &attn_max, &kv4_part, &kv4_ticket, &rows_counts, &rows_tickets, &layer};
+                &mla, &hcs, &fp8mm_ws, &fp8mm_cnt, &moe_dyn, &attn_max, &kv4_part, &kv4_ticket, &rows_counts, &rows_part, &rows_tickets, &layer};
     }
 };
 
@@ -4948,9 +4949,12 @@ int rows_mm_go(wh_ctx* c, const Tensor& t, size_t row_start, wh_rows_mm_args& a,
     a.special = t.special;
     a.odd_scale = t.odd_scale;
     a.tickets = c->rows_tickets.as<uint32_t>();
-    if (!wh_rows_mm_fits(a, bf16 != 0)) return WH_UNSUPPORTED;
+    const wh_rows_mm_plan p = wh_rows_mm_plan_of(a, bf16 != 0);
+    if (!p.fits) return WH_UNSUPPORTED;
     WH_HIP(hipSetDevice(c->device));
-    WH_HIP(wh_rows_mm_launch(a, bf16 != 0, c->stream));
+    WH_HIP(c->rows_part.ensure(p.part_bytes, false));
+    a.part = c->rows_part.as<float>();
+    WH_HIP(wh_rows_mm_launch(a, p, bf16 != 0, c->stream));
     return WH_OK;
 }
 
