@@ -508,7 +508,8 @@ def gpu_near(got, x, w, bf16, cols):
 
 
 @pytest.mark.parametrize("n,rows,cols", [(4096, 4096, 1280), (2048, 4096, 4096), (4100, 2112, 8320), (300, 704, 10240), (5000, 1008, 128),
-                                         (700, 512, 8192), (1024, 32768, 256), (33, 4096, 10240), (100, 16384, 4096)])
+                                         (700, 512, 8192), (1024, 32768, 256), (33, 4096, 10240), (100, 16384, 4096), (4300, 4112, 8576),
+                                         (9000, 4096, 384)])
 @pytest.mark.parametrize("bf16,f32", [(False, False), (False, True), (True, False), (True, True)])
 def test_large_products(ctx, n, rows, cols, bf16, f32):
     c = Large(ctx, n, n, rows, cols, f32)
@@ -522,7 +523,8 @@ def test_large_products(ctx, n, rows, cols, bf16, f32):
 
 
 @pytest.mark.parametrize("n_groups,n,rows,cols", [(64, 6000, 512, 1152), (5, 9000, 1024, 640), (16, 3000, 272, 8448), (300, 2000, 256, 256),
-                                                  (3, 500, 512, 4096), (1024, 3000, 16, 128)])
+                                                  (3, 500, 512, 4096), (1024, 3000, 16, 128), (64, 16000, 4096, 640),
+                                                  (8, 20000, 2048, 1152), (64, 9000, 4096, 2048)])
 @pytest.mark.parametrize("bf16", [False, True])
 def test_large_groups(ctx, n_groups, n, rows, cols, bf16):
     rng = np.random.default_rng(n)
