@@ -443,7 +443,7 @@ __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part
 }
 
 template <bool kBf16, bool kMant>
-__global__ void __launch_bounds__(64 * kThinWaves) k_rows_mm_thin(wh_rows_mm_args a, uint32_t ks_n) {
+__global__ void __launch_bounds__(64 * kThinWaves, 4) k_rows_mm_thin(wh_rows_mm_args a, uint32_t ks_n) {
     __shared__ __align__(16) float part[kThinWaves * 4][64][4];
     const uint32_t g = blockIdx.y, c0 = blockIdx.x * 16 * (kThinWaves / ks_n);
     uint32_t j0 = 0, j1 = a.n;
