@@ -1275,7 +1275,8 @@ wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
     if (rows_mm_matrix(a)) {
         const uint32_t each = 16 * (kThinWaves / rows_thin_split(a.cols));
         const double left = rows - 64 * std::floor(rows / 64);
-        const double chunk = 3.0 * std::floor(rows / 64) + (left == 0 ? 0 : left <= 16 ? 0.95 : left <= 32 ? 1.6 : 3.0);
+        const double chunk = a.n_groups > 1 ? 0.55 + 0.045 * rows
+                                            : 3.0 * std::floor(rows / 64) + (left == 0 ? 0 : left <= 16 ? 0.95 : left <= 32 ? 1.6 : 3.0);
         double best = 3.5 + std::max(1.0, groups * ((a.out_rows + each - 1) / each) / 256) *
                                 std::ceil((double)blocks / rows_thin_split(a.cols)) * chunk;
         p.kind = wh_rows_mm_plan::kThin;
@@ -1299,13 +1300,13 @@ wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
         }
         if (bf16 && !mant) {
             const double half = tiles(128, 256) / 256, tall = (tiles(256, 256) - (a.n_groups == 1 ? 0 : 0.2 * groups * ((a.out_rows + 255) / 256))) / 256;
-            offer(5 + std::max(1.0, half > 1 ? half + 0.25 : half) * (5 + blocks * (0.5 + 0.35 * std::min(1.0, half))),
+            const double uneven = a.n_groups > 1 ? 1.15 : 1.0;
+            offer(uneven * (5 + std::max(1.0, half > 1 ? half + 0.25 : half) * (5 + blocks * (0.5 + 0.35 * std::min(1.0, half)))),
                   wh_rows_mm_plan::kHalf, 1, blocks);
-            offer(4 + std::max(1.0, tall > 1 ? tall + 0.25 : tall) * (9 + blocks * (0.9 + 0.55 * std::min(1.0, tall))),
+            offer(uneven * (4 + std::max(1.0, tall > 1 ? tall + 0.25 : tall) * (9 + blocks * (0.9 + 0.55 * std::min(1.0, tall)))),
                   wh_rows_mm_plan::kTall, 1, blocks);
         }
     }
-    /*force*/
     switch (p.kind) {
         case wh_rows_mm_plan::kAny: p.grid = most(kAnyRows, 16); break;
         case wh_rows_mm_plan::kThin: {
