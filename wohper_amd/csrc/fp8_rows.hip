@@ -36,64 +36,135 @@ __device__ __forceinline__ float rows_scale(uint32_t byte) {
 
 // ------------------------------------------------------------------- rows
 
-// Rows to 8 bits.  Sixteen lanes take a block of 128 columns, lane q the codes
-// of bytes 8 q .. 8 q + 7: columns 16 i + q' with q' = 8 (q % 2) + q / 2, so that
-// each of its eight loads is 16 consecutive columns of the block over the lanes
-// and its store is consecutive bytes.  The scale is the least power of two, 2^-126
-// at least, under which the block's largest finite magnitude is at most 448: from
-// its bits, since 448 is 1.75 * 2^8.  Values times its inverse are exact (or round
-// to code 0), so each code is rounded once, to nearest even.  Infinities and NaN
-// become NaN and do not count for the scale.
+// Bytes [8] of the lanes 2 s + h (s < 8) of a row of 16 as an 8 x 8 matrix each for h = 0
+// and 1, transposed: byte l of lane 2 s + h goes to byte s of lane 2 l + h.  Three
+// exchanges of half of what a lane holds, with the lanes 8, 4 and 2 away.
+__device__ __forceinline__ wh_u2 rows_transpose(wh_u2 v) {
+    const uint32_t lane = threadIdx.x;
+    {
+        const bool hi = lane & 8;
+        const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(hi ? v.x : v.y), 0x128, 0xf, 0xf, false);
+        if (hi) v.x = got;
+        else v.y = got;
+    }
+    {
+        const bool hi = lane & 4;
+        const uint32_t give = __builtin_amdgcn_perm(v.y, v.x, hi ? 0x05040100u : 0x07060302u);
+        const uint32_t got = (uint32_t)__builtin_amdgcn_ds_swizzle((int)give, 0x101f);  // lane ^ 4
+        v = hi ? wh_u2{__builtin_amdgcn_perm(v.x, got, 0x07060100u), __builtin_amdgcn_perm(v.y, got, 0x07060302u)}
+               : wh_u2{__builtin_amdgcn_perm(got, v.x, 0x05040100u), __builtin_amdgcn_perm(got, v.y, 0x07060100u)};
+    }
+    {
+        const bool hi = lane & 2;
+        const uint32_t give = __builtin_amdgcn_perm(v.y, v.x, hi ? 0x06040200u : 0x07050301u);
+        const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0x4e, 0xf, 0xf, false);  // lane ^ 2
+        v = hi ? wh_u2{__builtin_amdgcn_perm(v.x, got, 0x07010500u), __builtin_amdgcn_perm(v.y, got, 0x07030502u)}
+               : wh_u2{__builtin_amdgcn_perm(got, v.x, 0x05020400u), __builtin_amdgcn_perm(got, v.y, 0x07020600u)};
+    }
+    return v;
+}
+
+// Eight values from p on.  Rows may begin at any value: the hardware takes a 16-byte load
+// at any address.
+template <bool kBf16>
+__device__ __forceinline__ void rows_load8(const void* p, uint64_t at, float (&v)[8]) {
+    if constexpr (kBf16) {
+        uint16_t w[8];
+        __builtin_memcpy(w, (const uint16_t*)p + at, sizeof(w));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float((uint32_t)w[i] << 16);
+    } else {
+        __builtin_memcpy(v, (const float*)p + at, sizeof(v));
+    }
+}
+
+// exp(-x), x >= 0 or NaN, within 3 units of 2^-24: a power of two of the product with
+// log2(e) in two pieces, whose rest goes in by the first terms of its series.  The
+// instruction has no results below 2^-126, where expf has.
+__device__ __forceinline__ void rows_exp(const float (&x)[8], float (&z)[8]) {
+    constexpr float kHi = -1.44269502f, kLo = -1.92596299e-8f, kLn2 = 0.693147182f;
+    float most = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) most = fmaxf(most, x[i]);
+    if (most < 87.0f) {  // fmaxf passes over NaN, which both ways keep
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float t = x[i] * kHi, rest = fmaf(x[i], kLo, fmaf(x[i], kHi, -t)), p = __builtin_amdgcn_exp2f(t);
+            z[i] = fmaf(p, rest * kLn2, p);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = expf(-x[i]);
+    }
+}
+
+// Rows to 8 bits.  Sixteen lanes take a block of 128 columns, lane q columns 8 q .. 8 q + 7;
+// their codes change places so that lane q has the store's bytes 8 q .. 8 q + 7.  The scale
+// is the least power of two, 2^-126 at least, under which the block's largest finite
+// magnitude is at most 448: from its bits, since 448 is 1.75 * 2^8.  Values times its
+// inverse are exact (or round to code 0), so each code is rounded once, to nearest even.
+// Infinities and NaN become NaN and do not count for the scale.
+// Bound by memory: 8192 x 4096 in bf16 there and back 41 us (52 with a lane's columns 16
+// apart, which needs no exchange but loads of two bytes), 24001 x 2048 behind SwiGLU there
+// and back 80.6 us, both 4.9 TB/s, the rate of a large copy.
 template <bool kBf16, bool kSwiglu>
 __global__ void __launch_bounds__(256) k_rows_quant(wh_rows_quant_args a) {
     const uint64_t unit = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16;
     const uint32_t q = threadIdx.x & 15;
     const uint64_t row = unit / a.blocks;
     const uint32_t block = (uint32_t)(unit - row * a.blocks);
-    if (row >= a.n) return;
-    const uint64_t at = row * a.x_stride + block * 128u + 8 * (q & 1) + (q >> 1);
-    auto load = [&](const void* p, uint32_t i) {
-        if constexpr (kBf16) return __uint_as_float((uint32_t)((const uint16_t*)p)[at + 16 * i] << 16);
-        else return ((const float*)p)[at + 16 * i];
-    };
+    if (row >= a.n) return;  // all sixteen lanes
+    const uint64_t at = row * a.x_stride + block * 128u + 8 * q;
     float v[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) v[i] = load(a.x, i);
+    rows_load8<kBf16>(a.x, at, v);
     if constexpr (kSwiglu) {
-        float u[8];
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) u[i] = load(a.up, i);
+        float u[8], x[8], z[8];
+        rows_load8<kBf16>(a.up, at, u);
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) {
             // NaN stays NaN through both clamps
-            const float g = v[i] > a.limit ? a.limit : v[i];
-            const float p = u[i] > a.limit ? a.limit : u[i] < -a.limit ? -a.limit : u[i];
-            // from exp(-|g|), which leaves no result behind that f32 has
-            const float z = expf(-fabsf(g));
-            v[i] = g * ((g < 0.0f ? z : 1.0f) / (1.0f + z)) * p;
+            v[i] = v[i] > a.limit ? a.limit : v[i];
+            u[i] = u[i] > a.limit ? a.limit : u[i] < -a.limit ? -a.limit : u[i];
+            x[i] = fabsf(v[i]);
+        }
+        rows_exp(x, z);
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            // 1 / (1 + z), between 1/2 and 1: an estimate within 2^-23 and a step of Newton's
+            const float d = 1.0f + z[i], r = __builtin_amdgcn_rcpf(d), s = fmaf(fmaf(-d, r, 1.0f), r, r);
+            v[i] = v[i] * ((v[i] < 0.0f ? z[i] : 1.0f) * s) * u[i];
         }
     }
     uint32_t top = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-        top = max(top, b < 0x7f800000u ? b : 0);
+    for (uint32_t i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    uint32_t bad = 0;
+    if (top >= 0x7f800000u) {  // these become NaN's code on code 0
+        top = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+            if (b < 0x7f800000u) top = max(top, b);
+            else v[i] = 0.0f, bad |= 1u << i;
+        }
     }
     top = rows_max16(top);
     int e = (int)(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
     e = max(e, -126);
     const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-    uint32_t codes[8];
+    wh_u2 codes;
+    codes.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+    codes.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, (int)codes.x, true);
+    codes.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, 0, false);
+    codes.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, (int)codes.y, true);
+    if (bad) {
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        const bool finite = (__float_as_uint(v[i]) & 0x7fffffffu) < 0x7f800000u;
-        const uint32_t c = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(finite ? v[i] * inv : 0.0f, 0.0f, 0, false) & 0xffu;
-        codes[i] = finite ? c : 0x7fu;
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (bad >> i & 1) codes.x |= 0x7fu << 8 * i;
+            if (bad >> (4 + i) & 1) codes.y |= 0x7fu << 8 * i;
+        }
     }
-    wh_u2 out;
-    out.x = codes[0] | codes[1] << 8 | codes[2] << 16 | codes[3] << 24;
-    out.y = codes[4] | codes[5] << 8 | codes[6] << 16 | codes[7] << 24;
-    *(wh_u2*)(a.out.codes + row * a.out.stride + block * 128u + 8 * q) = out;
+    *(wh_u2*)(a.out.codes + row * a.out.stride + block * 128u + 8 * q) = rows_transpose(codes);
     if (q == 0) a.out.scales[row * a.out.scale_stride + block] = top ? (uint8_t)(e + 127) : 0;
 }
 
@@ -104,20 +175,22 @@ __global__ void __launch_bounds__(256) k_rows_read(wh_rows_read_args a) {
     const uint32_t q = threadIdx.x & 15;
     const uint64_t row = unit / a.blocks;
     const uint32_t block = (uint32_t)(unit - row * a.blocks);
-    if (row >= a.n) return;
-    const wh_u2 codes = *(const wh_u2*)(a.in.codes + row * a.in.stride + block * 128u + 8 * q);
+    if (row >= a.n) return;  // all sixteen lanes
+    const wh_u2 codes = rows_transpose(*(const wh_u2*)(a.in.codes + row * a.in.stride + block * 128u + 8 * q));
     const float scale = rows_scale(a.in.scales[row * a.in.scale_stride + block]);
-    const uint64_t at = row * a.out_stride + block * 128u + 8 * (q & 1) + (q >> 1);
+    const uint64_t at = row * a.out_stride + block * 128u + 8 * q;
+    const wh_f2 p[4] = {wh_fp8x2<false, false>(codes.x), wh_fp8x2<false, true>(codes.x), wh_fp8x2<false, false>(codes.y),
+                        wh_fp8x2<false, true>(codes.y)};
+    if constexpr (kBf16) {
+        __bf16 o[8];
 #pragma unroll
-    for (uint32_t h = 0; h < 4; ++h) {
-        const uint32_t w = h < 2 ? codes.x : codes.y;
-        const wh_f2 v = h & 1 ? wh_fp8x2<false, true>(w) : wh_fp8x2<false, false>(w);
+        for (int i = 0; i < 8; ++i) o[i] = (__bf16)((i & 1 ? p[i / 2].y : p[i / 2].x) * scale);
+        __builtin_memcpy((__bf16*)a.out + at, o, sizeof(o));
+    } else {
+        float o[8];
 #pragma unroll
-        for (uint32_t j = 0; j < 2; ++j) {
-            const float x = (j ? v.y : v.x) * scale;
-            if constexpr (kBf16) ((__bf16*)a.out)[at + 16 * (2 * h + j)] = (__bf16)x;
-            else ((float*)a.out)[at + 16 * (2 * h + j)] = x;
-        }
+        for (int i = 0; i < 8; ++i) o[i] = (i & 1 ? p[i / 2].y : p[i / 2].x) * scale;
+        __builtin_memcpy((float*)a.out + at, o, sizeof(o));
     }
 }
 
@@ -1253,8 +1326,10 @@ hipError_t wh_rows_read_launch(const wh_rows_read_args& a, bool bf16, hipStream_
 // of these estimates of its time in us, fitted to 400 measured calls (one MI355X; 1 to
 // 4096 rows, 1 to 64 groups, weights from 1408 x 512 to 32768 x 1024 and 4096 x 8192).
 //  - thin: a wave's block of columns takes 0.95, 1.6 and 3 us for up to 16, 32 and 64
-//    rows, workgroups in rounds of 256: 4096 x 4096 with 16, 64 and 128 rows 7.7, 15.6 and
-//    29, where tiles take 23 to 25, cut up 13 to 18;
+//    rows (with groups of uneven lists 0.55 and 0.045 a row), workgroups in rounds of 256:
+//    4096 x 4096 with 16, 64 and 128 rows 7.7, 15.6 and 29, where tiles take 23 to 25, cut
+//    up 13 to 18; 64 groups with 4, 16 and 32 rows each in f32 228, 343 and 505, tiles 281,
+//    299 and 309;
 //  - tile: a block 0.56 us in bf16 (0.95 with factors of scales), 1.1 in f32, in rounds of
 //    256 workgroups; ranges divide that and add a launch and their parts' bytes: 4096 x
 //    4096 with 128 rows in 1, 2 and 4 ranges 24.6, 19.9 and 18.1, with 1024 27, 34 and 48;
