@@ -1122,8 +1122,9 @@ __global__ void __launch_bounds__(256) k_rows_scales(const uint8_t* scales, uint
 // ------------------------------------------------------------ expert lists
 
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-constexpr uint32_t kPlanChunk = 4096;                      // routes of a workgroup
-constexpr uint32_t kPlanPerWave = kPlanChunk / kPlanWaves;  // consecutive ones of a wave
+
+// Routes of a workgroup, a chunk: a wave takes `turns` times 64 consecutive ones.
+__host__ __device__ constexpr uint32_t plan_chunk(uint32_t turns) { return kPlanThreads * turns; }
 
 // What a wave's lanes have stored to LDS is there for its other lanes.
 __device__ __forceinline__ void plan_wave_sync() {
@@ -1144,11 +1145,11 @@ __device__ __forceinline__ uint64_t plan_same(uint32_t id, uint32_t bits) {
 }
 
 // How many routes of each expert a chunk has.
-__global__ void __launch_bounds__(kPlanThreads) k_expert_count(wh_expert_plan_args a) {
+__global__ void __launch_bounds__(kPlanThreads) k_expert_count(wh_expert_plan_args a, uint32_t chunk) {
     __shared__ uint32_t count[WH_ROWS_MAX_GROUPS];
     for (uint32_t e = threadIdx.x; e < a.n_groups; e += kPlanThreads) count[e] = 0;
     __syncthreads();
-    const uint32_t from = blockIdx.x * kPlanChunk, to = min(a.n, from + kPlanChunk);
+    const uint32_t from = blockIdx.x * chunk, to = min(a.n, from + chunk);
     for (uint32_t i = from + threadIdx.x; i < to; i += kPlanThreads) {
         const uint32_t id = a.ids[i];
         if (id < a.n_groups) atomicAdd(&count[id], 1u);
@@ -1157,25 +1158,47 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_count(wh_expert_plan_ar
     for (uint32_t e = threadIdx.x; e < a.n_groups; e += kPlanThreads) a.counts[(uint64_t)blockIdx.x * a.n_groups + e] = count[e];
 }
 
-// Expert lists: a counting sort that keeps the order of routes.  A workgroup
-// takes 4096 routes, a wave 256 consecutive ones 64 at a time; lanes of the same
-// expert find each other by ballots over the id's bits, so a route's place is
-// the expert's start, its routes of chunks and waves before, of this wave so far,
-// and of lanes before.  With one chunk this is the only launch.
+// Expert lists: a counting sort that keeps the order of routes.  A workgroup takes a
+// chunk of routes, a wave consecutive ones 64 at a time; lanes of the same expert find
+// each other by ballots over the id's bits, so a route's place is the expert's start, its
+// routes of chunks and waves before, of this wave so far, and of lanes before.  With one
+// chunk this is the only launch.
+template <uint32_t kTurns>
 __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_args a, uint32_t chunks, uint32_t bits) {
     extern __shared__ uint32_t lds[];
     uint32_t* const at = lds;  // [kPlanWaves][n_groups]: counts, then next places of a wave
-    __shared__ uint32_t wave_sum[kPlanWaves];
+    __shared__ uint32_t wave_sum[kPlanWaves], all_of[WH_ROWS_MAX_GROUPS], before_of[WH_ROWS_MAX_GROUPS];
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, E = a.n_groups;
     for (uint32_t i = t; i < kPlanWaves * E; i += kPlanThreads) at[i] = 0;
-    __syncthreads();
-    const uint32_t from = blockIdx.x * kPlanChunk + wave * kPlanPerWave;
-    uint32_t id[kPlanPerWave / 64];
-    uint64_t same[kPlanPerWave / 64];
+    if (t < E) all_of[t] = before_of[t] = 0;
+    const uint32_t from = blockIdx.x * plan_chunk(kTurns) + wave * 64 * kTurns;
+    uint32_t id[kTurns];
+    uint64_t same[kTurns];
 #pragma unroll
-    for (uint32_t k = 0; k < kPlanPerWave / 64; ++k) {
+    for (uint32_t k = 0; k < kTurns; ++k) {
         const uint32_t i = from + 64 * k + lane;
         id[k] = i < a.n ? a.ids[i] : kNone;
+    }
+    __syncthreads();
+    // all chunks' routes of expert e and those before this chunk, a range of chunks a thread
+    if (chunks > 1) {
+        uint32_t shift = 6;
+        while (1u << shift < E) ++shift;
+        const uint32_t e = t & ((1u << shift) - 1), parts = kPlanThreads >> shift;
+        if (e < E) {
+            uint32_t all = 0, before = 0;
+#pragma unroll 8
+            for (uint32_t c = t >> shift; c < chunks; c += parts) {
+                const uint32_t v = a.counts[(uint64_t)c * E + e];
+                before += c < blockIdx.x ? v : 0;
+                all += v;
+            }
+            if (all) atomicAdd(&all_of[e], all);
+            if (before) atomicAdd(&before_of[e], before);
+        }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kTurns; ++k) {
         if (id[k] >= E) id[k] = E;  // no expert: a number of its own, E < 2^bits
         same[k] = plan_same(id[k], bits);
         const bool leads = __builtin_ctzll(same[k]) == lane;
@@ -1183,17 +1206,13 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_ar
         plan_wave_sync();
     }
     __syncthreads();
-    // this chunk's and all chunks' routes of expert t, those before this chunk
     uint32_t all = 0, before = 0;
     if (t < E) {
         if (chunks == 1) {
             for (uint32_t w = 0; w < kPlanWaves; ++w) all += at[w * E + t];
         } else {
-            for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t v = a.counts[(uint64_t)c * E + t];
-                before += c < blockIdx.x ? v : 0;
-                all += v;
-            }
+            all = all_of[t];
+            before = before_of[t];
         }
     }
     uint32_t upto = all;
@@ -1223,7 +1242,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_ar
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t k = 0; k < kPlanPerWave / 64; ++k) {
+    for (uint32_t k = 0; k < kTurns; ++k) {
         const uint32_t i = from + 64 * k + lane;
         const bool some = id[k] < E;
         uint32_t place = kNone;
@@ -1285,11 +1304,12 @@ hipError_t wh_rows_setup() {
     if (hipGetDevice(&device) == hipSuccess &&
         hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) == hipSuccess && cus >= 8)
         g_workgroups = (uint32_t)cus / 8 * 8;
-    hipError_t e = hipFuncSetAttribute((const void*)k_expert_place, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)plan_lds(WH_ROWS_MAX_GROUPS));
+    hipError_t e = hipSuccess;
     auto tile = [&](const void* f, size_t lds) {
         if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     };
+    tile((const void*)k_expert_place<1>, plan_lds(WH_ROWS_MAX_GROUPS));
+    tile((const void*)k_expert_place<4>, plan_lds(WH_ROWS_MAX_GROUPS));
     constexpr size_t lds = rows_tile_shape<4, 4, 2, 2>::kLds;
     tile((const void*)k_rows_mm_tile<true, true>, lds);
     tile((const void*)k_rows_mm_tile<true, false>, lds);
@@ -1469,21 +1489,30 @@ hipError_t wh_rows_scales_launch(const uint8_t* scales, uint64_t n, uint32_t* fl
     return hipSuccess;
 }
 
+// How many times 64 routes a wave takes.  Once: 96 routes 3.6 us (four times: 5.4), 12000
+// over 256 experts 7.4 (9.8).  Four times where that saves the first launch, 1800 routes
+// 5.9 us (6.4), and where every workgroup would sum the counts of many chunks: 98304 routes
+// over 256 experts 12.0 us (13.1), 1048576 30.8 (126).
+static uint32_t plan_turns(size_t n, size_t n_groups) {
+    return n > plan_chunk(1) && (n <= plan_chunk(4) || n * std::max<size_t>(n_groups, 64) > 1u << 24) ? 4 : 1;
+}
+
 size_t wh_expert_plan_scratch(size_t n, size_t n_groups) {
-    const size_t chunks = (n + kPlanChunk - 1) / kPlanChunk;
+    const size_t chunk = plan_chunk(plan_turns(n, n_groups)), chunks = (n + chunk - 1) / chunk;
     return chunks > 1 ? chunks * n_groups * sizeof(uint32_t) : 0;
 }
 
 hipError_t wh_expert_plan_launch(const wh_expert_plan_args& a, hipStream_t stream) {
-    const uint32_t chunks = std::max(1u, (a.n + kPlanChunk - 1) / kPlanChunk);
+    const uint32_t turns = plan_turns(a.n, a.n_groups), chunk = plan_chunk(turns), chunks = std::max(1u, (a.n + chunk - 1) / chunk);
     uint32_t bits = 1;
     while ((a.n_groups >> bits) != 0) ++bits;
     if (chunks > 1) {
-        k_expert_count<<<chunks, kPlanThreads, 0, stream>>>(a);
+        k_expert_count<<<chunks, kPlanThreads, 0, stream>>>(a, chunk);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    k_expert_place<<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
+    if (turns > 1) k_expert_place<4><<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
+    else k_expert_place<1><<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
     return hipGetLastError();
 }
 
