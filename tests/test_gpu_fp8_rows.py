@@ -12,6 +12,8 @@ Tolerances, u = 2^-24 a rounding to f32, S = sum |w||x| of an output:
   largest and keep 13 bits under it, so that seven lose 7 * 2^-13 of the
   largest, at most 2^-10 S; then half a step of bf16, 2^-8;
   a weighted sum of k rows: (k + 2) u of sum |w||y|."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -824,6 +826,169 @@ def test_a_captured_layer_step_serves_other_routes(ctx):
     for g in graphs:
         ctx.graph_release(g)
     layer.close()
+
+
+def test_graphs_of_products_share_workspaces(ctx):
+    """Graphs whose products use parts of ranges and counters of tiles, replayed in turn
+    with eager products of other sizes between."""
+    sizes = [(128, 4096, 4096, True), (3000, 1024, 1024, True), (70, 1024, 2048, False), (1500, 4096, 512, True)]
+    calls = []
+    for i, (n, rows, cols, bf16) in enumerate(sizes):
+        c = Large(ctx, i, n, rows, cols, False)
+        y = torch.empty(n, rows, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+        calls.append((c, y, lambda c=c, y=y, n=n, rows=rows, bf16=bf16:
+                      ctx.fp8_rows_mm_async(c.h, 0, rows, c.rows.c, n, y.data_ptr(), rows, bf16)))
+    want = []
+    for c, y, f in calls:
+        f()
+        ctx.synchronize()
+        gpu_near(y, c.x, c.w, y.dtype == torch.bfloat16, c.cols)
+        want.append(y.clone())
+    graphs = [ctx.capture(lambda a=a, b=b: (calls[a][2](), calls[b][2]())) for a, b in ((0, 1), (2, 3), (1, 2))]
+    for turn in range(6):
+        for y in (y for _, y, _ in calls):
+            y.fill_(7.0)
+        torch.cuda.synchronize()
+        for g in graphs:
+            ctx.graph_launch(g)
+        calls[turn % 4][2]()
+        ctx.graph_launch(graphs[turn % 3])
+        ctx.synchronize()
+        assert all(torch.equal(y, w) for (_, y, _), w in zip(calls, want))
+    for g in graphs:
+        ctx.graph_release(g)
+    for c, _, _ in calls:
+        ctx.release(c.h)
+
+
+def test_two_contexts_at_once(ctx):
+    other = wa.Context(0)
+    jobs = []
+    for i, k in enumerate((ctx.raw, other)):
+        c = Large(k, i, 1500, 2048, 1024, False)
+        torch.cuda.synchronize()
+        jobs.append((k, c, [torch.zeros(1500, 2048, dtype=torch.bfloat16, device="cuda") for _ in range(30)]))
+    torch.cuda.synchronize()
+
+    def run(k, c, ys):
+        for y in ys:
+            k.fp8_rows_mm_async(c.h, 0, 2048, c.rows.c, 1500, y.data_ptr(), 2048, True)
+        k.synchronize()
+
+    threads = [threading.Thread(target=run, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k, c, ys in jobs:
+        gpu_near(ys[0], c.x, c.w, True, 1024)
+        assert all(torch.equal(y, ys[0]) for y in ys)
+        k.release(c.h)
+    other.close()
+
+
+# Offsets past 32 bits: three x rows 2^31 bytes apart, y rows over 3 * 2^31 values, a
+# weight of more than 2^32 codes.
+
+@pytest.mark.parametrize("n,special", [(3, False), (100, False), (2048, False), (20, True)])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_products_of_rows_far_apart(ctx, n, special, bf16):
+    rng = np.random.default_rng(n)
+    w = Weight(ctx, rng, 2048, 640, special=special)
+    rows, x = random_rows(rng, 3, 640)
+    far = 1 << 31
+    codes = torch.empty(2 * far + 640, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(2 * far + 8, dtype=torch.uint8, device="cuda")
+    for i in range(3):
+        codes[i * far:i * far + 640] = rows.codes[i]
+        scales[i * far:i * far + 5] = rows.scales[i, :5]
+    at = rng.integers(0, 3, n)
+    at[-1] = 2
+    stride = 3 * far // n // 8 * 8
+    y = torch.empty((n - 1) * stride + 1024, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    x8 = wa.WhFp8Rows(codes.data_ptr(), far, scales.data_ptr(), far)
+    starts = [0, n // 3, n]
+    r, s = i32(at), i32(starts)
+    ctx.fp8_rows_mm_groups_async(w.h, 0, 1024, 2, x8, 3, r.data_ptr(), s.data_ptr(), n, y.data_ptr(), stride, bf16)
+    ctx.synchronize()
+    got = f64(torch.as_strided(y, (n, 1024), (stride, 1)))
+    for g in range(2):
+        a, b = starts[g], starts[g + 1]
+        near(got[a:b], x[at[a:b]], w.values[g * 1024:(g + 1) * 1024], bf16, 640)
+    w.close()
+
+
+def test_products_with_a_weight_past_32_bits(ctx):
+    rows, cols = 1052672, 4096  # 257 groups of 4096
+    base = torch.from_numpy(quantise(np.random.default_rng(0).standard_normal((64, cols)) * 110)[0]).cuda()
+    codes = base.repeat(rows // 64, 1)
+    codes[-4096:] = base.flip(0).repeat(64, 1)
+    scales = torch.full((rows // 128, cols // 128), 120, dtype=torch.uint8, device="cuda")
+    scales[-32:] = 121
+    torch.cuda.synchronize()
+    h = ctx.store_fp8_device(codes.data_ptr(), rows, cols, scales.data_ptr(), *scales.shape)
+    v = gpu_values(codes[-4096:], torch.exp2(scales[-32:].double() - 127), 128)
+    del codes
+    g = torch.Generator(device="cuda")
+    for n in (4, 90, 700, 2500):
+        x = torch.randn(n, cols, generator=g, device="cuda")
+        x8 = Rows(n, cols)
+        ctx.fp8_quant_rows_async(x.data_ptr(), cols, False, n, cols, x8.c)
+        back = torch.empty(n, cols, device="cuda")
+        ctx.fp8_read_rows_async(x8.c, n, cols, back.data_ptr(), cols, False)
+        starts = i32([0] * 257 + [n])
+        for bf16 in (False, True):
+            for groups in (1, 257):
+                y = torch.zeros(n, 4096, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+                if groups == 1:
+                    ctx.fp8_rows_mm_async(h, rows - 4096, rows, x8.c, n, y.data_ptr(), 4096, bf16)
+                else:
+                    ctx.fp8_rows_mm_groups_async(h, 0, 4096, 257, x8.c, n, None, starts.data_ptr(), n, y.data_ptr(), 4096,
+                                                 bf16)
+                ctx.synchronize()
+                gpu_near(y, back.double(), v, bf16, cols)
+    ctx.release(h)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_rows_and_sums_far_apart(ctx, bf16):
+    rng = np.random.default_rng(4)
+    far, cols = 1 << 31, 256
+    dtype = torch.bfloat16 if bf16 else torch.float32
+    x = torch.empty(2 * far + 2 * cols, dtype=dtype, device="cuda")
+    v = dev(some(rng, 3, 2 * cols)).to(dtype)
+    codes = torch.empty(2 * far + cols, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(2 * far + 4, dtype=torch.uint8, device="cuda")
+    near_rows, near_glu = Rows(3, cols), Rows(3, cols)
+    c = wa.WhFp8Rows(codes.data_ptr(), far, scales.data_ptr(), far)
+    for i in range(3):
+        x[i * far:i * far + 2 * cols] = v[i]
+    up = cols * x.element_size()
+
+    def same(a):
+        return all(torch.equal(codes[i * far:i * far + cols], a.codes[i])
+                   and torch.equal(scales[i * far:i * far + 2], a.scales[i, :2]) for i in range(3))
+
+    ctx.fp8_quant_rows_async(v.data_ptr(), 2 * cols, bf16, 3, cols, near_rows.c)
+    ctx.fp8_swiglu_rows_async(v.data_ptr(), v.data_ptr() + up, 2 * cols, bf16, 3, cols, 10.0, near_glu.c)
+    ctx.fp8_swiglu_rows_async(x.data_ptr(), x.data_ptr() + up, far, bf16, 3, cols, 10.0, c)
+    ctx.synchronize()
+    assert same(near_glu)
+    ctx.fp8_quant_rows_async(x.data_ptr(), far, bf16, 3, cols, c)
+    ctx.synchronize()
+    assert same(near_rows)
+    back = torch.empty(3, cols, dtype=dtype, device="cuda")
+    ctx.fp8_read_rows_async(near_rows.c, 3, cols, back.data_ptr(), cols, bf16)
+    x.zero_()
+    ctx.fp8_read_rows_async(c, 3, cols, x.data_ptr(), far, bf16)
+    ctx.synchronize()
+    assert torch.equal(torch.as_strided(x, (3, cols), (far, 1)), back)
+    slots, w = i32([[2], [0], [1]]), torch.ones(3, 1, device="cuda")
+    out = torch.zeros(2 * far + cols, device="cuda")
+    ctx.expert_combine_async(x.data_ptr(), far, bf16, 3, slots.data_ptr(), w.data_ptr(), 3, 1, cols, out.data_ptr(), far,
+                             out.data_ptr(), far)
+    ctx.synchronize()
+    assert torch.equal(torch.as_strided(out, (3, cols), (far, 1)), back.float()[[2, 0, 1]])
 
 
 def test_calls_repeat_bit_for_bit(ctx):

@@ -10,6 +10,7 @@
 #include "fp8_rows.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "wh_device.h"
@@ -1297,7 +1298,7 @@ constexpr uint64_t kMaxGrid256 = 0xffffffull;
 
 constexpr size_t plan_lds(uint32_t n_groups) { return kPlanWaves * (size_t)n_groups * sizeof(uint32_t); }
 
-uint32_t g_workgroups = 256;  // a multiple of 8, one a CU
+std::atomic<uint32_t> g_workgroups{256};  // a multiple of 8, one a CU: devices of one machine are alike
 
 hipError_t wh_rows_setup() {
     int device = 0, cus = 0;
@@ -1411,8 +1412,8 @@ wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
             break;
         }
         case wh_rows_mm_plan::kTile: p.grid = (most(128, 128) + 7) / 8 * 8; break;
-        case wh_rows_mm_plan::kHalf: p.grid = std::min<uint64_t>((most(128, 256) + 7) / 8 * 8, g_workgroups); break;
-        case wh_rows_mm_plan::kTall: p.grid = std::min<uint64_t>((most(256, 256) + 7) / 8 * 8, g_workgroups); break;
+        case wh_rows_mm_plan::kHalf: p.grid = std::min<uint64_t>((most(128, 256) + 7) / 8 * 8, g_workgroups.load()); break;
+        case wh_rows_mm_plan::kTall: p.grid = std::min<uint64_t>((most(256, 256) + 7) / 8 * 8, g_workgroups.load()); break;
     }
     if (p.splits > 1) p.part_bytes = (size_t)p.splits * a.n * rows_part_stride(a) * sizeof(float);
     p.fits = p.grid * p.threads * p.splits <= 0xffffffffull;  // a grid's threads
