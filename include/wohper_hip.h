@@ -991,7 +991,8 @@ typedef struct {
  * finite magnitude is at most 448, and each value the nearest code, ties to
  * even; infinities and NaN become NaN.  The swiglu form rounds silu(min(gate,
  * limit)) * clamp(up, -limit, limit), in f32 (E/deepseek_v4.rs:590-594 with
- * limit 10; INFINITY: no clamp); a product beyond f32 becomes NaN. */
+ * limit 10; INFINITY: no clamp); a product beyond f32 becomes NaN.  Inputs may
+ * begin at any value; out overlaps none of them. */
 int wh_fp8_quant_rows_async(wh_ctx* ctx, const void* x_dev, size_t x_stride, int is_bf16, size_t n, size_t cols,
                             const wh_fp8_rows* out);
 int wh_fp8_swiglu_rows_async(wh_ctx* ctx, const void* gate_dev, const void* up_dev, size_t stride, int is_bf16, size_t n,
@@ -1002,23 +1003,28 @@ int wh_fp8_read_rows_async(wh_ctx* ctx, const wh_fp8_rows* rows, size_t n, size_
 
 /* y row i = rows [row_start, row_end) of w times x row i, f32 or bf16
  * (is_bf16), for n rows of w's columns.  w: an FP8 tensor of 128-column scale
- * groups.  Products of codes are exact; a block's sum times both scales, and the
- * sum over blocks, are f32 in any order, in both numerics modes: within
- * 1e-6 * sqrt(cols) * ||w_row||_2 * ||x_i||_2, then rounded once to bf16.  A NaN
- * in an x row makes its y row NaN and no other.  Weight codes 0x7F / 0xFF are
- * +-480 and UE8M0 bytes 0 and 255 are 0.0 and infinity, as in every product
- * here; tensors with such codes, and ranges or scale rows that are no multiples
- * of 16 rows, take a kernel without matrix instructions, many times as long.
- * y must not overlap x. */
+ * groups.  Products of codes are exact, sums are f32 in any order, in both
+ * numerics modes.  f32 results are within (cols + 8) * 2^-24 * sum |w| |x|.
+ * bf16 results come from 8-bit matrix instructions, which align eight products
+ * to the largest of them and keep 13 bits under it: at most 2^-10 * sum |w| |x|,
+ * usually 2e-5 to 6e-5 of the result's norm, before they are rounded once.  The
+ * order of a sum follows from the sizes (n, n_groups and the tensor's), so a row
+ * may differ by f32's rounding between calls of other sizes; a call repeats bit
+ * for bit.  A NaN in an x row makes its y row NaN and no other.  Weight codes
+ * 0x7F / 0xFF are +-480 and UE8M0 bytes 0 and 255 are 0.0 and infinity, as in
+ * every product here.  Tensors with such codes, and ranges or scale rows that
+ * are no multiples of 16 rows, take a kernel without matrix instructions, many
+ * times as long.  y must not overlap x.  Some sizes use memory of the context
+ * that grows: before a capture, run the call once (wh_graph_begin). */
 int wh_fp8_rows_mm_async(wh_ctx* ctx, wh_tensor w, size_t row_start, size_t row_end, const wh_fp8_rows* x, size_t n,
                          void* y_dev, size_t y_stride, int is_bf16);
 
 /* The same grouped by expert: y row j, starts_dev[g] <= j < starts_dev[g + 1],
  * is x row rows_dev[j] (NULL: j) times w's rows row_start + g * group_rows +
- * [0, group_rows).  starts_dev [n_groups + 1] ascends (not checked; groups that
- * overlap leave either one's result) and is cut off at n, the rows of y;
- * y rows in no group are left as they are.  rows_dev [n] entries of n_x or more
- * are no row: their y rows are 0.  At most 1024 groups. */
+ * [0, group_rows).  starts_dev [n_groups + 1] ascends (not checked: else the n
+ * rows of y are undefined) and is cut off at n; y rows in no group are left as
+ * they are.  rows_dev [n] entries of n_x or more are no row: their y rows are 0.
+ * The same row may be listed any number of times.  At most 1024 groups. */
 int wh_fp8_rows_mm_groups_async(wh_ctx* ctx, wh_tensor w, size_t row_start, size_t group_rows, size_t n_groups,
                                 const wh_fp8_rows* x, size_t n_x, const uint32_t* rows_dev, const uint32_t* starts_dev,
                                 size_t n, void* y_dev, size_t y_stride, int is_bf16);
@@ -1029,7 +1035,8 @@ int wh_fp8_rows_mm_groups_async(wh_ctx* ctx, wh_tensor w, size_t row_start, size
  * routes in order; rows_dev [npos * topk] gets each listed route's position
  * and 0xFFFFFFFF behind the last list, slots_dev [npos][topk] each route's
  * place in the lists or 0xFFFFFFFF.  At most 1024 experts; outputs overlap
- * neither each other nor ids_dev. */
+ * neither each other nor ids_dev.  Above 1024 routes it uses memory of the
+ * context that grows: before a capture, run the call once. */
 int wh_expert_plan_async(wh_ctx* ctx, const uint32_t* ids_dev, size_t npos, size_t topk, size_t n_experts,
                          uint32_t* starts_dev, uint32_t* rows_dev, uint32_t* slots_dev);
 
@@ -1037,7 +1044,8 @@ int wh_expert_plan_async(wh_ctx* ctx, const uint32_t* ids_dev, size_t npos, size
  * in the order of k, plus add row p (add_dev NULL: none; the shared expert's, it
  * may be out).  Slots of n_rows or more are passed over, whatever their weight; a
  * position of no slots gets 0 or its add row.  y is f32 or bf16; hidden and all
- * strides are multiples of 4 values, rows aligned to 4 values. */
+ * strides are multiples of 4 values, rows aligned to 4 values.  out overlaps
+ * neither y nor, unless it is add with add's stride, add. */
 int wh_expert_combine_async(wh_ctx* ctx, const void* y_dev, size_t y_stride, int is_bf16, size_t n_rows,
                             const uint32_t* slots_dev, const float* weights_dev, size_t npos, size_t topk, size_t hidden,
                             const float* add_dev, size_t add_stride, float* out_dev, size_t out_stride);
