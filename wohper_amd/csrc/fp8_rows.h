@@ -54,7 +54,6 @@ struct wh_rows_mm_args {
     uint32_t odd_scale;  // UE8M0 scale bytes 0 or 255 are there
     float* part;         // the plan's part_bytes
     uint32_t* tickets;   // [WH_ROWS_TICKETS], 0 between launches
-    uint32_t y_vec;      // y takes stores of four values (1), of 16 bytes (2)
 };
 // How a product is done: by sizes that the host knows.
 struct wh_rows_mm_plan {

@@ -386,14 +386,15 @@ __device__ __forceinline__ uint32_t rows_split_scale(const wh_rows_mm_args& a, u
     return e;
 }
 
+// Four values to any address: the hardware takes stores of 8 and 16 bytes there.
 template <bool kBf16>
 __device__ __forceinline__ void rows_put4(const wh_rows_mm_args& a, uint64_t row, uint32_t col, wh_f4 v) {
-    if (a.y_vec && col + 4 <= a.out_rows) {
+    if (col + 4 <= a.out_rows) {
         if constexpr (kBf16) {
-            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-            *(b4*)((__bf16*)a.y + row * a.y_stride + col) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+            const __bf16 b[4] = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+            __builtin_memcpy((__bf16*)a.y + row * a.y_stride + col, b, sizeof(b));
         } else {
-            *(wh_f4*)((float*)a.y + row * a.y_stride + col) = v;
+            __builtin_memcpy((float*)a.y + row * a.y_stride + col, &v, sizeof(v));
         }
         return;
     }
@@ -413,8 +414,8 @@ __device__ __forceinline__ uint32_t rows_source(const wh_rows_mm_args& a, uint32
 // every kS-th block of their columns for up to 16 kMt x rows, straight from memory
 // into registers; the kS waves of the same weight rows join in LDS.  Blocks come
 // kU at a time, all their loads before the first product.  Registers for two workgroups
-// a CU: 96 rows over 64 lists of 4096 x 4096 in f32 158 us (with one 226), which reads the
-// weights at 6.8 TB/s; 5 x 4096 x 8192 in f32 9.4 us, 3.6 TB/s with the launch.
+// a CU: 84 rows over 64 lists of 4096 x 4096, 43 of them not empty, in f32 158 us (with one
+// 226), 4.6 TB/s; 5 x 4096 x 8192 in f32 9.4 us, 3.6 TB/s with the launch.
 constexpr uint32_t kThinWaves = 8;
 template <int kMt, bool kBf16, bool kMant>
 __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part)[64][4], uint32_t ks_n, uint32_t g, uint32_t j0,
@@ -1022,8 +1023,8 @@ __device__ __forceinline__ void rows_big(const wh_rows_mm_args& a, uint8_t* lds,
         if (a.rows) rows_source(a, j, &is);
         if (!is) v = wh_u4{0, 0, 0, 0};
         uint16_t* const to = (uint16_t*)a.y + (uint64_t)j * a.y_stride + col;
-        if (a.y_vec == 2 && col + 8 <= a.out_rows) {
-            *(wh_u4*)to = v;
+        if (col + 8 <= a.out_rows) {
+            __builtin_memcpy(to, &v, sizeof(v));
         } else {
             for (uint32_t e = 0; e < 8 && col + e < a.out_rows; ++e) to[e] = (uint16_t)(v[e / 2] >> 16 * (e & 1));
         }

@@ -4935,8 +4935,6 @@ int rows_mm_args(const wh_fp8_rows* x, size_t n_x, const uint32_t* rows, const u
     a->n_groups = (uint32_t)n_groups;
     a->out_rows = (uint32_t)out_rows;
     a->cols = (uint32_t)cols;
-    if (y_stride % 4 == 0 && ((uintptr_t)y & (bf16 ? 7 : 15)) == 0)
-        a->y_vec = y_stride % (bf16 ? 8 : 4) == 0 && ((uintptr_t)y & 15) == 0 ? 2 : 1;
     return WH_OK;
 }
 
