@@ -1117,18 +1117,15 @@ uint64_t rows_tiles(const wh_rows_mm_args& a, uint32_t rows) {
 __global__ void __launch_bounds__(256) k_rows_store(const uint8_t* in, uint8_t* out, uint64_t blocks, uint32_t* flags) {
     const uint64_t unit = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16;
     const uint32_t q = threadIdx.x & 15;
-    if (unit >= blocks) return;
-    const uint8_t* const p = in + unit * 128 + 8 * (q & 1) + (q >> 1);
-    uint32_t c[8], special = 0;
+    if (unit >= blocks) return;  // all sixteen lanes
+    uint8_t c[8];
+    __builtin_memcpy(c, in + unit * 128 + 8 * q, sizeof(c));
+    uint32_t special = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        c[i] = p[16 * i];
-        special |= (c[i] & 0x7fu) == 0x7fu;
-    }
-    wh_u2 o;
-    o.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-    o.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-    *(wh_u2*)(out + unit * 128 + 8 * q) = o;
+    for (uint32_t i = 0; i < 8; ++i) special |= (c[i] & 0x7fu) == 0x7fu;
+    wh_u2 v;
+    __builtin_memcpy(&v, c, sizeof(v));
+    *(wh_u2*)(out + unit * 128 + 8 * q) = rows_transpose(v);
     if (special) atomicOr(flags, 1u);
 }
 
