@@ -579,24 +579,33 @@ constexpr uint32_t kBand = 8;
 template <uint32_t kM, uint32_t kN>
 struct rows_tiling {
     const wh_rows_mm_args& a;
-    uint32_t n_tiles;    // of columns
+    uint32_t n_tiles;     // of columns
     uint64_t total, per;  // tiles, and of them an XCD's
+    struct lane_group {
+        uint32_t s, e, tiles, upto;  // rows [s, e), their tiles, and all tiles up to it of these 64 groups
+    };
 
-    // Tiles of rows of the group at, and its rows.  64 bits over groups: starts that do
-    // not ascend may count rows more than once.
-    __device__ __forceinline__ uint32_t group(uint32_t at, uint32_t& s, uint32_t& e) const {
-        s = e = 0;
+    // This lane's group of the 64 from base on.  64 bits over all groups: starts that do not
+    // ascend may count rows more than once.
+    __device__ __forceinline__ lane_group groups(uint32_t base) const {
+        const uint32_t lane = threadIdx.x & 63, at = base + lane;
+        lane_group l = {0, 0, 0, 0};
         if (at < a.n_groups) {
-            s = a.starts ? min(a.starts[at], a.n) : 0;
-            e = a.starts ? max(s, min(a.starts[at + 1], a.n)) : a.n;
+            l.s = min(a.starts[at], a.n);
+            l.e = max(l.s, min(a.starts[at + 1], a.n));
         }
-        return (e - s + kM - 1) / kM;
+        l.tiles = l.upto = (l.e - l.s + kM - 1) / kM;
+#pragma unroll
+        for (uint32_t off = 1; off < 64; off <<= 1) {
+            const uint32_t y = __shfl_up(l.upto, off, 64);
+            if (lane >= off) l.upto += y;
+        }
+        return l;
     }
     __device__ __forceinline__ explicit rows_tiling(const wh_rows_mm_args& args) : a(args), n_tiles((args.out_rows + kN - 1) / kN), total(0) {
-        for (uint32_t base = 0; base < a.n_groups; base += 64) {
-            uint32_t s, e, sum = group(base + (threadIdx.x & 63), s, e);
-            for (uint32_t off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-            total += (uint32_t)__builtin_amdgcn_readfirstlane(sum);
+        if (!a.starts) total = (a.n + kM - 1) / kM;
+        for (uint32_t base = 0; a.starts && base < a.n_groups; base += 64) {
+            total += (uint32_t)__builtin_amdgcn_readlane((int)groups(base).upto, 63);
         }
         total *= n_tiles;
         per = (total + 7) / 8;
@@ -604,33 +613,30 @@ struct rows_tiling {
     __device__ __forceinline__ uint64_t count(uint32_t xcd) const { return xcd * per >= total ? 0 : min(per, total - xcd * per); }
     // The t-th tile of an XCD, t < count.
     __device__ __forceinline__ void at(uint32_t xcd, uint64_t t, uint32_t& g, uint32_t& r0, uint32_t& r1, uint32_t& c0) const {
-        const uint32_t lane = threadIdx.x & 63;
         t += xcd * per;
         g = r0 = r1 = c0 = 0;
+        // tile `own` of a group of `mine` tiles of rows [start, end), fewer than 2^32 tiles
+        // with their columns, since its y rows are in memory
+        auto place = [&](uint32_t own, uint32_t mine, uint32_t start, uint32_t end) {
+            const uint32_t band = own / (kBand * n_tiles), in = own % (kBand * n_tiles), high = min(kBand, mine - band * kBand);
+            r0 = start + (band * kBand + in % high) * kM;
+            r1 = min(end, r0 + kM);
+            c0 = in / high * kN;
+        };
+        if (!a.starts) return place((uint32_t)t, (a.n + kM - 1) / kM, 0, a.n);
         for (uint32_t base = 0; base < a.n_groups; base += 64) {
-            uint32_t s, e;
-            const uint32_t tiles = group(base + lane, s, e);
-            uint32_t upto = tiles;
-#pragma unroll
-            for (uint32_t off = 1; off < 64; off <<= 1) {
-                const uint32_t y = __shfl_up(upto, off, 64);
-                if (lane >= off) upto += y;
-            }
-            const uint64_t past = __ballot((uint64_t)upto * n_tiles > t);
+            const lane_group l = groups(base);
+            const uint64_t past = __ballot((uint64_t)l.upto * n_tiles > t);
             if (past) {
                 const uint32_t lead = (uint32_t)__builtin_ctzll(past);
-                const uint32_t mine = __builtin_amdgcn_readlane((int)tiles, lead);
-                const uint64_t own = t - (uint64_t)((uint32_t)__builtin_amdgcn_readlane((int)upto, lead) - mine) * n_tiles;
+                const uint32_t mine = __builtin_amdgcn_readlane((int)l.tiles, lead);
+                const uint64_t own = t - (uint64_t)((uint32_t)__builtin_amdgcn_readlane((int)l.upto, lead) - mine) * n_tiles;
                 g = base + lead;
-                const uint32_t band = (uint32_t)(own / (kBand * n_tiles)), in = (uint32_t)(own % (kBand * n_tiles));
-                const uint32_t high = min(kBand, mine - band * kBand);
-                const uint32_t end = __builtin_amdgcn_readlane((int)e, lead);
-                r0 = __builtin_amdgcn_readlane((int)s, lead) + (band * kBand + in % high) * kM;
-                r1 = min(end, r0 + kM);
-                c0 = __builtin_amdgcn_readfirstlane(in / high * kN);
+                place(__builtin_amdgcn_readfirstlane((int)own), mine, __builtin_amdgcn_readlane((int)l.s, lead),
+                      __builtin_amdgcn_readlane((int)l.e, lead));
                 return;
             }
-            t -= (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * n_tiles;
+            t -= (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)l.upto, 63) * n_tiles;
         }
     }
 };
