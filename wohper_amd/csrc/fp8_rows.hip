@@ -1331,6 +1331,7 @@ hipError_t wh_rows_setup() {
         if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     };
     tile((const void*)k_expert_place<1>, plan_lds(WH_ROWS_MAX_GROUPS));
+    tile((const void*)k_expert_place<2>, plan_lds(WH_ROWS_MAX_GROUPS));
     tile((const void*)k_expert_place<4>, plan_lds(WH_ROWS_MAX_GROUPS));
     constexpr size_t lds = rows_tile_shape<4, 4, 2, 2>::kLds;
     tile((const void*)k_rows_mm_tile<true, true>, lds);
@@ -1511,12 +1512,15 @@ hipError_t wh_rows_scales_launch(const uint8_t* scales, uint64_t n, uint32_t* fl
     return hipSuccess;
 }
 
-// How many times 64 routes a wave takes.  Once: 96 routes 3.6 us (four times: 5.4), 12000
-// over 256 experts 7.4 (9.8).  Four times where that saves the first launch, 1800 routes
-// 5.9 us (6.4), and where every workgroup would sum the counts of many chunks: 98304 routes
-// over 256 experts 12.0 us (13.1), 1048576 30.8 (126).
+// How many times 64 routes a wave takes: as few as make one launch of up to 4096 routes (96
+// once 3.7 us, four times 5.4; 1800 twice 4.8, in two launches 6.4), then once (12000 routes
+// over 256 experts 7.4 us, four times 9.8) until every workgroup would sum the counts of
+// too many chunks: 98304 routes over 256 experts once 13.1 us, twice 11.1, four times 12.0;
+// 1048576 132, 49 and 31.
 static uint32_t plan_turns(size_t n, size_t n_groups) {
-    return n > plan_chunk(1) && (n <= plan_chunk(4) || n * std::max<size_t>(n_groups, 64) > 1u << 24) ? 4 : 1;
+    if (n <= plan_chunk(4)) return n <= plan_chunk(1) ? 1 : n <= plan_chunk(2) ? 2 : 4;
+    const size_t counts = n * std::max<size_t>(n_groups, 64);  // 1024 times what a workgroup sums, of chunks of 1024
+    return counts <= 1u << 24 ? 1 : counts <= 1u << 25 ? 2 : 4;
 }
 
 size_t wh_expert_plan_scratch(size_t n, size_t n_groups) {
@@ -1533,7 +1537,8 @@ hipError_t wh_expert_plan_launch(const wh_expert_plan_args& a, hipStream_t strea
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (turns > 1) k_expert_place<4><<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
+    if (turns == 4) k_expert_place<4><<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
+    else if (turns == 2) k_expert_place<2><<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
     else k_expert_place<1><<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
     return hipGetLastError();
 }
