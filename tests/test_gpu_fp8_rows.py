@@ -648,7 +648,7 @@ def plain_plan(ids, n_experts):
 @pytest.mark.parametrize("npos,topk,n_experts", [(0, 6, 4), (1, 1, 1), (1, 6, 256), (16, 6, 256), (64, 8, 5), (683, 6, 256),
                                                  (4096, 1, 3), (4097, 1, 1024), (5000, 3, 1000), (2000, 8, 63), (9000, 2, 64),
                                                  (16385, 6, 256), (30000, 1, 1024), (270001, 1, 5), (300, 6, 256),
-                                                 (341, 8, 30), (20000, 7, 256)])
+                                                 (341, 8, 30), (20000, 7, 256), (700001, 1, 257), (40000, 4, 13), (300000, 1, 1023)])
 def test_plans(ctx, npos, topk, n_experts):
     rng = np.random.default_rng(npos)
     ids = rng.integers(0, n_experts, (npos, topk))

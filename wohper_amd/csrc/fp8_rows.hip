@@ -1147,6 +1147,9 @@ constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 // Routes of a workgroup, a chunk: a wave takes `turns` times 64 consecutive ones.
 __host__ __device__ constexpr uint32_t plan_chunk(uint32_t turns) { return kPlanThreads * turns; }
 
+// Counts of a chunk: four experts a load.
+__host__ __device__ constexpr uint32_t plan_padded(uint32_t n_groups) { return (n_groups + 3) / 4 * 4; }
+
 // What a wave's lanes have stored to LDS is there for its other lanes.
 __device__ __forceinline__ void plan_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -1168,7 +1171,8 @@ __device__ __forceinline__ uint64_t plan_same(uint32_t id, uint32_t bits) {
 // How many routes of each expert a chunk has.
 __global__ void __launch_bounds__(kPlanThreads) k_expert_count(wh_expert_plan_args a, uint32_t chunk) {
     __shared__ uint32_t count[WH_ROWS_MAX_GROUPS];
-    for (uint32_t e = threadIdx.x; e < a.n_groups; e += kPlanThreads) count[e] = 0;
+    const uint32_t padded = plan_padded(a.n_groups);
+    for (uint32_t e = threadIdx.x; e < padded; e += kPlanThreads) count[e] = 0;
     __syncthreads();
     const uint32_t from = blockIdx.x * chunk, to = min(a.n, from + chunk);
     for (uint32_t i = from + threadIdx.x; i < to; i += kPlanThreads) {
@@ -1176,7 +1180,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_count(wh_expert_plan_ar
         if (id < a.n_groups) atomicAdd(&count[id], 1u);
     }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < a.n_groups; e += kPlanThreads) a.counts[(uint64_t)blockIdx.x * a.n_groups + e] = count[e];
+    for (uint32_t e = threadIdx.x; e < padded; e += kPlanThreads) a.counts[(uint64_t)blockIdx.x * padded + e] = count[e];
 }
 
 // Expert lists: a counting sort that keeps the order of routes.  A workgroup takes a
@@ -1188,7 +1192,7 @@ template <uint32_t kTurns>
 __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_args a, uint32_t chunks, uint32_t bits) {
     extern __shared__ uint32_t lds[];
     uint32_t* const at = lds;  // [kPlanWaves][n_groups]: counts, then next places of a wave
-    __shared__ uint32_t wave_sum[kPlanWaves], all_of[WH_ROWS_MAX_GROUPS], before_of[WH_ROWS_MAX_GROUPS];
+    __shared__ uint32_t wave_sum[kPlanWaves], all_of[WH_ROWS_MAX_GROUPS], before_of[WH_ROWS_MAX_GROUPS], listed;
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, E = a.n_groups;
     for (uint32_t i = t; i < kPlanWaves * E; i += kPlanThreads) at[i] = 0;
     if (t < E) all_of[t] = before_of[t] = 0;
@@ -1201,21 +1205,26 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_ar
         id[k] = i < a.n ? a.ids[i] : kNone;
     }
     __syncthreads();
-    // all chunks' routes of expert e and those before this chunk, a range of chunks a thread
+    // all chunks' routes of four experts a lane and those before this chunk; a wave (or as
+    // many as have them all) takes every so manieth chunk
     if (chunks > 1) {
+        const uint32_t fours = plan_padded(E) / 4;
         uint32_t shift = 6;
-        while (1u << shift < E) ++shift;
-        const uint32_t e = t & ((1u << shift) - 1), parts = kPlanThreads >> shift;
-        if (e < E) {
-            uint32_t all = 0, before = 0;
-#pragma unroll 8
-            for (uint32_t c = t >> shift; c < chunks; c += parts) {
-                const uint32_t v = a.counts[(uint64_t)c * E + e];
-                before += c < blockIdx.x ? v : 0;
+        while (1u << shift < fours) ++shift;
+        const uint32_t four = t & ((1u << shift) - 1), parts = kPlanThreads >> shift;
+        wh_u4 all = {0, 0, 0, 0}, before = {0, 0, 0, 0};
+        if (four < fours) {
+#pragma unroll 4
+            for (uint32_t c = __builtin_amdgcn_readfirstlane(t >> shift); c < chunks; c += parts) {
+                const wh_u4 v = ((const wh_u4*)a.counts)[(uint64_t)c * fours + four];
                 all += v;
+                if (c < blockIdx.x) before += v;
             }
-            if (all) atomicAdd(&all_of[e], all);
-            if (before) atomicAdd(&before_of[e], before);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            if (all[j]) atomicAdd(&all_of[4 * four + j], all[j]);
+            if (before[j]) atomicAdd(&before_of[4 * four + j], before[j]);
         }
     }
 #pragma unroll
@@ -1227,38 +1236,42 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_ar
         plan_wave_sync();
     }
     __syncthreads();
-    uint32_t all = 0, before = 0;
-    if (t < E) {
-        if (chunks == 1) {
-            for (uint32_t w = 0; w < kPlanWaves; ++w) all += at[w * E + t];
-        } else {
-            all = all_of[t];
-            before = before_of[t];
+    // waves that have experts: their starts, and each wave's first place in them
+    const bool has = wave * 64 < E;
+    uint32_t all = 0, upto = 0;
+    if (has) {
+        if (t < E) {
+            if (chunks == 1) {
+#pragma unroll
+                for (uint32_t w = 0; w < kPlanWaves; ++w) all += at[w * E + t];
+            } else {
+                all = all_of[t];
+            }
         }
+        upto = all;
+        for (uint32_t off = 1; off < 64; off <<= 1) {
+            const uint32_t y = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += y;
+        }
+        if (lane == 63) wave_sum[wave] = upto;
     }
-    uint32_t upto = all;
-    for (uint32_t off = 1; off < 64; off <<= 1) {
-        const uint32_t y = __shfl_up(upto, off, 64);
-        if (lane >= off) upto += y;
-    }
-    if (lane == 63) wave_sum[wave] = upto;
     __syncthreads();
-    uint32_t total = 0, waves_before = 0;
-    for (uint32_t w = 0; w < kPlanWaves; ++w) {
-        if (w < wave) waves_before += wave_sum[w];
-        total += wave_sum[w];
-    }
-    if (t < E) {
-        const uint32_t start = waves_before + upto - all;
-        uint32_t next = start + before;
-        for (uint32_t w = 0; w < kPlanWaves; ++w) {
-            const uint32_t v = at[w * E + t];
-            at[w * E + t] = next;
-            next += v;
-        }
-        if (blockIdx.x == 0) {
-            a.starts[t] = start;
-            if (t == E - 1) a.starts[E] = start + all;
+    if (has) {
+        for (uint32_t w = 0; w < wave; ++w) upto += wave_sum[w];
+        if (t < E) {
+            const uint32_t start = upto - all;
+            uint32_t next = start + before_of[t];
+#pragma unroll
+            for (uint32_t w = 0; w < kPlanWaves; ++w) {
+                const uint32_t v = at[w * E + t];
+                at[w * E + t] = next;
+                next += v;
+            }
+            if (blockIdx.x == 0) a.starts[t] = start;
+            if (t == E - 1) {
+                listed = upto;
+                if (blockIdx.x == 0) a.starts[E] = upto;
+            }
         }
     }
     __syncthreads();
@@ -1274,7 +1287,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_ar
         if (i < a.n) {
             a.slots[i] = place;
             if (some) a.rows[place] = i / a.topk;
-            if (i >= total) a.rows[i] = kNone;  // behind the lists
+            if (i >= listed) a.rows[i] = kNone;  // behind the lists
         }
     }
 }
@@ -1513,19 +1526,19 @@ hipError_t wh_rows_scales_launch(const uint8_t* scales, uint64_t n, uint32_t* fl
 }
 
 // How many times 64 routes a wave takes: as few as make one launch of up to 4096 routes (96
-// once 3.7 us, four times 5.4; 1800 twice 4.8, in two launches 6.4), then once (12000 routes
-// over 256 experts 7.4 us, four times 9.8) until every workgroup would sum the counts of
-// too many chunks: 98304 routes over 256 experts once 13.1 us, twice 11.1, four times 12.0;
-// 1048576 132, 49 and 31.
+// once 3.7 us, four times 5.5; 1800 twice 4.7, in two launches 6.4), then once (12000 routes
+// over 256 experts 6.8 us, four times 9.8) until every workgroup would sum the counts of
+// too many chunks: over 256 experts 98304 routes once 9.0 us, twice 9.2, four times 11.0;
+// 262144 13.1, 11.4 and 12.4; 1048576 53, 24 and 20.
 static uint32_t plan_turns(size_t n, size_t n_groups) {
     if (n <= plan_chunk(4)) return n <= plan_chunk(1) ? 1 : n <= plan_chunk(2) ? 2 : 4;
-    const size_t counts = n * std::max<size_t>(n_groups, 64);  // 1024 times what a workgroup sums, of chunks of 1024
-    return counts <= 1u << 24 ? 1 : counts <= 1u << 25 ? 2 : 4;
+    const size_t counts = n * std::max<size_t>(n_groups, 256);  // a wave sums at least 256 a chunk
+    return counts <= 1u << 25 ? 1 : counts <= 1u << 27 ? 2 : 4;
 }
 
 size_t wh_expert_plan_scratch(size_t n, size_t n_groups) {
     const size_t chunk = plan_chunk(plan_turns(n, n_groups)), chunks = (n + chunk - 1) / chunk;
-    return chunks > 1 ? chunks * n_groups * sizeof(uint32_t) : 0;
+    return chunks > 1 ? chunks * plan_padded((uint32_t)n_groups) * sizeof(uint32_t) : 0;
 }
 
 hipError_t wh_expert_plan_launch(const wh_expert_plan_args& a, hipStream_t stream) {
