@@ -362,18 +362,20 @@ __device__ __forceinline__ wh_f4 rows_scaled(wh_f4 acc, wh_f4 block, int e, floa
     return acc;
 }
 
-// A weight scale as the byte of a power of two and a factor: 1 for ordinary UE8M0
-// bytes, else in [1, 2), or the scale itself where it is no normal number.
-__device__ __forceinline__ uint32_t rows_split_scale(const wh_rows_mm_args& a, uint64_t at, float* m) {
+// A weight scale's bits, and they as the byte of a power of two and a factor: 1 for
+// ordinary UE8M0 bytes, else in [1, 2), or the scale itself where it is no normal number.
+__device__ __forceinline__ uint32_t rows_scale_bits(const wh_rows_mm_args& a, uint64_t at) {
+    return a.scale_f32 ? ((const uint32_t*)a.w_scales)[at] : ((const uint8_t*)a.w_scales)[at];
+}
+__device__ __forceinline__ uint32_t rows_split_bits(const wh_rows_mm_args& a, uint32_t u, float* m) {
     *m = 1.0f;
     if (!a.scale_f32) {
-        const uint32_t byte = ((const uint8_t*)a.w_scales)[at];
-        if (byte != 0 && byte != 255) return byte;
-        *m = wh_ue8m0(byte);
+        if (u != 0 && u != 255) return u;
+        *m = wh_ue8m0(u);
         return 127;
     }
-    const float s = ((const float*)a.w_scales)[at];
-    const uint32_t u = __float_as_uint(s), e = u >> 23 & 0xff;
+    const float s = __uint_as_float(u);
+    const uint32_t e = u >> 23 & 0xff;
     if (e == 255 || (u & 0x7fffffffu) == 0) {
         *m = s;
         return 127;
@@ -384,6 +386,9 @@ __device__ __forceinline__ uint32_t rows_split_scale(const wh_rows_mm_args& a, u
     }
     *m = __uint_as_float((u & 0x807fffffu) | 0x3f800000u);
     return e;
+}
+__device__ __forceinline__ uint32_t rows_split_scale(const wh_rows_mm_args& a, uint64_t at, float* m) {
+    return rows_split_bits(a, rows_scale_bits(a, at), m);
 }
 
 // Four values to any address: the hardware takes stores of 8 and 16 bytes there.
@@ -427,12 +432,12 @@ __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part
     const bool works = col0 < a.out_rows;
     wh_f4 acc[kMt];
     const uint8_t *xp[kMt], *xs[kMt];
+    uint32_t src[kMt];
     bool have[kMt], nan[kMt];
 #pragma unroll
     for (int t = 0; t < kMt; ++t) {
-        const uint32_t src = rows_source(a, min(j0 + 16 * t + l16, j1 - 1), &have[t]);
-        xp[t] = a.x.codes + (uint64_t)src * a.x.stride + 16 * q;
-        xs[t] = a.x.scales + (uint64_t)src * a.x.scale_stride;
+        const uint32_t j = min(j0 + 16 * t + l16, j1 - 1);
+        src[t] = a.rows ? a.rows[j] : j;
         acc[t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
         nan[t] = false;
     }
@@ -440,9 +445,9 @@ __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part
         const uint64_t w_row = a.row_start + (uint64_t)g * a.out_rows + col0;
         const uint8_t* const wp = a.w + (w_row + min(l16, a.out_rows - 1 - col0)) * a.cols + 16 * q;
         // scales of this wave's blocks, one a lane: 16 rows share one
+        const uint32_t bits = rows_scale_bits(a, w_row / a.row_block * blocks + min(ks + ks_n * lane, blocks - 1));
+        uint32_t wb = 0;
         float wm = 1.0f;
-        uint32_t wb = 127;
-        if (ks + ks_n * lane < blocks) wb = rows_split_scale(a, w_row / a.row_block * blocks + ks + ks_n * lane, &wm);
         const uint32_t mine = (blocks - ks + ks_n - 1) / ks_n;  // 64 at most
         for (uint32_t i0 = 0; i0 < mine; i0 += kU) {
             rows_frag w[kU], x[kU][kMt];
@@ -452,6 +457,20 @@ __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part
                 const uint32_t b = min(ks + ks_n * (i0 + u), blocks - 1);
                 w[u].a = *(const wh_u4*)(wp + b * 128u);
                 w[u].b = *(const wh_u4*)(wp + b * 128u + 64);
+            }
+            if (i0 == 0) {  // the first weights are under way: what lists and scales say
+                wb = rows_split_bits(a, bits, &wm);
+#pragma unroll
+                for (int t = 0; t < kMt; ++t) {
+                    have[t] = src[t] < a.n_x;
+                    const uint32_t r = have[t] ? src[t] : 0;
+                    xp[t] = a.x.codes + (uint64_t)r * a.x.stride + 16 * q;
+                    xs[t] = a.x.scales + (uint64_t)r * a.x.scale_stride;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const uint32_t b = min(ks + ks_n * (i0 + u), blocks - 1);
 #pragma unroll
                 for (int t = 0; t < kMt; ++t) {
                     x[u][t].a = *(const wh_u4*)(xp[t] + b * 128u);
