@@ -1227,8 +1227,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_ar
         id[k] = i < a.n ? a.ids[i] : kNone;
     }
     __syncthreads();
-    // all chunks' routes of four experts a lane and those before this chunk; a wave (or as
-    // many as have them all) takes every so manieth chunk
+    // all chunks' routes of four experts a lane, and those before this chunk: the chunks
+    // are dealt out to waves, or to as many waves together as hold all experts
     if (chunks > 1) {
         const uint32_t fours = plan_padded(E) / 4;
         uint32_t shift = 6;
