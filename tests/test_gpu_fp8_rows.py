@@ -511,7 +511,8 @@ def gpu_near(got, x, w, bf16, cols):
 
 @pytest.mark.parametrize("n,rows,cols", [(4096, 4096, 1280), (2048, 4096, 4096), (4100, 2112, 8320), (300, 704, 10240), (5000, 1008, 128),
                                          (700, 512, 8192), (1024, 32768, 256), (33, 4096, 10240), (100, 16384, 4096), (4300, 4112, 8576),
-                                         (9000, 4096, 384)])
+                                         (9000, 4096, 384), (4, 8192, 4096), (16, 16384, 2176), (17, 8192, 8192), (31, 65536, 512),
+                                         (14, 32768, 1408), (40, 16384, 4224)])
 @pytest.mark.parametrize("bf16,f32", [(False, False), (False, True), (True, False), (True, True)])
 def test_large_products(ctx, n, rows, cols, bf16, f32):
     c = Large(ctx, n, n, rows, cols, f32)

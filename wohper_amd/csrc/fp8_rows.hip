@@ -415,98 +415,122 @@ __device__ __forceinline__ uint32_t rows_source(const wh_rows_mm_args& a, uint32
     return *is ? r : 0;
 }
 
-// Few rows a group: bound by the weights' bytes.  A wave takes 16 weight rows and
-// every kS-th block of their columns for up to 16 kMt x rows, straight from memory
-// into registers; the kS waves of the same weight rows join in LDS.  Blocks come
-// kU at a time, all their loads before the first product.  Registers for two workgroups
-// a CU: 84 rows over 64 lists of 4096 x 4096, 43 of them not empty, in f32 158 us (with one
-// 226), 4.6 TB/s; 5 x 4096 x 8192 in f32 9.4 us, 3.6 TB/s with the launch.
+// Few rows a group: bound by the weights' bytes.  A wave takes 16 kNt weight rows and one
+// of ks_n ranges of their columns for up to 16 kMt x rows, straight from memory into
+// registers; the waves of the same weight rows join in LDS.  Blocks come kU at a time, all
+// their loads before the first product; a range's blocks lie side by side, so that one
+// word holds a row's scales of four.  Registers for two workgroups a CU: 84 rows over 64
+// lists of 4096 x 4096, 43 of them not empty, in f32 147 us (with one 226), 4.9 TB/s.
+// x is read again for each 16 kNt weight rows: 16 x 8192 x 8192 in bf16 18.8 us with one, 16.1
+// (4.2 TB/s) with two; 5 x 4096 x 8192 in f32 9.1 us, 3.7 TB/s with the launch.
 constexpr uint32_t kThinWaves = 8;
-template <int kMt, bool kBf16, bool kMant>
+template <int kMt, int kNt, bool kBf16, bool kMant>
 __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part)[64][4], uint32_t ks_n, uint32_t g, uint32_t j0,
                                           uint32_t j1, uint32_t c0) {
-    constexpr int kU = kMt == 1 ? 4 : kMt == 2 ? 2 : 1;
+    constexpr int kU = kMt * kNt == 1 ? 4 : kMt * kNt == 2 ? 2 : 1;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t ks = wave & (ks_n - 1), l16 = lane & 15, q = lane >> 4;
-    const uint32_t blocks = a.cols / 128u, col0 = c0 + 16 * (wave / ks_n);
+    const uint32_t blocks = a.cols / 128u, col0 = c0 + 16 * kNt * (wave / ks_n);
     const bool works = col0 < a.out_rows;
-    wh_f4 acc[kMt];
+    wh_f4 acc[kNt][kMt];
     const uint8_t *xp[kMt], *xs[kMt];
     uint32_t src[kMt];
-    bool have[kMt], nan[kMt];
+    bool nan[kMt];
 #pragma unroll
     for (int t = 0; t < kMt; ++t) {
         const uint32_t j = min(j0 + 16 * t + l16, j1 - 1);
         src[t] = a.rows ? a.rows[j] : j;
-        acc[t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
         nan[t] = false;
+#pragma unroll
+        for (int i = 0; i < kNt; ++i) acc[i][t] = wh_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    if (works) {
+    // this wave's blocks, 64 at most
+    const uint32_t len = (blocks + ks_n - 1) / ks_n, first = min(ks * len, blocks), mine = works ? min(len, blocks - first) : 0;
+    if (mine) {
         const uint64_t w_row = a.row_start + (uint64_t)g * a.out_rows + col0;
-        const uint8_t* const wp = a.w + (w_row + min(l16, a.out_rows - 1 - col0)) * a.cols + 16 * q;
-        // scales of this wave's blocks, one a lane: 16 rows share one
-        const uint32_t bits = rows_scale_bits(a, w_row / a.row_block * blocks + min(ks + ks_n * lane, blocks - 1));
-        uint32_t wb = 0;
-        float wm = 1.0f;
-        const uint32_t mine = (blocks - ks + ks_n - 1) / ks_n;  // 64 at most
+        const uint8_t* wp[kNt];
+        uint32_t bits[kNt], wb[kNt];
+        float wm[kNt];
+#pragma unroll
+        for (int i = 0; i < kNt; ++i) {
+            wp[i] = a.w + (w_row + min(16 * i + l16, a.out_rows - 1 - col0)) * a.cols + 16 * q;
+            // scales of this wave's blocks, one a lane: 16 rows share one
+            bits[i] = rows_scale_bits(a, (w_row + min(16u * i, a.out_rows - 1 - col0)) / a.row_block * blocks +
+                                             min(first + lane, blocks - 1));
+        }
         for (uint32_t i0 = 0; i0 < mine; i0 += kU) {
-            rows_frag w[kU], x[kU][kMt];
-            uint32_t xb[kU][kMt];
+            rows_frag w[kU][kNt], x[kU][kMt];
+            uint32_t x0[kMt], x1[kMt];  // the words of the rows' scales that hold these blocks'
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
-                const uint32_t b = min(ks + ks_n * (i0 + u), blocks - 1);
-                w[u].a = *(const wh_u4*)(wp + b * 128u);
-                w[u].b = *(const wh_u4*)(wp + b * 128u + 64);
+                const uint32_t b = first + min(i0 + u, mine - 1);
+#pragma unroll
+                for (int i = 0; i < kNt; ++i) {
+                    w[u][i].a = *(const wh_u4*)(wp[i] + b * 128u);
+                    w[u][i].b = *(const wh_u4*)(wp[i] + b * 128u + 64);
+                }
             }
             if (i0 == 0) {  // the first weights are under way: what lists and scales say
-                wb = rows_split_bits(a, bits, &wm);
+#pragma unroll
+                for (int i = 0; i < kNt; ++i) wb[i] = rows_split_bits(a, bits[i], &wm[i]);
 #pragma unroll
                 for (int t = 0; t < kMt; ++t) {
-                    have[t] = src[t] < a.n_x;
-                    const uint32_t r = have[t] ? src[t] : 0;
+                    const uint32_t r = src[t] < a.n_x ? src[t] : 0;
                     xp[t] = a.x.codes + (uint64_t)r * a.x.stride + 16 * q;
                     xs[t] = a.x.scales + (uint64_t)r * a.x.scale_stride;
                 }
             }
+            const uint32_t b0 = first + i0, word = b0 / 4, at = b0 & 3;
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const uint32_t b = min(ks + ks_n * (i0 + u), blocks - 1);
+            for (int t = 0; t < kMt; ++t) {
 #pragma unroll
-                for (int t = 0; t < kMt; ++t) {
+                for (int u = 0; u < kU; ++u) {
+                    const uint32_t b = first + min(i0 + u, mine - 1);
                     x[u][t].a = *(const wh_u4*)(xp[t] + b * 128u);
                     x[u][t].b = *(const wh_u4*)(xp[t] + b * 128u + 64);
-                    xb[u][t] = xs[t][b];
                 }
+                x0[t] = ((const uint32_t*)xs[t])[word];
+                x1[t] = 0;
+            }
+            if (at + kU > 4) {
+#pragma unroll
+                for (int t = 0; t < kMt; ++t) x1[t] = ((const uint32_t*)xs[t])[min(word + 1, (blocks - 1) / 4)];
             }
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
                 if (i0 + u < mine) {
-                    const int byte = __builtin_amdgcn_readlane((int)wb, i0 + u);
-                    const float m = kMant ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wm), i0 + u)) : 1.0f;
-                    if constexpr (kBf16) {
-                        const wh_i8 wc = rows_codes(w[u]);
+                    uint32_t xb[kMt];
 #pragma unroll
-                        for (int t = 0; t < kMt; ++t) {
-                            const wh_f4 from = kMant ? wh_f4{0.0f, 0.0f, 0.0f, 0.0f} : acc[t];
-                            const wh_f4 s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wc, rows_codes(x[u][t]), from, 0,
-                                                                                             0, 0, byte, 0, (int)xb[u][t]);
-                            if constexpr (kMant) {
+                    for (int t = 0; t < kMt; ++t) xb[t] = __builtin_amdgcn_alignbyte(x1[t], x0[t], at) >> 8 * u & 0xff;
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(s[i], m, acc[t][i]);
-                            } else {
-                                acc[t] = s;
+                    for (int i = 0; i < kNt; ++i) {
+                        const int byte = __builtin_amdgcn_readlane((int)wb[i], i0 + u);
+                        const float m = kMant ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wm[i]), i0 + u)) : 1.0f;
+                        if constexpr (kBf16) {
+                            const wh_i8 wc = rows_codes(w[u][i]);
+#pragma unroll
+                            for (int t = 0; t < kMt; ++t) {
+                                const wh_f4 from = kMant ? wh_f4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][t];
+                                const wh_f4 s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wc, rows_codes(x[u][t]), from, 0,
+                                                                                                 0, 0, byte, 0, (int)xb[t]);
+                                if constexpr (kMant) {
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) acc[i][t][k] = fmaf(s[k], m, acc[i][t][k]);
+                                } else {
+                                    acc[i][t] = s;
+                                }
                             }
-                        }
-                    } else {
-                        const rows_f16x4 wv = rows_decode(w[u]);
+                        } else {
+                            const rows_f16x4 wv = rows_decode(w[u][i]);
 #pragma unroll
-                        for (int t = 0; t < kMt; ++t) {
-                            const rows_f16x4 xv = rows_decode(x[u][t]);
-                            wh_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+                            for (int t = 0; t < kMt; ++t) {
+                                const rows_f16x4 xv = rows_decode(x[u][t]);
+                                wh_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv.v[j], xv.v[j], s, 0, 0, 0);
-                            acc[t] = rows_scaled(acc[t], s, (int)xb[u][t] + byte - 254, m);
-                            nan[t] |= xb[u][t] == 255;
+                                for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv.v[j], xv.v[j], s, 0, 0, 0);
+                                acc[i][t] = rows_scaled(acc[i][t], s, (int)xb[t] + byte - 254, m);
+                                nan[t] |= xb[t] == 255;
+                            }
                         }
                     }
                 }
@@ -515,34 +539,43 @@ __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part
         if constexpr (!kBf16) {
 #pragma unroll
             for (int t = 0; t < kMt; ++t)
-                if (nan[t]) acc[t] = wh_f4{1.0f, 1.0f, 1.0f, 1.0f} * __uint_as_float(0x7fc00000u);
+#pragma unroll
+                for (int i = 0; i < kNt; ++i)
+                    if (nan[t]) acc[i][t] = wh_f4{1.0f, 1.0f, 1.0f, 1.0f} * __uint_as_float(0x7fc00000u);
         }
     }
     if (ks_n > 1) {
         __syncthreads();  // the parts of the rows before have been read
 #pragma unroll
-        for (int t = 0; t < kMt; ++t) *(wh_f4*)part[wave * kMt + t][lane] = acc[t];
+        for (int t = 0; t < kMt; ++t)
+#pragma unroll
+            for (int i = 0; i < kNt; ++i) *(wh_f4*)part[(wave * kMt + t) * kNt + i][lane] = acc[i][t];
         __syncthreads();
     }
     if (!works) return;
 #pragma unroll
     for (int t = 0; t < kMt; ++t) {
-        if ((t & (ks_n - 1)) != ks) continue;
-        wh_f4 v = acc[t];
-        if (ks_n > 1) {
-            const uint32_t first = wave - ks;
-            v = *(const wh_f4*)part[first * kMt + t][lane];
-            for (uint32_t s = 1; s < ks_n; ++s) v += *(const wh_f4*)part[(first + s) * kMt + t][lane];
-        }
         const uint32_t j = j0 + 16 * t + l16;
-        if (j < j1) rows_put4<kBf16>(a, j, col0 + 4 * q, have[t] ? v : wh_f4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+        for (int i = 0; i < kNt; ++i) {
+            if (((t * kNt + i) & (ks_n - 1)) != ks) continue;
+            wh_f4 v = acc[i][t];
+            if (ks_n > 1) {
+                const uint32_t at = ((wave - ks) * kMt + t) * kNt + i;
+                v = *(const wh_f4*)part[at][lane];
+                for (uint32_t s = 1; s < ks_n; ++s) v += *(const wh_f4*)part[at + s * kMt * kNt][lane];
+            }
+            const uint32_t col = col0 + 16 * i + 4 * q;
+            if (j < j1 && col < a.out_rows) rows_put4<kBf16>(a, j, col, src[t] < a.n_x ? v : wh_f4{0.0f, 0.0f, 0.0f, 0.0f});
+        }
     }
 }
 
-template <bool kBf16, bool kMant>
+// kNt: blocks of 16 weight rows a wave.
+template <bool kBf16, bool kMant, int kNt>
 __global__ void __launch_bounds__(64 * kThinWaves, 4) k_rows_mm_thin(wh_rows_mm_args a, uint32_t ks_n) {
     __shared__ __align__(16) float part[kThinWaves * 4][64][4];
-    const uint32_t g = blockIdx.y, c0 = blockIdx.x * 16 * (kThinWaves / ks_n);
+    const uint32_t g = blockIdx.y, step = 16 * (kThinWaves / ks_n), c0 = blockIdx.x * step * kNt;
     uint32_t j0 = 0, j1 = a.n;
     if (a.starts) {
         j0 = min(a.starts[g], a.n);
@@ -551,14 +584,14 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) k_rows_mm_thin(wh_rows_mm_
     while (j0 < j1) {
         const uint32_t left = j1 - j0;
         if (left <= 16) {
-            rows_thin<1, kBf16, kMant>(a, part, ks_n, g, j0, j1, c0);
+            rows_thin<1, kNt, kBf16, kMant>(a, part, ks_n, g, j0, j1, c0);
             return;
         }
         if (left <= 32) {
-            rows_thin<2, kBf16, kMant>(a, part, ks_n, g, j0, j1, c0);
+            rows_thin<2, kNt, kBf16, kMant>(a, part, ks_n, g, j0, j1, c0);
             return;
         }
-        rows_thin<4, kBf16, kMant>(a, part, ks_n, g, j0, j1, c0);
+        for (int i = 0; i < kNt; ++i) rows_thin<4, 1, kBf16, kMant>(a, part, ks_n, g, j0, j1, c0 + i * step);
         j0 += 64;
     }
 }
@@ -1125,6 +1158,14 @@ uint32_t rows_thin_split(const wh_rows_mm_args& a) {
     while (ks < kThinWaves && 2 * ks <= blocks && (blocks >= 8 * ks || tiles * ks <= 128 * kThinWaves)) ks *= 2;
     return ks;
 }
+// Blocks of 16 weight rows a wave: two where that leaves a workgroup for every CU and there
+// are rows enough that reading them half as often counts.  8192 x 4096 with 4, 8 and 16 rows
+// in bf16 8.1, 8.9 and 10.3 us with one, 7.7, 8.0 and 8.8 with two; with 8 and 16 in f32 9.2
+// and 10.7, 9.4 and 10.1.  Lists gain nothing: 16 of 2048 x 8192 with 4 rows each 58.6, 57.7.
+uint32_t rows_thin_tiles(const wh_rows_mm_args& a, bool bf16) {
+    const uint64_t waves = (uint64_t)((a.out_rows + 15) / 16) * rows_thin_split(a);
+    return a.n_groups == 1 && a.n >= (bf16 ? 4 : 12) && waves >= 2 * 256 * kThinWaves ? 2 : 1;
+}
 
 // Whether the matrix instructions take a call: every 16 rows of a tile share a
 // scale, and codes mean the same.
@@ -1403,9 +1444,9 @@ hipError_t wh_rows_read_launch(const wh_rows_read_args& a, bool bf16, hipStream_
 // Which kernel takes a product, and how many ranges its columns are cut into: the least
 // of these estimates of its time in us, fitted to 400 measured calls (one MI355X; 1 to
 // 4096 rows, 1 to 64 groups, weights from 1408 x 512 to 32768 x 1024 and 4096 x 8192).
-//  - thin: a wave's block of columns takes 0.95, 1.6 and 3 us for up to 16, 32 and 64
+//  - thin: a wave's block of columns takes 0.8, 1.6 and 3 us for up to 16, 32 and 64
 //    rows (with groups of uneven lists 0.55 and 0.045 a row), workgroups in rounds of 256:
-//    4096 x 4096 with 16, 64 and 128 rows 7.7, 15.6 and 29, where tiles take 23 to 25, cut
+//    4096 x 4096 with 16, 64 and 128 rows 7.2, 15.6 and 29, where tiles take 23 to 25, cut
 //    up 13 to 18; 64 groups with 4, 16 and 32 rows each in f32 228, 343 and 505, tiles 281,
 //    299 and 309;
 //  - tile: a block 0.56 us in bf16 (0.95 with factors of scales), 1.1 in f32, in rounds of
@@ -1429,7 +1470,7 @@ wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
         const uint32_t each = 16 * (kThinWaves / rows_thin_split(a));
         const double left = rows - 64 * std::floor(rows / 64);
         const double chunk = a.n_groups > 1 ? 0.55 + 0.045 * rows
-                                            : 3.0 * std::floor(rows / 64) + (left == 0 ? 0 : left <= 16 ? 0.95 : left <= 32 ? 1.6 : 3.0);
+                                            : 3.0 * std::floor(rows / 64) + (left == 0 ? 0 : left <= 16 ? 0.8 : left <= 32 ? 1.6 : 3.0);
         double best = 3.5 + std::max(1.0, groups * ((a.out_rows + each - 1) / each) / 256) *
                                 std::ceil((double)blocks / rows_thin_split(a)) * chunk;
         p.kind = wh_rows_mm_plan::kThin;
@@ -1464,7 +1505,7 @@ wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
         case wh_rows_mm_plan::kAny: p.grid = most(kAnyRows, 16); break;
         case wh_rows_mm_plan::kThin: {
             p.threads = 64 * kThinWaves;
-            const uint32_t each = 16 * (kThinWaves / rows_thin_split(a));
+            const uint32_t each = 16 * (kThinWaves / rows_thin_split(a)) * rows_thin_tiles(a, bf16);
             p.grid = (uint64_t)((a.out_rows + each - 1) / each) * a.n_groups;
             break;
         }
@@ -1490,13 +1531,18 @@ hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, const wh_rows_mm_plan& p,
         case wh_rows_mm_plan::kThin: {
             const uint32_t ks = rows_thin_split(a);
             auto thin = [&](auto kern) { kern<<<dim3(grid / a.n_groups, a.n_groups), p.threads, 0, stream>>>(a, ks); };
-            if (bf16) {
-                if (mant) thin(k_rows_mm_thin<true, true>);
-                else thin(k_rows_mm_thin<true, false>);
-            } else {
-                if (mant) thin(k_rows_mm_thin<false, true>);
-                else thin(k_rows_mm_thin<false, false>);
-            }
+            auto of = [&](auto nt) {
+                constexpr int kNt = decltype(nt)::value;
+                if (bf16) {
+                    if (mant) thin(k_rows_mm_thin<true, true, kNt>);
+                    else thin(k_rows_mm_thin<true, false, kNt>);
+                } else {
+                    if (mant) thin(k_rows_mm_thin<false, true, kNt>);
+                    else thin(k_rows_mm_thin<false, false, kNt>);
+                }
+            };
+            if (rows_thin_tiles(a, bf16) > 1) of(std::integral_constant<int, 2>{});
+            else of(std::integral_constant<int, 1>{});
             break;
         }
         case wh_rows_mm_plan::kTile: {
