@@ -427,7 +427,8 @@ constexpr uint32_t kThinWaves = 8;
 template <int kMt, int kNt, bool kBf16, bool kMant>
 __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part)[64][4], uint32_t ks_n, uint32_t g, uint32_t j0,
                                           uint32_t j1, uint32_t c0) {
-    constexpr int kU = kMt * kNt == 1 ? 4 : kMt * kNt == 2 ? 2 : 1;
+    // blocks whose weights, and whose x, are asked for at once
+    constexpr int kU = kMt * kNt == 1 ? 4 : kMt * kNt == 2 && (kBf16 || kNt == 2) ? 2 : 1, kW = kNt == 2 || kMt == 4 ? kU : 4;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t ks = wave & (ks_n - 1), l16 = lane & 15, q = lane >> 4;
     const uint32_t blocks = a.cols / 128u, col0 = c0 + 16 * kNt * (wave / ks_n);
@@ -458,11 +459,11 @@ __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part
             bits[i] = rows_scale_bits(a, (w_row + min(16u * i, a.out_rows - 1 - col0)) / a.row_block * blocks +
                                              min(first + lane, blocks - 1));
         }
-        for (uint32_t i0 = 0; i0 < mine; i0 += kU) {
-            rows_frag w[kU][kNt], x[kU][kMt];
+        for (uint32_t i0 = 0; i0 < mine; i0 += kW) {
+            rows_frag w[kW][kNt];
             uint32_t x0[kMt], x1[kMt];  // the words of the rows' scales that hold these blocks'
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
+            for (int u = 0; u < kW; ++u) {
                 const uint32_t b = first + min(i0 + u, mine - 1);
 #pragma unroll
                 for (int i = 0; i < kNt; ++i) {
@@ -482,54 +483,63 @@ __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part
             }
             const uint32_t b0 = first + i0, word = b0 / 4, at = b0 & 3;
 #pragma unroll
-            for (int t = 0; t < kMt; ++t) {
+            for (int v = 0; v < kW; v += kU) {
+                rows_frag x[kU][kMt];
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
-                    const uint32_t b = first + min(i0 + u, mine - 1);
-                    x[u][t].a = *(const wh_u4*)(xp[t] + b * 128u);
-                    x[u][t].b = *(const wh_u4*)(xp[t] + b * 128u + 64);
+                    const uint32_t b = first + min(i0 + v + u, mine - 1);
+#pragma unroll
+                    for (int t = 0; t < kMt; ++t) {
+                        x[u][t].a = *(const wh_u4*)(xp[t] + b * 128u);
+                        x[u][t].b = *(const wh_u4*)(xp[t] + b * 128u + 64);
+                    }
                 }
-                x0[t] = ((const uint32_t*)xs[t])[word];
-                x1[t] = 0;
-            }
-            if (at + kU > 4) {
+                if (v == 0) {
 #pragma unroll
-                for (int t = 0; t < kMt; ++t) x1[t] = ((const uint32_t*)xs[t])[min(word + 1, (blocks - 1) / 4)];
-            }
+                    for (int t = 0; t < kMt; ++t) {
+                        x0[t] = ((const uint32_t*)xs[t])[word];
+                        x1[t] = 0;
+                    }
+                    if (at + kW > 4) {
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                if (i0 + u < mine) {
-                    uint32_t xb[kMt];
+                        for (int t = 0; t < kMt; ++t) x1[t] = ((const uint32_t*)xs[t])[min(word + 1, (blocks - 1) / 4)];
+                    }
+                }
 #pragma unroll
-                    for (int t = 0; t < kMt; ++t) xb[t] = __builtin_amdgcn_alignbyte(x1[t], x0[t], at) >> 8 * u & 0xff;
+                for (int u = 0; u < kU; ++u) {
+                    if (i0 + v + u < mine) {
+                        uint32_t xb[kMt];
 #pragma unroll
-                    for (int i = 0; i < kNt; ++i) {
-                        const int byte = __builtin_amdgcn_readlane((int)wb[i], i0 + u);
-                        const float m = kMant ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wm[i]), i0 + u)) : 1.0f;
-                        if constexpr (kBf16) {
-                            const wh_i8 wc = rows_codes(w[u][i]);
+                        for (int t = 0; t < kMt; ++t) xb[t] = __builtin_amdgcn_alignbyte(x1[t], x0[t], at) >> 8 * (v + u) & 0xff;
 #pragma unroll
-                            for (int t = 0; t < kMt; ++t) {
-                                const wh_f4 from = kMant ? wh_f4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][t];
-                                const wh_f4 s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wc, rows_codes(x[u][t]), from, 0,
-                                                                                                 0, 0, byte, 0, (int)xb[t]);
-                                if constexpr (kMant) {
+                        for (int i = 0; i < kNt; ++i) {
+                            const int byte = __builtin_amdgcn_readlane((int)wb[i], i0 + v + u);
+                            const float m = kMant ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wm[i]), i0 + v + u)) : 1.0f;
+                            if constexpr (kBf16) {
+                                const wh_i8 wc = rows_codes(w[v + u][i]);
 #pragma unroll
-                                    for (int k = 0; k < 4; ++k) acc[i][t][k] = fmaf(s[k], m, acc[i][t][k]);
-                                } else {
-                                    acc[i][t] = s;
+                                for (int t = 0; t < kMt; ++t) {
+                                    const wh_f4 from = kMant ? wh_f4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][t];
+                                    const wh_f4 s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                                        wc, rows_codes(x[u][t]), from, 0, 0, 0, byte, 0, (int)xb[t]);
+                                    if constexpr (kMant) {
+#pragma unroll
+                                        for (int k = 0; k < 4; ++k) acc[i][t][k] = fmaf(s[k], m, acc[i][t][k]);
+                                    } else {
+                                        acc[i][t] = s;
+                                    }
                                 }
-                            }
-                        } else {
-                            const rows_f16x4 wv = rows_decode(w[u][i]);
+                            } else {
+                                const rows_f16x4 wv = rows_decode(w[v + u][i]);
 #pragma unroll
-                            for (int t = 0; t < kMt; ++t) {
-                                const rows_f16x4 xv = rows_decode(x[u][t]);
-                                wh_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+                                for (int t = 0; t < kMt; ++t) {
+                                    const rows_f16x4 xv = rows_decode(x[u][t]);
+                                    wh_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv.v[j], xv.v[j], s, 0, 0, 0);
-                                acc[i][t] = rows_scaled(acc[i][t], s, (int)xb[t] + byte - 254, m);
-                                nan[t] |= xb[t] == 255;
+                                    for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv.v[j], xv.v[j], s, 0, 0, 0);
+                                    acc[i][t] = rows_scaled(acc[i][t], s, (int)xb[t] + byte - 254, m);
+                                    nan[t] |= xb[t] == 255;
+                                }
                             }
                         }
                     }
