@@ -1454,7 +1454,7 @@ hipError_t wh_rows_read_launch(const wh_rows_read_args& a, bool bf16, hipStream_
 // Which kernel takes a product, and how many ranges its columns are cut into: the least
 // of these estimates of its time in us, fitted to 400 measured calls (one MI355X; 1 to
 // 4096 rows, 1 to 64 groups, weights from 1408 x 512 to 32768 x 1024 and 4096 x 8192).
-//  - thin: a wave's block of columns takes 0.8, 1.6 and 3 us for up to 16, 32 and 64
+//  - thin: a wave's block of columns takes 0.8, 1.05 and 3 us for up to 16, 32 and 64
 //    rows (with groups of uneven lists 0.55 and 0.045 a row), workgroups in rounds of 256:
 //    4096 x 4096 with 16, 64 and 128 rows 7.2, 15.6 and 29, where tiles take 23 to 25, cut
 //    up 13 to 18; 64 groups with 4, 16 and 32 rows each in f32 228, 343 and 505, tiles 281,
@@ -1480,7 +1480,7 @@ wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
         const uint32_t each = 16 * (kThinWaves / rows_thin_split(a));
         const double left = rows - 64 * std::floor(rows / 64);
         const double chunk = a.n_groups > 1 ? 0.55 + 0.045 * rows
-                                            : 3.0 * std::floor(rows / 64) + (left == 0 ? 0 : left <= 16 ? 0.8 : left <= 32 ? 1.6 : 3.0);
+                                            : 3.0 * std::floor(rows / 64) + (left == 0 ? 0 : left <= 16 ? 0.8 : left <= 32 ? 1.05 : 3.0);
         double best = 3.5 + std::max(1.0, groups * ((a.out_rows + each - 1) / each) / 256) *
                                 std::ceil((double)blocks / rows_thin_split(a)) * chunk;
         p.kind = wh_rows_mm_plan::kThin;
