@@ -4,8 +4,8 @@ plain computations in 64 bits.
 
 Tolerances, u = 2^-24 a rounding to f32, S = sum |w||x| of an output:
   codes and scales are whole numbers: equal.  Behind SwiGLU, whose f32 steps
-  (exp 2 u, sum, quotient and three products) leave 8 u, a value nearer than
-  that to a border between codes may get the code beside its own;
+  (exp 3 u, sum 1 u, reciprocal 1.5 u, three products) leave 8.5 u, a value nearer
+  than 16 u to a border between codes may get the code beside its own;
   f32 products: products of codes are exact; a sum of cols terms in any order is
   within cols u S, two scale steps and the sum over parts 8 u S more;
   bf16 products: the 8-bit matrix instructions align eight products to the
@@ -244,6 +244,31 @@ def test_swiglu_rows(ctx, n, cols, limit, bf16):
     sure = margin > 2 * 8 * U
     assert np.array_equal(got[sure], codes[sure])
     assert np.abs((got & 127).astype(int) - (codes & 127)).max() <= 1 and sure.mean() > 0.99
+
+
+@pytest.mark.parametrize("limit", [10.0, np.inf])
+def test_swiglu_of_infinities_and_nan(ctx, limit):
+    """They become NaN, or what the clamps make of them, and leave the rest alone; some
+    lanes take exp of ordinary gates, others of far ones."""
+    rng = np.random.default_rng(6)
+    x = np.clip(some(rng, 4, 512), -80, 80)
+    x[0, [3, 130, 140]] = np.nan, np.inf, -np.inf
+    x[1, [256 + 5, 256 + 133, 256 + 150]] = np.nan, np.inf, -np.inf
+    x[2, :256], x[3, 9], x[3, 256 + 9] = np.nan, -90.0, np.nan
+    t = dev(x)
+    rows = Rows(4, 256)
+    ctx.fp8_swiglu_rows_async(t.data_ptr(), t.data_ptr() + 1024, 512, False, 4, 256, limit, rows.c)
+    ctx.synchronize()
+    g, u = x[:, :256].astype(np.float64), x[:, 256:].astype(np.float64)
+    with np.errstate(all="ignore"):
+        g = np.minimum(g, limit)
+        v = g / (1 + np.exp(-g)) * np.clip(u, -limit, limit)
+    codes, scales, margin = quantise(v)
+    got, got_s = rows.get()
+    assert np.array_equal(got_s, scales)
+    assert np.array_equal((got & 127) == 127, ~np.isfinite(v))
+    sure = np.isfinite(v) & (margin > 2 * 8 * U)
+    assert sure.sum() > 700 and np.array_equal(got[sure], codes[sure])
 
 
 def test_swiglu_where_exp_leaves_f32(ctx):
