@@ -1029,6 +1029,14 @@ int wh_fp8_rows_mm_groups_async(wh_ctx* ctx, wh_tensor w, size_t row_start, size
                                 const wh_fp8_rows* x, size_t n_x, const uint32_t* rows_dev, const uint32_t* starts_dev,
                                 size_t n, void* y_dev, size_t y_stride, int is_bf16);
 
+/* Test support, host only: how a product of such sizes is done, for a tensor whose
+ * scales are shared by 128 rows, from its first row on.  lists: grouped by expert;
+ * special: the tensor has codes 0x7F / 0xFF.  plan: [0] the kernel (0 vector, 1
+ * thin, 2 tiles of 128 x 128, 3 of 128 x 256, 4 of 256 x 256), [1] ranges of
+ * columns, [2] workgroups of each, [3] most tiles that such a call can have. */
+int wh_debug_fp8_rows_plan(size_t n, size_t n_groups, int lists, size_t group_rows, size_t cols, int scale_f32, int special,
+                           int is_bf16, uint64_t plan[4]);
+
 /* Expert lists of npos positions' routes ids_dev [npos][topk]: an id of
  * n_experts or more is no expert (padding, an expert elsewhere).  Expert e's
  * list is starts_dev[e] .. starts_dev[e + 1] (starts_dev [n_experts + 1]), its

@@ -105,6 +105,7 @@ EXPORTED = (
     "wh_kv_plan_async", "wh_kv4_write_async", "wh_kv4_read_async", "wh_kv4_attention_async",
     "wh_store_fp8_device", "wh_fp8_quant_rows_async", "wh_fp8_swiglu_rows_async", "wh_fp8_read_rows_async",
     "wh_fp8_rows_mm_async", "wh_fp8_rows_mm_groups_async", "wh_expert_plan_async", "wh_expert_combine_async",
+    "wh_debug_fp8_rows_plan",
 )
 
 ROUTER_RAW_LOGITS = 0
@@ -333,6 +334,7 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         "wh_fp8_rows_mm_async": (c.c_int, [vp, c.c_uint64, sz, sz, c.POINTER(WhFp8Rows), sz, vp, sz, c.c_int]),
         "wh_fp8_rows_mm_groups_async": (c.c_int, [vp, c.c_uint64, sz, sz, sz, c.POINTER(WhFp8Rows), sz, vp, vp, sz, vp,
                                                   sz, c.c_int]),
+        "wh_debug_fp8_rows_plan": (c.c_int, [sz, sz, c.c_int, sz, sz, c.c_int, c.c_int, c.c_int, c.POINTER(c.c_uint64)]),
         "wh_expert_plan_async": (c.c_int, [vp, vp, sz, sz, sz, vp, vp, vp]),
         "wh_expert_combine_async": (c.c_int, [vp, vp, sz, c.c_int, sz, vp, vp, sz, sz, sz, vp, sz, vp, sz]),
         "wh_route_experts_async": (c.c_int, [vp, c.c_uint32, vp, sz, sz, vp, sz, c.POINTER(WhRouteOptions), vp, vp,

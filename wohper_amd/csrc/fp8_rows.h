@@ -60,6 +60,7 @@ struct wh_rows_mm_plan {
     enum kind_t { kAny, kThin, kTile, kHalf, kTall } kind;
     uint32_t splits, per;  // ranges that its columns are cut into, and blocks of each
     uint32_t threads;
+    uint64_t tiles;        // at most, of the kernel's
     uint64_t grid;         // workgroups for each range
     size_t part_bytes;     // scratch for the ranges' parts
     bool fits;             // within the limits of a launch

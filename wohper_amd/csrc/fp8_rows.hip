@@ -1469,7 +1469,7 @@ hipError_t wh_rows_read_launch(const wh_rows_read_args& a, bool bf16, hipStream_
 wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
     const uint32_t blocks = a.cols / 128u;
     const bool mant = a.scale_f32 || a.odd_scale;
-    wh_rows_mm_plan p{wh_rows_mm_plan::kAny, 1, blocks, 256, 0, 0, false};
+    wh_rows_mm_plan p{wh_rows_mm_plan::kAny, 1, blocks, 256, 0, 0, 0, false};
     const double groups = std::min(a.n_groups, a.n), rows = a.n / groups;
     // tiles, of groups that end in a tile half full on average
     auto tiles = [&](double m, uint32_t n) {
@@ -1512,16 +1512,16 @@ wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
         }
     }
     switch (p.kind) {
-        case wh_rows_mm_plan::kAny: p.grid = most(kAnyRows, 16); break;
+        case wh_rows_mm_plan::kAny: p.grid = p.tiles = most(kAnyRows, 16); break;
         case wh_rows_mm_plan::kThin: {
             p.threads = 64 * kThinWaves;
             const uint32_t each = 16 * (kThinWaves / rows_thin_split(a)) * rows_thin_tiles(a, bf16);
-            p.grid = (uint64_t)((a.out_rows + each - 1) / each) * a.n_groups;
+            p.grid = p.tiles = (uint64_t)((a.out_rows + each - 1) / each) * a.n_groups;
             break;
         }
-        case wh_rows_mm_plan::kTile: p.grid = (most(128, 128) + 7) / 8 * 8; break;
-        case wh_rows_mm_plan::kHalf: p.grid = std::min<uint64_t>((most(128, 256) + 7) / 8 * 8, g_workgroups.load()); break;
-        case wh_rows_mm_plan::kTall: p.grid = std::min<uint64_t>((most(256, 256) + 7) / 8 * 8, g_workgroups.load()); break;
+        case wh_rows_mm_plan::kTile: p.grid = ((p.tiles = most(128, 128)) + 7) / 8 * 8; break;
+        case wh_rows_mm_plan::kHalf: p.grid = std::min<uint64_t>(((p.tiles = most(128, 256)) + 7) / 8 * 8, g_workgroups.load()); break;
+        case wh_rows_mm_plan::kTall: p.grid = std::min<uint64_t>(((p.tiles = most(256, 256)) + 7) / 8 * 8, g_workgroups.load()); break;
     }
     if (p.splits > 1) p.part_bytes = (size_t)p.splits * a.n * rows_part_stride(a) * sizeof(float);
     p.fits = p.grid * p.threads * p.splits <= 0xffffffffull;  // a grid's threads

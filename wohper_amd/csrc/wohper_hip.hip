@@ -5024,6 +5024,31 @@ int wh_fp8_rows_mm_groups_async(wh_ctx* c, wh_tensor w, size_t row_start, size_t
     return rows_mm_go(c, *t, row_start, a, is_bf16);
 }
 
+int wh_debug_fp8_rows_plan(size_t n, size_t n_groups, int lists, size_t group_rows, size_t cols, int scale_f32, int special,
+                           int is_bf16, uint64_t plan[4]) {
+    if (!plan) return WH_INVALID_ARGUMENT;
+    if (n == 0 || n_groups == 0 || group_rows == 0 || cols == 0) return WH_EMPTY_SHAPE;
+    if (cols % 128) return WH_INVALID_SHAPE;
+    if (n > 0x7fffffffu || n_groups > WH_ROWS_MAX_GROUPS || group_rows > 0xffffffffu / n_groups || cols > 0xffffff80u)
+        return WH_UNSUPPORTED;
+    static const uint32_t some = 0;  // the plan asks only whether there are lists
+    wh_rows_mm_args a{};
+    a.starts = lists ? &some : nullptr;
+    a.n = a.n_x = (uint32_t)n;
+    a.n_groups = (uint32_t)n_groups;
+    a.out_rows = (uint32_t)group_rows;
+    a.cols = (uint32_t)cols;
+    a.row_block = 128;
+    a.scale_f32 = scale_f32 != 0;
+    a.special = special != 0;
+    const wh_rows_mm_plan p = wh_rows_mm_plan_of(a, is_bf16 != 0);
+    plan[0] = p.kind;
+    plan[1] = p.splits;
+    plan[2] = p.grid;
+    plan[3] = p.tiles;
+    return p.fits ? WH_OK : WH_UNSUPPORTED;
+}
+
 int wh_expert_plan_async(wh_ctx* c, const uint32_t* ids_dev, size_t npos, size_t topk, size_t n_experts,
                          uint32_t* starts_dev, uint32_t* rows_dev, uint32_t* slots_dev) {
     if (!c || !starts_dev) return WH_INVALID_ARGUMENT;
