@@ -38,3 +38,14 @@ def test_refusals():
         assert lib.wh_debug_fp8_rows_plan(sizes[0], sizes[1], 0, sizes[2], sizes[3], 0, 0, 0, p) == EMPTY
     assert plan(1, 16, 192)[0] == SHAPE
     assert plan(1 << 31, 16, 128)[0] == plan(1, 1 << 23, 128, groups=1024)[0] == plan(1, 16, 128, groups=1025)[0] == UNSUPPORTED
+
+
+@pytest.mark.parametrize("n,rows,cols,groups", [(65600, 65552, 128, 0), (1 << 21, 1 << 16, 128, 0), (3, 1 << 30, 128, 0),
+                                                ((1 << 31) - 1, 16, 256, 0), (1 << 24, 1 << 13, 128, 1024), (1 << 20, 1 << 18, 640, 64)])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_sizes_that_are_taken_do_not_depend_on_codes(n, rows, cols, groups, bf16):
+    """Above 2^32 outputs too, a thread each in the vector kernel."""
+    for special in (False, True):
+        status, kind, splits, grid, tiles = plan(n, rows, cols, groups, special=special, bf16=bf16)
+        assert status == 0 and grid * splits * (512 if kind == THIN else 256) < 1 << 32
+        assert kind == VECTOR if special else grid >= tiles or kind in (VECTOR, HALF, TALL)

@@ -63,7 +63,6 @@ struct wh_rows_mm_plan {
     uint64_t tiles;        // at most, of the kernel's
     uint64_t grid;         // workgroups for each range
     size_t part_bytes;     // scratch for the ranges' parts
-    bool fits;             // within the limits of a launch
 };
 wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16);
 hipError_t wh_rows_mm_launch(const wh_rows_mm_args& a, const wh_rows_mm_plan& p, bool bf16, hipStream_t stream);

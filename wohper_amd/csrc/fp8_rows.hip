@@ -239,6 +239,13 @@ __device__ __forceinline__ bool rows_tile(const wh_rows_mm_args& a, uint32_t t, 
     return false;
 }
 
+// Most tiles of `rows` listed rows that a call can have.
+__host__ __device__ __forceinline__ uint64_t rows_tiles(const wh_rows_mm_args& a, uint32_t rows) {
+    const uint64_t full = ((uint64_t)a.n + rows - 1) / rows;
+    // each group may end in a tile that is not full, and has at least a row then
+    return a.starts ? full + (a.n_groups < a.n ? a.n_groups : a.n) : full;
+}
+
 // Scale of weight row `row` in block b as mantissa * 2^exponent, so that its
 // product with a row's power of two leaves f32's range only where the result does.
 __device__ __forceinline__ float rows_w_scale(const wh_rows_mm_args& a, uint64_t row, uint32_t b, int* e) {
@@ -264,16 +271,15 @@ __device__ __forceinline__ void rows_put(const wh_rows_mm_args& a, uint64_t row,
 // Any product: 16 x 16 outputs a workgroup, one a thread, the block's values of
 // both sides decoded into LDS.  For what the matrix instructions read otherwise or
 // do not take: weight codes 0x7F / 0xFF (+-480 here, NaN there) and scales shared
-// by a number of rows that is no multiple of 16.  Bound by LDS reads and vector
-// products: 5 x 4096 x 8192 in f32 101 us, 4096 x 4096 x 8192 26 ms.
+// by a number of rows that is no multiple of 16, and for sizes whose tiles there are more
+// than a launch has threads for.  A workgroup here takes further tiles where they are more
+// than a grid has workgroups, so it takes any sizes, whatever the weight's codes.  Bound by LDS reads and vector products: 5 x 4096 x 8192
+// in f32 95 us, 4096 x 4096 x 8192 25 ms.
 constexpr uint32_t kAnyRows = 16;
 template <bool kBf16>
-__global__ void __launch_bounds__(256) k_rows_mm_any(wh_rows_mm_args a) {
-    __shared__ float xs[kAnyRows][132], ws[16][132];
-    const uint32_t n_cols = (a.out_rows + 15) / 16, t = threadIdx.x, lane16 = t & 15, row16 = t >> 4;
-    uint32_t g = 0, r0 = 0, r1 = 0;
-    if (!rows_tile<kAnyRows>(a, blockIdx.x / n_cols, g, r0, r1)) return;
-    const uint32_t c0 = (blockIdx.x % n_cols) * 16;
+__device__ __forceinline__ void rows_any(const wh_rows_mm_args& a, float (*xs)[132], float (*ws)[132], uint32_t g, uint32_t r0,
+                                         uint32_t r1, uint32_t c0) {
+    const uint32_t t = threadIdx.x, lane16 = t & 15, row16 = t >> 4;
     const uint64_t w0 = a.row_start + (uint64_t)g * a.out_rows;
     // staging: thread (row16, lane16) brings 8 codes of row row16 of both sides
     uint32_t src = 0;
@@ -311,6 +317,18 @@ __global__ void __launch_bounds__(256) k_rows_mm_any(wh_rows_mm_args a) {
         }
     }
     if (r0 + row16 < r1 && c0 + lane16 < a.out_rows) rows_put<kBf16>(a, r0 + row16, c0 + lane16, acc);
+}
+
+template <bool kBf16>
+__global__ void __launch_bounds__(256) k_rows_mm_any(wh_rows_mm_args a) {
+    __shared__ float xs[kAnyRows][132], ws[16][132];
+    const uint32_t n_cols = (a.out_rows + 15) / 16;
+    const uint64_t tiles = rows_tiles(a, kAnyRows) * n_cols;
+    for (uint64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        uint32_t g = 0, r0 = 0, r1 = 0;
+        if (!rows_tile<kAnyRows>(a, (uint32_t)(tile / n_cols), g, r0, r1)) return;
+        rows_any<kBf16>(a, xs, ws, g, r0, r1, (uint32_t)(tile % n_cols) * 16);
+    }
 }
 
 // ------------------------------------------------- matrix instructions
@@ -1183,13 +1201,6 @@ bool rows_mm_matrix(const wh_rows_mm_args& a) {
     return !a.special && a.row_block % 16 == 0 && a.row_start % 16 == 0 && (a.out_rows % 16 == 0 || a.n_groups == 1);
 }
 
-// Most tiles of kRows listed rows that a call can have.
-uint64_t rows_tiles(const wh_rows_mm_args& a, uint32_t rows) {
-    const uint64_t full = ((uint64_t)a.n + rows - 1) / rows;
-    // each group may end in a tile that is not full, and has at least a row then
-    return a.starts ? full + std::min<uint64_t>(a.n_groups, a.n) : full;
-}
-
 // ------------------------------------------------------------------ store
 
 // Row-major codes into the store's order, and whether one is 0x7F or 0xFF.
@@ -1469,7 +1480,7 @@ hipError_t wh_rows_read_launch(const wh_rows_read_args& a, bool bf16, hipStream_
 wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
     const uint32_t blocks = a.cols / 128u;
     const bool mant = a.scale_f32 || a.odd_scale;
-    wh_rows_mm_plan p{wh_rows_mm_plan::kAny, 1, blocks, 256, 0, 0, 0, false};
+    wh_rows_mm_plan p{wh_rows_mm_plan::kAny, 1, blocks, 256, 0, 0, 0};
     const double groups = std::min(a.n_groups, a.n), rows = a.n / groups;
     // tiles, of groups that end in a tile half full on average
     auto tiles = [&](double m, uint32_t n) {
@@ -1511,20 +1522,29 @@ wh_rows_mm_plan wh_rows_mm_plan_of(const wh_rows_mm_args& a, bool bf16) {
                   wh_rows_mm_plan::kTall, 1, blocks);
         }
     }
-    switch (p.kind) {
-        case wh_rows_mm_plan::kAny: p.grid = p.tiles = most(kAnyRows, 16); break;
-        case wh_rows_mm_plan::kThin: {
-            p.threads = 64 * kThinWaves;
-            const uint32_t each = 16 * (kThinWaves / rows_thin_split(a)) * rows_thin_tiles(a, bf16);
-            p.grid = p.tiles = (uint64_t)((a.out_rows + each - 1) / each) * a.n_groups;
-            break;
+    auto size = [&] {
+        switch (p.kind) {
+            case wh_rows_mm_plan::kAny: p.grid = std::min(p.tiles = most(kAnyRows, 16), kMaxGrid256); break;
+            case wh_rows_mm_plan::kThin: {
+                p.threads = 64 * kThinWaves;
+                const uint32_t each = 16 * (kThinWaves / rows_thin_split(a)) * rows_thin_tiles(a, bf16);
+                p.grid = p.tiles = (uint64_t)((a.out_rows + each - 1) / each) * a.n_groups;
+                break;
+            }
+            case wh_rows_mm_plan::kTile: p.grid = ((p.tiles = most(128, 128)) + 7) / 8 * 8; break;
+            case wh_rows_mm_plan::kHalf: p.grid = std::min<uint64_t>(((p.tiles = most(128, 256)) + 7) / 8 * 8, g_workgroups.load()); break;
+            case wh_rows_mm_plan::kTall: p.grid = std::min<uint64_t>(((p.tiles = most(256, 256)) + 7) / 8 * 8, g_workgroups.load()); break;
         }
-        case wh_rows_mm_plan::kTile: p.grid = ((p.tiles = most(128, 128)) + 7) / 8 * 8; break;
-        case wh_rows_mm_plan::kHalf: p.grid = std::min<uint64_t>(((p.tiles = most(128, 256)) + 7) / 8 * 8, g_workgroups.load()); break;
-        case wh_rows_mm_plan::kTall: p.grid = std::min<uint64_t>(((p.tiles = most(256, 256)) + 7) / 8 * 8, g_workgroups.load()); break;
+    };
+    size();
+    if (p.grid * p.threads * p.splits > 0xffffffffull) {  // a grid's threads: the vector kernel takes any number of tiles
+        p.kind = wh_rows_mm_plan::kAny;
+        p.splits = 1;
+        p.per = blocks;
+        p.threads = 256;
+        size();
     }
     if (p.splits > 1) p.part_bytes = (size_t)p.splits * a.n * rows_part_stride(a) * sizeof(float);
-    p.fits = p.grid * p.threads * p.splits <= 0xffffffffull;  // a grid's threads
     return p;
 }
 

@@ -4948,7 +4948,6 @@ int rows_mm_go(wh_ctx* c, const Tensor& t, size_t row_start, wh_rows_mm_args& a,
     a.odd_scale = t.odd_scale;
     a.tickets = c->rows_tickets.as<uint32_t>();
     const wh_rows_mm_plan p = wh_rows_mm_plan_of(a, bf16 != 0);
-    if (!p.fits) return WH_UNSUPPORTED;
     WH_HIP(hipSetDevice(c->device));
     WH_HIP(c->rows_part.ensure(p.part_bytes, false));
     a.part = c->rows_part.as<float>();
@@ -5046,7 +5045,7 @@ int wh_debug_fp8_rows_plan(size_t n, size_t n_groups, int lists, size_t group_ro
     plan[1] = p.splits;
     plan[2] = p.grid;
     plan[3] = p.tiles;
-    return p.fits ? WH_OK : WH_UNSUPPORTED;
+    return WH_OK;
 }
 
 int wh_expert_plan_async(wh_ctx* c, const uint32_t* ids_dev, size_t npos, size_t topk, size_t n_experts,
