@@ -1,5 +1,7 @@
-"""8-bit rows at the ends of what their calls take: sizes that pass a launch's threads.
-Tolerances as in test_gpu_fp8_rows."""
+"""8-bit rows at the ends of what their calls take: sizes that pass a launch's threads,
+many routes.  Tolerances as in test_gpu_fp8_rows."""
+import time
+
 import pytest
 import torch
 
@@ -30,3 +32,61 @@ def test_products_of_more_outputs_than_a_launch_has_threads(ctx, special):
     for a, b in ((0, 20), (40000, 40001), (rows - 17, rows)):
         gpu_near(y[:n, a:b], x, w[a:b], True, cols)
     c.close()
+
+
+class Routes:
+    """Random routes, an eighth of them to no expert, and a plan's buffers."""
+
+    def __init__(self, npos, topk, n_experts, seed=0):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        self.npos, self.topk, self.n_experts, n = npos, topk, n_experts, npos * topk
+        self.ids = torch.randint(0, n_experts + n_experts // 8 + 1, (n,), generator=g, device="cuda", dtype=torch.int32)
+        self.ids[n // 2:n // 2 + 3] = -1
+        self.starts, self.rows, self.slots = (torch.full((k + 1,), 77, dtype=torch.int32, device="cuda")
+                                              for k in (n_experts + 1, n, n))
+
+    def run(self, ctx):
+        ctx.expert_plan_async(self.ids.data_ptr(), self.npos, self.topk, self.n_experts, self.starts.data_ptr(),
+                              self.rows.data_ptr(), self.slots.data_ptr())
+
+
+@pytest.mark.parametrize("npos,topk,n_experts", [(1 << 20, 1, 256), ((1 << 20) - 4096, 1, 300), (1050001, 1, 1), (700001, 3, 5),
+                                                 (1000003, 5, 1023), (3000000, 2, 1024), (2500000, 8, 17)])
+def test_plans_of_many_routes(ctx, npos, topk, n_experts):
+    """From 256 chunks of 4096 routes on, the chunks' counts are added up by a launch of its own."""
+    r = Routes(npos, topk, n_experts)
+    for _ in range(2):
+        r.run(ctx)
+    ctx.synchronize()
+    n = npos * topk
+    key = torch.where((r.ids >= 0) & (r.ids < n_experts), r.ids, n_experts).long()
+    order = torch.argsort(key, stable=True)
+    starts = torch.cat([key.new_zeros(1), torch.bincount(key, minlength=n_experts + 1)[:n_experts].cumsum(0)])
+    listed = int(starts[-1])
+    slots = torch.full_like(key, -1)
+    slots[order[:listed]] = torch.arange(listed, device="cuda")
+    rows = torch.full_like(key, -1)
+    rows[:listed] = order[:listed] // topk
+    assert torch.equal(r.starts[:-1].long(), starts)
+    assert torch.equal(r.rows[:-1].long(), rows) and torch.equal(r.slots[:-1].long(), slots)
+    assert r.starts[-1] == r.rows[-1] == r.slots[-1] == 77
+
+
+def test_a_plan_costs_what_its_routes_do(ctx):
+    """Eight times the routes: about eight times as long, where every chunk that adds up
+    all others' counts takes 64 times."""
+    took = []
+    for npos in (1 << 20, 1 << 23):
+        r = Routes(npos, 8, 1024)
+        r.run(ctx)
+        ctx.synchronize()
+        best = 1e9
+        for _ in range(5):
+            torch.cuda.synchronize()
+            t = time.perf_counter()
+            r.run(ctx)
+            ctx.raw.synchronize()
+            best = min(best, time.perf_counter() - t)
+        took.append(best)
+    assert took[1] <= 24 * took[0]

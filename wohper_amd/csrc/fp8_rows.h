@@ -79,7 +79,7 @@ hipError_t wh_rows_scales_launch(const uint8_t* scales, uint64_t n, uint32_t* fl
 struct wh_expert_plan_args {
     const uint32_t* ids;
     uint32_t *starts, *rows, *slots;
-    uint32_t* counts;  // scratch [chunks][n_groups, padded to 4], where there is more than one chunk
+    uint32_t* counts;  // scratch [chunks + 1][n_groups, padded to 4], where there is more than one chunk
     uint32_t n, topk, n_groups;
 };
 size_t wh_expert_plan_scratch(size_t n, size_t n_groups);

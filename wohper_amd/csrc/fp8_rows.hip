@@ -1267,19 +1267,48 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_count(wh_expert_plan_ar
     for (uint32_t e = threadIdx.x; e < padded; e += kPlanThreads) a.counts[(uint64_t)blockIdx.x * padded + e] = count[e];
 }
 
+// The counts of each expert become those of the chunks before, and the sum of all in a row
+// behind the last.  A workgroup takes 16 experts, a thread a run of chunks of one.
+constexpr uint32_t kSumExperts = 16, kSumRuns = 64;
+__global__ void __launch_bounds__(kSumExperts* kSumRuns) k_expert_sum(wh_expert_plan_args a, uint32_t chunks) {
+    __shared__ uint32_t run_sum[kSumRuns][kSumExperts];
+    const uint32_t padded = plan_padded(a.n_groups), in = threadIdx.x % kSumExperts, run = threadIdx.x / kSumExperts;
+    const uint32_t e = blockIdx.x * kSumExperts + in, len = (chunks + kSumRuns - 1) / kSumRuns;
+    const uint32_t from = min(run * len, chunks), to = e < padded ? min(from + len, chunks) : from;
+    uint32_t* const at = a.counts + e;
+    uint32_t sum = 0;
+#pragma unroll 8
+    for (uint32_t c = from; c < to; ++c) sum += at[(uint64_t)c * padded];
+    run_sum[run][in] = sum;
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t r = 0; r < run; ++r) before += run_sum[r][in];
+    if (run == kSumRuns - 1 && e < padded) at[(uint64_t)chunks * padded] = before + sum;
+#pragma unroll 8
+    for (uint32_t c = from; c < to; ++c) {
+        const uint32_t v = at[(uint64_t)c * padded];
+        at[(uint64_t)c * padded] = before;
+        before += v;
+    }
+}
+
 // Expert lists: a counting sort that keeps the order of routes.  A workgroup takes a
 // chunk of routes, a wave consecutive ones 64 at a time; lanes of the same expert find
 // each other by ballots over the id's bits, so a route's place is the expert's start, its
 // routes of chunks and waves before, of this wave so far, and of lanes before.  With one
-// chunk this is the only launch.
-template <uint32_t kTurns>
+// chunk this is the only launch.  kSummed: k_expert_sum has added the chunks' counts up.
+template <uint32_t kTurns, bool kSummed>
 __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_args a, uint32_t chunks, uint32_t bits) {
     extern __shared__ uint32_t lds[];
     uint32_t* const at = lds;  // [kPlanWaves][n_groups]: counts, then next places of a wave
     __shared__ uint32_t wave_sum[kPlanWaves], all_of[WH_ROWS_MAX_GROUPS], before_of[WH_ROWS_MAX_GROUPS], listed;
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, E = a.n_groups;
     for (uint32_t i = t; i < kPlanWaves * E; i += kPlanThreads) at[i] = 0;
-    if (t < E) all_of[t] = before_of[t] = 0;
+    if (t < E) {
+        const uint32_t padded = plan_padded(E);
+        all_of[t] = kSummed ? a.counts[(uint64_t)chunks * padded + t] : 0;
+        before_of[t] = kSummed ? a.counts[(uint64_t)blockIdx.x * padded + t] : 0;
+    }
     const uint32_t from = blockIdx.x * plan_chunk(kTurns) + wave * 64 * kTurns;
     uint32_t id[kTurns];
     uint64_t same[kTurns];
@@ -1291,7 +1320,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_expert_place(wh_expert_plan_ar
     __syncthreads();
     // all chunks' routes of four experts a lane, and those before this chunk: the chunks
     // are dealt out to waves, or to as many waves together as hold all experts
-    if (chunks > 1) {
+    if (!kSummed && chunks > 1) {
         const uint32_t fours = plan_padded(E) / 4;
         uint32_t shift = 6;
         while (1u << shift < fours) ++shift;
@@ -1427,9 +1456,10 @@ hipError_t wh_rows_setup() {
     auto tile = [&](const void* f, size_t lds) {
         if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     };
-    tile((const void*)k_expert_place<1>, plan_lds(WH_ROWS_MAX_GROUPS));
-    tile((const void*)k_expert_place<2>, plan_lds(WH_ROWS_MAX_GROUPS));
-    tile((const void*)k_expert_place<4>, plan_lds(WH_ROWS_MAX_GROUPS));
+    tile((const void*)k_expert_place<1, false>, plan_lds(WH_ROWS_MAX_GROUPS));
+    tile((const void*)k_expert_place<2, false>, plan_lds(WH_ROWS_MAX_GROUPS));
+    tile((const void*)k_expert_place<4, false>, plan_lds(WH_ROWS_MAX_GROUPS));
+    tile((const void*)k_expert_place<4, true>, plan_lds(WH_ROWS_MAX_GROUPS));
     constexpr size_t lds = rows_tile_shape<4, 4, 2, 2>::kLds;
     tile((const void*)k_rows_mm_tile<true, true>, lds);
     tile((const void*)k_rows_mm_tile<true, false>, lds);
@@ -1634,9 +1664,15 @@ static uint32_t plan_turns(size_t n, size_t n_groups) {
     return counts <= 1u << 25 ? 1 : counts <= 1u << 27 ? 2 : 4;
 }
 
+// From how many chunks on a launch of its own adds their counts up, which every workgroup
+// does for itself below: that grows with the square of the routes.  1048576 routes (256
+// chunks) over 8, 256 and 1024 experts 12.8, 18.8 and 23.4 us, without it 14.3, 20.1 and
+// 39.4; 67108864 353, 584 and 843 us, without it 7.7, 11.4 and 44 ms.
+constexpr uint32_t kPlanSummed = 256;
+
 size_t wh_expert_plan_scratch(size_t n, size_t n_groups) {
     const size_t chunk = plan_chunk(plan_turns(n, n_groups)), chunks = (n + chunk - 1) / chunk;
-    return chunks > 1 ? chunks * plan_padded((uint32_t)n_groups) * sizeof(uint32_t) : 0;
+    return chunks > 1 ? (chunks + 1) * plan_padded((uint32_t)n_groups) * sizeof(uint32_t) : 0;
 }
 
 hipError_t wh_expert_plan_launch(const wh_expert_plan_args& a, hipStream_t stream) {
@@ -1648,9 +1684,19 @@ hipError_t wh_expert_plan_launch(const wh_expert_plan_args& a, hipStream_t strea
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (turns == 4) k_expert_place<4><<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
-    else if (turns == 2) k_expert_place<2><<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
-    else k_expert_place<1><<<chunks, kPlanThreads, plan_lds(a.n_groups), stream>>>(a, chunks, bits);
+    const size_t lds = plan_lds(a.n_groups);
+    if (turns == 4 && chunks >= kPlanSummed) {
+        k_expert_sum<<<(plan_padded(a.n_groups) + kSumExperts - 1) / kSumExperts, kSumExperts * kSumRuns, 0, stream>>>(a, chunks);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        k_expert_place<4, true><<<chunks, kPlanThreads, lds, stream>>>(a, chunks, bits);
+    } else if (turns == 4) {
+        k_expert_place<4, false><<<chunks, kPlanThreads, lds, stream>>>(a, chunks, bits);
+    } else if (turns == 2) {
+        k_expert_place<2, false><<<chunks, kPlanThreads, lds, stream>>>(a, chunks, bits);
+    } else {
+        k_expert_place<1, false><<<chunks, kPlanThreads, lds, stream>>>(a, chunks, bits);
+    }
     return hipGetLastError();
 }
 
