@@ -1,12 +1,14 @@
 """8-bit rows at the ends of what their calls take: sizes that pass a launch's threads,
-many routes.  Tolerances as in test_gpu_fp8_rows."""
+many routes, bf16 results where every error is as large as it can be.  Other tolerances
+as in test_gpu_fp8_rows."""
 import time
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_fp8_rows import gpu_near, ordered_ctx  # noqa: F401
-from test_gpu_fp8_rows_tiles import Case
+from test_gpu_fp8_rows import BLOCK, COLUMN, E4M3, Rows, gpu_near, ordered_ctx  # noqa: F401
+from test_gpu_fp8_rows_tiles import HALF, TALL, THIN, TILE, Case, plan
 
 pytestmark = pytest.mark.gpu
 
@@ -32,6 +34,46 @@ def test_products_of_more_outputs_than_a_launch_has_threads(ctx, special):
     for a, b in ((0, 20), (40000, 40001), (rows - 17, rows)):
         gpu_near(y[:n, a:b], x, w[a:b], True, cols)
     c.close()
+
+
+def codes_of(v):
+    return torch.from_numpy(np.asarray(v, np.float32)).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+
+
+@pytest.mark.parametrize("kind,n,rows,cols", [
+    (THIN, 3, 4096, 4096), (THIN, 3, 4096, 8192), (TILE, 3, 4096, 40704), (TILE, 700, 4096, 8192), (TILE, 600, 8192, 40704),
+    (HALF, 2000, 4096, 4096), (HALF, 2000, 4096, 40704), (TALL, 4300, 4112, 4096), (TALL, 4300, 4112, 40704)])
+def test_bf16_products_that_lose_most(ctx, kind, n, rows, cols):
+    """Eight bytes side by side are a group.  In the first block and, with the other sign,
+    the last one, each group has a product of 2^16 and seven of 7.875, which lie more than
+    13 bits under it; groups between sum up to less than half a step of the f32 sum so far,
+    2^20.  So everything that does not cancel may be lost: 7 * 2^-13 of S = sum |w||x| by the
+    alignment, and by cols / 8 additions to an f32 sum, at most 2^-23 of S each, cols *
+    2^-26; the header says 2^-10 for the first.  Then half a step of bf16, 2^-8."""
+    assert plan(n, rows, cols)[0] == kind
+    w, x = np.full(cols, 1.125 / 16), np.full(cols, 1.75 / 16)
+    for at, sign in ((slice(0, BLOCK), 1), (slice(cols - BLOCK, cols), -1)):
+        w[at], x[at] = 2.25, 3.5
+        w[at][::8], x[at][::8] = sign * 256, 256
+    wc, xc = codes_of(w), codes_of(x)  # by bytes
+    p = E4M3[wc] * E4M3[xc]
+    want, size = p.sum(), np.abs(p).sum()
+    in_columns = np.empty(cols, np.uint8)
+    in_columns.reshape(-1, BLOCK)[:, COLUMN] = wc.reshape(-1, BLOCK)
+    h = ctx.store_fp8(np.repeat(in_columns[None], rows, 0), rows, cols, np.full((rows // 16, cols // BLOCK), 127, np.uint8),
+                      rows // 16, cols // BLOCK)
+    r = Rows(n, cols)
+    r.codes[:, :cols] = torch.from_numpy(xc).cuda()
+    r.scales[:, :cols // BLOCK] = 127
+    for bf16 in (True, False):
+        y = torch.empty(n, rows, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+        ctx.fp8_rows_mm_async(h, 0, rows, r.c, n, y.data_ptr(), rows, bf16)
+        ctx.synchronize()
+        err = float((y.double() - want).abs().max())
+        bound = (2.0 ** -10 + cols * 2.0 ** -26) * size + 2.0 ** -8 * abs(want) if bf16 else (cols + 8) * 2.0 ** -24 * size
+        print(f"{kind} {cols} {'bf16' if bf16 else 'f32'}: {err / size * 1024:.4f} of 2^-10 S, bound {bound / size * 1024:.4f}")
+        assert err <= bound
+    ctx.release(h)
 
 
 class Routes:
