@@ -183,9 +183,9 @@ pub struct WhKvPlan {
     pub positions_dev: *mut u32,
 }
 
-/// Attention of new tokens over a 4-bit cache.
+/// 8-bit rows by their device buffers.
 #[repr(C)]
-#[derive(Clone, Copy)]
+#[derive(Clone, Copy, Debug)]
 pub struct WhFp8Rows {
     pub codes: *mut u8,
     pub stride: usize,
@@ -193,6 +193,7 @@ pub struct WhFp8Rows {
     pub scale_stride: usize,
 }
 
+/// Attention of new tokens over a 4-bit cache.
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
 pub struct WhKv4Attention {
