@@ -258,8 +258,9 @@ void wh_synth_fp4_host(uint64_t seed, uint64_t stream, uint8_t* packed, size_t p
 
 /* wh_store_fp8 of a weight and scales in device memory, whole when the call is
  * made: no counterpart in the reference.  128-column scale groups only (cols /
- * scale_cols == 128, else WH_INVALID_SHAPE), f32 scales 4-byte aligned.  Waits
- * for its copy, so the caller may reuse the memory; not inside a graph capture. */
+ * scale_cols == 128, else WH_INVALID_SHAPE) and at most 40704 columns (else
+ * WH_UNSUPPORTED), f32 scales 4-byte aligned.  Waits for its copy, so the caller
+ * may reuse the memory; not inside a graph capture. */
 int wh_store_fp8_device(wh_ctx* ctx, const uint8_t* weight_dev, size_t rows, size_t cols, const void* scales_dev,
                         size_t scale_rows, size_t scale_cols, int scale_format, wh_tensor* out);
 
@@ -961,12 +962,17 @@ int wh_kv4_attention_async(wh_ctx* ctx, const wh_kv4_cache* cache, const wh_kv4_
 /* ------------------------------------------------------------------
  * Products of 8-bit rows, no counterpart in the reference (its products take
  * f32 inputs, as wh_fp8_gemv_multi does): for prompts and large batches, where
- * both sides in 8 bits take a sixth of the matrix instructions.
+ * both sides in 8 bits take a sixth of the matrix instructions.  Their weights
+ * are FP8 tensors: the store's FP4 experts, which the reference's MoE entry
+ * points take, are refused (WH_INVALID_QUANT_FORMAT).
  *
  * A row of cols values (a multiple of 128) is E4M3 codes and a UE8M0 scale byte
  * for every 128 columns: value = code * 2^(byte - 127); code 0x7F / 0xFF and
  * byte 255 stand for NaN.  Codes lie in the weight store's order: byte 16 l + i
- * of a block is its column 16 (i % 8) + 8 (i / 8) + l (l < 8, i < 16).
+ * of a block is its column 16 (i % 8) + 8 (i / 8) + l (l < 8, i < 16).  These are
+ * not wh_act_quant_dequant's values: that takes blocks of 64 and rounds ties
+ * toward minus infinity, and a row that it has rounded is rounded again here
+ * wherever the two halves of a block of 128 have scales apart.
  *
  * An MoE layer's step: wh_fp8_quant_rows_async of the positions,
  * wh_expert_plan_async of their routes, wh_fp8_rows_mm_groups_async with gate
@@ -992,7 +998,8 @@ typedef struct {
  * even; infinities and NaN become NaN.  The swiglu form rounds silu(min(gate,
  * limit)) * clamp(up, -limit, limit), in f32 (E/deepseek_v4.rs:590-594 with
  * limit 10; INFINITY: no clamp); a product beyond f32 becomes NaN.  Inputs may
- * begin at any value; out overlaps none of them. */
+ * begin at any value; out overlaps none of them.  A call takes up to 268435440
+ * blocks, n * cols / 128, as does reading them back. */
 int wh_fp8_quant_rows_async(wh_ctx* ctx, const void* x_dev, size_t x_stride, int is_bf16, size_t n, size_t cols,
                             const wh_fp8_rows* out);
 int wh_fp8_swiglu_rows_async(wh_ctx* ctx, const void* gate_dev, const void* up_dev, size_t stride, int is_bf16, size_t n,
@@ -1003,28 +1010,29 @@ int wh_fp8_read_rows_async(wh_ctx* ctx, const wh_fp8_rows* rows, size_t n, size_
 
 /* y row i = rows [row_start, row_end) of w times x row i, f32 or bf16
  * (is_bf16), for n rows of w's columns.  w: an FP8 tensor of 128-column scale
- * groups.  Products of codes are exact, sums are f32 in any order, in both
- * numerics modes.  f32 results are within (cols + 8) * 2^-24 * sum |w| |x|.
- * bf16 results come from 8-bit matrix instructions, which align eight products
- * to the largest of them, keep 13 bits under it and add that to an f32 sum: at
- * most (2^-10 + cols * 2^-26) * sum |w| |x| off, usually 2e-5 to 6e-5 of the
- * result's norm, before they are rounded once.  So about one bf16 result in a
- * hundred is the neighbour of the correctly rounded one; f32 results rounded to
- * bf16 by the caller are not.  The
- * order of a sum follows from the sizes (n, n_groups and the tensor's), so a row
- * may differ by f32's rounding between calls of other sizes; a call repeats bit
- * for bit.  A NaN in an x row makes its y row NaN and no other.  Weight codes
- * 0x7F / 0xFF are +-480 and UE8M0 bytes 0 and 255 are 0.0 and infinity, as in
- * every product here.  Tensors with such codes, and ranges or scale rows that
- * are no multiples of 16 rows, take a kernel without matrix instructions, many
- * times as long.  y must not overlap x.  Some sizes use memory of the context
- * that grows: before a capture, run the call once (wh_graph_begin). */
+ * groups and at most 40704 columns (else WH_UNSUPPORTED).  Products of codes are
+ * exact, sums are f32 in any order, in both numerics modes.  f32 results are
+ * within (cols + 8) * 2^-24 * sum |w| |x|.  bf16 results come from 8-bit matrix
+ * instructions, which align eight products to the largest of them, keep 13 bits
+ * under it and add that to an f32 sum: at most (2^-10 + cols * 2^-26) * sum |w|
+ * |x| off, usually 2e-5 to 6e-5 of the result's norm, before they are rounded
+ * once.  So about one bf16 result in a hundred is the neighbour of the correctly
+ * rounded one; f32 results that the caller rounds to bf16 hardly ever are.  The
+ * order of a sum follows from the output's type and the sizes (n, n_groups, the
+ * length of the range and the tensor's), so a row may differ by f32's rounding
+ * between calls that differ in those; a call repeats bit for bit.  A NaN in an x
+ * row makes its y row NaN and no other.  Weight codes 0x7F / 0xFF are +-480 and
+ * UE8M0 bytes 0 and 255 are 0.0 and infinity, as in every product here.  Tensors
+ * with such codes, and ranges or scale rows that are no multiples of 16 rows,
+ * take a kernel without matrix instructions, many times as long.  y must not
+ * overlap x.  Some sizes use memory of the context that grows: before a capture,
+ * run the call once (wh_graph_begin). */
 int wh_fp8_rows_mm_async(wh_ctx* ctx, wh_tensor w, size_t row_start, size_t row_end, const wh_fp8_rows* x, size_t n,
                          void* y_dev, size_t y_stride, int is_bf16);
 
 /* The same grouped by expert: y row j, starts_dev[g] <= j < starts_dev[g + 1],
  * is x row rows_dev[j] (NULL: j) times w's rows row_start + g * group_rows +
- * [0, group_rows).  starts_dev [n_groups + 1] ascends (not checked: else the n
+ * [0, group_rows); without rows_dev n_x is at least n.  starts_dev [n_groups + 1] ascends (not checked: else the n
  * rows of y are undefined) and is cut off at n; y rows in no group are left as
  * they are.  rows_dev [n] entries of n_x or more are no row: their y rows are 0.
  * The same row may be listed any number of times.  At most 1024 groups. */
@@ -1046,8 +1054,9 @@ int wh_debug_fp8_rows_plan(size_t n, size_t n_groups, int lists, size_t group_ro
  * routes in order; rows_dev [npos * topk] gets each listed route's position
  * and 0xFFFFFFFF behind the last list, slots_dev [npos][topk] each route's
  * place in the lists or 0xFFFFFFFF.  At most 1024 experts; outputs overlap
- * neither each other nor ids_dev.  Above 1024 routes it uses memory of the
- * context that grows: before a capture, run the call once. */
+ * neither each other nor ids_dev.  Above 4096 routes it uses memory of the
+ * context that grows: before a capture, run the call once.  Fewer than 2^31
+ * routes, topk at most 65536. */
 int wh_expert_plan_async(wh_ctx* ctx, const uint32_t* ids_dev, size_t npos, size_t topk, size_t n_experts,
                          uint32_t* starts_dev, uint32_t* rows_dev, uint32_t* slots_dev);
 
@@ -1056,7 +1065,8 @@ int wh_expert_plan_async(wh_ctx* ctx, const uint32_t* ids_dev, size_t npos, size
  * may be out).  Slots of n_rows or more are passed over, whatever their weight; a
  * position of no slots gets 0 or its add row.  y is f32 or bf16; hidden and all
  * strides are multiples of 4 values, rows aligned to 4 values.  out overlaps
- * neither y nor, unless it is add with add's stride, add. */
+ * neither y nor, unless it is add with add's stride, add.  npos * (hidden / 1024,
+ * rounded up) is below 2^24. */
 int wh_expert_combine_async(wh_ctx* ctx, const void* y_dev, size_t y_stride, int is_bf16, size_t n_rows,
                             const uint32_t* slots_dev, const float* weights_dev, size_t npos, size_t topk, size_t hidden,
                             const float* add_dev, size_t add_stride, float* out_dev, size_t out_stride);

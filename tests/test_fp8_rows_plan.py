@@ -1,10 +1,11 @@
 """CPU checks of how products of 8-bit rows are done: the rule that picks a kernel
-needs no device."""
+needs no device.  Also the sizes that calls on rows are refused from on."""
 import ctypes
 
 import pytest
 
 import wohper_amd as wa
+from test_fp8_rows_host import every_row_call, lib_and_ctx, rows  # noqa: F401
 
 EMPTY, SHAPE, ARGUMENT, UNSUPPORTED = 1, 2, 13, 15
 VECTOR, THIN, TILE, HALF, TALL = range(5)
@@ -49,3 +50,11 @@ def test_sizes_that_are_taken_do_not_depend_on_codes(n, rows, cols, groups, bf16
         status, kind, splits, grid, tiles = plan(n, rows, cols, groups, special=special, bf16=bf16)
         assert status == 0 and grid * splits * (512 if kind == THIN else 256) < 1 << 32
         assert kind == VECTOR if special else grid >= tiles or kind in (VECTOR, HALF, TALL)
+
+
+def test_blocks_of_a_call_are_counted(lib_and_ctx):  # noqa: F811
+    """268435440 blocks, as the header says: one more is refused before the context is touched."""
+    cols = 128 * 268435441
+    wide = rows(stride=cols, scale_stride=268435444)
+    assert every_row_call(*lib_and_ctx, r=wide, n=1, cols=cols, stride=cols) == [UNSUPPORTED] * 3
+    assert every_row_call(*lib_and_ctx, n=134217721) == [UNSUPPORTED] * 3

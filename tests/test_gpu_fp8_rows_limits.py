@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 import torch
 
+import wohper_amd as wa
 from test_gpu_fp8_rows import BLOCK, COLUMN, E4M3, Rows, gpu_near, ordered_ctx  # noqa: F401
 from test_gpu_fp8_rows_tiles import HALF, TALL, THIN, TILE, Case, plan
 
@@ -132,3 +133,52 @@ def test_a_plan_costs_what_its_routes_do(ctx):
             best = min(best, time.perf_counter() - t)
         took.append(best)
     assert took[1] <= 24 * took[0]
+
+
+def test_plans_of_one_launch_need_no_call_before_a_capture():
+    """Up to 4096 routes a plan uses no memory of the context: the first call of a new one
+    is captured."""
+    for npos, topk, n_experts in ((4096, 1, 1024), (512, 8, 256), (682, 6, 64)):
+        r = Routes(npos, topk, n_experts)
+        torch.cuda.synchronize()
+        fresh = wa.Context(0)
+        g = fresh.graph_capture(lambda: r.run(fresh))
+        for _ in range(3):
+            r.slots.fill_(77)
+            torch.cuda.synchronize()
+            fresh.graph_launch(g)
+            fresh.synchronize()
+            ids = r.ids.cpu().numpy()
+            order = np.argsort(np.where((ids >= 0) & (ids < n_experts), ids, n_experts), kind="stable")
+            listed = int(r.starts[n_experts])
+            want = np.full(npos * topk, -1)
+            want[order[:listed]] = np.arange(listed)
+            assert listed == ((ids >= 0) & (ids < n_experts)).sum() and np.array_equal(r.slots[:-1].cpu().numpy(), want)
+        fresh.graph_release(g)
+        fresh.close()
+
+
+def test_the_widest_tensors(ctx):
+    """40704 columns are the most that the resident layout and its products take."""
+    rng = np.random.default_rng(1)
+    w, s = rng.integers(0, 127, (16, 40832), dtype=np.uint8), np.full((1, 319), 120, np.uint8)
+    wide = ctx.store_fp8(w, 16, 40832, s, 1, 319)
+    x = Rows(2, 40832)
+    y = torch.zeros(2, 16, device="cuda")
+    d, sd = torch.from_numpy(w[:, :40704].copy()).cuda(), torch.from_numpy(s[:, :318].copy()).cuda()
+    torch.cuda.synchronize()
+    with pytest.raises(wa.DeepSeekV4KernelError) as e:
+        ctx.fp8_rows_mm_async(wide, 0, 16, x.c, 2, y.data_ptr(), 16, False)
+    assert e.value.code == 15
+    with pytest.raises(wa.DeepSeekV4KernelError) as e:
+        ctx.store_fp8_device(d.data_ptr(), 16, 40832, sd.data_ptr(), 1, 319)  # refused before it is read
+    assert e.value.code == 15
+    ctx.release(wide)
+    h = ctx.store_fp8_device(d.data_ptr(), 16, 40704, sd.data_ptr(), 1, 318)
+    x.codes.fill_(0x38)  # 1.0
+    x.scales.fill_(127)
+    ctx.fp8_rows_mm_async(h, 0, 16, x.c, 2, y.data_ptr(), 16, False)
+    ctx.synchronize()
+    want = E4M3[w[:, :40704]].sum(1) * 2.0 ** -7
+    assert (np.abs(y.cpu().double().numpy() - want) <= 40712 * 2.0 ** -24 * want).all()
+    ctx.release(h)
