@@ -207,3 +207,32 @@ def test_counters_of_two_contexts(ctx):
         assert all(torch.equal(y, w) for y in out)
         j.case.close()
     other.close()
+
+
+@pytest.mark.parametrize("kind,n_groups,n,rows,cols,bf16", [
+    (THIN, 64, 1000, 256, 640, True), (THIN, 64, 1000, 256, 640, False), (TILE, 16, 3000, 272, 8448, True),
+    (TILE, 16, 3000, 272, 8448, False), (TILE, 64, 6000, 512, 1152, True), (HALF, 64, 4000, 1024, 4096, True),
+    (TALL, 64, 16000, 4096, 4096, True)])
+def test_results_do_not_depend_on_how_rows_are_spread(ctx, kind, n_groups, n, rows, cols, bf16):
+    """The same x row in every list, over lists of all lengths: the same bits, whichever
+    tile, place in it and number of rows beside it."""
+    assert plan(n, rows, cols, n_groups, bf16=bf16)[0] == kind
+    c = Case(ctx, n, 40, n_groups * rows, cols)
+    rng = np.random.default_rng(n)
+    first = {}
+    for spread in range(3):
+        starts = lists(rng, n_groups, n, ("ragged", "even", "one")[spread])
+        at = rng.integers(0, 40, n)
+        at[rng.integers(0, n, n // 2)] = 7
+        s, r = i32(starts), i32(at)
+        y = torch.zeros(n, rows, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+        ctx.fp8_rows_mm_groups_async(c.h, 0, rows, n_groups, c.rows.c, 40, r.data_ptr(), s.data_ptr(), n, y.data_ptr(), rows, bf16)
+        ctx.synchronize()
+        at_dev = torch.from_numpy(at).cuda()
+        for g in range(n_groups):
+            a, b = int(starts[g]), int(starts[g + 1])
+            sevens = y[a:b][at_dev[a:b] == 7]
+            if len(sevens):
+                assert torch.equal(sevens, first.setdefault(g, sevens[0]).expand_as(sevens))
+    assert len(first) == n_groups
+    c.close()

@@ -441,9 +441,11 @@ __device__ __forceinline__ uint32_t rows_source(const wh_rows_mm_args& a, uint32
 // registers; the waves of the same weight rows join in LDS.  Blocks come kU at a time, all
 // their loads before the first product; a range's blocks lie side by side, so that one
 // word holds a row's scales of four.  Registers for two workgroups a CU: 84 rows over 64
-// lists of 4096 x 4096, 43 of them not empty, in f32 147 us (with one 226), 4.9 TB/s.
+// lists of 4096 x 4096, 43 of them not empty, in f32 145 to 157 us (with one workgroup
+// 226), 4.6 to 5.0 TB/s, where a large read reaches 6.2.
 // x is read again for each 16 kNt weight rows: 16 x 8192 x 8192 in bf16 18.8 us with one, 16.1
-// (4.2 TB/s) with two; 5 x 4096 x 8192 in f32 9.1 us, 3.7 TB/s with the launch.
+// (4.2 TB/s) with two; 5 x 4096 x 8192 in f32 9.4 us, 3.6 TB/s with the launch.  The f32
+// form with two spills 5 or 6 registers, two reloaded in the loop over 64 rows.
 constexpr uint32_t kThinWaves = 8;
 template <int kMt, int kNt, bool kBf16, bool kMant>
 __device__ __forceinline__ void rows_thin(const wh_rows_mm_args& a, float (*part)[64][4], uint32_t ks_n, uint32_t g, uint32_t j0,
@@ -784,10 +786,10 @@ __device__ __forceinline__ void rows_tile_scales(const wh_rows_mm_args& a, uint8
 // multiple of 4), whose parts go to a.part in f32 and k_rows_join adds up: 128 x 4096 x
 // 4096 in bf16 24.6 us whole, 18 in four ranges.  f32 results are bound by the vector
 // instructions beside the matrix ones, two a product for decoding and two for scales, and
-// by the power that the f16 instructions draw: 4096 x 4096 x 4096 163 us, 0.84 PFLOP/s
-// (a library's f16 product 1.46); 333 x 32768 x 1024 with f32 scales 34.5.  Applying both
-// scales as one factor saves 4 to 10 percent, but loses bits where its power of two
-// leaves f32's range.
+// by the power that the f16 instructions draw: 4096 x 4096 x 4096 138 us, 1.0 PFLOP/s (a
+// library's f16 product 1.46), 165 behind idle time, when clocks are low; 333 x 32768 x
+// 1024 with f32 scales 34.  Applying both scales as one factor saves 4 to 10 percent, but
+// loses bits where its power of two leaves f32's range.
 template <bool kBf16, bool kMant>
 __global__ void __launch_bounds__(256, 2) k_rows_mm_tile(wh_rows_mm_args a, uint32_t per) {
     constexpr int kMt = 4, kNt = 4, kWm = 2, kWn = 2;
@@ -1124,11 +1126,12 @@ __device__ __forceinline__ void rows_big(const wh_rows_mm_args& a, uint8_t* lds,
 // workgroup a CU takes its XCD's tiles until there are none left (half tiles take half
 // as long), then other XCDs': the first by its id, the next from a counter that it asks a
 // tile ahead.  tickets: [8] tiles taken, workgroups done; 0 between launches.
-// 4096 x 4096 x 8192 97 us, 2.8 PFLOP/s, where the clock falls under the matrix
-// instructions' power (a library's 8-bit product there 3.0); 24000 rows over 64 uneven
-// lists of 4096 x 4096 412 us, 1.7: 18 percent of the tiles' rows are empty, 12 percent of
+// 4096 x 4096 x 8192 99 us, 2.8 PFLOP/s, where the clock falls under the matrix
+// instructions' power (a library's 8-bit product there 3.0); 21000 rows over 64 uneven
+// lists of 4096 x 4096 425 us, 1.7: 18 percent of the tiles' rows are empty, 12 percent of
 // the time is the last tiles', and a tile's beginning and end take 9 us beside 46 of
-// products.
+// products.  kTall takes all 512 registers and spills 20 vector and 118 scalar ones, 84
+// bytes of scratch, outside the loop over blocks.
 template <bool kTall>
 __global__ void __launch_bounds__(256, 1) k_rows_mm_big(wh_rows_mm_args a) {
     extern __shared__ __align__(128) uint8_t tile_lds[];
@@ -1497,7 +1500,9 @@ hipError_t wh_rows_read_launch(const wh_rows_read_args& a, bool bf16, hipStream_
 
 // Which kernel takes a product, and how many ranges its columns are cut into: the least
 // of these estimates of its time in us, fitted to 400 measured calls (one MI355X; 1 to
-// 4096 rows, 1 to 64 groups, weights from 1408 x 512 to 32768 x 1024 and 4096 x 8192).
+// 4096 rows, 1 to 64 groups, weights from 1408 x 512 to 32768 x 1024 and 4096 x 8192; call
+// after call on the same weight, which the Infinity Cache holds up to 256 MB: from memory
+// one of 4096 x 4096 takes 1 to 6 us more).
 //  - thin: a wave's block of columns takes 0.8, 1.05 and 3 us for up to 16, 32 and 64
 //    rows (with groups of uneven lists 0.55 and 0.045 a row), workgroups in rounds of 256:
 //    4096 x 4096 with 16, 64 and 128 rows 7.2, 15.6 and 29, where tiles take 23 to 25, cut
