@@ -182,3 +182,48 @@ def test_the_widest_tensors(ctx):
     want = E4M3[w[:, :40704]].sum(1) * 2.0 ** -7
     assert (np.abs(y.cpu().double().numpy() - want) <= 40712 * 2.0 ** -24 * want).all()
     ctx.release(h)
+
+
+@pytest.mark.parametrize("kind,n", [(THIN, 3), (THIN, 30), (TILE, 300)])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("zero", ["byte 0", 0.0, -0.0])
+def test_scales_of_zero_meet_rows_near_the_largest_f32(ctx, kind, n, bf16, zero):
+    """x of 448 * 2^120 in a block whose weight scale is 0.0: nothing is added, though the
+    block's codes times the row's scale alone are past f32."""
+    rows, cols, f32 = 256, 640, zero != "byte 0"
+    assert plan(n, rows, cols, f32=f32, bf16=bf16)[0] == kind
+    codes = np.full((rows, cols), 0x7E, np.uint8)  # 448
+    scales = np.full((2, 5), 2.0 ** -110, np.float32) if f32 else np.full((2, 5), 17, np.uint8)
+    scales[0, 1] = scales[1, 0] = zero if f32 else 0
+    h = ctx.store_fp8(codes, rows, cols, scales, 2, 5, int(f32))
+    r = Rows(n, cols)
+    r.codes.fill_(0x7E)
+    r.scales.fill_(247)
+    y = torch.empty(n, rows, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    ctx.fp8_rows_mm_async(h, 0, rows, r.c, n, y.data_ptr(), rows, bf16)
+    ctx.synchronize()
+    want = 448.0 * 448 * 128 * 4 * 2.0 ** 10  # four blocks of equal products
+    assert bool(((y.double() - want).abs() <= (2.0 ** -8 if bf16 else 648 * 2.0 ** -24) * want).all())
+    ctx.release(h)
+
+
+@pytest.mark.parametrize("kind,n", [(THIN, 3), (THIN, 30), (TILE, 300)])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("f32", [False, True])
+def test_infinite_scales_meet_the_smallest_rows(ctx, kind, n, bf16, f32):
+    """Rows of 2^-9 * 2^-126, the least that are not 0: infinite with the sign of the product."""
+    rows, cols = 256, 640
+    assert plan(n, rows, cols, f32=f32, bf16=bf16)[0] == kind
+    codes = np.full((rows, cols), 0x01, np.uint8)  # 2^-9
+    codes[::2] = 0x81
+    scales = np.full((2, 5), 2.0 ** -20, np.float32) if f32 else np.full((2, 5), 107, np.uint8)
+    scales[0, 1] = scales[1, 0] = np.inf if f32 else 255
+    h = ctx.store_fp8(codes, rows, cols, scales, 2, 5, int(f32))
+    r = Rows(n, cols)
+    r.codes.fill_(0x01)
+    r.scales.fill_(1)
+    y = torch.empty(n, rows, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    ctx.fp8_rows_mm_async(h, 0, rows, r.c, n, y.data_ptr(), rows, bf16)
+    ctx.synchronize()
+    assert bool((y[:, 1::2] == float("inf")).all()) and bool((y[:, ::2] == -float("inf")).all())
+    ctx.release(h)

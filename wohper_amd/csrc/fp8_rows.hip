@@ -385,6 +385,9 @@ __device__ __forceinline__ wh_f4 rows_scaled(wh_f4 acc, wh_f4 block, int e, floa
 
 // A weight scale's bits, and they as the byte of a power of two and a factor: 1 for
 // ordinary UE8M0 bytes, else in [1, 2), or the scale itself where it is no normal number.
+// 0 goes with the least power of two and infinity with the largest, so that neither the
+// largest nor the smallest rows leave f32's range before they meet it, where the product
+// would be NaN.
 __device__ __forceinline__ uint32_t rows_scale_bits(const wh_rows_mm_args& a, uint64_t at) {
     return a.scale_f32 ? ((const uint32_t*)a.w_scales)[at] : ((const uint8_t*)a.w_scales)[at];
 }
@@ -393,15 +396,15 @@ __device__ __forceinline__ uint32_t rows_split_bits(const wh_rows_mm_args& a, ui
     if (!a.scale_f32) {
         if (u != 0 && u != 255) return u;
         *m = wh_ue8m0(u);
-        return 127;
+        return u ? 254 : 0;
     }
     const float s = __uint_as_float(u);
     const uint32_t e = u >> 23 & 0xff;
-    if (e == 255 || (u & 0x7fffffffu) == 0) {
+    if (e == 255) {
         *m = s;
-        return 127;
+        return 254;
     }
-    if (e == 0) {
+    if (e == 0) {  // 0 too
         *m = s * 1.70141183460469231732e38f;  // 2^127
         return 0;
     }
