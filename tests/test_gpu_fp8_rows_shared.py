@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+import wohper_amd as wa
 from test_gpu_fp8_rows import Layer, Step, f64, ordered_ctx  # noqa: F401
 from test_gpu_fp8_rows_tiles import TALL, TILE, Case, check, plan
 
@@ -93,3 +94,51 @@ def test_a_graph_serves_batches_of_every_fill(ctx):
         assert used == 0 or float(eager[:used].abs().max()) > 0
     ctx.graph_release(g)
     layer.close()
+
+
+def test_a_capture_that_needs_more_memory_fails_and_leaves_the_context():
+    """A product whose parts, or a plan whose counts, do not fit what the context has: the
+    capture ends in an error, is never launched, and eager calls go on."""
+    fresh = wa.Context(0)
+    sizes = [(128, 1024, 4096), (128, 4096, 4096)]
+    assert all(plan(*s)[0] == TILE and plan(*s)[1] > 1 for s in sizes)
+    cases = [Case(fresh, i, *s) for i, s in enumerate(sizes)]
+    ys = [torch.zeros(n, rows, dtype=torch.bfloat16, device="cuda") for n, rows, _ in sizes]
+    ids = torch.randint(0, 64, (20000,), dtype=torch.int32, device="cuda")
+    out = [torch.zeros(k, dtype=torch.int32, device="cuda") for k in (65, 20000, 20000)]
+    torch.cuda.synchronize()
+
+    def product(i):
+        fresh.fp8_rows_mm_async(cases[i].h, 0, sizes[i][1], cases[i].rows.c, sizes[i][0], ys[i].data_ptr(), sizes[i][1], True)
+
+    def lists_of():
+        fresh.expert_plan_async(ids.data_ptr(), 20000, 1, 64, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr())
+
+    for calls in ((lists_of,), (lambda: product(0),)):
+        with pytest.raises(wa.DeepSeekV4KernelError):
+            fresh.graph_capture(lambda calls=calls: [c() for c in calls])
+    product(0)
+    fresh.synchronize()
+    with pytest.raises(wa.DeepSeekV4KernelError):
+        fresh.graph_capture(lambda: (product(0), product(1)))
+    lists_of()
+    for i in range(2):
+        product(i)
+    fresh.synchronize()
+    for i, (n, rows, cols) in enumerate(sizes):
+        check(ys[i], cases[i].x(), cases[i].w(0, rows), cols)
+    assert torch.equal(torch.bincount(ids, minlength=64).cumsum(0), out[0][1:].long())
+    g = fresh.graph_capture(lambda: (product(0), product(1), lists_of()))
+    for _ in range(3):
+        for t in ys + out:
+            t.fill_(3)
+        torch.cuda.synchronize()
+        fresh.graph_launch(g)
+        fresh.synchronize()
+        for i, (n, rows, cols) in enumerate(sizes):
+            check(ys[i], cases[i].x(), cases[i].w(0, rows), cols)
+        assert torch.equal(torch.bincount(ids, minlength=64).cumsum(0), out[0][1:].long())
+    fresh.graph_release(g)
+    for c in cases:
+        c.close()
+    fresh.close()
