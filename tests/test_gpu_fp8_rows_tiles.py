@@ -236,3 +236,27 @@ def test_results_do_not_depend_on_how_rows_are_spread(ctx, kind, n_groups, n, ro
                 assert torch.equal(sevens, first.setdefault(g, sevens[0]).expand_as(sevens))
     assert len(first) == n_groups
     c.close()
+
+
+@pytest.mark.parametrize("kind,n,rows", [(TALL, 16000, 4096), (HALF, 4000, 1024)])
+def test_starts_that_do_not_ascend_leave_counters_and_neighbours(ctx, kind, n, rows):
+    """Lists that overlap count rows more than once: the n rows of y are undefined, those
+    behind them stay, and the next call finds the counters at 0."""
+    n_groups, cols = 64, 4096
+    assert plan(n, rows, cols, n_groups)[0] == kind
+    c = Case(ctx, n, 300, n_groups * rows, cols)
+    rng = np.random.default_rng(n)
+    at = rng.integers(0, 300, n)
+    r, y = i32(at), torch.full((n + 300, rows), 5.0, dtype=torch.bfloat16, device="cuda")
+    good = lists(rng, n_groups, n, "ragged")
+    for starts in ([0, n] * 32 + [0], [n, 0] * 32 + [n], list(range(0, 4000000000, 61000000))[:65], good[::-1].copy(), good):
+        s = i32(starts)
+        ctx.fp8_rows_mm_groups_async(c.h, 0, rows, n_groups, c.rows.c, 300, r.data_ptr(), s.data_ptr(), n, y.data_ptr(), rows, True)
+        ctx.synchronize()
+        assert bool((y[n:] == 5.0).all())
+    x, at_dev = c.x(), torch.from_numpy(at).cuda()
+    for g in range(n_groups):
+        a, b = int(good[g]), int(good[g + 1])
+        if b > a:
+            check(y[a:b], x[at_dev[a:b]], c.w(g * rows, (g + 1) * rows), cols)
+    c.close()
