@@ -260,3 +260,31 @@ def test_starts_that_do_not_ascend_leave_counters_and_neighbours(ctx, kind, n, r
         if b > a:
             check(y[a:b], x[at_dev[a:b]], c.w(g * rows, (g + 1) * rows), cols)
     c.close()
+
+
+@pytest.mark.parametrize("kind,n_groups,n,rows,cols,bf16,special", [
+    (0, 5, 200, 256, 384, True, True), (THIN, 8, 100, 256, 640, True, False), (THIN, 1, 20, 8192, 4096, True, False),
+    (TILE, 16, 3000, 272, 8448, True, False), (TILE, 16, 3000, 272, 8448, False, False), (TILE, 1, 700, 4090, 1152, False, False),
+    (HALF, 64, 4000, 1024, 4096, True, False), (TALL, 64, 16000, 4096, 4096, True, False)])
+def test_lists_that_begin_behind_the_first_row(ctx, kind, n_groups, n, rows, cols, bf16, special):
+    """Some of a longer plan's experts: starts begin and end inside y, whose other rows stay."""
+    assert plan(n, rows, cols, n_groups, bf16=bf16, special=special)[0] == kind
+    total = -(-n_groups * rows // 16) * 16
+    c = Case(ctx, n, n, total, cols)
+    if special:
+        ctx.release(c.h)
+        c.codes[3, 3] = 0x7F
+        torch.cuda.synchronize()
+        c.h = ctx.store_fp8_device(c.codes.data_ptr(), total, cols, c.scales.data_ptr(), *c.scales.shape)
+    starts = n // 5 + lists(np.random.default_rng(n), n_groups, n // 2, "ragged")
+    s = i32(starts)
+    y = torch.full((n + 1, rows), 5.0, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    ctx.fp8_rows_mm_groups_async(c.h, 0, rows, n_groups, c.rows.c, n, None, s.data_ptr(), n, y.data_ptr(), rows, bf16)
+    ctx.synchronize()
+    assert bool((y[:starts[0]] == 5.0).all()) and bool((y[starts[-1]:] == 5.0).all())
+    x = c.x()
+    for g in range(n_groups):
+        a, b = int(starts[g]), int(starts[g + 1])
+        if b > a:
+            gpu_near(y[a:b], x[a:b], c.w(g * rows, (g + 1) * rows), bf16, cols)
+    c.close()
